@@ -7,11 +7,13 @@
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include <atomic>
 #include <initializer_list>
 
 #include "mfma_common.h"
+#include "pages4.h"
 
 namespace {
 
@@ -548,6 +550,100 @@ int run_step(const tsattn_step_desc &d, const StepPlan &s, char *ws, hipStream_t
                     "step down projection launch");
 }
 
+// The 4-bit paged cache: what every call over it checks.
+bool pages4_sizes_ok(int32_t heads, int32_t page_size, int32_t dim) {
+  return heads > 0 && heads <= 4096 && page_size >= tsattn::kTile && page_size <= 4096 &&
+         !(page_size & (page_size - 1)) && (dim == 32 || dim == 64 || dim == 128 || dim == 256);
+}
+
+int check_pages4(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t len, const int32_t *rows,
+                 const int32_t *lens, tsattn::Pages4 *out) {
+  if (!p || !rows || !lens) return fail(TSATTN_ERR_INVALID, "paged cache: descriptor, rows or lengths are NULL");
+  if (dtype != TSATTN_F32 && dtype != TSATTN_F16 && dtype != TSATTN_BF16)
+    return fail(TSATTN_ERR_INVALID, "a paged cache's rows are f32, f16 or bf16 (got dtype %d)", dtype);
+  if (n <= 0 || len <= 0 || p->num_pages <= 0 || p->table_rows <= 0 || p->table_stride <= 0 || p->heads <= 0)
+    return fail(TSATTN_ERR_INVALID, "paged cache: sizes must be positive");
+  if (!pages4_sizes_ok(p->heads, p->page_size, p->dim) || p->num_pages > INT32_MAX || p->table_rows > INT32_MAX)
+    return fail(TSATTN_ERR_UNSUPPORTED,
+                "a paged cache takes head dims 32, 64, 128 and 256, up to 4096 heads and pages of 32, 64, .. 4096 "
+                "positions");
+  if (!p->pool || !p->table) return fail(TSATTN_ERR_INVALID, "paged cache: data pointer is NULL");
+  if (reinterpret_cast<uintptr_t>(p->pool) % 16)
+    return fail(TSATTN_ERR_UNSUPPORTED, "a paged cache's pool must be 16-byte aligned");
+  const int64_t room = p->table_stride * p->page_size;
+  for (int32_t i = 0; i < n; ++i) {
+    if (rows[i] < 0 || rows[i] >= p->table_rows)
+      return fail(TSATTN_ERR_INVALID, "paged cache: sequence %d has table row %d of %lld", i, rows[i],
+                  static_cast<long long>(p->table_rows));
+    if (lens[i] < 0 || lens[i] > room || lens[i] > INT32_MAX / 4)
+      return fail(TSATTN_ERR_INVALID, "paged cache: sequence %d has %d positions in a table of %lld", i, lens[i],
+                  static_cast<long long>(room));
+  }
+  out->pool = static_cast<char *>(p->pool);
+  out->page_bytes = tsattn::page4_bytes(p->heads, p->page_size, p->dim);
+  out->pages = static_cast<int32_t>(p->num_pages);
+  out->heads = p->heads;
+  out->per_page = 0;
+  while ((tsattn::kTile << out->per_page) < p->page_size) ++out->per_page;
+  out->dim = p->dim;
+  out->table = p->table;
+  out->stride = p->table_stride;
+  return TSATTN_OK;
+}
+
+// Rows of an operand beside a paged cache: every stride and the base 16-byte aligned.
+int check_rows4(const tsattn_view *v, int32_t dtype, const char *name) {
+  int rc = check_view(v, name);
+  if (rc) return rc;
+  const int64_t unit = dtype == TSATTN_F32 ? 4 : 8;
+  if (reinterpret_cast<uintptr_t>(v->data) % 16 || v->stride[0] % unit || v->stride[1] % unit || v->stride[2] % unit)
+    return fail(TSATTN_ERR_UNSUPPORTED, "%s rows must be 16-byte aligned beside a paged cache", name);
+  return TSATTN_OK;
+}
+
+int check_tables4(const void *cos, const void *sin) {
+  if (!cos != !sin) return fail(TSATTN_ERR_INVALID, "RoPE needs both cos and sin tables");
+  if ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) % 16)
+    return fail(TSATTN_ERR_UNSUPPORTED, "RoPE tables must be 16-byte aligned beside a paged cache");
+  return TSATTN_OK;
+}
+
+// Whether the n numbers are all different, each below `below` (> 0); `seen` [below] is clear.
+bool distinct(int32_t n, const int32_t *x, char *seen) {
+  for (int32_t i = 0; i < n; ++i) {
+    if (seen[x[i]]) return false;
+    seen[x[i]] = 1;
+  }
+  return true;
+}
+
+// Sequences i0 .. i0 + m - 1 of a call.
+int take_seqs(tsattn::Seqs *s, int32_t n, int32_t i0, const int32_t *rows, const int32_t *lens) {
+  const int m = n - i0 < tsattn::kSeqs ? n - i0 : tsattn::kSeqs;
+  for (int i = 0; i < m; ++i) s->row[i] = rows[i0 + i], s->len[i] = lens[i0 + i];
+  return m;
+}
+tsattn::View seq_view(const tsattn_view *v, int32_t i0, int32_t dtype) {
+  tsattn::View x = tsattn::make_view(v);
+  x.data = static_cast<const char *>(x.data) + i0 * x.s0 * (dtype == TSATTN_F32 ? 4 : 2);
+  return x;
+}
+
+// The splits of sequences i0 .. i0 + m - 1, and the scratch that they take.
+size_t plan_attend4(const tsattn_pages4 *p, int32_t dtype, int32_t m, int32_t rows, const int32_t *lens,
+                    int *split, int *splits) {
+  int64_t total = 0;
+  int longest = 0;
+  for (int i = 0; i < m; ++i) {
+    total += lens[i];
+    longest = lens[i] > longest ? lens[i] : longest;
+  }
+  *split = tsattn::attend4_split(dtype, p->dim, p->heads, rows, total, longest);
+  *splits = longest ? (longest + *split - 1) / *split : 1;
+  return *splits == 1 ? 0
+                      : static_cast<size_t>(m) * p->heads * *splits * rows * (p->dim + 2) * sizeof(float);
+}
+
 }  // namespace
 
 extern "C" {
@@ -934,6 +1030,148 @@ int tsattn_key_mask_lengths(const uint8_t *mask, int64_t stride_b, int64_t strid
   return hip_status(tsattn::launch_key_mask_lengths(mask, stride_b, stride_k, batch, len_kv, kv_len,
                                                     kv_prefix, static_cast<hipStream_t>(stream)),
                     "key mask lengths launch");
+}
+
+size_t tsattn_pages4_page_bytes(int32_t heads, int32_t page_size, int32_t dim) {
+  return pages4_sizes_ok(heads, page_size, dim) ? tsattn::page4_bytes(heads, page_size, dim) : 0;
+}
+
+int tsattn_pages4_append(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t len, const tsattn_view *k,
+                         const tsattn_view *v, const int32_t *rows, const int32_t *lens, const void *cos,
+                         const void *sin, void *stream) {
+  tsattn::Pages4 pg;
+  int rc = check_pages4(p, dtype, n, len, rows, lens, &pg);
+  if (rc || (rc = check_rows4(k, dtype, "key rows")) || (rc = check_rows4(v, dtype, "value rows")) ||
+      (rc = check_tables4(cos, sin)))
+    return rc;
+  for (int32_t i = 0; i < n; ++i)
+    if (static_cast<int64_t>(lens[i]) + len > p->table_stride * p->page_size ||
+        static_cast<int64_t>(lens[i]) + len > INT32_MAX / 4)
+      return fail(TSATTN_ERR_INVALID, "paged cache: %d positions after %d of sequence %d exceed its table", len,
+                  lens[i], i);
+  char *seen = static_cast<char *>(calloc(static_cast<size_t>(p->table_rows), 1));
+  if (!seen) return fail(TSATTN_ERR_INVALID, "paged cache: out of host memory");
+  const bool ok = distinct(n, rows, seen);
+  free(seen);
+  if (!ok) return fail(TSATTN_ERR_INVALID, "paged cache: an append needs different table rows");
+  for (int32_t i0 = 0; i0 < n && !rc; i0 += tsattn::kSeqs) {
+    tsattn::Seqs s;
+    const int m = take_seqs(&s, n, i0, rows, lens);
+    rc = hip_status(tsattn::launch_pages4_append(pg, dtype, m, len, seq_view(k, i0, dtype), seq_view(v, i0, dtype), s,
+                                                 cos, sin, static_cast<hipStream_t>(stream)),
+                    "paged append launch");
+  }
+  return rc;
+}
+
+int tsattn_pages4_read(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t len, const tsattn_view *k,
+                       const tsattn_view *v, const int32_t *rows, const int32_t *lens, const int32_t *first,
+                       void *stream) {
+  tsattn::Pages4 pg;
+  int rc = check_pages4(p, dtype, n, len, rows, lens, &pg);
+  if (rc || (rc = check_rows4(k, dtype, "key output")) || (rc = check_rows4(v, dtype, "value output"))) return rc;
+  if (!first) return fail(TSATTN_ERR_INVALID, "paged cache: first positions are NULL");
+  for (int32_t i = 0; i < n; ++i)
+    if (first[i] < 0 || static_cast<int64_t>(first[i]) + len > INT32_MAX / 4)
+      return fail(TSATTN_ERR_INVALID, "paged cache: sequence %d is read from position %d", i, first[i]);
+  for (int32_t i0 = 0; i0 < n && !rc; i0 += tsattn::kSeqs) {
+    tsattn::Seqs s;
+    const int m = take_seqs(&s, n, i0, rows, lens);
+    rc = hip_status(tsattn::launch_pages4_read(pg, dtype, m, len, seq_view(k, i0, dtype), seq_view(v, i0, dtype), s,
+                                               first + i0, static_cast<hipStream_t>(stream)),
+                    "paged read launch");
+  }
+  return rc;
+}
+
+size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q,
+                                      int32_t len_q, const int32_t *lens) {
+  if (!p || !lens || n <= 0 || heads_q <= 0 || len_q <= 0 || !pages4_sizes_ok(p->heads, p->page_size, p->dim) ||
+      heads_q % p->heads || static_cast<int64_t>(heads_q / p->heads) * len_q > (1 << 18))
+    return 0;
+  size_t most = 0;
+  for (int32_t i0 = 0; i0 < n; i0 += tsattn::kSeqs) {  // (groups of sequences follow each other in it)
+    int split, splits;
+    const size_t need = plan_attend4(p, dtype, n - i0 < tsattn::kSeqs ? n - i0 : tsattn::kSeqs,
+                                     heads_q / p->heads * len_q, lens + i0, &split, &splits);
+    most = need > most ? need : most;
+  }
+  return most;
+}
+
+int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q, int32_t len_q,
+                         double scale, int32_t is_causal, const tsattn_view *q, const tsattn_view *out,
+                         const int32_t *rows, const int32_t *lens, const void *cos, const void *sin,
+                         void *workspace, size_t workspace_bytes, void *stream) {
+  tsattn::Attend4 a{};
+  int rc = check_pages4(p, dtype, n, len_q, rows, lens, &a.p);
+  if (rc || (rc = check_rows4(q, dtype, "query")) || (rc = check_rows4(out, dtype, "output")) ||
+      (rc = check_tables4(cos, sin)))
+    return rc;
+  if (heads_q <= 0 || heads_q % p->heads)
+    return fail(TSATTN_ERR_INVALID,
+                "grouped-query attention requires enable_gqa and query heads divisible by KV heads");
+  if (!isfinite(scale)) return fail(TSATTN_ERR_INVALID, "attention scale must be finite");
+  const int64_t r = static_cast<int64_t>(heads_q / p->heads) * len_q;
+  if (r > (1 << 18))
+    return fail(TSATTN_ERR_UNSUPPORTED, "paged attention takes fewer query rows: %lld per KV head",
+                static_cast<long long>(r));
+  const size_t need = tsattn_pages4_attend_workspace(p, dtype, n, heads_q, len_q, lens);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 4))
+    return fail(TSATTN_ERR_INVALID, "paged attention workspace too small: %zu < %zu bytes", workspace_bytes, need);
+  a.ws = static_cast<float *>(workspace);
+  a.cos = cos, a.sin = sin;
+  a.heads_q = heads_q, a.rep = heads_q / p->heads, a.len_q = len_q, a.rows = static_cast<int>(r);
+  a.causal = is_causal ? 1 : 0;
+  a.sl = static_cast<float>(scale) * tsattn::kLog2e;
+  g_last_path = 3;
+  for (int32_t i0 = 0; i0 < n && !rc; i0 += tsattn::kSeqs) {
+    a.n = take_seqs(&a.s, n, i0, rows, lens);
+    plan_attend4(p, dtype, a.n, a.rows, lens + i0, &a.split, &a.splits);
+    a.q = seq_view(q, i0, dtype), a.o = seq_view(out, i0, dtype);
+    rc = hip_status(tsattn::launch_attend4(a, dtype, static_cast<hipStream_t>(stream)), "paged attention launch");
+  }
+  return rc;
+}
+
+int tsattn_pages4_copy(const void *from, int64_t from_pages, void *to, int64_t to_pages, size_t page_bytes,
+                       int32_t n, const int32_t *src, const int32_t *dst, void *stream) {
+  if (!from || !to || !src || !dst) return fail(TSATTN_ERR_INVALID, "page copy: pointer is NULL");
+  if (n <= 0 || from_pages <= 0 || to_pages <= 0 || from_pages > INT32_MAX || to_pages > INT32_MAX || !page_bytes)
+    return fail(TSATTN_ERR_INVALID, "page copy: sizes must be positive");
+  if (page_bytes % 16 || (reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to)) % 16)
+    return fail(TSATTN_ERR_UNSUPPORTED, "page copy: pools and pages must be 16-byte aligned");
+  for (int32_t i = 0; i < n; ++i)
+    if (src[i] < 0 || src[i] >= from_pages || dst[i] < 0 || dst[i] >= to_pages)
+      return fail(TSATTN_ERR_INVALID, "page copy: page %d -> %d out of range", src[i], dst[i]);
+  // written pages are marked; within one pool none of them may be read
+  char *seen = static_cast<char *>(calloc(static_cast<size_t>(to_pages), 1));
+  if (!seen) return fail(TSATTN_ERR_INVALID, "page copy: out of host memory");
+  bool ok = distinct(n, dst, seen);
+  if (from == to)
+    for (int32_t i = 0; i < n && ok; ++i) ok = src[i] >= to_pages || !seen[src[i]];
+  free(seen);
+  if (!ok) return fail(TSATTN_ERR_INVALID, "page copy: a page is written twice, or read and written");
+  return hip_status(tsattn::launch_pages4_copy(static_cast<const char *>(from), static_cast<char *>(to),
+                                               static_cast<int64_t>(page_bytes), n, src, dst,
+                                               static_cast<hipStream_t>(stream)),
+                    "page copy launch");
+}
+
+int tsattn_pages4_set(int32_t *table, int64_t entries, int32_t n, const int32_t *at, const int32_t *value,
+                      void *stream) {
+  if (!table || !at || !value) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  if (n <= 0 || entries <= 0 || entries > INT32_MAX)
+    return fail(TSATTN_ERR_INVALID, "page table: sizes must be positive");
+  for (int32_t i = 0; i < n; ++i)
+    if (at[i] < 0 || at[i] >= entries) return fail(TSATTN_ERR_INVALID, "page table: entry %d out of range", at[i]);
+  char *seen = static_cast<char *>(calloc(static_cast<size_t>(entries), 1));
+  if (!seen) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
+  const bool ok = distinct(n, at, seen);
+  free(seen);
+  if (!ok) return fail(TSATTN_ERR_INVALID, "page table: an entry is set twice");
+  return hip_status(tsattn::launch_pages4_set(table, n, at, value, static_cast<hipStream_t>(stream)),
+                    "page table launch");
 }
 
 }  // extern "C"

@@ -42,26 +42,6 @@ namespace {
 
 constexpr int BN = 32;  // keys per tile
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-// 16x16x32, lane l = 16 g + c: A[c][8 g + j], B[8 g + j][c], j = 0..7;
-// C[4 g + i][c], i = 0..3.
-template <typename T>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (std::is_same_v<T, bf16>)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// Max over the four lanes c, c + 16, c + 32, c + 48 (v_permlane16_swap trades
-// the odd 16-lane rows of one register for the even ones of the other).
-__device__ __forceinline__ float quad_row_max(float x) {
-  unsigned a = __builtin_bit_cast(unsigned, x), b = a;
-  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-  return half_swap_max3(fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
-}
-
 // Waves per workgroup: 64 KiB of tiles, so two workgroups share a CU and one's
 // prologue and merge run under the other's stream.
 template <int D, bool Q8>

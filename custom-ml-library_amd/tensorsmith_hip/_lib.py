@@ -111,7 +111,23 @@ class StepDesc(ctypes.Structure):
     ]
 
 
+class Pages4(ctypes.Structure):
+    """``tsattn_pages4``: a 4-bit paged cache's pool and page table."""
+
+    _fields_ = [
+        ("pool", c_void_p),
+        ("num_pages", c_int64),
+        ("heads", c_int32),
+        ("page_size", c_int32),
+        ("dim", c_int32),
+        ("table", c_void_p),
+        ("table_rows", c_int64),
+        ("table_stride", c_int64),
+    ]
+
+
 _PV = POINTER(View)
+_P4 = POINTER(Pages4)
 _PP = POINTER(Problem)
 _PR = POINTER(RopeDesc)
 
@@ -206,6 +222,27 @@ SIGNATURES = {
     ),
     "tsattn_cached_step_workspace": (c_size_t, [POINTER(StepDesc)]),
     "tsattn_cached_step": (c_int, [POINTER(StepDesc), c_void_p, c_size_t, c_void_p]),
+    "tsattn_pages4_page_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "tsattn_pages4_append": (
+        c_int,
+        [_P4, c_int32, c_int32, c_int32, _PV, _PV, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "tsattn_pages4_read": (
+        c_int,
+        [_P4, c_int32, c_int32, c_int32, _PV, _PV, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "tsattn_pages4_attend_workspace": (
+        c_size_t, [_P4, c_int32, c_int32, c_int32, c_int32, c_void_p]),
+    "tsattn_pages4_attend": (
+        c_int,
+        [_P4, c_int32, c_int32, c_int32, c_int32, c_double, c_int32, _PV, _PV, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "tsattn_pages4_copy": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_size_t, c_int32, c_void_p, c_void_p, c_void_p],
+    ),
+    "tsattn_pages4_set": (c_int, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p]),
     "tsattn_key_mask_lengths": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p],

@@ -6,6 +6,7 @@ from .cache import KVCache
 from .checkpoint import checkpoint
 from .layers import GELU, Dropout, Embedding, LayerNorm, Linear
 from .module import Module, Parameter
+from .paged import PagedKVCache, paged_attention
 from .transformer import (
     MultiHeadAttention, RMSNorm, SiLU, SwiGLU, TransformerConfig, TransformerDecoderBlock,
     TransformerLM, sample_logits,
@@ -13,7 +14,7 @@ from .transformer import (
 
 __all__ = [
     "Dropout", "Embedding", "GELU", "KVCache", "LayerNorm", "Linear", "Module",
-    "MultiHeadAttention", "Parameter", "RMSNorm", "SiLU", "SwiGLU", "TransformerConfig",
-    "TransformerDecoderBlock", "TransformerLM", "checkpoint", "functional", "rotary_embedding",
-    "sample_logits", "scaled_dot_product_attention",
+    "MultiHeadAttention", "PagedKVCache", "Parameter", "RMSNorm", "SiLU", "SwiGLU", "TransformerConfig",
+    "TransformerDecoderBlock", "TransformerLM", "checkpoint", "functional", "paged_attention",
+    "rotary_embedding", "sample_logits", "scaled_dot_product_attention",
 ]

@@ -1,0 +1,484 @@
+"""A key/value cache held in 4 bits, in pages, and the attention that reads it.
+
+Beside ``KVCache`` (one array, one length for all rows, 16 / 32 bits or int8): a
+``PagedKVCache`` holds 4.5 bits a channel, its rows have lengths of their own, and a
+row takes pages of ``page_size`` positions from a common pool as it grows.  Rows may
+share pages -- beams, answers to one prompt -- until one of them appends into a
+shared page, which is then copied for it.
+
+The format (``include/tsattn.h``, ``tsattn_pages4``): e2m1 codes and a scale of 6
+significant bits for each 32 channels, so that what the cache stands for is exact in
+16 bits.  ``paged_attention`` reads the codes themselves for few query rows per KV
+head (``tsattn_pages4_attend``); for a prompt's many rows the pages are
+dequantised once and attended on the 16-bit or fp32 matrix cores.
+
+Page tables and reference counts are the host's; lengths travel with each launch.
+Calls captured into a HIP graph replay the positions they were captured at.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+
+from .. import _lib
+from ..device import device as parse_device
+from ..device import launch
+from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
+from .attention import (_aligned16, _dtype_code, _rope_rows, _view, rope_tables,
+                        scaled_dot_product_attention)
+
+# Query rows per KV head from which dequantising the pages once and attending on
+# the matrix cores is the faster way.
+PROMPT_ROWS = 128
+_MOST_SET = 1024  # table entries written by the kernel; more go up as one copy
+
+
+def _ints(x):
+    return np.ascontiguousarray(x, np.int32)
+
+
+def _ptr(x) -> ctypes.c_void_p:
+    return ctypes.c_void_p(x.ctypes.data)
+
+
+def _rows(t):
+    """``t`` with rows that the kernels read as they are: 16-byte aligned, channels side by side."""
+    import torch
+
+    return t if t.stride(-1) == 1 and _aligned16(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+class _Pages:
+    """The pool, the page table (host and device) and the rows' lengths."""
+
+    def __init__(self, rows: int, heads: int, dim: int, columns: int, page_size: int, num_pages: int, dev):
+        import torch
+
+        self.heads, self.dim, self.page_size, self.device = heads, dim, page_size, dev
+        self.page_bytes = int(_lib.load().tsattn_pages4_page_bytes(heads, page_size, dim))
+        if not self.page_bytes:
+            raise NotImplementedError("paged caches take head dims 32, 64, 128 and 256, up to 4096 heads and "
+                                      "pages of 32, 64, .. 4096 positions")
+        # (what no append has written weighs nothing: positions past a row's length are masked)
+        self.pool = torch.empty((num_pages, self.page_bytes), dtype=torch.uint8, device=dev.torch)
+        self.table = torch.zeros((rows, columns), dtype=torch.int32, device=dev.torch)
+        self.host = np.full((rows, columns), -1, np.int32)
+        self.lengths = np.zeros(rows, np.int32)
+        self.refs = np.zeros(num_pages, np.int32)
+        self.stack = np.arange(num_pages - 1, -1, -1, dtype=np.int32)  # free pages, the next one last
+        self.free = num_pages
+        self.quiet = 0  # positions that every row can take before any page changes
+        self.describe()
+
+    def describe(self) -> None:
+        d = _lib.Pages4()
+        d.pool, d.num_pages = self.pool.data_ptr(), self.pool.shape[0]
+        d.heads, d.page_size, d.dim = self.heads, self.page_size, self.dim
+        d.table, d.table_rows, d.table_stride = self.table.data_ptr(), *self.host.shape
+        self.desc = d
+
+    # -- pages ----------------------------------------------------------------
+
+    def take(self, n: int):
+        self.free -= n
+        pages = self.stack[self.free:self.free + n][::-1].copy()
+        self.refs[pages] = 1
+        return pages
+
+    def drop(self, pages) -> None:
+        """One reference less for each of ``pages`` (a page may be named twice)."""
+        np.subtract.at(self.refs, pages, 1)
+        gone = np.unique(pages)
+        gone = gone[self.refs[gone] == 0][::-1]
+        self.stack[self.free:self.free + len(gone)] = gone
+        self.free += len(gone)
+
+    def upload(self, rows, columns) -> None:
+        """Entries of the host's table to the device's."""
+        if not len(rows):
+            return
+        if len(rows) > _MOST_SET:
+            import torch
+
+            self.table.copy_(torch.from_numpy(np.maximum(self.host, 0)))
+            return
+        at, value = _ints(rows * self.host.shape[1] + columns), _ints(self.host[rows, columns])
+        _lib.check(launch(self.device, _lib.load().tsattn_pages4_set, self.table.data_ptr(), self.host.size,
+                          len(at), _ptr(at), _ptr(value)), "page table")
+
+    def move(self, source, target, src, dst) -> None:
+        src, dst = _ints(src), _ints(dst)
+        _lib.check(launch(self.device, _lib.load().tsattn_pages4_copy, source.data_ptr(), source.shape[0],
+                          target.data_ptr(), target.shape[0], self.page_bytes, len(src), _ptr(src), _ptr(dst)),
+                   "page copy")
+
+    def grow(self, rows, n: int) -> None:
+        """Pages of their own for the next ``n`` positions of ``rows``; nothing changes if there are too few."""
+        size, lens = self.page_size, self.lengths[rows]
+        first, stop = lens // size, -(-(lens + n) // size)
+        # a page that a row appends into and shares: all its rows but one get copies
+        into = np.flatnonzero(lens % size)
+        page = self.host[rows[into], first[into]]
+        shared = into[self.refs[page] > 1]
+        page = self.host[rows[shared], first[shared]]
+        order = np.argsort(page, kind="stable")
+        shared, page = shared[order], page[order]
+        nth = np.arange(len(page)) - np.searchsorted(page, page)  # of the appending rows of its page
+        copied = nth < self.refs[page] - 1
+        shared, page = shared[copied], page[copied]
+        span = int((stop - first).max())
+        columns = first[:, None] + np.arange(span)
+        wanted = columns < stop[:, None]
+        wanted &= self.host[rows[:, None], np.minimum(columns, self.host.shape[1] - 1)] < 0
+        at, j = np.nonzero(wanted)
+        if len(page) + len(at) > self.free:
+            raise ValueError(f"page pool exhausted: {len(page) + len(at)} pages needed, {self.free} free")
+        if len(page):
+            own = self.take(len(page))
+            self.move(self.pool, self.pool, page, own)
+            self.host[rows[shared], first[shared]] = own
+            self.drop(page)
+        if len(at):
+            self.host[rows[at], columns[at, j]] = self.take(len(at))
+        self.upload(np.concatenate((rows[shared], rows[at])), np.concatenate((first[shared], columns[at, j])))
+
+    def advance(self, rows, n: int, whole: bool) -> None:
+        self.lengths[rows] += n
+        self.quiet = max(self.quiet - n, 0)
+        if whole and not self.quiet:  # what is left in each row's last page, if the row has it alone
+            part = self.lengths % self.page_size
+            pages = self.host[np.arange(len(part)), self.lengths // self.page_size % self.host.shape[1]]
+            alone = (part > 0) & (self.refs[np.maximum(pages, 0)] == 1)
+            self.quiet = int(np.where(alone, self.page_size - part, 0).min())
+
+    def cut(self, rows, lengths) -> None:
+        """``rows`` end at ``lengths``; pages wholly past them are given back."""
+        self.quiet = 0
+        self.lengths[rows] = lengths
+        past = np.arange(self.host.shape[1])[None, :] >= -(-self.lengths[rows] // self.page_size)[:, None]
+        past &= self.host[rows] >= 0
+        at, column = np.nonzero(past)
+        if len(at):
+            pages = self.host[rows[at], column]
+            self.host[rows[at], column] = -1
+            self.drop(pages)
+
+
+class PagedKVCache:
+    """4-bit keys and values of ``batch_size`` sequences of up to ``max_seq_len`` positions.
+
+    ``num_pages`` pages of ``page_size`` (32, 64, 128, .. 4096) positions are
+    allocated at once; by default as many as the rows can need.  ``dtype`` (float32,
+    float16 or bfloat16) is that of the keys and values given and read back.
+    Inference only, like ``KVCache``.
+    """
+
+    def __init__(self, batch_size: int, num_heads: int, head_dim: int, max_seq_len: int, *, device=None,
+                 dtype="float32", page_size: int = 64, num_pages: int | None = None):
+        if min(batch_size, num_heads, head_dim, max_seq_len, page_size) <= 0:
+            raise ValueError("cache dimensions and capacity must be positive")
+        dev = parse_device(device)
+        if dev.type != "hip":
+            raise RuntimeError("tensorsmith_hip keeps KV caches on hip devices")
+        self.dtype = backend_dtype(dtype, dev)
+        if str(self.dtype).split(".")[-1] not in ("float32", "float16", "bfloat16"):
+            raise TypeError("paged caches hold float32, float16 or bfloat16 rows")
+        columns = -(-max_seq_len // page_size)
+        if num_pages is None:
+            num_pages = batch_size * columns
+        if num_pages <= 0:
+            raise ValueError("cache dimensions and capacity must be positive")
+        self.max_seq_len = max_seq_len
+        self._core = _Pages(batch_size, num_heads, head_dim, columns, page_size, num_pages, dev)
+        self._select(np.arange(batch_size, dtype=np.int32))
+
+    def _select(self, rows) -> None:
+        self._rows = rows
+        self._whole = len(rows) == len(self._core.lengths) and bool((rows == np.arange(len(rows))).all())
+
+    # -- what it is -----------------------------------------------------------
+
+    batch_size = property(lambda self: len(self._rows))
+    num_heads = property(lambda self: self._core.heads)
+    head_dim = property(lambda self: self._core.dim)
+    value_dim = head_dim
+    device = property(lambda self: self._core.device)
+    page_size = property(lambda self: self._core.page_size)
+    num_pages = property(lambda self: self._core.pool.shape[0])
+    quantized = True
+
+    @property
+    def lengths(self) -> tuple:
+        """Cached positions of every row."""
+        return tuple(self._core.lengths[self._rows].tolist())
+
+    @property
+    def length(self) -> int:
+        """Cached positions of the longest row."""
+        return int(self._core.lengths[self._rows].max())
+
+    @property
+    def pages_in_use(self) -> int:
+        return self.num_pages - self._core.free
+
+    @property
+    def memory_bytes(self) -> int:
+        """Allocated persistent payload: the pool and its table."""
+        return self._core.pool.numel() + 4 * self._core.table.numel()
+
+    def __len__(self):
+        return self.length
+
+    def __repr__(self):
+        return (f"PagedKVCache(rows={self.batch_size}, length={self.length}, capacity={self.max_seq_len}, "
+                f"pages={self.pages_in_use}/{self.num_pages}, device='{self.device}')")
+
+    # -- rows in and out ------------------------------------------------------
+
+    def append(self, key: Tensor, value: Tensor, *, rotary_base: float | None = None) -> None:
+        """Quantise and append ``key`` and ``value`` [B, H, T, D], each row at its own length.
+
+        ``rotary_base``: rotate the keys by RoPE at those positions first, as
+        ``rotary_embedding`` does.  Nothing changes if the pool has too few free pages.
+        """
+        self._check(key, value)
+        core, steps = self._core, key.shape[2]
+        lens = core.lengths if self._whole else core.lengths[self._rows]
+        most = int(lens.max()) + steps
+        if steps == 0 or most > self.max_seq_len:
+            raise ValueError(f"cache capacity {self.max_seq_len} exceeded or empty append")
+        cos = sin = None
+        if rotary_base is not None:
+            if rotary_base <= 0 or not math.isfinite(rotary_base):
+                raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
+            cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
+        k, v = (_rows(t._data.to(self.dtype)) for t in (key, value))
+        if not (self._whole and steps <= core.quiet):
+            core.grow(self._rows, steps)
+        _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, _dtype_code(self.dtype), len(lens),
+                          steps, _view(k), _view(v), _ptr(self._rows), _ptr(lens), cos, sin), "paged append")
+        core.advance(self._rows, steps, self._whole)
+
+    def _check(self, key: Tensor, value: Tensor) -> None:
+        """``KVCache``'s refusals, in its order."""
+        if key.device != self.device or value.device != self.device:
+            raise ValueError("cache and key/value tensors must be on the same device")
+        if is_grad_enabled() and (key.requires_grad or value.requires_grad):
+            raise RuntimeError("KVCache is inference-only; use no_grad() for differentiable inputs")
+        if key.ndim != 4 or key.shape[:2] != (self.batch_size, self.num_heads) or key.shape[-1] != self.head_dim:
+            raise ValueError("key shape does not match cache configuration")
+        if value.shape != key.shape:
+            raise ValueError("value shape does not match cache configuration")
+
+    def get(self, last: int | None = None) -> tuple[Tensor, Tensor]:
+        """Keys and values as they are held [B, H, T, D]: all positions up to the longest
+        row's length (zero past a row's own), or the ``last`` positions of every row."""
+        import torch
+
+        core = self._core
+        lens = core.lengths[self._rows]
+        if last is not None and not 0 < last <= lens.min():
+            raise ValueError("the last positions read must be between one and the shortest row's length")
+        steps = int(lens.max()) if last is None else last
+        first = np.zeros_like(lens) if last is None else lens - np.int32(last)
+        out = [torch.empty((len(lens), core.heads, steps, core.dim), dtype=self.dtype, device=core.pool.device)
+               for _ in range(2)]
+        if steps:
+            _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, _dtype_code(self.dtype),
+                              len(lens), steps, _view(out[0]), _view(out[1]), _ptr(self._rows), _ptr(lens),
+                              _ptr(first)), "paged read")
+        return tuple(Tensor(x, device=core.device) for x in out)
+
+    # -- rows and pages -------------------------------------------------------
+
+    def rows(self, indices) -> "PagedKVCache":
+        """These rows as a cache of their own over the same pages: to fill a row that was
+        freed, or to step some rows alone.  Both change together."""
+        index = self._indices(indices, None)
+        if len(index) == 0 or len(np.unique(index)) != len(index):
+            raise ValueError("rows must be different and at least one")
+        view = object.__new__(PagedKVCache)
+        view.dtype, view.max_seq_len, view._core = self.dtype, self.max_seq_len, self._core
+        view._select(np.ascontiguousarray(self._rows[index]))
+        return view
+
+    def _indices(self, indices, shape):
+        host = np.asarray(to_numpy(indices._data if isinstance(indices, Tensor) else indices))
+        if host.ndim != 1 or (shape is not None and host.shape != shape) or (host.size and host.dtype.kind not in "iu"):
+            raise ValueError("beam indices must be one integer per cache batch row" if shape is not None
+                             else "row indices must be integers")
+        if host.size and ((host < 0).any() or (host >= self.batch_size).any()):
+            raise ValueError("beam index out of range" if shape is not None else "row index out of range")
+        return host.astype(np.int32)
+
+    def reset(self) -> None:
+        """Every row empty, its pages given back."""
+        self._core.cut(self._rows, 0)
+
+    def free(self, indices) -> None:
+        """These rows empty, their pages given back."""
+        index = self._indices(indices, None)
+        if len(index):
+            self._core.cut(self._rows[np.unique(index)], 0)
+
+    def truncate(self, length) -> None:
+        """Cut every row to ``length`` positions, or to a length of its own (a sequence of them);
+        pages wholly past it are given back."""
+        want = np.asarray(length)
+        if want.dtype.kind not in "iu" or want.shape not in ((), (self.batch_size,)):
+            raise ValueError("truncate takes one integer length, or one per row")
+        lens = self._core.lengths[self._rows]
+        if (want < 0).any() or (want > lens).any():
+            raise ValueError("truncate length must be between zero and the current length")
+        if (want != lens).any():
+            self._core.cut(self._rows, want)
+
+    def reorder(self, indices) -> None:
+        """Row i becomes row ``indices[i]``, sharing its pages: no keys or values move.  Rows that
+        take over the same row share until one appends (``append`` copies the page)."""
+        core, index = self._core, self._indices(indices, (self.batch_size,))
+        old, new = core.host[self._rows], core.host[self._rows[index]]
+        core.quiet = 0
+        core.lengths[self._rows] = core.lengths[self._rows[index]]
+        core.host[self._rows] = new
+        np.add.at(core.refs, new[new >= 0], 1)
+        core.drop(old[old >= 0])
+        at, column = np.nonzero((new != old) & (new >= 0))
+        core.upload(self._rows[at], column)
+
+    def copy(self, num_pages: int | None = None) -> "PagedKVCache":
+        """A cache of these rows with a pool of its own (``num_pages``, by default as many as this
+        one has), its pages in use side by side; rows that share pages share them there."""
+        core = self._core
+        host = core.host[self._rows]
+        live = np.unique(host[host >= 0])
+        num_pages = self.num_pages if num_pages is None else num_pages
+        if num_pages < max(len(live), 1):
+            raise ValueError(f"{len(live)} pages are in use")
+        other = object.__new__(PagedKVCache)
+        other.dtype, other.max_seq_len = self.dtype, self.max_seq_len
+        there = other._core = _Pages(len(host), core.heads, core.dim, host.shape[1], core.page_size, num_pages,
+                                     core.device)
+        other._select(np.arange(len(host), dtype=np.int32))
+        there.lengths[:] = core.lengths[self._rows]
+        if len(live):
+            there.take(len(live))
+            core.move(core.pool, there.pool, live, np.arange(len(live)))
+            self._renumber(there, host, live)
+        return other
+
+    def compact(self, num_pages: int | None = None) -> int:
+        """Move the pages in use to the front of the pool, and with ``num_pages`` into a pool of that
+        size (smaller or larger); returns how many are in use."""
+        core = self._core
+        live = np.unique(core.host[core.host >= 0])
+        n = len(live)
+        if num_pages is not None and num_pages < max(n, 1):
+            raise ValueError(f"{n} pages are in use")
+        if num_pages is None:
+            moved, holes = live[live >= n], np.setdiff1d(np.arange(n, dtype=np.int32), live)
+            to = live.copy()
+            to[live >= n] = holes
+            if len(moved):
+                core.move(core.pool, core.pool, moved, holes)
+            num_pages = self.num_pages
+        else:
+            import torch
+
+            to = np.arange(n, dtype=np.int32)
+            pool = torch.empty((num_pages, core.page_bytes), dtype=torch.uint8, device=core.pool.device)
+            if n:
+                core.move(core.pool, pool, live, to)
+            core.pool = pool
+        core.refs = np.zeros(num_pages, np.int32)
+        core.stack = np.arange(num_pages - 1, -1, -1, dtype=np.int32)
+        core.free = num_pages - n
+        core.quiet = 0
+        if n:
+            self._renumber(core, core.host, live, to)
+        core.describe()
+        return n
+
+    @staticmethod
+    def _renumber(core, host, live, to=None) -> None:
+        """``core``'s table: ``host`` with the pages ``live`` numbered ``to`` (0, 1, ..)."""
+        to = np.arange(len(live), dtype=np.int32) if to is None else to
+        held = host >= 0
+        new = np.full_like(host, -1)
+        new[held] = to[np.searchsorted(live, host[held])]
+        at, column = np.nonzero(held & (new != core.host))
+        core.host = new
+        core.refs[:] = np.bincount(new[held], minlength=len(core.refs))
+        core.upload(at, column)
+
+
+def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = True, scale: float | None = None,
+                    rotary_base: float | None = None) -> Tensor:
+    """Attention of ``query`` [B, Hq, T, D] over a ``PagedKVCache``'s rows.
+
+    The queries are at the last T positions of their row (append their keys and values
+    first): with ``is_causal`` each sees the positions up to its own, else all.  Query
+    heads may be a multiple of the cache's.  ``rotary_base`` rotates the queries by
+    RoPE at those positions.  A query that sees nothing gives zero.  Inference only.
+    """
+    if query.ndim != 4:
+        raise ValueError("attention expects [batch, heads, sequence, channels]")
+    if query.device != cache.device:
+        raise ValueError("attention tensors must be on the same device")
+    if query._data.dtype != cache.dtype:
+        raise TypeError("attention inputs must have the same floating-point dtype")
+    b, heads, steps, dim = query.shape
+    if b != cache.batch_size or dim != cache.head_dim:
+        raise ValueError("query shape does not match cache configuration")
+    if heads % cache.num_heads or min(query.shape) <= 0:
+        raise ValueError("grouped-query attention requires enable_gqa and query heads divisible by KV heads")
+    if is_grad_enabled() and query.requires_grad:
+        raise RuntimeError("KVCache is inference-only; use no_grad() for differentiable inputs")
+    multiplier = 1 / math.sqrt(dim) if scale is None else scale
+    if not math.isfinite(multiplier):
+        raise ValueError("attention scale must be finite")
+    if rotary_base is not None and (rotary_base <= 0 or not math.isfinite(rotary_base)):
+        raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
+    import torch
+
+    core = cache._core
+    lens = core.lengths if cache._whole else core.lengths[cache._rows]
+    if heads // cache.num_heads * steps >= PROMPT_ROWS and dim <= 128 and lens.min() >= steps:
+        return _prompt(query, cache, lens, is_causal, multiplier, rotary_base)
+    q = _rows(query._data)
+    cos = sin = None
+    if rotary_base is not None:
+        cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, dim, q.dtype, q.device,
+                                                      max(int(lens.max()), steps)))
+    out = torch.empty((b, heads, steps, dim), dtype=q.dtype, device=q.device)
+    lib, code = _lib.load(), _dtype_code(q.dtype)
+    nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, _ptr(lens))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.check(launch(core.device, lib.tsattn_pages4_attend, core.desc, code, b, heads, steps, multiplier,
+                      int(is_causal), _view(q), _view(out), _ptr(cache._rows), _ptr(lens), cos, sin,
+                      None if ws is None else ws.data_ptr(), nbytes), "paged attention")
+    return Tensor._from_op(out, (query,), None, "paged_attention")
+
+
+def _prompt(query: Tensor, cache: PagedKVCache, lens, is_causal: bool, scale: float, rotary_base) -> Tensor:
+    """Many query rows: the values dequantised once, then the attention of arrays; rows of
+    unequal length one after the other."""
+    import torch
+
+    def attend(q, held, n):
+        if rotary_base is not None:
+            q = _rope_rows(q, n - q.shape[2], rotary_base, q.shape[3], False, cache.device)
+        k, v = held.get()
+        return scaled_dot_product_attention(
+            Tensor(q, device=cache.device), k, v, None, 0.0, is_causal, scale=scale,
+            causal_offset=n - q.shape[2] if is_causal else 0, enable_gqa=q.shape[1] != held.num_heads)._data
+
+    with torch.cuda.device(cache.device.index):  # (attention launches on the current device)
+        if lens.min() == lens.max():
+            out = attend(query._data, cache, int(lens[0]))
+        else:
+            out = torch.cat([attend(query._data[i:i + 1], cache.rows([i]), int(n)) for i, n in enumerate(lens)])
+    return Tensor._from_op(out, (query,), None, "paged_attention")

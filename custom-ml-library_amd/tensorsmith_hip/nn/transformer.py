@@ -41,6 +41,7 @@ from .cache import KVCache
 from .checkpoint import checkpoint
 from .layers import Dropout, Embedding, Linear
 from .module import Module, Parameter
+from .paged import PagedKVCache, paged_attention
 
 random_uniform = _device.random_uniform
 
@@ -179,12 +180,15 @@ class MultiHeadAttention(Module):
         self.out_proj = Linear(embed_dim, embed_dim, bias=bias, device=device)
 
     def new_cache(self, batch_size: int, max_seq_len: int, *, dtype="float32",
-                  quantized: bool = False) -> KVCache:
+                  quantized: bool = False, paged: bool = False) -> KVCache | PagedKVCache:
+        if paged:
+            return PagedKVCache(batch_size, self.num_kv_heads, self.head_dim, max_seq_len,
+                                device=self.q_proj.weight.device, dtype=dtype)
         return KVCache(batch_size, self.num_kv_heads, self.head_dim, max_seq_len,
                        device=self.q_proj.weight.device, dtype=dtype, quantized=quantized)
 
     def forward(self, input: Tensor, context: Tensor | None = None, *, attn_mask=None,
-                is_causal: bool = True, cache: KVCache | None = None) -> Tensor:
+                is_causal: bool = True, cache: KVCache | PagedKVCache | None = None) -> Tensor:
         if input.ndim != 3 or input.shape[-1] != self.embed_dim:
             raise ValueError("attention input must be [batch, sequence, embed_dim]")
         source = input if context is None else context
@@ -209,6 +213,8 @@ class MultiHeadAttention(Module):
                     raise TypeError("attention masks must be boolean or floating point")
             except ValueError as error:
                 raise ValueError("attention mask is not broadcastable to [B,H,Q,K]") from error
+        if isinstance(cache, PagedKVCache):
+            return self._paged(input, cache, attn_mask, is_causal)
         if cache is not None and context is None and attn_mask is None:
             stepped = _cached_step(input, self, cache, is_causal)
             if stepped is not None:
@@ -268,6 +274,29 @@ class MultiHeadAttention(Module):
                 q, k, v, attn_mask, self.dropout_p if self.training else 0.0, is_causal,
                 causal_offset=offset, backend=self.backend,
                 enable_gqa=self.num_kv_heads != self.num_heads, _rope=rope)
+        return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
+
+
+    def _paged(self, input: Tensor, cache: PagedKVCache, attn_mask, is_causal: bool) -> Tensor:
+        """Self-attention over a paged 4-bit cache, each row at its own position."""
+        batch, steps, _ = input.shape
+        lens = cache.lengths
+        if attn_mask is not None and min(lens) != max(lens):
+            raise ValueError("attention masks over a paged cache need rows of one length")
+        q, k, v = (proj(input).reshape(batch, steps, heads, self.head_dim).permute(0, 2, 1, 3)
+                   for proj, heads in ((self.q_proj, self.num_heads), (self.k_proj, self.num_kv_heads),
+                                       (self.v_proj, self.num_kv_heads)))
+        base = 10000.0 if self.rotary else None
+        cache.append(k, v, rotary_base=base)
+        if attn_mask is None:
+            attended = paged_attention(q, cache, is_causal=is_causal, rotary_base=base)
+        else:
+            if self.rotary:
+                q = rotary_embedding(q, lens[0])
+            k, v = cache.get()
+            attended = scaled_dot_product_attention(
+                q, k, v, attn_mask, 0.0, is_causal, causal_offset=lens[0], backend=self.backend,
+                enable_gqa=self.num_kv_heads != self.num_heads)
         return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
 
 
@@ -392,13 +421,15 @@ class TransformerLM(Module):
             raise ValueError("tokens must be a nonempty integer [batch, time] tensor")
         if not isinstance(logits_to_keep, int) or not 0 <= logits_to_keep <= tokens.shape[1]:
             raise ValueError("logits_to_keep must be between zero (all) and the input length")
-        offset = 0
+        offset = before = 0
         if caches is not None:
-            if len(caches) != len(self.blocks) or len({cache.length for cache in caches}) != 1:
+            # (a paged cache's rows have positions of their own)
+            at = [cache.lengths if isinstance(cache, PagedKVCache) else cache.length for cache in caches]
+            if len(caches) != len(self.blocks) or len(set(at)) != 1:
                 raise ValueError("provide one cache per block, all at the same sequence position")
             if self.training or is_grad_enabled():
                 raise RuntimeError("cached decoding requires eval() and no_grad()")
-            offset = caches[0].length
+            offset, before = caches[0].length, at[0]
             for block, cache in zip(self.blocks, caches):
                 if cache.batch_size != tokens.shape[0] or cache.device != tokens.device:
                     raise ValueError("cache batch/device does not match tokens")
@@ -427,7 +458,7 @@ class TransformerLM(Module):
         except Exception:
             if caches is not None:
                 for cache in caches:
-                    cache.truncate(offset)
+                    cache.truncate(before)
             raise
 
     def loss(self, tokens: Tensor, targets: Tensor, *, ignore_index=-100,
@@ -436,10 +467,14 @@ class TransformerLM(Module):
                                label_smoothing=label_smoothing)
 
     def new_cache(self, batch_size: int, max_seq_len: int | None = None, *,
-                  quantized=False) -> list[KVCache]:
+                  quantized=False, paged=False) -> list[KVCache] | list[PagedKVCache]:
+        """One cache per block: in the weights' dtype, ``quantized`` in int8, or ``paged`` in 4 bits."""
         capacity = self.config.max_seq_len if max_seq_len is None else max_seq_len
         if capacity <= 0 or capacity > self.config.max_seq_len:
             raise ValueError("cache capacity must fit the model context")
+        if paged:
+            return [block.attention.new_cache(batch_size, capacity, dtype=self.token_embedding.weight.dtype,
+                                              paged=True) for block in self.blocks]
         return [
             KVCache(batch_size, block.attention.num_kv_heads, block.attention.head_dim, capacity,
                     device=self.token_embedding.weight.device,
@@ -450,8 +485,9 @@ class TransformerLM(Module):
     @no_grad()
     def generate(self, prompt: Tensor, max_new_tokens: int, *, temperature=1.0,
                  top_k: int | None = None, top_p: float = 1.0, eos_token_id: int | None = None,
-                 use_cache: bool = True, quantized_cache: bool = False) -> Tensor:
-        """Batched greedy/top-k/nucleus sampling; returns prompt plus generated tokens."""
+                 use_cache: bool = True, quantized_cache: bool = False, paged_cache: bool = False) -> Tensor:
+        """Batched greedy/top-k/nucleus sampling; returns prompt plus generated tokens.  The caches are
+        in the weights' dtype, with ``quantized_cache`` in int8, with ``paged_cache`` in 4 bits."""
         if (prompt.ndim != 2 or prompt.shape[1] == 0 or max_new_tokens < 0
                 or "int" not in str(prompt.dtype)):
             raise ValueError("invalid prompt or generation length")
@@ -469,7 +505,7 @@ class TransformerLM(Module):
         try:
             self.eval()
             caches = (self.new_cache(prompt.shape[0], prompt.shape[1] + max_new_tokens,
-                                     quantized=quantized_cache)
+                                     quantized=quantized_cache, paged=paged_cache)
                       if use_cache and max_new_tokens else None)
             result, current = prompt, prompt
             finished = torch.zeros((prompt.shape[0],), dtype=torch.bool, device=prompt._data.device)

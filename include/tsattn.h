@@ -520,6 +520,86 @@ int tsattn_key_mask_lengths(const uint8_t *mask, int64_t stride_b, int64_t strid
                             int32_t batch, int32_t len_kv, int32_t *kv_len, int32_t *kv_prefix,
                             void *stream);
 
+/*
+ * A key/value cache held in 4 bits, in pages (no counterpart in the reference, whose
+ * quantised cache is int8 and one array: src/tensorsmith/nn/cache.py:12-142).
+ *
+ * Values: each 32 channels of a row share a scale s, max|x| / 6 (in fp32) rounded to
+ * 6 significant bits (ties to even), at least 2^-27 and at most the largest whose 6 s
+ * the cache's dtype holds, NaN when one of the 32 is not finite; a channel's code is
+ * the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 to |x| / s (ties to the even code) and a
+ * sign.  The value is level * s: exact in bf16 and fp32, in f16 where s >= 2^-18.
+ *
+ * Pages: `pool` holds num_pages pages of tsattn_pages4_page_bytes each, their layout
+ * the library's own; page p of a sequence, its positions page_size p .., is the pool's
+ * page table[row * table_stride + p] for the sequence's `row` of the table.  The calls
+ * take the rows and the cached positions of their n sequences as host arrays, which
+ * are read before the call returns (a captured call replays these values).  The
+ * table's entries for the positions touched must be filled: an entry out of range is
+ * taken for page 0.  Two rows may share pages; the caller gives each row its own
+ * before it appends there.
+ */
+typedef struct tsattn_pages4 {
+  void *pool;        /* 16-byte aligned */
+  int64_t num_pages;
+  int32_t heads;     /* KV heads */
+  int32_t page_size; /* positions: 32, 64, 128, .. 4096 */
+  int32_t dim;       /* channels: 32, 64, 128 or 256 */
+  const int32_t *table; /* device [table_rows, table_stride] */
+  int64_t table_rows, table_stride;
+} tsattn_pages4;
+
+/* Bytes of one page (0: sizes the library does not take). */
+size_t tsattn_pages4_page_bytes(int32_t heads, int32_t page_size, int32_t dim);
+
+/*
+ * Quantise the rows k, v [n, heads, len, dim] (f32, f16 or bf16: the cache's dtype,
+ * rows 16-byte aligned) into positions lens[i] .. lens[i] + len - 1 of each
+ * sequence; cos / sin (tables [*, dim / 2] in dtype, 16-byte aligned, or both NULL)
+ * rotate the keys by RoPE at those positions first, bit for bit tsattn_rope.  Other
+ * positions keep what they held.  rows must differ.
+ */
+int tsattn_pages4_append(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t len, const tsattn_view *k,
+                         const tsattn_view *v, const int32_t *rows, const int32_t *lens, const void *cos,
+                         const void *sin, void *stream);
+
+/*
+ * The values of positions first[i] .. first[i] + len - 1 of each sequence into k, v
+ * [n, heads, len, dim], rounded to dtype; zero at and past its lens[i] positions.
+ */
+int tsattn_pages4_read(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t len, const tsattn_view *k,
+                       const tsattn_view *v, const int32_t *rows, const int32_t *lens, const int32_t *first,
+                       void *stream);
+
+/* Bytes of scratch tsattn_pages4_attend needs (0: none, or sizes it does not take). */
+size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q,
+                                      int32_t len_q, const int32_t *lens);
+
+/*
+ * Attention (src/tensorsmith/nn/attention.py:102-145, :175-198) of q [n, heads_q,
+ * len_q, dim] over the lens[i] cached positions of each sequence, read in 4 bits.
+ * The queries' own positions are the last len_q: with is_causal query t sees
+ * positions up to lens[i] - len_q + t, else all.  A query that sees none gives 0.
+ * cos / sin as in the append: rotate the queries at their positions.  Rows of q and
+ * out 16-byte aligned, q in the cache's dtype.
+ */
+int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q, int32_t len_q,
+                         double scale, int32_t is_causal, const tsattn_view *q, const tsattn_view *out,
+                         const int32_t *rows, const int32_t *lens, const void *cos, const void *sin,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Copy pages src[i] of a pool to pages dst[i] of a pool (the same one or another),
+ * n of them, host arrays.  Destinations must differ, and within one pool no page may
+ * be both read and written: TSATTN_ERR_INVALID.
+ */
+int tsattn_pages4_copy(const void *from, int64_t from_pages, void *to, int64_t to_pages, size_t page_bytes,
+                       int32_t n, const int32_t *src, const int32_t *dst, void *stream);
+
+/* table[at[i]] = value[i] for n entries (host arrays; at[i] < entries, all different). */
+int tsattn_pages4_set(int32_t *table, int64_t entries, int32_t n, const int32_t *at, const int32_t *value,
+                      void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,368 @@
+"""The paged 4-bit cache on the host: page tables, reference counts and copies on
+write against rows kept as lists, and the refusals of both interfaces.
+
+The kernels stand in as functions over CPU memory that keep a tag a position: what
+they are told to copy, set and append has to leave every row its own tags.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import importlib
+import random
+from contextlib import ExitStack, nullcontext
+from unittest.mock import patch
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import tensorsmith_hip as ts  # noqa: E402
+from tensorsmith_hip import _lib, nn  # noqa: E402
+
+D = importlib.import_module("tensorsmith_hip.device")
+P = importlib.import_module("tensorsmith_hip.nn.paged")
+
+
+def _at(address, n, kind):
+    address = getattr(address, "value", address)
+    return np.frombuffer((ctypes.c_char * (n * np.dtype(kind).itemsize)).from_address(address), kind)
+
+
+class Memory:
+    """The entry points over CPU memory: a page is one float64 tag a position."""
+
+    def __init__(self):
+        self.calls, self.fail = [], False
+
+    def tsattn_pages4_page_bytes(self, heads, page, dim):
+        return page * 8 if dim in (32, 64, 128, 256) else 0
+
+    def tsattn_pages4_copy(self, source, sn, target, tn, page_bytes, n, src, dst, stream):
+        src, dst = _at(src, n, np.int32), _at(dst, n, np.int32)
+        assert len(set(dst)) == n and (source != target or not set(dst) & set(src))
+        old, new = (_at(x, m * page_bytes, np.uint8).reshape(m, -1) for x, m in ((source, sn), (target, tn)))
+        new[dst] = old[src]
+        self.calls.append(("copy", n))
+        return 0
+
+    def tsattn_pages4_set(self, table, entries, n, at, value, stream):
+        at = _at(at, n, np.int32)
+        assert len(set(at)) == n
+        _at(table, entries, np.int32)[at] = _at(value, n, np.int32)
+        self.calls.append(("set", n))
+        return 0
+
+    def tsattn_pages4_append(self, desc, dtype, n, steps, k, v, rows, lens, cos, sin, stream):
+        if self.fail:
+            return _lib.ERR_HIP
+        table = _at(desc.table, desc.table_rows * desc.table_stride, np.int32).reshape(desc.table_rows, -1)
+        pool = _at(desc.pool, desc.num_pages * desc.page_size, np.float64).reshape(desc.num_pages, -1)
+        for i, (row, length) in enumerate(zip(_at(rows, n, np.int32), _at(lens, n, np.int32))):
+            for t in range(steps):
+                tag = _at(k.data + 4 * (i * k.stride[0] + t * k.stride[2]), 1, np.float32)[0]
+                pool[table[row, (length + t) // desc.page_size], (length + t) % desc.page_size] = tag
+        self.calls.append(("append", steps))
+        return 0
+
+
+@pytest.fixture
+def memory():
+    memory = Memory()
+    with ExitStack() as stack:
+        for patched in (patch.object(D.Device, "torch", torch.device("cpu")),
+                        patch.object(D, "is_available", lambda value: True),
+                        patch.object(D, "current_stream", lambda dev: 0),
+                        patch.object(torch.cuda, "current_device", lambda: 0),
+                        patch.object(torch.cuda, "device", lambda index: nullcontext()),
+                        patch.object(_lib, "load", lambda: memory),
+                        patch.object(_lib, "last_error", lambda: "")):
+            stack.enter_context(patched)
+        yield memory
+
+
+def _held(cache, row):
+    core = cache._core
+    pool = core.pool.numpy().view(np.float64).reshape(core.pool.shape[0], -1)
+    table = core.table.numpy()
+    n = core.lengths[row]
+    return [pool[table[row, p // core.page_size], p % core.page_size] for p in range(n)]
+
+
+def _sound(cache, want):
+    core = cache._core
+    used = core.host[core.host >= 0]
+    assert (np.bincount(used, minlength=len(core.refs)) == core.refs).all()
+    free = core.stack[:core.free]
+    assert len(set(free.tolist())) == core.free and not set(free.tolist()) & set(used.tolist())
+    assert core.free + len(set(used.tolist())) == len(core.refs) == cache.num_pages
+    assert list(cache.lengths) == [len(x) for x in want]
+    assert (core.host >= 0).sum(1).tolist() == [-(-len(x) // core.page_size) for x in want]
+    for row, tags in enumerate(want):
+        assert _held(cache, row) == tags, row
+
+
+def _rows(tags):
+    """Keys (and values) whose first channel is the tag: tags [B][T]."""
+    x = torch.zeros(len(tags), 2, len(tags[0]), 32)
+    x[:, :, :, 0] = torch.tensor(tags, dtype=torch.float32)[:, None]
+    return ts.Tensor(x, device="hip")
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_rows_keep_their_own_positions(memory, seed):
+    """Random appends, forks, cuts, frees and moves; a pool that sometimes runs out."""
+    rng = random.Random(seed)
+    b, most, page = rng.choice([1, 3, 5]), rng.choice([150, 400]), rng.choice([32, 64])
+    full = b * -(-most // page)
+    cache = nn.PagedKVCache(b, 2, 32, most, device="hip", page_size=page,
+                            num_pages=rng.choice([full, full, max(2, full * 2 // 3)]))
+    want, tag = [[] for _ in range(b)], [1.0]
+
+    def fresh(rows, n):
+        out = [[tag[0] + i * n + j for j in range(n)] for i in range(rows)]
+        tag[0] += rows * n
+        return out
+
+    for _ in range(60):
+        what = rng.choice(["append"] * 5 + ["some", "reorder", "truncate", "cut", "free", "compact", "resize", "copy"])
+        if what in ("append", "some"):
+            index = list(range(b)) if what == "append" else rng.sample(range(b), rng.randint(1, b))
+            n = rng.choice([1, 1, 1, 2, rng.randint(1, 90)])
+            if max(len(want[i]) for i in index) + n > most:
+                continue
+            new, target = fresh(len(index), n), cache if what == "append" else cache.rows(index)
+            try:
+                target.append(_rows(new), _rows(new))
+            except ValueError as error:
+                assert "pool exhausted" in str(error)
+            else:
+                for i, x in zip(index, new):
+                    want[i] = want[i] + x
+        elif what == "reorder":
+            index = [rng.randrange(b) for _ in range(b)]
+            memory.calls.clear()
+            cache.reorder(index)
+            assert not any(name == "copy" for name, _ in memory.calls)
+            want = [list(want[i]) for i in index]
+        elif what == "truncate":
+            n = rng.randint(0, min(len(x) for x in want))
+            cache.truncate(n)
+            want = [x[:n] for x in want]
+        elif what == "cut":
+            lens = [max(0, len(x) - rng.choice([0, 1, 40])) for x in want]
+            cache.truncate(lens)
+            want = [x[:n] for x, n in zip(want, lens)]
+        elif what == "free":
+            index = rng.sample(range(b), rng.randint(0, b))
+            cache.free(index)
+            want = [[] if i in index else x for i, x in enumerate(want)]
+        elif what == "compact":
+            assert cache.compact() == cache.pages_in_use
+            assert cache._core.host.max() < max(cache.pages_in_use, 1)
+        elif what == "resize":
+            n = cache.pages_in_use + rng.choice([0, 1, full])
+            cache.compact(max(n, 1))
+            assert cache.num_pages == max(n, 1)
+        else:
+            other = cache.copy()
+            _sound(other, want)
+            if b and max(len(x) for x in want) < most and other.pages_in_use + 2 * b <= other.num_pages:
+                other.append(_rows(fresh(b, 1)), _rows(fresh(b, 1)))  # its pages are its own
+        _sound(cache, want)
+
+
+def test_beams_copy_one_page_each(memory):
+    """Eight rows of one prompt: no copies until they append, then all but one copy its last page once."""
+    cache = nn.PagedKVCache(8, 2, 32, 300, device="hip", page_size=64)
+    cache.rows([0]).append(_rows([[float(i) for i in range(100)]]), _rows([[0.0] * 100]))
+    cache.reorder([0] * 8)
+    assert cache.pages_in_use == 2 and cache.lengths == (100,) * 8
+    memory.calls.clear()
+    cache.append(_rows([[1000.0 + i] for i in range(8)]), _rows([[0.0]] * 8))
+    assert ("copy", 7) in memory.calls and cache.pages_in_use == 1 + 8
+    memory.calls.clear()
+    for _ in range(26):  # up to and past the page's end: no more copies
+        cache.append(_rows([[1.0]] * 8), _rows([[1.0]] * 8))
+    assert not any(name == "copy" for name, _ in memory.calls)
+    # positions 102 .. 127 touch no page but their own: nothing but the append is called
+    assert [x for x in memory.calls if x[0] == "set"] == []
+
+
+def test_a_failed_append_leaves_the_lengths(memory):
+    cache = nn.PagedKVCache(2, 2, 32, 100, device="hip")
+    cache.append(_rows([[1.0], [2.0]]), _rows([[1.0], [2.0]]))
+    memory.fail = True
+    with pytest.raises(RuntimeError):
+        cache.append(_rows([[3.0] * 70, [4.0] * 70]), _rows([[3.0] * 70, [4.0] * 70]))
+    memory.fail = False
+    assert cache.lengths == (1, 1)
+    cache.append(_rows([[5.0], [6.0]]), _rows([[5.0], [6.0]]))
+    assert _held(cache, 0) == [1.0, 5.0] and _held(cache, 1) == [2.0, 6.0]
+
+
+def test_refusals(memory):
+    for sizes in ((0, 2, 32, 10), (1, 2, 32, 0)):
+        with pytest.raises(ValueError, match="positive"):
+            nn.PagedKVCache(*sizes, device="hip")
+    for kw in ({"page_size": 0}, {"num_pages": 0}):
+        with pytest.raises(ValueError, match="positive"):
+            nn.PagedKVCache(1, 2, 32, 10, device="hip", **kw)
+    with pytest.raises(NotImplementedError, match="head dims"):
+        nn.PagedKVCache(1, 2, 48, 10, device="hip")
+    with pytest.raises(RuntimeError, match="hip devices"):
+        nn.PagedKVCache(1, 2, 32, 10, device="cpu")
+    with pytest.raises(TypeError):
+        nn.PagedKVCache(1, 2, 32, 10, device="hip", dtype="float64")
+    cache = nn.PagedKVCache(2, 2, 32, 100, device="hip", num_pages=3)
+    x = lambda *s, **kw: ts.Tensor(torch.zeros(s), device="hip", **kw)  # noqa: E731
+    good = x(2, 2, 1, 32)
+    for k, v, what in ((x(2, 2, 1, 64), good, "key shape"), (x(2, 3, 1, 32), good, "key shape"),
+                       (x(2, 2, 32), good, "key shape"), (good, x(2, 2, 2, 32), "value shape"),
+                       (x(2, 2, 0, 32), x(2, 2, 0, 32), "capacity 100"), (x(2, 2, 101, 32), x(2, 2, 101, 32), "capacity"),
+                       (ts.Tensor(np.zeros((2, 2, 1, 32), np.float32)), good, "same device")):
+        with pytest.raises(ValueError, match=what):
+            cache.append(k, v)
+    with pytest.raises(RuntimeError, match="inference-only"):
+        cache.append(x(2, 2, 1, 32, requires_grad=True), good)
+    for base in (0.0, -1.0, float("inf")):
+        with pytest.raises(ValueError, match="RoPE"):
+            cache.append(good, good, rotary_base=base)
+    with pytest.raises(ValueError, match="exhausted: 4 pages needed, 3 free"):
+        cache.append(x(2, 2, 65, 32), x(2, 2, 65, 32))
+    assert cache.lengths == (0, 0) and cache.pages_in_use == 0 and (cache._core.host < 0).all()
+    cache.append(good, good)
+    for length in (2, -1, [1], [1, 2], 1.0, [[1, 1]]):
+        with pytest.raises(ValueError, match="truncate"):
+            cache.truncate(length)
+    for index in ([0], [0, 2], [0, -1], [0.0, 1.0]):
+        with pytest.raises(ValueError, match="beam ind"):
+            cache.reorder(index)
+    for index in ([], [0, 0], [2], [-1], [0.5], 0):
+        with pytest.raises(ValueError, match="row"):
+            cache.rows(index)
+    for index in ([2], [-1], [0.5], [[0]]):
+        with pytest.raises(ValueError, match="row ind"):
+            cache.free(index)
+    for last in (0, 2, -1):
+        with pytest.raises(ValueError, match="last positions"):
+            cache.get(last=last)
+    for call in (cache.compact, cache.copy):
+        with pytest.raises(ValueError, match="2 pages are in use"):
+            call(1)
+    q = x(2, 4, 1, 32)
+    for query, what, error in ((x(2, 4, 32), "expects", ValueError), (x(1, 4, 1, 32), "query shape", ValueError),
+                               (x(2, 4, 1, 64), "query shape", ValueError), (x(2, 3, 1, 32), "grouped", ValueError),
+                               (x(2, 4, 0, 32), "grouped", ValueError),
+                               (ts.Tensor(torch.zeros(2, 4, 1, 32).half(), device="hip"), "dtype", TypeError),
+                               (x(2, 4, 1, 32, requires_grad=True), "inference-only", RuntimeError)):
+        with pytest.raises(error, match=what):
+            nn.paged_attention(query, cache)
+    for kw in ({"scale": float("nan")}, {"rotary_base": 0.0}):
+        with pytest.raises(ValueError):
+            nn.paged_attention(q, cache, **kw)
+    attention = nn.MultiHeadAttention(64, 2, device="hip").eval()
+    ragged = attention.new_cache(2, 100, paged=True)
+    ragged.rows([1]).append(x(1, 2, 3, 32), x(1, 2, 3, 32))
+    with ts.no_grad(), pytest.raises(ValueError, match="one length"):
+        attention(x(2, 1, 64), cache=ragged, attn_mask=ts.Tensor(torch.ones(2, 1, 1, 4, dtype=torch.bool), device="hip"))
+
+
+# -- the C entry points: every refusal comes before a launch --------------------------
+
+
+def _ints(*x):
+    return (ctypes.c_int32 * len(x))(*x)
+
+
+def _desc(**kw):
+    d = _lib.Pages4()
+    d.pool, d.num_pages, d.heads, d.page_size, d.dim = 0x10000, 8, 2, 64, 128
+    d.table, d.table_rows, d.table_stride = 0x20000, 4, 3
+    for name, value in kw.items():
+        setattr(d, name, value)
+    return d
+
+
+def _rows_view(d=128, heads=2, steps=1, **kw):
+    v = _lib.View()
+    v.data = kw.get("data", 0x40000)
+    for i, s in enumerate(kw.get("stride", (heads * steps * d, steps * d, d, 1))):
+        v.stride[i] = s
+    return v
+
+
+OK_CALL = {"desc": {}, "dtype": _lib.F16, "rows": (0, 1), "lens": (5, 6), "steps": 1, "view": {}, "cos": None, "sin": None}
+BAD = [
+    ({"dtype": _lib.F64}, _lib.ERR_INVALID, "dtype"),
+    ({"rows": (0, 4)}, _lib.ERR_INVALID, "table row 4"),
+    ({"rows": (-1, 0)}, _lib.ERR_INVALID, "table row -1"),
+    ({"lens": (5, 193)}, _lib.ERR_INVALID, "193 positions"),
+    ({"lens": (-1, 0)}, _lib.ERR_INVALID, "-1 positions"),
+    ({"steps": 0}, _lib.ERR_INVALID, "positive"),
+    ({"desc": {"num_pages": 0}}, _lib.ERR_INVALID, "positive"),
+    ({"desc": {"pool": None}}, _lib.ERR_INVALID, "NULL"),
+    ({"desc": {"table": None}}, _lib.ERR_INVALID, "NULL"),
+    ({"desc": {"pool": 0x10008}}, _lib.ERR_UNSUPPORTED, "16-byte"),
+    ({"desc": {"dim": 96}}, _lib.ERR_UNSUPPORTED, "head dims"),
+    ({"desc": {"page_size": 48}}, _lib.ERR_UNSUPPORTED, "pages of"),
+    ({"desc": {"page_size": 8192}}, _lib.ERR_UNSUPPORTED, "pages of"),
+    ({"view": {"data": None}}, _lib.ERR_INVALID, "NULL"),
+    ({"view": {"data": 0x40008}}, _lib.ERR_UNSUPPORTED, "16-byte"),
+    ({"view": {"stride": (256, 128, 4, 1)}}, _lib.ERR_UNSUPPORTED, "16-byte"),
+    ({"view": {"stride": (256, 128, 128, 2)}}, _lib.ERR_INVALID, "innermost"),
+    ({"cos": 0x1000}, _lib.ERR_INVALID, "both"),
+    ({"cos": 0x1000, "sin": 0x2008}, _lib.ERR_UNSUPPORTED, "16-byte"),
+]
+
+
+def _calls(**kw):
+    c = {**OK_CALL, **kw}
+    lib, d, v = _lib.load(), _desc(**c["desc"]), _rows_view(**c["view"])
+    rows, lens = _ints(*c["rows"]), _ints(*c["lens"])
+    n = len(c["rows"])
+    append = lambda: lib.tsattn_pages4_append(d, c["dtype"], n, c["steps"], v, v, rows, lens, c["cos"], c["sin"], None)  # noqa: E731
+    attend = lambda: lib.tsattn_pages4_attend(d, c["dtype"], n, 4, c["steps"], 0.1, 1, v, v, rows, lens, c["cos"],  # noqa: E731
+                                              c["sin"], None, 0, None)
+    read = lambda: lib.tsattn_pages4_read(d, c["dtype"], n, c["steps"], v, v, rows, lens, _ints(*[0] * n), None)  # noqa: E731
+    return append, attend, read
+
+
+@pytest.mark.parametrize("change,status,what", BAD, ids=lambda x: str(x) if isinstance(x, dict) else None)
+def test_c_calls_refuse(change, status, what):
+    calls = _calls(**change)
+    for call in calls[:2] if "cos" in change else calls:
+        assert call() == status and what in _lib.last_error()
+
+
+def test_c_appends_attention_reads_copies_and_tables_refuse():
+    lib = _lib.load()
+    append, _, _ = _calls(rows=(1, 1))
+    assert append() == _lib.ERR_INVALID and "different" in _lib.last_error()
+    append, _, _ = _calls(lens=(5, 190), steps=3)
+    assert append() == _lib.ERR_INVALID and "exceed" in _lib.last_error()
+    d, v, rows, lens = _desc(), _rows_view(), _ints(0), _ints(150)
+    call = lambda heads=4, scale=0.1, steps=1: lib.tsattn_pages4_attend(  # noqa: E731
+        d, _lib.F16, 1, heads, steps, scale, 1, v, v, rows, lens, None, None, None, 0, None)
+    assert call(heads=3) == _lib.ERR_INVALID and "divisible" in _lib.last_error()
+    assert call(heads=0) == _lib.ERR_INVALID
+    assert call(scale=float("inf")) == _lib.ERR_INVALID and "finite" in _lib.last_error()
+    assert call(steps=1 << 20) == _lib.ERR_UNSUPPORTED
+    d.table_stride, lens = 300, _ints(19000)
+    need = lib.tsattn_pages4_attend_workspace(d, _lib.F16, 1, 4, 1, lens)
+    assert need > 0
+    assert lib.tsattn_pages4_attend(d, _lib.F16, 1, 4, 1, 0.1, 1, v, v, rows, lens, None, None, 0x1000, need - 1,
+                                    None) == _lib.ERR_INVALID and "too small" in _lib.last_error()
+    assert lib.tsattn_pages4_read(d, _lib.F16, 1, 1, v, v, rows, lens, _ints(-1), None) == _lib.ERR_INVALID
+    copy = lambda src, dst, to=0x10000, pages=8, size=1024: lib.tsattn_pages4_copy(  # noqa: E731
+        0x10000, 8, to, pages, size, len(src), _ints(*src), _ints(*dst), None)
+    for bad in (copy([0, 1], [2, 2]), copy([0, 1], [1, 2]), copy([8], [0]), copy([0], [8]), copy([-1], [0]),
+                copy([0], [3], to=0x50000, pages=3), copy([3], [3]), copy([], [])):
+        assert bad == _lib.ERR_INVALID
+    assert copy([0], [1], size=1000) == _lib.ERR_UNSUPPORTED
+    set_ = lambda at: lib.tsattn_pages4_set(0x1000, 4, len(at), _ints(*at), _ints(*at), None)  # noqa: E731
+    for bad in (set_([4]), set_([-1]), set_([1, 1]), set_([])):
+        assert bad == _lib.ERR_INVALID
+    assert lib.tsattn_pages4_page_bytes(8, 64, 128) == 8 * 2 * 36 * 128
+    assert [lib.tsattn_pages4_page_bytes(*s) for s in ((8, 64, 96), (8, 33, 64), (0, 64, 64), (8, 16, 64))] == [0] * 4
