@@ -644,6 +644,22 @@ size_t plan_attend4(const tsattn_pages4 *p, int32_t dtype, int32_t m, int32_t ro
                       : static_cast<size_t>(m) * p->heads * *splits * rows * (p->dim + 2) * sizeof(float);
 }
 
+// The host's side of a paged cache, and n different rows of it.
+int check_host4(const tsattn_pages4_host *h, int32_t n, const int32_t *rows) {
+  if (!h || !rows || !h->table || !h->lengths || !h->refs || !h->stack)
+    return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  if (n <= 0 || h->rows <= 0 || h->columns <= 0 || h->page_size <= 0 || h->pages <= 0 || h->free < 0 ||
+      h->free > h->pages || static_cast<int64_t>(h->rows) * h->columns > INT32_MAX)
+    return fail(TSATTN_ERR_INVALID, "page table: sizes must be positive");
+  for (int32_t i = 0; i < n; ++i)
+    if (rows[i] < 0 || rows[i] >= h->rows) return fail(TSATTN_ERR_INVALID, "page table: row %d out of range", rows[i]);
+  char *seen = static_cast<char *>(calloc(static_cast<size_t>(h->rows), 1));
+  if (!seen) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
+  const bool ok = distinct(n, rows, seen);
+  free(seen);
+  return ok ? TSATTN_OK : fail(TSATTN_ERR_INVALID, "page table: a row is named twice");
+}
+
 }  // namespace
 
 extern "C" {
@@ -1172,6 +1188,45 @@ int tsattn_pages4_set(int32_t *table, int64_t entries, int32_t n, const int32_t 
   if (!ok) return fail(TSATTN_ERR_INVALID, "page table: an entry is set twice");
   return hip_status(tsattn::launch_pages4_set(table, n, at, value, static_cast<hipStream_t>(stream)),
                     "page table launch");
+}
+
+int tsattn_pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
+                       int32_t *dst, int32_t *at, int32_t *value, int32_t *counts) {
+  int rc = check_host4(h, n, rows);
+  if (rc) return rc;
+  if (!src || !dst || !at || !value || !counts) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  for (int32_t i = 0; i < n; ++i)
+    if (steps <= 0 || static_cast<int64_t>(h->lengths[rows[i]]) + steps > static_cast<int64_t>(h->columns) * h->page_size)
+      return fail(TSATTN_ERR_INVALID, "page table: %d positions after %d of row %d exceed it", steps,
+                  h->lengths[rows[i]], rows[i]);
+  const int32_t need = tsattn::pages4_grow(h, n, rows, steps, src, dst, at, value, counts, counts + 1);
+  if (need) return fail(TSATTN_ERR_INVALID, "page pool exhausted: %d pages needed, %d free", need, h->free);
+  return TSATTN_OK;
+}
+
+int tsattn_pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *lengths) {
+  int rc = check_host4(h, n, rows);
+  if (rc) return rc;
+  if (!lengths) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  for (int32_t i = 0; i < n; ++i)
+    if (lengths[i] < 0 || lengths[i] > h->lengths[rows[i]])
+      return fail(TSATTN_ERR_INVALID, "truncate length must be between zero and the current length");
+  tsattn::pages4_cut(h, n, rows, lengths);
+  return TSATTN_OK;
+}
+
+int tsattn_pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *index, int32_t *at,
+                          int32_t *value, int32_t *count) {
+  int rc = check_host4(h, n, rows);
+  if (rc) return rc;
+  if (!index || !at || !value || !count) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  for (int32_t i = 0; i < n; ++i)
+    if (index[i] < 0 || index[i] >= n) return fail(TSATTN_ERR_INVALID, "beam index out of range");
+  int32_t *old = static_cast<int32_t *>(malloc(sizeof(int32_t) * n * (static_cast<size_t>(h->columns) + 1)));
+  if (!old) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
+  tsattn::pages4_reorder(h, n, rows, index, old, at, value, count);
+  free(old);
+  return TSATTN_OK;
 }
 
 }  // extern "C"

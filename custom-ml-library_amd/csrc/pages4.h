@@ -34,7 +34,7 @@ namespace tsattn {
 
 constexpr int kTile = 32;     // positions a tile
 constexpr int kSeqs = 256;    // sequences a launch: their numbers travel by value
-constexpr int kMoves = 256;   // pages, or table entries, a launch
+constexpr int kMoves = 480;   // pages, or table entries, a launch (under 4 KiB of arguments)
 
 // Sequences of a launch: row of the page table, cached positions (the kernels'
 // arguments hold them, so no copy to the device precedes a launch and a captured
@@ -98,6 +98,13 @@ hipError_t launch_pages4_read(const Pages4 &p, int dtype, int n, int len, View k
 hipError_t launch_pages4_copy(const char *from, char *to, int64_t page_bytes, int n, const int32_t *src,
                               const int32_t *dst, hipStream_t st);
 hipError_t launch_pages4_set(int32_t *table, int n, const int32_t *at, const int32_t *value, hipStream_t st);
+
+// pages4_table.hip
+int32_t pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
+                    int32_t *dst, int32_t *at, int32_t *value, int32_t *copies, int32_t *sets);
+void pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *lengths);
+void pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *index, int32_t *old,
+                    int32_t *at, int32_t *value, int32_t *sets);
 
 // Attention of len_q queries a sequence (q, out: [n, heads_q, len_q, dim]) over
 // the cached positions, the queries' own the last len_q of them.

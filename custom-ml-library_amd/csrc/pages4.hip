@@ -351,7 +351,7 @@ struct SetArgs {
   int32_t at[kMoves], value[kMoves];
 };
 
-__global__ __launch_bounds__(kMoves) void set_kernel(SetArgs a, int n) {
+__global__ __launch_bounds__(512) void set_kernel(SetArgs a, int n) {
   const int i = threadIdx.x;
   if (i < n) a.table[a.at[i]] = a.value[i];
 }
@@ -418,7 +418,8 @@ hipError_t launch_pages4_set(int32_t *table, int n, const int32_t *at, const int
     SetArgs a{table, {}, {}};
     const int m = n - i0 < kMoves ? n - i0 : kMoves;
     for (int i = 0; i < m; ++i) a.at[i] = at[i0 + i], a.value[i] = value[i0 + i];
-    set_kernel<<<dim3(1), dim3(kMoves), 0, st>>>(a, m);
+    static_assert(kMoves <= 512, "one lane an entry");
+    set_kernel<<<dim3(1), dim3((m + 63) / 64 * 64), 0, st>>>(a, m);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -126,7 +126,24 @@ class Pages4(ctypes.Structure):
     ]
 
 
+class Pages4Host(ctypes.Structure):
+    """``tsattn_pages4_host``: a paged cache's tables on the host."""
+
+    _fields_ = [
+        ("rows", c_int32),
+        ("columns", c_int32),
+        ("page_size", c_int32),
+        ("pages", c_int32),
+        ("table", c_void_p),
+        ("lengths", c_void_p),
+        ("refs", c_void_p),
+        ("stack", c_void_p),
+        ("free", c_int32),
+    ]
+
+
 _PV = POINTER(View)
+_PH = POINTER(Pages4Host)
 _P4 = POINTER(Pages4)
 _PP = POINTER(Problem)
 _PR = POINTER(RopeDesc)
@@ -243,6 +260,13 @@ SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_int64, c_size_t, c_int32, c_void_p, c_void_p, c_void_p],
     ),
     "tsattn_pages4_set": (c_int, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p]),
+    "tsattn_pages4_grow": (
+        c_int,
+        [_PH, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "tsattn_pages4_cut": (c_int, [_PH, c_int32, c_void_p, c_void_p]),
+    "tsattn_pages4_reorder": (
+        c_int, [_PH, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "tsattn_key_mask_lengths": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p],

@@ -18,7 +18,6 @@ Calls captured into a HIP graph replay the positions they were captured at.
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import numpy as np
@@ -40,10 +39,6 @@ def _ints(x):
     return np.ascontiguousarray(x, np.int32)
 
 
-def _ptr(x) -> ctypes.c_void_p:
-    return ctypes.c_void_p(x.ctypes.data)
-
-
 def _rows(t):
     """``t`` with rows that the kernels read as they are: 16-byte aligned, channels side by side."""
     import torch
@@ -52,7 +47,9 @@ def _rows(t):
 
 
 class _Pages:
-    """The pool, the page table (host and device) and the rows' lengths."""
+    """The pool, the page table (host and device) and the rows' lengths.  Pages are given out and
+    taken back by the library's host calls over these arrays (``tsattn_pages4_grow`` / ``_cut`` /
+    ``_reorder``)."""
 
     def __init__(self, rows: int, heads: int, dim: int, columns: int, page_size: int, num_pages: int, dev):
         import torch
@@ -62,109 +59,71 @@ class _Pages:
         if not self.page_bytes:
             raise NotImplementedError("paged caches take head dims 32, 64, 128 and 256, up to 4096 heads and "
                                       "pages of 32, 64, .. 4096 positions")
+        self.lengths = np.zeros(rows, np.int32)
+        self.lengths_at = self.lengths.ctypes.data
+        # what the host calls give back: page copies, table entries, how many of each
+        self.src, self.dst = np.empty(rows, np.int32), np.empty(rows, np.int32)
+        self.at, self.value = np.empty(rows * columns, np.int32), np.empty(rows * columns, np.int32)
+        self.counts = np.zeros(2, np.int32)
+        self.out = tuple(x.ctypes.data for x in (self.src, self.dst, self.at, self.value, self.counts))
         # (what no append has written weighs nothing: positions past a row's length are masked)
         self.pool = torch.empty((num_pages, self.page_bytes), dtype=torch.uint8, device=dev.torch)
         self.table = torch.zeros((rows, columns), dtype=torch.int32, device=dev.torch)
-        self.host = np.full((rows, columns), -1, np.int32)
-        self.lengths = np.zeros(rows, np.int32)
-        self.refs = np.zeros(num_pages, np.int32)
-        self.stack = np.arange(num_pages - 1, -1, -1, dtype=np.int32)  # free pages, the next one last
-        self.free = num_pages
-        self.quiet = 0  # positions that every row can take before any page changes
-        self.describe()
+        self.start(np.full((rows, columns), -1, np.int32), 0)
 
-    def describe(self) -> None:
-        d = _lib.Pages4()
-        d.pool, d.num_pages = self.pool.data_ptr(), self.pool.shape[0]
+    def start(self, host, used: int) -> None:
+        """Begin with the table ``host``, whose pages are the pool's first ``used``."""
+        pages = self.pool.shape[0]
+        self.host = host
+        self.refs = np.bincount(host[host >= 0], minlength=pages).astype(np.int32)
+        self.stack = np.arange(pages - 1, -1, -1, dtype=np.int32)  # free pages, the next one last
+        self.tables = t = _lib.Pages4Host()
+        t.rows, t.columns = host.shape
+        t.page_size, t.pages, t.free = self.page_size, pages, pages - used
+        t.table, t.lengths, t.refs = host.ctypes.data, self.lengths_at, self.refs.ctypes.data
+        t.stack = self.stack.ctypes.data
+        self.desc = d = _lib.Pages4()
+        d.pool, d.num_pages = self.pool.data_ptr(), pages
         d.heads, d.page_size, d.dim = self.heads, self.page_size, self.dim
-        d.table, d.table_rows, d.table_stride = self.table.data_ptr(), *self.host.shape
-        self.desc = d
+        d.table, d.table_rows, d.table_stride = self.table.data_ptr(), *host.shape
 
-    # -- pages ----------------------------------------------------------------
+    @property
+    def free(self) -> int:
+        return self.tables.free
 
-    def take(self, n: int):
-        self.free -= n
-        pages = self.stack[self.free:self.free + n][::-1].copy()
-        self.refs[pages] = 1
-        return pages
-
-    def drop(self, pages) -> None:
-        """One reference less for each of ``pages`` (a page may be named twice)."""
-        np.subtract.at(self.refs, pages, 1)
-        gone = np.unique(pages)
-        gone = gone[self.refs[gone] == 0][::-1]
-        self.stack[self.free:self.free + len(gone)] = gone
-        self.free += len(gone)
-
-    def upload(self, rows, columns) -> None:
-        """Entries of the host's table to the device's."""
-        if not len(rows):
-            return
-        if len(rows) > _MOST_SET:
+    def upload(self, n: int) -> None:
+        """The first ``n`` entries of ``at`` / ``value`` to the device's table."""
+        if n > _MOST_SET:
             import torch
 
             self.table.copy_(torch.from_numpy(np.maximum(self.host, 0)))
-            return
-        at, value = _ints(rows * self.host.shape[1] + columns), _ints(self.host[rows, columns])
-        _lib.check(launch(self.device, _lib.load().tsattn_pages4_set, self.table.data_ptr(), self.host.size,
-                          len(at), _ptr(at), _ptr(value)), "page table")
+        elif n:
+            _lib.check(launch(self.device, _lib.load().tsattn_pages4_set, self.desc.table, self.host.size, n,
+                              self.out[2], self.out[3]), "page table")
 
-    def move(self, source, target, src, dst) -> None:
-        src, dst = _ints(src), _ints(dst)
+    def move(self, source, target, n: int, src, dst) -> None:
         _lib.check(launch(self.device, _lib.load().tsattn_pages4_copy, source.data_ptr(), source.shape[0],
-                          target.data_ptr(), target.shape[0], self.page_bytes, len(src), _ptr(src), _ptr(dst)),
-                   "page copy")
+                          target.data_ptr(), target.shape[0], self.page_bytes, n, src, dst), "page copy")
 
-    def grow(self, rows, n: int) -> None:
-        """Pages of their own for the next ``n`` positions of ``rows``; nothing changes if there are too few."""
-        size, lens = self.page_size, self.lengths[rows]
-        first, stop = lens // size, -(-(lens + n) // size)
-        # a page that a row appends into and shares: all its rows but one get copies
-        into = np.flatnonzero(lens % size)
-        page = self.host[rows[into], first[into]]
-        shared = into[self.refs[page] > 1]
-        page = self.host[rows[shared], first[shared]]
-        order = np.argsort(page, kind="stable")
-        shared, page = shared[order], page[order]
-        nth = np.arange(len(page)) - np.searchsorted(page, page)  # of the appending rows of its page
-        copied = nth < self.refs[page] - 1
-        shared, page = shared[copied], page[copied]
-        span = int((stop - first).max())
-        columns = first[:, None] + np.arange(span)
-        wanted = columns < stop[:, None]
-        wanted &= self.host[rows[:, None], np.minimum(columns, self.host.shape[1] - 1)] < 0
-        at, j = np.nonzero(wanted)
-        if len(page) + len(at) > self.free:
-            raise ValueError(f"page pool exhausted: {len(page) + len(at)} pages needed, {self.free} free")
-        if len(page):
-            own = self.take(len(page))
-            self.move(self.pool, self.pool, page, own)
-            self.host[rows[shared], first[shared]] = own
-            self.drop(page)
-        if len(at):
-            self.host[rows[at], columns[at, j]] = self.take(len(at))
-        self.upload(np.concatenate((rows[shared], rows[at])), np.concatenate((first[shared], columns[at, j])))
-
-    def advance(self, rows, n: int, whole: bool) -> None:
-        self.lengths[rows] += n
-        self.quiet = max(self.quiet - n, 0)
-        if whole and not self.quiet:  # what is left in each row's last page, if the row has it alone
-            part = self.lengths % self.page_size
-            pages = self.host[np.arange(len(part)), self.lengths // self.page_size % self.host.shape[1]]
-            alone = (part > 0) & (self.refs[np.maximum(pages, 0)] == 1)
-            self.quiet = int(np.where(alone, self.page_size - part, 0).min())
+    def grow(self, n: int, rows: int, steps: int) -> None:
+        """Pages of their own for the next ``steps`` positions of the ``n`` rows (an address)."""
+        _lib.check(_lib.load().tsattn_pages4_grow(self.tables, n, rows, steps, *self.out), "page table")
+        copies, sets = self.counts.tolist()
+        if copies:
+            self.move(self.pool, self.pool, copies, *self.out[:2])
+        if sets:
+            self.upload(sets)
 
     def cut(self, rows, lengths) -> None:
         """``rows`` end at ``lengths``; pages wholly past them are given back."""
-        self.quiet = 0
-        self.lengths[rows] = lengths
-        past = np.arange(self.host.shape[1])[None, :] >= -(-self.lengths[rows] // self.page_size)[:, None]
-        past &= self.host[rows] >= 0
-        at, column = np.nonzero(past)
-        if len(at):
-            pages = self.host[rows[at], column]
-            self.host[rows[at], column] = -1
-            self.drop(pages)
+        rows, lengths = _ints(rows), _ints(lengths)
+        _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows.ctypes.data, lengths.ctypes.data),
+                   "page table")
+
+    def reorder(self, rows, index) -> None:
+        _lib.check(_lib.load().tsattn_pages4_reorder(self.tables, len(rows), rows.ctypes.data, index.ctypes.data,
+                                                     *self.out[2:]), "page table")
+        self.upload(int(self.counts[0]))
 
 
 class PagedKVCache:
@@ -196,7 +155,7 @@ class PagedKVCache:
         self._select(np.arange(batch_size, dtype=np.int32))
 
     def _select(self, rows) -> None:
-        self._rows = rows
+        self._rows, self._rows_at = rows, rows.ctypes.data
         self._whole = len(rows) == len(self._core.lengths) and bool((rows == np.arange(len(rows))).all())
 
     # -- what it is -----------------------------------------------------------
@@ -246,7 +205,7 @@ class PagedKVCache:
         """
         self._check(key, value)
         core, steps = self._core, key.shape[2]
-        lens = core.lengths if self._whole else core.lengths[self._rows]
+        lens, lens_at = self._lens()
         most = int(lens.max()) + steps
         if steps == 0 or most > self.max_seq_len:
             raise ValueError(f"cache capacity {self.max_seq_len} exceeded or empty append")
@@ -256,11 +215,29 @@ class PagedKVCache:
                 raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
             cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
         k, v = (_rows(t._data.to(self.dtype)) for t in (key, value))
-        if not (self._whole and steps <= core.quiet):
-            core.grow(self._rows, steps)
-        _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, _dtype_code(self.dtype), len(lens),
-                          steps, _view(k), _view(v), _ptr(self._rows), _ptr(lens), cos, sin), "paged append")
-        core.advance(self._rows, steps, self._whole)
+        core.grow(len(lens), self._rows_at, steps)
+        try:
+            _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
+                              _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
+        except BaseException:
+            core.lengths[self._rows] += steps  # (the new pages go back)
+            core.cut(self._rows, lens - steps if self._whole else lens)
+            raise
+        if self._whole:
+            core.lengths += steps
+        else:
+            core.lengths[self._rows] += steps
+
+    def _lens(self):
+        """The rows' lengths and their address."""
+        if self._whole:
+            return self._core.lengths, self._core.lengths_at
+        lens = self._core.lengths[self._rows]
+        return lens, lens.ctypes.data
+
+    @property
+    def _code(self) -> int:
+        return _dtype_code(self.dtype)
 
     def _check(self, key: Tensor, value: Tensor) -> None:
         """``KVCache``'s refusals, in its order."""
@@ -279,17 +256,16 @@ class PagedKVCache:
         import torch
 
         core = self._core
-        lens = core.lengths[self._rows]
+        lens, lens_at = self._lens()
         if last is not None and not 0 < last <= lens.min():
             raise ValueError("the last positions read must be between one and the shortest row's length")
         steps = int(lens.max()) if last is None else last
         first = np.zeros_like(lens) if last is None else lens - np.int32(last)
-        out = [torch.empty((len(lens), core.heads, steps, core.dim), dtype=self.dtype, device=core.pool.device)
-               for _ in range(2)]
+        shape, dev = (len(lens), core.heads, steps, core.dim), core.pool.device
+        out = [torch.empty(shape, dtype=self.dtype, device=dev) for _ in range(2)]
         if steps:
-            _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, _dtype_code(self.dtype),
-                              len(lens), steps, _view(out[0]), _view(out[1]), _ptr(self._rows), _ptr(lens),
-                              _ptr(first)), "paged read")
+            _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
+                              _view(out[0]), _view(out[1]), self._rows_at, lens_at, first.ctypes.data), "paged read")
         return tuple(Tensor(x, device=core.device) for x in out)
 
     # -- rows and pages -------------------------------------------------------
@@ -316,13 +292,13 @@ class PagedKVCache:
 
     def reset(self) -> None:
         """Every row empty, its pages given back."""
-        self._core.cut(self._rows, 0)
+        self._core.cut(self._rows, np.zeros_like(self._rows))
 
     def free(self, indices) -> None:
         """These rows empty, their pages given back."""
-        index = self._indices(indices, None)
+        index = np.unique(self._indices(indices, None))
         if len(index):
-            self._core.cut(self._rows[np.unique(index)], 0)
+            self._core.cut(self._rows[index], np.zeros_like(index))
 
     def truncate(self, length) -> None:
         """Cut every row to ``length`` positions, or to a length of its own (a sequence of them);
@@ -330,31 +306,22 @@ class PagedKVCache:
         want = np.asarray(length)
         if want.dtype.kind not in "iu" or want.shape not in ((), (self.batch_size,)):
             raise ValueError("truncate takes one integer length, or one per row")
-        lens = self._core.lengths[self._rows]
+        lens, _ = self._lens()
         if (want < 0).any() or (want > lens).any():
             raise ValueError("truncate length must be between zero and the current length")
-        if (want != lens).any():
-            self._core.cut(self._rows, want)
+        self._core.cut(self._rows, want if want.shape else np.full_like(self._rows, want))
 
     def reorder(self, indices) -> None:
         """Row i becomes row ``indices[i]``, sharing its pages: no keys or values move.  Rows that
         take over the same row share until one appends (``append`` copies the page)."""
-        core, index = self._core, self._indices(indices, (self.batch_size,))
-        old, new = core.host[self._rows], core.host[self._rows[index]]
-        core.quiet = 0
-        core.lengths[self._rows] = core.lengths[self._rows[index]]
-        core.host[self._rows] = new
-        np.add.at(core.refs, new[new >= 0], 1)
-        core.drop(old[old >= 0])
-        at, column = np.nonzero((new != old) & (new >= 0))
-        core.upload(self._rows[at], column)
+        self._core.reorder(self._rows, self._indices(indices, (self.batch_size,)))
 
     def copy(self, num_pages: int | None = None) -> "PagedKVCache":
         """A cache of these rows with a pool of its own (``num_pages``, by default as many as this
         one has), its pages in use side by side; rows that share pages share them there."""
         core = self._core
-        host = core.host[self._rows]
-        live = np.unique(host[host >= 0])
+        host = core.host if self._whole else core.host[self._rows]
+        live, new = self._renumber(host, self.num_pages)
         num_pages = self.num_pages if num_pages is None else num_pages
         if num_pages < max(len(live), 1):
             raise ValueError(f"{len(live)} pages are in use")
@@ -364,55 +331,57 @@ class PagedKVCache:
                                      core.device)
         other._select(np.arange(len(host), dtype=np.int32))
         there.lengths[:] = core.lengths[self._rows]
+        there.start(new, len(live))
         if len(live):
-            there.take(len(live))
-            core.move(core.pool, there.pool, live, np.arange(len(live)))
-            self._renumber(there, host, live)
+            to = np.arange(len(live), dtype=np.int32)
+            core.move(core.pool, there.pool, len(live), live.ctypes.data, to.ctypes.data)
+            self._tell(there)
         return other
 
     def compact(self, num_pages: int | None = None) -> int:
         """Move the pages in use to the front of the pool, and with ``num_pages`` into a pool of that
         size (smaller or larger); returns how many are in use."""
         core = self._core
-        live = np.unique(core.host[core.host >= 0])
-        n = len(live)
-        if num_pages is not None and num_pages < max(n, 1):
-            raise ValueError(f"{n} pages are in use")
         if num_pages is None:
-            moved, holes = live[live >= n], np.setdiff1d(np.arange(n, dtype=np.int32), live)
-            to = live.copy()
-            to[live >= n] = holes
+            # the pages past the front move into its holes: none is both read and written
+            live = np.flatnonzero(core.refs).astype(np.int32)
+            n = len(live)
+            moved, holes = live[live >= n], np.flatnonzero(core.refs[:n] == 0).astype(np.int32)
             if len(moved):
-                core.move(core.pool, core.pool, moved, holes)
-            num_pages = self.num_pages
+                core.move(core.pool, core.pool, len(moved), moved.ctypes.data, holes.ctypes.data)
+            to = np.arange(self.num_pages, dtype=np.int32)
+            to[moved] = holes
+            new = np.where(core.host >= 0, to[core.host], np.int32(-1))
         else:
             import torch
 
-            to = np.arange(n, dtype=np.int32)
+            live, new = self._renumber(core.host, self.num_pages)
+            n = len(live)
+            if num_pages < max(n, 1):
+                raise ValueError(f"{n} pages are in use")
             pool = torch.empty((num_pages, core.page_bytes), dtype=torch.uint8, device=core.pool.device)
             if n:
-                core.move(core.pool, pool, live, to)
+                to = np.arange(n, dtype=np.int32)
+                core.move(core.pool, pool, n, live.ctypes.data, to.ctypes.data)
             core.pool = pool
-        core.refs = np.zeros(num_pages, np.int32)
-        core.stack = np.arange(num_pages - 1, -1, -1, dtype=np.int32)
-        core.free = num_pages - n
-        core.quiet = 0
-        if n:
-            self._renumber(core, core.host, live, to)
-        core.describe()
+        core.start(np.ascontiguousarray(new, np.int32), n)
+        self._tell(core)
         return n
 
     @staticmethod
-    def _renumber(core, host, live, to=None) -> None:
-        """``core``'s table: ``host`` with the pages ``live`` numbered ``to`` (0, 1, ..)."""
-        to = np.arange(len(live), dtype=np.int32) if to is None else to
-        held = host >= 0
-        new = np.full_like(host, -1)
-        new[held] = to[np.searchsorted(live, host[held])]
-        at, column = np.nonzero(held & (new != core.host))
-        core.host = new
-        core.refs[:] = np.bincount(new[held], minlength=len(core.refs))
-        core.upload(at, column)
+    def _renumber(host, pages: int):
+        """The pages of a table, ascending, and the table with them numbered 0, 1, .."""
+        used = np.zeros(pages, bool)
+        used[host[host >= 0]] = True
+        number = np.cumsum(used, dtype=np.int32) - 1
+        return np.flatnonzero(used).astype(np.int32), np.where(host >= 0, number[host], np.int32(-1))
+
+    @staticmethod
+    def _tell(core) -> None:
+        """The whole of the host's table to the device's."""
+        at = np.flatnonzero(core.host >= 0)
+        core.at[:len(at)], core.value[:len(at)] = at, core.host.reshape(-1)[at]
+        core.upload(len(at))
 
 
 def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = True, scale: float | None = None,
@@ -445,7 +414,7 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
     import torch
 
     core = cache._core
-    lens = core.lengths if cache._whole else core.lengths[cache._rows]
+    lens, lens_at = cache._lens()
     if heads // cache.num_heads * steps >= PROMPT_ROWS and dim <= 128 and lens.min() >= steps:
         return _prompt(query, cache, lens, is_causal, multiplier, rotary_base)
     q = _rows(query._data)
@@ -454,11 +423,11 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
         cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, dim, q.dtype, q.device,
                                                       max(int(lens.max()), steps)))
     out = torch.empty((b, heads, steps, dim), dtype=q.dtype, device=q.device)
-    lib, code = _lib.load(), _dtype_code(q.dtype)
-    nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, _ptr(lens))
+    lib, code = _lib.load(), cache._code
+    nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, lens_at)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _lib.check(launch(core.device, lib.tsattn_pages4_attend, core.desc, code, b, heads, steps, multiplier,
-                      int(is_causal), _view(q), _view(out), _ptr(cache._rows), _ptr(lens), cos, sin,
+                      int(is_causal), _view(q), _view(out), cache._rows_at, lens_at, cos, sin,
                       None if ws is None else ws.data_ptr(), nbytes), "paged attention")
     return Tensor._from_op(out, (query,), None, "paged_attention")
 

@@ -600,6 +600,41 @@ int tsattn_pages4_copy(const void *from, int64_t from_pages, void *to, int64_t t
 int tsattn_pages4_set(int32_t *table, int64_t entries, int32_t n, const int32_t *at, const int32_t *value,
                       void *stream);
 
+/*
+ * The host's side of a paged cache, in the caller's arrays: the next three calls change
+ * them and launch nothing.  They give the page copies and the table entries that the
+ * device needs (for tsattn_pages4_copy and tsattn_pages4_set, in this order, before
+ * the next append) in arrays of the caller's.
+ */
+typedef struct tsattn_pages4_host {
+  int32_t rows, columns, page_size, pages;
+  int32_t *table;   /* [rows, columns] page numbers, -1: none (as many held as the length needs) */
+  int32_t *lengths; /* [rows] cached positions */
+  int32_t *refs;    /* [pages] rows that hold the page */
+  int32_t *stack;   /* [pages] the free pages; the next one is stack[free - 1] */
+  int32_t free;
+} tsattn_pages4_host;
+
+/*
+ * Pages for `steps` more positions of the n different rows.  A row that would append
+ * into a page that others hold gets a copy: src[i] -> dst[i], counts[0] of them (room
+ * for n).  at, value: counts[1] table entries (room for rows * columns).  Too few free
+ * pages: TSATTN_ERR_INVALID, nothing changed.  The lengths stay: the caller adds
+ * `steps` once the rows are there.
+ */
+int tsattn_pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
+                       int32_t *dst, int32_t *at, int32_t *value, int32_t *counts);
+
+/* The n different rows end at lengths[i] <= their own; pages wholly past them are free. */
+int tsattn_pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *lengths);
+
+/*
+ * Row rows[i] takes over pages and length of rows[index[i]], for all i at once, and
+ * shares the pages with it.  at, value: *count table entries (room for n * columns).
+ */
+int tsattn_pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *index, int32_t *at,
+                          int32_t *value, int32_t *count);
+
 #ifdef __cplusplus
 }
 #endif

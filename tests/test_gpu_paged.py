@@ -287,7 +287,7 @@ def test_many_sequences_and_far_pages():
     cache = nn.PagedKVCache(b, h, d, 64, device="hip", dtype=BF16, num_pages=65000)
     assert cache._core.pool.numel() > 2**32
     core = cache._core
-    core.stack = core.stack[::-1].copy()  # the last pages are given out first
+    core.stack[:] = core.stack[::-1].copy()  # the last pages are given out first
     k, v = (draw(gen, b, h, 40, d, dtype=BF16) for _ in range(2))
     cache.append(wrap(k), wrap(v))
     assert int(core.host[core.host >= 0].min()) * core.page_bytes > 2**32
