@@ -629,19 +629,12 @@ tsattn::View seq_view(const tsattn_view *v, int32_t i0, int32_t dtype) {
   return x;
 }
 
-// The splits of sequences i0 .. i0 + m - 1, and the scratch that they take.
-size_t plan_attend4(const tsattn_pages4 *p, int32_t dtype, int32_t m, int32_t rows, const int32_t *lens,
-                    int *split, int *splits) {
-  int64_t total = 0;
-  int longest = 0;
-  for (int i = 0; i < m; ++i) {
-    total += lens[i];
-    longest = lens[i] > longest ? lens[i] : longest;
-  }
-  *split = tsattn::attend4_split(dtype, p->dim, p->heads, rows, total, longest);
-  *splits = longest ? (longest + *split - 1) / *split : 1;
-  return *splits == 1 ? 0
-                      : static_cast<size_t>(m) * p->heads * *splits * rows * (p->dim + 2) * sizeof(float);
+// The plan of sequences i0 .. of a call (m of them), and the scratch that they take.
+size_t plan4(tsattn::Attend4 *a, int32_t dtype, int32_t n, int32_t i0, const int32_t *lens) {
+  a->n = n - i0 < tsattn::kSeqs ? n - i0 : tsattn::kSeqs;
+  tsattn::plan_attend4(a, dtype, lens + i0);
+  return a->splits == 1 ? 0
+                        : static_cast<size_t>(a->n) * a->p.heads * a->splits * a->rows * (a->p.dim + 2) * sizeof(float);
 }
 
 // The host's side of a paged cache, and n different rows of it.
@@ -1105,11 +1098,12 @@ size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int
   if (!p || !lens || n <= 0 || heads_q <= 0 || len_q <= 0 || !pages4_sizes_ok(p->heads, p->page_size, p->dim) ||
       heads_q % p->heads || static_cast<int64_t>(heads_q / p->heads) * len_q > (1 << 18))
     return 0;
+  tsattn::Attend4 a{};
+  a.p.heads = p->heads, a.p.dim = p->dim;
+  a.rows = heads_q / p->heads * len_q;
   size_t most = 0;
   for (int32_t i0 = 0; i0 < n; i0 += tsattn::kSeqs) {  // (groups of sequences follow each other in it)
-    int split, splits;
-    const size_t need = plan_attend4(p, dtype, n - i0 < tsattn::kSeqs ? n - i0 : tsattn::kSeqs,
-                                     heads_q / p->heads * len_q, lens + i0, &split, &splits);
+    const size_t need = plan4(&a, dtype, n, i0, lens);
     most = need > most ? need : most;
   }
   return most;
@@ -1137,13 +1131,17 @@ int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
     return fail(TSATTN_ERR_INVALID, "paged attention workspace too small: %zu < %zu bytes", workspace_bytes, need);
   a.ws = static_cast<float *>(workspace);
   a.cos = cos, a.sin = sin;
-  a.heads_q = heads_q, a.rep = heads_q / p->heads, a.len_q = len_q, a.rows = static_cast<int>(r);
+  a.rep = heads_q / p->heads, a.len_q = len_q, a.rows = static_cast<int>(r);
+  a.by_len_q = tsattn::make_fastdiv(len_q);
   a.causal = is_causal ? 1 : 0;
-  a.sl = static_cast<float>(scale) * tsattn::kLog2e;
+  const float sl = static_cast<float>(scale) * tsattn::kLog2e;
+  a.sign = sl > 0.f ? 1.f : sl < 0.f ? -1.f : 0.f;
+  a.sl = sl == 0.f ? 1.f : fabsf(sl);
+  if (!isfinite(a.sl)) return fail(TSATTN_ERR_INVALID, "attention scale must be finite");
   g_last_path = 3;
   for (int32_t i0 = 0; i0 < n && !rc; i0 += tsattn::kSeqs) {
-    a.n = take_seqs(&a.s, n, i0, rows, lens);
-    plan_attend4(p, dtype, a.n, a.rows, lens + i0, &a.split, &a.splits);
+    plan4(&a, dtype, n, i0, lens);
+    take_seqs(&a.s, n, i0, rows, lens);
     a.q = seq_view(q, i0, dtype), a.o = seq_view(out, i0, dtype);
     rc = hip_status(tsattn::launch_attend4(a, dtype, static_cast<hipStream_t>(stream)), "paged attention launch");
   }

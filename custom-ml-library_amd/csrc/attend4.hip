@@ -16,7 +16,7 @@
 // Precision.  q enters exactly: bf16 in one part, f16 in two, fp32 in three. P sv
 // enters as two bf16 parts (2^-17 of each), for fp32 as three (2^-25).
 //
-// A wave works alone on the tiles w, w + 4, ... of its split, two tiles ahead in
+// A wave works alone on every fourth or eighth tile of its split, two tiles ahead in
 // registers, straight from memory in operand order (pages4.h); waves merge in LDS,
 // splits in a second kernel where there is more than one.
 #include "pages4.h"
@@ -25,7 +25,8 @@
 namespace tsattn {
 namespace {
 
-constexpr int NWV = 4;
+// Tiles a wave at most (of four waves; its lanes hold their page numbers).
+constexpr int kSplitTiles = 32;
 
 template <typename T>
 constexpr int q_parts() { return std::is_same_v<T, bf16> ? 1 : std::is_same_v<T, f16> ? 2 : 3; }
@@ -49,7 +50,7 @@ __device__ __forceinline__ void split_bf16(float a, float b, uint32_t (&out)[N])
 template <int G>
 __device__ __forceinline__ float group_sum4(float x) {
   auto dpp = [](float v, auto ctrl) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF, 0xF, false));
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF, 0xF, true));
   };
   if constexpr (G >= 2) x += dpp(x, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
   if constexpr (G >= 4) x += dpp(x, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
@@ -68,70 +69,100 @@ struct Held {
   __device__ __forceinline__ uint32_t vw(int w) const { return G == 1 ? v[0][w] : v[w >> 2][w & 3]; }
 };
 
-template <typename T, int G, int NB>
+template <typename T, int G, int NB, int NWV>
 __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 : 2)) void attend4_kernel(Attend4 a) {
   constexpr int D = 32 * G, W = 2 * G, NQ = q_parts<T>(), NP = p_parts<T>();
   constexpr int RB = 16 / G, ROWS = RB * NB;  // rows a column block, a workgroup
-  __shared__ float part[NWV][ROWS][D + 2];
+  constexpr int LD = D + 4;                   // (rows of the merge start in different banks)
+  __shared__ __attribute__((aligned(16))) float part[NWV][ROWS][LD];
+  __shared__ float state[NWV][ROWS][2];  // their maximum and sum
 
   const int b = blockIdx.z, split = blockIdx.y;
-  const int blocks = (a.rows + ROWS - 1) / ROWS;
-  const int hk = blockIdx.x / blocks, row0 = (blockIdx.x - hk * blocks) * ROWS;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rl = c / G, grp = c % G;  // the lane's row in its column block, its group
-  const int len = a.s.len[b];
+  const int len = a.s.len[b], trow = a.s.row[b];
+  const int hk = a.blocks == 1 ? blockIdx.x : blockIdx.x / a.blocks;
+  const int row0 = (blockIdx.x - hk * a.blocks) * ROWS;
   const int begin = split * a.split;
   const int live_rows = min(ROWS, a.rows - row0);
+  auto out_row = [&](int r) __attribute__((always_inline)) {
+    const int rr = fdiv(row0 + r, a.by_len_q), qi = row0 + r - rr * a.len_q;
+    return static_cast<T *>(const_cast<void *>(a.o.data)) + b * a.o.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.o.s1 +
+           qi * a.o.s2;
+  };
   if (begin >= len) {  // no positions here: an empty sequence's rows are zero
     if (a.splits == 1)
-      for (int i = tid; i < live_rows * D; i += 64 * NWV) {
-        const int r = row0 + i / D, d = i % D, rr = r / a.len_q, qi = r - rr * a.len_q;
-        static_cast<T *>(const_cast<void *>(a.o.data))[b * a.o.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.o.s1 +
-                                                       qi * a.o.s2 + d] = static_cast<T>(0.f);
-      }
+      for (int r = w; r < live_rows; r += NWV)
+        for (int d = lane; d < D; d += 64) out_row(r)[d] = static_cast<T>(0.f);
     return;
   }
   const int keys = min(a.split, len - begin);
   const int n_tiles = (keys + kTile - 1) / kTile;
   const int mine = n_tiles > w ? (n_tiles - 1 - w) / NWV + 1 : 0;
   const int tile0 = begin / kTile + w;
-  const int32_t *ids = a.p.table + a.s.row[b] * a.p.stride;
 
-  // queries: row r of the block, channels 32 grp + 8 g .. + 7, in k-step grp
+  // the queries' rows, on their way first: row r of the block, channels 32 grp + 8 g .. + 7
+  constexpr int QW = sizeof(T) / 2;  // 16-byte loads a row piece
+  u32x4 raw[NB][QW];
+  int qpos[NB];  // the row's query's number
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int r = nb * RB + rl < live_rows ? row0 + nb * RB + rl : row0;
+    const int rr = fdiv(r, a.by_len_q);
+    qpos[nb] = r - rr * a.len_q;
+    const T *qp = static_cast<const T *>(a.q.data) + b * a.q.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.q.s1 +
+                  qpos[nb] * a.q.s2 + 32 * grp + 8 * g;
+#pragma unroll
+    for (int i = 0; i < QW; ++i) raw[nb][i] = reinterpret_cast<const u32x4 *>(qp)[i];
+  }
+  // the wave's page numbers, lane t's for its tile t: one load, and none in the loop
+  // (kSplitTiles of a wave at most)
+  const int ids = a.p.table[trow * a.p.stride + ((tile0 + NWV * min(lane, max(mine, 1) - 1)) >> a.p.per_page)];
+  auto load = [&](Held<G> &x, int t) __attribute__((always_inline)) {
+    using C = typename Held<G>::Chunk;
+    const char *base = tile4_at(a.p, static_cast<uint32_t>(__builtin_amdgcn_readlane(ids, t)), tile0 + NWV * t, hk);
+#pragma unroll
+    for (int q = 0; q < Held<G>::N; ++q) {
+      x.k[q] = __builtin_nontemporal_load(reinterpret_cast<const C *>(base) + 64 * q + lane);
+      x.v[q] = __builtin_nontemporal_load(reinterpret_cast<const C *>(base + 16 * D) + 64 * q + lane);
+    }
+    x.ks = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(base + 32 * D) + g * G + grp);
+    x.vs = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(base + 34 * D) + g * G + grp);
+  };
+  Held<G> x0, x1;
+  if (mine > 0) load(x0, 0);
+  if (mine > 1) load(x1, 1);
+
+  // the B operand: the row's piece in k-step grp, zero in the others
   u32x4 qf[NB][NQ][G];
   int klim[NB];  // positions of the split that the row sees: [0, klim)
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const int r = row0 + nb * RB + rl;
     const bool live = nb * RB + rl < live_rows;
-    const int rr = live ? r / a.len_q : 0, qi = live ? r - rr * a.len_q : 0;
-    const T *qp = static_cast<const T *>(a.q.data) + b * a.q.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.q.s1 +
-                  qi * a.q.s2 + 32 * grp + 8 * g;
     T x[8];
-    if constexpr (sizeof(T) == 2) {
-      const u32x4 raw = ld16(qp);
-      const T *e = reinterpret_cast<const T *>(&raw);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = e[i];
-    } else {
+    for (int i = 0; i < QW; ++i) {
+      const T *e = reinterpret_cast<const T *>(&raw[nb][i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = qp[i];
+      for (int j = 0; j < 8 / QW; ++j) x[i * (8 / QW) + j] = e[j];
     }
-    const int at = max(len - a.len_q + qi, 0);  // the query's position
+    const int at = len - a.len_q + qpos[nb];  // the query's position
     if (a.cos) {
-      const int64_t e = static_cast<int64_t>(at) * (D / 2) + 16 * grp + 4 * g;
+      const int64_t e = static_cast<int64_t>(max(at, 0)) * (D / 2) + 16 * grp + 4 * g;
+      T cw[4], sw[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        rotate_pair(x[2 * i], x[2 * i + 1], static_cast<const T *>(a.cos)[e + i], static_cast<const T *>(a.sin)[e + i],
-                    false);
+      for (int i = 0; i < 4; ++i) cw[i] = static_cast<const T *>(a.cos)[e + i], sw[i] = static_cast<const T *>(a.sin)[e + i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rotate_pair(x[2 * i], x[2 * i + 1], cw[i], sw[i], false);
     }
-    klim[nb] = a.causal ? min(keys, len - a.len_q + qi + 1 - begin) : keys;
+    klim[nb] = a.causal ? min(keys, at + 1 - begin) : keys;
     uint32_t pt[NQ][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t two[NQ];
-      split_bf16<NQ>(live ? static_cast<float>(x[2 * i]) : 0.f, live ? static_cast<float>(x[2 * i + 1]) : 0.f, two);
+      split_bf16<NQ>(live ? static_cast<float>(x[2 * i]) * a.sign : 0.f,
+                     live ? static_cast<float>(x[2 * i + 1]) * a.sign : 0.f, two);
 #pragma unroll
       for (int n = 0; n < NQ; ++n) pt[n][i] = two[n];
     }
@@ -153,52 +184,47 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
     for (int i = 0; i < W; ++i) oacc[nb][i] = f32x4{};
   }
 
-  auto id_of = [&](int t) __attribute__((always_inline)) {
-    return static_cast<uint32_t>(ids[(tile0 + NWV * min(t, mine - 1)) >> a.p.per_page]);
-  };
-  auto load = [&](Held<G> &x, int t, uint32_t id) __attribute__((always_inline)) {
-    using C = typename Held<G>::Chunk;
-    const char *base = tile4_at(a.p, id, tile0 + NWV * t, hk);
-#pragma unroll
-    for (int q = 0; q < Held<G>::N; ++q) {
-      x.k[q] = __builtin_nontemporal_load(reinterpret_cast<const C *>(base) + 64 * q + lane);
-      x.v[q] = __builtin_nontemporal_load(reinterpret_cast<const C *>(base + 16 * D) + 64 * q + lane);
-    }
-    x.ks = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(base + 32 * D) + g * G + grp);
-    x.vs = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(base + 34 * D) + g * G + grp);
-  };
+  // Chains of dependent MFMAs alternate: the two halves of the scores, pairs of
+  // value blocks.
   auto compute = [&](const Held<G> &t4, int t) __attribute__((always_inline)) {
     const int tile = w + NWV * t;  // of the split
     f32x4 s[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = f32x4{};
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int ks = 0; ks < G; ++ks) {
+      u32x4 kf[2];
 #pragma unroll
-      for (int ks = 0; ks < G; ++ks) {
-        const u32x4 kf = levels_bf16(t4.kw(kb * G + ks));
+      for (int kb = 0; kb < 2; ++kb) kf[kb] = levels_bf16(t4.kw(kb * G + ks));
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) s[nb][kb] = mfma16<bf16>(kf, qf[nb][n][ks], s[nb][kb]);
-      }
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) s[nb][kb] = mfma16<bf16>(kf[kb], qf[nb][n][ks], s[nb][kb]);
+    }
     u32x4 pb[NB][NP];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      float x[8];
+      float x[8], vs[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = group_sum4<G>(s[nb][i >> 2][i & 3] * from_bf16((t4.ks[i >> 1] >> (16 * (i & 1))) & 0xFFFFu)) * a.sl;
-      if (tile >= edge) {
+      for (int i = 0; i < 8; i += 2) {
+        const uint32_t k2 = t4.ks[i >> 1], v2 = t4.vs[i >> 1];
+        x[i] = group_sum4<G>(s[nb][i >> 2][i & 3] * __builtin_bit_cast(float, k2 << 16));
+        x[i + 1] = group_sum4<G>(s[nb][i >> 2][(i & 3) + 1] * __builtin_bit_cast(float, k2 & 0xFFFF0000u));
+        vs[i] = __builtin_bit_cast(float, v2 << 16);
+        vs[i + 1] = __builtin_bit_cast(float, v2 & 0xFFFF0000u);
+      }
+      if (tile >= edge) {  // what a row does not see weighs nothing, whatever its scales are
         const int lim = klim[nb] - tile * kTile - 4 * g;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (16 * (i >> 2) + (i & 3) >= lim) x[i] = -INFINITY;
+          if (16 * (i >> 2) + (i & 3) >= lim) x[i] = -INFINITY, vs[i] = 0.f;
       }
       float mx = x[0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
-      mx = quad_row_max(mx);
+      mx = quad_row_max(mx) * a.sl;  // (sl > 0)
       if (__ballot(mx > m[nb]) != 0ull) {
         const float mn = fmaxf(m[nb], mx);
         const float corr = mn == -INFINITY ? 1.f : fast_exp2(m[nb] - mn);
@@ -207,50 +233,40 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
 #pragma unroll
         for (int i = 0; i < W; ++i) oacc[nb][i] *= corr;
       }
-      const float base = m[nb] == -INFINITY ? 0.f : m[nb];
+      const float base = m[nb] == -INFINITY ? 0.f : -m[nb];
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const float p0 = fast_exp2(x[i] - base), p1 = fast_exp2(x[i + 1] - base);
+        const float p0 = fast_exp2(fmaf(x[i], a.sl, base)), p1 = fast_exp2(fmaf(x[i + 1], a.sl, base));
         l[nb] += p0 + p1;
-        const uint32_t sc = t4.vs[i >> 1];
-        // a position that the row does not see weighs nothing, whatever its scale is
-        const float v0 = p0 == 0.f ? 0.f : p0 * from_bf16(sc & 0xFFFFu);
-        const float v1 = p1 == 0.f ? 0.f : p1 * __builtin_bit_cast(float, sc & 0xFFFF0000u);
         uint32_t two[NP];
-        split_bf16<NP>(v0, v1, two);
+        split_bf16<NP>(p0 * vs[i], p1 * vs[i + 1], two);
 #pragma unroll
         for (int n = 0; n < NP; ++n) pb[nb][n][i >> 1] = two[n];
       }
     }
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const u32x4 vf = levels_bf16(t4.vw(i));
+    for (int i = 0; i < W; i += 2) {
+      const u32x4 vf[2] = {levels_bf16(t4.vw(i)), levels_bf16(t4.vw(i + 1))};
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int n = 0; n < NP; ++n) oacc[nb][i] = mfma16<bf16>(vf, pb[nb][n], oacc[nb][i]);
+        for (int n = 0; n < NP; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) oacc[nb][i + e] = mfma16<bf16>(vf[e], pb[nb][n], oacc[nb][i + e]);
     }
   };
 
-  if (mine > 0) {
-    Held<G> x0, x1;
-    load(x0, 0, id_of(0));
-    if (mine > 1) load(x1, 1, id_of(1));
-    uint32_t n0 = id_of(2), n1 = id_of(3);
-    for (int t = 0; t < mine; t += 2) {
-      compute(x0, t);
-      if (t + 2 < mine) load(x0, t + 2, n0);
-      n0 = id_of(t + 4);
-      if (t + 1 < mine) {
-        compute(x1, t + 1);
-        if (t + 3 < mine) load(x1, t + 3, n1);
-        n1 = id_of(t + 5);
-      }
+  for (int t = 0; t < mine; t += 2) {
+    compute(x0, t);
+    if (t + 2 < mine) load(x0, t + 2);
+    if (t + 1 < mine) {
+      compute(x1, t + 1);
+      if (t + 3 < mine) load(x1, t + 3);
     }
   }
 
   // Merge the waves.  Lane (c, g) has row rl's channels 16 i + 4 g .. + 3 for the
-  // blocks i of its group.
+  // blocks i of its group; then a wave sums a row over the waves, PER channels a lane.
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     float lt = l[nb] + __shfl_xor(l[nb], 16, 64);
@@ -258,76 +274,84 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
     float *to = part[w][nb * RB + rl];
 #pragma unroll
     for (int i = 0; i < W; ++i)
-      if (i / 2 == grp) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) to[16 * i + 4 * g + e] = oacc[nb][i][e];
-      }
+      if (i / 2 == grp) *reinterpret_cast<f32x4 *>(to + 16 * i + 4 * g) = oacc[nb][i];
     if (g == 0 && grp == 0) {
-      to[D] = m[nb];
-      to[D + 1] = lt;
+      state[w][nb * RB + rl][0] = m[nb];
+      state[w][nb * RB + rl][1] = lt;
     }
   }
   __syncthreads();
-  for (int i = tid; i < live_rows * (D + 2); i += 64 * NWV) {
-    const int r = i / (D + 2), d = i - r * (D + 2);
-    float M = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < NWV; ++v) M = fmaxf(M, part[v][r][D]);
-    const float base = M == -INFINITY ? 0.f : M;
-    float sum = 0.f, total = 0.f;
+  constexpr int PER = D < 64 ? 1 : D / 64;
+  using Piece = std::conditional_t<PER == 1, float, std::conditional_t<PER == 2, f32x2, f32x4>>;
+  for (int r = w; r < live_rows; r += NWV) {
+    float mv[NWV], M = -INFINITY, total = 0.f, sum[PER] = {};
+    Piece x[NWV];
 #pragma unroll
     for (int v = 0; v < NWV; ++v) {
-      const float f = fast_exp2(part[v][r][D] - base);
-      sum = fmaf(part[v][r][d], f, sum);
-      total = fmaf(part[v][r][D + 1], f, total);
+      mv[v] = state[v][r][0];
+      x[v] = *reinterpret_cast<const Piece *>(part[v][r] + (D < 64 ? lane & (D - 1) : PER * lane));
     }
-    const int row = row0 + r;
-    if (a.splits > 1) {
-      a.ws[((static_cast<int64_t>(b * a.p.heads + hk) * a.splits + split) * a.rows + row) * (D + 2) + d] = d == D ? M : sum;
-    } else if (d < D) {
-      const int rr = row / a.len_q, qi = row - rr * a.len_q;
-      static_cast<T *>(const_cast<void *>(a.o.data))[b * a.o.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.o.s1 +
-                                                     qi * a.o.s2 + d] =
-          static_cast<T>(total == 0.f ? 0.f : sum / total);
+#pragma unroll
+    for (int v = 0; v < NWV; ++v) M = fmaxf(M, mv[v]);
+    const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int v = 0; v < NWV; ++v) {
+      const float f = fast_exp2(mv[v] - base);
+      const float *e = reinterpret_cast<const float *>(&x[v]);
+      total = fmaf(state[v][r][1], f, total);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sum[i] = fmaf(e[i], f, sum[i]);
+    }
+    if (lane * PER < D) {
+      if (a.splits > 1) {
+        float *to = a.ws + ((static_cast<int64_t>(b * a.p.heads + hk) * a.splits + split) * a.rows + row0 + r) * (D + 2);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) to[PER * lane + i] = sum[i];
+        if (lane == 0) to[D] = M, to[D + 1] = total;
+      } else {
+        T *to = out_row(r);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) to[PER * lane + i] = static_cast<T>(total == 0.f ? 0.f : sum[i] / total);
+      }
     }
   }
 }
 
-// One wave an output row: the splits' partial states, rescaled to their largest
-// maximum.  Every lane takes the splits' (max, sum) of its share, then the wave
-// walks the splits with lane d on channels d, d + 64, ...
+// One wave an output row: the splits' partial states rescaled to their largest
+// maximum, 16 splits' loads in flight.
 template <typename T, int D>
 __global__ __launch_bounds__(64) void attend4_merge_kernel(Attend4 a) {
   const int lane = threadIdx.x, b = blockIdx.z, hk = blockIdx.y, r = blockIdx.x;
   const int n = (a.s.len[b] + a.split - 1) / a.split;
   const float *base = a.ws + (static_cast<int64_t>(b * a.p.heads + hk) * a.splits * a.rows + r) * (D + 2);
   const int64_t stride = static_cast<int64_t>(a.rows) * (D + 2);
-  constexpr int PER = (D + 63) / 64, U = 8;
-  float M = -INFINITY;
-  for (int s = lane; s < n; s += 64) M = fmaxf(M, base[s * stride + D]);
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor(M, x, 64));
-  const float at = M == -INFINITY ? 0.f : M;
-  float acc[PER] = {}, L = 0.f;
+  constexpr int PER = (D + 63) / 64, U = 16;
+  float acc[PER] = {}, L = 0.f, M = -INFINITY;
   for (int s0 = 0; s0 < n; s0 += U) {
-    float f[U], ls[U], x[U][PER];
+    float ms[U], ls[U], x[U][PER];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float *from = base + min(s0 + u, n - 1) * stride;
-      f[u] = from[D], ls[u] = from[D + 1];
+      ms[u] = from[D], ls[u] = from[D + 1];
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[u][i] = from[min(lane + 64 * i, D - 1)];
     }
+    const float before = M;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (s0 + u < n) {
-        const float e = fast_exp2(f[u] - at);
-        L = fmaf(ls[u], e, L);
+    for (int u = 0; u < U; ++u) M = fmaxf(M, ms[u]);
+    const float at = M == -INFINITY ? 0.f : M, corr = fast_exp2(before - at);
+    L *= corr;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = fmaf(x[u][i], e, acc[i]);
-      }
+    for (int i = 0; i < PER; ++i) acc[i] *= corr;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float e = s0 + u < n ? fast_exp2(ms[u] - at) : 0.f;  // (the last split again: finite, or NaN as it is)
+      L = fmaf(ls[u], e, L);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] = fmaf(x[u][i], e, acc[i]);
+    }
   }
-  const int rr = r / a.len_q, qi = r - rr * a.len_q;
+  const int rr = fdiv(r, a.by_len_q), qi = r - rr * a.len_q;
   T *out = static_cast<T *>(const_cast<void *>(a.o.data)) + b * a.o.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.o.s1 +
            qi * a.o.s2;
 #pragma unroll
@@ -344,29 +368,68 @@ int column_blocks(int dtype, int dim, int rows) {
 
 }  // namespace
 
-int attend4_split(int dtype, int dim, int heads_kv, int rows, int64_t total, int longest) {
-  const int per = 512 / dim * column_blocks(dtype, dim, rows);
-  const int64_t blocks = static_cast<int64_t>(heads_kv) * ((rows + per - 1) / per);
-  int64_t split = total * blocks / 1024;
-  split = split < 256 ? 256 : split > 4096 ? 4096 : split;
-  const int64_t n = (longest + split - 1) / split;  // splits; then of equal length
-  const int64_t even = n > 0 ? (longest + n - 1) / n : 0;
-  return static_cast<int>((even + 127) / 128 * 128 ? (even + 127) / 128 * 128 : 128);
+// Few workgroups are worth eight waves each, which take a CU by themselves; many
+// run four, two or three workgroups a CU.  The split is the one that a model of
+// the kernel's time likes best: every round of workgroups that fit the chip costs
+// its prologue and merge and its waves' tiles, a tile the larger of its own
+// latency and its share of the memory's rate; a split, the second kernel.
+void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
+  int64_t total = 0;
+  int longest = 1;
+  for (int i = 0; i < a->n; ++i) {
+    total += lens[i];
+    longest = lens[i] > longest ? lens[i] : longest;
+  }
+  const int dim = a->p.dim, nb = column_blocks(dtype, dim, a->rows), per = 512 / dim * nb;
+  a->blocks = (a->rows + per - 1) / per;
+  const double groups = static_cast<double>(a->p.heads) * a->blocks;
+  double best = 1e30;
+  for (int waves = 4; waves <= 8; waves += 4) {
+    if (waves == 8 && (dtype == TSATTN_F32 && dim == 256)) continue;  // (more registers than eight waves have)
+    const double slots = waves == 8 ? 256. : nb == 2 || dim == 256 ? 512. : 768.;
+    for (int split = 256; split <= kSplitTiles * kTile * 4; split *= 2) {
+      const int n = (longest + split - 1) / split;
+      const int even = ((longest + n - 1) / n + kTile * waves - 1) / (kTile * waves) * (kTile * waves);
+      if (even > kSplitTiles * kTile * 4) continue;
+      const double wgs = groups * (n == 1 ? a->n : static_cast<double>(total) / even + 0.5 * a->n);
+      const double tiles = static_cast<double>(even) / (kTile * waves);
+      const double busy = (wgs < slots ? wgs : slots) * waves;
+      const double rate = busy * 36 * dim / 6.2e6;  // us a tile at 6.2 TB/s
+      const double tile = rate > 0.8 ? rate : 0.8;
+      const double rounds = wgs <= slots ? 1. : wgs / slots + 0.3;
+      const double cost = rounds * (2.5 + tiles * tile) + (n > 1 ? 4.5 : 0.);
+      if (cost < best) {
+        best = cost;
+        a->waves = waves, a->split = even, a->splits = (longest + even - 1) / even;
+      }
+    }
+  }
 }
 
 hipError_t launch_attend4(const Attend4 &a, int dtype, hipStream_t st) {
-  const int dim = a.p.dim, nb = column_blocks(dtype, dim, a.rows), per = 512 / dim * nb;
-  const dim3 grid(a.p.heads * ((a.rows + per - 1) / per), a.splits, a.n);
+  const int dim = a.p.dim, nb = column_blocks(dtype, dim, a.rows);
+  const dim3 grid(a.p.heads * a.blocks, a.splits, a.n);
   auto launch = [&](auto t, auto g) {
     using T = decltype(t);
     constexpr int G = decltype(g)::value;
+    constexpr bool f32 = std::is_same_v<T, float>;
     {
       Probe pr_("attend4", st);
-      if constexpr (!std::is_same_v<T, float> && G < 8) {
-        if (nb == 2) attend4_kernel<T, G, 2><<<grid, dim3(64 * NWV), 0, st>>>(a);
-        else attend4_kernel<T, G, 1><<<grid, dim3(64 * NWV), 0, st>>>(a);
+      auto run = [&](auto n) {
+        constexpr int NB = decltype(n)::value;
+        if constexpr (!(f32 && G == 8)) {
+          if (a.waves == 8) {
+            attend4_kernel<T, G, NB, 8><<<grid, dim3(512), 0, st>>>(a);
+            return;
+          }
+        }
+        attend4_kernel<T, G, NB, 4><<<grid, dim3(256), 0, st>>>(a);
+      };
+      if constexpr (!f32 && G < 8) {
+        if (nb == 2) run(std::integral_constant<int, 2>{});
+        else run(std::integral_constant<int, 1>{});
       } else {
-        attend4_kernel<T, G, 1><<<grid, dim3(64 * NWV), 0, st>>>(a);
+        run(std::integral_constant<int, 1>{});
       }
     }
     if (a.splits > 1) {

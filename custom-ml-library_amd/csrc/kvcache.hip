@@ -48,21 +48,6 @@ __global__ __launch_bounds__(NT) void kv_append_int8_kernel(int B, int H, int T_
     static_cast<float *>(const_cast<void *>(scale.data))[b * scale.s0 + h * scale.s1 + (pos + t) * scale.s2] = s;
 }
 
-// n / d for 0 <= n < 2^31 as (mulhi(n, m) + n) >> l with l = ceil(log2 d)
-// and m = floor(2^32 (2^l - d) / d) + 1 (Granlund and Montgomery, "Division
-// by invariant integers using multiplication", PLDI 1994).
-struct FastDiv {
-  uint32_t m, l;
-};
-
-FastDiv make_fastdiv(uint32_t d) {
-  uint32_t l = 0;
-  while ((uint64_t(1) << l) < d) ++l;
-  return FastDiv{static_cast<uint32_t>((uint64_t(1) << 32) * ((uint64_t(1) << l) - d) / d + 1), l};
-}
-
-__device__ __forceinline__ uint32_t fdiv(uint32_t n, FastDiv f) { return (__umulhi(n, f.m) + n) >> f.l; }
-
 // max over each aligned group of G lanes (G = 8, 16, 32) of a non-negative
 // float, on its bit pattern: DPP quad swaps, the half-row and row mirrors,
 // then a swizzle across the two rows of a 32-lane half.

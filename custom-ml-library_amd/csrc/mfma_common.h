@@ -575,4 +575,19 @@ __device__ __forceinline__ float quad_row_max(float x) {
   return half_swap_max3(fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
 }
 
+// n / d for 0 <= n < 2^31 as (mulhi(n, m) + n) >> l with l = ceil(log2 d)
+// and m = floor(2^32 (2^l - d) / d) + 1 (Granlund and Montgomery, "Division
+// by invariant integers using multiplication", PLDI 1994).
+struct FastDiv {
+  uint32_t m, l;
+};
+
+inline FastDiv make_fastdiv(uint32_t d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < d) ++l;
+  return FastDiv{static_cast<uint32_t>((uint64_t(1) << 32) * ((uint64_t(1) << l) - d) / d + 1), l};
+}
+
+__device__ __forceinline__ uint32_t fdiv(uint32_t n, FastDiv f) { return (__umulhi(n, f.m) + n) >> f.l; }
+
 }  // namespace tsattn

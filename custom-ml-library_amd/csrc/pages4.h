@@ -110,17 +110,18 @@ void pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const
 // the cached positions, the queries' own the last len_q of them.
 struct Attend4 {
   Pages4 p;
-  Seqs s;
   View q, o;
   float *ws;
   const void *cos, *sin;  // rotate the queries; or NULL
-  int n, heads_q, rep, len_q, rows, causal;
+  int n, rep, len_q, rows, causal;
   int split, splits;      // positions a split (a multiple of 32), splits of the longest sequence
-  float sl;               // scale * log2(e)
+  int waves, blocks;      // of a workgroup; workgroups a KV head's rows take
+  float sl, sign;         // |scale| * log2(e) and the scale's sign, with the queries; 1 and 0 for no scale
+  FastDiv by_len_q;
+  Seqs s;
 };
-// Positions a split (a multiple of 32) for sequences of `total` positions together,
-// the longest `longest`, and `rows` query rows a KV head.
-int attend4_split(int dtype, int dim, int heads_kv, int rows, int64_t total, int longest);
+// Fills split, splits, waves and blocks in for the sequences' lengths.
+void plan_attend4(Attend4 *a, int dtype, const int32_t *lens);
 hipError_t launch_attend4(const Attend4 &a, int dtype, hipStream_t st);
 
 }  // namespace tsattn
