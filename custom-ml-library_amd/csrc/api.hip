@@ -638,12 +638,19 @@ size_t plan4(tsattn::Attend4 *a, int32_t dtype, int32_t n, int32_t i0, const int
 }
 
 // The host's side of a paged cache, and n different rows of it.
-int check_host4(const tsattn_pages4_host *h, int32_t n, const int32_t *rows) {
-  if (!h || !rows || !h->table || !h->lengths || !h->refs || !h->stack)
+int check_host4(const tsattn_pages4_host *h) {
+  if (!h || !h->table || !h->lengths || !h->refs || !h->stack || !h->changed || !h->dirty)
     return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
-  if (n <= 0 || h->rows <= 0 || h->columns <= 0 || h->page_size <= 0 || h->pages <= 0 || h->free < 0 ||
-      h->free > h->pages || static_cast<int64_t>(h->rows) * h->columns > INT32_MAX)
+  if (h->rows <= 0 || h->columns <= 0 || h->page_size <= 0 || h->pages <= 0 || h->free < 0 || h->free > h->pages ||
+      h->n_changed < 0 || static_cast<int64_t>(h->rows) * h->columns > INT32_MAX || h->n_changed > h->rows * h->columns)
     return fail(TSATTN_ERR_INVALID, "page table: sizes must be positive");
+  return TSATTN_OK;
+}
+
+int check_host_rows4(const tsattn_pages4_host *h, int32_t n, const int32_t *rows) {
+  int rc = check_host4(h);
+  if (rc) return rc;
+  if (!rows || n <= 0) return fail(TSATTN_ERR_INVALID, "page table: rows must be given");
   for (int32_t i = 0; i < n; ++i)
     if (rows[i] < 0 || rows[i] >= h->rows) return fail(TSATTN_ERR_INVALID, "page table: row %d out of range", rows[i]);
   char *seen = static_cast<char *>(calloc(static_cast<size_t>(h->rows), 1));
@@ -1172,38 +1179,22 @@ int tsattn_pages4_copy(const void *from, int64_t from_pages, void *to, int64_t t
                     "page copy launch");
 }
 
-int tsattn_pages4_set(int32_t *table, int64_t entries, int32_t n, const int32_t *at, const int32_t *value,
-                      void *stream) {
-  if (!table || !at || !value) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
-  if (n <= 0 || entries <= 0 || entries > INT32_MAX)
-    return fail(TSATTN_ERR_INVALID, "page table: sizes must be positive");
-  for (int32_t i = 0; i < n; ++i)
-    if (at[i] < 0 || at[i] >= entries) return fail(TSATTN_ERR_INVALID, "page table: entry %d out of range", at[i]);
-  char *seen = static_cast<char *>(calloc(static_cast<size_t>(entries), 1));
-  if (!seen) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
-  const bool ok = distinct(n, at, seen);
-  free(seen);
-  if (!ok) return fail(TSATTN_ERR_INVALID, "page table: an entry is set twice");
-  return hip_status(tsattn::launch_pages4_set(table, n, at, value, static_cast<hipStream_t>(stream)),
-                    "page table launch");
-}
-
 int tsattn_pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
-                       int32_t *dst, int32_t *at, int32_t *value, int32_t *counts) {
-  int rc = check_host4(h, n, rows);
+                       int32_t *dst, int32_t *copies) {
+  int rc = check_host_rows4(h, n, rows);
   if (rc) return rc;
-  if (!src || !dst || !at || !value || !counts) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  if (!src || !dst || !copies) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
   for (int32_t i = 0; i < n; ++i)
     if (steps <= 0 || static_cast<int64_t>(h->lengths[rows[i]]) + steps > static_cast<int64_t>(h->columns) * h->page_size)
       return fail(TSATTN_ERR_INVALID, "page table: %d positions after %d of row %d exceed it", steps,
                   h->lengths[rows[i]], rows[i]);
-  const int32_t need = tsattn::pages4_grow(h, n, rows, steps, src, dst, at, value, counts, counts + 1);
+  const int32_t need = tsattn::pages4_grow(h, n, rows, steps, src, dst, copies);
   if (need) return fail(TSATTN_ERR_INVALID, "page pool exhausted: %d pages needed, %d free", need, h->free);
   return TSATTN_OK;
 }
 
 int tsattn_pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *lengths) {
-  int rc = check_host4(h, n, rows);
+  int rc = check_host_rows4(h, n, rows);
   if (rc) return rc;
   if (!lengths) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
   for (int32_t i = 0; i < n; ++i)
@@ -1213,18 +1204,60 @@ int tsattn_pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, con
   return TSATTN_OK;
 }
 
-int tsattn_pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *index, int32_t *at,
-                          int32_t *value, int32_t *count) {
-  int rc = check_host4(h, n, rows);
+int tsattn_pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *index) {
+  int rc = check_host_rows4(h, n, rows);
   if (rc) return rc;
-  if (!index || !at || !value || !count) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  if (!index) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
   for (int32_t i = 0; i < n; ++i)
     if (index[i] < 0 || index[i] >= n) return fail(TSATTN_ERR_INVALID, "beam index out of range");
   int32_t *old = static_cast<int32_t *>(malloc(sizeof(int32_t) * n * (static_cast<size_t>(h->columns) + 1)));
   if (!old) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
-  tsattn::pages4_reorder(h, n, rows, index, old, at, value, count);
+  tsattn::pages4_reorder(h, n, rows, index, old);
   free(old);
   return TSATTN_OK;
+}
+
+int tsattn_pages4_clone(const tsattn_pages4_host *h, int32_t n, const int32_t *rows, tsattn_pages4_host *to,
+                        int32_t *src, int32_t *dst, int32_t *copies) {
+  int rc = check_host_rows4(h, n, rows);
+  if (rc || (rc = check_host4(to))) return rc;
+  if (!src || !dst || !copies) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  if (to->rows != n || to->columns != h->columns || to->page_size != h->page_size)
+    return fail(TSATTN_ERR_INVALID, "page table: a clone has the rows' number, columns and page size");
+  int32_t *number = static_cast<int32_t *>(malloc(sizeof(int32_t) * static_cast<size_t>(h->pages)));
+  if (!number) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
+  const int32_t used = tsattn::pages4_clone(h, n, rows, to, number, src, dst);
+  free(number);
+  if (used > to->pages) return fail(TSATTN_ERR_INVALID, "%d pages are in use", used);
+  *copies = used;
+  return TSATTN_OK;
+}
+
+int tsattn_pages4_compact(tsattn_pages4_host *h, int32_t *src, int32_t *dst, int32_t *copies) {
+  int rc = check_host4(h);
+  if (rc) return rc;
+  if (!src || !dst || !copies) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  int32_t *number = static_cast<int32_t *>(malloc(sizeof(int32_t) * static_cast<size_t>(h->pages)));
+  if (!number) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
+  tsattn::pages4_compact(h, number, src, dst, copies);
+  free(number);
+  return TSATTN_OK;
+}
+
+int tsattn_pages4_sync(tsattn_pages4_host *h, int32_t *table, void *stream) {
+  int rc = check_host4(h);
+  if (rc) return rc;
+  if (!table) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  if (!h->n_changed) return TSATTN_OK;
+  int32_t *at = static_cast<int32_t *>(malloc(sizeof(int32_t) * 2 * static_cast<size_t>(h->n_changed)));
+  if (!at) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
+  int32_t *value = at + h->n_changed;
+  const int32_t n = tsattn::pages4_changes(h, at, value);
+  rc = n ? hip_status(tsattn::launch_pages4_set(table, n, at, value, static_cast<hipStream_t>(stream)),
+                      "page table launch")
+         : TSATTN_OK;
+  free(at);
+  return rc;
 }
 
 }  // extern "C"

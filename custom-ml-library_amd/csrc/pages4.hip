@@ -22,21 +22,6 @@ constexpr float most_scale() {
   return std::is_same_v<T, f16> ? 10752.f : 1.3125f * 0x1p125f;
 }
 
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, T (&x)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    const u32x4 r = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
-    const T *e = reinterpret_cast<const T *>(&r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = e[i];
-  } else {
-    const f32x4 *q = reinterpret_cast<const f32x4 *>(p);
-    const f32x4 a = __builtin_nontemporal_load(q), b = __builtin_nontemporal_load(q + 1);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
-  }
-}
-
 // Four consecutive table entries.
 template <typename T>
 __device__ __forceinline__ void load4(const T *p, T (&x)[4]) {
@@ -58,28 +43,27 @@ __device__ __forceinline__ float scale_of(uint32_t m) {
   return m >= 0x7F800000u ? __builtin_nanf("") : s;
 }
 
-// Eight codes.  The quotient comes from the reciprocal and one correction: within
-// half an ulp of x / s, and exact where x / s is half way between two levels.
-// For 16-bit x no other quotient comes that near to such a point (x has at most 11
-// significant bits, the point times s 9), so the conversion's rounding (to nearest,
-// ties to even, saturating) decides as the real quotient does.  fp32 quotients
-// are truncated with a sticky last bit instead, so that none rounds onto one.
+// Eight codes.  The quotient is x / s to within an ulp's rounding: x times the
+// reciprocal in two parts, rounded once, so it is exact where x / s is half way
+// between two levels.  For 16-bit x no other quotient comes that near to such a point
+// (x has at most 11 significant bits, the point times s 9), so the conversion's
+// rounding (to nearest, ties to even, saturating) decides as the real quotient does.
+// fp32 quotients are truncated with a sticky last bit instead, so that none rounds
+// onto one.
 template <typename T>
-__device__ __forceinline__ uint32_t codes_of(const T (&x)[8], float s) {
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
 #pragma clang fp contract(off)
-  const float rc = 1.f / s;
+  const float rc = 1.f / s, rl = __builtin_fmaf(-rc, s, 1.f) * rc;
   float q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float a = static_cast<float>(x[i]);
-    const float q0 = a * rc;
-    q[i] = __builtin_fmaf(__builtin_fmaf(-q0, s, a), rc, q0);
+    q[i] = __builtin_fmaf(x[i], rc, x[i] * rl);
     if constexpr (std::is_same_v<T, float>) {
-      const float m = fabsf(q[i]), r = __builtin_fmaf(-m, s, fabsf(a));
+      const float m = fabsf(q[i]), r = __builtin_fmaf(-m, s, fabsf(x[i]));
       uint32_t u = __builtin_bit_cast(uint32_t, m);
       if (r < 0.f && u != 0u) --u;
       if (r != 0.f) u |= 1u;
-      q[i] = copysignf(__builtin_bit_cast(float, u), a);
+      q[i] = copysignf(__builtin_bit_cast(float, u), x[i]);
     }
   }
   uint32_t w = 0;
@@ -90,32 +74,103 @@ __device__ __forceinline__ uint32_t codes_of(const T (&x)[8], float s) {
   return w;
 }
 
+// Largest of four lanes c, c + 16, c + 32, c + 48.
+__device__ __forceinline__ uint32_t quad_row_umax(uint32_t x) {
+  uint32_t a = x, b = x;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  x = a = b = max(a, b);
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+  return max(a, b);
+}
+
+// Keys' words <-> values' words.  Lane 4 g' + q (of any g) has, of channels 8 o .. + 7,
+// the codes of key 4 g' + q in word a and of key 16 + 4 g' + q in word b; the quad's
+// transpose gives it channels 8 o + q (in a) and 8 o + 4 + q (in b) of the quad's eight
+// keys: a value word each.  Two butterflies inside the quad (codes between lanes q
+// and q ^ 1, bytes between q and q ^ 2), each its own inverse, then halves.
+struct Transpose {
+  uint32_t m1, m2, r1, r2;
+  __device__ __forceinline__ explicit Transpose(int lane)
+      : m1(lane & 1 ? 0xF0F0F0F0u : 0x0F0F0F0Fu), m2(lane & 2 ? 0xFF00FF00u : 0x00FF00FFu),
+        r1(lane & 1 ? 4u : 28u), r2(lane & 2 ? 8u : 24u) {}
+  template <int CTRL>
+  __device__ __forceinline__ static uint32_t exchange(uint32_t x, uint32_t mask, uint32_t turn) {
+    const uint32_t y = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xF, 0xF, true));
+    return (x & mask) | (__builtin_amdgcn_alignbit(y, y, turn) & ~mask);
+  }
+  __device__ __forceinline__ uint32_t codes(uint32_t x) const { return exchange<0xB1>(x, m1, r1); }  // lanes q, q ^ 1
+  __device__ __forceinline__ uint32_t bytes(uint32_t x) const { return exchange<0x4E>(x, m2, r2); }  // lanes q, q ^ 2
+  __device__ __forceinline__ void to_values(uint32_t &a, uint32_t &b) const {
+    const uint32_t x = bytes(codes(a)), y = bytes(codes(b));
+    a = __builtin_amdgcn_perm(y, x, 0x05040100u);  // low halves: the first channel, keys of x then of y
+    b = __builtin_amdgcn_perm(y, x, 0x07060302u);
+  }
+  __device__ __forceinline__ void to_keys(uint32_t &a, uint32_t &b) const {
+    const uint32_t x = __builtin_amdgcn_perm(b, a, 0x05040100u), y = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    a = codes(bytes(x));
+    b = codes(bytes(y));
+  }
+};
+
+// Where a lane's word of channel 32 ks + 8 g + 4 e + q (c = 4 g' + q) lies among the
+// values' words: lane 16 g' + 8 (g & 1) + 4 e + q, word 2 ks + g / 2.
+template <int G>
+__device__ __forceinline__ int value_at(int c, int g, int ks, int e) {
+  return word4<G>(2 * ks + (g >> 1), 16 * (c >> 2) + 8 * (g & 1) + 4 * e + (c & 3));
+}
+
+template <int G>
+__device__ __forceinline__ void store_words(char *to, int lane, const uint32_t (&word)[2 * G]) {
+  if constexpr (G == 1) {
+    *reinterpret_cast<u32x2 *>(to + 8 * lane) = u32x2{word[0], word[1]};
+  } else {
+#pragma unroll
+    for (int q = 0; q < G / 2; ++q)
+      *reinterpret_cast<u32x4 *>(to + (64 * q + lane) * 16) =
+          u32x4{word[4 * q], word[4 * q + 1], word[4 * q + 2], word[4 * q + 3]};
+  }
+}
+template <int G>
+__device__ __forceinline__ void load_words(const char *from, int lane, uint32_t (&word)[2 * G]) {
+  if constexpr (G == 1) {
+    const u32x2 r = *reinterpret_cast<const u32x2 *>(from + 8 * lane);
+    word[0] = r[0], word[1] = r[1];
+  } else {
+#pragma unroll
+    for (int q = 0; q < G / 2; ++q) {
+      const u32x4 r = *reinterpret_cast<const u32x4 *>(from + (64 * q + lane) * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word[4 * q + i] = r[i];
+    }
+  }
+}
+
 // One wave quantises the new positions of one tile, head and side (keys or
 // values).  Lane (c, g) takes keys c and 16 + c and their channels 32 ks + 8 g .. + 7:
 // 16-byte loads of which four make a group, and the words of the keys' layout.
-// Values' words hold one channel of eight keys: the codes cross the wave through
-// LDS.  A tile that is only partly new keeps its other positions: keys' words
-// belong to one position each, values' are read, merged and written.
+// Values' words hold one channel of eight keys: a transpose in each quad of lanes, and
+// one trip through LDS to the lanes that store them.  A tile that is only partly new
+// keeps its other positions: keys' words belong to one position each, values' are
+// read, merged and written.
 template <typename T, int G>
 __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
   constexpr int D = 32 * G, W = 2 * G;
-  __shared__ __attribute__((aligned(16))) uint32_t lds[NW][kTile * (D / 8)];
+  __shared__ __attribute__((aligned(16))) char lds[NW][16 * D];
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x * NW + wv;  // (tile, side, head), the tile fastest
   const int b = blockIdx.y;
+  const int pos = a.s.len[b], row = a.s.row[b];
   const int hs = unit / a.tiles, ti = unit - hs * a.tiles;
   const bool values = hs & 1;
   const int h = hs >> 1;
-  const int pos = a.s.len[b];
   const int tile = pos / kTile + ti, first = tile * kTile - pos;  // new position of the tile's first
   if (h >= a.p.heads || first >= a.len) return;                   // (a whole wave; no barrier follows)
   const bool full = first >= 0 && first + kTile <= a.len;
-  char *to = tile4(a.p, a.s.row[b], tile, h) + (values ? 16 * D : 0);
-  uint16_t *sto = reinterpret_cast<uint16_t *>(tile4(a.p, a.s.row[b], tile, h) + (values ? 34 : 32) * D);
   const View &v = values ? a.v : a.k;
   const T *src = static_cast<const T *>(v.data) + b * v.s0 + h * v.s1 + 8 * g;
-  T x[2][G][8];
+  constexpr int QW = sizeof(T) / 2;  // 16-byte loads a piece
+  u32x4 raw[W][QW];
   bool live[2];
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
@@ -123,34 +178,56 @@ __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
     live[kb] = t >= 0 && t < a.len;
     const int64_t at = live[kb] ? t : (first < 0 ? 0 : first);  // (else a new position's row: in bounds)
 #pragma unroll
-    for (int ks = 0; ks < G; ++ks) load8<T>(src + at * v.s2 + 32 * ks, x[kb][ks]);
-    if (a.cos && !values) {
+    for (int ks = 0; ks < G; ++ks)
+#pragma unroll
+      for (int i = 0; i < QW; ++i) raw[kb * G + ks][i] = reinterpret_cast<const u32x4 *>(src + at * v.s2 + 32 * ks)[i];
+  }
+  char *tp = tile4(a.p, row, tile, h);
+  char *to = tp + (values ? 16 * D : 0);
+  uint16_t *sto = reinterpret_cast<uint16_t *>(tp + (values ? 34 : 32) * D);
+  if (a.cos && !values) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int64_t at = live[kb] ? first + 16 * kb + c : (first < 0 ? 0 : first);
 #pragma unroll
       for (int ks = 0; ks < G; ++ks) {
         T cw[4], sw[4];
         const int64_t e = (pos + at) * (D / 2) + 16 * ks + 4 * g;
         load4<T>(static_cast<const T *>(a.cos) + e, cw);
         load4<T>(static_cast<const T *>(a.sin) + e, sw);
+        u32x4(&x)[QW] = raw[kb * G + ks];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rotate_pair(x[kb][ks][2 * i], x[kb][ks][2 * i + 1], cw[i], sw[i], false);
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(T) == 2) {
+            x[0][i] = rotate_word<T>(x[0][i], cw[i], sw[i], false);
+          } else {
+            const uint32_t u0 = x[i >> 1][2 * (i & 1)], u1 = x[i >> 1][2 * (i & 1) + 1];
+            T x0 = __builtin_bit_cast(T, u0), x1 = __builtin_bit_cast(T, u1);
+            rotate_pair(x0, x1, cw[i], sw[i], false);
+            x[i >> 1][2 * (i & 1)] = __builtin_bit_cast(uint32_t, x0);
+            x[i >> 1][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, x1);
+          }
+        }
       }
     }
   }
   uint32_t word[W], sc[W];
 #pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
+  for (int w = 0; w < W; ++w) {
+    float x[8];
 #pragma unroll
-    for (int ks = 0; ks < G; ++ks) {
-      uint32_t m = 0;
+    for (int i = 0; i < QW; ++i) {
+      const T *e = reinterpret_cast<const T *>(&raw[w][i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        m = max(m, __builtin_bit_cast(uint32_t, static_cast<float>(x[kb][ks][i])) & 0x7FFFFFFFu);
-      m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16, 64)));
-      m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32, 64)));
-      const float s = scale_of<T>(m);
-      sc[kb * G + ks] = __builtin_bit_cast(uint32_t, s) >> 16;
-      word[kb * G + ks] = codes_of<T>(x[kb][ks], s == s ? s : 1.f);
+      for (int j = 0; j < 8 / QW; ++j) x[i * (8 / QW) + j] = static_cast<float>(e[j]);
     }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
+    const float s = scale_of<T>(quad_row_umax(m));
+    sc[w] = __builtin_bit_cast(uint32_t, s) >> 16;
+    word[w] = codes_of<T>(x, s == s ? s : 1.f);
+  }
   // scales: lane g stores those of words g, g + 4, ..
 #pragma unroll
   for (int w0 = 0; w0 < W; w0 += 4) {
@@ -163,14 +240,7 @@ __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
   }
   if (!values) {
     if (full) {
-      if constexpr (G == 1) {
-        *reinterpret_cast<u32x2 *>(to + 8 * lane) = u32x2{word[0], word[1]};
-      } else {
-#pragma unroll
-        for (int q = 0; q < W / 4; ++q)
-          *reinterpret_cast<u32x4 *>(to + (64 * q + lane) * 16) =
-              u32x4{word[4 * q], word[4 * q + 1], word[4 * q + 2], word[4 * q + 3]};
-      }
+      store_words<G>(to, lane, word);
     } else {
 #pragma unroll
       for (int w = 0; w < W; ++w)
@@ -178,45 +248,34 @@ __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
     }
     return;
   }
-  // [key][D / 2 bytes] in LDS, then each lane picks its channels' codes
-  uint32_t *mine = lds[wv];
+  char *mine = lds[wv];
+  const Transpose tr(lane);
 #pragma unroll
-  for (int w = 0; w < W; ++w) mine[(16 * (w / G) + c) * (D / 8) + 4 * (w % G) + g] = word[w];
+  for (int ks = 0; ks < G; ++ks) {
+    uint32_t x = word[ks], y = word[G + ks];
+    tr.to_values(x, y);
+    *reinterpret_cast<uint32_t *>(mine + value_at<G>(c, g, ks, 0)) = x;
+    *reinterpret_cast<uint32_t *>(mine + value_at<G>(c, g, ks, 1)) = y;
+  }
   wait_lgkm0();  // (own wave's writes)
   __builtin_amdgcn_sched_barrier(0);
-  const uint8_t *bytes = reinterpret_cast<const uint8_t *>(mine);
-  uint32_t keep = 0;  // codes of positions that are not new
-  if (!full)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int t = first + 16 * (j >> 2) + 4 * g + (j & 3);
-      if (t < 0 || t >= a.len) keep |= 0xFu << (4 * j);
-    }
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    uint32_t y = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = 16 * (j >> 2) + 4 * g + (j & 3);
-      const uint32_t two = bytes[key * (D / 2) + 8 * w + (c >> 1)];
-      y |= ((two >> (4 * (c & 1))) & 0xFu) << (4 * j);
-    }
-    word[w] = y;
+  load_words<G>(mine, lane, word);
+  if (full) {
+    store_words<G>(to, lane, word);
+    return;
   }
-  if (keep) {
+  uint32_t keep = 0;  // codes of positions that are not new
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int t = first + 16 * (j >> 2) + 4 * g + (j & 3);
+    if (t < 0 || t >= a.len) keep |= 0xFu << (4 * j);
+  }
+  if (keep != 0xFFFFFFFFu)
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       uint32_t *at = reinterpret_cast<uint32_t *>(to + word4<G>(w, lane));
-      if (keep != 0xFFFFFFFFu) *at = (*at & keep) | (word[w] & ~keep);
+      *at = (*at & keep) | (word[w] & ~keep);
     }
-  } else if constexpr (G == 1) {
-    *reinterpret_cast<u32x2 *>(to + 8 * lane) = u32x2{word[0], word[1]};
-  } else {
-#pragma unroll
-    for (int q = 0; q < W / 4; ++q)
-      *reinterpret_cast<u32x4 *>(to + (64 * q + lane) * 16) =
-          u32x4{word[4 * q], word[4 * q + 1], word[4 * q + 2], word[4 * q + 3]};
-  }
 }
 
 struct ReadArgs {
@@ -248,12 +307,12 @@ __device__ __forceinline__ void store8(T *p, uint32_t w, float s, bool live) {
 
 // The values of positions first .. first + len - 1 of every sequence into k, v
 // [n, heads, len, D], zero past its length.  One wave a tile, head and side;
-// values' codes cross the wave through LDS as in the append.
+// values' words go the append's way back.
 template <typename T, int G>
 __global__ __launch_bounds__(NT) void read_kernel(ReadArgs ra) {
   constexpr int D = 32 * G, W = 2 * G;
   const RowArgs &a = ra.r;
-  __shared__ __attribute__((aligned(16))) uint32_t lds[NW][kTile * (D / 8)];
+  __shared__ __attribute__((aligned(16))) char lds[NW][16 * D];
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x * NW + wv;
@@ -266,55 +325,34 @@ __global__ __launch_bounds__(NT) void read_kernel(ReadArgs ra) {
   if (h >= a.p.heads || first >= a.len) return;                   // (a whole wave; no barrier follows)
   const View &v = values ? a.v : a.k;
   T *out = static_cast<T *>(const_cast<void *>(v.data)) + b * v.s0 + h * v.s1;
-  uint32_t word[W];
-  const uint16_t *sfrom = nullptr;
   const bool held = tile * kTile < n;  // (a tile past the length may have no page)
+  uint32_t word[W] = {};
+  float sc[W] = {};
   if (held) {
     const char *base = tile4(a.p, a.s.row[b], tile, h);
-    const char *from = base + (values ? 16 * D : 0);
-    sfrom = reinterpret_cast<const uint16_t *>(base + (values ? 34 : 32) * D);
-    if constexpr (G == 1) {
-      const u32x2 r = *reinterpret_cast<const u32x2 *>(from + 8 * lane);
-      word[0] = r[0], word[1] = r[1];
-    } else {
+    load_words<G>(base + (values ? 16 * D : 0), lane, word);
+    const uint16_t *sfrom = reinterpret_cast<const uint16_t *>(base + (values ? 34 : 32) * D);
 #pragma unroll
-      for (int q = 0; q < W / 4; ++q) {
-        const u32x4 r = *reinterpret_cast<const u32x4 *>(from + (64 * q + lane) * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) word[4 * q + i] = r[i];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int w = 0; w < W; ++w) word[w] = 0;
+    for (int w = 0; w < W; ++w) sc[w] = from_bf16(sfrom[scale4<G>(16 * (w / G) + c, w % G)]);
   }
-  if (values) {
-    uint32_t *mine = lds[wv];
-    // words back in (q, lane) order: byte word4(w, lane)
-#pragma unroll
-    for (int w = 0; w < W; ++w) mine[word4<G>(w, lane) / 4] = word[w];
+  if (values && held) {  // to keys' words
+    char *mine = lds[wv];
+    store_words<G>(mine, lane, word);
     wait_lgkm0();  // (own wave's writes)
     __builtin_amdgcn_sched_barrier(0);
-    const uint8_t *bytes = reinterpret_cast<const uint8_t *>(mine);
+    const Transpose tr(lane);
 #pragma unroll
-    for (int w = 0; w < W; ++w) {  // as keys' words: key 16 (w / G) + c, channels 32 (w % G) + 8 g .. + 7
-      uint32_t y = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = 32 * (w % G) + 8 * g + i;
-        const int j = 4 * (w / G) + (c & 3);
-        const uint32_t two = bytes[word4<G>(d >> 4, 16 * (c >> 2) + (d & 15)) + (j >> 1)];
-        y |= ((two >> (4 * (j & 1))) & 0xFu) << (4 * i);
-      }
-      word[w] = y;
+    for (int ks = 0; ks < G; ++ks) {
+      word[ks] = *reinterpret_cast<const uint32_t *>(mine + value_at<G>(c, g, ks, 0));
+      word[G + ks] = *reinterpret_cast<const uint32_t *>(mine + value_at<G>(c, g, ks, 1));
+      tr.to_keys(word[ks], word[G + ks]);
     }
   }
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     const int key = 16 * (w / G) + c, t = first + key;
     if (t < 0 || t >= a.len) continue;
-    const float s = held ? from_bf16(sfrom[scale4<G>(key, w % G)]) : 0.f;
-    store8<T>(out + static_cast<int64_t>(t) * v.s2 + 32 * (w % G) + 8 * g, word[w], s, tile * kTile + key < n);
+    store8<T>(out + static_cast<int64_t>(t) * v.s2 + 32 * (w % G) + 8 * g, word[w], sc[w], tile * kTile + key < n);
   }
 }
 

@@ -26,13 +26,11 @@ from .. import _lib
 from ..device import device as parse_device
 from ..device import launch
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
-from .attention import (_aligned16, _dtype_code, _rope_rows, _view, rope_tables,
-                        scaled_dot_product_attention)
+from .attention import _dtype_code, _rope_rows, rope_tables, scaled_dot_product_attention
 
 # Query rows per KV head from which dequantising the pages once and attending on
 # the matrix cores is the faster way.
 PROMPT_ROWS = 128
-_MOST_SET = 1024  # table entries written by the kernel; more go up as one copy
 
 
 def _ints(x):
@@ -43,13 +41,22 @@ def _rows(t):
     """``t`` with rows that the kernels read as they are: 16-byte aligned, channels side by side."""
     import torch
 
-    return t if t.stride(-1) == 1 and _aligned16(t) else t.clone(memory_format=torch.contiguous_format)
+    a, b, c, d = t.stride()
+    if d == 1 and not (a | b | c) & 7 and not t.data_ptr() & 15:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _view(t) -> _lib.View:
+    v = _lib.View()
+    v.data = t.data_ptr()
+    v.stride[:] = t.stride()
+    return v
 
 
 class _Pages:
     """The pool, the page table (host and device) and the rows' lengths.  Pages are given out and
-    taken back by the library's host calls over these arrays (``tsattn_pages4_grow`` / ``_cut`` /
-    ``_reorder``)."""
+    taken back by the library's host calls over these arrays (``tsattn_pages4_host``)."""
 
     def __init__(self, rows: int, heads: int, dim: int, columns: int, page_size: int, num_pages: int, dev):
         import torch
@@ -59,60 +66,56 @@ class _Pages:
         if not self.page_bytes:
             raise NotImplementedError("paged caches take head dims 32, 64, 128 and 256, up to 4096 heads and "
                                       "pages of 32, 64, .. 4096 positions")
-        self.lengths = np.zeros(rows, np.int32)
-        self.lengths_at = self.lengths.ctypes.data
-        # what the host calls give back: page copies, table entries, how many of each
-        self.src, self.dst = np.empty(rows, np.int32), np.empty(rows, np.int32)
-        self.at, self.value = np.empty(rows * columns, np.int32), np.empty(rows * columns, np.int32)
-        self.counts = np.zeros(2, np.int32)
-        self.out = tuple(x.ctypes.data for x in (self.src, self.dst, self.at, self.value, self.counts))
+        # the host's arrays, side by side; src, dst: page copies that a call asks for
+        most, entries = max(rows, num_pages), rows * columns
+        sizes = {"host": entries, "lengths": rows, "refs": num_pages, "stack": num_pages, "changed": entries,
+                 "src": most, "dst": most, "copies": 1, "dirty": (entries + 3) // 4}
+        memory, at, where = np.zeros(sum(sizes.values()), np.int32), 0, {}
+        base = memory.ctypes.data
+        for name, n in sizes.items():
+            setattr(self, name, memory[at:at + n])
+            where[name] = base + 4 * at
+            at += n
+        self.host = self.host.reshape(rows, columns)
+        self.lengths_at = where["lengths"]
+        self.out = where["src"], where["dst"], where["copies"]
+        self.tables = t = _lib.Pages4Host()
+        t.rows, t.columns, t.page_size, t.pages = rows, columns, page_size, num_pages
+        t.table, t.lengths, t.refs, t.stack = (where[x] for x in ("host", "lengths", "refs", "stack"))
+        t.changed, t.dirty = where["changed"], where["dirty"]
         # (what no append has written weighs nothing: positions past a row's length are masked)
         self.pool = torch.empty((num_pages, self.page_bytes), dtype=torch.uint8, device=dev.torch)
-        self.table = torch.zeros((rows, columns), dtype=torch.int32, device=dev.torch)
-        self.start(np.full((rows, columns), -1, np.int32), 0)
-
-    def start(self, host, used: int) -> None:
-        """Begin with the table ``host``, whose pages are the pool's first ``used``."""
-        pages = self.pool.shape[0]
-        self.host = host
-        self.refs = np.bincount(host[host >= 0], minlength=pages).astype(np.int32)
-        self.stack = np.arange(pages - 1, -1, -1, dtype=np.int32)  # free pages, the next one last
-        self.tables = t = _lib.Pages4Host()
-        t.rows, t.columns = host.shape
-        t.page_size, t.pages, t.free = self.page_size, pages, pages - used
-        t.table, t.lengths, t.refs = host.ctypes.data, self.lengths_at, self.refs.ctypes.data
-        t.stack = self.stack.ctypes.data
+        self.table = torch.empty((rows, columns), dtype=torch.int32, device=dev.torch)
         self.desc = d = _lib.Pages4()
-        d.pool, d.num_pages = self.pool.data_ptr(), pages
-        d.heads, d.page_size, d.dim = self.heads, self.page_size, self.dim
-        d.table, d.table_rows, d.table_stride = self.table.data_ptr(), *host.shape
+        d.pool, d.num_pages, d.heads, d.page_size, d.dim = self.pool.data_ptr(), num_pages, heads, page_size, dim
+        d.table, d.table_rows, d.table_stride = self.table.data_ptr(), rows, columns
+
+    def clear(self) -> None:
+        """Every page free, every row empty."""
+        pages = len(self.refs)
+        self.host.fill(-1)
+        self.stack[:] = np.arange(pages - 1, -1, -1)  # (the next one is the last)
+        self.tables.free = pages
 
     @property
     def free(self) -> int:
         return self.tables.free
 
-    def upload(self, n: int) -> None:
-        """The first ``n`` entries of ``at`` / ``value`` to the device's table."""
-        if n > _MOST_SET:
-            import torch
+    def sync(self) -> None:
+        """The device's table up to date."""
+        if self.tables.n_changed:
+            _lib.check(launch(self.device, _lib.load().tsattn_pages4_sync, self.tables, self.desc.table), "page table")
 
-            self.table.copy_(torch.from_numpy(np.maximum(self.host, 0)))
-        elif n:
-            _lib.check(launch(self.device, _lib.load().tsattn_pages4_set, self.desc.table, self.host.size, n,
-                              self.out[2], self.out[3]), "page table")
-
-    def move(self, source, target, n: int, src, dst) -> None:
-        _lib.check(launch(self.device, _lib.load().tsattn_pages4_copy, source.data_ptr(), source.shape[0],
-                          target.data_ptr(), target.shape[0], self.page_bytes, n, src, dst), "page copy")
+    def move(self, source, target) -> None:
+        """The page copies that the last host call asked for."""
+        n = int(self.copies[0])
+        if n:
+            _lib.check(launch(self.device, _lib.load().tsattn_pages4_copy, source.data_ptr(), source.shape[0],
+                              target.data_ptr(), target.shape[0], self.page_bytes, n, *self.out[:2]), "page copy")
 
     def grow(self, n: int, rows: int, steps: int) -> None:
         """Pages of their own for the next ``steps`` positions of the ``n`` rows (an address)."""
         _lib.check(_lib.load().tsattn_pages4_grow(self.tables, n, rows, steps, *self.out), "page table")
-        copies, sets = self.counts.tolist()
-        if copies:
-            self.move(self.pool, self.pool, copies, *self.out[:2])
-        if sets:
-            self.upload(sets)
 
     def cut(self, rows, lengths) -> None:
         """``rows`` end at ``lengths``; pages wholly past them are given back."""
@@ -120,10 +123,13 @@ class _Pages:
         _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows.ctypes.data, lengths.ctypes.data),
                    "page table")
 
-    def reorder(self, rows, index) -> None:
-        _lib.check(_lib.load().tsattn_pages4_reorder(self.tables, len(rows), rows.ctypes.data, index.ctypes.data,
-                                                     *self.out[2:]), "page table")
-        self.upload(int(self.counts[0]))
+    def clone(self, rows, num_pages: int) -> "_Pages":
+        """The rows with pages of their own, in a pool of ``num_pages``."""
+        other = _Pages(len(rows), self.heads, self.dim, self.host.shape[1], self.page_size, num_pages, self.device)
+        _lib.check(_lib.load().tsattn_pages4_clone(self.tables, len(rows), rows.ctypes.data, other.tables, *self.out),
+                   "page table")
+        self.move(self.pool, other.pool)
+        return other
 
 
 class PagedKVCache:
@@ -150,8 +156,9 @@ class PagedKVCache:
             num_pages = batch_size * columns
         if num_pages <= 0:
             raise ValueError("cache dimensions and capacity must be positive")
-        self.max_seq_len = max_seq_len
+        self.max_seq_len, self._code = max_seq_len, _dtype_code(self.dtype)
         self._core = _Pages(batch_size, num_heads, head_dim, columns, page_size, num_pages, dev)
+        self._core.clear()
         self._select(np.arange(batch_size, dtype=np.int32))
 
     def _select(self, rows) -> None:
@@ -204,7 +211,7 @@ class PagedKVCache:
         ``rotary_embedding`` does.  Nothing changes if the pool has too few free pages.
         """
         self._check(key, value)
-        core, steps = self._core, key.shape[2]
+        core, steps = self._core, key._data.shape[2]
         lens, lens_at = self._lens()
         most = int(lens.max()) + steps
         if steps == 0 or most > self.max_seq_len:
@@ -217,11 +224,13 @@ class PagedKVCache:
         k, v = (_rows(t._data.to(self.dtype)) for t in (key, value))
         core.grow(len(lens), self._rows_at, steps)
         try:
+            core.move(core.pool, core.pool)
+            core.sync()
             _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
                               _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
         except BaseException:
             core.lengths[self._rows] += steps  # (the new pages go back)
-            core.cut(self._rows, lens - steps if self._whole else lens)
+            core.cut(self._rows, core.lengths[self._rows] - steps)
             raise
         if self._whole:
             core.lengths += steps
@@ -235,19 +244,17 @@ class PagedKVCache:
         lens = self._core.lengths[self._rows]
         return lens, lens.ctypes.data
 
-    @property
-    def _code(self) -> int:
-        return _dtype_code(self.dtype)
-
     def _check(self, key: Tensor, value: Tensor) -> None:
         """``KVCache``'s refusals, in its order."""
-        if key.device != self.device or value.device != self.device:
+        dev = self._core.device
+        if any(x.device is not dev and x.device != dev for x in (key, value)):
             raise ValueError("cache and key/value tensors must be on the same device")
-        if is_grad_enabled() and (key.requires_grad or value.requires_grad):
+        if (key.requires_grad or value.requires_grad) and is_grad_enabled():
             raise RuntimeError("KVCache is inference-only; use no_grad() for differentiable inputs")
-        if key.ndim != 4 or key.shape[:2] != (self.batch_size, self.num_heads) or key.shape[-1] != self.head_dim:
+        shape = tuple(key._data.shape)
+        if len(shape) != 4 or shape[:2] != (len(self._rows), self._core.heads) or shape[3] != self._core.dim:
             raise ValueError("key shape does not match cache configuration")
-        if value.shape != key.shape:
+        if tuple(value._data.shape) != shape:
             raise ValueError("value shape does not match cache configuration")
 
     def get(self, last: int | None = None) -> tuple[Tensor, Tensor]:
@@ -264,6 +271,7 @@ class PagedKVCache:
         shape, dev = (len(lens), core.heads, steps, core.dim), core.pool.device
         out = [torch.empty(shape, dtype=self.dtype, device=dev) for _ in range(2)]
         if steps:
+            core.sync()
             _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
                               _view(out[0]), _view(out[1]), self._rows_at, lens_at, first.ctypes.data), "paged read")
         return tuple(Tensor(x, device=core.device) for x in out)
@@ -277,7 +285,7 @@ class PagedKVCache:
         if len(index) == 0 or len(np.unique(index)) != len(index):
             raise ValueError("rows must be different and at least one")
         view = object.__new__(PagedKVCache)
-        view.dtype, view.max_seq_len, view._core = self.dtype, self.max_seq_len, self._core
+        view.dtype, view.max_seq_len, view._code, view._core = self.dtype, self.max_seq_len, self._code, self._core
         view._select(np.ascontiguousarray(self._rows[index]))
         return view
 
@@ -304,38 +312,26 @@ class PagedKVCache:
         """Cut every row to ``length`` positions, or to a length of its own (a sequence of them);
         pages wholly past it are given back."""
         want = np.asarray(length)
-        if want.dtype.kind not in "iu" or want.shape not in ((), (self.batch_size,)):
+        if want.dtype.kind not in "iu" or want.shape not in ((), self._rows.shape):
             raise ValueError("truncate takes one integer length, or one per row")
-        lens, _ = self._lens()
-        if (want < 0).any() or (want > lens).any():
+        if want.max() >= 2**31 or want.min() < -(2**31):
             raise ValueError("truncate length must be between zero and the current length")
         self._core.cut(self._rows, want if want.shape else np.full_like(self._rows, want))
 
     def reorder(self, indices) -> None:
         """Row i becomes row ``indices[i]``, sharing its pages: no keys or values move.  Rows that
         take over the same row share until one appends (``append`` copies the page)."""
-        self._core.reorder(self._rows, self._indices(indices, (self.batch_size,)))
+        index = self._indices(indices, self._rows.shape)
+        _lib.check(_lib.load().tsattn_pages4_reorder(self._core.tables, len(index), self._rows_at, index.ctypes.data),
+                   "page table")
 
     def copy(self, num_pages: int | None = None) -> "PagedKVCache":
         """A cache of these rows with a pool of its own (``num_pages``, by default as many as this
         one has), its pages in use side by side; rows that share pages share them there."""
-        core = self._core
-        host = core.host if self._whole else core.host[self._rows]
-        live, new = self._renumber(host, self.num_pages)
-        num_pages = self.num_pages if num_pages is None else num_pages
-        if num_pages < max(len(live), 1):
-            raise ValueError(f"{len(live)} pages are in use")
         other = object.__new__(PagedKVCache)
-        other.dtype, other.max_seq_len = self.dtype, self.max_seq_len
-        there = other._core = _Pages(len(host), core.heads, core.dim, host.shape[1], core.page_size, num_pages,
-                                     core.device)
-        other._select(np.arange(len(host), dtype=np.int32))
-        there.lengths[:] = core.lengths[self._rows]
-        there.start(new, len(live))
-        if len(live):
-            to = np.arange(len(live), dtype=np.int32)
-            core.move(core.pool, there.pool, len(live), live.ctypes.data, to.ctypes.data)
-            self._tell(there)
+        other.dtype, other.max_seq_len, other._code = self.dtype, self.max_seq_len, self._code
+        other._core = self._core.clone(self._rows, self._pool_size(num_pages))
+        other._select(np.arange(len(self._rows), dtype=np.int32))
         return other
 
     def compact(self, num_pages: int | None = None) -> int:
@@ -343,45 +339,22 @@ class PagedKVCache:
         size (smaller or larger); returns how many are in use."""
         core = self._core
         if num_pages is None:
-            # the pages past the front move into its holes: none is both read and written
-            live = np.flatnonzero(core.refs).astype(np.int32)
-            n = len(live)
-            moved, holes = live[live >= n], np.flatnonzero(core.refs[:n] == 0).astype(np.int32)
-            if len(moved):
-                core.move(core.pool, core.pool, len(moved), moved.ctypes.data, holes.ctypes.data)
-            to = np.arange(self.num_pages, dtype=np.int32)
-            to[moved] = holes
-            new = np.where(core.host >= 0, to[core.host], np.int32(-1))
+            _lib.check(_lib.load().tsattn_pages4_compact(core.tables, *core.out), "page table")
+            core.move(core.pool, core.pool)
         else:
-            import torch
+            core.__dict__.update(core.clone(np.arange(len(core.lengths), dtype=np.int32),
+                                            self._pool_size(num_pages)).__dict__)
+        return self.pages_in_use
 
-            live, new = self._renumber(core.host, self.num_pages)
-            n = len(live)
-            if num_pages < max(n, 1):
-                raise ValueError(f"{n} pages are in use")
-            pool = torch.empty((num_pages, core.page_bytes), dtype=torch.uint8, device=core.pool.device)
-            if n:
-                to = np.arange(n, dtype=np.int32)
-                core.move(core.pool, pool, n, live.ctypes.data, to.ctypes.data)
-            core.pool = pool
-        core.start(np.ascontiguousarray(new, np.int32), n)
-        self._tell(core)
-        return n
-
-    @staticmethod
-    def _renumber(host, pages: int):
-        """The pages of a table, ascending, and the table with them numbered 0, 1, .."""
-        used = np.zeros(pages, bool)
-        used[host[host >= 0]] = True
-        number = np.cumsum(used, dtype=np.int32) - 1
-        return np.flatnonzero(used).astype(np.int32), np.where(host >= 0, number[host], np.int32(-1))
-
-    @staticmethod
-    def _tell(core) -> None:
-        """The whole of the host's table to the device's."""
-        at = np.flatnonzero(core.host >= 0)
-        core.at[:len(at)], core.value[:len(at)] = at, core.host.reshape(-1)[at]
-        core.upload(len(at))
+    def _pool_size(self, num_pages) -> int:
+        """``num_pages``, by default as many as there are; refused if fewer than are in use here."""
+        if num_pages is None:
+            return self.num_pages
+        rows = self._core.host if self._whole else self._core.host[self._rows]
+        used = len(np.unique(rows[rows >= 0]))
+        if num_pages < max(used, 1):
+            raise ValueError(f"{used} pages are in use")
+        return num_pages
 
 
 def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = True, scale: float | None = None,
@@ -393,18 +366,19 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
     heads may be a multiple of the cache's.  ``rotary_base`` rotates the queries by
     RoPE at those positions.  A query that sees nothing gives zero.  Inference only.
     """
+    core, q = cache._core, query._data
     if query.ndim != 4:
         raise ValueError("attention expects [batch, heads, sequence, channels]")
-    if query.device != cache.device:
+    if query.device is not core.device and query.device != core.device:
         raise ValueError("attention tensors must be on the same device")
-    if query._data.dtype != cache.dtype:
+    if q.dtype != cache.dtype:
         raise TypeError("attention inputs must have the same floating-point dtype")
-    b, heads, steps, dim = query.shape
-    if b != cache.batch_size or dim != cache.head_dim:
+    b, heads, steps, dim = q.shape
+    if b != len(cache._rows) or dim != core.dim:
         raise ValueError("query shape does not match cache configuration")
-    if heads % cache.num_heads or min(query.shape) <= 0:
+    if not heads or not steps or heads % core.heads:
         raise ValueError("grouped-query attention requires enable_gqa and query heads divisible by KV heads")
-    if is_grad_enabled() and query.requires_grad:
+    if query.requires_grad and is_grad_enabled():
         raise RuntimeError("KVCache is inference-only; use no_grad() for differentiable inputs")
     multiplier = 1 / math.sqrt(dim) if scale is None else scale
     if not math.isfinite(multiplier):
@@ -413,15 +387,15 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
         raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
     import torch
 
-    core = cache._core
     lens, lens_at = cache._lens()
-    if heads // cache.num_heads * steps >= PROMPT_ROWS and dim <= 128 and lens.min() >= steps:
+    if heads // core.heads * steps >= PROMPT_ROWS and dim <= 128 and lens.min() >= steps:
         return _prompt(query, cache, lens, is_causal, multiplier, rotary_base)
-    q = _rows(query._data)
+    q = _rows(q)
     cos = sin = None
     if rotary_base is not None:
         cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, dim, q.dtype, q.device,
                                                       max(int(lens.max()), steps)))
+    core.sync()
     out = torch.empty((b, heads, steps, dim), dtype=q.dtype, device=q.device)
     lib, code = _lib.load(), cache._code
     nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, lens_at)

@@ -596,44 +596,53 @@ int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
 int tsattn_pages4_copy(const void *from, int64_t from_pages, void *to, int64_t to_pages, size_t page_bytes,
                        int32_t n, const int32_t *src, const int32_t *dst, void *stream);
 
-/* table[at[i]] = value[i] for n entries (host arrays; at[i] < entries, all different). */
-int tsattn_pages4_set(int32_t *table, int64_t entries, int32_t n, const int32_t *at, const int32_t *value,
-                      void *stream);
-
 /*
- * The host's side of a paged cache, in the caller's arrays: the next three calls change
- * them and launch nothing.  They give the page copies and the table entries that the
- * device needs (for tsattn_pages4_copy and tsattn_pages4_set, in this order, before
- * the next append) in arrays of the caller's.
+ * The host's side of a paged cache, in the caller's arrays.  The calls below change
+ * them and launch nothing, but for tsattn_pages4_sync, which brings the device's table
+ * up to date (before the next append, read or attention).  Page copies that they ask
+ * for, src[i] -> dst[i], are the caller's to launch (tsattn_pages4_copy) before the next
+ * append.  A new cache's table holds -1, its stack pages - 1, .., 0 and free == pages;
+ * lengths, refs, dirty and n_changed are 0.  `rows` of a call are n different rows.
  */
 typedef struct tsattn_pages4_host {
   int32_t rows, columns, page_size, pages;
-  int32_t *table;   /* [rows, columns] page numbers, -1: none (as many held as the length needs) */
+  int32_t *table;   /* [rows, columns] page numbers, as many as the row's length needs; then -1 */
   int32_t *lengths; /* [rows] cached positions */
   int32_t *refs;    /* [pages] rows that hold the page */
   int32_t *stack;   /* [pages] the free pages; the next one is stack[free - 1] */
-  int32_t free;
+  int32_t *changed; /* [rows * columns] the entries that the device's table lacks, n_changed of them */
+  uint8_t *dirty;   /* [rows * columns] 1: the entry is among them */
+  int32_t free, n_changed;
 } tsattn_pages4_host;
 
 /*
- * Pages for `steps` more positions of the n different rows.  A row that would append
- * into a page that others hold gets a copy: src[i] -> dst[i], counts[0] of them (room
- * for n).  at, value: counts[1] table entries (room for rows * columns).  Too few free
+ * Pages for `steps` more positions of the rows.  A row that would append into a page
+ * that others hold gets a copy of it: *copies of them (room for n).  Too few free
  * pages: TSATTN_ERR_INVALID, nothing changed.  The lengths stay: the caller adds
- * `steps` once the rows are there.
+ * `steps` once the positions are there.
  */
 int tsattn_pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
-                       int32_t *dst, int32_t *at, int32_t *value, int32_t *counts);
+                       int32_t *dst, int32_t *copies);
 
-/* The n different rows end at lengths[i] <= their own; pages wholly past them are free. */
+/* The rows end at lengths[i] <= their own; pages wholly past them are free. */
 int tsattn_pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *lengths);
 
+/* Row rows[i] takes over pages and length of rows[index[i]], for all i at once, and shares the pages. */
+int tsattn_pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *index);
+
 /*
- * Row rows[i] takes over pages and length of rows[index[i]], for all i at once, and
- * shares the pages with it.  at, value: *count table entries (room for n * columns).
+ * `to` (its sizes and arrays set, as many rows as n and columns as h) becomes a table
+ * of the rows: pages 0, 1, .. of another pool, *copies of them to copy there (room for
+ * h's pages).  More than `to` has: TSATTN_ERR_INVALID, nothing changed.
  */
-int tsattn_pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *index, int32_t *at,
-                          int32_t *value, int32_t *count);
+int tsattn_pages4_clone(const tsattn_pages4_host *h, int32_t n, const int32_t *rows, tsattn_pages4_host *to,
+                        int32_t *src, int32_t *dst, int32_t *copies);
+
+/* The pages in use become the first of the pool: *copies of them move (room for h's pages). */
+int tsattn_pages4_compact(tsattn_pages4_host *h, int32_t *src, int32_t *dst, int32_t *copies);
+
+/* The changed entries to the device's table [rows, columns]. */
+int tsattn_pages4_sync(tsattn_pages4_host *h, int32_t *table, void *stream);
 
 #ifdef __cplusplus
 }

@@ -40,7 +40,7 @@ class Memory:
         self.calls, self.fail = [], False
 
     def __getattr__(self, name):  # the calls that change the host's tables alone
-        assert name in ("tsattn_pages4_grow", "tsattn_pages4_cut", "tsattn_pages4_reorder"), name
+        assert name in ("tsattn_pages4_" + x for x in ("grow", "cut", "reorder", "clone", "compact")), name
         return getattr(REAL, name)
 
     def tsattn_pages4_page_bytes(self, heads, page, dim):
@@ -54,11 +54,16 @@ class Memory:
         self.calls.append(("copy", n))
         return 0
 
-    def tsattn_pages4_set(self, table, entries, n, at, value, stream):
-        at = _at(at, n, np.int32)
-        assert len(set(at)) == n
-        _at(table, entries, np.int32)[at] = _at(value, n, np.int32)
-        self.calls.append(("set", n))
+    def tsattn_pages4_sync(self, host, table, stream):
+        entries = host.rows * host.columns
+        at, want = _at(host.changed, entries, np.int32)[:host.n_changed], _at(host.table, entries, np.int32)
+        assert len(set(at)) == len(at) and _at(host.dirty, entries, np.uint8).sum() == len(at)
+        assert _at(host.dirty, entries, np.uint8)[at].all()
+        at = at[want[at] >= 0]
+        _at(table, entries, np.int32)[at] = want[at]
+        _at(host.dirty, entries, np.uint8)[:] = 0
+        host.n_changed = 0
+        self.calls.append(("sync", len(at)))
         return 0
 
     def tsattn_pages4_append(self, desc, dtype, n, steps, k, v, rows, lens, cos, sin, stream):
@@ -91,6 +96,7 @@ def memory():
 
 def _held(cache, row):
     core = cache._core
+    core.sync()
     pool = core.pool.numpy().view(np.float64).reshape(core.pool.shape[0], -1)
     table = core.table.numpy()
     n = core.lengths[row]
@@ -194,7 +200,7 @@ def test_beams_copy_one_page_each(memory):
         cache.append(_rows([[1.0]] * 8), _rows([[1.0]] * 8))
     assert not any(name == "copy" for name, _ in memory.calls)
     # positions 102 .. 127 touch no page but their own: nothing but the append is called
-    assert [x for x in memory.calls if x[0] == "set"] == []
+    assert {name for name, _ in memory.calls} == {"append"}
 
 
 def test_a_failed_append_leaves_the_lengths(memory):
@@ -368,8 +374,42 @@ def test_c_appends_attention_reads_copies_and_tables_refuse():
                 copy([0], [3], to=0x50000, pages=3), copy([3], [3]), copy([], [])):
         assert bad == _lib.ERR_INVALID
     assert copy([0], [1], size=1000) == _lib.ERR_UNSUPPORTED
-    set_ = lambda at: lib.tsattn_pages4_set(0x1000, 4, len(at), _ints(*at), _ints(*at), None)  # noqa: E731
-    for bad in (set_([4]), set_([-1]), set_([1, 1]), set_([])):
-        assert bad == _lib.ERR_INVALID
     assert lib.tsattn_pages4_page_bytes(8, 64, 128) == 8 * 2 * 36 * 128
     assert [lib.tsattn_pages4_page_bytes(*s) for s in ((8, 64, 96), (8, 33, 64), (0, 64, 64), (8, 16, 64))] == [0] * 4
+
+
+def test_c_tables_refuse():
+    lib = _lib.load()
+    arrays = {name: np.zeros(n, np.int32) for name, n in (("table", 6), ("lengths", 3), ("refs", 4), ("stack", 4),
+                                                          ("changed", 6), ("dirty", 2))}
+    h = _lib.Pages4Host()
+    h.rows, h.columns, h.page_size, h.pages, h.free = 3, 2, 32, 4, 4
+    arrays["table"][:], arrays["stack"][:] = -1, (3, 2, 1, 0)
+    for name, x in arrays.items():
+        setattr(h, name, x.ctypes.data)
+    src, dst, copies = _ints(*[0] * 4), _ints(*[0] * 4), _ints(0)
+    grow = lambda rows, steps, src=src: lib.tsattn_pages4_grow(h, len(rows), _ints(*rows), steps, src, dst, copies)  # noqa: E731
+    for bad in (grow([3], 1), grow([-1], 1), grow([0, 0], 1), grow([], 1), grow([0], 0), grow([0], 65),
+                grow([0], 1, None), lib.tsattn_pages4_grow(None, 1, _ints(0), 1, src, dst, copies),
+                grow([0, 1, 2], 64)):
+        assert bad == _lib.ERR_INVALID
+    assert "6 pages needed, 4 free" in _lib.last_error() and h.free == 4 and (arrays["table"] < 0).all()
+    assert grow([0, 2], 33) == 0 and h.free == 0 and h.n_changed == 4
+    arrays["lengths"][:] = (33, 0, 33)
+    cut = lambda rows, lens: lib.tsattn_pages4_cut(h, len(rows), _ints(*rows), _ints(*lens))  # noqa: E731
+    assert [cut([0], [34]), cut([0], [-1]), cut([1], [1]), cut([0, 0], [1, 1])] == [_lib.ERR_INVALID] * 4
+    order = lambda index: lib.tsattn_pages4_reorder(h, len(index), _ints(0, 1, 2), _ints(*index))  # noqa: E731
+    assert [order([0, 1, 3]), order([-1, 0, 0])] == [_lib.ERR_INVALID] * 2
+    to = _lib.Pages4Host()
+    for name, _ in _lib.Pages4Host._fields_:
+        setattr(to, name, getattr(h, name))
+    clone = lambda n: lib.tsattn_pages4_clone(h, n, _ints(0, 1, 2), to, src, dst, copies)  # noqa: E731
+    assert clone(2) == _lib.ERR_INVALID and "columns" in _lib.last_error()
+    to.pages = 3
+    assert clone(3) == _lib.ERR_INVALID and "4 pages are in use" in _lib.last_error()
+    to.table = None
+    assert clone(3) == _lib.ERR_INVALID
+    assert lib.tsattn_pages4_sync(h, None, None) == _lib.ERR_INVALID
+    assert lib.tsattn_pages4_compact(h, src, None, copies) == _lib.ERR_INVALID
+    h.free = 5
+    assert lib.tsattn_pages4_compact(h, src, dst, copies) == _lib.ERR_INVALID
