@@ -22,29 +22,42 @@ constexpr float most_scale() {
   return std::is_same_v<T, f16> ? 10752.f : 1.3125f * 0x1p125f;
 }
 
-// Four consecutive table entries.
-template <typename T>
-__device__ __forceinline__ void load4(const T *p, T (&x)[4]) {
-  using V = std::conditional_t<sizeof(T) == 2, u32x2, u32x4>;
-  const V r = *reinterpret_cast<const V *>(p);
-  const T *e = reinterpret_cast<const T *>(&r);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = e[i];
-}
-
 // A group's scale from the largest magnitude's bits (compared as integers, in
-// which a NaN is the largest of all).
+// which a NaN is the largest of all).  The fp32 quotient m / 6 by the reciprocal, its
+// exact remainder and one correction (Markstein, "Computation of elementary functions
+// on the IBM RISC System/6000 processor", 1990: correctly rounded); where that
+// remainder would underflow, the scale is its least value either way.
 template <typename T>
 __device__ __forceinline__ float scale_of(uint32_t m) {
-  const float q = __builtin_bit_cast(float, m) / 6.f;
-  uint32_t u = __builtin_bit_cast(uint32_t, q);
+#pragma clang fp contract(off)
+  constexpr float r = 1.f / 6.f;
+  const float x = __builtin_bit_cast(float, m), q0 = x * r;
+  uint32_t u = __builtin_bit_cast(uint32_t, __builtin_fmaf(__builtin_fmaf(-q0, 6.f, x), r, q0));
   u = (u + 0x1FFFFu + ((u >> 18) & 1u)) & ~0x3FFFFu;  // 5 mantissa bits
   const float s = fminf(fmaxf(__builtin_bit_cast(float, u), 0x1p-27f), most_scale<T>());
   return m >= 0x7F800000u ? __builtin_nanf("") : s;
 }
 
+// The largest magnitude's bits of eight values.
+template <typename T>
+__device__ __forceinline__ uint32_t most_of(const u32x4 (&raw)[sizeof(T) / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, raw[i >> 2][i & 3] & 0x7FFFFFFFu);
+    return m;
+  } else {  // (16-bit integers order as the values do: pairs at a time)
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    auto two = [&](int i) { return __builtin_bit_cast(u16x2, raw[0][i] & 0x7FFF7FFFu); };
+    const u16x2 x = __builtin_elementwise_max(__builtin_elementwise_max(two(0), two(1)),
+                                              __builtin_elementwise_max(two(2), two(3)));
+    const uint16_t most = x[0] > x[1] ? x[0] : x[1];
+    return __builtin_bit_cast(uint32_t, static_cast<float>(__builtin_bit_cast(T, most)));
+  }
+}
+
 // Eight codes.  The quotient is x / s to within an ulp's rounding: x times the
-// reciprocal in two parts, rounded once, so it is exact where x / s is half way
+// reciprocal in two parts (45 bits), rounded once, so it is exact where x / s is half way
 // between two levels.  For 16-bit x no other quotient comes that near to such a point
 // (x has at most 11 significant bits, the point times s 9), so the conversion's
 // rounding (to nearest, ties to even, saturating) decides as the real quotient does.
@@ -53,7 +66,7 @@ __device__ __forceinline__ float scale_of(uint32_t m) {
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
 #pragma clang fp contract(off)
-  const float rc = 1.f / s, rl = __builtin_fmaf(-rc, s, 1.f) * rc;
+  const float rc = __builtin_amdgcn_rcpf(s), rl = __builtin_fmaf(-rc, s, 1.f) * rc;
   float q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -74,13 +87,10 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
   return w;
 }
 
-// Largest of four lanes c, c + 16, c + 32, c + 48.
-__device__ __forceinline__ uint32_t quad_row_umax(uint32_t x) {
-  uint32_t a = x, b = x;
-  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-  x = a = b = max(a, b);
-  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-  return max(a, b);
+// Largest of four neighbouring lanes.
+__device__ __forceinline__ uint32_t quad_umax(uint32_t x) {
+  x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0xB1, 0xF, 0xF, true)));
+  return max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x4E, 0xF, 0xF, true)));
 }
 
 // Keys' words <-> values' words.  Lane 4 g' + q (of any g) has, of channels 8 o .. + 7,
@@ -145,17 +155,21 @@ __device__ __forceinline__ void load_words(const char *from, int lane, uint32_t 
   }
 }
 
-// One wave quantises the new positions of one tile, head and side (keys or
-// values).  Lane (c, g) takes keys c and 16 + c and their channels 32 ks + 8 g .. + 7:
-// 16-byte loads of which four make a group, and the words of the keys' layout.
-// Values' words hold one channel of eight keys: a transpose in each quad of lanes, and
-// one trip through LDS to the lanes that store them.  A tile that is only partly new
-// keeps its other positions: keys' words belong to one position each, values' are
-// read, merged and written.
+// One wave quantises the new positions of one tile, head and side (keys or values).
+// A load takes whole rows, PPR lanes of 8 channels a row, so that four neighbouring
+// lanes make a group and the angles' loads take whole lines of their tables too (four
+// 64-byte pieces a row from the operand order's lanes: 44 us where this takes 38,
+// 4 x 8 heads x 8192 positions of D128 in bf16, rotated).  Codes and scales then cross
+// the wave through LDS into operand order; values' words, one channel of eight keys
+// each, take a transpose in each quad of lanes and a second trip.  A tile that is
+// only partly new keeps its other positions: keys' words belong to one position each,
+// values' are read, merged and written.
 template <typename T, int G>
 __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
   constexpr int D = 32 * G, W = 2 * G;
-  __shared__ __attribute__((aligned(16))) char lds[NW][16 * D];
+  constexpr int PPR = D / 8, KPI = 64 / PPR;  // pieces a row, rows a load
+  constexpr int QW = sizeof(T) / 2;           // 16-byte loads a piece
+  __shared__ __attribute__((aligned(16))) char lds[NW][18 * D];
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int unit = blockIdx.x * NW + wv;  // (tile, side, head), the tile fastest
@@ -168,42 +182,46 @@ __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
   if (h >= a.p.heads || first >= a.len) return;                   // (a whole wave; no barrier follows)
   const bool full = first >= 0 && first + kTile <= a.len;
   const View &v = values ? a.v : a.k;
-  const T *src = static_cast<const T *>(v.data) + b * v.s0 + h * v.s1 + 8 * g;
-  constexpr int QW = sizeof(T) / 2;  // 16-byte loads a piece
+  const int piece = lane % PPR, sub = lane / PPR;
+  const T *src = static_cast<const T *>(v.data) + b * v.s0 + h * v.s1 + 8 * piece;
   u32x4 raw[W][QW];
-  bool live[2];
+  int at[W];  // the new position of each load's row (not one: the nearest, in bounds)
 #pragma unroll
-  for (int kb = 0; kb < 2; ++kb) {
-    const int t = first + 16 * kb + c;
-    live[kb] = t >= 0 && t < a.len;
-    const int64_t at = live[kb] ? t : (first < 0 ? 0 : first);  // (else a new position's row: in bounds)
+  for (int w = 0; w < W; ++w) {
+    at[w] = min(max(first + KPI * w + sub, 0), a.len - 1);
 #pragma unroll
-    for (int ks = 0; ks < G; ++ks)
-#pragma unroll
-      for (int i = 0; i < QW; ++i) raw[kb * G + ks][i] = reinterpret_cast<const u32x4 *>(src + at * v.s2 + 32 * ks)[i];
+    for (int i = 0; i < QW; ++i) raw[w][i] = reinterpret_cast<const u32x4 *>(src + at[w] * v.s2)[i];
   }
   char *tp = tile4(a.p, row, tile, h);
   char *to = tp + (values ? 16 * D : 0);
-  uint16_t *sto = reinterpret_cast<uint16_t *>(tp + (values ? 34 : 32) * D);
+  char *sto = tp + (values ? 34 : 32) * D;
   if (a.cos && !values) {
+    // the angles' loads all before their first use (an empty statement holds them there)
+    constexpr int STEP = sizeof(T) == 2 ? W : G;  // rows at a time
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const int64_t at = live[kb] ? first + 16 * kb + c : (first < 0 ? 0 : first);
+    for (int w0 = 0; w0 < W; w0 += STEP) {
+      using Angles = std::conditional_t<sizeof(T) == 2, u32x2, u32x4>;
+      Angles cw[STEP], sw[STEP];
 #pragma unroll
-      for (int ks = 0; ks < G; ++ks) {
-        T cw[4], sw[4];
-        const int64_t e = (pos + at) * (D / 2) + 16 * ks + 4 * g;
-        load4<T>(static_cast<const T *>(a.cos) + e, cw);
-        load4<T>(static_cast<const T *>(a.sin) + e, sw);
-        u32x4(&x)[QW] = raw[kb * G + ks];
+      for (int j = 0; j < STEP; ++j) {
+        const int64_t e = (static_cast<int64_t>(pos) + at[w0 + j]) * (D / 2) + 4 * piece;
+        cw[j] = *reinterpret_cast<const Angles *>(static_cast<const T *>(a.cos) + e);
+        sw[j] = *reinterpret_cast<const Angles *>(static_cast<const T *>(a.sin) + e);
+      }
+#pragma unroll
+      for (int j = 0; j < STEP; ++j) asm volatile("" : "+v"(cw[j]), "+v"(sw[j]));
+#pragma unroll
+      for (int j = 0; j < STEP; ++j) {
+        u32x4(&x)[QW] = raw[w0 + j];
+        const T *cs = reinterpret_cast<const T *>(&cw[j]), *sn = reinterpret_cast<const T *>(&sw[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (sizeof(T) == 2) {
-            x[0][i] = rotate_word<T>(x[0][i], cw[i], sw[i], false);
+            x[0][i] = rotate_word<T>(x[0][i], cs[i], sn[i], false);
           } else {
             const uint32_t u0 = x[i >> 1][2 * (i & 1)], u1 = x[i >> 1][2 * (i & 1) + 1];
             T x0 = __builtin_bit_cast(T, u0), x1 = __builtin_bit_cast(T, u1);
-            rotate_pair(x0, x1, cw[i], sw[i], false);
+            rotate_pair(x0, x1, cs[i], sn[i], false);
             x[i >> 1][2 * (i & 1)] = __builtin_bit_cast(uint32_t, x0);
             x[i >> 1][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, x1);
           }
@@ -211,7 +229,8 @@ __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
       }
     }
   }
-  uint32_t word[W], sc[W];
+  char *mine = lds[wv];
+  uint16_t *scales = reinterpret_cast<uint16_t *>(mine + 16 * D);
 #pragma unroll
   for (int w = 0; w < W; ++w) {
     float x[8];
@@ -221,35 +240,41 @@ __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
 #pragma unroll
       for (int j = 0; j < 8 / QW; ++j) x[i * (8 / QW) + j] = static_cast<float>(e[j]);
     }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
-    const float s = scale_of<T>(quad_row_umax(m));
-    sc[w] = __builtin_bit_cast(uint32_t, s) >> 16;
-    word[w] = codes_of<T>(x, s == s ? s : 1.f);
+    const float s = scale_of<T>(quad_umax(most_of<T>(raw[w])));
+    const int key = KPI * w + sub;
+    *reinterpret_cast<uint32_t *>(mine + word4<G>((key >> 4) * G + (piece >> 2), 16 * (piece & 3) + (key & 15))) =
+        codes_of<T>(x, s == s ? s : 1.f);
+    if ((piece & 3) == 0)
+      scales[scale4<G>(key, piece >> 2)] = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, s) >> 16);
   }
-  // scales: lane g stores those of words g, g + 4, ..
+  wait_lgkm0();  // (own wave's writes)
+  __builtin_amdgcn_sched_barrier(0);
+  uint32_t word[W];
+  load_words<G>(mine, lane, word);
+  if (full) {
+    if (lane < 4 * G) reinterpret_cast<u32x4 *>(sto)[lane] = reinterpret_cast<const u32x4 *>(scales)[lane];
+  } else {
 #pragma unroll
-  for (int w0 = 0; w0 < W; w0 += 4) {
-    uint32_t s = sc[w0];
-#pragma unroll
-    for (int i = 1; i < 4; ++i)
-      if (w0 + i < W && g == i) s = sc[w0 + i];
-    const int w = w0 + g, kb = w / G, ks = w - kb * G;
-    if (w < W && (kb ? live[1] : live[0])) sto[scale4<G>(16 * kb + c, ks)] = static_cast<uint16_t>(s);
+    for (int e0 = 0; e0 < 32 * G; e0 += 64) {
+      const int e = e0 + lane, t = first + 16 * ((e >> 2) & 1) + 4 * (e / (8 * G)) + (e & 3);
+      if (e < 32 * G && t >= 0 && t < a.len) reinterpret_cast<uint16_t *>(sto)[e] = scales[e];
+    }
   }
   if (!values) {
     if (full) {
       store_words<G>(to, lane, word);
     } else {
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-        if (live[w / G]) *reinterpret_cast<uint32_t *>(to + word4<G>(w, lane)) = word[w];
+      for (int w = 0; w < W; ++w) {
+        const int t = first + 16 * (w / G) + c;
+        if (t >= 0 && t < a.len) *reinterpret_cast<uint32_t *>(to + word4<G>(w, lane)) = word[w];
+      }
     }
     return;
   }
-  char *mine = lds[wv];
   const Transpose tr(lane);
+  wait_lgkm0();  // (read before the next writes)
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int ks = 0; ks < G; ++ks) {
     uint32_t x = word[ks], y = word[G + ks];
@@ -273,8 +298,8 @@ __global__ __launch_bounds__(NT) void append_kernel(RowArgs a) {
   if (keep != 0xFFFFFFFFu)
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      uint32_t *at = reinterpret_cast<uint32_t *>(to + word4<G>(w, lane));
-      *at = (*at & keep) | (word[w] & ~keep);
+      uint32_t *old = reinterpret_cast<uint32_t *>(to + word4<G>(w, lane));
+      *old = (*old & keep) | (word[w] & ~keep);
     }
 }
 
