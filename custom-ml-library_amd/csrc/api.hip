@@ -575,7 +575,7 @@ int check_pages4(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t len, 
     if (rows[i] < 0 || rows[i] >= p->table_rows)
       return fail(TSATTN_ERR_INVALID, "paged cache: sequence %d has table row %d of %lld", i, rows[i],
                   static_cast<long long>(p->table_rows));
-    if (lens[i] < 0 || lens[i] > room || lens[i] > INT32_MAX / 4)
+    if (lens[i] < 0 || lens[i] > room || lens[i] > tsattn::kLongest)
       return fail(TSATTN_ERR_INVALID, "paged cache: sequence %d has %d positions in a table of %lld", i, lens[i],
                   static_cast<long long>(room));
   }
@@ -1062,7 +1062,7 @@ int tsattn_pages4_append(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
     return rc;
   for (int32_t i = 0; i < n; ++i)
     if (static_cast<int64_t>(lens[i]) + len > p->table_stride * p->page_size ||
-        static_cast<int64_t>(lens[i]) + len > INT32_MAX / 4)
+        static_cast<int64_t>(lens[i]) + len > tsattn::kLongest)
       return fail(TSATTN_ERR_INVALID, "paged cache: %d positions after %d of sequence %d exceed its table", len,
                   lens[i], i);
   char *seen = static_cast<char *>(calloc(static_cast<size_t>(p->table_rows), 1));
@@ -1088,7 +1088,7 @@ int tsattn_pages4_read(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t
   if (rc || (rc = check_rows4(k, dtype, "key output")) || (rc = check_rows4(v, dtype, "value output"))) return rc;
   if (!first) return fail(TSATTN_ERR_INVALID, "paged cache: first positions are NULL");
   for (int32_t i = 0; i < n; ++i)
-    if (first[i] < 0 || static_cast<int64_t>(first[i]) + len > INT32_MAX / 4)
+    if (first[i] < 0 || static_cast<int64_t>(first[i]) + len > tsattn::kLongest)
       return fail(TSATTN_ERR_INVALID, "paged cache: sequence %d is read from position %d", i, first[i]);
   for (int32_t i0 = 0; i0 < n && !rc; i0 += tsattn::kSeqs) {
     tsattn::Seqs s;

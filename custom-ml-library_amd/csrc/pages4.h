@@ -33,6 +33,7 @@
 namespace tsattn {
 
 constexpr int kTile = 32;     // positions a tile
+constexpr int kLongest = 1 << 27;  // positions a sequence: splits of 4096 stay within a grid's 65535
 constexpr int kSeqs = 256;    // sequences a launch: their numbers travel by value
 constexpr int kMoves = 480;   // pages, or table entries, a launch (under 4 KiB of arguments)
 

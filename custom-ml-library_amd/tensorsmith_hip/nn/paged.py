@@ -13,7 +13,9 @@ head (``tsattn_pages4_attend``); for a prompt's many rows the pages are
 dequantised once and attended on the 16-bit or fp32 matrix cores.
 
 Page tables and reference counts are the host's; lengths travel with each launch.
-Calls captured into a HIP graph replay the positions they were captured at.
+Calls captured into a HIP graph replay the positions, and the pages, that they were
+captured at, so a replay is for as long as its rows keep both; a call that takes or
+copies a page is refused there.
 """
 
 from __future__ import annotations
@@ -28,13 +30,22 @@ from ..device import launch
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
 from .attention import _dtype_code, _rope_rows, rope_tables, scaled_dot_product_attention
 
-# Query rows per KV head from which dequantising the pages once and attending on
-# the matrix cores is the faster way.
-PROMPT_ROWS = 128
+def _reads_codes(rows: int, heads: int, dim: int, wide: bool, lens) -> bool:
+    """Whether attention reads the codes themselves: ``rows`` query rows per KV head over sequences
+    of ``lens``.  Its time grows with rows and positions; dequantising once and attending on the
+    matrix cores costs mostly host time, per run of rows of one length, but fp32's kernel waits on
+    every key of one row block.  Microseconds, codes / dequantised, 8 KV heads of D128 over 8000 positions: bf16 64
+    rows 32 / 53, 128 51 / 54, 256 80 / 53, 1024 247 / 60; fp32 1024 rows 420 / 1125; over 500
+    positions bf16 1024 rows 25 / 49.  2 heads of D64 over 8000: 1024 rows 34 / 53."""
+    size = (dim / 128) ** 1.5
+    codes = 12 + (6.4e-6 if wide else 4e-6) * size * rows * heads * int(lens.sum())
+    whole = 50 * len(_runs(lens)) + (0.14 * (dim / 128) ** 3 * int(lens.max()) if wide else 0)
+    return codes <= whole
 
 
-def _ints(x):
-    return np.ascontiguousarray(x, np.int32)
+def _runs(lens) -> list:
+    """Ends of the runs of rows of one length."""
+    return [*(np.flatnonzero(lens[1:] != lens[:-1]) + 1).tolist(), len(lens)]
 
 
 def _rows(t):
@@ -104,6 +115,7 @@ class _Pages:
     def sync(self) -> None:
         """The device's table up to date."""
         if self.tables.n_changed:
+            self._eager()
             _lib.check(launch(self.device, _lib.load().tsattn_pages4_sync, self.tables, self.desc.table), "page table")
 
     def move(self, source, target) -> None:
@@ -113,18 +125,32 @@ class _Pages:
             _lib.check(launch(self.device, _lib.load().tsattn_pages4_copy, source.data_ptr(), source.shape[0],
                               target.data_ptr(), target.shape[0], self.page_bytes, n, *self.out[:2]), "page copy")
 
+    def _eager(self, rows=None, steps: int = 0) -> None:
+        """Refuses page changes under capture: a captured call's pages would be the host's at once and
+        the device's with each replay.  With ``rows``: only if they need other pages for ``steps``."""
+        import torch
+
+        if not torch.cuda.is_current_stream_capturing():
+            return
+        if rows is not None and not self.tables.n_changed:
+            lens = self.lengths[rows]
+            page = self.host[rows, lens // self.page_size % self.host.shape[1]]
+            part = lens % self.page_size
+            if ((part > 0) & (part + steps <= self.page_size) & (self.refs[np.maximum(page, 0)] == 1)).all():
+                return
+        raise RuntimeError("a paged cache's pages cannot change while a graph is captured")
+
     def grow(self, n: int, rows: int, steps: int) -> None:
         """Pages of their own for the next ``steps`` positions of the ``n`` rows (an address)."""
         _lib.check(_lib.load().tsattn_pages4_grow(self.tables, n, rows, steps, *self.out), "page table")
 
-    def cut(self, rows, lengths) -> None:
-        """``rows`` end at ``lengths``; pages wholly past them are given back."""
-        rows, lengths = _ints(rows), _ints(lengths)
-        _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows.ctypes.data, lengths.ctypes.data),
-                   "page table")
+    def cut(self, rows, rows_at: int, lengths) -> None:
+        """``rows`` (at an address) end at ``lengths``; pages wholly past them are given back."""
+        _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows_at, lengths.ctypes.data), "page table")
 
     def clone(self, rows, num_pages: int) -> "_Pages":
         """The rows with pages of their own, in a pool of ``num_pages``."""
+        self._eager()
         other = _Pages(len(rows), self.heads, self.dim, self.host.shape[1], self.page_size, num_pages, self.device)
         _lib.check(_lib.load().tsattn_pages4_clone(self.tables, len(rows), rows.ctypes.data, other.tables, *self.out),
                    "page table")
@@ -222,6 +248,7 @@ class PagedKVCache:
                 raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
             cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
         k, v = (_rows(t._data.to(self.dtype)) for t in (key, value))
+        core._eager(self._rows, steps)
         core.grow(len(lens), self._rows_at, steps)
         try:
             core.move(core.pool, core.pool)
@@ -230,7 +257,7 @@ class PagedKVCache:
                               _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
         except BaseException:
             core.lengths[self._rows] += steps  # (the new pages go back)
-            core.cut(self._rows, core.lengths[self._rows] - steps)
+            core.cut(self._rows, self._rows_at, core.lengths[self._rows] - np.int32(steps))
             raise
         if self._whole:
             core.lengths += steps
@@ -247,7 +274,7 @@ class PagedKVCache:
     def _check(self, key: Tensor, value: Tensor) -> None:
         """``KVCache``'s refusals, in its order."""
         dev = self._core.device
-        if any(x.device is not dev and x.device != dev for x in (key, value)):
+        if (key.device is not dev and key.device != dev) or (value.device is not dev and value.device != dev):
             raise ValueError("cache and key/value tensors must be on the same device")
         if (key.requires_grad or value.requires_grad) and is_grad_enabled():
             raise RuntimeError("KVCache is inference-only; use no_grad() for differentiable inputs")
@@ -290,23 +317,24 @@ class PagedKVCache:
         return view
 
     def _indices(self, indices, shape):
-        host = np.asarray(to_numpy(indices._data if isinstance(indices, Tensor) else indices))
+        host = np.asarray(to_numpy(indices._data) if isinstance(indices, Tensor) else indices)
         if host.ndim != 1 or (shape is not None and host.shape != shape) or (host.size and host.dtype.kind not in "iu"):
             raise ValueError("beam indices must be one integer per cache batch row" if shape is not None
                              else "row indices must be integers")
-        if host.size and ((host < 0).any() or (host >= self.batch_size).any()):
+        index = host.astype(np.int32)
+        if shape is None and index.size and (index.min() < 0 or index.max() >= len(self._rows)) or (index != host).any():
             raise ValueError("beam index out of range" if shape is not None else "row index out of range")
-        return host.astype(np.int32)
+        return index  # (a beam index's range is checked with the tables)
 
     def reset(self) -> None:
         """Every row empty, its pages given back."""
-        self._core.cut(self._rows, np.zeros_like(self._rows))
+        self._core.cut(self._rows, self._rows_at, np.zeros_like(self._rows))
 
     def free(self, indices) -> None:
         """These rows empty, their pages given back."""
-        index = np.unique(self._indices(indices, None))
-        if len(index):
-            self._core.cut(self._rows[index], np.zeros_like(index))
+        rows = self._rows[np.unique(self._indices(indices, None))]
+        if len(rows):
+            self._core.cut(rows, rows.ctypes.data, np.zeros_like(rows))
 
     def truncate(self, length) -> None:
         """Cut every row to ``length`` positions, or to a length of its own (a sequence of them);
@@ -314,9 +342,10 @@ class PagedKVCache:
         want = np.asarray(length)
         if want.dtype.kind not in "iu" or want.shape not in ((), self._rows.shape):
             raise ValueError("truncate takes one integer length, or one per row")
-        if want.max() >= 2**31 or want.min() < -(2**31):
+        lens = want.astype(np.int32)
+        if (lens != want).any():
             raise ValueError("truncate length must be between zero and the current length")
-        self._core.cut(self._rows, want if want.shape else np.full_like(self._rows, want))
+        self._core.cut(self._rows, self._rows_at, lens if lens.shape else np.full_like(self._rows, lens))
 
     def reorder(self, indices) -> None:
         """Row i becomes row ``indices[i]``, sharing its pages: no keys or values move.  Rows that
@@ -339,6 +368,7 @@ class PagedKVCache:
         size (smaller or larger); returns how many are in use."""
         core = self._core
         if num_pages is None:
+            core._eager()
             _lib.check(_lib.load().tsattn_pages4_compact(core.tables, *core.out), "page table")
             core.move(core.pool, core.pool)
         else:
@@ -388,7 +418,9 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
     import torch
 
     lens, lens_at = cache._lens()
-    if heads // core.heads * steps >= PROMPT_ROWS and dim <= 128 and lens.min() >= steps:
+    rows = heads // core.heads * steps
+    if (rows > 32 and dim <= 128 and lens.min() >= steps
+            and not _reads_codes(rows, core.heads, dim, q.dtype == torch.float32, lens)):
         return _prompt(query, cache, lens, is_causal, multiplier, rotary_base)
     q = _rows(q)
     cos = sin = None
@@ -407,8 +439,8 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
 
 
 def _prompt(query: Tensor, cache: PagedKVCache, lens, is_causal: bool, scale: float, rotary_base) -> Tensor:
-    """Many query rows: the values dequantised once, then the attention of arrays; rows of
-    unequal length one after the other."""
+    """Many query rows: the values dequantised once, then the attention of arrays; runs of rows of
+    one length one after the other."""
     import torch
 
     def attend(q, held, n):
@@ -419,9 +451,11 @@ def _prompt(query: Tensor, cache: PagedKVCache, lens, is_causal: bool, scale: fl
             Tensor(q, device=cache.device), k, v, None, 0.0, is_causal, scale=scale,
             causal_offset=n - q.shape[2] if is_causal else 0, enable_gqa=q.shape[1] != held.num_heads)._data
 
+    q, parts, first = query._data, [], 0
     with torch.cuda.device(cache.device.index):  # (attention launches on the current device)
-        if lens.min() == lens.max():
-            out = attend(query._data, cache, int(lens[0]))
-        else:
-            out = torch.cat([attend(query._data[i:i + 1], cache.rows([i]), int(n)) for i, n in enumerate(lens)])
+        for stop in _runs(lens):
+            held = cache if stop - first == len(lens) else cache.rows(range(first, stop))
+            parts.append(attend(q[first:stop], held, int(lens[first])))
+            first = stop
+    out = parts[0] if len(parts) == 1 else torch.cat(parts)
     return Tensor._from_op(out, (query,), None, "paged_attention")

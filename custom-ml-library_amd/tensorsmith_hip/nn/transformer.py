@@ -182,6 +182,8 @@ class MultiHeadAttention(Module):
     def new_cache(self, batch_size: int, max_seq_len: int, *, dtype="float32",
                   quantized: bool = False, paged: bool = False) -> KVCache | PagedKVCache:
         if paged:
+            if quantized:
+                raise ValueError("a paged cache is in 4 bits: quantized does not apply")
             return PagedKVCache(batch_size, self.num_kv_heads, self.head_dim, max_seq_len,
                                 device=self.q_proj.weight.device, dtype=dtype)
         return KVCache(batch_size, self.num_kv_heads, self.head_dim, max_seq_len,
@@ -474,7 +476,7 @@ class TransformerLM(Module):
             raise ValueError("cache capacity must fit the model context")
         if paged:
             return [block.attention.new_cache(batch_size, capacity, dtype=self.token_embedding.weight.dtype,
-                                              paged=True) for block in self.blocks]
+                                              quantized=quantized, paged=True) for block in self.blocks]
         return [
             KVCache(batch_size, block.attention.num_kv_heads, block.attention.head_dim, capacity,
                     device=self.token_embedding.weight.device,

@@ -12,7 +12,9 @@ rounds each probability to 16 bits once more.
 
 from __future__ import annotations
 
+import importlib
 import math
+from unittest.mock import patch
 
 import pytest
 
@@ -25,6 +27,7 @@ if not torch.cuda.is_available():  # pragma: no cover - CPU containers
 import tensorsmith_hip as ts  # noqa: E402
 from tensorsmith_hip import nn  # noqa: E402
 
+P = importlib.import_module("tensorsmith_hip.nn.paged")
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 HALF = {F16: 2.0**-11, BF16: 2.0**-8, F32: 2.0**-24}
 LEVELS = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
@@ -250,7 +253,7 @@ def test_any_scale(scale, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("d,heads,hkv,steps,lens", [(64, 4, 2, 70, (70, 70)), (128, 2, 2, 150, (333, 333)),
-                                                    (32, 8, 2, 40, (41, 90, 40)), (128, 8, 1, 33, (50, 700)),
+                                                    (32, 8, 2, 40, (41, 90, 90, 40)), (128, 8, 1, 33, (50, 700)),
                                                     (128, 8, 1, 33, (20, 100)), (256, 2, 1, 100, (130, 250))])
 def test_prompts_match_float64(d, heads, hkv, steps, lens, dtype):
     """Chunks of prompts: rows of one length, of several, and with fewer positions than queries."""
@@ -262,8 +265,10 @@ def test_prompts_match_float64(d, heads, hkv, steps, lens, dtype):
     cache.truncate(lens)
     q = draw(gen, b, heads, steps, d, dtype=dtype)
     for causal in (True, False):
-        want, tol = reference(q, stored(k), stored(v), lens, causal, 1 / math.sqrt(d), True)
-        check(nn.paged_attention(wrap(q), cache, is_causal=causal)._data, want, tol, dtype)
+        for codes in (True, False):  # from the codes, and from values dequantised once
+            want, tol = reference(q, stored(k), stored(v), lens, causal, 1 / math.sqrt(d), not codes)
+            with patch.object(P, "_reads_codes", lambda *a: codes):
+                check(nn.paged_attention(wrap(q), cache, is_causal=causal)._data, want, tol, dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -277,7 +282,10 @@ def test_queries_rotate_at_their_positions(d, heads, steps, dtype):
     cache.truncate(lens)
     q = draw(gen, 2, heads, steps, d, dtype=dtype)
     turned = torch.cat([nn.rotary_embedding(wrap(q[i:i + 1]), n - steps, base=500.0)._data for i, n in enumerate(lens)])
-    assert torch.equal(nn.paged_attention(wrap(q), cache, rotary_base=500.0)._data, nn.paged_attention(wrap(turned), cache)._data)
+    for codes in (True, False):
+        with patch.object(P, "_reads_codes", lambda *a: codes):
+            got = nn.paged_attention(wrap(q), cache, rotary_base=500.0)._data
+            assert torch.equal(got, nn.paged_attention(wrap(turned), cache)._data)
 
 
 def test_many_sequences_and_far_pages():
@@ -378,8 +386,17 @@ def test_on_another_stream_and_captured():
         lens = [n - 1 for n in cache.lengths]
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
+    full = nn.PagedKVCache(3, 2, 64, 128, device="hip", dtype=BF16)
+    full.append(*(wrap(x[:, :, :64].contiguous()) for x in (k, v)))
+    shared = full.copy()
+    shared.truncate(40)
+    shared.reorder([0, 0, 1])
+    assert all(torch.equal(x, y[[0, 0, 1], :, :40]) for x, y in zip(held(shared), held(full)))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
+        for call in (lambda: full.append(wrap(kt), wrap(vt)), full.copy, full.compact, lambda: shared.append(wrap(kt), wrap(vt))):
+            with pytest.raises(RuntimeError, match="cannot change while a graph"):
+                call()
         core = cache._core
         core.lengths -= 1  # (the captured append writes where the eager one did)
         cache.append(wrap(kt), wrap(vt), rotary_base=100.0)
@@ -393,6 +410,10 @@ def test_on_another_stream_and_captured():
         cache.append(wrap(new[i % 3]), wrap(new[(i + 1) % 3]), rotary_base=100.0)
         assert torch.equal(got, nn.paged_attention(wrap((q * (i + 1))), cache, rotary_base=100.0)._data), i
         assert all(torch.equal(x, y._data) for x, y in zip(keys, cache.get(last=1)))
+    assert full.lengths == (64, 64, 64) and full.pages_in_use == 3  # the refused call left nothing
+    assert all(torch.equal(x, y[[0, 0, 1], :, :40]) for x, y in zip(held(shared), held(full)))
+    full.append(wrap(kt), wrap(vt))
+    assert same(held(full)[0][:, :, 64:], stored(kt), BF16) and same(held(full)[1][:, :, :64], stored(v[:, :, :64]), BF16)
 
 
 # -- layers and models -------------------------------------------------------------

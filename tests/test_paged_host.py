@@ -87,6 +87,7 @@ def memory():
                         patch.object(D, "is_available", lambda value: True),
                         patch.object(D, "current_stream", lambda dev: 0),
                         patch.object(torch.cuda, "current_device", lambda: 0),
+                        patch.object(torch.cuda, "is_current_stream_capturing", lambda: False),
                         patch.object(torch.cuda, "device", lambda index: nullcontext()),
                         patch.object(_lib, "load", lambda: memory),
                         patch.object(_lib, "last_error", lambda: REAL.tsattn_last_error().decode())):
@@ -276,10 +277,25 @@ def test_refusals(memory):
         with pytest.raises(ValueError):
             nn.paged_attention(q, cache, **kw)
     attention = nn.MultiHeadAttention(64, 2, device="hip").eval()
+    with pytest.raises(ValueError, match="4 bits"):
+        attention.new_cache(2, 100, quantized=True, paged=True)
     ragged = attention.new_cache(2, 100, paged=True)
     ragged.rows([1]).append(x(1, 2, 3, 32), x(1, 2, 3, 32))
     with ts.no_grad(), pytest.raises(ValueError, match="one length"):
         attention(x(2, 1, 64), cache=ragged, attn_mask=ts.Tensor(torch.ones(2, 1, 1, 4, dtype=torch.bool), device="hip"))
+
+
+def test_the_prompt_rule():
+    """Both sides of each measured crossing, runs of equal rows counted once."""
+    lens = lambda *n: np.array(n, np.int32)  # noqa: E731
+    for rows, heads, dim, wide, n, codes in (
+            (64, 8, 128, False, lens(8000), True), (256, 8, 128, False, lens(8000), False),
+            (1024, 8, 128, False, lens(500), True), (1024, 8, 128, False, lens(2000), False),
+            (1024, 8, 128, True, lens(8000), True), (1024, 2, 64, False, lens(8000), True),
+            (128, 8, 128, False, lens(8000, 8000, 8000), False), (128, 8, 128, False, lens(8000, 7000, 8000), True),
+            (4096, 8, 128, True, lens(32000), False), (32, 4, 64, False, lens(0), True)):
+        assert P._reads_codes(rows, heads, dim, wide, n) is codes, (rows, heads, dim, wide, n)
+    assert P._runs(lens(3, 3, 5, 3)) == [2, 3, 4] and P._runs(lens(7)) == [1]
 
 
 # -- the C entry points: every refusal comes before a launch --------------------------
