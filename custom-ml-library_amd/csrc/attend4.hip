@@ -25,8 +25,9 @@
 namespace tsattn {
 namespace {
 
-// Tiles a wave at most (of four waves; its lanes hold their page numbers).
-constexpr int kSplitTiles = 32;
+// Positions a split at most: 32 tiles a wave of four, whose lanes hold their page numbers.
+constexpr int kMostSplit = 4096;
+static_assert(kMostSplit / kTile / 4 <= 64, "one lane a tile");
 
 template <typename T>
 constexpr int q_parts() { return std::is_same_v<T, bf16> ? 1 : std::is_same_v<T, f16> ? 2 : 3; }
@@ -117,7 +118,6 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
     for (int i = 0; i < QW; ++i) raw[nb][i] = reinterpret_cast<const u32x4 *>(qp)[i];
   }
   // the wave's page numbers, lane t's for its tile t: one load, and none in the loop
-  // (kSplitTiles of a wave at most)
   const int ids = a.p.table[trow * a.p.stride + ((tile0 + NWV * min(lane, max(mine, 1) - 1)) >> a.p.per_page)];
   auto load = [&](Held<G> &x, int t) __attribute__((always_inline)) {
     using C = typename Held<G>::Chunk;
@@ -368,11 +368,16 @@ int column_blocks(int dtype, int dim, int rows) {
 
 }  // namespace
 
-// Few workgroups are worth eight waves each, which take a CU by themselves; many
-// run four, two or three workgroups a CU.  The split is the one that a model of
-// the kernel's time likes best: every round of workgroups that fit the chip costs
-// its prologue and merge and its waves' tiles, a tile the larger of its own
-// latency and its share of the memory's rate; a split, the second kernel.
+// Waves a workgroup (four, two or three workgroups a CU; or eight, which take one by
+// themselves) and splits: those that a model of the time likes best.  In us: a
+// workgroup's prologue and merge 2.2; a tile of a wave the largest of its own latency
+// (by its MFMAs; fp32 D128 1.5, bf16 D256 2.0, bf16 D128 1.0 with one column block
+// and 2.2 with two), of the issue slots of the waves beside it and of the memory's
+// rate; where the workgroups do not fit the chip at once, their sum over it and half a
+// workgroup's end; the second kernel 3.  Measured, what it picks and the other end:
+// 16 sequences of 8 KV heads up to 3000 positions, 8 rows of f16 D128: 2 splits 21.6,
+// one 31.1; 3 of one head over 1500, fp32 D128: 12 splits 7.2, one 13.1; 64 of 8
+// heads over 1025, 4 rows of f16 D128: one split 18.8, three 24.
 void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
   int64_t total = 0;
   int longest = 1;
@@ -383,21 +388,40 @@ void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
   const int dim = a->p.dim, nb = column_blocks(dtype, dim, a->rows), per = 512 / dim * nb;
   a->blocks = (a->rows + per - 1) / per;
   const double groups = static_cast<double>(a->p.heads) * a->blocks;
+  const int parts = dtype == TSATTN_F32 ? 6 : dtype == TSATTN_F16 ? 4 : 3;
+  const double latency = 0.2 + 0.034 * nb * (dim / 16) * parts;
+  const int fewest = (longest + kMostSplit - 1) / kMostSplit;
   double best = 1e30;
   for (int waves = 4; waves <= 8; waves += 4) {
-    if (waves == 8 && (dtype == TSATTN_F32 && dim == 256)) continue;  // (more registers than eight waves have)
+    if (waves == 8 && dtype == TSATTN_F32 && dim == 256) continue;  // (more registers than eight waves have)
     const double slots = waves == 8 ? 256. : nb == 2 || dim == 256 ? 512. : 768.;
-    for (int split = 256; split <= kSplitTiles * kTile * 4; split *= 2) {
-      const int n = (longest + split - 1) / split;
-      const int even = ((longest + n - 1) / n + kTile * waves - 1) / (kTile * waves) * (kTile * waves);
-      if (even > kSplitTiles * kTile * 4) continue;
-      const double wgs = groups * (n == 1 ? a->n : static_cast<double>(total) / even + 0.5 * a->n);
-      const double tiles = static_cast<double>(even) / (kTile * waves);
+    const int unit = kTile * waves;
+    for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      const int n = k > fewest ? k : fewest;
+      int even = ((longest + n - 1) / n + unit - 1) / unit * unit;
+      if (n > 1 && even < kMostSplit) even = (even / 128 | 1) * 128;
+      if (k > 1 && (k <= fewest || even < 128 || n > longest)) continue;
+      int live = 0;
+      if (total == static_cast<int64_t>(a->n) * longest) {
+        live = a->n * ((longest + even - 1) / even);
+      } else {
+        const float per_split = 1.f / even;
+        for (int i = 0; i < a->n; ++i) live += 1 + static_cast<int>(static_cast<float>(lens[i] - 1) * per_split);
+      }
+      const double wgs = groups * live;
+      const double tiles = static_cast<double>(even < longest ? even : longest) / unit;
       const double busy = (wgs < slots ? wgs : slots) * waves;
-      const double rate = busy * 36 * dim / 6.2e6;  // us a tile at 6.2 TB/s
-      const double tile = rate > 0.8 ? rate : 0.8;
-      const double rounds = wgs <= slots ? 1. : wgs / slots + 0.3;
-      const double cost = rounds * (2.5 + tiles * tile) + (n > 1 ? 4.5 : 0.);
+      const double rate = busy * 36 * dim / 6.2e6, issue = 0.65 * latency * busy / 1024;
+      const double alone = latency > issue ? latency : issue, start = waves == 8 ? 2.8 : 2.2;
+      const double one = start + (tiles > 1 ? tiles : 1) * (alone > rate ? alone : rate);
+      double cost = one;
+      if (wgs > 3 * slots) {
+        const double sum = groups * total / unit, most = wgs * start + sum * alone;
+        cost = ((most > sum * rate ? most : sum * rate) + 0.5 * wgs * start) / slots + 0.25 * one;
+      } else if (wgs > slots) {
+        cost = one * (wgs > 2 * slots ? 2.5 : 1.8);
+      }
+      if (n > 1) cost += 2.5 + 0.5 * ((n + 15) / 16) + 8. * a->n * a->p.heads * n * a->rows * (dim + 2) / 6.2e6;
       if (cost < best) {
         best = cost;
         a->waves = waves, a->split = even, a->splits = (longest + even - 1) / even;
