@@ -639,7 +639,7 @@ size_t plan4(tsattn::Attend4 *a, int32_t dtype, int32_t n, int32_t i0, const int
 
 // The host's side of a paged cache, and n different rows of it.
 int check_host4(const tsattn_pages4_host *h) {
-  if (!h || !h->table || !h->lengths || !h->refs || !h->stack || !h->changed || !h->dirty)
+  if (!h || !h->table || !h->lengths || !h->refs || !h->stack || !h->shown || !h->changed || !h->dirty)
     return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
   if (h->rows <= 0 || h->columns <= 0 || h->page_size <= 0 || h->pages <= 0 || h->free < 0 || h->free > h->pages ||
       h->n_changed < 0 || static_cast<int64_t>(h->rows) * h->columns > INT32_MAX || h->n_changed > h->rows * h->columns)
@@ -1155,30 +1155,6 @@ int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
   return rc;
 }
 
-int tsattn_pages4_copy(const void *from, int64_t from_pages, void *to, int64_t to_pages, size_t page_bytes,
-                       int32_t n, const int32_t *src, const int32_t *dst, void *stream) {
-  if (!from || !to || !src || !dst) return fail(TSATTN_ERR_INVALID, "page copy: pointer is NULL");
-  if (n <= 0 || from_pages <= 0 || to_pages <= 0 || from_pages > INT32_MAX || to_pages > INT32_MAX || !page_bytes)
-    return fail(TSATTN_ERR_INVALID, "page copy: sizes must be positive");
-  if (page_bytes % 16 || (reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to)) % 16)
-    return fail(TSATTN_ERR_UNSUPPORTED, "page copy: pools and pages must be 16-byte aligned");
-  for (int32_t i = 0; i < n; ++i)
-    if (src[i] < 0 || src[i] >= from_pages || dst[i] < 0 || dst[i] >= to_pages)
-      return fail(TSATTN_ERR_INVALID, "page copy: page %d -> %d out of range", src[i], dst[i]);
-  // written pages are marked; within one pool none of them may be read
-  char *seen = static_cast<char *>(calloc(static_cast<size_t>(to_pages), 1));
-  if (!seen) return fail(TSATTN_ERR_INVALID, "page copy: out of host memory");
-  bool ok = distinct(n, dst, seen);
-  if (from == to)
-    for (int32_t i = 0; i < n && ok; ++i) ok = src[i] >= to_pages || !seen[src[i]];
-  free(seen);
-  if (!ok) return fail(TSATTN_ERR_INVALID, "page copy: a page is written twice, or read and written");
-  return hip_status(tsattn::launch_pages4_copy(static_cast<const char *>(from), static_cast<char *>(to),
-                                               static_cast<int64_t>(page_bytes), n, src, dst,
-                                               static_cast<hipStream_t>(stream)),
-                    "page copy launch");
-}
-
 int tsattn_pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
                        int32_t *dst, int32_t *copies) {
   int rc = check_host_rows4(h, n, rows);
@@ -1244,18 +1220,39 @@ int tsattn_pages4_compact(tsattn_pages4_host *h, int32_t *src, int32_t *dst, int
   return TSATTN_OK;
 }
 
-int tsattn_pages4_sync(tsattn_pages4_host *h, int32_t *table, void *stream) {
+int tsattn_pages4_apply(tsattn_pages4_host *h, int32_t *table, const void *from, int64_t from_pages, void *to,
+                        int64_t to_pages, size_t page_bytes, int32_t n, const int32_t *src, const int32_t *dst,
+                        void *stream) {
   int rc = check_host4(h);
   if (rc) return rc;
-  if (!table) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
-  if (!h->n_changed) return TSATTN_OK;
-  int32_t *at = static_cast<int32_t *>(malloc(sizeof(int32_t) * 2 * static_cast<size_t>(h->n_changed)));
+  if (!table || n < 0 || (n && (!from || !to || !src || !dst)))
+    return fail(TSATTN_ERR_INVALID, "page copy: pointer is NULL");
+  if (n) {
+    if (from_pages <= 0 || to_pages <= 0 || from_pages > INT32_MAX || to_pages > INT32_MAX || !page_bytes)
+      return fail(TSATTN_ERR_INVALID, "page copy: sizes must be positive");
+    if (page_bytes % 16 || (reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(to)) % 16)
+      return fail(TSATTN_ERR_UNSUPPORTED, "page copy: pools and pages must be 16-byte aligned");
+    for (int32_t i = 0; i < n; ++i)
+      if (src[i] < 0 || src[i] >= from_pages || dst[i] < 0 || dst[i] >= to_pages)
+        return fail(TSATTN_ERR_INVALID, "page copy: page %d -> %d out of range", src[i], dst[i]);
+    // written pages are marked; within one pool none of them may be read
+    char *seen = static_cast<char *>(calloc(static_cast<size_t>(to_pages), 1));
+    if (!seen) return fail(TSATTN_ERR_INVALID, "page copy: out of host memory");
+    bool ok = distinct(n, dst, seen);
+    if (from == to)
+      for (int32_t i = 0; i < n && ok; ++i) ok = src[i] >= to_pages || !seen[src[i]];
+    free(seen);
+    if (!ok) return fail(TSATTN_ERR_INVALID, "page copy: a page is written twice, or read and written");
+  }
+  int32_t *at = static_cast<int32_t *>(malloc(sizeof(int32_t) * (2 * static_cast<size_t>(h->n_changed) + 1)));
   if (!at) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
   int32_t *value = at + h->n_changed;
-  const int32_t n = tsattn::pages4_changes(h, at, value);
-  rc = n ? hip_status(tsattn::launch_pages4_set(table, n, at, value, static_cast<hipStream_t>(stream)),
-                      "page table launch")
-         : TSATTN_OK;
+  const int32_t sets = tsattn::pages4_changes(h, at, value);
+  rc = n || sets ? hip_status(tsattn::launch_pages4_apply(static_cast<const char *>(from), static_cast<char *>(to),
+                                                          static_cast<int64_t>(page_bytes), n, src, dst, table, sets,
+                                                          at, value, static_cast<hipStream_t>(stream)),
+                              "page update launch")
+                 : TSATTN_OK;
   free(at);
   return rc;
 }

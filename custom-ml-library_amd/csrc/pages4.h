@@ -35,7 +35,7 @@ namespace tsattn {
 constexpr int kTile = 32;     // positions a tile
 constexpr int kLongest = 1 << 27;  // positions a sequence: splits of 4096 stay within a grid's 65535
 constexpr int kSeqs = 256;    // sequences a launch: their numbers travel by value
-constexpr int kMoves = 480;   // pages, or table entries, a launch (under 4 KiB of arguments)
+constexpr int kMoves = 240;   // page copies, and table entries, a launch (under 4 KiB of arguments)
 
 // Sequences of a launch: row of the page table, cached positions (the kernels'
 // arguments hold them, so no copy to the device precedes a launch and a captured
@@ -96,9 +96,9 @@ hipError_t launch_pages4_append(const Pages4 &p, int dtype, int n, int len, View
                                 const void *cos, const void *sin, hipStream_t st);
 hipError_t launch_pages4_read(const Pages4 &p, int dtype, int n, int len, View k, View v, const Seqs &s,
                               const int32_t *first, hipStream_t st);
-hipError_t launch_pages4_copy(const char *from, char *to, int64_t page_bytes, int n, const int32_t *src,
-                              const int32_t *dst, hipStream_t st);
-hipError_t launch_pages4_set(int32_t *table, int n, const int32_t *at, const int32_t *value, hipStream_t st);
+hipError_t launch_pages4_apply(const char *from, char *to, int64_t page_bytes, int moves, const int32_t *src,
+                               const int32_t *dst, int32_t *table, int sets, const int32_t *at,
+                               const int32_t *value, hipStream_t st);
 
 // pages4_table.hip
 int32_t pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,

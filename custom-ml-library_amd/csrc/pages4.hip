@@ -381,17 +381,27 @@ __global__ __launch_bounds__(NT) void read_kernel(ReadArgs ra) {
   }
 }
 
-struct MoveArgs {
+struct ApplyArgs {
   const char *from;
   char *to;
   int64_t page_bytes;
-  int32_t src[kMoves], dst[kMoves];
+  int32_t *table;
+  int32_t moves, sets;
+  int32_t src[kMoves], dst[kMoves], at[kMoves], value[kMoves];
 };
 
-// Page blockIdx.y's share of a copy: 16 bytes a lane, four loads in flight.
-__global__ __launch_bounds__(NT) void copy_kernel(MoveArgs a) {
-  const u32x4 *from = reinterpret_cast<const u32x4 *>(a.from + a.src[blockIdx.y] * a.page_bytes);
-  u32x4 *to = reinterpret_cast<u32x4 *>(a.to + a.dst[blockIdx.y] * a.page_bytes);
+// Page copies, blockIdx.y's share of each: 16 bytes a lane, four loads in flight.
+// The row of blocks past them writes table entries (whose pages the stream's next
+// kernel reads: none here does).
+__global__ __launch_bounds__(NT) void apply_kernel(ApplyArgs a) {
+  const int move = blockIdx.y;
+  if (move == a.moves) {
+    const int i = blockIdx.x * NT + threadIdx.x;
+    if (i < a.sets) a.table[a.at[i]] = a.value[i];
+    return;
+  }
+  const u32x4 *from = reinterpret_cast<const u32x4 *>(a.from + a.src[move] * a.page_bytes);
+  u32x4 *to = reinterpret_cast<u32x4 *>(a.to + a.dst[move] * a.page_bytes);
   const int64_t n = a.page_bytes / 16;
   constexpr int U = 4;
   for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * NT * U; i0 < n; i0 += static_cast<int64_t>(gridDim.x) * NT * U) {
@@ -407,16 +417,6 @@ __global__ __launch_bounds__(NT) void copy_kernel(MoveArgs a) {
       if (i < n) __builtin_nontemporal_store(r[u], to + i);
     }
   }
-}
-
-struct SetArgs {
-  int32_t *table;
-  int32_t at[kMoves], value[kMoves];
-};
-
-__global__ __launch_bounds__(512) void set_kernel(SetArgs a, int n) {
-  const int i = threadIdx.x;
-  if (i < n) a.table[a.at[i]] = a.value[i];
 }
 
 // f(T, G) for the cache's dtype and head dim (both checked by the caller).
@@ -461,28 +461,20 @@ hipError_t launch_pages4_read(const Pages4 &p, int dtype, int n, int len, View k
   return hipGetLastError();
 }
 
-hipError_t launch_pages4_copy(const char *from, char *to, int64_t page_bytes, int n, const int32_t *src,
-                              const int32_t *dst, hipStream_t st) {
-  Probe pr_("pages4_copy", st);
-  for (int i0 = 0; i0 < n; i0 += kMoves) {
-    MoveArgs a{from, to, page_bytes, {}, {}};
-    const int m = n - i0 < kMoves ? n - i0 : kMoves;
-    for (int i = 0; i < m; ++i) a.src[i] = src[i0 + i], a.dst[i] = dst[i0 + i];
-    const int64_t blocks = (page_bytes / 16 + NT * 4 - 1) / (NT * 4);
-    copy_kernel<<<dim3(static_cast<unsigned>(blocks < 64 ? blocks : 64), m), dim3(NT), 0, st>>>(a);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  }
-  return hipSuccess;
-}
-
-hipError_t launch_pages4_set(int32_t *table, int n, const int32_t *at, const int32_t *value, hipStream_t st) {
-  Probe pr_("pages4_set", st);
-  for (int i0 = 0; i0 < n; i0 += kMoves) {
-    SetArgs a{table, {}, {}};
-    const int m = n - i0 < kMoves ? n - i0 : kMoves;
-    for (int i = 0; i < m; ++i) a.at[i] = at[i0 + i], a.value[i] = value[i0 + i];
-    static_assert(kMoves <= 512, "one lane an entry");
-    set_kernel<<<dim3(1), dim3((m + 63) / 64 * 64), 0, st>>>(a, m);
+hipError_t launch_pages4_apply(const char *from, char *to, int64_t page_bytes, int moves, const int32_t *src,
+                               const int32_t *dst, int32_t *table, int sets, const int32_t *at,
+                               const int32_t *value, hipStream_t st) {
+  const int64_t whole = moves ? (page_bytes / 16 + NT * 4 - 1) / (NT * 4) : 1;
+  const unsigned least = (kMoves + NT - 1) / NT, most = 64;  // (the entries' blocks; enough for a page)
+  const unsigned bx = whole < least ? least : whole < most ? static_cast<unsigned>(whole) : most;
+  Probe pr_("pages4_apply", st);
+  for (int i0 = 0; i0 < moves || i0 < sets; i0 += kMoves) {
+    ApplyArgs a{from, to, page_bytes, table, 0, 0, {}, {}, {}, {}};
+    for (; a.moves < kMoves && i0 + a.moves < moves; ++a.moves)
+      a.src[a.moves] = src[i0 + a.moves], a.dst[a.moves] = dst[i0 + a.moves];
+    for (; a.sets < kMoves && i0 + a.sets < sets; ++a.sets)
+      a.at[a.sets] = at[i0 + a.sets], a.value[a.sets] = value[i0 + a.sets];
+    apply_kernel<<<dim3(bx, a.moves + (a.sets ? 1 : 0)), dim3(NT), 0, st>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;

@@ -29,7 +29,7 @@ int32_t pages_of(const tsattn_pages4_host *h, int64_t positions) {
 void put(tsattn_pages4_host *h, int32_t row, int32_t column, int32_t page) {
   const int32_t at = row * h->columns + column;
   h->table[at] = page;
-  if (!h->dirty[at]) {
+  if (h->shown[at] != page && !h->dirty[at]) {
     h->dirty[at] = 1;
     h->changed[h->n_changed++] = at;
   }
@@ -39,13 +39,15 @@ void put(tsattn_pages4_host *h, int32_t row, int32_t column, int32_t page) {
 
 // Pages of their own for the next `steps` positions of the rows.  A row that appends
 // into a page that others hold too gets a copy of it (src -> dst); of the holders
-// that all append, the last keeps the page.  Counted first, so that too few free
-// pages change nothing: returns how many are needed then, else 0.
+// that all append, the first keeps the page.  Counted first, so that too few free
+// pages change nothing: returns how many are needed then, else 0.  Rows give pages
+// back last to first and take them first to last, so that those which are cut and
+// grow again, or fork again, find the pages that the device's table shows.
 int32_t pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
                     int32_t *dst, int32_t *copies) {
   int64_t need = 0;
   int32_t shared = 0;
-  for (int32_t i = 0; i < n; ++i) {
+  for (int32_t i = n; i-- > 0;) {
     const int32_t len = h->lengths[rows[i]], *row = row_of(h, rows[i]);
     int32_t c = len / h->page_size;
     if (len - c * h->page_size) {
@@ -65,7 +67,7 @@ int32_t pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32
   }
   *copies = shared;
   if (!need) return 0;
-  for (int32_t i = 0; i < shared; ++i) {
+  for (int32_t i = shared; i-- > 0;) {
     const int32_t row = dst[i];
     dst[i] = take(h);
     put(h, row, h->lengths[row] / h->page_size, dst[i]);
@@ -80,7 +82,7 @@ int32_t pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32
 
 // The rows end at `lengths`; pages wholly past them are given back.
 void pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const int32_t *lengths) {
-  for (int32_t i = 0; i < n; ++i) {
+  for (int32_t i = n; i-- > 0;) {
     int32_t *row = row_of(h, rows[i]);
     if (lengths[i] == h->lengths[rows[i]]) continue;
     for (int32_t c = pages_of(h, h->lengths[rows[i]]), stop = pages_of(h, lengths[i]); c-- > stop;) {
@@ -109,7 +111,7 @@ void pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const
     for (int32_t c = has; c < had; ++c) row_of(h, rows[i])[c] = -1;
     h->lengths[rows[i]] = from[h->columns];
   }
-  for (int32_t i = 0; i < n; ++i)
+  for (int32_t i = n; i-- > 0;)
     for (int32_t c = pages_of(h, old[i * width + h->columns]); c-- > 0;) let_go(h, old[i * width + c]);
 }
 
@@ -127,6 +129,7 @@ int32_t pages4_clone(const tsattn_pages4_host *from, int32_t n, const int32_t *r
     }
   if (k > to->pages) return k;
   memset(to->table, 0xFF, sizeof(int32_t) * to->rows * static_cast<size_t>(to->columns));
+  memset(to->shown, 0xFF, sizeof(int32_t) * to->rows * static_cast<size_t>(to->columns));
   memset(to->refs, 0, sizeof(int32_t) * to->pages);
   memset(to->dirty, 0, static_cast<size_t>(to->rows) * to->columns);
   to->n_changed = 0;
@@ -166,13 +169,16 @@ int32_t pages4_compact(tsattn_pages4_host *h, int32_t *number, int32_t *src, int
   return n;
 }
 
-// The changed entries that hold a page: at, value (room for n_changed); none is left.
+// The changed entries that hold another page than the device's: at, value (room for
+// n_changed); none is left.
 int32_t pages4_changes(tsattn_pages4_host *h, int32_t *at, int32_t *value) {
   int32_t k = 0;
   for (int32_t i = 0; i < h->n_changed; ++i) {
     const int32_t a = h->changed[i];
     h->dirty[a] = 0;
-    if (h->table[a] >= 0) at[k] = a, value[k++] = h->table[a];
+    if (h->table[a] < 0 || h->table[a] == h->shown[a]) continue;
+    at[k] = a;
+    value[k++] = h->shown[a] = h->table[a];
   }
   h->n_changed = 0;
   return k;

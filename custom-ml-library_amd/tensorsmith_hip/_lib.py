@@ -138,6 +138,7 @@ class Pages4Host(ctypes.Structure):
         ("lengths", c_void_p),
         ("refs", c_void_p),
         ("stack", c_void_p),
+        ("shown", c_void_p),
         ("changed", c_void_p),
         ("dirty", c_void_p),
         ("free", c_int32),
@@ -258,10 +259,6 @@ SIGNATURES = {
         [_P4, c_int32, c_int32, c_int32, c_int32, c_double, c_int32, _PV, _PV, c_void_p, c_void_p,
          c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
-    "tsattn_pages4_copy": (
-        c_int,
-        [c_void_p, c_int64, c_void_p, c_int64, c_size_t, c_int32, c_void_p, c_void_p, c_void_p],
-    ),
     "tsattn_pages4_grow": (
         c_int, [_PH, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
     "tsattn_pages4_cut": (c_int, [_PH, c_int32, c_void_p, c_void_p]),
@@ -269,7 +266,11 @@ SIGNATURES = {
     "tsattn_pages4_clone": (
         c_int, [_PH, c_int32, c_void_p, _PH, c_void_p, c_void_p, c_void_p]),
     "tsattn_pages4_compact": (c_int, [_PH, c_void_p, c_void_p, c_void_p]),
-    "tsattn_pages4_sync": (c_int, [_PH, c_void_p, c_void_p]),
+    "tsattn_pages4_apply": (
+        c_int,
+        [_PH, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_size_t, c_int32, c_void_p, c_void_p,
+         c_void_p],
+    ),
     "tsattn_key_mask_lengths": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p],

@@ -79,8 +79,8 @@ class _Pages:
                                       "pages of 32, 64, .. 4096 positions")
         # the host's arrays, side by side; src, dst: page copies that a call asks for
         most, entries = max(rows, num_pages), rows * columns
-        sizes = {"host": entries, "lengths": rows, "refs": num_pages, "stack": num_pages, "changed": entries,
-                 "src": most, "dst": most, "copies": 1, "dirty": (entries + 3) // 4}
+        sizes = {"host": entries, "lengths": rows, "refs": num_pages, "stack": num_pages, "shown": entries,
+                 "changed": entries, "src": most, "dst": most, "copies": 1, "dirty": (entries + 3) // 4}
         memory, at, where = np.zeros(sum(sizes.values()), np.int32), 0, {}
         base = memory.ctypes.data
         for name, n in sizes.items():
@@ -93,7 +93,7 @@ class _Pages:
         self.tables = t = _lib.Pages4Host()
         t.rows, t.columns, t.page_size, t.pages = rows, columns, page_size, num_pages
         t.table, t.lengths, t.refs, t.stack = (where[x] for x in ("host", "lengths", "refs", "stack"))
-        t.changed, t.dirty = where["changed"], where["dirty"]
+        t.shown, t.changed, t.dirty = (where[x] for x in ("shown", "changed", "dirty"))
         # (what no append has written weighs nothing: positions past a row's length are masked)
         self.pool = torch.empty((num_pages, self.page_bytes), dtype=torch.uint8, device=dev.torch)
         self.table = torch.empty((rows, columns), dtype=torch.int32, device=dev.torch)
@@ -105,6 +105,7 @@ class _Pages:
         """Every page free, every row empty."""
         pages = len(self.refs)
         self.host.fill(-1)
+        self.shown.fill(-1)
         self.stack[:] = np.arange(pages - 1, -1, -1)  # (the next one is the last)
         self.tables.free = pages
 
@@ -112,18 +113,16 @@ class _Pages:
     def free(self) -> int:
         return self.tables.free
 
-    def sync(self) -> None:
-        """The device's table up to date."""
-        if self.tables.n_changed:
-            self._eager()
-            _lib.check(launch(self.device, _lib.load().tsattn_pages4_sync, self.tables, self.desc.table), "page table")
-
-    def move(self, source, target) -> None:
-        """The page copies that the last host call asked for."""
-        n = int(self.copies[0])
-        if n:
-            _lib.check(launch(self.device, _lib.load().tsattn_pages4_copy, source.data_ptr(), source.shape[0],
-                              target.data_ptr(), target.shape[0], self.page_bytes, n, *self.out[:2]), "page copy")
+    def apply(self, source=None) -> None:
+        """To the device, on the current stream: the page copies that the last host call asked for
+        (from the pool of ``source``, by default this one's) and the changed table entries."""
+        source = source or self
+        n = int(source.copies[0])
+        if n or self.tables.n_changed:
+            source.copies[0] = 0
+            _lib.check(launch(self.device, _lib.load().tsattn_pages4_apply, self.tables, self.desc.table,
+                              source.desc.pool, source.desc.num_pages, self.desc.pool, self.desc.num_pages,
+                              self.page_bytes, n, *source.out[:2]), "page update")
 
     def _eager(self, rows=None, steps: int = 0) -> None:
         """Refuses page changes under capture: a captured call's pages would be the host's at once and
@@ -132,7 +131,7 @@ class _Pages:
 
         if not torch.cuda.is_current_stream_capturing():
             return
-        if rows is not None and not self.tables.n_changed:
+        if rows is not None:
             lens = self.lengths[rows]
             page = self.host[rows, lens // self.page_size % self.host.shape[1]]
             part = lens % self.page_size
@@ -154,7 +153,7 @@ class _Pages:
         other = _Pages(len(rows), self.heads, self.dim, self.host.shape[1], self.page_size, num_pages, self.device)
         _lib.check(_lib.load().tsattn_pages4_clone(self.tables, len(rows), rows.ctypes.data, other.tables, *self.out),
                    "page table")
-        self.move(self.pool, other.pool)
+        other.apply(self)
         return other
 
 
@@ -251,8 +250,7 @@ class PagedKVCache:
         core._eager(self._rows, steps)
         core.grow(len(lens), self._rows_at, steps)
         try:
-            core.move(core.pool, core.pool)
-            core.sync()
+            core.apply()
             _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
                               _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
         except BaseException:
@@ -298,7 +296,6 @@ class PagedKVCache:
         shape, dev = (len(lens), core.heads, steps, core.dim), core.pool.device
         out = [torch.empty(shape, dtype=self.dtype, device=dev) for _ in range(2)]
         if steps:
-            core.sync()
             _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
                               _view(out[0]), _view(out[1]), self._rows_at, lens_at, first.ctypes.data), "paged read")
         return tuple(Tensor(x, device=core.device) for x in out)
@@ -350,9 +347,11 @@ class PagedKVCache:
     def reorder(self, indices) -> None:
         """Row i becomes row ``indices[i]``, sharing its pages: no keys or values move.  Rows that
         take over the same row share until one appends (``append`` copies the page)."""
-        index = self._indices(indices, self._rows.shape)
-        _lib.check(_lib.load().tsattn_pages4_reorder(self._core.tables, len(index), self._rows_at, index.ctypes.data),
+        core, index = self._core, self._indices(indices, self._rows.shape)
+        core._eager()
+        _lib.check(_lib.load().tsattn_pages4_reorder(core.tables, len(index), self._rows_at, index.ctypes.data),
                    "page table")
+        core.apply()
 
     def copy(self, num_pages: int | None = None) -> "PagedKVCache":
         """A cache of these rows with a pool of its own (``num_pages``, by default as many as this
@@ -370,7 +369,7 @@ class PagedKVCache:
         if num_pages is None:
             core._eager()
             _lib.check(_lib.load().tsattn_pages4_compact(core.tables, *core.out), "page table")
-            core.move(core.pool, core.pool)
+            core.apply()
         else:
             core.__dict__.update(core.clone(np.arange(len(core.lengths), dtype=np.int32),
                                             self._pool_size(num_pages)).__dict__)
@@ -427,7 +426,6 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
     if rotary_base is not None:
         cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, dim, q.dtype, q.device,
                                                       max(int(lens.max()), steps)))
-    core.sync()
     out = torch.empty((b, heads, steps, dim), dtype=q.dtype, device=q.device)
     lib, code = _lib.load(), cache._code
     nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, lens_at)

@@ -589,19 +589,10 @@ int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
                          void *workspace, size_t workspace_bytes, void *stream);
 
 /*
- * Copy pages src[i] of a pool to pages dst[i] of a pool (the same one or another),
- * n of them, host arrays.  Destinations must differ, and within one pool no page may
- * be both read and written: TSATTN_ERR_INVALID.
- */
-int tsattn_pages4_copy(const void *from, int64_t from_pages, void *to, int64_t to_pages, size_t page_bytes,
-                       int32_t n, const int32_t *src, const int32_t *dst, void *stream);
-
-/*
  * The host's side of a paged cache, in the caller's arrays.  The calls below change
- * them and launch nothing, but for tsattn_pages4_sync, which brings the device's table
- * up to date (before the next append, read or attention).  Page copies that they ask
- * for, src[i] -> dst[i], are the caller's to launch (tsattn_pages4_copy) before the next
- * append.  A new cache's table holds -1, its stack pages - 1, .., 0 and free == pages;
+ * them and launch nothing, but for tsattn_pages4_apply: the page copies that they ask
+ * for, src[i] -> dst[i], and the changed entries are the caller's to bring to the device
+ * with it before the next append, read or attention on any stream.  A new cache's table holds -1, its stack pages - 1, .., 0 and free == pages;
  * lengths, refs, dirty and n_changed are 0.  `rows` of a call are n different rows.
  */
 typedef struct tsattn_pages4_host {
@@ -610,7 +601,8 @@ typedef struct tsattn_pages4_host {
   int32_t *lengths; /* [rows] cached positions */
   int32_t *refs;    /* [pages] rows that hold the page */
   int32_t *stack;   /* [pages] the free pages; the next one is stack[free - 1] */
-  int32_t *changed; /* [rows * columns] the entries that the device's table lacks, n_changed of them */
+  int32_t *shown;   /* [rows * columns] what the device's table holds */
+  int32_t *changed; /* [rows * columns] the entries that it may lack, n_changed of them */
   uint8_t *dirty;   /* [rows * columns] 1: the entry is among them */
   int32_t free, n_changed;
 } tsattn_pages4_host;
@@ -641,8 +633,15 @@ int tsattn_pages4_clone(const tsattn_pages4_host *h, int32_t n, const int32_t *r
 /* The pages in use become the first of the pool: *copies of them move (room for h's pages). */
 int tsattn_pages4_compact(tsattn_pages4_host *h, int32_t *src, int32_t *dst, int32_t *copies);
 
-/* The changed entries to the device's table [rows, columns]. */
-int tsattn_pages4_sync(tsattn_pages4_host *h, int32_t *table, void *stream);
+/*
+ * One launch for what the calls above leave to do: pages src[i] of the pool `from` copied
+ * to pages dst[i] of the pool `to` (the same or another; n of them, or none), and the
+ * changed entries to the device's table [rows, columns].  Destinations must differ,
+ * and within one pool no page may be both read and written: TSATTN_ERR_INVALID.
+ */
+int tsattn_pages4_apply(tsattn_pages4_host *h, int32_t *table, const void *from, int64_t from_pages, void *to,
+                        int64_t to_pages, size_t page_bytes, int32_t n, const int32_t *src, const int32_t *dst,
+                        void *stream);
 
 #ifdef __cplusplus
 }

@@ -46,24 +46,24 @@ class Memory:
     def tsattn_pages4_page_bytes(self, heads, page, dim):
         return page * 8 if dim in (32, 64, 128, 256) else 0
 
-    def tsattn_pages4_copy(self, source, sn, target, tn, page_bytes, n, src, dst, stream):
-        src, dst = _at(src, n, np.int32), _at(dst, n, np.int32)
-        assert len(set(dst)) == n and (source != target or not set(dst) & set(src))
-        old, new = (_at(x, m * page_bytes, np.uint8).reshape(m, -1) for x, m in ((source, sn), (target, tn)))
-        new[dst] = old[src]
-        self.calls.append(("copy", n))
-        return 0
-
-    def tsattn_pages4_sync(self, host, table, stream):
+    def tsattn_pages4_apply(self, host, table, source, sn, target, tn, page_bytes, n, src, dst, stream):
+        if n:
+            src, dst = _at(src, n, np.int32), _at(dst, n, np.int32)
+            assert len(set(dst)) == n and (source != target or not set(dst) & set(src))
+            old, new = (_at(x, m * page_bytes, np.uint8).reshape(m, -1) for x, m in ((source, sn), (target, tn)))
+            new[dst] = old[src]
+            self.calls.append(("copy", n))
         entries = host.rows * host.columns
         at, want = _at(host.changed, entries, np.int32)[:host.n_changed], _at(host.table, entries, np.int32)
         assert len(set(at)) == len(at) and _at(host.dirty, entries, np.uint8).sum() == len(at)
         assert _at(host.dirty, entries, np.uint8)[at].all()
-        at = at[want[at] >= 0]
-        _at(table, entries, np.int32)[at] = want[at]
+        shown = _at(host.shown, entries, np.int32)
+        at = at[(want[at] >= 0) & (want[at] != shown[at])]
+        _at(table, entries, np.int32)[at] = shown[at] = want[at]
         _at(host.dirty, entries, np.uint8)[:] = 0
         host.n_changed = 0
-        self.calls.append(("sync", len(at)))
+        if len(at):
+            self.calls.append(("set", len(at)))
         return 0
 
     def tsattn_pages4_append(self, desc, dtype, n, steps, k, v, rows, lens, cos, sin, stream):
@@ -97,7 +97,6 @@ def memory():
 
 def _held(cache, row):
     core = cache._core
-    core.sync()
     pool = core.pool.numpy().view(np.float64).reshape(core.pool.shape[0], -1)
     table = core.table.numpy()
     n = core.lengths[row]
@@ -106,6 +105,8 @@ def _held(cache, row):
 
 def _sound(cache, want):
     core = cache._core
+    held = core.host >= 0
+    assert core.tables.n_changed == 0 and (core.table.numpy()[held] == core.host[held]).all() and (core.shown.reshape(core.host.shape)[held] == core.host[held]).all()
     used = core.host[core.host >= 0]
     assert (np.bincount(used, minlength=len(core.refs)) == core.refs).all()
     free = core.stack[:core.free]
@@ -202,6 +203,67 @@ def test_beams_copy_one_page_each(memory):
     assert not any(name == "copy" for name, _ in memory.calls)
     # positions 102 .. 127 touch no page but their own: nothing but the append is called
     assert {name for name, _ in memory.calls} == {"append"}
+
+
+def test_rows_that_grow_or_fork_again_find_their_pages(memory):
+    """Drafted tokens that are dropped change no table entry; beams that start over, no more than their own."""
+    cache = nn.PagedKVCache(4, 2, 32, 300, device="hip", page_size=32)
+    cache.append(_rows([[0.0] * 100] * 4), _rows([[0.0] * 100] * 4))
+    cache.truncate([64, 65, 90, 32])
+    for _ in range(3):
+        cache.append(_rows([[1.0] * 70] * 4), _rows([[1.0] * 70] * 4))
+        cache.truncate([64, 65, 90, 32])
+    memory.calls.clear()
+    cache.append(_rows([[1.0] * 70] * 4), _rows([[1.0] * 70] * 4))
+    assert [x for x in memory.calls if x[0] == "set"] == []
+    for i in range(3):
+        memory.calls.clear()
+        cache.truncate([40] * 4 if i else [40, 64, 64, 64])
+        cache.reorder([0] * 4)
+        cache.append(_rows([[2.0]] * 4), _rows([[2.0]] * 4))
+        assert ("copy", 3) in memory.calls
+    assert [n for name, n in memory.calls if name == "set"] == [3, 3]  # the shared page, and back
+
+
+@pytest.mark.parametrize("index", [0, 1])
+def test_calls_launch_on_the_caches_device(memory, index):
+    """With the cache's device current, on its current stream, whichever was current before."""
+    seen, state = [], {"device": 0}
+
+    class on:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            self.before, state["device"] = state["device"], self.device
+
+        def __exit__(self, *_):
+            state["device"] = self.before
+
+    class Noting:
+        def __getattr__(self, name):
+            if name == "tsattn_pages4_attend_workspace":
+                return lambda *a: 64
+            launches = name in ("tsattn_pages4_" + x for x in ("append", "apply", "read", "attend"))
+            call = (lambda *a: 0) if name.endswith(("read", "attend")) else getattr(memory, name)
+            return lambda *a: (launches and seen.append((name, state["device"], a[-1]))) or call(*a)
+
+    with patch.object(torch.cuda, "current_device", lambda: state["device"]), patch.object(torch.cuda, "device", on), \
+            patch.object(D, "current_stream", lambda dev: 0x100 + dev.index), patch.object(_lib, "load", lambda: Noting()):
+        dev = f"hip:{index}"
+        x = lambda *s: ts.Tensor(torch.zeros(s), device=dev)  # noqa: E731
+        cache = nn.PagedKVCache(2, 2, 32, 100, device=dev)
+        cache.append(x(2, 2, 3, 32), x(2, 2, 3, 32), rotary_base=100.0)
+        cache.reorder([1, 1])
+        cache.append(x(2, 2, 1, 32), x(2, 2, 1, 32))
+        cache.get(), cache.copy(), cache.compact(7)
+        nn.paged_attention(x(2, 4, 1, 32), cache, rotary_base=100.0)
+        with pytest.raises(ValueError, match="same device"):
+            other = ts.Tensor(torch.zeros(2, 4, 1, 32), device=f"hip:{1 - index}")
+            nn.paged_attention(other, cache)
+    assert {name for name, _, _ in seen} == {"tsattn_pages4_" + x for x in ("append", "apply", "read", "attend")}
+    assert all(device == index and stream == 0x100 + index for _, device, stream in seen), seen
+    assert state["device"] == 0
 
 
 def test_a_failed_append_leaves_the_lengths(memory):
@@ -365,7 +427,7 @@ def test_c_calls_refuse(change, status, what):
         assert call() == status and what in _lib.last_error()
 
 
-def test_c_appends_attention_reads_copies_and_tables_refuse():
+def test_c_appends_attention_and_reads_refuse():
     lib = _lib.load()
     append, _, _ = _calls(rows=(1, 1))
     assert append() == _lib.ERR_INVALID and "different" in _lib.last_error()
@@ -384,12 +446,6 @@ def test_c_appends_attention_reads_copies_and_tables_refuse():
     assert lib.tsattn_pages4_attend(d, _lib.F16, 1, 4, 1, 0.1, 1, v, v, rows, lens, None, None, 0x1000, need - 1,
                                     None) == _lib.ERR_INVALID and "too small" in _lib.last_error()
     assert lib.tsattn_pages4_read(d, _lib.F16, 1, 1, v, v, rows, lens, _ints(-1), None) == _lib.ERR_INVALID
-    copy = lambda src, dst, to=0x10000, pages=8, size=1024: lib.tsattn_pages4_copy(  # noqa: E731
-        0x10000, 8, to, pages, size, len(src), _ints(*src), _ints(*dst), None)
-    for bad in (copy([0, 1], [2, 2]), copy([0, 1], [1, 2]), copy([8], [0]), copy([0], [8]), copy([-1], [0]),
-                copy([0], [3], to=0x50000, pages=3), copy([3], [3]), copy([], [])):
-        assert bad == _lib.ERR_INVALID
-    assert copy([0], [1], size=1000) == _lib.ERR_UNSUPPORTED
     assert lib.tsattn_pages4_page_bytes(8, 64, 128) == 8 * 2 * 36 * 128
     assert [lib.tsattn_pages4_page_bytes(*s) for s in ((8, 64, 96), (8, 33, 64), (0, 64, 64), (8, 16, 64))] == [0] * 4
 
@@ -397,10 +453,10 @@ def test_c_appends_attention_reads_copies_and_tables_refuse():
 def test_c_tables_refuse():
     lib = _lib.load()
     arrays = {name: np.zeros(n, np.int32) for name, n in (("table", 6), ("lengths", 3), ("refs", 4), ("stack", 4),
-                                                          ("changed", 6), ("dirty", 2))}
+                                                          ("shown", 6), ("changed", 6), ("dirty", 2))}
     h = _lib.Pages4Host()
     h.rows, h.columns, h.page_size, h.pages, h.free = 3, 2, 32, 4, 4
-    arrays["table"][:], arrays["stack"][:] = -1, (3, 2, 1, 0)
+    arrays["table"][:], arrays["shown"][:], arrays["stack"][:] = -1, -1, (3, 2, 1, 0)
     for name, x in arrays.items():
         setattr(h, name, x.ctypes.data)
     src, dst, copies = _ints(*[0] * 4), _ints(*[0] * 4), _ints(0)
@@ -425,7 +481,13 @@ def test_c_tables_refuse():
     assert clone(3) == _lib.ERR_INVALID and "4 pages are in use" in _lib.last_error()
     to.table = None
     assert clone(3) == _lib.ERR_INVALID
-    assert lib.tsattn_pages4_sync(h, None, None) == _lib.ERR_INVALID
+    copy = lambda src, dst, to=0x10000, pages=8, size=1024, table=0x1000: lib.tsattn_pages4_apply(  # noqa: E731
+        h, table, 0x10000, 8, to, pages, size, len(src), _ints(*src), _ints(*dst), None)
+    for bad in (copy([0, 1], [2, 2]), copy([0, 1], [1, 2]), copy([8], [0]), copy([0], [8]), copy([-1], [0]),
+                copy([0], [3], to=0x50000, pages=3), copy([3], [3]), copy([], [], table=None), copy([0], [1], to=None),
+                lib.tsattn_pages4_apply(h, 0x1000, 0x10000, 8, 0x10000, 8, 1024, -1, None, None, None)):
+        assert bad == _lib.ERR_INVALID
+    assert copy([0], [1], size=1000) == copy([0], [1], to=0x50008) == _lib.ERR_UNSUPPORTED and h.n_changed == 4
     assert lib.tsattn_pages4_compact(h, src, None, copies) == _lib.ERR_INVALID
     h.free = 5
     assert lib.tsattn_pages4_compact(h, src, dst, copies) == _lib.ERR_INVALID
