@@ -568,6 +568,8 @@ int check_pages4(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t len, 
                 "a paged cache takes head dims 32, 64, 128 and 256, up to 4096 heads and pages of 32, 64, .. 4096 "
                 "positions");
   if (!p->pool || !p->table) return fail(TSATTN_ERR_INVALID, "paged cache: data pointer is NULL");
+  if ((len / tsattn::kTile + 2ll) * p->heads > INT32_MAX / 4)  // (the kernels number tiles, heads and sides)
+    return fail(TSATTN_ERR_UNSUPPORTED, "paged cache: too many positions and heads for one call");
   if (reinterpret_cast<uintptr_t>(p->pool) % 16)
     return fail(TSATTN_ERR_UNSUPPORTED, "a paged cache's pool must be 16-byte aligned");
   const int64_t room = p->table_stride * p->page_size;
@@ -647,12 +649,28 @@ int check_host4(const tsattn_pages4_host *h) {
   return TSATTN_OK;
 }
 
+bool length_fits(const tsattn_pages4_host *h, int32_t row) {
+  return h->lengths[row] >= 0 && h->lengths[row] <= static_cast<int64_t>(h->columns) * h->page_size;
+}
+
+// The pages of positions from .. to - 1 of a row are pages of the pool.
+int check_held4(const tsattn_pages4_host *h, int32_t row, int64_t from, int64_t to) {
+  for (int64_t c = from / h->page_size; c * h->page_size < to; ++c) {
+    const int32_t page = h->table[static_cast<int64_t>(row) * h->columns + c];
+    if (page < 0 || page >= h->pages)
+      return fail(TSATTN_ERR_INVALID, "page table: row %d has page %d of %d", row, page, h->pages);
+  }
+  return TSATTN_OK;
+}
+
 int check_host_rows4(const tsattn_pages4_host *h, int32_t n, const int32_t *rows) {
   int rc = check_host4(h);
   if (rc) return rc;
   if (!rows || n <= 0) return fail(TSATTN_ERR_INVALID, "page table: rows must be given");
-  for (int32_t i = 0; i < n; ++i)
+  for (int32_t i = 0; i < n; ++i) {
     if (rows[i] < 0 || rows[i] >= h->rows) return fail(TSATTN_ERR_INVALID, "page table: row %d out of range", rows[i]);
+    if (!length_fits(h, rows[i])) return fail(TSATTN_ERR_INVALID, "page table: row %d has no such length", rows[i]);
+  }
   char *seen = static_cast<char *>(calloc(static_cast<size_t>(h->rows), 1));
   if (!seen) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
   const bool ok = distinct(n, rows, seen);
@@ -1105,6 +1123,8 @@ size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int
   if (!p || !lens || n <= 0 || heads_q <= 0 || len_q <= 0 || !pages4_sizes_ok(p->heads, p->page_size, p->dim) ||
       heads_q % p->heads || static_cast<int64_t>(heads_q / p->heads) * len_q > (1 << 18))
     return 0;
+  for (int32_t i = 0; i < n; ++i)
+    if (lens[i] < 0 || lens[i] > tsattn::kLongest) return 0;
   tsattn::Attend4 a{};
   a.p.heads = p->heads, a.p.dim = p->dim;
   a.rows = heads_q / p->heads * len_q;
@@ -1164,7 +1184,12 @@ int tsattn_pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, in
     if (steps <= 0 || static_cast<int64_t>(h->lengths[rows[i]]) + steps > static_cast<int64_t>(h->columns) * h->page_size)
       return fail(TSATTN_ERR_INVALID, "page table: %d positions after %d of row %d exceed it", steps,
                   h->lengths[rows[i]], rows[i]);
+  for (int32_t i = 0; i < n; ++i) {
+    const int32_t len = h->lengths[rows[i]];
+    if (len % h->page_size && (rc = check_held4(h, rows[i], len - 1, len))) return rc;
+  }
   const int32_t need = tsattn::pages4_grow(h, n, rows, steps, src, dst, copies);
+  if (need < 0) return fail(TSATTN_ERR_INVALID, "page table: a free page is not one of the pool");
   if (need) return fail(TSATTN_ERR_INVALID, "page pool exhausted: %d pages needed, %d free", need, h->free);
   return TSATTN_OK;
 }
@@ -1176,6 +1201,8 @@ int tsattn_pages4_cut(tsattn_pages4_host *h, int32_t n, const int32_t *rows, con
   for (int32_t i = 0; i < n; ++i)
     if (lengths[i] < 0 || lengths[i] > h->lengths[rows[i]])
       return fail(TSATTN_ERR_INVALID, "truncate length must be between zero and the current length");
+  for (int32_t i = 0; i < n; ++i)
+    if (lengths[i] < h->lengths[rows[i]] && (rc = check_held4(h, rows[i], lengths[i], h->lengths[rows[i]]))) return rc;
   tsattn::pages4_cut(h, n, rows, lengths);
   return TSATTN_OK;
 }
@@ -1186,6 +1213,8 @@ int tsattn_pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows,
   if (!index) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
   for (int32_t i = 0; i < n; ++i)
     if (index[i] < 0 || index[i] >= n) return fail(TSATTN_ERR_INVALID, "beam index out of range");
+  for (int32_t i = 0; i < n; ++i)
+    if ((rc = check_held4(h, rows[i], 0, h->lengths[rows[i]]))) return rc;
   int32_t *old = static_cast<int32_t *>(malloc(sizeof(int32_t) * n * (static_cast<size_t>(h->columns) + 1)));
   if (!old) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
   tsattn::pages4_reorder(h, n, rows, index, old);
@@ -1200,6 +1229,8 @@ int tsattn_pages4_clone(const tsattn_pages4_host *h, int32_t n, const int32_t *r
   if (!src || !dst || !copies) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
   if (to->rows != n || to->columns != h->columns || to->page_size != h->page_size)
     return fail(TSATTN_ERR_INVALID, "page table: a clone has the rows' number, columns and page size");
+  for (int32_t i = 0; i < n; ++i)
+    if ((rc = check_held4(h, rows[i], 0, h->lengths[rows[i]]))) return rc;
   int32_t *number = static_cast<int32_t *>(malloc(sizeof(int32_t) * static_cast<size_t>(h->pages)));
   if (!number) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
   const int32_t used = tsattn::pages4_clone(h, n, rows, to, number, src, dst);
@@ -1213,6 +1244,14 @@ int tsattn_pages4_compact(tsattn_pages4_host *h, int32_t *src, int32_t *dst, int
   int rc = check_host4(h);
   if (rc) return rc;
   if (!src || !dst || !copies) return fail(TSATTN_ERR_INVALID, "page table: pointer is NULL");
+  int32_t held = 0;
+  for (int32_t p = 0; p < h->pages; ++p) held += h->refs[p] != 0;
+  if (held != h->pages - h->free)
+    return fail(TSATTN_ERR_INVALID, "page table: %d pages are held and %d free of %d", held, h->free, h->pages);
+  for (int32_t row = 0; row < h->rows; ++row) {
+    if (!length_fits(h, row)) return fail(TSATTN_ERR_INVALID, "page table: row %d has no such length", row);
+    if ((rc = check_held4(h, row, 0, h->lengths[row]))) return rc;
+  }
   int32_t *number = static_cast<int32_t *>(malloc(sizeof(int32_t) * static_cast<size_t>(h->pages)));
   if (!number) return fail(TSATTN_ERR_INVALID, "page table: out of host memory");
   tsattn::pages4_compact(h, number, src, dst, copies);

@@ -13,7 +13,7 @@ namespace {
 int32_t *row_of(const tsattn_pages4_host *h, int32_t row) { return h->table + static_cast<int64_t>(row) * h->columns; }
 
 void let_go(tsattn_pages4_host *h, int32_t page) {
-  if (--h->refs[page] == 0) h->stack[h->free++] = page;
+  if (--h->refs[page] == 0 && h->free < h->pages) h->stack[h->free++] = page;
 }
 
 int32_t take(tsattn_pages4_host *h) {
@@ -40,9 +40,10 @@ void put(tsattn_pages4_host *h, int32_t row, int32_t column, int32_t page) {
 // Pages of their own for the next `steps` positions of the rows.  A row that appends
 // into a page that others hold too gets a copy of it (src -> dst); of the holders
 // that all append, the first keeps the page.  Counted first, so that too few free
-// pages change nothing: returns how many are needed then, else 0.  Rows give pages
-// back last to first and take them first to last, so that those which are cut and
-// grow again, or fork again, find the pages that the device's table shows.
+// pages change nothing: returns how many are needed then, -1 where a free page is not
+// one of the pool, else 0.  Rows give pages back last to first and take them first to
+// last, so that those which are cut and grow again, or fork again, find the pages that
+// the device's table shows.
 int32_t pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32_t steps, int32_t *src,
                     int32_t *dst, int32_t *copies) {
   int64_t need = 0;
@@ -61,9 +62,14 @@ int32_t pages4_grow(tsattn_pages4_host *h, int32_t n, const int32_t *rows, int32
     }
     need += pages_of(h, static_cast<int64_t>(len) + steps) - c;
   }
-  if (need > h->free) {
+  bool known = true;
+  for (int64_t i = 0; i < need && need <= h->free; ++i) {
+    const int32_t page = h->stack[h->free - 1 - i];
+    known = known && page >= 0 && page < h->pages;
+  }
+  if (need > h->free || !known) {
     for (int32_t i = 0; i < shared; ++i) ++h->refs[src[i]];
-    return static_cast<int32_t>(need < INT32_MAX ? need : INT32_MAX);
+    return !known ? -1 : static_cast<int32_t>(need < INT32_MAX ? need : INT32_MAX);
   }
   *copies = shared;
   if (!need) return 0;
@@ -154,6 +160,7 @@ int32_t pages4_compact(tsattn_pages4_host *h, int32_t *number, int32_t *src, int
   const int32_t n = h->pages - h->free;
   int32_t hole = 0, k = 0;
   for (int32_t p = n; p < h->pages; ++p) {
+    number[p] = p;
     if (!h->refs[p]) continue;
     while (h->refs[hole]) ++hole;
     h->refs[hole] = h->refs[p];

@@ -592,8 +592,10 @@ int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
  * The host's side of a paged cache, in the caller's arrays.  The calls below change
  * them and launch nothing, but for tsattn_pages4_apply: the page copies that they ask
  * for, src[i] -> dst[i], and the changed entries are the caller's to bring to the device
- * with it before the next append, read or attention on any stream.  A new cache's table holds -1, its stack pages - 1, .., 0 and free == pages;
- * lengths, refs, dirty and n_changed are 0.  `rows` of a call are n different rows.
+ * with it before the next append, read or attention on any stream.  A new cache's table
+ * and `shown` hold -1, its stack pages - 1, .., 0 and free == pages; lengths, refs, dirty
+ * and n_changed are 0.  `rows` of a call are n different rows.  A length past the table,
+ * or a page number that is not one of the pool, is refused.
  */
 typedef struct tsattn_pages4_host {
   int32_t rows, columns, page_size, pages;

@@ -446,6 +446,12 @@ def test_c_appends_attention_and_reads_refuse():
     assert lib.tsattn_pages4_attend(d, _lib.F16, 1, 4, 1, 0.1, 1, v, v, rows, lens, None, None, 0x1000, need - 1,
                                     None) == _lib.ERR_INVALID and "too small" in _lib.last_error()
     assert lib.tsattn_pages4_read(d, _lib.F16, 1, 1, v, v, rows, lens, _ints(-1), None) == _lib.ERR_INVALID
+    for lens in ((-1,), (1 << 28,)):
+        assert lib.tsattn_pages4_attend_workspace(d, _lib.F16, 1, 4, 1, _ints(*lens)) == 0
+    d.heads, d.table_stride = 4096, 1 << 21  # (more tiles, heads and sides than a launch numbers)
+    for call in (lambda: lib.tsattn_pages4_append(d, _lib.F16, 1, 1 << 26, v, v, rows, _ints(0), None, None, None),
+                 lambda: lib.tsattn_pages4_read(d, _lib.F16, 1, 1 << 26, v, v, rows, _ints(0), _ints(0), None)):
+        assert call() == _lib.ERR_UNSUPPORTED and "too many" in _lib.last_error()
     assert lib.tsattn_pages4_page_bytes(8, 64, 128) == 8 * 2 * 36 * 128
     assert [lib.tsattn_pages4_page_bytes(*s) for s in ((8, 64, 96), (8, 33, 64), (0, 64, 64), (8, 16, 64))] == [0] * 4
 
@@ -466,12 +472,28 @@ def test_c_tables_refuse():
                 grow([0, 1, 2], 64)):
         assert bad == _lib.ERR_INVALID
     assert "6 pages needed, 4 free" in _lib.last_error() and h.free == 4 and (arrays["table"] < 0).all()
+    for stack in ((3, 2, 1, 4), (3, 2, -1, 0)):  # (a free page that the pool does not have)
+        arrays["stack"][:] = stack
+        assert grow([0, 1], 1) == _lib.ERR_INVALID and h.free == 4 and (arrays["table"] < 0).all()
+    arrays["stack"][:] = (3, 2, 1, 0)
+    for length in (-1, 65):  # (past the table)
+        arrays["lengths"][1] = length
+        assert grow([1], 1) == lib.tsattn_pages4_compact(h, src, dst, copies) == _lib.ERR_INVALID
+    arrays["lengths"][1] = 0
     assert grow([0, 2], 33) == 0 and h.free == 0 and h.n_changed == 4
     arrays["lengths"][:] = (33, 0, 33)
     cut = lambda rows, lens: lib.tsattn_pages4_cut(h, len(rows), _ints(*rows), _ints(*lens))  # noqa: E731
     assert [cut([0], [34]), cut([0], [-1]), cut([1], [1]), cut([0, 0], [1, 1])] == [_lib.ERR_INVALID] * 4
     order = lambda index: lib.tsattn_pages4_reorder(h, len(index), _ints(0, 1, 2), _ints(*index))  # noqa: E731
     assert [order([0, 1, 3]), order([-1, 0, 0])] == [_lib.ERR_INVALID] * 2
+    held, after = arrays["table"].copy(), arrays["refs"].copy()
+    for page in (-1, 4):  # (a held page that the pool does not have)
+        arrays["table"][1] = page
+        for bad in (grow([0], 1), cut([0], [0]), order([1, 0, 2]), lib.tsattn_pages4_compact(h, src, dst, copies)):
+            assert bad == _lib.ERR_INVALID and f"page {page} of 4" in _lib.last_error()
+        assert lib.tsattn_pages4_clone(h, 3, _ints(0, 1, 2), h, src, dst, copies) == _lib.ERR_INVALID
+    arrays["table"][:] = held
+    assert (arrays["refs"] == after).all() and h.free == 0 and arrays["lengths"].tolist() == [33, 0, 33]
     to = _lib.Pages4Host()
     for name, _ in _lib.Pages4Host._fields_:
         setattr(to, name, getattr(h, name))
@@ -489,5 +511,7 @@ def test_c_tables_refuse():
         assert bad == _lib.ERR_INVALID
     assert copy([0], [1], size=1000) == copy([0], [1], to=0x50008) == _lib.ERR_UNSUPPORTED and h.n_changed == 4
     assert lib.tsattn_pages4_compact(h, src, None, copies) == _lib.ERR_INVALID
+    h.free = 1  # (every page is held)
+    assert lib.tsattn_pages4_compact(h, src, dst, copies) == _lib.ERR_INVALID and "4 pages are held" in _lib.last_error()
     h.free = 5
     assert lib.tsattn_pages4_compact(h, src, dst, copies) == _lib.ERR_INVALID
