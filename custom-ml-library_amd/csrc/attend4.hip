@@ -118,7 +118,8 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
     for (int i = 0; i < QW; ++i) raw[nb][i] = reinterpret_cast<const u32x4 *>(qp)[i];
   }
   // the wave's page numbers, lane t's for its tile t: one load, and none in the loop
-  const int ids = a.p.table[trow * a.p.stride + ((tile0 + NWV * min(lane, max(mine, 1) - 1)) >> a.p.per_page)];
+  // (lanes past the wave's tiles: the split's last, as the table need not go on)
+  const int ids = a.p.table[trow * a.p.stride + ((begin / kTile + min(w + NWV * lane, n_tiles - 1)) >> a.p.per_page)];
   auto load = [&](Held<G> &x, int t) __attribute__((always_inline)) {
     using C = typename Held<G>::Chunk;
     const char *base = tile4_at(a.p, static_cast<uint32_t>(__builtin_amdgcn_readlane(ids, t)), tile0 + NWV * t, hk);
