@@ -47,16 +47,19 @@ __device__ __forceinline__ void split_bf16(float a, float b, uint32_t (&out)[N])
   out[N - 1] = pack2<bf16>(a, b);
 }
 
-// Sum over the G neighbouring lanes of a row's groups.
+// Sum of a x over the G neighbouring lanes of a row's groups.  (Contracted, the first
+// addition would take a multiply-add and a move of its own from the other lane.)
 template <int G>
-__device__ __forceinline__ float group_sum4(float x) {
+__device__ __forceinline__ float scaled_sum(float a, float x) {
+#pragma clang fp contract(off)
   auto dpp = [](float v, auto ctrl) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF, 0xF, true));
   };
-  if constexpr (G >= 2) x += dpp(x, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
-  if constexpr (G >= 4) x += dpp(x, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
-  if constexpr (G >= 8) x += dpp(x, std::integral_constant<int, 0x141>{});  // half-row mirror: the other quad
-  return x;
+  float y = a * x;
+  if constexpr (G >= 2) y += dpp(y, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  if constexpr (G >= 4) y += dpp(y, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  if constexpr (G >= 8) y += dpp(y, std::integral_constant<int, 0x141>{});  // half-row mirror: the other quad
+  return y;
 }
 
 // A lane's share of a tile: codes of keys and values, eight scales of each.
@@ -211,8 +214,8 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const uint32_t k2 = t4.ks[i >> 1], v2 = t4.vs[i >> 1];
-        x[i] = group_sum4<G>(s[nb][i >> 2][i & 3] * __builtin_bit_cast(float, k2 << 16));
-        x[i + 1] = group_sum4<G>(s[nb][i >> 2][(i & 3) + 1] * __builtin_bit_cast(float, k2 & 0xFFFF0000u));
+        x[i] = scaled_sum<G>(s[nb][i >> 2][i & 3], __builtin_bit_cast(float, k2 << 16));
+        x[i + 1] = scaled_sum<G>(s[nb][i >> 2][(i & 3) + 1], __builtin_bit_cast(float, k2 & 0xFFFF0000u));
         vs[i] = __builtin_bit_cast(float, v2 << 16);
         vs[i + 1] = __builtin_bit_cast(float, v2 & 0xFFFF0000u);
       }
