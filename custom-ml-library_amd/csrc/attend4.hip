@@ -363,25 +363,22 @@ __global__ __launch_bounds__(64) void attend4_merge_kernel(Attend4 a) {
     if (lane + 64 * i < D) out[lane + 64 * i] = static_cast<T>(L == 0.f ? 0.f : acc[i] / L);
 }
 
-// Column blocks of a workgroup.  Two read the cache once for twice the rows;
-// their operands are more registers than fp32 queries (three parts) and 256
-// channels leave.
-int column_blocks(int dtype, int dim, int rows) {
-  return rows > 512 / dim && dtype != TSATTN_F32 && dim < 256 ? 2 : 1;
-}
-
 }  // namespace
 
-// Waves a workgroup (four, two or three workgroups a CU; or eight, which take one by
-// themselves) and splits: those that a model of the time likes best.  In us: a
-// workgroup's prologue and merge 2.2; a tile of a wave the largest of its own latency
-// (by its MFMAs; fp32 D128 1.5, bf16 D256 2.0, bf16 D128 1.0 with one column block
-// and 2.2 with two), of the issue slots of the waves beside it and of the memory's
-// rate; where the workgroups do not fit the chip at once, their sum over it and half a
-// workgroup's end; the second kernel 3.  Measured, what it picks and the other end:
-// 16 sequences of 8 KV heads up to 3000 positions, 8 rows of f16 D128: 2 splits 21.6,
-// one 31.1; 3 of one head over 1500, fp32 D128: 12 splits 7.2, one 13.1; 64 of 8
-// heads over 1025, 4 rows of f16 D128: one split 18.8, three 24.
+// Column blocks and waves of a workgroup, and splits: those that a model of the time
+// likes best.  Two blocks read the cache once for twice the rows; one, where the
+// memory is not what a call waits for, has twice the workgroups.  Four waves (two or
+// three workgroups a CU) or eight, which take a CU by themselves.  In us: a workgroup's
+// prologue and merge 2.3 or 2.5; a tile of a wave the largest of its own latency (by its
+// MFMAs; bf16 D128 0.94 with one block, 1.8 with two, fp32 D128 1.7, bf16 D256 1.7), of the
+// issue slots of the waves beside it and of the memory's rate; where the workgroups do
+// not fit the chip at once, their rounds over it; the second kernel 2.6.  Its constants
+// are fitted to 34 shapes, of which it takes 4% longer than the best choice in the
+// mean.  Measured, what it picks and another: 7 sequences of 4 KV heads up to 4001, 20
+// rows of bf16 D128: one block and 7 splits 17.4, two and 8 19.1; 64 of 4 heads over
+// 2000, 16 rows: two blocks 42, one 53; 4 of 32 heads over 4000, f16 D128: eight waves
+// and 2 splits 19.0, four and 3 22.4; 3 of one head over 1500, fp32 D128: 12 splits 7.1,
+// one 13.1; 64 of 8 heads over 1025, 4 rows of f16 D128: one split 18.6, three 24.
 void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
   int64_t total = 0;
   int longest = 1;
@@ -389,16 +386,12 @@ void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
     total += lens[i];
     longest = lens[i] > longest ? lens[i] : longest;
   }
-  const int dim = a->p.dim, nb = column_blocks(dtype, dim, a->rows), per = 512 / dim * nb;
-  a->blocks = (a->rows + per - 1) / per;
-  const double groups = static_cast<double>(a->p.heads) * a->blocks;
+  const int dim = a->p.dim;
   const int parts = dtype == TSATTN_F32 ? 6 : dtype == TSATTN_F16 ? 4 : 3;
-  const double latency = 0.2 + 0.034 * nb * (dim / 16) * parts;
   const int fewest = (longest + kMostSplit - 1) / kMostSplit;
   double best = 1e30;
   for (int waves = 4; waves <= 8; waves += 4) {
-    if (waves == 8 && dtype == TSATTN_F32 && dim == 256) continue;  // (more registers than eight waves have)
-    const double slots = waves == 8 ? 256. : nb == 2 || dim == 256 ? 512. : 768.;
+    if (waves == 8 && dtype != TSATTN_BF16 && dim == 256) continue;  // (more registers than eight waves have)
     const int unit = kTile * waves;
     for (int k : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       const int n = k > fewest ? k : fewest;
@@ -412,30 +405,38 @@ void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
         const float per_split = 1.f / even;
         for (int i = 0; i < a->n; ++i) live += 1 + static_cast<int>(static_cast<float>(lens[i] - 1) * per_split);
       }
-      const double wgs = groups * live;
       const double tiles = static_cast<double>(even < longest ? even : longest) / unit;
-      const double busy = (wgs < slots ? wgs : slots) * waves;
-      const double rate = busy * 36 * dim / 6.2e6, issue = 0.65 * latency * busy / 1024;
-      const double alone = latency > issue ? latency : issue, start = waves == 8 ? 2.8 : 2.2;
-      const double one = start + (tiles > 1 ? tiles : 1) * (alone > rate ? alone : rate);
-      double cost = one;
-      if (wgs > 3 * slots) {
-        const double sum = groups * total / unit, most = wgs * start + sum * alone;
-        cost = ((most > sum * rate ? most : sum * rate) + 0.5 * wgs * start) / slots + 0.25 * one;
-      } else if (wgs > slots) {
-        cost = one * (wgs > 2 * slots ? 2.5 : 1.8);
-      }
-      if (n > 1) cost += 2.5 + 0.5 * ((n + 15) / 16) + 8. * a->n * a->p.heads * n * a->rows * (dim + 2) / 6.2e6;
-      if (cost < best) {
-        best = cost;
-        a->waves = waves, a->split = even, a->splits = (longest + even - 1) / even;
+      for (int nb = 1; nb <= 2; ++nb) {
+        const int per = 512 / dim * nb, blocks = (a->rows + per - 1) / per;
+        // (two blocks' operands are more registers than fp32 queries, three parts, and 256 channels leave)
+        if (nb == 2 && (a->rows <= per / 2 || dtype == TSATTN_F32 || dim == 256)) break;
+        const double latency = 0.2 + (nb == 2 ? 0.068 : 0.031) * (dim / 16) * parts;
+        const double slots = waves == 8 ? 256. : nb == 2 || dim == 256 ? 512. : 768.;
+        const double groups = static_cast<double>(a->p.heads) * blocks, wgs = groups * live;
+        const double busy = (wgs < slots ? wgs : slots) * waves;
+        const double rate = busy * 36 * dim / 7.3e6, issue = 0.62 * latency * busy / 1024;
+        const double alone = latency > issue ? latency : issue, start = waves == 8 ? 2.5 : 2.3;
+        const double one = start + (tiles > 1 ? tiles : 1) * (alone > rate ? alone : rate);
+        double cost = one;
+        if (wgs > 3 * slots) {
+          const double sum = groups * total / unit, most = wgs * start + sum * alone;
+          cost = ((most > sum * rate ? most : sum * rate) + 0.3 * wgs * start) / slots + 0.15 * one;
+        } else if (wgs > slots) {
+          cost = one * (1.6 + 0.52 * (wgs / slots - 1));
+        }
+        if (n > 1) cost += 2.1 + 0.5 * ((n + 15) / 16) + 8. * a->n * a->p.heads * n * a->rows * (dim + 2) / 7.3e6;
+        if (cost < best) {
+          best = cost;
+          a->columns = nb, a->blocks = blocks, a->waves = waves;
+          a->split = even, a->splits = (longest + even - 1) / even;
+        }
       }
     }
   }
 }
 
 hipError_t launch_attend4(const Attend4 &a, int dtype, hipStream_t st) {
-  const int dim = a.p.dim, nb = column_blocks(dtype, dim, a.rows);
+  const int dim = a.p.dim;
   const dim3 grid(a.p.heads * a.blocks, a.splits, a.n);
   auto launch = [&](auto t, auto g) {
     using T = decltype(t);
@@ -445,7 +446,7 @@ hipError_t launch_attend4(const Attend4 &a, int dtype, hipStream_t st) {
       Probe pr_("attend4", st);
       auto run = [&](auto n) {
         constexpr int NB = decltype(n)::value;
-        if constexpr (!(f32 && G == 8)) {
+        if constexpr (G < 8 || std::is_same_v<T, bf16>) {
           if (a.waves == 8) {
             attend4_kernel<T, G, NB, 8><<<grid, dim3(512), 0, st>>>(a);
             return;
@@ -454,7 +455,7 @@ hipError_t launch_attend4(const Attend4 &a, int dtype, hipStream_t st) {
         attend4_kernel<T, G, NB, 4><<<grid, dim3(256), 0, st>>>(a);
       };
       if constexpr (!f32 && G < 8) {
-        if (nb == 2) run(std::integral_constant<int, 2>{});
+        if (a.columns == 2) run(std::integral_constant<int, 2>{});
         else run(std::integral_constant<int, 1>{});
       } else {
         run(std::integral_constant<int, 1>{});

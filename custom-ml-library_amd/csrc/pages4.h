@@ -119,12 +119,12 @@ struct Attend4 {
   const void *cos, *sin;  // rotate the queries; or NULL
   int n, rep, len_q, rows, causal;
   int split, splits;      // positions a split (a multiple of 32), splits of the longest sequence
-  int waves, blocks;      // of a workgroup; workgroups a KV head's rows take
+  int columns, waves, blocks;  // column blocks (1 or 2) and waves of a workgroup; workgroups a KV head's rows take
   float sl, sign;         // |scale| * log2(e) and the scale's sign, with the queries; 1 and 0 for no scale
   FastDiv by_len_q;
   Seqs s;
 };
-// Fills split, splits, waves and blocks in for the sequences' lengths.
+// Fills split, splits, columns, waves and blocks in for the sequences' lengths.
 void plan_attend4(Attend4 *a, int dtype, const int32_t *lens);
 hipError_t launch_attend4(const Attend4 &a, int dtype, hipStream_t st);
 
