@@ -35,11 +35,12 @@ def _reads_codes(rows: int, heads: int, dim: int, wide: bool, lens) -> bool:
     of ``lens``.  Its time grows with rows and positions; dequantising once and attending on the
     matrix cores costs mostly host time, per run of rows of one length, but fp32's kernel waits on
     every key of one row block.  Microseconds, codes / dequantised, 8 KV heads of D128 over 8000 positions: bf16 64
-    rows 32 / 53, 128 51 / 54, 256 80 / 53, 1024 247 / 60; fp32 1024 rows 420 / 1125; over 500
-    positions bf16 1024 rows 25 / 49.  2 heads of D64 over 8000: 1024 rows 34 / 53."""
+    rows 28 / 57, 128 42 / 57, 256 74 / 57, 1024 231 / 61; fp32 1024 rows 357 / 1122; over 500
+    positions bf16 1024 rows 26 / 52.  2 heads of D64 over 8000: 1024 rows 33 / 56, fp32 43 / 170;
+    12 heads of D32, fp32 896 rows 73 / 173."""
     size = (dim / 128) ** 1.5
     codes = 12 + (6.4e-6 if wide else 4e-6) * size * rows * heads * int(lens.sum())
-    whole = 50 * len(_runs(lens)) + (0.14 * (dim / 128) ** 3 * int(lens.max()) if wide else 0)
+    whole = 50 * len(_runs(lens)) + ((0.14 if dim == 128 else 0.02) * int(lens.max()) if wide else 0)
     return codes <= whole
 
 
