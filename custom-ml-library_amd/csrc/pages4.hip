@@ -159,7 +159,8 @@ __device__ __forceinline__ void load_words(const char *from, int lane, uint32_t 
 // A load takes whole rows, PPR lanes of 8 channels a row, so that four neighbouring
 // lanes make a group and the angles' loads take whole lines of their tables too (four
 // 64-byte pieces a row from the operand order's lanes: 44 us where this takes 38,
-// 4 x 8 heads x 8192 positions of D128 in bf16, rotated).  Codes and scales then cross
+// 4 x 8 heads x 8192 positions of D128 in bf16, rotated: 172 MB at 4.5 TB/s, where a
+// large copy reaches 4.9).  Codes and scales then cross
 // the wave through LDS into operand order; values' words, one channel of eight keys
 // each, take a transpose in each quad of lanes and a second trip.  A tile that is
 // only partly new keeps its other positions: keys' words belong to one position each,
@@ -332,7 +333,8 @@ __device__ __forceinline__ void store8(T *p, uint32_t w, float s, bool live) {
 
 // The values of positions first .. first + len - 1 of every sequence into k, v
 // [n, heads, len, D], zero past its length.  One wave a tile, head and side;
-// values' words go the append's way back.
+// values' words go the append's way back.  Bound by memory, most of it what is
+// written: 4 x 8 heads x 8192 positions of D128 in bf16, 172 MB, 29 us, 5.9 TB/s.
 template <typename T, int G>
 __global__ __launch_bounds__(NT) void read_kernel(ReadArgs ra) {
   constexpr int D = 32 * G, W = 2 * G;
@@ -390,7 +392,9 @@ struct ApplyArgs {
   int32_t src[kMoves], dst[kMoves], at[kMoves], value[kMoves];
 };
 
-// Page copies, blockIdx.y's share of each: 16 bytes a lane, four loads in flight.
+// Page copies, blockIdx.y's share of each: 16 bytes a lane, four loads in flight.  A
+// launch of 168 pages of 73,728 bytes takes 7.2 us (3.3 TB/s), one of a few pages the
+// launch's own 3; what a call has to copy is shorter than a second kernel for the table.
 // The row of blocks past them writes table entries (whose pages the stream's next
 // kernel reads: none here does).
 __global__ __launch_bounds__(NT) void apply_kernel(ApplyArgs a) {

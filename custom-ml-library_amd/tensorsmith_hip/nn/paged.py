@@ -30,6 +30,7 @@ from ..device import launch
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
 from .attention import _dtype_code, _rope_rows, rope_tables, scaled_dot_product_attention
 
+
 def _reads_codes(rows: int, heads: int, dim: int, wide: bool, lens) -> bool:
     """Whether attention reads the codes themselves: ``rows`` query rows per KV head over sequences
     of ``lens``.  Its time grows with rows and positions; dequantising once and attending on the
