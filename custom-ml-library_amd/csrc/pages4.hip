@@ -323,21 +323,26 @@ __device__ __forceinline__ void store8(T *p, uint32_t w, float s, bool live) {
     y[i][1] = live ? y[i][1] * s : 0.f;
   }
   if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<u32x4 *>(p) = u32x4{pack2<T>(y[0][0], y[0][1]), pack2<T>(y[1][0], y[1][1]),
-                                          pack2<T>(y[2][0], y[2][1]), pack2<T>(y[3][0], y[3][1])};
+    __builtin_nontemporal_store(u32x4{pack2<T>(y[0][0], y[0][1]), pack2<T>(y[1][0], y[1][1]),
+                                      pack2<T>(y[2][0], y[2][1]), pack2<T>(y[3][0], y[3][1])},
+                                reinterpret_cast<u32x4 *>(p));
   } else {
-    reinterpret_cast<f32x4 *>(p)[0] = f32x4{y[0][0], y[0][1], y[1][0], y[1][1]};
-    reinterpret_cast<f32x4 *>(p)[1] = f32x4{y[2][0], y[2][1], y[3][0], y[3][1]};
+    __builtin_nontemporal_store(f32x4{y[0][0], y[0][1], y[1][0], y[1][1]}, reinterpret_cast<f32x4 *>(p));
+    __builtin_nontemporal_store(f32x4{y[2][0], y[2][1], y[3][0], y[3][1]}, reinterpret_cast<f32x4 *>(p) + 1);
   }
 }
 
 // The values of positions first .. first + len - 1 of every sequence into k, v
-// [n, heads, len, D], zero past its length.  One wave a tile, head and side;
-// values' words go the append's way back.  Bound by memory, most of it what is
-// written: 4 x 8 heads x 8192 positions of D128 in bf16, 172 MB, 29 us, 5.9 TB/s.
+// [n, heads, len, D], zero past its length.  One wave a tile, head and side; the words
+// go the append's way back, so that a store takes whole rows.  Bound by memory, most of
+// it what is written, which nothing here reads again (stored past the caches): 4 x 8
+// heads x 8192 positions of D128 in bf16, 172 MB, 27 us, 6.4 TB/s; 16 x 8 heads x 4001,
+// 337 MB, 51 us, 6.6 TB/s (64 with ordinary stores, 82 with the operand order's 64-byte
+// pieces of rows).
 template <typename T, int G>
 __global__ __launch_bounds__(NT) void read_kernel(ReadArgs ra) {
   constexpr int D = 32 * G, W = 2 * G;
+  constexpr int PPR = D / 8, KPI = 64 / PPR;  // pieces a row, rows a store
   const RowArgs &a = ra.r;
   __shared__ __attribute__((aligned(16))) char lds[NW][16 * D];
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
@@ -352,6 +357,7 @@ __global__ __launch_bounds__(NT) void read_kernel(ReadArgs ra) {
   if (h >= a.p.heads || first >= a.len) return;                   // (a whole wave; no barrier follows)
   const View &v = values ? a.v : a.k;
   T *out = static_cast<T *>(const_cast<void *>(v.data)) + b * v.s0 + h * v.s1;
+  const int piece = lane % PPR, sub = lane / PPR;
   const bool held = tile * kTile < n;  // (a tile past the length may have no page)
   uint32_t word[W] = {};
   float sc[W] = {};
@@ -360,26 +366,37 @@ __global__ __launch_bounds__(NT) void read_kernel(ReadArgs ra) {
     load_words<G>(base + (values ? 16 * D : 0), lane, word);
     const uint16_t *sfrom = reinterpret_cast<const uint16_t *>(base + (values ? 34 : 32) * D);
 #pragma unroll
-    for (int w = 0; w < W; ++w) sc[w] = from_bf16(sfrom[scale4<G>(16 * (w / G) + c, w % G)]);
-  }
-  if (values && held) {  // to keys' words
+    for (int w = 0; w < W; ++w) sc[w] = from_bf16(sfrom[scale4<G>(KPI * w + sub, piece >> 2)]);
     char *mine = lds[wv];
+    if (values) {  // to keys' words
+      store_words<G>(mine, lane, word);
+      wait_lgkm0();  // (own wave's writes)
+      __builtin_amdgcn_sched_barrier(0);
+      const Transpose tr(lane);
+#pragma unroll
+      for (int ks = 0; ks < G; ++ks) {
+        word[ks] = *reinterpret_cast<const uint32_t *>(mine + value_at<G>(c, g, ks, 0));
+        word[G + ks] = *reinterpret_cast<const uint32_t *>(mine + value_at<G>(c, g, ks, 1));
+        tr.to_keys(word[ks], word[G + ks]);
+      }
+      wait_lgkm0();  // (read before the next writes)
+      __builtin_amdgcn_sched_barrier(0);
+    }
     store_words<G>(mine, lane, word);
     wait_lgkm0();  // (own wave's writes)
     __builtin_amdgcn_sched_barrier(0);
-    const Transpose tr(lane);
 #pragma unroll
-    for (int ks = 0; ks < G; ++ks) {
-      word[ks] = *reinterpret_cast<const uint32_t *>(mine + value_at<G>(c, g, ks, 0));
-      word[G + ks] = *reinterpret_cast<const uint32_t *>(mine + value_at<G>(c, g, ks, 1));
-      tr.to_keys(word[ks], word[G + ks]);
+    for (int w = 0; w < W; ++w) {
+      const int key = KPI * w + sub;
+      word[w] = *reinterpret_cast<const uint32_t *>(
+          mine + word4<G>((key >> 4) * G + (piece >> 2), 16 * (piece & 3) + (key & 15)));
     }
   }
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    const int key = 16 * (w / G) + c, t = first + key;
+    const int key = KPI * w + sub, t = first + key;
     if (t < 0 || t >= a.len) continue;
-    store8<T>(out + static_cast<int64_t>(t) * v.s2 + 32 * (w % G) + 8 * g, word[w], sc[w], tile * kTile + key < n);
+    store8<T>(out + static_cast<int64_t>(t) * v.s2 + 8 * piece, word[w], sc[w], tile * kTile + key < n);
   }
 }
 
