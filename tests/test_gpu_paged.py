@@ -238,6 +238,30 @@ def test_attention_matches_float64(case):
     assert torch.equal(got, nn.paged_attention(wrap(off), cache, is_causal=causal)._data)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch,hkv,rep,steps,keys,d", [
+    (16, 8, 4, 25, 40, 32), (24, 2, 4, 25, 500, 32), (1, 8, 4, 16, 4000, 32), (24, 1, 1, 1, 4000, 32),
+    (8, 8, 4, 25, 40, 64), (24, 1, 4, 25, 500, 64), (1, 8, 4, 16, 4000, 64), (1, 1, 8, 8, 2500, 64),
+    (4, 8, 4, 25, 40, 128), (24, 2, 4, 25, 300, 128), (1, 4, 8, 8, 1500, 128), (1, 4, 4, 16, 2500, 128),
+    (1, 1, 1, 1, 200, 32), (1, 1, 1, 1, 2500, 32), (1, 1, 1, 1, 200, 64), (1, 1, 1, 1, 1500, 64),
+    (1, 1, 1, 1, 200, 128), (1, 1, 1, 1, 1000, 128), (1, 1, 1, 1, 200, 256), (1, 1, 4, 25, 1500, 256),
+])
+def test_workgroups_of_every_make(batch, hkv, rep, steps, keys, d, dtype):
+    """Shapes over which the plan takes one and two column blocks, four and eight waves, one split
+    and several, for every head dim that has them; over the codes, whatever the rows' number."""
+    say("paged workgroups", batch, hkv, rep, steps, keys, d, dtype)
+    gen = seeded(keys + d)
+    cache = nn.PagedKVCache(batch, hkv, d, keys, device="hip", dtype=dtype)
+    k, v = (draw(gen, batch, hkv, keys, d, dtype=dtype) for _ in range(2))
+    cache.append(wrap(k), wrap(v))
+    lens = [keys - i % 3 * (keys // 7) for i in range(batch)]
+    cache.truncate(lens)
+    q = draw(gen, batch, hkv * rep, steps, d, dtype=dtype)
+    want, tol = reference(q, stored(k), stored(v), lens, True, 1 / math.sqrt(d), False)
+    with patch.object(P, "_reads_codes", return_value=True):
+        check(nn.paged_attention(wrap(q), cache)._data, want, tol, dtype)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_any_scale(scale, dtype):
