@@ -248,7 +248,7 @@ class PagedKVCache:
             if rotary_base <= 0 or not math.isfinite(rotary_base):
                 raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
             cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
-        k, v = (_rows(t._data.to(self.dtype)) for t in (key, value))
+        k, v = (_rows(t if t.dtype == self.dtype else t.to(self.dtype)) for t in (key._data, value._data))
         core._eager(self._rows, steps)
         core.grow(len(lens), self._rows_at, steps)
         try:
@@ -295,12 +295,12 @@ class PagedKVCache:
             raise ValueError("the last positions read must be between one and the shortest row's length")
         steps = int(lens.max()) if last is None else last
         first = np.zeros_like(lens) if last is None else lens - np.int32(last)
-        shape, dev = (len(lens), core.heads, steps, core.dim), core.pool.device
-        out = [torch.empty(shape, dtype=self.dtype, device=dev) for _ in range(2)]
+        k = torch.empty((len(lens), core.heads, steps, core.dim), dtype=self.dtype, device=core.pool.device)
+        v = torch.empty_like(k)
         if steps:
             _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
-                              _view(out[0]), _view(out[1]), self._rows_at, lens_at, first.ctypes.data), "paged read")
-        return tuple(Tensor(x, device=core.device) for x in out)
+                              _view(k), _view(v), self._rows_at, lens_at, first.ctypes.data), "paged read")
+        return Tensor._leaf(k, core.device), Tensor._leaf(v, core.device)
 
     # -- rows and pages -------------------------------------------------------
 

@@ -212,6 +212,14 @@ class Tensor:
         self._graph_freed = False
 
     @classmethod
+    def _leaf(cls, data: Any, device: Device) -> Tensor:
+        """A tensor over an array of the backend that is on ``device`` already."""
+        obj = cls.__new__(cls)
+        obj._data, obj.device, obj.requires_grad = data, device, False
+        obj._grad, obj._parents, obj._backward, obj._op, obj._graph_freed = None, (), None, "", False
+        return obj
+
+    @classmethod
     def _from_op(cls, data: Any, parents: tuple[Tensor, ...], backward: Backward, op: str) -> Tensor:
         obj = cls.__new__(cls)
         obj._data = data
