@@ -429,6 +429,7 @@ def decode_int8_cache(query: Tensor, cache, *, is_causal: bool, causal_offset: i
 
 
 _ROPE_TABLES: dict = {}
+_OUTGROWN: list = []  # shorter tables: a captured launch may read them still (together no longer than the newest)
 
 
 def _ROPE_KERNEL_DTYPES():
@@ -456,6 +457,8 @@ def rope_tables(base: float, dim: int, dtype, dev, length: int):
     angles = np.arange(0, n, dtype=np.float32)[:, None] * freqs[None, :]
     made = tuple(torch.from_numpy(np.ascontiguousarray(f(angles))).to(device=dev, dtype=dtype)
                  for f in (np.cos, np.sin))
+    if have is not None:
+        _OUTGROWN.append(have)
     _ROPE_TABLES[key] = made
     return made
 

@@ -440,6 +440,38 @@ def test_on_another_stream_and_captured():
     assert same(held(full)[0][:, :, 64:], stored(kt), BF16) and same(held(full)[1][:, :, :64], stored(v[:, :, :64]), BF16)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_a_captured_rotation_outlives_its_table(dtype):
+    """The tables of angles grow for longer rows; a captured call goes on reading its own."""
+    say("paged capture, longer tables", dtype)
+    gen, base = seeded(61), 41.0 if dtype == F32 else 43.0  # (no other test's tables)
+    cache = nn.PagedKVCache(2, 2, 64, 200, device="hip", dtype=dtype)
+    first = [draw(gen, 2, 2, 70, 64, dtype=dtype) for _ in range(2)]
+    new, q = draw(gen, 2, 2, 1, 64, dtype=dtype), draw(gen, 2, 4, 1, 64, dtype=dtype)
+    cache.append(*map(wrap, first), rotary_base=base)
+    cache.append(wrap(new), wrap(new), rotary_base=base)
+    want = nn.paged_attention(wrap(q), cache, rotary_base=base)._data
+    cache.truncate(70)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        nn.paged_attention(wrap(q), cache, rotary_base=base)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        cache.append(wrap(new), wrap(new), rotary_base=base)
+        out = nn.paged_attention(wrap(q), cache, rotary_base=base)._data
+    for n in (700, 3000, 9000):
+        far = nn.PagedKVCache(1, 2, 64, n, device="hip", dtype=dtype)
+        x = draw(gen, 1, 2, n, 64, dtype=dtype)
+        far.append(wrap(x), wrap(x), rotary_base=base)
+        junk = [torch.full((m, 32), 9.0, dtype=dtype, device="cuda") for m in (256, 256, 700, 700)]
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), n
+        del junk, far
+
+
 # -- layers and models -------------------------------------------------------------
 
 

@@ -8,8 +8,10 @@ they are told to copy, set and append has to leave every row its own tags.
 from __future__ import annotations
 
 import ctypes
+import gc
 import importlib
 import random
+import weakref
 from contextlib import ExitStack, nullcontext
 from unittest.mock import patch
 
@@ -358,6 +360,17 @@ def test_the_prompt_rule():
             (4096, 8, 128, True, lens(32000), False), (32, 4, 64, False, lens(0), True)):
         assert P._reads_codes(rows, heads, dim, wide, n) is codes, (rows, heads, dim, wide, n)
     assert P._runs(lens(3, 3, 5, 3)) == [2, 3, 4] and P._runs(lens(7)) == [1]
+
+
+def test_outgrown_rope_tables_stay():
+    """A captured append reads the table that it was captured with."""
+    A = importlib.import_module("tensorsmith_hip.nn.attention")
+    make = lambda n: A.rope_tables(77.0, 32, torch.float32, torch.device("cpu"), n)  # noqa: E731
+    kept = [(weakref.ref(t), t.clone()) for t in make(10)]
+    long = make(3000)
+    gc.collect()
+    assert all(ref() is not None and torch.equal(ref(), old) for ref, old in kept)
+    assert all(torch.equal(t[:len(old)], old) for t, (_, old) in zip(long, kept)) and make(20) is long
 
 
 # -- the C entry points: every refusal comes before a launch --------------------------
