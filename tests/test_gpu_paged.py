@@ -262,6 +262,23 @@ def test_workgroups_of_every_make(batch, hkv, rep, steps, keys, d, dtype):
         check(nn.paged_attention(wrap(q), cache)._data, want, tol, dtype)
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 32), (F32, 64)])
+def test_rows_of_hundreds_of_thousands(dtype, d):
+    """More splits than the second kernel has loads in flight, beside a row of one position."""
+    say("paged long rows", dtype, d)
+    gen, n = seeded(d), 300_001
+    cache = nn.PagedKVCache(2, 1, d, n, device="hip", dtype=dtype, page_size=4096, num_pages=75)
+    k, v = (draw(gen, 1, 1, n, d, dtype=dtype) for _ in range(2))
+    cache.rows([0]).append(wrap(k), wrap(v))
+    cache.rows([1]).append(wrap(k[:, :, :1]), wrap(v[:, :, :1]))
+    assert cache.pages_in_use == 75
+    q = draw(gen, 2, 2, 1, d, dtype=dtype, scale=3.0)
+    sk, sv = (stored(x).expand(2, -1, -1, -1) for x in (k, v))
+    want, tol = reference(q, sk, sv, (n, 1), True, 1 / math.sqrt(d), False)
+    check(nn.paged_attention(wrap(q), cache)._data, want, tol, dtype)
+    assert same(cache.rows([0]).get(last=5000)[0]._data, sk[:1, :, -5000:], dtype)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_any_scale(scale, dtype):
