@@ -5,16 +5,21 @@
 //   S[j] = sum_s sk[j, s] (q_s . c_j,s),   P = softmax of scale S,
 //   O_s = sum_j (P[j] sv[j, s]) c_j,s      for each group s of 32 channels:
 // the scales stay outside the matrix products, so no dequantised value is formed.
-// The groups take columns of the 16-wide B operand beside the rows: column
-// c = G r + s holds row r's group s, zero in the other groups' channels.  One
-// chain of MFMAs then sums each group of each row by itself, a score takes one
-// multiply by its key's scale and a sum over G neighbouring lanes, and the value
-// product takes P sv of its own column: a lane scales 8 probabilities a tile
-// where it would scale 8 G otherwise.  The price is in MFMAs, which have time (a
-// value block is multiplied for all columns and used by those of its group).
+// Where a KV head has few rows, the groups take columns of the 16-wide B operand beside
+// them: column c = G r + s holds row r's group s, zero in the other groups' channels.
+// One chain of MFMAs then sums each group of each row by itself, a score takes one
+// multiply by its key's scale and a sum over G neighbouring lanes, and the value product
+// takes P sv of its own column: a lane scales 8 probabilities a tile where it would
+// scale 8 G otherwise.  The price is in MFMAs, which have time (a value block is
+// multiplied for all columns and used by those of its group).  Where there are many
+// (WIDE), a column is a row: a key's scales multiply the groups' scores one after the
+// other, and values are dequantised, exactly, as they go to the matrix cores.  Scales
+// reach the lanes from the one that loaded them.  In the tiles that some rows see and
+// others do not, a value's scale goes to the probabilities instead: NaN there is
+// no business of a row that does not see it.
 //
-// Precision.  q enters exactly: bf16 in one part, f16 in two, fp32 in three. P sv
-// enters as two bf16 parts (2^-17 of each), for fp32 as three (2^-25).
+// Precision.  q enters exactly: bf16 in one part, f16 in two, fp32 in three.  P sv
+// (WIDE: P) enters as two bf16 parts (2^-17 of each), for fp32 as three (2^-25).
 //
 // A wave works alone on every fourth or eighth tile of its split, two tiles ahead in
 // registers, straight from memory in operand order (pages4.h); waves merge in LDS,
@@ -25,7 +30,10 @@
 // time and 56% of the vector units'.  Middling ones by the start of a workgroup and a
 // tile's latency: 64 x 8 KV heads over 1025, 4 rows (f16, D128), 77 MB, 18.4 us, of
 // which 4 pass before the second tile.  Small ones by latency alone: 8 heads over 200,
-// 4 us.
+// 4 us.  Many rows by the vector units (levels, scales and roundings; a tile of 32
+// positions and 16 rows takes about 1.9 us alone): 3 sequences of 2 heads up to 15686,
+// 496 rows of fp32 D256, 32.8 GFLOP, 194 us, 169 TFLOP/s, where groups as columns took
+// 808; 8 heads over 8000, 1024 rows of fp32 D128 160 (382).
 #include "pages4.h"
 #include "rope_math.h"
 
@@ -69,6 +77,30 @@ __device__ __forceinline__ float scaled_sum(float a, float x) {
   return y;
 }
 
+// The value of lane S of the 16 that share a lane's g.
+template <int S>
+__device__ __forceinline__ float from_lane(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x150 + S, 0xF, 0xF, true));  // row_newbcast
+}
+
+// Eight codes, four bits each, times their keys' scales: exact in bf16.
+__device__ __forceinline__ u32x4 values_bf16(uint32_t w, const float (&s)[8]) {
+  const f32x2 y0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), y1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
+  const f32x2 y2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), y3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+  return u32x4{pack2<bf16>(y0[0] * s[0], y0[1] * s[1]), pack2<bf16>(y1[0] * s[2], y1[1] * s[3]),
+               pack2<bf16>(y2[0] * s[4], y2[1] * s[5]), pack2<bf16>(y3[0] * s[6], y3[1] * s[7])};
+}
+
+// f(integral constants 0 .. N - 1).
+template <int N, typename F>
+__device__ __forceinline__ void each(F &&f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
 // A lane's share of a tile: codes of keys and values, eight scales of each.
 template <int G>
 struct Held {
@@ -80,18 +112,20 @@ struct Held {
   __device__ __forceinline__ uint32_t vw(int w) const { return G == 1 ? v[0][w] : v[w >> 2][w & 3]; }
 };
 
-template <typename T, int G, int NB, int NWV>
-__global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 : 2)) void attend4_kernel(Attend4 a) {
+template <typename T, int G, int NB, int NWV, bool WIDE>
+__global__ __launch_bounds__(64 * NWV, (WIDE || (std::is_same_v<T, float> && G == 8) ? 1 : 2)) void attend4_kernel(Attend4 a) {
   constexpr int D = 32 * G, W = 2 * G, NQ = q_parts<T>(), NP = p_parts<T>();
-  constexpr int RB = 16 / G, ROWS = RB * NB;  // rows a column block, a workgroup
-  constexpr int LD = D + 4;                   // (rows of the merge start in different banks)
-  __shared__ __attribute__((aligned(16))) float part[NWV][ROWS][LD];
+  constexpr int RB = WIDE ? 16 : 16 / G, ROWS = RB * NB;  // rows a column block, a workgroup
+  constexpr int PIECES = WIDE ? G : 1;                    // of a row that a lane holds
+  constexpr int MR = WIDE ? 16 : ROWS, MD = WIDE && D > 128 ? 128 : D;  // rows, channels merged at a time
+  constexpr int LD = MD + 4;                              // (rows of the merge start in different banks)
+  __shared__ __attribute__((aligned(16))) float part[NWV][MR][LD];
   __shared__ float state[NWV][ROWS][2];  // their maximum and sum
 
   const int b = blockIdx.z, split = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rl = c / G, grp = c % G;  // the lane's row in its column block, its group
+  const int rl = WIDE ? c : c / G, grp = c % G;  // the lane's row in its column block, its group
   const int len = a.s.len[b], trow = a.s.row[b];
   const int hk = a.blocks == 1 ? blockIdx.x : blockIdx.x / a.blocks;
   const int row0 = (blockIdx.x - hk * a.blocks) * ROWS;
@@ -115,7 +149,7 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
 
   // the queries' rows, on their way first: row r of the block, channels 32 grp + 8 g .. + 7
   constexpr int QW = sizeof(T) / 2;  // 16-byte loads a row piece
-  u32x4 raw[NB][QW];
+  u32x4 raw[NB][PIECES][QW];
   int qpos[NB];  // the row's query's number
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -123,9 +157,11 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
     const int rr = fdiv(r, a.by_len_q);
     qpos[nb] = r - rr * a.len_q;
     const T *qp = static_cast<const T *>(a.q.data) + b * a.q.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.q.s1 +
-                  qpos[nb] * a.q.s2 + 32 * grp + 8 * g;
+                  qpos[nb] * a.q.s2 + (WIDE ? 0 : 32 * grp) + 8 * g;
 #pragma unroll
-    for (int i = 0; i < QW; ++i) raw[nb][i] = reinterpret_cast<const u32x4 *>(qp)[i];
+    for (int e = 0; e < PIECES; ++e)
+#pragma unroll
+      for (int i = 0; i < QW; ++i) raw[nb][e][i] = reinterpret_cast<const u32x4 *>(qp + 32 * e)[i];
   }
   // the wave's page numbers, lane t's for its tile t: one load, and none in the loop
   // (lanes past the wave's tiles: the split's last, as the table need not go on)
@@ -145,43 +181,51 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
   if (mine > 0) load(x0, 0);
   if (mine > 1) load(x1, 1);
 
-  // the B operand: the row's piece in k-step grp, zero in the others
+  // the B operand: the row's pieces in their k-steps; of a lane's one piece, zero in the others
   u32x4 qf[NB][NQ][G];
   int klim[NB];  // positions of the split that the row sees: [0, klim)
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const bool live = nb * RB + rl < live_rows;
-    T x[8];
-#pragma unroll
-    for (int i = 0; i < QW; ++i) {
-      const T *e = reinterpret_cast<const T *>(&raw[nb][i]);
-#pragma unroll
-      for (int j = 0; j < 8 / QW; ++j) x[i * (8 / QW) + j] = e[j];
-    }
     const int at = len - a.len_q + qpos[nb];  // the query's position
-    if (a.cos) {
-      const int64_t e = static_cast<int64_t>(max(at, 0)) * (D / 2) + 16 * grp + 4 * g;
-      T cw[4], sw[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cw[i] = static_cast<const T *>(a.cos)[e + i], sw[i] = static_cast<const T *>(a.sin)[e + i];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) rotate_pair(x[2 * i], x[2 * i + 1], cw[i], sw[i], false);
-    }
     klim[nb] = a.causal ? min(keys, at + 1 - begin) : keys;
-    uint32_t pt[NQ][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t two[NQ];
-      split_bf16<NQ>(live ? static_cast<float>(x[2 * i]) * a.sign : 0.f,
-                     live ? static_cast<float>(x[2 * i + 1]) * a.sign : 0.f, two);
+    for (int piece = 0; piece < PIECES; ++piece) {
+      T x[8];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) pt[n][i] = two[n];
+      for (int i = 0; i < QW; ++i) {
+        const T *e = reinterpret_cast<const T *>(&raw[nb][piece][i]);
+#pragma unroll
+        for (int j = 0; j < 8 / QW; ++j) x[i * (8 / QW) + j] = e[j];
+      }
+      if (a.cos) {
+        const int64_t e = static_cast<int64_t>(max(at, 0)) * (D / 2) + 16 * (WIDE ? piece : grp) + 4 * g;
+        T cw[4], sw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cw[i] = static_cast<const T *>(a.cos)[e + i], sw[i] = static_cast<const T *>(a.sin)[e + i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rotate_pair(x[2 * i], x[2 * i + 1], cw[i], sw[i], false);
+      }
+      uint32_t pt[NQ][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t two[NQ];
+        split_bf16<NQ>(live ? static_cast<float>(x[2 * i]) * a.sign : 0.f,
+                       live ? static_cast<float>(x[2 * i + 1]) * a.sign : 0.f, two);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) pt[n][i] = two[n];
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const u32x4 y{pt[n][0], pt[n][1], pt[n][2], pt[n][3]};
+        if constexpr (WIDE) {
+          qf[nb][n][piece] = y;
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < G; ++ks) qf[nb][n][ks] = ks == grp ? y : u32x4{0, 0, 0, 0};
+        }
+      }
     }
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int ks = 0; ks < G; ++ks)
-        qf[nb][n][ks] = ks == grp ? u32x4{pt[n][0], pt[n][1], pt[n][2], pt[n][3]} : u32x4{0, 0, 0, 0};
   }
   // tiles before `edge` are seen whole by every row
   const int edge = (a.causal ? min(keys, len - a.len_q + 1 - begin) : keys) / kTile;
@@ -199,42 +243,80 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
   // value blocks.
   auto compute = [&](const Held<G> &t4, int t) __attribute__((always_inline)) {
     const int tile = w + NWV * t;  // of the split
-    f32x4 s[NB][2];
+    float ksc[8], vsc[8];  // the scales of the lane's group, keys 4 g .. + 3 and 16 + 4 g .. + 3
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = f32x4{};
-#pragma unroll
-    for (int ks = 0; ks < G; ++ks) {
-      u32x4 kf[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) kf[kb] = levels_bf16(t4.kw(kb * G + ks));
+    for (int i = 0; i < 8; i += 2) {
+      ksc[i] = __builtin_bit_cast(float, t4.ks[i >> 1] << 16);
+      ksc[i + 1] = __builtin_bit_cast(float, t4.ks[i >> 1] & 0xFFFF0000u);
+      vsc[i] = __builtin_bit_cast(float, t4.vs[i >> 1] << 16);
+      vsc[i + 1] = __builtin_bit_cast(float, t4.vs[i >> 1] & 0xFFFF0000u);
+    }
+    float x[NB][8];  // the scores
+    if constexpr (WIDE) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+        for (int i = 0; i < 8; ++i) x[nb][i] = 0.f;
+      each<G>([&](auto group) __attribute__((always_inline)) {
+        constexpr int ks = decltype(group)::value;
+        f32x4 s[NB][2];
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) s[nb][kb] = mfma16<bf16>(kf[kb], qf[nb][n][ks], s[nb][kb]);
+        for (int kb = 0; kb < 2; ++kb) {
+          const u32x4 kf = levels_bf16(t4.kw(kb * G + ks));
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            s[nb][kb] = f32x4{};
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) s[nb][kb] = mfma16<bf16>(kf, qf[nb][n][ks], s[nb][kb]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float sc = from_lane<ks>(ksc[i]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) x[nb][i] = fmaf(s[nb][i >> 2][i & 3], sc, x[nb][i]);
+        }
+      });
+    } else {
+      f32x4 s[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = f32x4{};
+#pragma unroll
+      for (int ks = 0; ks < G; ++ks) {
+        u32x4 kf[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) kf[kb] = levels_bf16(t4.kw(kb * G + ks));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[nb][kb] = mfma16<bf16>(kf[kb], qf[nb][n][ks], s[nb][kb]);
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[nb][i] = scaled_sum<G>(s[nb][i >> 2][i & 3], ksc[i]);
     }
+    const bool whole = tile < edge;
     u32x4 pb[NB][NP];
+    float pr[NB][8];   // WIDE: the probabilities
+    uint32_t seen[NB]; // and, of a tile that is not whole, which the row sees
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      float x[8], vs[8];
+      float vs[8];
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const uint32_t k2 = t4.ks[i >> 1], v2 = t4.vs[i >> 1];
-        x[i] = scaled_sum<G>(s[nb][i >> 2][i & 3], __builtin_bit_cast(float, k2 << 16));
-        x[i + 1] = scaled_sum<G>(s[nb][i >> 2][(i & 3) + 1], __builtin_bit_cast(float, k2 & 0xFFFF0000u));
-        vs[i] = __builtin_bit_cast(float, v2 << 16);
-        vs[i + 1] = __builtin_bit_cast(float, v2 & 0xFFFF0000u);
-      }
-      if (tile >= edge) {  // what a row does not see weighs nothing, whatever its scales are
+      for (int i = 0; i < 8; ++i) vs[i] = vsc[i];
+      seen[nb] = 0xFFu;
+      if (!whole) {  // what a row does not see weighs nothing, whatever its scales are
         const int lim = klim[nb] - tile * kTile - 4 * g;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (16 * (i >> 2) + (i & 3) >= lim) x[i] = -INFINITY, vs[i] = 0.f;
+          if (16 * (i >> 2) + (i & 3) >= lim) x[nb][i] = -INFINITY, vs[i] = 0.f, seen[nb] &= ~(1u << i);
       }
-      float mx = x[0];
+      float mx = x[nb][0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[nb][i]);
       mx = quad_row_max(mx) * a.sl;  // (sl > 0)
       if (__ballot(mx > m[nb]) != 0ull) {
         const float mn = fmaxf(m[nb], mx);
@@ -247,24 +329,59 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
       const float base = m[nb] == -INFINITY ? 0.f : -m[nb];
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        const float p0 = fast_exp2(fmaf(x[i], a.sl, base)), p1 = fast_exp2(fmaf(x[i + 1], a.sl, base));
+        const float p0 = fast_exp2(fmaf(x[nb][i], a.sl, base)), p1 = fast_exp2(fmaf(x[nb][i + 1], a.sl, base));
         l[nb] += p0 + p1;
+        pr[nb][i] = p0, pr[nb][i + 1] = p1;
         uint32_t two[NP];
-        split_bf16<NP>(p0 * vs[i], p1 * vs[i + 1], two);
+        split_bf16<NP>(WIDE ? p0 : p0 * vs[i], WIDE ? p1 : p1 * vs[i + 1], two);
 #pragma unroll
         for (int n = 0; n < NP; ++n) pb[nb][n][i >> 1] = two[n];
       }
     }
+    if (WIDE && !whole) {  // (a key that some rows see and others do not: its scale goes to the probabilities)
+      each<G>([&](auto group) __attribute__((always_inline)) {
+        constexpr int s = decltype(group)::value;
+        const u32x4 vf[2] = {levels_bf16(t4.vw(2 * s)), levels_bf16(t4.vw(2 * s + 1))};
+        float sc[8];
 #pragma unroll
-    for (int i = 0; i < W; i += 2) {
-      const u32x4 vf[2] = {levels_bf16(t4.vw(i)), levels_bf16(t4.vw(i + 1))};
+        for (int i = 0; i < 8; ++i) sc[i] = from_lane<s>(vsc[i]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          u32x4 ps[NP];
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            uint32_t two[NP];
+            split_bf16<NP>(seen[nb] >> i & 1 ? pr[nb][i] * sc[i] : 0.f,
+                           seen[nb] >> (i + 1) & 1 ? pr[nb][i + 1] * sc[i + 1] : 0.f, two);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) ps[n][i >> 1] = two[n];
+          }
+#pragma unroll
+          for (int n = 0; n < NP; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) oacc[nb][2 * s + e] = mfma16<bf16>(vf[e], ps[n], oacc[nb][2 * s + e]);
+        }
+      });
+      return;
+    }
+    each<G>([&](auto group) __attribute__((always_inline)) {
+      constexpr int i = 2 * decltype(group)::value;
+      u32x4 vf[2];
+      if constexpr (WIDE) {
+        float sc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = from_lane<i / 2>(vsc[j]);
+        vf[0] = values_bf16(t4.vw(i), sc), vf[1] = values_bf16(t4.vw(i + 1), sc);
+      } else {
+        vf[0] = levels_bf16(t4.vw(i)), vf[1] = levels_bf16(t4.vw(i + 1));
+      }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int n = 0; n < NP; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) oacc[nb][i + e] = mfma16<bf16>(vf[e], pb[nb][n], oacc[nb][i + e]);
-    }
+    });
   };
 
   for (int t = 0; t < mine; t += 2) {
@@ -276,53 +393,65 @@ __global__ __launch_bounds__(64 * NWV, (std::is_same_v<T, float> && G == 8 ? 1 :
     }
   }
 
-  // Merge the waves.  Lane (c, g) has row rl's channels 16 i + 4 g .. + 3 for the
-  // blocks i of its group; then a wave sums a row over the waves, PER channels a lane.
+  // Merge the waves, MR rows and MD channels at a time.  Lane (c, g) has row rl's
+  // channels 16 i + 4 g .. + 3 (for the blocks i of its group, unless WIDE); then a wave
+  // sums a row over the waves, PER channels a lane.
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     float lt = l[nb] + __shfl_xor(l[nb], 16, 64);
     lt += __shfl_xor(lt, 32, 64);
-    float *to = part[w][nb * RB + rl];
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      if (i / 2 == grp) *reinterpret_cast<f32x4 *>(to + 16 * i + 4 * g) = oacc[nb][i];
-    if (g == 0 && grp == 0) {
+    if (g == 0 && (WIDE || grp == 0)) {
       state[w][nb * RB + rl][0] = m[nb];
       state[w][nb * RB + rl][1] = lt;
     }
   }
-  __syncthreads();
-  constexpr int PER = D < 64 ? 1 : D / 64;
+  constexpr int PER = MD < 64 ? 1 : MD / 64;
   using Piece = std::conditional_t<PER == 1, float, std::conditional_t<PER == 2, f32x2, f32x4>>;
-  for (int r = w; r < live_rows; r += NWV) {
-    float mv[NWV], M = -INFINITY, total = 0.f, sum[PER] = {};
-    Piece x[NWV];
 #pragma unroll
-    for (int v = 0; v < NWV; ++v) {
-      mv[v] = state[v][r][0];
-      x[v] = *reinterpret_cast<const Piece *>(part[v][r] + (D < 64 ? lane & (D - 1) : PER * lane));
-    }
+  for (int r0 = 0; r0 < ROWS; r0 += MR) {
 #pragma unroll
-    for (int v = 0; v < NWV; ++v) M = fmaxf(M, mv[v]);
-    const float base = M == -INFINITY ? 0.f : M;
+    for (int d0 = 0; d0 < D; d0 += MD) {
+      if (r0 + d0 > 0) __syncthreads();  // (the rows and channels before are read)
 #pragma unroll
-    for (int v = 0; v < NWV; ++v) {
-      const float f = fast_exp2(mv[v] - base);
-      const float *e = reinterpret_cast<const float *>(&x[v]);
-      total = fmaf(state[v][r][1], f, total);
+      for (int nb = r0 / RB; nb < (r0 + MR) / RB; ++nb) {
+        float *to = part[w][nb * RB - r0 + rl];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum[i] = fmaf(e[i], f, sum[i]);
-    }
-    if (lane * PER < D) {
-      if (a.splits > 1) {
-        float *to = a.ws + ((static_cast<int64_t>(b * a.p.heads + hk) * a.splits + split) * a.rows + row0 + r) * (D + 2);
+        for (int i = 0; i < MD / 16; ++i)
+          if (WIDE || i / 2 == grp) *reinterpret_cast<f32x4 *>(to + 16 * i + 4 * g) = oacc[nb][d0 / 16 + i];
+      }
+      __syncthreads();
+      for (int r = r0 + w; r < min(r0 + MR, live_rows); r += NWV) {
+        float mv[NWV], M = -INFINITY, total = 0.f, sum[PER] = {};
+        Piece x[NWV];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) to[PER * lane + i] = sum[i];
-        if (lane == 0) to[D] = M, to[D + 1] = total;
-      } else {
-        T *to = out_row(r);
+        for (int v = 0; v < NWV; ++v) {
+          mv[v] = state[v][r][0];
+          x[v] = *reinterpret_cast<const Piece *>(part[v][r - r0] + (MD < 64 ? lane & (MD - 1) : PER * lane));
+        }
 #pragma unroll
-        for (int i = 0; i < PER; ++i) to[PER * lane + i] = static_cast<T>(total == 0.f ? 0.f : sum[i] / total);
+        for (int v = 0; v < NWV; ++v) M = fmaxf(M, mv[v]);
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int v = 0; v < NWV; ++v) {
+          const float f = fast_exp2(mv[v] - base);
+          const float *e = reinterpret_cast<const float *>(&x[v]);
+          total = fmaf(state[v][r][1], f, total);
+#pragma unroll
+          for (int i = 0; i < PER; ++i) sum[i] = fmaf(e[i], f, sum[i]);
+        }
+        if (lane * PER < MD) {
+          const int d = d0 + PER * lane;
+          if (a.splits > 1) {
+            float *to = a.ws + ((static_cast<int64_t>(b * a.p.heads + hk) * a.splits + split) * a.rows + row0 + r) * (D + 2);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) to[d + i] = sum[i];
+            if (d == 0) to[D] = M, to[D + 1] = total;
+          } else {
+            T *to = out_row(r);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) to[d + i] = static_cast<T>(total == 0.f ? 0.f : sum[i] / total);
+          }
+        }
       }
     }
   }
@@ -372,20 +501,22 @@ __global__ __launch_bounds__(64) void attend4_merge_kernel(Attend4 a) {
 
 }  // namespace
 
-// Column blocks and waves of a workgroup, and splits: those that a model of the time
-// likes best.  Two blocks read the cache once for twice the rows; one, where the
-// memory is not what a call waits for, has twice the workgroups.  Four waves (two or
-// three workgroups a CU) or eight, which take a CU by themselves.  In us: a workgroup's
-// prologue and merge 2.3 or 2.5; a tile of a wave the largest of its own latency (by its
-// MFMAs; bf16 D128 0.94 with one block, 1.8 with two, fp32 D128 1.7, bf16 D256 1.7), of the
-// issue slots of the waves beside it and of the memory's rate; where the workgroups do
-// not fit the chip at once, their rounds over it; the second kernel 2.6.  Its constants
-// are fitted to 34 shapes, of which it takes 4% longer than the best choice in the
-// mean.  Measured, what it picks and another: 7 sequences of 4 KV heads up to 4001, 20
-// rows of bf16 D128: one block and 7 splits 17.4, two and 8 19.1; 64 of 4 heads over
-// 2000, 16 rows: two blocks 42, one 53; 4 of 32 heads over 4000, f16 D128: eight waves
-// and 2 splits 19.0, four and 3 22.4; 3 of one head over 1500, fp32 D128: 12 splits 7.1,
-// one 13.1; 64 of 8 heads over 1025, 4 rows of f16 D128: one split 18.6, three 24.
+// How a workgroup is made -- columns of groups, one block of them or two, with four
+// waves (two or three workgroups a CU) or eight, which take a CU by themselves; or
+// columns of rows with four -- and splits: those that a model of the time likes best.
+// Two blocks read the cache once for twice the rows; one, where the memory is not what
+// a call waits for, has twice the workgroups.  In us: a workgroup's prologue and merge
+// 2.3 or 2.5, of rows 3.7 to 4.4; a tile of a wave the largest of its own latency (by
+// its products; bf16 D128 0.94 with one block, 1.8 with two, 1.8 of rows; fp32 D128 1.7,
+// of rows 2.0; bf16 D256 1.7, of rows 2.9), of the issue slots of the waves beside it and
+// of the memory's rate; where the workgroups do not fit the chip at once, their rounds
+// over it; the second kernel 2.6.  Its constants are fitted to 60 shapes, of which it
+// takes 3% longer than the best choice in the mean.  Measured, what it picks and
+// another: 7 sequences of 4 KV heads up to 4001, 20 rows of bf16 D128: rows 15.7, groups
+// in one block 17.4, in two 19.1; 8 of 8 heads over 8000, 16 rows: rows 32, groups 44;
+// 4 of 32 heads over 4000, f16 D128: eight waves and 2 splits 19.0, four and 3 22.4; 3 of
+// one head over 1500, fp32 D128: 12 splits 7.1, one 13.1; 64 of 8 heads over 1025, 4 rows
+// of f16 D128: one split 18.5, three 24.
 void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
   int64_t total = 0;
   int longest = 1;
@@ -413,16 +544,25 @@ void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
         for (int i = 0; i < a->n; ++i) live += 1 + static_cast<int>(static_cast<float>(lens[i] - 1) * per_split);
       }
       const double tiles = static_cast<double>(even < longest ? even : longest) / unit;
-      for (int nb = 1; nb <= 2; ++nb) {
-        const int per = 512 / dim * nb, blocks = (a->rows + per - 1) / per;
+      for (int make = 0; make < 3; ++make) {
+        const bool wide = make == 2;
+        const int nb = make == 1 ? 2 : 1, one_block = 512 / dim;
+        if (make && a->rows <= one_block) break;
         // (two blocks' operands are more registers than fp32 queries, three parts, and 256 channels leave)
-        if (nb == 2 && (a->rows <= per / 2 || dtype == TSATTN_F32 || dim == 256)) break;
-        const double latency = 0.2 + (nb == 2 ? 0.068 : 0.031) * (dim / 16) * parts;
-        const double slots = waves == 8 ? 256. : nb == 2 || dim == 256 ? 512. : 768.;
+        if (make == 1 && (dtype == TSATTN_F32 || dim == 256)) continue;
+        if (wide && (waves == 8 || dim == 32)) continue;  // (32 channels: a row is one group)
+        const int per = wide ? 16 : one_block * nb, blocks = (a->rows + per - 1) / per;
+        const double latency = wide      ? 0.76 + dim / 32 * (0.23 + 0.014 * parts)
+                               : nb == 2 ? 0.2 + 0.068 * (dim / 16) * parts
+                                         : 0.2 + 0.031 * (dim / 16) * parts;
+        const double start = wide ? 3.5 + 0.0034 * dim : waves == 8 ? 2.5 : 2.3;
+        const double slots = waves == 8 || (wide && dim == 256)             ? 256.
+                             : nb == 2 || dim == 256 || (wide && dim == 128) ? 512.
+                                                                            : 768.;
         const double groups = static_cast<double>(a->p.heads) * blocks, wgs = groups * live;
         const double busy = (wgs < slots ? wgs : slots) * waves;
         const double rate = busy * 36 * dim / 7.3e6, issue = 0.62 * latency * busy / 1024;
-        const double alone = latency > issue ? latency : issue, start = waves == 8 ? 2.5 : 2.3;
+        const double alone = latency > issue ? latency : issue;
         const double one = start + (tiles > 1 ? tiles : 1) * (alone > rate ? alone : rate);
         double cost = one;
         if (wgs > 3 * slots) {
@@ -434,7 +574,7 @@ void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
         if (n > 1) cost += 2.1 + 0.5 * ((n + 15) / 16) + 8. * a->n * a->p.heads * n * a->rows * (dim + 2) / 7.3e6;
         if (cost < best) {
           best = cost;
-          a->columns = nb, a->blocks = blocks, a->waves = waves;
+          a->wide = wide, a->columns = nb, a->blocks = blocks, a->waves = waves;
           a->split = even, a->splits = (longest + even - 1) / even;
         }
       }
@@ -455,13 +595,15 @@ hipError_t launch_attend4(const Attend4 &a, int dtype, hipStream_t st) {
         constexpr int NB = decltype(n)::value;
         if constexpr (G < 8 || std::is_same_v<T, bf16>) {
           if (a.waves == 8) {
-            attend4_kernel<T, G, NB, 8><<<grid, dim3(512), 0, st>>>(a);
+            attend4_kernel<T, G, NB, 8, false><<<grid, dim3(512), 0, st>>>(a);
             return;
           }
         }
-        attend4_kernel<T, G, NB, 4><<<grid, dim3(256), 0, st>>>(a);
+        attend4_kernel<T, G, NB, 4, false><<<grid, dim3(256), 0, st>>>(a);
       };
-      if constexpr (!f32 && G < 8) {
+      if (a.wide) {
+        if constexpr (G > 1) attend4_kernel<T, G, 1, 4, true><<<grid, dim3(256), 0, st>>>(a);
+      } else if constexpr (!f32 && G < 8) {
         if (a.columns == 2) run(std::integral_constant<int, 2>{});
         else run(std::integral_constant<int, 1>{});
       } else {

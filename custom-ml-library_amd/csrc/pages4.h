@@ -119,6 +119,7 @@ struct Attend4 {
   const void *cos, *sin;  // rotate the queries; or NULL
   int n, rep, len_q, rows, causal;
   int split, splits;      // positions a split (a multiple of 32), splits of the longest sequence
+  int wide;                    // whether a column is a row, not a group of one
   int columns, waves, blocks;  // column blocks (1 or 2) and waves of a workgroup; workgroups a KV head's rows take
   float sl, sign;         // |scale| * log2(e) and the scale's sign, with the queries; 1 and 0 for no scale
   FastDiv by_len_q;

@@ -9,8 +9,8 @@ shared page, which is then copied for it.
 The format (``include/tsattn.h``, ``tsattn_pages4``): e2m1 codes and a scale of 6
 significant bits for each 32 channels, so that what the cache stands for is exact in
 16 bits.  ``paged_attention`` reads the codes themselves for few query rows per KV
-head (``tsattn_pages4_attend``); for a prompt's many rows the pages are
-dequantised once and attended on the 16-bit or fp32 matrix cores.
+head, and for any number in fp32 or of 256 channels (``tsattn_pages4_attend``); for a
+prompt's many rows of 16 bits the pages are dequantised once and attended as arrays.
 
 Page tables and reference counts are the host's; lengths travel with each launch.
 Calls captured into a HIP graph replay the positions, and the pages, that they were
@@ -33,16 +33,16 @@ from .attention import _dtype_code, _rope_rows, rope_tables, scaled_dot_product_
 
 def _reads_codes(rows: int, heads: int, dim: int, wide: bool, lens) -> bool:
     """Whether attention reads the codes themselves: ``rows`` query rows per KV head over sequences
-    of ``lens``.  Its time grows with rows and positions; dequantising once and attending on the
-    matrix cores costs mostly host time, per run of rows of one length, but fp32's kernel waits on
-    every key of one row block.  Microseconds, codes / dequantised, 8 KV heads of D128 over 8000 positions: bf16 64
-    rows 28 / 57, 128 42 / 57, 256 74 / 57, 1024 231 / 61; fp32 1024 rows 357 / 1122; over 500
-    positions bf16 1024 rows 26 / 52.  2 heads of D64 over 8000: 1024 rows 33 / 56, fp32 43 / 170;
-    12 heads of D32, fp32 896 rows 73 / 173."""
-    size = (dim / 128) ** 1.5
-    codes = 12 + (6.4e-6 if wide else 4e-6) * size * rows * heads * int(lens.sum())
-    whole = 50 * len(_runs(lens)) + ((0.14 if dim == 128 else 0.02) * int(lens.max()) if wide else 0)
-    return codes <= whole
+    of ``lens``.  Dequantising once costs host time for each run of rows of one length, and memory
+    traffic, and has the faster matrix products afterwards; of fp32 (``wide``) it has not: three bf16
+    parts take a third of the fp32 cores' time.  Microseconds, codes / dequantised, 8 KV heads of
+    D128, bf16: over 8000 positions 128 rows 32 / 48, 256 55 / 49, 1024 142 / 62; over 2000, 1024
+    rows 41 / 49, 2048 71 / 49; 4 sequences of 8000, 128 rows 81 / 122, 512 265 / 123; 8 heads of D64,
+    2 of 2000, 1024 rows 49 / 48.  fp32, 8 heads of D128 over 8000: 1024 rows 172 / 1136."""
+    pairs, size = rows * heads * int(lens.sum()), (dim / 128) ** 0.85
+    codes = 15 + 2.3e-6 * size * pairs
+    whole = 42 * len(_runs(lens)) + 1.5e-6 * dim * heads * int(lens.sum()) + 4e-7 * size * pairs
+    return wide or codes <= whole
 
 
 def _runs(lens) -> list:

@@ -262,6 +262,32 @@ def test_workgroups_of_every_make(batch, hkv, rep, steps, keys, d, dtype):
         check(nn.paged_attention(wrap(q), cache)._data, want, tol, dtype)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("d,rep", [(32, 1), (64, 4), (128, 1), (128, 8), (256, 8)])
+def test_what_is_not_seen_does_not_count(d, rep, dtype):
+    """NaN in later positions of the chunk, in cut ones and in pages never written: rows that do not
+    see them are as they are without."""
+    say("paged unseen NaN", d, rep, dtype)
+    gen, steps, n = seeded(d + rep), 37, 150
+    k, v = (draw(gen, 1, 2, n, d, dtype=dtype) for _ in range(2))
+    q = draw(gen, 1, 2 * rep, steps, d, dtype=dtype)
+    outs = []
+    for bad in (False, True):
+        kk, vv = k.clone(), v.clone()
+        cache = nn.PagedKVCache(1, 2, d, 256, device="hip", dtype=dtype)
+        if bad:
+            kk[:, :, n - 5:], vv[:, :, n - 9] = math.nan, math.nan  # seen by the last 5, by the last 9 queries
+            cache._core.pool.fill_(0xFF)                            # (codes of 6, scales of NaN)
+            x = torch.full((1, 2, 256, d), math.nan, dtype=dtype, device="cuda")
+            cache.append(wrap(x), wrap(x))
+            cache.truncate(0)
+        cache.append(wrap(kk), wrap(vv))
+        with patch.object(P, "_reads_codes", return_value=True):
+            outs.append(nn.paged_attention(wrap(q), cache)._data)
+    assert torch.equal(outs[0][:, :, :-9], outs[1][:, :, :-9])
+    assert torch.isfinite(outs[0]).all() and torch.isnan(outs[1][:, :, -9:]).all()
+
+
 @pytest.mark.parametrize("dtype,d", [(BF16, 32), (F32, 64)])
 def test_rows_of_hundreds_of_thousands(dtype, d):
     """More splits than the second kernel has loads in flight, beside a row of one position."""

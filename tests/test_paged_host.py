@@ -353,11 +353,11 @@ def test_the_prompt_rule():
     """Both sides of each measured crossing, runs of equal rows counted once."""
     lens = lambda *n: np.array(n, np.int32)  # noqa: E731
     for rows, heads, dim, wide, n, codes in (
-            (64, 8, 128, False, lens(8000), True), (256, 8, 128, False, lens(8000), False),
-            (1024, 8, 128, False, lens(500), True), (1024, 8, 128, False, lens(2000), False),
+            (128, 8, 128, False, lens(8000), True), (512, 8, 128, False, lens(8000), False),
+            (1024, 8, 128, False, lens(500), True), (2048, 8, 128, False, lens(2000), False),
             (1024, 8, 128, True, lens(8000), True), (1024, 2, 64, False, lens(8000), True),
-            (128, 8, 128, False, lens(8000, 8000, 8000), False), (128, 8, 128, False, lens(8000, 7000, 8000), True),
-            (4096, 8, 128, True, lens(32000), False), (32, 4, 64, False, lens(0), True)):
+            (256, 8, 128, False, lens(8000, 8000, 8000), False), (256, 8, 128, False, lens(8000, 7000, 7500), True),
+            (4096, 8, 128, True, lens(32000), True), (32, 4, 64, False, lens(0), True)):
         assert P._reads_codes(rows, heads, dim, wide, n) is codes, (rows, heads, dim, wide, n)
     assert P._runs(lens(3, 3, 5, 3)) == [2, 3, 4] and P._runs(lens(7)) == [1]
 
