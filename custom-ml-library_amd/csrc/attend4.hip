@@ -12,11 +12,9 @@
 // takes P sv of its own column: a lane scales 8 probabilities a tile where it would
 // scale 8 G otherwise.  The price is in MFMAs, which have time (a value block is
 // multiplied for all columns and used by those of its group).  Where there are many
-// (WIDE), a column is a row: a key's scales multiply the groups' scores one after the
-// other, and values are dequantised, exactly, as they go to the matrix cores.  Scales
-// reach the lanes from the one that loaded them.  In the tiles that some rows see and
-// others do not, a value's scale goes to the probabilities instead: NaN there is
-// no business of a row that does not see it.
+// (WIDE), a column is a row, and the scales multiply the groups' scores, and the
+// probabilities, one group after the other; they reach the lanes from the one that
+// loaded them.
 //
 // Precision.  q enters exactly: bf16 in one part, f16 in two, fp32 in three.  P sv
 // (WIDE: P) enters as two bf16 parts (2^-17 of each), for fp32 as three (2^-25).
@@ -50,8 +48,11 @@ template <typename T>
 constexpr int p_parts() { return std::is_same_v<T, float> ? 3 : 2; }
 
 // Two floats as N pairs of bf16 whose sums they are: all but the last truncated.
+// (A subtraction contracted with the product before it would keep a scale from being
+// that product's own operand.)
 template <int N>
 __device__ __forceinline__ void split_bf16(float a, float b, uint32_t (&out)[N]) {
+#pragma clang fp contract(off)
 #pragma unroll
   for (int i = 0; i < N - 1; ++i) {
     const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
@@ -84,14 +85,6 @@ __device__ __forceinline__ float from_lane(float x) {
       float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x150 + S, 0xF, 0xF, true));  // row_newbcast
 }
 
-// Eight codes, four bits each, times their keys' scales: exact in bf16.
-__device__ __forceinline__ u32x4 values_bf16(uint32_t w, const float (&s)[8]) {
-  const f32x2 y0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), y1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
-  const f32x2 y2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), y3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
-  return u32x4{pack2<bf16>(y0[0] * s[0], y0[1] * s[1]), pack2<bf16>(y1[0] * s[2], y1[1] * s[3]),
-               pack2<bf16>(y2[0] * s[4], y2[1] * s[5]), pack2<bf16>(y3[0] * s[6], y3[1] * s[7])};
-}
-
 // f(integral constants 0 .. N - 1).
 template <int N, typename F>
 __device__ __forceinline__ void each(F &&f) {
@@ -113,7 +106,7 @@ struct Held {
 };
 
 template <typename T, int G, int NB, int NWV, bool WIDE>
-__global__ __launch_bounds__(64 * NWV, (WIDE || (std::is_same_v<T, float> && G == 8) ? 1 : 2)) void attend4_kernel(Attend4 a) {
+__global__ __launch_bounds__(64 * NWV, (G == 8 && (WIDE || std::is_same_v<T, float>) ? 1 : 2)) void attend4_kernel(Attend4 a) {
   constexpr int D = 32 * G, W = 2 * G, NQ = q_parts<T>(), NP = p_parts<T>();
   constexpr int RB = WIDE ? 16 : 16 / G, ROWS = RB * NB;  // rows a column block, a workgroup
   constexpr int PIECES = WIDE ? G : 1;                    // of a row that a lane holds
@@ -253,10 +246,6 @@ __global__ __launch_bounds__(64 * NWV, (WIDE || (std::is_same_v<T, float> && G =
     }
     float x[NB][8];  // the scores
     if constexpr (WIDE) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[nb][i] = 0.f;
       each<G>([&](auto group) __attribute__((always_inline)) {
         constexpr int ks = decltype(group)::value;
         f32x4 s[NB][2];
@@ -274,7 +263,8 @@ __global__ __launch_bounds__(64 * NWV, (WIDE || (std::is_same_v<T, float> && G =
         for (int i = 0; i < 8; ++i) {
           const float sc = from_lane<ks>(ksc[i]);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) x[nb][i] = fmaf(s[nb][i >> 2][i & 3], sc, x[nb][i]);
+          for (int nb = 0; nb < NB; ++nb)
+            x[nb][i] = ks == 0 ? s[nb][i >> 2][i & 3] * sc : fmaf(s[nb][i >> 2][i & 3], sc, x[nb][i]);
         }
       });
     } else {
@@ -333,55 +323,53 @@ __global__ __launch_bounds__(64 * NWV, (WIDE || (std::is_same_v<T, float> && G =
         l[nb] += p0 + p1;
         pr[nb][i] = p0, pr[nb][i + 1] = p1;
         uint32_t two[NP];
-        split_bf16<NP>(WIDE ? p0 : p0 * vs[i], WIDE ? p1 : p1 * vs[i + 1], two);
+        split_bf16<NP>(p0 * vs[i], p1 * vs[i + 1], two);
 #pragma unroll
         for (int n = 0; n < NP; ++n) pb[nb][n][i >> 1] = two[n];
       }
     }
-    if (WIDE && !whole) {  // (a key that some rows see and others do not: its scale goes to the probabilities)
-      each<G>([&](auto group) __attribute__((always_inline)) {
-        constexpr int s = decltype(group)::value;
-        const u32x4 vf[2] = {levels_bf16(t4.vw(2 * s)), levels_bf16(t4.vw(2 * s + 1))};
-        float sc[8];
+    if constexpr (WIDE) {  // the probabilities times one group's scales after the other's
+      auto values = [&](auto every) __attribute__((always_inline)) {
+        each<G>([&](auto group) __attribute__((always_inline)) {
+          constexpr int s = decltype(group)::value;
+          const u32x4 vf[2] = {levels_bf16(t4.vw(2 * s)), levels_bf16(t4.vw(2 * s + 1))};
+          float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sc[i] = from_lane<s>(vsc[i]);
+          for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          u32x4 ps[NP];
+            for (int i = 0; i < 8; ++i) {
+              y[i] = pr[nb][i] * from_lane<s>(vsc[i]);
+              if (!decltype(every)::value) y[i] = seen[nb] >> i & 1 ? y[i] : 0.f;
+            }
+            u32x4 ps[NP];
 #pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            uint32_t two[NP];
-            split_bf16<NP>(seen[nb] >> i & 1 ? pr[nb][i] * sc[i] : 0.f,
-                           seen[nb] >> (i + 1) & 1 ? pr[nb][i + 1] * sc[i + 1] : 0.f, two);
+            for (int i = 0; i < 8; i += 2) {
+              uint32_t two[NP];
+              split_bf16<NP>(y[i], y[i + 1], two);
 #pragma unroll
-            for (int n = 0; n < NP; ++n) ps[n][i >> 1] = two[n];
+              for (int n = 0; n < NP; ++n) ps[n][i >> 1] = two[n];
+            }
+#pragma unroll
+            for (int n = 0; n < NP; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) oacc[nb][2 * s + e] = mfma16<bf16>(vf[e], ps[n], oacc[nb][2 * s + e]);
           }
+        });
+      };
+      if (whole) values(std::true_type{});
+      else values(std::false_type{});
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; i += 2) {
+        const u32x4 vf[2] = {levels_bf16(t4.vw(i)), levels_bf16(t4.vw(i + 1))};
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int n = 0; n < NP; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) oacc[nb][2 * s + e] = mfma16<bf16>(vf[e], ps[n], oacc[nb][2 * s + e]);
-        }
-      });
-      return;
-    }
-    each<G>([&](auto group) __attribute__((always_inline)) {
-      constexpr int i = 2 * decltype(group)::value;
-      u32x4 vf[2];
-      if constexpr (WIDE) {
-        float sc[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j] = from_lane<i / 2>(vsc[j]);
-        vf[0] = values_bf16(t4.vw(i), sc), vf[1] = values_bf16(t4.vw(i + 1), sc);
-      } else {
-        vf[0] = levels_bf16(t4.vw(i)), vf[1] = levels_bf16(t4.vw(i + 1));
+            for (int e = 0; e < 2; ++e) oacc[nb][i + e] = mfma16<bf16>(vf[e], pb[nb][n], oacc[nb][i + e]);
       }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int n = 0; n < NP; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) oacc[nb][i + e] = mfma16<bf16>(vf[e], pb[nb][n], oacc[nb][i + e]);
-    });
+    }
   };
 
   for (int t = 0; t < mine; t += 2) {
