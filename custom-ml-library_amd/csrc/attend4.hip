@@ -28,10 +28,8 @@
 // time and 56% of the vector units'.  Middling ones by the start of a workgroup and a
 // tile's latency: 64 x 8 KV heads over 1025, 4 rows (f16, D128), 77 MB, 18.4 us, of
 // which 4 pass before the second tile.  Small ones by latency alone: 8 heads over 200,
-// 4 us.  Many rows by the vector units (levels, scales and roundings; a tile of 32
-// positions and 16 rows takes about 1.9 us alone): 3 sequences of 2 heads up to 15686,
-// 496 rows of fp32 D256, 32.8 GFLOP, 194 us, 169 TFLOP/s, where groups as columns took
-// 808; 8 heads over 8000, 1024 rows of fp32 D128 160 (382).
+// 4 us.  Many rows by the vector units (levels, scales, roundings: about 320 instructions
+// a tile of 32 positions and 16 rows of bf16 D128).
 #include "pages4.h"
 #include "rope_math.h"
 
@@ -494,17 +492,18 @@ __global__ __launch_bounds__(64) void attend4_merge_kernel(Attend4 a) {
 // columns of rows with four -- and splits: those that a model of the time likes best.
 // Two blocks read the cache once for twice the rows; one, where the memory is not what
 // a call waits for, has twice the workgroups.  In us: a workgroup's prologue and merge
-// 2.3 or 2.5, of rows 3.7 to 4.4; a tile of a wave the largest of its own latency (by
-// its products; bf16 D128 0.94 with one block, 1.8 with two, 1.8 of rows; fp32 D128 1.7,
-// of rows 2.0; bf16 D256 1.7, of rows 2.9), of the issue slots of the waves beside it and
+// 2.4 or 2.6, of rows 3.9 to 6.3; a tile of a wave the largest of its own latency (by
+// its products; bf16 D128 1.0 with one block, 2.1 with two, 1.1 of rows; fp32 D128 1.8,
+// of rows 1.3; bf16 D256 1.9, of rows 2.0), of the issue slots of the waves beside it and
 // of the memory's rate; where the workgroups do not fit the chip at once, their rounds
-// over it; the second kernel 2.6.  Its constants are fitted to 60 shapes, of which it
-// takes 3% longer than the best choice in the mean.  Measured, what it picks and
-// another: 7 sequences of 4 KV heads up to 4001, 20 rows of bf16 D128: rows 15.7, groups
-// in one block 17.4, in two 19.1; 8 of 8 heads over 8000, 16 rows: rows 32, groups 44;
-// 4 of 32 heads over 4000, f16 D128: eight waves and 2 splits 19.0, four and 3 22.4; 3 of
-// one head over 1500, fp32 D128: 12 splits 7.1, one 13.1; 64 of 8 heads over 1025, 4 rows
-// of f16 D128: one split 18.5, three 24.
+// over it; the second kernel 3.4.  Its constants are fitted to 104 shapes, of which it
+// takes 3% longer than the best choice in the mean (groups alone 34%, for the 70 with
+// more rows than one block).  Measured, what it picks and another: 7 sequences of 4 KV
+// heads up to 4001, 20 rows of bf16 D128: rows 14.4, groups in one block 17.4, in two
+// 19.1; 8 of 8 heads over 8000, 16 rows: rows 27, groups 44; 4 of 32 heads over 4000, f16
+// D128: eight waves and 2 splits 19.0, four and 3 22.4; 3 of one head over 1500, fp32
+// D128: 12 splits 7.1, one 13.1; 64 of 8 heads over 1025, 4 rows of f16 D128: one split
+// 18.5, three 24.
 void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
   int64_t total = 0;
   int longest = 1;
@@ -540,26 +539,26 @@ void plan_attend4(Attend4 *a, int dtype, const int32_t *lens) {
         if (make == 1 && (dtype == TSATTN_F32 || dim == 256)) continue;
         if (wide && (waves == 8 || dim == 32)) continue;  // (32 channels: a row is one group)
         const int per = wide ? 16 : one_block * nb, blocks = (a->rows + per - 1) / per;
-        const double latency = wide      ? 0.76 + dim / 32 * (0.23 + 0.014 * parts)
-                               : nb == 2 ? 0.2 + 0.068 * (dim / 16) * parts
-                                         : 0.2 + 0.031 * (dim / 16) * parts;
-        const double start = wide ? 3.5 + 0.0034 * dim : waves == 8 ? 2.5 : 2.3;
+        const double latency = wide ? 0.33 + dim / 32 * (0.17 + 0.011 * parts)
+                                    : nb * (0.21 + dim / 16 * (0.008 + 0.032 * parts));
+        const double start = wide ? 3.1 + 0.4 * (dim / 32) : waves == 8 ? 2.6 : 2.4;
         const double slots = waves == 8 || (wide && dim == 256)             ? 256.
                              : nb == 2 || dim == 256 || (wide && dim == 128) ? 512.
                                                                             : 768.;
-        const double groups = static_cast<double>(a->p.heads) * blocks, wgs = groups * live;
+        const double groups = static_cast<double>(a->p.heads) * blocks, wgs = groups * live, rounds = wgs / slots;
         const double busy = (wgs < slots ? wgs : slots) * waves;
-        const double rate = busy * 36 * dim / 7.3e6, issue = 0.62 * latency * busy / 1024;
+        const double rate = busy * 36 * dim / 7.4e6, issue = (wide ? 0.69 : 0.55) * latency * busy / 1024;
         const double alone = latency > issue ? latency : issue;
         const double one = start + (tiles > 1 ? tiles : 1) * (alone > rate ? alone : rate);
         double cost = one;
-        if (wgs > 3 * slots) {
+        if (rounds > 3) {
           const double sum = groups * total / unit, most = wgs * start + sum * alone;
-          cost = ((most > sum * rate ? most : sum * rate) + 0.3 * wgs * start) / slots + 0.15 * one;
-        } else if (wgs > slots) {
-          cost = one * (1.6 + 0.52 * (wgs / slots - 1));
+          cost = ((most > sum * rate ? most : sum * rate) + (wide ? 0.83 : 0.05) * wgs * start) / slots +
+                 (wide ? 0.02 : 0.14) * one;
+        } else if (rounds > 1) {
+          cost = one * (wide ? 1.1 * rounds : 1.3 + 0.62 * (rounds - 1));
         }
-        if (n > 1) cost += 2.1 + 0.5 * ((n + 15) / 16) + 8. * a->n * a->p.heads * n * a->rows * (dim + 2) / 7.3e6;
+        if (n > 1) cost += 2.9 + 0.5 * ((n + 15) / 16) + 8. * a->n * a->p.heads * n * a->rows * (dim + 2) / 7.4e6;
         if (cost < best) {
           best = cost;
           a->wide = wide, a->columns = nb, a->blocks = blocks, a->waves = waves;

@@ -35,12 +35,13 @@ def _reads_codes(rows: int, heads: int, dim: int, wide: bool, lens) -> bool:
     """Whether attention reads the codes themselves: ``rows`` query rows per KV head over sequences
     of ``lens``.  Dequantising once costs host time for each run of rows of one length, and memory
     traffic, and has the faster matrix products afterwards; of fp32 (``wide``) it has not: three bf16
-    parts take a third of the fp32 cores' time.  Microseconds, codes / dequantised, 8 KV heads of
-    D128, bf16: over 8000 positions 128 rows 32 / 48, 256 55 / 49, 1024 142 / 62; over 2000, 1024
-    rows 41 / 49, 2048 71 / 49; 4 sequences of 8000, 128 rows 81 / 122, 512 265 / 123; 8 heads of D64,
-    2 of 2000, 1024 rows 49 / 48.  fp32, 8 heads of D128 over 8000: 1024 rows 172 / 1136."""
+    parts take a seventh of the fp32 kernels' time.  Microseconds, codes / dequantised, 8 KV heads of
+    D128, bf16: over 8000 positions 128 rows 28 / 50, 256 48 / 51, 512 65 / 50, 1024 119 / 59; over
+    2000, 1024 rows 36 / 50, 2048 60 / 50; 4 sequences of 8000, 128 rows 72 / 122, 512 224 / 120; 8
+    heads of D64, 2 of 2000, 1024 rows 38 / 50, 2048 64 / 45.  fp32, 8 heads of D128 over 8000: 1024
+    rows 158 / 1135."""
     pairs, size = rows * heads * int(lens.sum()), (dim / 128) ** 0.85
-    codes = 15 + 2.3e-6 * size * pairs
+    codes = 15 + 1.8e-6 * size * pairs
     whole = 42 * len(_runs(lens)) + 1.5e-6 * dim * heads * int(lens.sum()) + 4e-7 * size * pairs
     return wide or codes <= whole
 
