@@ -357,7 +357,9 @@ def test_the_prompt_rule():
             (1024, 8, 128, False, lens(500), True), (2048, 8, 128, False, lens(2000), False),
             (1024, 8, 128, True, lens(8000), True), (1024, 2, 64, False, lens(8000), True),
             (256, 8, 128, False, lens(8000, 8000, 8000), False), (256, 8, 128, False, lens(8000, 7000, 7500), True),
-            (4096, 8, 128, True, lens(32000), True), (32, 4, 64, False, lens(0), True)):
+            (4096, 8, 128, True, lens(32000), True), (32, 4, 64, False, lens(0), True),
+            (1 << 18, 1, 64, True, lens(300), True), ((1 << 18) + 1, 1, 64, True, lens(300), False),
+            (1 << 17, 8, 128, True, lens(16384), True), (1 << 17, 8, 128, True, lens(32769), False)):
         assert P._reads_codes(rows, heads, dim, wide, n) is codes, (rows, heads, dim, wide, n)
     assert P._runs(lens(3, 3, 5, 3)) == [2, 3, 4] and P._runs(lens(7)) == [1]
 
