@@ -17,7 +17,7 @@
 // loaded them.
 //
 // Precision.  q enters exactly: bf16 in one part, f16 in two, fp32 in three.  P sv
-// (WIDE: P) enters as two bf16 parts (2^-17 of each), for fp32 as three (2^-25).
+// enters as two bf16 parts (2^-17 of each), for fp32 as three (2^-25).
 //
 // A wave works alone on every fourth or eighth tile of its split, two tiles ahead in
 // registers, straight from memory in operand order (pages4.h); waves merge in LDS,
@@ -230,8 +230,8 @@ __global__ __launch_bounds__(64 * NWV, (G == 8 && (WIDE || std::is_same_v<T, flo
     for (int i = 0; i < W; ++i) oacc[nb][i] = f32x4{};
   }
 
-  // Chains of dependent MFMAs alternate: the two halves of the scores, pairs of
-  // value blocks.
+  // Chains of dependent MFMAs alternate: the two halves of the scores (WIDE: of each
+  // group), pairs of value blocks.
   auto compute = [&](const Held<G> &t4, int t) __attribute__((always_inline)) {
     const int tile = w + NWV * t;  // of the split
     float ksc[8], vsc[8];  // the scales of the lane's group, keys 4 g .. + 3 and 16 + 4 g .. + 3

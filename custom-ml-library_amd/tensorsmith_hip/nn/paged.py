@@ -87,25 +87,22 @@ class _Pages:
         most, entries = max(rows, num_pages), rows * columns
         sizes = {"host": entries, "lengths": rows, "refs": num_pages, "stack": num_pages, "shown": entries,
                  "changed": entries, "src": most, "dst": most, "copies": 1, "dirty": (entries + 3) // 4}
-        memory, at, where = np.zeros(sum(sizes.values()), np.int32), 0, {}
+        memory, at, where, part = np.zeros(sum(sizes.values()), np.int32), 0, {}, {}
         base = memory.ctypes.data
         for name, n in sizes.items():
-            setattr(self, name, memory[at:at + n])
-            where[name] = base + 4 * at
+            part[name], where[name] = memory[at:at + n], base + 4 * at
             at += n
-        self.host = self.host.reshape(rows, columns)
+        self.host, self.lengths, self.refs = part["host"].reshape(rows, columns), part["lengths"], part["refs"]
+        self.stack, self.shown, self.copies = part["stack"], part["shown"], part["copies"]
         self.lengths_at = where["lengths"]
         self.out = where["src"], where["dst"], where["copies"]
-        self.tables = t = _lib.Pages4Host()
-        t.rows, t.columns, t.page_size, t.pages = rows, columns, page_size, num_pages
-        t.table, t.lengths, t.refs, t.stack = (where[x] for x in ("host", "lengths", "refs", "stack"))
-        t.shown, t.changed, t.dirty = (where[x] for x in ("shown", "changed", "dirty"))
+        self.tables = _lib.Pages4Host(rows, columns, page_size, num_pages, where["host"], where["lengths"], where["refs"],
+                                      where["stack"], where["shown"], where["changed"], where["dirty"], 0, 0)
         # (what no append has written weighs nothing: positions past a row's length are masked)
         self.pool = torch.empty((num_pages, self.page_bytes), dtype=torch.uint8, device=dev.torch)
         self.table = torch.empty((rows, columns), dtype=torch.int32, device=dev.torch)
-        self.desc = d = _lib.Pages4()
-        d.pool, d.num_pages, d.heads, d.page_size, d.dim = self.pool.data_ptr(), num_pages, heads, page_size, dim
-        d.table, d.table_rows, d.table_stride = self.table.data_ptr(), rows, columns
+        self.desc = _lib.Pages4(self.pool.data_ptr(), num_pages, heads, page_size, dim, self.table.data_ptr(), rows,
+                                columns)
 
     def clear(self) -> None:
         """Every page free, every row empty."""
@@ -190,11 +187,14 @@ class PagedKVCache:
         self.max_seq_len, self._code = max_seq_len, _dtype_code(self.dtype)
         self._core = _Pages(batch_size, num_heads, head_dim, columns, page_size, num_pages, dev)
         self._core.clear()
-        self._select(np.arange(batch_size, dtype=np.int32))
+        self._select()
 
-    def _select(self, rows) -> None:
-        self._rows, self._rows_at = rows, rows.ctypes.data
-        self._whole = len(rows) == len(self._core.lengths) and bool((rows == np.arange(len(rows))).all())
+    def _select(self, rows=None) -> None:
+        """The core's rows that this cache is; all of them by default."""
+        every = len(self._core.lengths)
+        self._whole = rows is None or (len(rows) == every and bool((rows == np.arange(every)).all()))
+        self._rows = np.arange(every, dtype=np.int32) if rows is None else rows
+        self._rows_at = self._rows.ctypes.data
 
     # -- what it is -----------------------------------------------------------
 
@@ -365,7 +365,7 @@ class PagedKVCache:
         other = object.__new__(PagedKVCache)
         other.dtype, other.max_seq_len, other._code = self.dtype, self.max_seq_len, self._code
         other._core = self._core.clone(self._rows, self._pool_size(num_pages))
-        other._select(np.arange(len(self._rows), dtype=np.int32))
+        other._select()
         return other
 
     def compact(self, num_pages: int | None = None) -> int:
