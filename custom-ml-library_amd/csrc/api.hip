@@ -1292,6 +1292,7 @@ int tsattn_pages4_apply(tsattn_pages4_host *h, int32_t *table, const void *from,
                                                           at, value, static_cast<hipStream_t>(stream)),
                               "page update launch")
                  : TSATTN_OK;
+  if (!rc) tsattn::pages4_sent(h, sets, at, value);
   free(at);
   return rc;
 }

@@ -108,7 +108,8 @@ void pages4_reorder(tsattn_pages4_host *h, int32_t n, const int32_t *rows, const
 int32_t pages4_clone(const tsattn_pages4_host *from, int32_t n, const int32_t *rows, tsattn_pages4_host *to,
                      int32_t *number, int32_t *src, int32_t *dst);
 int32_t pages4_compact(tsattn_pages4_host *h, int32_t *number, int32_t *src, int32_t *dst, int32_t *copies);
-int32_t pages4_changes(tsattn_pages4_host *h, int32_t *at, int32_t *value);
+int32_t pages4_changes(const tsattn_pages4_host *h, int32_t *at, int32_t *value);
+void pages4_sent(tsattn_pages4_host *h, int32_t sets, const int32_t *at, const int32_t *value);
 
 // Attention of len_q queries a sequence (q, out: [n, heads_q, len_q, dim]) over
 // the cached positions, the queries' own the last len_q of them.

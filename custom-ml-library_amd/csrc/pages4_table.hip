@@ -177,18 +177,23 @@ int32_t pages4_compact(tsattn_pages4_host *h, int32_t *number, int32_t *src, int
 }
 
 // The changed entries that hold another page than the device's: at, value (room for
-// n_changed); none is left.
-int32_t pages4_changes(tsattn_pages4_host *h, int32_t *at, int32_t *value) {
+// n_changed).  They stay among the changed ones until they are sent.
+int32_t pages4_changes(const tsattn_pages4_host *h, int32_t *at, int32_t *value) {
   int32_t k = 0;
   for (int32_t i = 0; i < h->n_changed; ++i) {
     const int32_t a = h->changed[i];
-    h->dirty[a] = 0;
     if (h->table[a] < 0 || h->table[a] == h->shown[a]) continue;
     at[k] = a;
-    value[k++] = h->shown[a] = h->table[a];
+    value[k++] = h->table[a];
   }
-  h->n_changed = 0;
   return k;
+}
+
+// The device's table has what pages4_changes gave: no entry is changed.
+void pages4_sent(tsattn_pages4_host *h, int32_t sets, const int32_t *at, const int32_t *value) {
+  for (int32_t i = 0; i < h->n_changed; ++i) h->dirty[h->changed[i]] = 0;
+  for (int32_t i = 0; i < sets; ++i) h->shown[at[i]] = value[i];
+  h->n_changed = 0;
 }
 
 }  // namespace tsattn

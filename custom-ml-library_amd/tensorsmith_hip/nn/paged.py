@@ -95,6 +95,7 @@ class _Pages:
         self.host, self.lengths, self.refs = part["host"].reshape(rows, columns), part["lengths"], part["refs"]
         self.stack, self.shown, self.copies = part["stack"], part["shown"], part["copies"]
         self.lengths_at = where["lengths"]
+        self.pending = False  # whether page copies or entries may be left to bring to the device
         self.out = where["src"], where["dst"], where["copies"]
         self.tables = _lib.Pages4Host(rows, columns, page_size, num_pages, where["host"], where["lengths"], where["refs"],
                                       where["stack"], where["shown"], where["changed"], where["dirty"], 0, 0)
@@ -116,16 +117,25 @@ class _Pages:
     def free(self) -> int:
         return self.tables.free
 
+    def ready(self) -> None:
+        """What an earlier call's page changes left to do, if it failed before they were on the device.
+        Every call begins with it, so nothing is taken, given back or read in between."""
+        if self.pending:
+            if self.copies[0] or self.tables.n_changed:
+                self._eager()
+            self.apply()
+
     def apply(self, source=None) -> None:
         """To the device, on the current stream: the page copies that the last host call asked for
         (from the pool of ``source``, by default this one's) and the changed table entries."""
-        source = source or self
-        n = int(source.copies[0])
+        n = int(self.copies[0])
         if n or self.tables.n_changed:
-            source.copies[0] = 0
+            pool = (source or self).desc
             _lib.check(launch(self.device, _lib.load().tsattn_pages4_apply, self.tables, self.desc.table,
-                              source.desc.pool, source.desc.num_pages, self.desc.pool, self.desc.num_pages,
-                              self.page_bytes, n, *source.out[:2]), "page update")
+                              pool.pool, pool.num_pages, self.desc.pool, self.desc.num_pages,
+                              self.page_bytes, n, *self.out[:2]), "page update")
+            self.copies[0] = 0
+        self.pending = False
 
     def _eager(self, rows=None, steps: int = 0) -> None:
         """Refuses page changes under capture: a captured call's pages would be the host's at once and
@@ -144,17 +154,27 @@ class _Pages:
 
     def grow(self, n: int, rows: int, steps: int) -> None:
         """Pages of their own for the next ``steps`` positions of the ``n`` rows (an address)."""
+        self.pending = True
         _lib.check(_lib.load().tsattn_pages4_grow(self.tables, n, rows, steps, *self.out), "page table")
 
     def cut(self, rows, rows_at: int, lengths) -> None:
         """``rows`` (at an address) end at ``lengths``; pages wholly past them are given back."""
         _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows_at, lengths.ctypes.data), "page table")
 
+    def take_back(self, rows, steps: int) -> None:
+        """Gives back the pages that ``grow`` took past the rows' lengths, if it got so far.  Copies of
+        shared pages stay: they are the rows' own, made with the next call if they are not there yet."""
+        held = ((self.host[rows] >= 0).sum(1) * self.page_size).astype(np.int32)
+        lens = self.lengths[rows]
+        self.lengths[rows] = np.maximum(lens, np.minimum(lens + np.int32(steps), held))
+        self.cut(rows, rows.ctypes.data, lens)
+
     def clone(self, rows, num_pages: int) -> "_Pages":
         """The rows with pages of their own, in a pool of ``num_pages``."""
         self._eager()
+        self.ready()
         other = _Pages(len(rows), self.heads, self.dim, self.host.shape[1], self.page_size, num_pages, self.device)
-        _lib.check(_lib.load().tsattn_pages4_clone(self.tables, len(rows), rows.ctypes.data, other.tables, *self.out),
+        _lib.check(_lib.load().tsattn_pages4_clone(self.tables, len(rows), rows.ctypes.data, other.tables, *other.out),
                    "page table")
         other.apply(self)
         return other
@@ -166,7 +186,9 @@ class PagedKVCache:
     ``num_pages`` pages of ``page_size`` (32, 64, 128, .. 4096) positions are
     allocated at once; by default as many as the rows can need.  ``dtype`` (float32,
     float16 or bfloat16) is that of the keys and values given and read back.
-    Inference only, like ``KVCache``.
+    Inference only, like ``KVCache``.  Where a launch fails, ``append`` leaves the rows as
+    they were; ``reorder`` and ``compact`` have taken place on the host, and the next call
+    first brings to the device what it lacks.
     """
 
     def __init__(self, batch_size: int, num_heads: int, head_dim: int, max_seq_len: int, *, device=None,
@@ -254,14 +276,14 @@ class PagedKVCache:
             cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
         k, v = (_rows(t if t.dtype == self.dtype else t.to(self.dtype)) for t in (key._data, value._data))
         core._eager(self._rows, steps)
-        core.grow(len(lens), self._rows_at, steps)
+        core.ready()
         try:
+            core.grow(len(lens), self._rows_at, steps)
             core.apply()
             _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
                               _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
         except BaseException:
-            core.lengths[self._rows] += steps  # (the new pages go back)
-            core.cut(self._rows, self._rows_at, core.lengths[self._rows] - np.int32(steps))
+            core.take_back(self._rows, steps)
             raise
         if self._whole:
             core.lengths += steps
@@ -294,6 +316,7 @@ class PagedKVCache:
         import torch
 
         core = self._core
+        core.ready()
         lens, lens_at = self._lens()
         if last is not None and not 0 < last <= lens.min():
             raise ValueError("the last positions read must be between one and the shortest row's length")
@@ -331,12 +354,14 @@ class PagedKVCache:
 
     def reset(self) -> None:
         """Every row empty, its pages given back."""
+        self._core.ready()
         self._core.cut(self._rows, self._rows_at, np.zeros_like(self._rows))
 
     def free(self, indices) -> None:
         """These rows empty, their pages given back."""
         rows = self._rows[np.unique(self._indices(indices, None))]
         if len(rows):
+            self._core.ready()
             self._core.cut(rows, rows.ctypes.data, np.zeros_like(rows))
 
     def truncate(self, length) -> None:
@@ -348,6 +373,7 @@ class PagedKVCache:
         lens = want.astype(np.int32)
         if (lens != want).any():
             raise ValueError("truncate length must be between zero and the current length")
+        self._core.ready()
         self._core.cut(self._rows, self._rows_at, lens if lens.shape else np.full_like(self._rows, lens))
 
     def reorder(self, indices) -> None:
@@ -355,6 +381,8 @@ class PagedKVCache:
         take over the same row share until one appends (``append`` copies the page)."""
         core, index = self._core, self._indices(indices, self._rows.shape)
         core._eager()
+        core.ready()
+        core.pending = True
         _lib.check(_lib.load().tsattn_pages4_reorder(core.tables, len(index), self._rows_at, index.ctypes.data),
                    "page table")
         core.apply()
@@ -374,6 +402,8 @@ class PagedKVCache:
         core = self._core
         if num_pages is None:
             core._eager()
+            core.ready()
+            core.pending = True
             _lib.check(_lib.load().tsattn_pages4_compact(core.tables, *core.out), "page table")
             core.apply()
         else:
@@ -422,6 +452,7 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
         raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
     import torch
 
+    core.ready()
     lens, lens_at = cache._lens()
     rows = heads // core.heads * steps
     if (rows > 32 and dim <= 128 and lens.min() >= steps

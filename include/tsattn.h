@@ -640,6 +640,8 @@ int tsattn_pages4_compact(tsattn_pages4_host *h, int32_t *src, int32_t *dst, int
  * to pages dst[i] of the pool `to` (the same or another; n of them, or none), and the
  * changed entries to the device's table [rows, columns].  Destinations must differ,
  * and within one pool no page may be both read and written: TSATTN_ERR_INVALID.
+ * After an error the entries are still to be sent, and the copies to be made: the same
+ * call may be made again, as long as no other has changed h.
  */
 int tsattn_pages4_apply(tsattn_pages4_host *h, int32_t *table, const void *from, int64_t from_pages, void *to,
                         int64_t to_pages, size_t page_bytes, int32_t n, const int32_t *src, const int32_t *dst,
