@@ -15,12 +15,14 @@ prompt's many rows of 16 bits the pages are dequantised once and attended as arr
 Page tables and reference counts are the host's; lengths travel with each launch.
 Calls captured into a HIP graph replay the positions, and the pages, that they were
 captured at, so a replay is for as long as its rows keep both; a call that takes or
-copies a page is refused there.
+copies a page is refused there.  Calls on a cache and on its ``rows`` from several
+threads take turns.
 """
 
 from __future__ import annotations
 
 import math
+import threading
 
 import numpy as np
 
@@ -79,6 +81,7 @@ class _Pages:
         import torch
 
         self.heads, self.dim, self.page_size, self.device = heads, dim, page_size, dev
+        self.lock = threading.RLock()  # (a call's changes, its update and its launch belong together)
         self.page_bytes = int(_lib.load().tsattn_pages4_page_bytes(heads, page_size, dim))
         if not self.page_bytes:
             raise NotImplementedError("paged caches take head dims 32, 64, 128 and 256, up to 4096 heads and "
@@ -265,30 +268,31 @@ class PagedKVCache:
         """
         self._check(key, value)
         core, steps = self._core, key._data.shape[2]
-        lens, lens_at = self._lens()
-        most = int(lens.max()) + steps
-        if steps == 0 or most > self.max_seq_len:
-            raise ValueError(f"cache capacity {self.max_seq_len} exceeded or empty append")
-        cos = sin = None
-        if rotary_base is not None:
-            if rotary_base <= 0 or not math.isfinite(rotary_base):
-                raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
-            cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
-        k, v = (_rows(t if t.dtype == self.dtype else t.to(self.dtype)) for t in (key._data, value._data))
-        core._eager(self._rows, steps)
-        core.ready()
-        try:
-            core.grow(len(lens), self._rows_at, steps)
-            core.apply()
-            _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
-                              _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
-        except BaseException:
-            core.take_back(self._rows, steps)
-            raise
-        if self._whole:
-            core.lengths += steps
-        else:
-            core.lengths[self._rows] += steps
+        with core.lock:
+            lens, lens_at = self._lens()
+            most = int(lens.max()) + steps
+            if steps == 0 or most > self.max_seq_len:
+                raise ValueError(f"cache capacity {self.max_seq_len} exceeded or empty append")
+            cos = sin = None
+            if rotary_base is not None:
+                if rotary_base <= 0 or not math.isfinite(rotary_base):
+                    raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
+                cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
+            k, v = (_rows(t if t.dtype == self.dtype else t.to(self.dtype)) for t in (key._data, value._data))
+            core._eager(self._rows, steps)
+            core.ready()
+            try:
+                core.grow(len(lens), self._rows_at, steps)
+                core.apply()
+                _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
+                                  _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
+            except BaseException:
+                core.take_back(self._rows, steps)
+                raise
+            if self._whole:
+                core.lengths += steps
+            else:
+                core.lengths[self._rows] += steps
 
     def _lens(self):
         """The rows' lengths and their address."""
@@ -316,17 +320,18 @@ class PagedKVCache:
         import torch
 
         core = self._core
-        core.ready()
-        lens, lens_at = self._lens()
-        if last is not None and not 0 < last <= lens.min():
-            raise ValueError("the last positions read must be between one and the shortest row's length")
-        steps = int(lens.max()) if last is None else last
-        first = np.zeros_like(lens) if last is None else lens - np.int32(last)
-        k = torch.empty((len(lens), core.heads, steps, core.dim), dtype=self.dtype, device=core.pool.device)
-        v = torch.empty_like(k)
-        if steps:
-            _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
-                              _view(k), _view(v), self._rows_at, lens_at, first.ctypes.data), "paged read")
+        with core.lock:
+            core.ready()
+            lens, lens_at = self._lens()
+            if last is not None and not 0 < last <= lens.min():
+                raise ValueError("the last positions read must be between one and the shortest row's length")
+            steps = int(lens.max()) if last is None else last
+            first = np.zeros_like(lens) if last is None else lens - np.int32(last)
+            k = torch.empty((len(lens), core.heads, steps, core.dim), dtype=self.dtype, device=core.pool.device)
+            v = torch.empty_like(k)
+            if steps:
+                _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
+                                  _view(k), _view(v), self._rows_at, lens_at, first.ctypes.data), "paged read")
         return Tensor._leaf(k, core.device), Tensor._leaf(v, core.device)
 
     # -- rows and pages -------------------------------------------------------
@@ -354,15 +359,17 @@ class PagedKVCache:
 
     def reset(self) -> None:
         """Every row empty, its pages given back."""
-        self._core.ready()
-        self._core.cut(self._rows, self._rows_at, np.zeros_like(self._rows))
+        with self._core.lock:
+            self._core.ready()
+            self._core.cut(self._rows, self._rows_at, np.zeros_like(self._rows))
 
     def free(self, indices) -> None:
         """These rows empty, their pages given back."""
         rows = self._rows[np.unique(self._indices(indices, None))]
         if len(rows):
-            self._core.ready()
-            self._core.cut(rows, rows.ctypes.data, np.zeros_like(rows))
+            with self._core.lock:
+                self._core.ready()
+                self._core.cut(rows, rows.ctypes.data, np.zeros_like(rows))
 
     def truncate(self, length) -> None:
         """Cut every row to ``length`` positions, or to a length of its own (a sequence of them);
@@ -373,26 +380,29 @@ class PagedKVCache:
         lens = want.astype(np.int32)
         if (lens != want).any():
             raise ValueError("truncate length must be between zero and the current length")
-        self._core.ready()
-        self._core.cut(self._rows, self._rows_at, lens if lens.shape else np.full_like(self._rows, lens))
+        with self._core.lock:
+            self._core.ready()
+            self._core.cut(self._rows, self._rows_at, lens if lens.shape else np.full_like(self._rows, lens))
 
     def reorder(self, indices) -> None:
         """Row i becomes row ``indices[i]``, sharing its pages: no keys or values move.  Rows that
         take over the same row share until one appends (``append`` copies the page)."""
         core, index = self._core, self._indices(indices, self._rows.shape)
-        core._eager()
-        core.ready()
-        core.pending = True
-        _lib.check(_lib.load().tsattn_pages4_reorder(core.tables, len(index), self._rows_at, index.ctypes.data),
-                   "page table")
-        core.apply()
+        with core.lock:
+            core._eager()
+            core.ready()
+            core.pending = True
+            _lib.check(_lib.load().tsattn_pages4_reorder(core.tables, len(index), self._rows_at, index.ctypes.data),
+                       "page table")
+            core.apply()
 
     def copy(self, num_pages: int | None = None) -> "PagedKVCache":
         """A cache of these rows with a pool of its own (``num_pages``, by default as many as this
         one has), its pages in use side by side; rows that share pages share them there."""
         other = object.__new__(PagedKVCache)
         other.dtype, other.max_seq_len, other._code = self.dtype, self.max_seq_len, self._code
-        other._core = self._core.clone(self._rows, self._pool_size(num_pages))
+        with self._core.lock:
+            other._core = self._core.clone(self._rows, self._pool_size(num_pages))
         other._select()
         return other
 
@@ -400,16 +410,17 @@ class PagedKVCache:
         """Move the pages in use to the front of the pool, and with ``num_pages`` into a pool of that
         size (smaller or larger); returns how many are in use."""
         core = self._core
-        if num_pages is None:
-            core._eager()
-            core.ready()
-            core.pending = True
-            _lib.check(_lib.load().tsattn_pages4_compact(core.tables, *core.out), "page table")
-            core.apply()
-        else:
-            core.__dict__.update(core.clone(np.arange(len(core.lengths), dtype=np.int32),
-                                            self._pool_size(num_pages)).__dict__)
-        return self.pages_in_use
+        with core.lock:
+            if num_pages is None:
+                core._eager()
+                core.ready()
+                core.pending = True
+                _lib.check(_lib.load().tsattn_pages4_compact(core.tables, *core.out), "page table")
+                core.apply()
+            else:
+                new = core.clone(np.arange(len(core.lengths), dtype=np.int32), self._pool_size(num_pages))
+                core.__dict__.update({**new.__dict__, "lock": core.lock})
+            return self.pages_in_use
 
     def _pool_size(self, num_pages) -> int:
         """``num_pages``, by default as many as there are; refused if fewer than are in use here."""
@@ -452,24 +463,25 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
         raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
     import torch
 
-    core.ready()
-    lens, lens_at = cache._lens()
-    rows = heads // core.heads * steps
-    if (rows > 32 and dim <= 128 and lens.min() >= steps
-            and not _reads_codes(rows, core.heads, dim, q.dtype == torch.float32, lens)):
-        return _prompt(query, cache, lens, is_causal, multiplier, rotary_base)
-    q = _rows(q)
-    cos = sin = None
-    if rotary_base is not None:
-        cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, dim, q.dtype, q.device,
-                                                      max(int(lens.max()), steps)))
-    out = torch.empty((b, heads, steps, dim), dtype=q.dtype, device=q.device)
-    lib, code = _lib.load(), cache._code
-    nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, lens_at)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.check(launch(core.device, lib.tsattn_pages4_attend, core.desc, code, b, heads, steps, multiplier,
-                      int(is_causal), _view(q), _view(out), cache._rows_at, lens_at, cos, sin,
-                      None if ws is None else ws.data_ptr(), nbytes), "paged attention")
+    with core.lock:
+        core.ready()
+        lens, lens_at = cache._lens()
+        rows = heads // core.heads * steps
+        if (rows > 32 and dim <= 128 and lens.min() >= steps
+                and not _reads_codes(rows, core.heads, dim, q.dtype == torch.float32, lens)):
+            return _prompt(query, cache, lens, is_causal, multiplier, rotary_base)
+        q = _rows(q)
+        cos = sin = None
+        if rotary_base is not None:
+            cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, dim, q.dtype, q.device,
+                                                          max(int(lens.max()), steps)))
+        out = torch.empty((b, heads, steps, dim), dtype=q.dtype, device=q.device)
+        lib, code = _lib.load(), cache._code
+        nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, lens_at)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        _lib.check(launch(core.device, lib.tsattn_pages4_attend, core.desc, code, b, heads, steps, multiplier,
+                          int(is_causal), _view(q), _view(out), cache._rows_at, lens_at, cos, sin,
+                          None if ws is None else ws.data_ptr(), nbytes), "paged attention")
     return Tensor._from_op(out, (query,), None, "paged_attention")
 
 
