@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import numpy as np
 
@@ -429,6 +430,7 @@ def decode_int8_cache(query: Tensor, cache, *, is_causal: bool, causal_offset: i
 
 
 _ROPE_TABLES: dict = {}
+_ROPE_LOCK = threading.Lock()
 _OUTGROWN: list = []  # shorter tables: a captured launch may read them still (together no longer than the newest)
 
 
@@ -452,15 +454,19 @@ def rope_tables(base: float, dim: int, dtype, dev, length: int):
     have = _ROPE_TABLES.get(key)
     if have is not None and have[0].shape[0] >= length:
         return have
-    n = max(length, 2 * (have[0].shape[0] if have is not None else 0), 256)
-    freqs = base ** (-(np.arange(0, dim, 2, dtype=np.float32)) / np.float32(dim))
-    angles = np.arange(0, n, dtype=np.float32)[:, None] * freqs[None, :]
-    made = tuple(torch.from_numpy(np.ascontiguousarray(f(angles))).to(device=dev, dtype=dtype)
-                 for f in (np.cos, np.sin))
-    if have is not None:
-        _OUTGROWN.append(have)
-    _ROPE_TABLES[key] = made
-    return made
+    with _ROPE_LOCK:  # (a table that another thread replaced meanwhile would not be kept)
+        have = _ROPE_TABLES.get(key)
+        if have is not None and have[0].shape[0] >= length:
+            return have
+        n = max(length, 2 * (have[0].shape[0] if have is not None else 0), 256)
+        freqs = base ** (-(np.arange(0, dim, 2, dtype=np.float32)) / np.float32(dim))
+        angles = np.arange(0, n, dtype=np.float32)[:, None] * freqs[None, :]
+        made = tuple(torch.from_numpy(np.ascontiguousarray(f(angles))).to(device=dev, dtype=dtype)
+                     for f in (np.cos, np.sin))
+        if have is not None:
+            _OUTGROWN.append(have)
+        _ROPE_TABLES[key] = made
+        return made
 
 
 def _rope_launch(x, out, offset: int, base: float, dim: int, inverse: bool, dev) -> None:
