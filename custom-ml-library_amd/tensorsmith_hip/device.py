@@ -222,3 +222,27 @@ def launch(dev: Device, function, *args) -> int:
         return function(*args, stream)
     with _cuda().device(dev.index):
         return function(*args, stream)
+
+
+def follow(dev: Device, last: int | None = None, *arrays) -> int:
+    """``dev``'s current stream, made to wait for what is queued on the stream ``last``: for work on
+    ``arrays`` that more than one stream uses.  Under capture nothing waits, and ``last`` stays: a
+    graph's replays are ordered by who replays them."""
+    stream = current_stream(dev)
+    if last is None or stream == last:
+        return stream
+    cuda = _cuda()
+    with cuda.device(dev.index):
+        if cuda.is_current_stream_capturing():
+            return last
+        before, event = cuda.ExternalStream(last, device=dev.index), cuda.Event()
+        with cuda.stream(before):
+            if cuda.is_current_stream_capturing():
+                raise RuntimeError("the stream of the cache's last call is being captured")
+            event.record()
+        now = cuda.current_stream()
+        now.wait_event(event)
+        for array in arrays:
+            if array.is_cuda:
+                array.record_stream(now)
+    return stream

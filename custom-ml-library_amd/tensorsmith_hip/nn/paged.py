@@ -15,8 +15,10 @@ prompt's many rows of 16 bits the pages are dequantised once and attended as arr
 Page tables and reference counts are the host's; lengths travel with each launch.
 Calls captured into a HIP graph replay the positions, and the pages, that they were
 captured at, so a replay is for as long as its rows keep both; a call that takes or
-copies a page is refused there.  Calls on a cache and on its ``rows`` from several
-threads take turns.
+copies a page is refused there.  Calls on a cache and on its ``rows`` follow each
+other: from several threads they take turns, and on another stream than the last
+call's they wait for that stream (which has to live as long).  Replays are ordered by
+who replays them.
 """
 
 from __future__ import annotations
@@ -28,7 +30,7 @@ import numpy as np
 
 from .. import _lib
 from ..device import device as parse_device
-from ..device import launch
+from ..device import follow, launch
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
 from .attention import _dtype_code, _rope_rows, rope_tables, scaled_dot_product_attention
 
@@ -98,6 +100,7 @@ class _Pages:
         self.host, self.lengths, self.refs = part["host"].reshape(rows, columns), part["lengths"], part["refs"]
         self.stack, self.shown, self.copies = part["stack"], part["shown"], part["copies"]
         self.lengths_at = where["lengths"]
+        self.stream = follow(dev)  # of the last call: a call on another waits for it
         self.pending = False  # whether page copies or entries may be left to bring to the device
         self.out = where["src"], where["dst"], where["copies"]
         self.tables = _lib.Pages4Host(rows, columns, page_size, num_pages, where["host"], where["lengths"], where["refs"],
@@ -121,8 +124,10 @@ class _Pages:
         return self.tables.free
 
     def ready(self) -> None:
-        """What an earlier call's page changes left to do, if it failed before they were on the device.
-        Every call begins with it, so nothing is taken, given back or read in between."""
+        """Every call begins with it: what was queued before on another stream comes first (a page that
+        is given back and taken again may still be read there), and what an earlier call's page
+        changes left to do, if it failed before they were on the device."""
+        self.stream = follow(self.device, self.stream, self.pool, self.table)
         if self.pending:
             if self.copies[0] or self.tables.n_changed:
                 self._eager()
