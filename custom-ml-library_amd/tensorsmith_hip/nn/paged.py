@@ -14,8 +14,8 @@ prompt's many rows of 16 bits the pages are dequantised once and attended as arr
 
 Page tables and reference counts are the host's; lengths travel with each launch.
 Calls captured into a HIP graph replay the positions, and the pages, that they were
-captured at, so a replay is for as long as its rows keep both; a call that takes or
-copies a page is refused there.  Calls on a cache and on its ``rows`` follow each
+captured at, so a replay is for as long as its rows keep both; a call that takes,
+copies or gives back a page is refused there.  Calls on a cache and on its ``rows`` follow each
 other: from several threads they take turns, and on another stream than the last
 call's they wait for that stream (which has to live as long).  Replays are ordered by
 who replays them.
@@ -166,7 +166,14 @@ class _Pages:
         _lib.check(_lib.load().tsattn_pages4_grow(self.tables, n, rows, steps, *self.out), "page table")
 
     def cut(self, rows, rows_at: int, lengths) -> None:
-        """``rows`` (at an address) end at ``lengths``; pages wholly past them are given back."""
+        """``rows`` (at an address) end at ``lengths``; pages wholly past them are given back (under
+        capture refused: the captured calls would go on with them)."""
+        import torch
+
+        if torch.cuda.is_current_stream_capturing():
+            pages = -(-self.lengths[rows] // self.page_size)
+            if ((lengths >= 0) & (-(-lengths // self.page_size) < pages)).any():
+                self._eager()
         _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows_at, lengths.ctypes.data), "page table")
 
     def take_back(self, rows, steps: int) -> None:
@@ -175,7 +182,7 @@ class _Pages:
         held = ((self.host[rows] >= 0).sum(1) * self.page_size).astype(np.int32)
         lens = self.lengths[rows]
         self.lengths[rows] = np.maximum(lens, np.minimum(lens + np.int32(steps), held))
-        self.cut(rows, rows.ctypes.data, lens)
+        _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows.ctypes.data, lens.ctypes.data), "page table")
 
     def clone(self, rows, num_pages: int) -> "_Pages":
         """The rows with pages of their own, in a pool of ``num_pages``."""

@@ -119,3 +119,25 @@ def test_nothing_waits_under_capture(streams):
     streams.capturing = set()
     cache.get()
     assert streams.order[2:] == [("wait", 0x30, 0x10), ("read", 0x30)]
+
+
+def test_a_captured_call_keeps_its_pages(streams):
+    """Cuts that give pages back are refused under capture and change nothing; shorter ones are not."""
+    cache = nn.PagedKVCache(3, 2, 32, 100, device="hip", page_size=32)
+    cache.append(_rows([[1.0] * 40] * 3), _rows([[1.0] * 40] * 3))
+    cache.reorder([0, 0, 2])
+    cache.free([2])
+    table, refs = cache._core.host.copy(), cache._core.refs.copy()
+    streams.capturing = {0x10}
+    for call in (cache.reset, lambda: cache.free([0]), lambda: cache.truncate([40, 32, 0]), lambda: cache.rows([1]).reset()):
+        with pytest.raises(RuntimeError, match="cannot change while a graph"):
+            call()
+    assert cache.lengths == (40, 40, 0) and (cache._core.host == table).all() and (cache._core.refs == refs).all()
+    cache.truncate([33, 40, 0]), cache.free([2]), cache.free([])
+    assert cache.lengths == (33, 40, 0)
+    for length in (41, -1):
+        with pytest.raises(ValueError, match="truncate length"):
+            cache.truncate([33, length, 0])
+    streams.capturing = set()
+    cache.reset()
+    assert cache.pages_in_use == 0
