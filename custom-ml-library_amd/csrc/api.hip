@@ -631,12 +631,24 @@ tsattn::View seq_view(const tsattn_view *v, int32_t i0, int32_t dtype) {
   return x;
 }
 
-// The plan of sequences i0 .. of a call (m of them), and the scratch that they take.
-size_t plan4(tsattn::Attend4 *a, int32_t dtype, int32_t n, int32_t i0, const int32_t *lens) {
-  a->n = n - i0 < tsattn::kSeqs ? n - i0 : tsattn::kSeqs;
-  tsattn::plan_attend4(a, dtype, lens + i0);
-  return a->splits == 1 ? 0
-                        : static_cast<size_t>(a->n) * a->p.heads * a->splits * a->rows * (a->p.dim + 2) * sizeof(float);
+// The next launch of an attention over n sequences of `rows` rows a KV head: from
+// sequence i0 and row `first`, how many of them, their plan, and the scratch that they
+// take.  Scratch goes by the longest sequence of a launch, so where it would pass 4 GiB a
+// launch takes fewer sequences, then one sequence's rows in parts.
+constexpr size_t kMostScratch = size_t(1) << 32;
+size_t plan4(tsattn::Attend4 *a, int32_t dtype, int32_t n, int32_t i0, int32_t rows, int32_t first,
+             const int32_t *lens) {
+  a->n = first ? 1 : n - i0 < tsattn::kSeqs ? n - i0 : tsattn::kSeqs;
+  a->first = first, a->rows = rows - first;
+  for (;;) {
+    tsattn::plan_attend4(a, dtype, lens + i0);
+    const size_t need =
+        a->splits == 1 ? 0
+                       : static_cast<size_t>(a->n) * a->p.heads * a->splits * a->rows * (a->p.dim + 2) * sizeof(float);
+    if (need <= kMostScratch || (a->n == 1 && a->rows <= 32)) return need;
+    if (a->n > 1) a->n = (a->n + 1) / 2;
+    else a->rows = (a->rows / 2 + 31) / 32 * 32;
+  }
 }
 
 // The host's side of a paged cache, and n different rows of it.
@@ -1127,12 +1139,13 @@ size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int
     if (lens[i] < 0 || lens[i] > tsattn::kLongest) return 0;
   tsattn::Attend4 a{};
   a.p.heads = p->heads, a.p.dim = p->dim;
-  a.rows = heads_q / p->heads * len_q;
+  const int32_t rows = heads_q / p->heads * len_q;
   size_t most = 0;
-  for (int32_t i0 = 0; i0 < n; i0 += tsattn::kSeqs) {  // (groups of sequences follow each other in it)
-    const size_t need = plan4(&a, dtype, n, i0, lens);
-    most = need > most ? need : most;
-  }
+  for (int32_t i0 = 0; i0 < n; i0 += a.n)  // (launches follow each other in it)
+    for (int32_t r0 = 0; r0 < rows; r0 += a.rows) {
+      const size_t need = plan4(&a, dtype, n, i0, rows, r0, lens);
+      most = need > most ? need : most;
+    }
   return most;
 }
 
@@ -1158,7 +1171,7 @@ int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
     return fail(TSATTN_ERR_INVALID, "paged attention workspace too small: %zu < %zu bytes", workspace_bytes, need);
   a.ws = static_cast<float *>(workspace);
   a.cos = cos, a.sin = sin;
-  a.rep = heads_q / p->heads, a.len_q = len_q, a.rows = static_cast<int>(r);
+  a.rep = heads_q / p->heads, a.len_q = len_q;
   a.by_len_q = tsattn::make_fastdiv(len_q);
   a.causal = is_causal ? 1 : 0;
   const float sl = static_cast<float>(scale) * tsattn::kLog2e;
@@ -1166,12 +1179,13 @@ int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32
   a.sl = sl == 0.f ? 1.f : fabsf(sl);
   if (!isfinite(a.sl)) return fail(TSATTN_ERR_INVALID, "attention scale must be finite");
   g_last_path = 3;
-  for (int32_t i0 = 0; i0 < n && !rc; i0 += tsattn::kSeqs) {
-    plan4(&a, dtype, n, i0, lens);
-    take_seqs(&a.s, n, i0, rows, lens);
-    a.q = seq_view(q, i0, dtype), a.o = seq_view(out, i0, dtype);
-    rc = hip_status(tsattn::launch_attend4(a, dtype, static_cast<hipStream_t>(stream)), "paged attention launch");
-  }
+  for (int32_t i0 = 0; i0 < n && !rc; i0 += a.n)
+    for (int32_t r0 = 0; r0 < r && !rc; r0 += a.rows) {
+      plan4(&a, dtype, n, i0, static_cast<int32_t>(r), r0, lens);
+      take_seqs(&a.s, i0 + a.n, i0, rows, lens);
+      a.q = seq_view(q, i0, dtype), a.o = seq_view(out, i0, dtype);
+      rc = hip_status(tsattn::launch_attend4(a, dtype, static_cast<hipStream_t>(stream)), "paged attention launch");
+    }
   return rc;
 }
 

@@ -119,9 +119,9 @@ __global__ __launch_bounds__(64 * NWV, (G == 8 && (WIDE || std::is_same_v<T, flo
   const int rl = WIDE ? c : c / G, grp = c % G;  // the lane's row in its column block, its group
   const int len = a.s.len[b], trow = a.s.row[b];
   const int hk = a.blocks == 1 ? blockIdx.x : blockIdx.x / a.blocks;
-  const int row0 = (blockIdx.x - hk * a.blocks) * ROWS;
+  const int row0 = a.first + (blockIdx.x - hk * a.blocks) * ROWS;
   const int begin = split * a.split;
-  const int live_rows = min(ROWS, a.rows - row0);
+  const int live_rows = min(ROWS, a.first + a.rows - row0);
   auto out_row = [&](int r) __attribute__((always_inline)) {
     const int rr = fdiv(row0 + r, a.by_len_q), qi = row0 + r - rr * a.len_q;
     return static_cast<T *>(const_cast<void *>(a.o.data)) + b * a.o.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.o.s1 +
@@ -428,7 +428,8 @@ __global__ __launch_bounds__(64 * NWV, (G == 8 && (WIDE || std::is_same_v<T, flo
         if (lane * PER < MD) {
           const int d = d0 + PER * lane;
           if (a.splits > 1) {
-            float *to = a.ws + ((static_cast<int64_t>(b * a.p.heads + hk) * a.splits + split) * a.rows + row0 + r) * (D + 2);
+            float *to = a.ws + ((static_cast<int64_t>(b * a.p.heads + hk) * a.splits + split) * a.rows + row0 - a.first + r) *
+                                   (D + 2);
 #pragma unroll
             for (int i = 0; i < PER; ++i) to[d + i] = sum[i];
             if (d == 0) to[D] = M, to[D + 1] = total;
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(64) void attend4_merge_kernel(Attend4 a) {
       for (int i = 0; i < PER; ++i) acc[i] = fmaf(x[u][i], e, acc[i]);
     }
   }
-  const int rr = fdiv(r, a.by_len_q), qi = r - rr * a.len_q;
+  const int rr = fdiv(a.first + r, a.by_len_q), qi = a.first + r - rr * a.len_q;
   T *out = static_cast<T *>(const_cast<void *>(a.o.data)) + b * a.o.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.o.s1 +
            qi * a.o.s2;
 #pragma unroll

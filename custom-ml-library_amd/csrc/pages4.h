@@ -118,7 +118,7 @@ struct Attend4 {
   View q, o;
   float *ws;
   const void *cos, *sin;  // rotate the queries; or NULL
-  int n, rep, len_q, rows, causal;
+  int n, rep, len_q, first, rows, causal;  // rows: of a KV head, rep len_q in all, from the launch's first
   int split, splits;      // positions a split (a multiple of 32), splits of the longest sequence
   int wide;                    // whether a column is a row, not a group of one
   int columns, waves, blocks;  // column blocks (1 or 2) and waves of a workgroup; workgroups a KV head's rows take

@@ -571,7 +571,10 @@ int tsattn_pages4_read(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t
                        const tsattn_view *v, const int32_t *rows, const int32_t *lens, const int32_t *first,
                        void *stream);
 
-/* Bytes of scratch tsattn_pages4_attend needs (0: none, or sizes it does not take). */
+/*
+ * Bytes of scratch tsattn_pages4_attend needs (0: none, or sizes it does not take): at
+ * most 4 GiB, as it takes sequences, then a sequence's rows, in parts beyond.
+ */
 size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q,
                                       int32_t len_q, const int32_t *lens);
 
