@@ -651,6 +651,15 @@ size_t plan4(tsattn::Attend4 *a, int32_t dtype, int32_t n, int32_t i0, int32_t r
   }
 }
 
+bool attend4_sizes_ok(const tsattn_pages4 *p, int32_t n, int32_t heads_q, int32_t len_q, const int32_t *lens) {
+  if (!p || !lens || n <= 0 || heads_q <= 0 || len_q <= 0 || !pages4_sizes_ok(p->heads, p->page_size, p->dim) ||
+      heads_q % p->heads || static_cast<int64_t>(heads_q / p->heads) * len_q > (1 << 18))
+    return false;
+  for (int32_t i = 0; i < n; ++i)
+    if (lens[i] < 0 || lens[i] > tsattn::kLongest) return false;
+  return true;
+}
+
 // The host's side of a paged cache, and n different rows of it.
 int check_host4(const tsattn_pages4_host *h) {
   if (!h || !h->table || !h->lengths || !h->refs || !h->stack || !h->shown || !h->changed || !h->dirty)
@@ -1132,11 +1141,7 @@ int tsattn_pages4_read(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t
 
 size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q,
                                       int32_t len_q, const int32_t *lens) {
-  if (!p || !lens || n <= 0 || heads_q <= 0 || len_q <= 0 || !pages4_sizes_ok(p->heads, p->page_size, p->dim) ||
-      heads_q % p->heads || static_cast<int64_t>(heads_q / p->heads) * len_q > (1 << 18))
-    return 0;
-  for (int32_t i = 0; i < n; ++i)
-    if (lens[i] < 0 || lens[i] > tsattn::kLongest) return 0;
+  if (!attend4_sizes_ok(p, n, heads_q, len_q, lens)) return 0;
   tsattn::Attend4 a{};
   a.p.heads = p->heads, a.p.dim = p->dim;
   const int32_t rows = heads_q / p->heads * len_q;
@@ -1147,6 +1152,18 @@ size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int
       most = need > most ? need : most;
     }
   return most;
+}
+
+int tsattn_pages4_attend_plan(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q, int32_t len_q,
+                              const int32_t *lens, tsattn_pages4_plan *plan) {
+  if (!plan || !attend4_sizes_ok(p, n, heads_q, len_q, lens) ||
+      (dtype != TSATTN_F32 && dtype != TSATTN_F16 && dtype != TSATTN_BF16))
+    return fail(TSATTN_ERR_INVALID, "paged attention has no plan for these sizes");
+  tsattn::Attend4 a{};
+  a.p.heads = p->heads, a.p.dim = p->dim;
+  plan4(&a, dtype, n, 0, heads_q / p->heads * len_q, 0, lens);
+  *plan = tsattn_pages4_plan{a.n, a.rows, a.splits, a.split, a.waves, a.columns, a.wide};
+  return TSATTN_OK;
 }
 
 int tsattn_pages4_attend(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q, int32_t len_q,

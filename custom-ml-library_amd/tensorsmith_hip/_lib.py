@@ -126,6 +126,12 @@ class Pages4(ctypes.Structure):
     ]
 
 
+class Pages4Plan(ctypes.Structure):
+    """``tsattn_pages4_plan``: how a paged attention is run."""
+
+    _fields_ = [(name, c_int32) for name in ("sequences", "rows", "splits", "split", "waves", "columns", "wide")]
+
+
 class Pages4Host(ctypes.Structure):
     """``tsattn_pages4_host``: a paged cache's tables on the host."""
 
@@ -254,6 +260,8 @@ SIGNATURES = {
     ),
     "tsattn_pages4_attend_workspace": (
         c_size_t, [_P4, c_int32, c_int32, c_int32, c_int32, c_void_p]),
+    "tsattn_pages4_attend_plan": (
+        c_int, [_P4, c_int32, c_int32, c_int32, c_int32, c_void_p, POINTER(Pages4Plan)]),
     "tsattn_pages4_attend": (
         c_int,
         [_P4, c_int32, c_int32, c_int32, c_int32, c_double, c_int32, _PV, _PV, c_void_p, c_void_p,

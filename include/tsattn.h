@@ -579,6 +579,18 @@ size_t tsattn_pages4_attend_workspace(const tsattn_pages4 *p, int32_t dtype, int
                                       int32_t len_q, const int32_t *lens);
 
 /*
+ * How such an attention is run, without running it (for tests and measurements): its
+ * first launch's sequences, rows per KV head and splits, positions a split, waves and
+ * column blocks of a workgroup, and whether a column is a row.  Sizes that the attention
+ * does not take: TSATTN_ERR_INVALID.
+ */
+typedef struct tsattn_pages4_plan {
+  int32_t sequences, rows, splits, split, waves, columns, wide;
+} tsattn_pages4_plan;
+int tsattn_pages4_attend_plan(const tsattn_pages4 *p, int32_t dtype, int32_t n, int32_t heads_q, int32_t len_q,
+                              const int32_t *lens, tsattn_pages4_plan *plan);
+
+/*
  * Attention (src/tensorsmith/nn/attention.py:102-145, :175-198) of q [n, heads_q,
  * len_q, dim] over the lens[i] cached positions of each sequence, read in 4 bits.
  * The queries' own positions are the last len_q: with is_causal query t sees
