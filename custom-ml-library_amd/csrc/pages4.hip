@@ -62,10 +62,19 @@ __device__ __forceinline__ uint32_t most_of(const u32x4 (&raw)[sizeof(T) / 2]) {
 // (x has at most 11 significant bits, the point times s 9), so the conversion's
 // rounding (to nearest, ties to even, saturating) decides as the real quotient does.
 // fp32 quotients are truncated with a sticky last bit instead, so that none rounds
-// onto one.
+// onto one.  The reciprocal's low part has its bits while it is a normal number, for
+// scales under 2^100: larger ones and their values come down by 2^64 first, exactly (what
+// falls out of fp32 there has code 0 either way).
 template <typename T>
-__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float s) {
+__device__ __forceinline__ uint32_t codes_of(float (&x)[8], float s) {
 #pragma clang fp contract(off)
+  if constexpr (most_scale<T>() > 0x1p64f) {
+    if (s > 0x1p64f) {
+      s *= 0x1p-64f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= 0x1p-64f;
+    }
+  }
   const float rc = __builtin_amdgcn_rcpf(s), rl = __builtin_fmaf(-rc, s, 1.f) * rc;
   float q[8];
 #pragma unroll
