@@ -224,6 +224,15 @@ def launch(dev: Device, function, *args) -> int:
         return function(*args, stream)
 
 
+def capturing(dev: Device) -> bool:
+    """Whether ``dev``'s current stream is being captured into a graph."""
+    cuda = _cuda()
+    if cuda.current_device() == dev.index:
+        return cuda.is_current_stream_capturing()
+    with cuda.device(dev.index):
+        return cuda.is_current_stream_capturing()
+
+
 def follow(dev: Device, last: int | None = None, *arrays) -> int:
     """``dev``'s current stream, made to wait for what is queued on the stream ``last``: for work on
     ``arrays`` that more than one stream uses.  Under capture nothing waits, and ``last`` stays: a

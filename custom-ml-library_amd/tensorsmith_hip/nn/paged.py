@@ -30,7 +30,7 @@ import numpy as np
 
 from .. import _lib
 from ..device import device as parse_device
-from ..device import follow, launch
+from ..device import capturing, follow, launch
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
 from .attention import _dtype_code, _rope_rows, rope_tables, scaled_dot_product_attention
 
@@ -149,9 +149,7 @@ class _Pages:
     def _eager(self, rows=None, steps: int = 0) -> None:
         """Refuses page changes under capture: a captured call's pages would be the host's at once and
         the device's with each replay.  With ``rows``: only if they need other pages for ``steps``."""
-        import torch
-
-        if not torch.cuda.is_current_stream_capturing():
+        if not capturing(self.device):
             return
         if rows is not None:
             lens = self.lengths[rows]
@@ -169,9 +167,7 @@ class _Pages:
     def cut(self, rows, rows_at: int, lengths) -> None:
         """``rows`` (at an address) end at ``lengths``; pages wholly past them are given back (under
         capture refused: the captured calls would go on with them)."""
-        import torch
-
-        if torch.cuda.is_current_stream_capturing():
+        if capturing(self.device):
             pages = -(-self.lengths[rows] // self.page_size)
             if ((lengths >= 0) & (-(-lengths // self.page_size) < pages)).any():
                 self._eager()

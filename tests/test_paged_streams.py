@@ -15,6 +15,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from test_paged_host import _rows, memory  # noqa: E402, F401
+import tensorsmith_hip as ts  # noqa: E402
 from tensorsmith_hip import nn  # noqa: E402
 
 D = importlib.import_module("tensorsmith_hip.device")
@@ -141,3 +142,28 @@ def test_a_captured_call_keeps_its_pages(streams):
     streams.capturing = set()
     cache.reset()
     assert cache.pages_in_use == 0
+
+
+def test_another_devices_capture_is_not_this_ones(memory):  # noqa: F811
+    """Page changes go by the stream of the cache's device, whichever device is current."""
+    state = {"device": 0, "captured": None}
+
+    @contextmanager
+    def on(device):
+        before, state["device"] = state["device"], device
+        try:
+            yield
+        finally:
+            state["device"] = before
+
+    with patch.object(torch.cuda, "current_device", lambda: state["device"]), patch.object(torch.cuda, "device", on), \
+            patch.object(torch.cuda, "is_current_stream_capturing", lambda: state["device"] == state["captured"]):
+        cache = nn.PagedKVCache(1, 2, 32, 100, device="hip:1")
+        rows = lambda n: ts.Tensor(_rows([[1.0] * n])._data, device="hip:1")  # noqa: E731
+        state["captured"] = 0
+        cache.append(rows(40), rows(40))
+        cache.reset()
+        state["captured"] = 1
+        for call in (lambda: cache.append(rows(40), rows(40)), cache.compact, cache.copy, lambda: cache.reorder([0])):
+            with pytest.raises(RuntimeError, match="cannot change while a graph"):
+                call()
