@@ -31,7 +31,7 @@ from ctypes import POINTER, c_char_p, c_double, c_int, c_int32, c_int64, c_size_
 import numpy as np
 import torch
 
-ABI_VERSION = 10
+ABI_VERSION = 9
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 MASK_NONE, MASK_BOOL, MASK_ADDITIVE = 0, 1, 2
 BOOL_CODE = 4
@@ -109,12 +109,12 @@ def load(path: str | None = None):
     if _lib is not None and path is None:
         return _lib
     lib = ctypes.CDLL(path or library_path())
-    version = lib.tsattn_abi_version()
-    if version != ABI_VERSION:
-        raise RuntimeError(f"libtsattn.so speaks ABI {version}; this binding needs {ABI_VERSION}")
     for name, (res, args) in _SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = res, args
+    version = lib.tsattn_abi_version()
+    if version != ABI_VERSION:
+        raise RuntimeError(f"libtsattn.so speaks ABI {version}; this binding needs {ABI_VERSION}")
     if path is None:
         _lib = lib
     return lib

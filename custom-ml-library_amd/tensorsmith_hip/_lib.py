@@ -16,7 +16,7 @@ from ctypes import POINTER, c_char_p, c_double, c_int, c_int32, c_int64, c_size_
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_native" / "libtsattn.so"
-ABI_VERSION = 10
+ABI_VERSION = 9
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP = 0, 1, 2, 3
 F32, F16, BF16, F64, BOOL, I8 = 0, 1, 2, 3, 4, 5
@@ -310,13 +310,13 @@ def load(path: Path | str | None = None):
                 "(hipcc --offload-arch=gfx950). tensorsmith_hip has no CPU fallback."
             )
         lib = ctypes.CDLL(str(target))
-        version = lib.tsattn_abi_version()  # (before the entry points, which an older library may lack)
-        if version != ABI_VERSION:
-            raise RuntimeError(f"libtsattn ABI {version} != expected {ABI_VERSION}; rebuild")
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
+        version = lib.tsattn_abi_version()
+        if version != ABI_VERSION:
+            raise RuntimeError(f"libtsattn ABI {version} != expected {ABI_VERSION}; rebuild")
         if path is None:
             _lib = lib
         return lib
