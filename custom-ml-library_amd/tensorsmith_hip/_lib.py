@@ -310,13 +310,15 @@ def load(path: Path | str | None = None):
                 "(hipcc --offload-arch=gfx950). tensorsmith_hip has no CPU fallback."
             )
         lib = ctypes.CDLL(str(target))
-        for name, (res, args) in SIGNATURES.items():
-            fn = getattr(lib, name)
-            fn.restype = res
-            fn.argtypes = args
-        version = lib.tsattn_abi_version()
+        version = lib.tsattn_abi_version()  # (before the entry points, which another version may lack)
         if version != ABI_VERSION:
             raise RuntimeError(f"libtsattn ABI {version} != expected {ABI_VERSION}; rebuild")
+        for name, (res, args) in SIGNATURES.items():
+            fn = getattr(lib, name, None)
+            if fn is None:  # (version 9 gained entry points)
+                raise RuntimeError(f"{target} was built before {name}; rebuild")
+            fn.restype = res
+            fn.argtypes = args
         if path is None:
             _lib = lib
         return lib
