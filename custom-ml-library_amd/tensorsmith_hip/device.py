@@ -224,34 +224,35 @@ def launch(dev: Device, function, *args) -> int:
         return function(*args, stream)
 
 
-def capturing(dev: Device) -> bool:
-    """Whether ``dev``'s current stream is being captured into a graph."""
+def state(dev: Device) -> tuple[bool, bool]:
+    """Whether ``dev`` is the current device, and whether its current stream is being captured into a
+    graph."""
     cuda = _cuda()
     if cuda.current_device() == dev.index:
-        return cuda.is_current_stream_capturing()
+        return True, cuda.is_current_stream_capturing()
     with cuda.device(dev.index):
-        return cuda.is_current_stream_capturing()
+        return False, cuda.is_current_stream_capturing()
 
 
-def follow(dev: Device, last: int | None = None, *arrays) -> int:
-    """``dev``'s current stream, made to wait for what is queued on the stream ``last``: for work on
-    ``arrays`` that more than one stream uses.  Under capture nothing waits, and ``last`` stays: a
-    graph's replays are ordered by who replays them."""
+def follow(dev: Device, last: int | None = None, *arrays) -> tuple[int, int]:
+    """``dev``'s current stream, made to wait for what is queued on the stream ``last``, and the stream
+    to wait for the next time: for work on ``arrays`` that several streams use.  Under capture nothing
+    waits, and it stays ``last``: a graph's replays are ordered by who replays them."""
     stream = current_stream(dev)
     if last is None or stream == last:
-        return stream
+        return stream, stream
     cuda = _cuda()
     with cuda.device(dev.index):
         if cuda.is_current_stream_capturing():
-            return last
+            return stream, last
         before, event = cuda.ExternalStream(last, device=dev.index), cuda.Event()
         with cuda.stream(before):
             if cuda.is_current_stream_capturing():
                 raise RuntimeError("the stream of the cache's last call is being captured")
             event.record()
-        now = cuda.current_stream()
-        now.wait_event(event)
+        here = cuda.current_stream()
+        here.wait_event(event)
         for array in arrays:
             if array.is_cuda:
-                array.record_stream(now)
-    return stream
+                array.record_stream(here)
+    return stream, stream

@@ -30,7 +30,7 @@ import numpy as np
 
 from .. import _lib
 from ..device import device as parse_device
-from ..device import capturing, follow, launch
+from ..device import _cuda, follow, state
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
 from .attention import _dtype_code, _rope_rows, rope_tables, scaled_dot_product_attention
 
@@ -89,10 +89,11 @@ class _Pages:
         if not self.page_bytes:
             raise NotImplementedError("paged caches take head dims 32, 64, 128 and 256, up to 4096 heads and "
                                       "pages of 32, 64, .. 4096 positions")
-        # the host's arrays, side by side; src, dst: page copies that a call asks for
+        # the host's arrays, side by side; src, dst: page copies that a call asks for; some: lengths or
+        # positions of a call's rows
         most, entries = max(rows, num_pages), rows * columns
         sizes = {"host": entries, "lengths": rows, "refs": num_pages, "stack": num_pages, "shown": entries,
-                 "changed": entries, "src": most, "dst": most, "copies": 1, "dirty": (entries + 3) // 4}
+                 "changed": entries, "src": most, "dst": most, "copies": 1, "some": rows, "dirty": (entries + 3) // 4}
         memory, at, where, part = np.zeros(sum(sizes.values()), np.int32), 0, {}, {}
         base = memory.ctypes.data
         for name, n in sizes.items():
@@ -100,8 +101,11 @@ class _Pages:
             at += n
         self.host, self.lengths, self.refs = part["host"].reshape(rows, columns), part["lengths"], part["refs"]
         self.stack, self.shown, self.copies = part["stack"], part["shown"], part["copies"]
-        self.lengths_at = where["lengths"]
-        self.stream = follow(dev)  # of the last call: a call on another waits for it
+        self.lengths_at, self.some, self.some_at = where["lengths"], part["some"], where["some"]
+        # the stream of the call at hand, and of the last one that was not captured; where it may change
+        # pages, whether its device is current, and whether it is captured
+        self.now, self.stream = follow(dev)
+        self.here = self.captured = False
         self.pending = False  # whether page copies or entries may be left to bring to the device
         self.out = where["src"], where["dst"], where["copies"]
         self.tables = _lib.Pages4Host(rows, columns, page_size, num_pages, where["host"], where["lengths"], where["refs"],
@@ -124,15 +128,24 @@ class _Pages:
     def free(self) -> int:
         return self.tables.free
 
-    def ready(self) -> None:
+    def ready(self, changes: bool = False) -> None:
         """Every call begins with it: what was queued before on another stream comes first (a page that
         is given back and taken again may still be read there), and what an earlier call's page
-        changes left to do, if it failed before they were on the device."""
-        self.stream = follow(self.device, self.stream, self.pool, self.table)
+        changes left to do, if it failed before they were on the device.  ``changes``: the call may
+        change pages."""
+        self.now, self.stream = follow(self.device, self.stream, self.pool, self.table)
+        self.here, self.captured = state(self.device) if changes or self.pending else (False, False)
         if self.pending:
             if self.copies[0] or self.tables.n_changed:
                 self._eager()
             self.apply()
+
+    def call(self, function, *args) -> int:
+        """``device.launch``, on the stream that ``ready`` found."""
+        if self.here or _cuda().current_device() == self.device.index:
+            return function(*args, self.now)
+        with _cuda().device(self.device.index):
+            return function(*args, self.now)
 
     def apply(self, source=None) -> None:
         """To the device, on the current stream: the page copies that the last host call asked for
@@ -140,16 +153,16 @@ class _Pages:
         n = int(self.copies[0])
         if n or self.tables.n_changed:
             pool = (source or self).desc
-            _lib.check(launch(self.device, _lib.load().tsattn_pages4_apply, self.tables, self.desc.table,
-                              pool.pool, pool.num_pages, self.desc.pool, self.desc.num_pages,
-                              self.page_bytes, n, *self.out[:2]), "page update")
+            _lib.check(self.call(_lib.load().tsattn_pages4_apply, self.tables, self.desc.table, pool.pool,
+                                 pool.num_pages, self.desc.pool, self.desc.num_pages, self.page_bytes, n,
+                                 *self.out[:2]), "page update")
             self.copies[0] = 0
         self.pending = False
 
     def _eager(self, rows=None, steps: int = 0) -> None:
         """Refuses page changes under capture: a captured call's pages would be the host's at once and
         the device's with each replay.  With ``rows``: only if they need other pages for ``steps``."""
-        if not capturing(self.device):
+        if not self.captured:
             return
         if rows is not None:
             lens = self.lengths[rows]
@@ -164,14 +177,19 @@ class _Pages:
         self.pending = True
         _lib.check(_lib.load().tsattn_pages4_grow(self.tables, n, rows, steps, *self.out), "page table")
 
-    def cut(self, rows, rows_at: int, lengths) -> None:
+    def cut(self, rows, rows_at: int, lengths=0) -> None:
         """``rows`` (at an address) end at ``lengths``; pages wholly past them are given back (under
         capture refused: the captured calls would go on with them)."""
-        if capturing(self.device):
+        self.ready(True)
+        to = self.some[:len(rows)]
+        to[:] = lengths
+        if (to != lengths).any():  # (more than 32 bits)
+            raise ValueError("truncate length must be between zero and the current length")
+        if self.captured:
             pages = -(-self.lengths[rows] // self.page_size)
-            if ((lengths >= 0) & (-(-lengths // self.page_size) < pages)).any():
+            if ((to >= 0) & (-(-to // self.page_size) < pages)).any():
                 self._eager()
-        _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows_at, lengths.ctypes.data), "page table")
+        _lib.check(_lib.load().tsattn_pages4_cut(self.tables, len(rows), rows_at, self.some_at), "page table")
 
     def take_back(self, rows, steps: int) -> None:
         """Gives back the pages that ``grow`` took past the rows' lengths, if it got so far.  Copies of
@@ -183,8 +201,8 @@ class _Pages:
 
     def clone(self, rows, num_pages: int) -> "_Pages":
         """The rows with pages of their own, in a pool of ``num_pages``."""
+        self.ready(True)
         self._eager()
-        self.ready()
         other = _Pages(len(rows), self.heads, self.dim, self.host.shape[1], self.page_size, num_pages, self.device)
         _lib.check(_lib.load().tsattn_pages4_clone(self.tables, len(rows), rows.ctypes.data, other.tables, *other.out),
                    "page table")
@@ -288,13 +306,14 @@ class PagedKVCache:
                     raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
                 cos, sin = (t.data_ptr() for t in rope_tables(rotary_base, core.dim, self.dtype, core.pool.device, most))
             k, v = (_rows(t if t.dtype == self.dtype else t.to(self.dtype)) for t in (key._data, value._data))
-            core._eager(self._rows, steps)
-            core.ready()
+            core.ready(True)
+            if core.captured:
+                core._eager(self._rows, steps)
             try:
                 core.grow(len(lens), self._rows_at, steps)
                 core.apply()
-                _lib.check(launch(core.device, _lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
-                                  _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
+                _lib.check(core.call(_lib.load().tsattn_pages4_append, core.desc, self._code, len(lens), steps,
+                                     _view(k), _view(v), self._rows_at, lens_at, cos, sin), "paged append")
             except BaseException:
                 core.take_back(self._rows, steps)
                 raise
@@ -335,12 +354,16 @@ class PagedKVCache:
             if last is not None and not 0 < last <= lens.min():
                 raise ValueError("the last positions read must be between one and the shortest row's length")
             steps = int(lens.max()) if last is None else last
-            first = np.zeros_like(lens) if last is None else lens - np.int32(last)
+            first = core.some[:len(lens)]
+            if last is None:
+                first[:] = 0
+            else:
+                np.subtract(lens, last, out=first)
             k = torch.empty((len(lens), core.heads, steps, core.dim), dtype=self.dtype, device=core.pool.device)
             v = torch.empty_like(k)
             if steps:
-                _lib.check(launch(core.device, _lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
-                                  _view(k), _view(v), self._rows_at, lens_at, first.ctypes.data), "paged read")
+                _lib.check(core.call(_lib.load().tsattn_pages4_read, core.desc, self._code, len(lens), steps,
+                                     _view(k), _view(v), self._rows_at, lens_at, core.some_at), "paged read")
         return Tensor._leaf(k, core.device), Tensor._leaf(v, core.device)
 
     # -- rows and pages -------------------------------------------------------
@@ -369,16 +392,14 @@ class PagedKVCache:
     def reset(self) -> None:
         """Every row empty, its pages given back."""
         with self._core.lock:
-            self._core.ready()
-            self._core.cut(self._rows, self._rows_at, np.zeros_like(self._rows))
+            self._core.cut(self._rows, self._rows_at)
 
     def free(self, indices) -> None:
         """These rows empty, their pages given back."""
         rows = self._rows[np.unique(self._indices(indices, None))]
         if len(rows):
             with self._core.lock:
-                self._core.ready()
-                self._core.cut(rows, rows.ctypes.data, np.zeros_like(rows))
+                self._core.cut(rows, rows.ctypes.data)
 
     def truncate(self, length) -> None:
         """Cut every row to ``length`` positions, or to a length of its own (a sequence of them);
@@ -386,20 +407,16 @@ class PagedKVCache:
         want = np.asarray(length)
         if want.dtype.kind not in "iu" or want.shape not in ((), self._rows.shape):
             raise ValueError("truncate takes one integer length, or one per row")
-        lens = want.astype(np.int32)
-        if (lens != want).any():
-            raise ValueError("truncate length must be between zero and the current length")
         with self._core.lock:
-            self._core.ready()
-            self._core.cut(self._rows, self._rows_at, lens if lens.shape else np.full_like(self._rows, lens))
+            self._core.cut(self._rows, self._rows_at, want)
 
     def reorder(self, indices) -> None:
         """Row i becomes row ``indices[i]``, sharing its pages: no keys or values move.  Rows that
         take over the same row share until one appends (``append`` copies the page)."""
         core, index = self._core, self._indices(indices, self._rows.shape)
         with core.lock:
+            core.ready(True)
             core._eager()
-            core.ready()
             core.pending = True
             _lib.check(_lib.load().tsattn_pages4_reorder(core.tables, len(index), self._rows_at, index.ctypes.data),
                        "page table")
@@ -421,8 +438,8 @@ class PagedKVCache:
         core = self._core
         with core.lock:
             if num_pages is None:
+                core.ready(True)
                 core._eager()
-                core.ready()
                 core.pending = True
                 _lib.check(_lib.load().tsattn_pages4_compact(core.tables, *core.out), "page table")
                 core.apply()
@@ -488,9 +505,9 @@ def paged_attention(query: Tensor, cache: PagedKVCache, *, is_causal: bool = Tru
         lib, code = _lib.load(), cache._code
         nbytes = lib.tsattn_pages4_attend_workspace(core.desc, code, b, heads, steps, lens_at)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _lib.check(launch(core.device, lib.tsattn_pages4_attend, core.desc, code, b, heads, steps, multiplier,
-                          int(is_causal), _view(q), _view(out), cache._rows_at, lens_at, cos, sin,
-                          None if ws is None else ws.data_ptr(), nbytes), "paged attention")
+        _lib.check(core.call(lib.tsattn_pages4_attend, core.desc, code, b, heads, steps, multiplier,
+                             int(is_causal), _view(q), _view(out), cache._rows_at, lens_at, cos, sin,
+                             None if ws is None else ws.data_ptr(), nbytes), "paged attention")
     return Tensor._from_op(out, (query,), None, "paged_attention")
 
 
