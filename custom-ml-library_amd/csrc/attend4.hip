@@ -17,7 +17,8 @@
 // loaded them.
 //
 // Precision.  q enters exactly: bf16 in one part, f16 in two, fp32 in three.  P sv
-// enters as two bf16 parts (2^-17 of each), for fp32 as three (2^-25).
+// enters as two bf16 parts (within 2^-16 of each: the first is truncated), for fp32 as
+// three (exactly).
 //
 // A wave works alone on every fourth or eighth tile of its split, two tiles ahead in
 // registers, straight from memory in operand order (pages4.h); waves merge in LDS,

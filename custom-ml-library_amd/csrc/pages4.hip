@@ -167,9 +167,9 @@ __device__ __forceinline__ void load_words(const char *from, int lane, uint32_t 
 // One wave quantises the new positions of one tile, head and side (keys or values).
 // A load takes whole rows, PPR lanes of 8 channels a row, so that four neighbouring
 // lanes make a group and the angles' loads take whole lines of their tables too (four
-// 64-byte pieces a row from the operand order's lanes: 44 us where this takes 38,
-// 4 x 8 heads x 8192 positions of D128 in bf16, rotated: 172 MB at 4.5 TB/s, where a
-// large copy reaches 4.9).  Codes and scales then cross
+// 64-byte pieces a row from the operand order's lanes: 44 us where this took 38, now
+// 35, 4 x 8 heads x 8192 positions of D128 in bf16, rotated: 172 MB at 4.9 TB/s, a
+// large copy's rate).  Codes and scales then cross
 // the wave through LDS into operand order; values' words, one channel of eight keys
 // each, take a transpose in each quad of lanes and a second trip.  A tile that is
 // only partly new keeps its other positions: keys' words belong to one position each,

@@ -45,7 +45,9 @@ def _reads_codes(rows: int, heads: int, dim: int, wide: bool, lens) -> bool:
     heads of D64, 2 of 2000, 1024 rows 38 / 50, 2048 64 / 45.  fp32, 8 heads of D128 over 8000: 1024
     rows 158 / 1135.  Not for more rows than the codes' kernel takes, nor where its splits of 4096
     positions would leave more than 4 GiB of partial sums (of positions that are there: the scratch
-    goes by the longest row, and is bounded by the library, which takes a call in parts)."""
+    goes by the longest row, and is bounded by the library, which takes a call in parts).  The two
+    keep P in different bits: the codes' kernel in two or three bf16 parts, within 2^-16 of it or
+    exactly, the kernels of arrays in the dtype (bf16 2^-8, f16 2^-11: the matrix cores' operand)."""
     if rows > 1 << 18 or 4 * rows * heads * dim * int((-(-lens // 4096)).sum()) > 1 << 32:
         return False
     pairs, size = rows * heads * int(lens.sum()), (dim / 128) ** 0.85

@@ -280,7 +280,8 @@ class MultiHeadAttention(Module):
 
 
     def _paged(self, input: Tensor, cache: PagedKVCache, attn_mask, is_causal: bool) -> Tensor:
-        """Self-attention over a paged 4-bit cache, each row at its own position."""
+        """Self-attention over a paged 4-bit cache, each row at its own position.  As over an int8 cache,
+        ``backend`` chooses only where a mask has the values read back as arrays."""
         batch, steps, _ = input.shape
         lens = cache.lengths
         if attn_mask is not None and min(lens) != max(lens):
