@@ -403,6 +403,24 @@ int check_rows(int32_t dtype, int32_t rows, int32_t k, int32_t n, int64_t xs, in
   return TSATTN_OK;
 }
 
+// Operands of the token probabilities: a workgroup each row (or part of one), 32-bit element offsets in a row.
+int check_probs(int32_t dtype, int64_t rows, int32_t vocab, const void *logits, int64_t row_stride,
+                const void *tokens, int32_t token_bytes, int32_t top) {
+  if (dtype != TSATTN_F32 && dtype != TSATTN_F16 && dtype != TSATTN_BF16)
+    return fail(TSATTN_ERR_INVALID, "token probabilities take dtype f32, f16 or bf16 (got dtype %d)", dtype);
+  if (rows <= 0 || vocab <= 0) return fail(TSATTN_ERR_INVALID, "token probabilities need positive sizes");
+  if (!logits || !tokens) return fail(TSATTN_ERR_INVALID, "data pointer is NULL");
+  if (token_bytes != 4 && token_bytes != 8) return fail(TSATTN_ERR_INVALID, "tokens are int32 or int64");
+  if (row_stride < 0) return fail(TSATTN_ERR_INVALID, "the logits' row stride must not be negative");
+  if (top < 0 || top > vocab) return fail(TSATTN_ERR_INVALID, "top must be within the vocabulary");
+  if (top > 64) return fail(TSATTN_ERR_UNSUPPORTED, "at most 64 top tokens are kept (got %d)", top);
+  if (rows >= (int64_t(1) << 31) || vocab > (1 << 30))
+    return fail(TSATTN_ERR_UNSUPPORTED, "token probabilities take up to 2^31 - 1 rows of 2^30 logits");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == TSATTN_F32 ? 4 : 2))
+    return fail(TSATTN_ERR_INVALID, "the logits' rows must be aligned to their elements");
+  return TSATTN_OK;
+}
+
 // A cached step: the workspace's layout and the attention problem.
 struct StepPlan {
   int rows, width;  // batch len, heads_q dim
@@ -1030,6 +1048,42 @@ int tsattn_rows_swiglu(int32_t dtype, int32_t rows, int32_t k, int32_t n, const 
   return hip_status(tsattn::launch_rows_swiglu(dtype, rows, k, n, x, x_stride, gate, up, out, out_stride,
                                                static_cast<hipStream_t>(stream)),
                     "rows SwiGLU launch");
+}
+
+size_t tsattn_token_probs_workspace(int64_t rows, int32_t vocab, int32_t top) {
+  return rows <= 0 || vocab <= 0 || top < 0 ? 0 : tsattn::token_probs_workspace(rows, vocab, top);
+}
+
+int tsattn_token_probs(int32_t dtype, int64_t rows, int32_t vocab, const void *logits, int64_t row_stride,
+                       const void *tokens, int32_t token_bytes, int64_t ignore, int32_t top, float *log_probs,
+                       float *entropy, float *stats, float *top_log_probs, int64_t *top_indices, void *workspace,
+                       size_t workspace_bytes, void *stream) {
+  int rc = check_probs(dtype, rows, vocab, logits, row_stride, tokens, token_bytes, top);
+  if (rc) return rc;
+  if (!log_probs || !entropy || (top && (!top_log_probs || !top_indices)))
+    return fail(TSATTN_ERR_INVALID, "data pointer is NULL");
+  const size_t need = tsattn::token_probs_workspace(rows, vocab, top);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 8))
+    return fail(TSATTN_ERR_INVALID, "token probabilities need %zu bytes of 8-byte aligned workspace", need);
+  return hip_status(tsattn::launch_token_probs(dtype, rows, vocab, logits, row_stride, tokens, token_bytes, ignore,
+                                               top, log_probs, entropy, stats, top_log_probs, top_indices, workspace,
+                                               static_cast<hipStream_t>(stream)),
+                    "token probabilities launch");
+}
+
+int tsattn_token_probs_backward(int32_t dtype, int64_t rows, int32_t vocab, const void *logits, int64_t row_stride,
+                                const void *tokens, int32_t token_bytes, int64_t ignore, int32_t top,
+                                const float *stats, const float *entropy, const int64_t *top_indices,
+                                const float *g_log_probs, const float *g_entropy, const float *g_top,
+                                void *dlogits, void *stream) {
+  int rc = check_probs(dtype, rows, vocab, logits, row_stride, tokens, token_bytes, top);
+  if (rc) return rc;
+  if (!stats || !dlogits || (g_entropy && !entropy) || (g_top && (!top || !top_indices)))
+    return fail(TSATTN_ERR_INVALID, "data pointer is NULL");
+  return hip_status(tsattn::launch_token_probs_backward(dtype, rows, vocab, logits, row_stride, tokens, token_bytes,
+                                                        ignore, top, stats, entropy, top_indices, g_log_probs,
+                                                        g_entropy, g_top, dlogits, static_cast<hipStream_t>(stream)),
+                    "token probabilities backward launch");
 }
 
 size_t tsattn_linear_wgrad_workspace(int32_t tokens, int32_t m, int32_t n) {

@@ -1,0 +1,584 @@
+// Log probabilities of given tokens, the entropy of their rows and the rows' most
+// likely tokens, with the VJP.  No counterpart in the reference, whose cross entropy
+// (src/tensorsmith/nn/functional.py:397-472) keeps the whole log-softmax.
+//
+// With m = max z, l = sum_j exp(z_j - m) over a row z of V logits:
+//   log p_y = (z_y - m) - ln l,   H = ln l - (1 / l) sum_j exp(z_j - m) (z_j - m),
+// where both terms of H are >= 0, so that nothing cancels; a logit of -inf adds
+// nothing.  The VJP, for upstream gradients g of log p_y, gh of H and t_i of the top
+// tokens' log probabilities (at indices k_i), G = g + sum_i t_i:
+//   dz_j = -p_j (G + gh (ln p_j + H)) + [j = y] g + sum_i [j = k_i] t_i.
+//
+// Bound by HBM: the forward reads the logits once, the VJP reads them and writes the
+// gradient.  One pass in each: a lane keeps a running (m, l, sum e x) and rescales it
+// once for every 16-byte piece.  A 16-bit logit takes about 11 vector instructions
+// (an exponential counts four), which at the chip's rate is some 7 TB/s of logits:
+// just above what HBM gives, so anything more an element would show.
+//
+// A row belongs to one wave (V <= kWaveRow), to a workgroup of four, or, when the rows
+// are too few to fill the chip, to several workgroups that each take a part of it; a
+// second kernel then combines the parts in their order.  Results depend on the sizes
+// alone, no atomics.
+//
+// The top tokens: each wave keeps the 64 best (logit, index) pairs it saw, sorted, one
+// a lane, as 64-bit keys whose order is the logits' with ties to the lower index, and a
+// threshold, the top-th best of them.  A piece whose largest logit is not above the
+// threshold, which is nearly every one, costs a comparison; keys above it go to a
+// buffer in LDS, 64 of which are sorted and merged at a time.  The first piece would
+// send every element there: when many lanes have candidates, the top-th best of the
+// lanes' own best becomes the threshold first (top elements at least are as good).
+#include <type_traits>
+
+#include "tsattn_internal.h"
+
+namespace tsattn {
+namespace {
+
+constexpr int NT = 256;
+constexpr int NW = NT / 64;
+constexpr int U = 4;         // 16-byte pieces a lane has in flight
+constexpr int PENDING = 64 + 64 * 8;  // keys a wave's buffer holds: < 64 left over, and one piece of each lane
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct ProbArgs {
+  int64_t rows;
+  int vocab, top, splits;
+  const void *z;
+  int64_t zs;  // row stride in elements
+  const void *tokens;
+  int token_bytes;
+  int64_t ignore;
+  float *logp, *entropy, *stats;  // stats: [rows][2] = m, ln l
+  float *top_logp;
+  int64_t *top_index;
+  float *part;                   // [rows][splits][4]: m, l, sum e x (log2 units)
+  unsigned long long *part_top;  // [rows][splits][top]
+  // VJP
+  const float *g, *gh, *gt, *saved_entropy;
+  const int64_t *saved_index;
+  void *dz;
+};
+
+typedef unsigned long long u64;
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+constexpr int kVE = 16 / sizeof(T);
+
+template <typename T>
+__device__ __forceinline__ void unpack(u32x4 raw, float (&x)[kVE<T>]) {
+  if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned bits = raw[e];  // (a bit cast of raw[e] itself takes the vector's first element)
+      x[e] = __builtin_bit_cast(float, bits);
+    }
+  } else if constexpr (std::is_same_v<T, bf16>) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned bits = (e & 1) ? raw[e >> 1] & 0xFFFF0000u : raw[e >> 1] << 16;
+      x[e] = __builtin_bit_cast(float, bits);
+    }
+  } else {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    const h8 h = __builtin_bit_cast(h8, raw);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(h[e]);
+  }
+}
+
+__device__ __forceinline__ int64_t token_of(const ProbArgs &a, int64_t row) {
+  return a.token_bytes == 8 ? static_cast<const int64_t *>(a.tokens)[row]
+                            : static_cast<const int32_t *>(a.tokens)[row];
+}
+
+// ---------------------------------------------------------------------------
+// Running sums: m, l = sum exp(z - m), w = sum exp(z - m) (z - m) log2 e.
+// ---------------------------------------------------------------------------
+struct Sums {
+  float m, l, w;
+};
+
+// (a base that keeps exp(-inf - base) = 0 while nothing but -inf has come)
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ void rebase(Sums &s, float m) {
+  const float d = (base_of(s.m) - base_of(m)) * kLog2e;
+  const float c = __builtin_amdgcn_exp2f(d);
+  // an empty sum stays empty whatever the bases (0 * inf is NaN)
+  s.w = s.l == 0.f ? s.w : c * fmaf(s.l, fmaxf(d, -1e30f), s.w);
+  s.l = s.l == 0.f ? s.l : s.l * c;
+  s.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b) {
+  const float m = fmaxf(a.m, b.m);
+  rebase(a, m);
+  rebase(b, m);
+  return Sums{m, a.l + b.l, a.w + b.w};
+}
+__device__ __forceinline__ Sums wave_join(Sums s) {
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1)
+    s = join(s, Sums{__shfl_xor(s.m, k, 64), __shfl_xor(s.l, k, 64), __shfl_xor(s.w, k, 64)});
+  return s;
+}
+
+// Adds N logits; `own` becomes their sum of exponentials (NaN where one is NaN or +inf).
+template <int N>
+__device__ __forceinline__ void add(Sums &s, const float (&x)[N], float mx, float &own) {
+  rebase(s, fmaxf(s.m, mx));
+  const float base = base_of(s.m);
+  float l = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float t = (x[e] - base) * kLog2e;
+    const float p = __builtin_amdgcn_exp2f(t);
+    l += p;
+    s.w = fmaf(p, fmaxf(t, -1e30f), s.w);  // (0 times -inf is NaN)
+  }
+  s.l += l;
+  own = l;
+}
+
+// ---------------------------------------------------------------------------
+// The best keys.
+// ---------------------------------------------------------------------------
+// Keys order as (logit, lower index first); a NaN is the largest, -0 equals 0.
+__device__ __forceinline__ u64 key_of(float z, unsigned index) {
+  unsigned u = __builtin_bit_cast(unsigned, z + 0.f);
+  u = z != z ? 0x7FFFFFFFu : u;
+  u ^= (u >> 31) ? 0xFFFFFFFFu : 0x80000000u;
+  return static_cast<u64>(u) << 32 | ~index;
+}
+__device__ __forceinline__ float key_logit(u64 key) {
+  const unsigned u = static_cast<unsigned>(key >> 32);
+  return __builtin_bit_cast(float, (u >> 31) ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ u64 from_lane(u64 x, int lane) {
+  const int lo = __shfl(static_cast<int>(x), lane, 64), hi = __shfl(static_cast<int>(x >> 32), lane, 64);
+  return static_cast<u64>(static_cast<unsigned>(hi)) << 32 | static_cast<unsigned>(lo);
+}
+// One exchange of a bitonic network: lanes l and l ^ stride, the larger to the lower
+// lane where `down`.
+__device__ __forceinline__ u64 exchange(u64 x, int lane, int stride, bool down) {
+  const u64 y = from_lane(x, lane ^ stride);
+  return (((lane & stride) == 0) == down) == (x > y) ? x : y;
+}
+__device__ __forceinline__ u64 sort_down(u64 x, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int stride = size >> 1; stride; stride >>= 1) x = exchange(x, lane, stride, (lane & size) == 0);
+  return x;
+}
+// The 64 best of two lists sorted down.
+__device__ __forceinline__ u64 merge_down(u64 best, u64 more, int lane) {
+  const u64 y = from_lane(more, 63 - lane);
+  u64 x = best > y ? best : y;
+#pragma unroll
+  for (int stride = 32; stride; stride >>= 1) x = exchange(x, lane, stride, true);
+  return x;
+}
+
+struct Best {
+  u64 best = 0;       // this lane's rank of the wave's list; 0: none
+  u64 least = 0;      // keys must be above it (0: all are)
+  float least_z = 0;  // its logit
+  int pending = 0;
+  u64 *buffer;
+
+  __device__ __forceinline__ void raise(u64 key) {
+    if (key > least) {
+      // (the same in every lane: kept where a comparison reads it as a scalar)
+      const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(key));
+      const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(key >> 32));
+      least = static_cast<u64>(hi) << 32 | lo;
+      least_z = key_logit(least);
+    }
+  }
+  __device__ __forceinline__ void take(int n, int top, int lane) {
+    // the buffer's last n <= 64 keys (other lanes wrote them)
+    pending -= n;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const u64 key = lane < n ? buffer[pending + lane] : 0;
+    best = merge_down(best, sort_down(key, lane), lane);
+    raise(from_lane(best, top - 1));
+  }
+  // N logits a lane from `index` on, n of them there; call in step, indexes rising.
+  template <int N>
+  __device__ __forceinline__ void offer(const float (&x)[N], float mx, float own, unsigned index, int n, int top,
+                                        int lane) {
+    const bool maybe = n > 0 && (least == 0 || !(mx <= least_z) || own != own);
+    const u64 lanes = __ballot(maybe);
+    if (lanes == 0) return;
+    const int count = __popcll(lanes);
+    if (count > top && count > 24) {
+      u64 key = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const u64 k = e < n ? key_of(x[e], index + e) : 0;
+        key = k > key ? k : key;
+      }
+      key = from_lane(sort_down(key, lane), top - 1);
+      if (key) raise(key - 1);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const u64 key = e < n ? key_of(x[e], index + e) : 0;
+      const u64 pass = __ballot(key > least);
+      if (pass == 0) continue;
+      if (key > least) buffer[pending + __popcll(pass & ((u64(1) << lane) - 1))] = key;
+      pending += __popcll(pass);
+    }
+    while (pending >= 64) take(64, top, lane);
+  }
+  __device__ __forceinline__ void finish(int top, int lane) {
+    if (pending) take(pending, top, lane);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Forward.
+// ---------------------------------------------------------------------------
+// What a row's sums (and with TOP its best keys, one a lane) say; one wave.
+template <typename T, bool TOP>
+__device__ __forceinline__ void results(const ProbArgs &a, int64_t row, Sums s, u64 best, int lane) {
+  const float ln = logf(s.l);
+  // (all logits -inf: l = 0; log p is NaN as -inf - -inf is)
+  const float m = s.m;
+  if (lane == 0) {
+    const int64_t y = token_of(a, row);
+    const float z = y >= 0 && y < a.vocab ? static_cast<float>(static_cast<const T *>(a.z)[row * a.zs + y]) : NAN;
+    a.logp[row] = (z - m) - ln;
+    a.entropy[row] = m == -INFINITY ? NAN : ln - s.w / s.l * kLn2;
+    if (a.stats) {
+      a.stats[2 * row] = m;
+      a.stats[2 * row + 1] = ln;
+    }
+  }
+  if constexpr (TOP) {
+    if (lane < a.top) {
+      a.top_logp[row * a.top + lane] = (key_logit(best) - m) - ln;
+      a.top_index[row * a.top + lane] = ~static_cast<unsigned>(best);
+    }
+  }
+}
+
+__device__ __forceinline__ void ignored(const ProbArgs &a, int64_t row, int lane, bool top) {
+  if (lane == 0) {
+    a.logp[row] = 0.f;
+    a.entropy[row] = 0.f;
+    if (a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.f;
+  }
+  if (top && lane < a.top) {
+    a.top_logp[row * a.top + lane] = -INFINITY;
+    a.top_index[row * a.top + lane] = -1;
+  }
+}
+
+// A row as 16-byte pieces: `head` elements before the first aligned one, `pieces`,
+// then what is left.
+template <typename T>
+struct Row {
+  const T *z;
+  int head, pieces, tail;
+  __device__ __forceinline__ Row(const T *p, int vocab) : z(p) {
+    const unsigned off = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) & 15u);
+    head = min(vocab, static_cast<int>((16u - off) % 16u / sizeof(T)));
+    pieces = (vocab - head) / kVE<T>;
+    tail = vocab - head - pieces * kVE<T>;
+  }
+};
+
+// WPR: waves a row has in the workgroup, 1 or NW.
+template <typename T, int WPR, bool TOP>
+__global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
+  constexpr int VE = kVE<T>, LANES = WPR * 64;
+  __shared__ u64 buffers[TOP ? NW * PENDING : 1];
+  __shared__ float red[NW][4];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (NW / WPR) + (WPR == 1 ? w : 0);
+  const int64_t row = WPR == 1 ? id : id / a.splits;
+  const int part = WPR == 1 ? 0 : static_cast<int>(id % a.splits);
+  if (row >= a.rows) return;  // (WPR = NW: of the whole workgroup, and no barrier follows for WPR = 1)
+  if (token_of(a, row) == a.ignore) {
+    if (part == 0 && (WPR == 1 || w == 0)) ignored(a, row, lane, TOP);
+    return;
+  }
+  const Row<T> r(static_cast<const T *>(a.z) + row * a.zs, a.vocab);
+  const int splits = WPR == 1 ? 1 : a.splits;
+  const int p0 = static_cast<int>(static_cast<int64_t>(r.pieces) * part / splits);
+  const int p1 = static_cast<int>(static_cast<int64_t>(r.pieces) * (part + 1) / splits);
+  Sums s{-INFINITY, 0.f, 0.f};
+  Best top;
+  top.buffer = buffers + (TOP ? w * PENDING : 0);
+  float own;
+  // the elements in front of the first piece, one a lane
+  auto single = [&](int first, int n) {
+    const float x[1] = {lane < n ? static_cast<float>(r.z[first + lane]) : -INFINITY};
+    add(s, x, x[0], own);
+    if constexpr (TOP) top.offer(x, x[0], own, first + lane, lane < n ? 1 : 0, a.top, lane);
+  };
+  const int l0 = (WPR == 1 ? 0 : w * 64) + lane;
+  if (part == 0 && (WPR == 1 || w == 0) && r.head) single(0, r.head);
+  const u32x4 *pieces = reinterpret_cast<const u32x4 *>(r.z + r.head);
+  for (int i = p0; i < p1; i += LANES * U) {
+    u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = i + u * LANES + l0;
+      if (at < p1) raw[u] = __builtin_nontemporal_load(pieces + at);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u * LANES >= p1) break;
+      const int at = i + u * LANES + l0;
+      float x[VE];
+      unpack<T>(raw[u], x);
+      if (at >= p1) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] = -INFINITY;
+      }
+      float mx = x[0];
+#pragma unroll
+      for (int e = 1; e < VE; ++e) mx = fmaxf(mx, x[e]);
+      add(s, x, mx, own);
+      if constexpr (TOP) top.offer(x, mx, own, r.head + at * VE, at < p1 ? VE : 0, a.top, lane);
+    }
+  }
+  if (part == splits - 1 && (WPR == 1 || w == NW - 1) && r.tail) single(a.vocab - r.tail, r.tail);
+  s = wave_join(s);
+  if constexpr (TOP) top.finish(a.top, lane);
+  if constexpr (WPR > 1) {
+    if (lane == 0) red[w][0] = s.m, red[w][1] = s.l, red[w][2] = s.w;
+    if constexpr (TOP) top.buffer[lane] = top.best;
+    __syncthreads();
+    if (w) return;
+#pragma unroll
+    for (int k = 1; k < NW; ++k) {
+      s = join(s, Sums{red[k][0], red[k][1], red[k][2]});
+      if constexpr (TOP) top.best = merge_down(top.best, buffers[k * PENDING + lane], lane);
+    }
+    if (splits > 1) {
+      if (lane == 0) {
+        float *p = a.part + 4 * id;
+        p[0] = s.m, p[1] = s.l, p[2] = s.w;
+      }
+      if constexpr (TOP)
+        if (lane < a.top) a.part_top[id * a.top + lane] = top.best;
+      return;
+    }
+  }
+  results<T, TOP>(a, row, s, top.best, lane);
+}
+
+// The parts of a row, in their order; a wave a row.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(NT) void probs_merge_kernel(ProbArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 6);
+  if (row >= a.rows || token_of(a, row) == a.ignore) return;
+  // (lane i starts with part i; more parts than lanes do not occur, kMaxSplits)
+  Sums s{-INFINITY, 0.f, 0.f};
+  if (lane < a.splits) {
+    const float *p = a.part + 4 * (row * a.splits + lane);
+    s = Sums{p[0], p[1], p[2]};
+  }
+  s = wave_join(s);
+  u64 best = 0;
+  if constexpr (TOP)
+    for (int i = 0; i < a.splits; ++i)
+      best = merge_down(best, lane < a.top ? a.part_top[(row * a.splits + i) * a.top + lane] : 0, lane);
+  results<T, TOP>(a, row, s, best, lane);
+}
+
+// ---------------------------------------------------------------------------
+// VJP.
+// ---------------------------------------------------------------------------
+template <typename T, int N>
+__device__ __forceinline__ void store_piece(T *p, const float (&x)[N]) {
+  typedef T V __attribute__((ext_vector_type(N)));
+  V y;
+#pragma unroll
+  for (int e = 0; e < N; ++e) y[e] = static_cast<T>(x[e]);
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4, y), reinterpret_cast<u32x4 *>(p));
+}
+
+// A workgroup takes part `part` of a row (WPR = NW), or each wave a row.  The gradient
+// is contiguous: its rows start where they may, so its pieces are the gradient's own
+// (the logits' are read by element where the two do not lie alike).
+template <typename T, int WPR, bool TOP>
+__global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
+  constexpr int VE = kVE<T>, LANES = WPR * 64;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (NW / WPR) + (WPR == 1 ? w : 0);
+  const int splits = WPR == 1 ? 1 : a.splits;
+  const int64_t row = id / splits;
+  const int part = static_cast<int>(id % splits);
+  if (row >= a.rows) return;
+  const T *z = static_cast<const T *>(a.z) + row * a.zs;
+  T *dz = static_cast<T *>(a.dz) + row * a.vocab;
+  const Row<T> r(dz, a.vocab);
+  const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15u) == 0;
+  const int p0 = static_cast<int>(static_cast<int64_t>(r.pieces) * part / splits);
+  const int p1 = static_cast<int>(static_cast<int64_t>(r.pieces) * (part + 1) / splits);
+  const int l0 = (WPR == 1 ? 0 : w * 64) + lane;
+  const bool has_head = part == 0 && (WPR == 1 || w == 0), has_tail = part == splits - 1 && (WPR == 1 || w == NW - 1);
+  const int64_t y = token_of(a, row);
+  if (y == a.ignore) {
+    const float none[VE] = {};
+    if (has_head && lane < r.head) dz[lane] = static_cast<T>(0.f);
+    for (int i = p0 + l0; i < p1; i += LANES) store_piece(dz + r.head + i * VE, none);
+    if (has_tail && lane < r.tail) dz[a.vocab - r.tail + lane] = static_cast<T>(0.f);
+    return;
+  }
+  const float m = a.stats[2 * row], ln = a.stats[2 * row + 1];
+  float g = a.g ? a.g[row] : 0.f;
+  if (y < 0 || y >= a.vocab) g = a.g ? NAN : 0.f;  // (its log probability is NaN)
+  const float gh = a.gh ? a.gh[row] : 0.f;
+  float all = g;
+  if constexpr (TOP)
+    for (int i = 0; i < a.top; ++i) all += a.gt[row * a.top + i];
+  const float c = gh == 0.f ? all : fmaf(gh, a.saved_entropy[row], all);
+  auto at_logit = [&](float x) {
+    const float lp = (x - m) - ln;
+    const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
+    return -p * fmaf(gh, fmaxf(lp, -1e30f), c);
+  };
+  const int yi = y >= 0 && y < a.vocab ? static_cast<int>(y) : -1;
+  auto single = [&](int j) {
+    const float d = at_logit(static_cast<float>(z[j]));
+    dz[j] = static_cast<T>(j == yi ? d + g : d);
+  };
+  if (has_head && lane < r.head) single(lane);
+  for (int i = p0 + l0; i < p1; i += LANES * U) {
+    u32x4 raw[U];
+    if (alike) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * LANES < p1)
+          raw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(z + r.head) + i + u * LANES);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * LANES < p1) {
+          typedef T V __attribute__((ext_vector_type(VE)));
+          V v;
+          const T *from = z + r.head + (i + u * LANES) * VE;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) v[e] = from[e];
+          raw[u] = __builtin_bit_cast(u32x4, v);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = i + u * LANES;
+      if (at >= p1) break;
+      float x[VE];
+      unpack<T>(raw[u], x);
+      const int j0 = r.head + at * VE;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[e] = at_logit(x[e]);
+      if (static_cast<unsigned>(yi - j0) < static_cast<unsigned>(VE)) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] += e == yi - j0 ? g : 0.f;
+      }
+      store_piece(dz + j0, x);
+    }
+  }
+  if (has_tail && lane < r.tail) single(a.vocab - r.tail + lane);
+  if constexpr (TOP) {
+    // the top tokens' elements again, whole, once the part's others are written
+    __threadfence();
+    if constexpr (WPR > 1) __syncthreads();
+    const int first = part == 0 ? 0 : r.head + p0 * VE, last = part == splits - 1 ? a.vocab : r.head + p1 * VE;
+    if (l0 < a.top) {
+      const int64_t j = a.saved_index[row * a.top + l0];
+      if (j >= first && j < last) {
+        float d = at_logit(static_cast<float>(z[j])) + a.gt[row * a.top + l0];
+        if (j == yi) d += g;
+        dz[j] = static_cast<T>(d);
+      }
+    }
+  }
+}
+
+// Vocabularies up to this many logits take a wave a row: then its 16 pieces a lane are
+// little more than the reduction costs (f16 pieces of 8; V 1009 f32: 4).
+constexpr int kWaveRow = 2048;
+constexpr int kMaxSplits = 64;
+
+bool wave_rows(int64_t rows, int vocab) { return vocab <= kWaveRow; }
+
+// Parts of a row: as many as give the chip's 256 CUs 4 workgroups each, of 8192 logits
+// or more (8 pieces a lane; shorter parts end before their loads pay for the start and
+// the second kernel).
+int prob_splits(int64_t rows, int vocab) {
+  if (wave_rows(rows, vocab)) return 1;
+  int64_t s = 1024 / rows;
+  if (s > vocab / 8192) s = vocab / 8192;
+  if (s > kMaxSplits) s = kMaxSplits;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+template <typename T, bool TOP>
+void forward(ProbArgs &a, hipStream_t st) {
+  if (wave_rows(a.rows, a.vocab)) {
+    probs_kernel<T, 1, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
+    return;
+  }
+  probs_kernel<T, NW, TOP><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(NT), 0, st>>>(a);
+  if (a.splits > 1)
+    probs_merge_kernel<T, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
+}
+
+template <typename T, bool TOP>
+void backward(ProbArgs &a, hipStream_t st) {
+  if (wave_rows(a.rows, a.vocab))
+    probs_vjp_kernel<T, 1, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
+  else
+    probs_vjp_kernel<T, NW, TOP><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(NT), 0, st>>>(a);
+}
+
+}  // namespace
+
+size_t token_probs_workspace(int64_t rows, int vocab, int top) {
+  const int s = prob_splits(rows, vocab);
+  return s < 2 ? 0 : static_cast<size_t>(rows) * s * (4 * sizeof(float) + top * sizeof(unsigned long long));
+}
+
+hipError_t launch_token_probs(int dtype, int64_t rows, int vocab, const void *z, int64_t zs, const void *tokens,
+                              int token_bytes, int64_t ignore, int top, float *logp, float *entropy, float *stats,
+                              float *top_logp, int64_t *top_index, void *ws, hipStream_t st) {
+  ProbArgs a{};
+  a.rows = rows, a.vocab = vocab, a.top = top, a.splits = prob_splits(rows, vocab);
+  a.z = z, a.zs = zs, a.tokens = tokens, a.token_bytes = token_bytes, a.ignore = ignore;
+  a.logp = logp, a.entropy = entropy, a.stats = stats, a.top_logp = top_logp, a.top_index = top_index;
+  a.part_top = static_cast<unsigned long long *>(ws);
+  a.part = reinterpret_cast<float *>(a.part_top + (a.splits > 1 ? rows * a.splits * top : 0));
+  Probe pr_("token_probs", st);
+  if (dtype == TSATTN_F32) top ? forward<float, true>(a, st) : forward<float, false>(a, st);
+  else if (dtype == TSATTN_F16) top ? forward<f16, true>(a, st) : forward<f16, false>(a, st);
+  else top ? forward<bf16, true>(a, st) : forward<bf16, false>(a, st);
+  return hipGetLastError();
+}
+
+hipError_t launch_token_probs_backward(int dtype, int64_t rows, int vocab, const void *z, int64_t zs,
+                                       const void *tokens, int token_bytes, int64_t ignore, int top,
+                                       const float *stats, const float *entropy, const int64_t *top_index,
+                                       const float *g, const float *gh, const float *gt, void *dz, hipStream_t st) {
+  ProbArgs a{};
+  a.rows = rows, a.vocab = vocab, a.top = top, a.splits = prob_splits(rows, vocab);
+  a.z = z, a.zs = zs, a.tokens = tokens, a.token_bytes = token_bytes, a.ignore = ignore;
+  a.stats = const_cast<float *>(stats), a.saved_entropy = entropy, a.saved_index = top_index;
+  a.g = g, a.gh = gh, a.gt = gt, a.dz = dz;
+  Probe pr_("token_probs_backward", st);
+  if (dtype == TSATTN_F32) gt ? backward<float, true>(a, st) : backward<float, false>(a, st);
+  else if (dtype == TSATTN_F16) gt ? backward<f16, true>(a, st) : backward<f16, false>(a, st);
+  else gt ? backward<bf16, true>(a, st) : backward<bf16, false>(a, st);
+  return hipGetLastError();
+}
+
+}  // namespace tsattn

@@ -298,6 +298,20 @@ size_t wgrad_workspace_bytes(int tokens, int M, int N);
 hipError_t launch_wgrad(int dtype, int out_dtype, int tokens, int M, int N, const void *g, int64_t gs, const void *x,
                         int64_t xs, void *dw, float *ws, hipStream_t st);
 
+// Log probabilities of tokens[rows] (int64 or int32 by token_bytes), entropies and the
+// `top` most likely tokens of rows of `vocab` logits (row stride zs), f32 / f16 / bf16;
+// rows whose token is `ignore` are not read.  stats: [rows][2], kept for the VJP, or
+// NULL.  ws: token_probs_workspace bytes (0: none), 8-byte aligned.
+size_t token_probs_workspace(int64_t rows, int vocab, int top);
+hipError_t launch_token_probs(int dtype, int64_t rows, int vocab, const void *z, int64_t zs, const void *tokens,
+                              int token_bytes, int64_t ignore, int top, float *logp, float *entropy, float *stats,
+                              float *top_logp, int64_t *top_index, void *ws, hipStream_t st);
+// Its VJP into contiguous dz [rows, vocab]; g, gh [rows] and gt [rows, top] may be NULL.
+hipError_t launch_token_probs_backward(int dtype, int64_t rows, int vocab, const void *z, int64_t zs,
+                                       const void *tokens, int token_bytes, int64_t ignore, int top,
+                                       const float *stats, const float *entropy, const int64_t *top_index,
+                                       const float *g, const float *gh, const float *gt, void *dz, hipStream_t st);
+
 hipError_t launch_key_mask_lengths(const uint8_t *mask, int64_t sb, int64_t sk, int B, int K,
                                    int32_t *kv_len, int32_t *kv_prefix, hipStream_t st);
 

@@ -241,6 +241,17 @@ SIGNATURES = {
         [c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64,
          c_void_p],
     ),
+    "tsattn_token_probs_workspace": (c_size_t, [c_int64, c_int32, c_int32]),
+    "tsattn_token_probs": (
+        c_int,
+        [c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int32, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "tsattn_token_probs_backward": (
+        c_int,
+        [c_int32, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int64, c_int32, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
     "tsattn_linear_wgrad_workspace": (c_size_t, [c_int32, c_int32, c_int32]),
     "tsattn_linear_wgrad": (
         c_int,

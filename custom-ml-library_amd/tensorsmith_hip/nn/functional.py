@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 from .. import _lib
 from ..amp import _autocast, _cast_inputs
@@ -21,7 +22,7 @@ from .attention import rotary_embedding, scaled_dot_product_attention
 
 __all__ = [
     "cross_entropy", "dropout", "embedding", "gelu", "layer_norm", "linear", "rms_norm",
-    "rotary_embedding", "scaled_dot_product_attention", "silu",
+    "rotary_embedding", "scaled_dot_product_attention", "silu", "token_log_probs",
 ]
 
 
@@ -407,3 +408,95 @@ def cross_entropy(input: Tensor, target: Tensor, reduction: str = "mean", *, axi
         return (grad.reshape(expected + (classes,)).permute(*inverse).to(input.dtype),)
 
     return Tensor._from_op(out, (input,), backward, "cross_entropy")
+
+
+class TokenLogProbs(NamedTuple):
+    """What ``token_log_probs`` gives: float32 tensors of the targets' shape, the top ones with a last dimension
+    of ``top_k`` (None without them), their indices in int64."""
+
+    log_probs: Tensor
+    entropy: Tensor
+    top_log_probs: Tensor | None
+    top_indices: Tensor | None
+
+
+class _Parts:
+    """Upstream gradients of a node with several results, one or None for each."""
+
+    def __init__(self, *grads):
+        self.grads, self.dtype = grads, next(g.dtype for g in grads if g is not None)
+
+    def __add__(self, other):
+        return _Parts(*(b if a is None else a if b is None else a + b for a, b in zip(self.grads, other.grads)))
+
+
+def token_log_probs(input: Tensor, target: Tensor, top_k: int = 0, *, ignore_index: int = -100) -> TokenLogProbs:
+    """Log probabilities of the tokens ``target`` [...] under logits [..., classes], the distributions' entropies
+    (in nats) and, with ``top_k`` (at most 64), their most likely tokens in falling order, ties to the lower index:
+    one pass over the logits (``tsattn_token_probs``), without a log-softmax in memory, and one for the gradient of
+    all of them.  Sums are in float32 whatever the logits' dtype.
+
+    A target of ``ignore_index`` is padding: its row is not read and gives 0, 0, -inf and -1, and no gradient.
+    Nothing waits for the device, so a target outside the classes is not refused: its log probability is NaN.  So are
+    the results of a row that holds a NaN or +inf, or nothing but -inf."""
+    if input.ndim < 1 or input.shape[-1] == 0:
+        raise ValueError("token_log_probs expects logits of [..., classes]")
+    if input.device != target.device or "float" not in str(input.dtype):
+        raise ValueError("token_log_probs needs floating logits and targets on the same device")
+    if target.requires_grad:
+        raise ValueError("target tokens cannot require gradients")
+    if "int" not in str(target.dtype):
+        raise TypeError("target tokens must have an integer dtype")
+    if target.shape != input.shape[:-1]:
+        raise ValueError(f"target shape {target.shape} does not match logits shape {input.shape}")
+    classes = input.shape[-1]
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(classes, 64):
+        raise ValueError("top_k must be between zero and 64 and within the classes")
+    _require_hip(input, "token_log_probs")
+    code = _code(input._data)
+    if code < 0:
+        raise TypeError("token_log_probs takes float32, float16 or bfloat16 logits")
+    import torch
+
+    z = input._data.reshape(-1, classes)
+    z = z if z.stride(1) == 1 or classes == 1 else z.contiguous()
+    y = target._data.reshape(-1)
+    if y.dtype not in (torch.int64, torch.int32):
+        y = y.long()
+    y = y.contiguous()
+    rows, dev = z.shape[0], input.device
+    recording = is_grad_enabled() and input.requires_grad
+    floats = torch.empty((2 + 2 * recording + top_k, rows), dtype=torch.float32, device=z.device)
+    logp, entropy = floats[0], floats[1]
+    stats = floats[2:4] if recording else None
+    top = floats[2 + 2 * recording:] if top_k else None
+    index = torch.empty((rows, top_k), dtype=torch.int64, device=z.device) if top_k else None
+    lib = _lib.load()
+    if rows:
+        nbytes = lib.tsattn_token_probs_workspace(rows, classes, top_k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device) if nbytes else None
+        _lib.check(launch(dev, lib.tsattn_token_probs, code, rows, classes, z.data_ptr(), z.stride(0), y.data_ptr(),
+                          y.element_size(), ignore_index, top_k, logp.data_ptr(), entropy.data_ptr(), _ptr(stats),
+                          _ptr(top), _ptr(index), _ptr(ws), nbytes), "token log probabilities")
+
+    def backward(parts):
+        g, gh, gt = parts.grads
+        g, gh, gt = (None if u is None else u.reshape(-1).contiguous() for u in (g, gh, gt))
+        dz = torch.empty((rows, classes), dtype=z.dtype, device=z.device)
+        if rows:
+            _lib.check(launch(dev, lib.tsattn_token_probs_backward, code, rows, classes, z.data_ptr(), z.stride(0),
+                              y.data_ptr(), y.element_size(), ignore_index, top_k, stats.data_ptr(),
+                              entropy.data_ptr(), _ptr(index), _ptr(g), _ptr(gh), _ptr(gt), dz.data_ptr()),
+                       "token log probabilities backward")
+        return (dz.reshape(input.shape),)
+
+    joint = Tensor._from_op(logp, (input,), backward, "token_log_probs")
+    shape = target.shape
+
+    def result(i, raw, op):
+        return Tensor._from_op(raw, (joint,), lambda u: (_Parts(*(u if k == i else None for k in range(3))),), op)
+
+    return TokenLogProbs(
+        result(0, logp.view(shape), "log_probs"), result(1, entropy.view(shape), "entropy"),
+        result(2, top.view(shape + (top_k,)), "top_log_probs") if top_k else None,
+        Tensor._leaf(index.view(shape + (top_k,)), dev) if top_k else None)

@@ -469,6 +469,12 @@ class TransformerLM(Module):
         return F.cross_entropy(self(tokens), targets, axis=-1, ignore_index=ignore_index,
                                label_smoothing=label_smoothing)
 
+    def token_log_probs(self, tokens: Tensor, targets: Tensor, top_k: int = 0, *,
+                        ignore_index=-100) -> F.TokenLogProbs:
+        """Log probabilities of ``targets`` [B, T] after each of ``tokens``, entropies and ``top_k`` alternatives
+        (``functional.token_log_probs``)."""
+        return F.token_log_probs(self(tokens), targets, top_k, ignore_index=ignore_index)
+
     def new_cache(self, batch_size: int, max_seq_len: int | None = None, *,
                   quantized=False, paged=False) -> list[KVCache] | list[PagedKVCache]:
         """One cache per block: in the weights' dtype, ``quantized`` in int8, or ``paged`` in 4 bits."""

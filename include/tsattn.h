@@ -477,6 +477,37 @@ int tsattn_linear_wgrad(int32_t dtype, int32_t out_dtype, int32_t tokens, int32_
 size_t tsattn_linear_wgrad_workspace(int32_t tokens, int32_t m, int32_t n);
 
 /*
+ * Log probabilities of given tokens, the rows' entropies and their most likely tokens
+ * (no counterpart in the reference: cross_entropy, src/tensorsmith/nn/functional.py:
+ * 397-472, keeps the whole log-softmax).  logits: `rows` rows of `vocab` (f32, f16 or
+ * bf16), row stride in elements; tokens: [rows], token_bytes 8 (int64) or 4 (int32).
+ * log_probs[r] = z[token] - lse(z), entropy[r] = -sum p ln p, in fp32; a logit of -inf
+ * adds nothing.  top > 0 (at most 64 and vocab): the largest log probabilities in
+ * falling order and their indices, ties to the lower index, a NaN counting as the
+ * largest.  A row whose token is `ignore` is not read: 0, 0, -inf and -1.  Another
+ * token outside the vocabulary, or a row with a NaN, +inf or nothing but -inf, has NaN.
+ * stats: [rows, 2] kept for the VJP, or NULL.  Outputs contiguous; deterministic.
+ */
+int tsattn_token_probs(int32_t dtype, int64_t rows, int32_t vocab, const void *logits, int64_t row_stride,
+                       const void *tokens, int32_t token_bytes, int64_t ignore, int32_t top, float *log_probs,
+                       float *entropy, float *stats, float *top_log_probs, int64_t *top_indices, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* Bytes of scratch tsattn_token_probs needs (0: none): parts of rows that are too few to fill the GPU. */
+size_t tsattn_token_probs_workspace(int64_t rows, int32_t vocab, int32_t top);
+
+/*
+ * Its VJP: dlogits [rows, vocab] (contiguous, dtype, every element written) from the
+ * saved stats, entropy and indices and the upstream gradients of log_probs, entropy
+ * [rows] and top_log_probs [rows, top], each of which may be NULL.  Ignored rows get 0.
+ */
+int tsattn_token_probs_backward(int32_t dtype, int64_t rows, int32_t vocab, const void *logits, int64_t row_stride,
+                                const void *tokens, int32_t token_bytes, int64_t ignore, int32_t top,
+                                const float *stats, const float *entropy, const int64_t *top_indices,
+                                const float *g_log_probs, const float *g_entropy, const float *g_top,
+                                void *dlogits, void *stream);
+
+/*
  * One cached decode step of the attention layer, or of a whole pre-norm
  * decoder block, as one call: MultiHeadAttention.forward with a cache
  * (src/tensorsmith/nn/transformer.py:124-155) and TransformerDecoderBlock.forward
