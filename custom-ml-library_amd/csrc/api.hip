@@ -150,17 +150,43 @@ int check_rope(const tsattn_rope_desc *r, const tsattn::Problem &pr, tsattn::Rop
   return TSATTN_OK;
 }
 
+// A problem with a sliding window, which only the MFMA kernels take.
+int check_window(const tsattn_problem *p, int64_t window, int32_t sinks, tsattn::Problem *pr) {
+  int rc = check_problem(p, pr);
+  if (rc) return rc;
+  if (window < 1 || sinks < 0)
+    return fail(TSATTN_ERR_INVALID, "a window holds at least one key, and the sinks are not negative");
+  if (!pr->causal) return fail(TSATTN_ERR_INVALID, "a window needs causal attention");
+  if (pr->drop.on || !tsattn::windowed_mask(*pr))
+    return fail(TSATTN_ERR_UNSUPPORTED, "windows take no dropout and no mask but key padding");
+  pr->window = static_cast<int>(window < (1 << 30) ? window : 1 << 30);
+  pr->sinks = sinks < pr->Sk ? sinks : pr->Sk;
+  return TSATTN_OK;
+}
+
+int window_unsupported() {
+  return fail(TSATTN_ERR_UNSUPPORTED,
+              "windows need the MFMA kernels (head dims 64 / 128 or 32 in f16 / bf16, 32 / 64 / 128 in f32, 16-byte "
+              "aligned views); give the window as a mask instead");
+}
+
 int rope_unsupported() {
   return fail(TSATTN_ERR_UNSUPPORTED,
               "RoPE folded into attention needs the MFMA kernels (f16/bf16, dim_qk and dim_v in "
               "{64, 128}, 16-byte aligned views); rotate with tsattn_rope instead");
 }
 
+struct Window {
+  int64_t keys;  // 0: none
+  int32_t sinks;
+  bool given;
+};
+
 int sdpa_forward(const tsattn_problem *p, const tsattn_rope_desc *rope, const tsattn_view *q,
                  const tsattn_view *k, const tsattn_view *v, const tsattn_view *out, void *lse,
-                 void *workspace, size_t workspace_bytes, void *stream) {
+                 void *workspace, size_t workspace_bytes, void *stream, Window win = Window{}) {
   tsattn::Problem pr;
-  int rc = check_problem(p, &pr);
+  int rc = win.given ? check_window(p, win.keys, win.sinks, &pr) : check_problem(p, &pr);
   if (rc) return rc;
   if ((rc = check_view(q, "query")) || (rc = check_view(k, "key")) ||
       (rc = check_view(v, "value")) || (rc = check_view(out, "output")))
@@ -187,6 +213,7 @@ int sdpa_forward(const tsattn_problem *p, const tsattn_rope_desc *rope, const ts
     return hip_status(tsattn::launch_mfma_f32_forward(pr, vq, vk, vv, vo, static_cast<float *>(lse), st),
                       "fp32 mfma forward launch");
   }
+  if (win.given) return window_unsupported();
   g_last_path = 1;
   rc = hip_status(tsattn::launch_generic_forward(pr, p->dtype, vq, vk, vv, vo, lse, st),
                   "generic forward launch");
@@ -240,9 +267,9 @@ int sdpa_backward(const tsattn_problem *p, const tsattn_rope_desc *rope, const t
                   const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
                   const tsattn_view *dout, const void *lse, const tsattn_view *dq,
                   const tsattn_view *dk, const tsattn_view *dv, void *workspace,
-                  size_t workspace_bytes, void *stream) {
+                  size_t workspace_bytes, void *stream, Window win = Window{}) {
   tsattn::Problem pr;
-  int rc = check_problem(p, &pr);
+  int rc = win.given ? check_window(p, win.keys, win.sinks, &pr) : check_problem(p, &pr);
   if (rc) return rc;
   if ((rc = check_view(q, "query")) || (rc = check_view(k, "key")) ||
       (rc = check_view(v, "value")) || (rc = check_view(out, "output")) ||
@@ -276,9 +303,13 @@ int sdpa_backward(const tsattn_problem *p, const tsattn_rope_desc *rope, const t
         return rc;
     }
     // stored dS when the workspace has room for it (as sized by the query)
+    // (a window: room for the sinks' partial sums, which it needs)
     void *ds = nullptr;
-    const size_t ds_bytes = tsattn::mfma_ds_bytes(pr);
+    const size_t ds_bytes = win.given ? tsattn::mfma_window_bytes(pr) : tsattn::mfma_ds_bytes(pr);
     const size_t ds_off = round256(with_bits(rows_need, pr));
+    if (win.given && ds_bytes && workspace_bytes < ds_off + ds_bytes)
+      return fail(TSATTN_ERR_INVALID, "backward workspace too small: %zu < %zu bytes", workspace_bytes,
+                  ds_off + ds_bytes);
     if (ds_bytes && workspace_bytes >= ds_off + ds_bytes) ds = static_cast<char *>(workspace) + ds_off;
     g_last_path = 2;
     return hip_status(tsattn::launch_mfma_backward(pr, p->dtype, vq, vk, vv, vo, vg,
@@ -296,6 +327,7 @@ int sdpa_backward(const tsattn_problem *p, const tsattn_rope_desc *rope, const t
                                                        vdq, vdk, vdv, static_cast<float *>(workspace), st),
                       "fp32 mfma backward launch");
   }
+  if (win.given) return window_unsupported();
   g_last_path = 1;
   return hip_status(tsattn::launch_generic_backward(pr, p->dtype, vq, vk, vv, vo, vg, lse, vdq,
                                                     vdk, vdv, workspace, st),
@@ -758,6 +790,28 @@ int tsattn_sdpa_forward_split(const tsattn_problem *p, const tsattn_rope_desc *r
 }
 
 size_t tsattn_sdpa_backward_workspace(const tsattn_problem *p) { return backward_workspace(p); }
+
+int tsattn_window_forward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
+                          const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
+                          void *lse, void *stream) {
+  return sdpa_forward(p, rope, q, k, v, out, lse, nullptr, 0, stream, Window{window, sinks, true});
+}
+
+size_t tsattn_window_backward_workspace(const tsattn_problem *p, int64_t window, int32_t sinks, int32_t rope) {
+  tsattn::Problem pr;
+  if (check_window(p, window, sinks, &pr)) return 0;
+  const size_t base = rope ? rope_rows_workspace(pr) : rows_workspace(p);
+  const size_t parts = tsattn::mfma_supported(pr, p->dtype) ? tsattn::mfma_window_bytes(pr) : 0;
+  return parts ? round256(base) + parts : base;
+}
+
+int tsattn_window_backward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
+                           const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
+                           const tsattn_view *dout, const void *lse, const tsattn_view *dq, const tsattn_view *dk,
+                           const tsattn_view *dv, void *workspace, size_t workspace_bytes, void *stream) {
+  return sdpa_backward(p, rope, q, k, v, out, dout, lse, dq, dk, dv, workspace, workspace_bytes, stream,
+                       Window{window, sinks, true});
+}
 
 size_t tsattn_sdpa_backward_rope_workspace(const tsattn_problem *p) {
   tsattn::Problem pr;

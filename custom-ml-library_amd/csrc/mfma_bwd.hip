@@ -26,6 +26,11 @@
 // the rounded gradients, so they are those of the unrotated queries and keys
 // (bit-identical to a separate inverse tsattn_rope).
 //
+// Windows (template WIN) as in the forward: dQ walks the run of key tiles that its rows
+// see, dK/dV the query rows that see its keys.  Those of the sinks' key blocks are all
+// rows, one chain many times the others' (S8192, window 1024: 256 query tiles against
+// 37): they are cut into parts whose sums another kernel adds up in order.
+//
 // Masks (template MK) as in the forward: a key mask reduced to lengths, or a
 // general boolean / additive mask read per (query row, key) on every tile
 // (additive: P = exp(S scale + mask - LSE)).
@@ -74,6 +79,10 @@ struct BwdArgs {
   // when the dS of all of them exceeds the region's cap: the region holds
   // the slices of one chunk's query heads (slice index (g - g0) rep + r).
   int g0, ng;
+  // Window: the key blocks with sinks, and the parts that each one's query rows are cut
+  // into (1: no partial sums), whose dK^T, dV^T registers are stored in `part`.
+  int sink_blocks, parts;
+  float *part;
 };
 
 // Start of query tile qt's dS row within its slice, in tiles.
@@ -158,8 +167,9 @@ constexpr int dkdv_wg_per_cu() {
 }
 
 // DK = head dim of q / k (and dK), DV = of v / dO (and dV); each 64 or 128.
-template <typename T, int DK, int DV, int MK, bool DR>
+template <typename T, int DK, int DV, int MK, bool DR, bool WIN>
 __global__ __launch_bounds__(NT, (dkdv_wg_per_cu<DK, DV, MK, DR>())) void dkdv_kernel(BwdArgs a) {
+  static_assert(!WIN || (MK == 0 && !DR), "windows have no general mask and no dropout");
   constexpr int TILE_Q = QT * DK * 2, TILE_G = QT * DV * 2;  // bytes of a Q / dO tile
   // A staged mask: the tile's [QT rows][KB keys] elements, row-major.
   constexpr bool MSTAGE = mask_staged(MK);
@@ -200,10 +210,24 @@ __global__ __launch_bounds__(NT, (dkdv_wg_per_cu<DK, DV, MK, DR>())) void dkdv_k
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n_kb = (p.Sk + KB - 1) / KB;
-  const int total = n_kb * a.ng;
+  // Window: the sinks' blocks see every query row from theirs on, the others 128 +
+  // window of them, so the former are cut into parts of about as many, which come first.
+  const int sunk = WIN ? a.sink_blocks * a.parts : 0;
+  const int n_units = WIN ? sunk + n_kb - a.sink_blocks : n_kb;
+  const int total = n_units * a.ng;
   const int logical = xcd_remap(blockIdx.x, total);
   int bhc, kb;  // early key blocks see the most queries: run them first
-  heavy_first(logical, n_kb, a.ng, 32 * dkdv_wg_per_cu<DK, DV, MK, DR>(), bhc, kb);  // slots per XCD
+  heavy_first(logical, n_units, a.ng, 32 * dkdv_wg_per_cu<DK, DV, MK, DR>(), bhc, kb);  // slots per XCD
+  int part = 0, parts = 1;
+  if constexpr (WIN) {
+    if (kb < sunk) {
+      parts = a.parts;
+      part = kb % parts;
+      kb /= parts;
+    } else {
+      kb += a.sink_blocks - sunk;
+    }
+  }
   const int bh = a.g0 + bhc;  // group (b, kv head); bhc: its index within the chunk
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int k0 = kb * KB, kw = k0 + 32 * w, key = kw + c;
@@ -229,8 +253,23 @@ __global__ __launch_bounds__(NT, (dkdv_wg_per_cu<DK, DV, MK, DR>())) void dkdv_k
     q_start = s0 <= 0 ? 0 : static_cast<int>(s0 < p.Sq ? s0 : p.Sq);
     q_start = (q_start / QT) * QT;
   }
+  // Window: a key past the sinks is seen by rows below kwin, every key of the wave by
+  // rows below q_far.
+  int q_stop = p.Sq, kwin = 1 << 30, q_far = 1 << 30;
+  if constexpr (WIN) {
+    auto end = [&](int k) {
+      const int64_t e = static_cast<int64_t>(k) - p.offset + p.window;
+      return static_cast<int>(e < -(1 << 30) ? -(1 << 30) : (e < (1 << 30) ? e : 1 << 30));
+    };
+    if (key >= p.sinks) kwin = end(key);
+    if (kw + 32 > p.sinks) q_far = end(max(kw, p.sinks));
+    if (k0 >= p.sinks) q_stop = max(q_start, min(p.Sq, end(k0 + KB - 1)));
+    const int tiles = (q_stop - q_start + QT - 1) / QT;
+    q_stop = min(q_stop, q_start + QT * static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / parts));
+    q_start += QT * static_cast<int>(static_cast<int64_t>(tiles) * part / parts);
+  }
   // wave-uniform by construction; readfirstlane keeps them in SGPRs
-  const int n_qt = __builtin_amdgcn_readfirstlane(k0 < kv_end ? (p.Sq - q_start + QT - 1) / QT : 0);
+  const int n_qt = __builtin_amdgcn_readfirstlane(k0 < kv_end ? (q_stop - q_start + QT - 1) / QT : 0);
   const int n_iter = __builtin_amdgcn_readfirstlane(n_qt * p.rep);
 
   const uint32_t qs_b = static_cast<uint32_t>(a.qk.s2) * 2, gs_b = static_cast<uint32_t>(a.dout.s2) * 2;
@@ -644,10 +683,10 @@ __global__ __launch_bounds__(NT, (dkdv_wg_per_cu<DK, DV, MK, DR>())) void dkdv_k
 
     // P = exp2(sacc sl), dS = P dpacc; rows crow(e, h) = 8 g + 4 h + e % 4.
     const bool edge = MK != 0 || keymask || kw + 32 > kv_end || q0 + QT > p.Sq ||
-                      (causal && q0 < q_diag);
+                      (causal && q0 < q_diag) || (WIN && q0 + QT > q_far);
     int lo = -64, hi = 64;
     if (edge) {
-      hi = key_live ? p.Sq - q0 - 4 * h : -64;
+      hi = key_live ? (WIN ? min(p.Sq, kwin) : p.Sq) - q0 - 4 * h : -64;
       if (causal) lo = min(64, max(-64, kdiff - q0 - 4 * h));
     }
     u32x4 pp[2], pd[2];
@@ -786,6 +825,22 @@ __global__ __launch_bounds__(NT, (dkdv_wg_per_cu<DK, DV, MK, DR>())) void dkdv_k
   // writes there.
   wait_vm_n<0>();
   if constexpr (!DR) __syncthreads();
+  if constexpr (WIN) {
+    if (parts > 1) {
+      // the accumulators as they lie, 256 bytes a register and wave
+      float *to = a.part + ((((static_cast<int64_t>(bhc) * a.sink_blocks + kb) * parts + part) * NW + w) *
+                            (16 * (PDK + PDV))) * 64 + lane;
+#pragma unroll
+      for (int dt = 0; dt < PDK; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) to[(16 * dt + e) * 64] = dk_acc[dt][e];
+#pragma unroll
+      for (int dt = 0; dt < PDV; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) to[(16 * (PDK + dt) + e) * 64] = dv_acc[dt][e];
+      return;
+    }
+  }
 
   // Epilogue.  The ring is free.  Each wave rounds its rows and stages them in its own
   // slice of the ring -- key row r (0..31) at r * 2DX bytes, 16-byte chunk q
@@ -883,6 +938,38 @@ __global__ __launch_bounds__(NT, (dkdv_wg_per_cu<DK, DV, MK, DR>())) void dkdv_k
   }
 }
 
+// Window: the parts of a sinks' key block, added up in their order; workgroup and lanes
+// hold what the dK/dV kernel's do.
+template <typename T, int DK, int DV>
+__global__ __launch_bounds__(NT) void sink_sum_kernel(BwdArgs a) {
+  constexpr int REGS = DK / 2 + DV / 2;
+  const Problem &p = a.p;
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, w = threadIdx.x >> 6;
+  const int bh = blockIdx.x / a.sink_blocks, kb = blockIdx.x % a.sink_blocks;
+  const int b = bh / p.Hkv, hk = bh - b * p.Hkv, key = kb * KB + 32 * w + c;
+  const float *from = a.part + ((static_cast<int64_t>(blockIdx.x) * a.parts * NW + w) * REGS) * 64 + lane;
+  T *rows[2] = {mut<T>(a.dk) + b * a.dk.s0 + hk * a.dk.s1 + static_cast<int64_t>(key) * a.dk.s2,
+                mut<T>(a.dv) + b * a.dv.s0 + hk * a.dv.s1 + static_cast<int64_t>(key) * a.dv.s2};
+  // register 16 dt + 4 g + r is channel 32 dt + 8 g + 4 h + r of the lane's key
+  for (int g = 0; g < REGS / 4; ++g) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.parts; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] += from[(static_cast<int64_t>(i) * NW * REGS + 4 * g + r) * 64];
+    if (key >= p.Sk) continue;
+    const bool is_k = g < DK / 8;
+    const int d = 8 * (is_k ? g : g - DK / 8) + 4 * h;
+    const float f = is_k ? a.scale : 1.f;
+    u32x2 y{pack2<T>(x[0] * f, x[1] * f), pack2<T>(x[2] * f, x[3] * f)};
+    if (is_k && d < p.rope.R) {  // (R is a multiple of 8)
+      const int64_t at = (p.rope.kpos0 + key) * (p.rope.R / 2) + d / 2;
+      const T *cs = static_cast<const T *>(p.rope.cos) + at, *sn = static_cast<const T *>(p.rope.sin) + at;
+      y = u32x2{rotate_word<T>(y[0], cs[0], sn[0], true), rotate_word<T>(y[1], cs[1], sn[1], true)};
+    }
+    *reinterpret_cast<u32x2 *>(rows[is_k ? 0 : 1] + d) = y;
+  }
+}
+
 // ---------------------------------------------------------------------------
 // dQ: one workgroup = 128 query rows of one (b, q head), 4 waves x 32 rows,
 // two workgroups per CU; a wave keeps its Q and dO rows as B operands in
@@ -899,8 +986,9 @@ constexpr int DQ_PD = 2;              // tiles issued ahead
 constexpr int DQ_NS = DQ_PD + 2;      // ring stages: tile j is read in iterations j and j + 1
 
 // DK = head dim of q / k (and dQ), DV = of v / dO; each 64 or 128.
-template <typename T, int DK, int DV, int MK, bool DR>
+template <typename T, int DK, int DV, int MK, bool DR, bool WIN>
 __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
+  static_assert(!WIN || (MK == 0 && !DR), "windows have no general mask and no dropout");
   constexpr int TILE_K = KT * DK * 2, TILE_V = KT * DV * 2;  // bytes per K / V tile
   // K | V | with dropout each wave's 32 keep-bit words (its rows, this key tile)
   constexpr int STAGE = TILE_K + TILE_V + (DR ? NW * 128 : 0);
@@ -945,10 +1033,17 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
   }
   if (qw >= p.Sq) wlim = 0;
   // wave-uniform by construction; readfirstlane keeps them in SGPRs
-  const int n_tiles =
+  int n_tiles =
       __builtin_amdgcn_readfirstlane(lim > 0 ? static_cast<int>((lim + KT - 1) / KT) : 0);
-  const int w_tiles =
+  int w_tiles =
       __builtin_amdgcn_readfirstlane(wlim > 0 ? static_cast<int>((wlim + KT - 1) / KT) : 0);
+  // Window: the run of tiles that the workgroup's rows see, as in the forward.
+  const WindowTiles run(p, q0);
+  if constexpr (WIN) {
+    n_tiles = run.count(n_tiles);
+    w_tiles = run.count(w_tiles);
+  }
+  auto phys = [&](int j) { return WIN ? run.phys(j) : j; };
 
   // The rows' Q, dO and O fragments (lane holds row qrow, channels 16 ks +
   // 8 h .. +7) and LSE, issued here; consumed after the first tiles' DMA
@@ -1000,8 +1095,8 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
     d.tile = tile;
     d.keep = ~static_cast<uint32_t>((n_tiles - 1 - tile) >> 31);  // sign fill
     d.far = ~d.keep & 0x80000000u;  // offsets >= 2^31 are past every range
-    d.krow = (static_cast<uint32_t>(tile * KT) * ks_b) | d.far;
-    d.vrow = (static_cast<uint32_t>(tile * KT) * vs_b) | d.far;
+    d.krow = (static_cast<uint32_t>(phys(tile) * KT) * ks_b) | d.far;
+    d.vrow = (static_cast<uint32_t>(phys(tile) * KT) * vs_b) | d.far;
     d.st = (lds0 + (tile % DQ_NS) * STAGE - spare) & d.keep;
     return d;
   };
@@ -1060,6 +1155,8 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
     const int64_t cl = static_cast<int64_t>(qrow) + p.offset + 1;
     if (cl < kv_end) klim = cl < 0 ? 0 : static_cast<int>(cl);
   }
+  const int klow = WIN ? window_low(p, qrow) : 0;
+  const int wlow = WIN ? __builtin_amdgcn_readfirstlane(window_low(p, min(qw + 32, p.Sq) - 1)) : 0;
   const uint8_t *kmask_b =
       keymask ? static_cast<const uint8_t *>(p.mask.data) + b * p.mask.s0 : nullptr;
   // General mask: the (b, hq) slice as a buffer; this lane reads row qrow.
@@ -1182,11 +1279,11 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
   };
 
   auto grad = [&](int j, int) {
-    const int kv0 = j * KT;
+    const int kv0 = phys(j) * KT;
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = s[i];
-    if (j >= j_edge) {
+    if (phys(j) >= j_edge || (WIN && kv0 < wlow && kv0 + KT > p.sinks)) {
       const int lim_l = klim - kv0 - 4 * h;
       if constexpr (MK == 0) {
         unsigned kbits = ~0u;
@@ -1198,7 +1295,8 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int kc = 8 * (i >> 2) + (i & 3);
-          const bool ok = (kc < lim_l) & (((kbits >> kc) & 1u) != 0);
+          bool ok = (kc < lim_l) & (((kbits >> kc) & 1u) != 0);
+          if constexpr (WIN) ok = ok & ((kc < p.sinks - kv0 - 4 * h) | (kc >= klow - kv0 - 4 * h));
           x[i] = ok ? x[i] : -INFINITY;
         }
       } else {
@@ -1639,7 +1737,7 @@ void launch_mk(const BwdArgs &a0, hipStream_t st) {
       a.ng = min(per_chunk, groups - a.g0);
       {
         Probe pr_(DR ? "bwd_dkdv_mfma_dropout" : (MK ? "bwd_dkdv_mfma_masked" : "bwd_dkdv_mfma"), st);
-        dkdv_kernel<T, DK, DV, MK, DR><<<dim3(n_kb * a.ng), dim3(NT), 0, st>>>(a);
+        dkdv_kernel<T, DK, DV, MK, DR, false><<<dim3(n_kb * a.ng), dim3(NT), 0, st>>>(a);
       }
       {
         Probe pr_(DR ? "bwd_dq_ds_dropout" : (MK ? "bwd_dq_ds_masked" : "bwd_dq_ds"), st);
@@ -1654,12 +1752,12 @@ void launch_mk(const BwdArgs &a0, hipStream_t st) {
   const int n_qb = (p.Sq + QB - 1) / QB;
   {
     Probe pr_(DR ? "bwd_dq_mfma_dropout" : (MK ? "bwd_dq_mfma_masked" : "bwd_dq_mfma"), st);
-    dq_kernel<T, DK, DV, MKQ, DR><<<dim3(n_qb * p.Hq * p.B), dim3(NT), 0, st>>>(a);
+    dq_kernel<T, DK, DV, MKQ, DR, false><<<dim3(n_qb * p.Hq * p.B), dim3(NT), 0, st>>>(a);
   }
   const int n_kb = (p.Sk + KB - 1) / KB;
   {
     Probe pr_(DR ? "bwd_dkdv_mfma_dropout" : (MK ? "bwd_dkdv_mfma_masked" : "bwd_dkdv_mfma"), st);
-    dkdv_kernel<T, DK, DV, MK, DR><<<dim3(n_kb * a.ng), dim3(NT), 0, st>>>(a);
+    dkdv_kernel<T, DK, DV, MK, DR, false><<<dim3(n_kb * a.ng), dim3(NT), 0, st>>>(a);
   }
 }
 
@@ -1676,8 +1774,29 @@ void launch_dr(const BwdArgs &a, int mkq, hipStream_t st) {
   }
 }
 
+// Window: dQ (and the row values) recomputing S and dP, dK/dV, the sinks' parts.
+template <typename T, int DK, int DV>
+void launch_window(const BwdArgs &a, hipStream_t st) {
+  const Problem &p = a.p;
+  const int n_qb = (p.Sq + QB - 1) / QB, n_kb = (p.Sk + KB - 1) / KB;
+  {
+    Probe pr_("bwd_dq_mfma_window", st);
+    dq_kernel<T, DK, DV, 0, false, true><<<dim3(n_qb * p.Hq * p.B), dim3(NT), 0, st>>>(a);
+  }
+  {
+    Probe pr_("bwd_dkdv_mfma_window", st);
+    dkdv_kernel<T, DK, DV, 0, false, true>
+        <<<dim3((n_kb + a.sink_blocks * (a.parts - 1)) * a.ng), dim3(NT), 0, st>>>(a);
+  }
+  if (a.sink_blocks && a.parts > 1) {
+    Probe pr_("bwd_sink_sum", st);
+    sink_sum_kernel<T, DK, DV><<<dim3(a.sink_blocks * a.ng), dim3(NT), 0, st>>>(a);
+  }
+}
+
 template <typename T, int DK, int DV>
 void launch_dims(const BwdArgs &a, hipStream_t st) {
+  if (a.p.window) return launch_window<T, DK, DV>(a, st);
   const int mkq = mfma_mask_mode_vec(a.p);
   if (a.p.drop.on) launch_dr<T, DK, DV, true>(a, mkq, st);
   else launch_dr<T, DK, DV, false>(a, mkq, st);
@@ -1751,6 +1870,20 @@ size_t mfma_ds_bytes(const Problem &p) {
   return static_cast<size_t>(bytes);
 }
 
+// Key blocks with sinks, and the parts of each: of about the query tiles that the other
+// blocks see (B2 Hkv4 S8192, window 1024: 7 parts of 37 tiles), at most 64.
+static int window_sink_blocks(const Problem &p) { return min((p.sinks + KB - 1) / KB, (p.Sk + KB - 1) / KB); }
+static int window_parts(const Problem &p) {
+  const int64_t all = (p.Sq + QT - 1) / QT, other = (KB + static_cast<int64_t>(p.window)) / QT + 1;
+  const int64_t parts = (all + other - 1) / other;
+  return static_cast<int>(parts < 64 ? parts : 64);
+}
+
+size_t mfma_window_bytes(const Problem &p) {
+  const int blocks = p.window ? window_sink_blocks(p) : 0, parts = blocks ? window_parts(p) : 1;
+  return parts < 2 ? 0 : static_cast<size_t>(p.B) * p.Hkv * blocks * parts * KB * (p.Dqk + p.Dv) * sizeof(float);
+}
+
 hipError_t launch_mfma_backward(const Problem &p, int dtype, View q, View k, View v, View o,
                                 View dout, const float *lse, View dq, View dk, View dv,
                                 float *delta, void *ds, hipStream_t st) {
@@ -1764,8 +1897,13 @@ hipError_t launch_mfma_backward(const Problem &p, int dtype, View q, View k, Vie
   }
   BwdArgs a{p, q, k, v, o, dout, dq, dk, dv, qk, lse, delta,
             static_cast<float>(p.scale) * kLog2e, static_cast<float>(p.scale),
-            static_cast<char *>(ds), ds_key_tiles(p), ds_packed(p), ds_slice_tiles(p),
-            0, p.B * p.Hkv};
+            p.window ? nullptr : static_cast<char *>(ds), ds_key_tiles(p), ds_packed(p), ds_slice_tiles(p),
+            0, p.B * p.Hkv, 0, 1, nullptr};
+  if (p.window) {
+    a.sink_blocks = window_sink_blocks(p);
+    a.parts = a.sink_blocks ? window_parts(p) : 1;
+    a.part = static_cast<float *>(ds);
+  }
   return dtype == TSATTN_BF16 ? launch<bf16>(a, st) : launch<f16>(a, st);
 }
 

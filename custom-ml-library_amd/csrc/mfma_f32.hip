@@ -24,6 +24,10 @@
 // by direct buffer loads (DMA), each lane fetching the global chunk its
 // swizzled position holds; rows past the buffer range arrive as zeros.
 //
+// Windows (template WIN) as in the 16-bit kernels: the forward and dQ walk the run of
+// key tiles that their rows see, dK/dV the query rows that see its keys (all rows for the
+// sinks' keys, one chain here: fp32 sequences are the short ones).
+//
 // Masks (template MK): 0 = none, or a [B,1,1,K] key mask reduced to kv_len /
 // kv_prefix; 1 = any other boolean mask; 2 / 3 = an additive f32 / (f16 or
 // bf16) mask, each of any broadcast strides.  A wave reads its next tile's
@@ -302,8 +306,9 @@ struct F32Args {
 // online softmax merges tiles: the key loop of a row block runs 4 ways
 // parallel.  One workgroup per CU.
 // ---------------------------------------------------------------------------
-template <int D, bool SPLIT, int MK>
+template <int D, bool SPLIT, int MK, bool WIN>
 __global__ __launch_bounds__(NT, SPLIT ? 1 : 2) void fwd_f32_kernel(F32Args a) {
+  static_assert(!WIN || MK == 0, "windows have no general mask");
   using TL = FTile<D>;
   constexpr int HD = D / 2;             // MFMA steps over the head dimension
   constexpr int PDT = D / 32;           // 32-row blocks of O^T
@@ -340,8 +345,15 @@ __global__ __launch_bounds__(NT, SPLIT ? 1 : 2) void fwd_f32_kernel(F32Args a) {
     wlim = min(wlim, static_cast<int64_t>(min(qw + 32, p.Sq) - 1) + p.offset + 1);
   }
   if (qw >= p.Sq) wlim = 0;
-  const int n_tiles = __builtin_amdgcn_readfirstlane(lim > 0 ? static_cast<int>((lim + BN - 1) / BN) : 0);
-  const int w_tiles = __builtin_amdgcn_readfirstlane(wlim > 0 ? static_cast<int>((wlim + BN - 1) / BN) : 0);
+  int n_tiles = __builtin_amdgcn_readfirstlane(lim > 0 ? static_cast<int>((lim + BN - 1) / BN) : 0);
+  int w_tiles = __builtin_amdgcn_readfirstlane(wlim > 0 ? static_cast<int>((wlim + BN - 1) / BN) : 0);
+  // window: the run of tiles that the workgroup's rows see (mfma_fwd.hip)
+  const WindowTiles run(p, q0);
+  if constexpr (WIN) {
+    n_tiles = run.count(n_tiles);
+    w_tiles = run.count(w_tiles);
+  }
+  auto phys = [&](int j) __attribute__((always_inline)) { return WIN ? run.phys(j) : j; };
   // this wave's tiles: j = first + STRIDE jj, jj < my_tiles
   const int first = SPLIT ? w : 0;
   const int my_tiles = SPLIT ? (n_tiles > w ? (n_tiles - 1 - w) / NW + 1 : 0) : n_tiles;
@@ -390,11 +402,11 @@ __global__ __launch_bounds__(NT, SPLIT ? 1 : 2) void fwd_f32_kernel(F32Args a) {
     const bool real = tile < n_tiles;
     const uint32_t st = real ? ring + (jj & 1) * STAGE : spare;
     if (n < TL::BLOCKS) {
-      const uint32_t so = real ? static_cast<uint32_t>(tile * BN + n * TL::RPB) * ks_b : 0x80000000u;
+      const uint32_t so = real ? static_cast<uint32_t>(phys(tile) * BN + n * TL::RPB) * ks_b : 0x80000000u;
       dma16(kdesc, st + (real ? n * 1024 : 0), TL::dma_off(n, lane, ks_b), so);
     } else {
       const int m = n - TL::BLOCKS;
-      const uint32_t so = real ? static_cast<uint32_t>(tile * BN + m * TL::RPB) * vs_b : 0x80000000u;
+      const uint32_t so = real ? static_cast<uint32_t>(phys(tile) * BN + m * TL::RPB) * vs_b : 0x80000000u;
       dma16(vdesc, st + (real ? TL::BYTES + m * 1024 : 0), TL::dma_off(m, lane, vs_b), so);
     }
   };
@@ -415,6 +427,8 @@ __global__ __launch_bounds__(NT, SPLIT ? 1 : 2) void fwd_f32_kernel(F32Args a) {
     const int64_t cl = static_cast<int64_t>(qrow) + p.offset + 1;
     if (cl < kv_end) klim = cl < 0 ? 0 : static_cast<int>(cl);
   }
+  const int klow = WIN ? window_low(p, qrow) : 0;
+  const int wlow = WIN ? __builtin_amdgcn_readfirstlane(window_low(p, min(qw + 32, p.Sq) - 1)) : 0;
   const uint8_t *kmask_b = keymask ? static_cast<const uint8_t *>(p.mask.data) + b * p.mask.s0 : nullptr;
   int j_edge = kv_end / BN;
   if (MK != 0 || keymask) j_edge = 0;
@@ -484,8 +498,8 @@ __global__ __launch_bounds__(NT, SPLIT ? 1 : 2) void fwd_f32_kernel(F32Args a) {
         }
       }
       // softmax of this lane's query column: element i is key kv0 + crow(i, h)
-      const int kv0 = j * BN;
-      if (j >= j_edge) {
+      const int kv0 = phys(j) * BN;
+      if (phys(j) >= j_edge || (WIN && kv0 < wlow && kv0 + BN > p.sinks)) {
         const int lm = klim - kv0 - 4 * h;
         unsigned kbits = ~0u;
         if (keymask) {
@@ -498,7 +512,9 @@ __global__ __launch_bounds__(NT, SPLIT ? 1 : 2) void fwd_f32_kernel(F32Args a) {
         for (int i = 0; i < 16; ++i) {
           const int kc_ = 8 * (i >> 2) + (i & 3);
           if constexpr (ADD) s[i] = fmaf(s[i], a.scale, mask.add[i]);
-          s[i] = ((kc_ < lm) & (((kbits >> kc_) & 1u) != 0)) ? s[i] : -INFINITY;
+          bool ok = (kc_ < lm) & (((kbits >> kc_) & 1u) != 0);
+          if constexpr (WIN) ok = ok & ((kc_ < p.sinks - kv0 - 4 * h) | (kc_ >= klow - kv0 - 4 * h));
+          s[i] = ok ? s[i] : -INFINITY;
         }
       }
       float mx = -INFINITY;
@@ -687,8 +703,9 @@ __global__ __launch_bounds__(NT) void rows_f32_kernel(F32Args a) {
 // tiles w, w + 4, ... through its own ring, and the waves' dQ^T partial sums
 // add up through LDS in wave order at the end.
 // ---------------------------------------------------------------------------
-template <int D, bool SPLIT, int MK>
+template <int D, bool SPLIT, int MK, bool WIN>
 __global__ __launch_bounds__(NT, 1) void dq_f32_kernel(F32Args a) {
+  static_assert(!WIN || MK == 0, "windows have no general mask");
   using TL = FTile<D>;
   constexpr int HD = D / 2, PDT = D / 32;
   constexpr int STAGE = 2 * TL::BYTES;  // K | V
@@ -721,8 +738,15 @@ __global__ __launch_bounds__(NT, 1) void dq_f32_kernel(F32Args a) {
     wlim = min(wlim, static_cast<int64_t>(min(qw + 32, p.Sq) - 1) + p.offset + 1);
   }
   if (qw >= p.Sq) wlim = 0;
-  const int n_tiles = __builtin_amdgcn_readfirstlane(lim > 0 ? static_cast<int>((lim + BN - 1) / BN) : 0);
-  const int w_tiles = __builtin_amdgcn_readfirstlane(wlim > 0 ? static_cast<int>((wlim + BN - 1) / BN) : 0);
+  int n_tiles = __builtin_amdgcn_readfirstlane(lim > 0 ? static_cast<int>((lim + BN - 1) / BN) : 0);
+  int w_tiles = __builtin_amdgcn_readfirstlane(wlim > 0 ? static_cast<int>((wlim + BN - 1) / BN) : 0);
+  // window: the run of tiles that the workgroup's rows see (mfma_fwd.hip)
+  const WindowTiles run(p, q0);
+  if constexpr (WIN) {
+    n_tiles = run.count(n_tiles);
+    w_tiles = run.count(w_tiles);
+  }
+  auto phys = [&](int j) __attribute__((always_inline)) { return WIN ? run.phys(j) : j; };
   const int first = SPLIT ? w : 0;
   const int my_tiles = SPLIT ? (n_tiles > w ? (n_tiles - 1 - w) / NW + 1 : 0) : n_tiles;
 
@@ -771,11 +795,11 @@ __global__ __launch_bounds__(NT, 1) void dq_f32_kernel(F32Args a) {
     const bool real = tile < n_tiles;
     const uint32_t st = real ? ring + (jj & 1) * STAGE : spare;
     if (n < TL::BLOCKS) {
-      const uint32_t so = real ? static_cast<uint32_t>(tile * BN + n * TL::RPB) * ks_b : 0x80000000u;
+      const uint32_t so = real ? static_cast<uint32_t>(phys(tile) * BN + n * TL::RPB) * ks_b : 0x80000000u;
       dma16(kdesc, st + (real ? n * 1024 : 0), TL::dma_off(n, lane, ks_b), so);
     } else {
       const int m = n - TL::BLOCKS;
-      const uint32_t so = real ? static_cast<uint32_t>(tile * BN + m * TL::RPB) * vs_b : 0x80000000u;
+      const uint32_t so = real ? static_cast<uint32_t>(phys(tile) * BN + m * TL::RPB) * vs_b : 0x80000000u;
       dma16(vdesc, st + (real ? TL::BYTES + m * 1024 : 0), TL::dma_off(m, lane, vs_b), so);
     }
   };
@@ -784,6 +808,8 @@ __global__ __launch_bounds__(NT, 1) void dq_f32_kernel(F32Args a) {
     const int64_t cl = static_cast<int64_t>(qrow) + p.offset + 1;
     if (cl < kv_end) klim = cl < 0 ? 0 : static_cast<int>(cl);
   }
+  const int klow = WIN ? window_low(p, qrow) : 0;
+  const int wlow = WIN ? __builtin_amdgcn_readfirstlane(window_low(p, min(qw + 32, p.Sq) - 1)) : 0;
   const uint8_t *kmask_b = keymask ? static_cast<const uint8_t *>(p.mask.data) + b * p.mask.s0 : nullptr;
   int j_edge = kv_end / BN;
   if (MK != 0 || keymask) j_edge = 0;
@@ -865,11 +891,12 @@ __global__ __launch_bounds__(NT, 1) void dq_f32_kernel(F32Args a) {
         }
       }
       // P = exp2((S + nl) sl), dS = P (dP + nd): element i is key kv0 + crow(i, h)
-      const int kv0 = j * BN;
+      const int kv0 = phys(j) * BN;
       unsigned kbits = ~0u;
-      int lm = 64;
-      if (j >= j_edge) {
+      int lm = 64, low = -64;
+      if (phys(j) >= j_edge || (WIN && kv0 < wlow && kv0 + BN > p.sinks)) {
         lm = klim - kv0 - 4 * h;
+        if constexpr (WIN) low = klow - kv0 - 4 * h;
         if (keymask) {
           const int key = kv0 + lane;
           const bool ok = key < p.Sk && kmask_b[static_cast<int64_t>(key) * p.mask.s3];
@@ -883,7 +910,9 @@ __global__ __launch_bounds__(NT, 1) void dq_f32_kernel(F32Args a) {
         float x;  // log2 P
         if constexpr (MK >= 2) x = (fmaf(s[i], a.scale, mask.add[i]) + nl) * kLog2e;
         else x = (s[i] + nl) * sl;
-        const float pv = ((kc_ < lm) & (((kbits >> kc_) & 1u) != 0)) ? fast_exp2(x) : 0.f;
+        bool ok = (kc_ < lm) & (((kbits >> kc_) & 1u) != 0);
+        if constexpr (WIN) ok = ok & ((kc_ >= low) | (kc_ < p.sinks - kv0 - 4 * h));
+        const float pv = ok ? fast_exp2(x) : 0.f;
         s[i] = pv * (dp[i] + nd);
         if (CAREFUL && pv == 0.f) s[i] = 0.f;
       }
@@ -984,8 +1013,9 @@ __global__ __launch_bounds__(NT, 1) void dq_f32_kernel(F32Args a) {
 // of the (query head, query tile) walk through its own ring, and the waves'
 // dK^T / dV^T partial sums add up through LDS in wave order at the end.
 // ---------------------------------------------------------------------------
-template <int D, bool SPLIT, int MK>
+template <int D, bool SPLIT, int MK, bool WIN>
 __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
+  static_assert(!WIN || MK == 0, "windows have no general mask");
   using TL = FTile<D>;
   constexpr int HD = D / 2, PDT = D / 32;
   constexpr int RV = 2 * BN * 4;                 // nl | nd of the tile's rows
@@ -1019,7 +1049,17 @@ __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
     q_start = s0 <= 0 ? 0 : static_cast<int>(s0 < p.Sq ? s0 : p.Sq);
     q_start = (q_start / BN) * BN;
   }
-  const int n_qt = __builtin_amdgcn_readfirstlane(k0 < kv_end ? (p.Sq - q_start + BN - 1) / BN : 0);
+  // window: a key past the sinks is seen by rows below kwin
+  int q_stop = p.Sq, kwin = 1 << 30;
+  if constexpr (WIN) {
+    auto end = [&](int k) {
+      const int64_t e = static_cast<int64_t>(k) - p.offset + p.window;
+      return static_cast<int>(e < -(1 << 30) ? -(1 << 30) : (e < (1 << 30) ? e : 1 << 30));
+    };
+    if (key >= p.sinks) kwin = end(key);
+    if (k0 >= p.sinks) q_stop = max(q_start, min(p.Sq, end(k0 + KEYS - 1)));
+  }
+  const int n_qt = __builtin_amdgcn_readfirstlane(k0 < kv_end ? (q_stop - q_start + BN - 1) / BN : 0);
   const int n_iter = __builtin_amdgcn_readfirstlane(n_qt * p.rep);
   // this wave's tiles: it = first + STRIDE jj, jj < my_iter
   const int first = SPLIT ? w : 0;
@@ -1170,6 +1210,7 @@ __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
       const int rr = 8 * (i >> 2) + 4 * h + (i & 3);
       bool ok = key_live && (q0 + rr < p.Sq) && (!p.causal || kdiff <= q0 + rr);
       if constexpr (MK == 1) ok = ok && ((mask.bits >> (8 * (i >> 2) + (i & 3))) & 1u);
+      if constexpr (WIN) ok = ok && q0 + rr < kwin;
       float x;  // log2 P
       if constexpr (MK >= 2) x = (fmaf(s[i], a.scale, mask.add[i]) + rvl[rr]) * kLog2e;
       else x = (s[i] + rvl[rr]) * sl;
@@ -1276,7 +1317,7 @@ __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
   }
 }
 
-template <int D, int MK>
+template <int D, int MK, bool WIN>
 void launch_bwd_dims(const F32Args &a, hipStream_t st) {
   const Problem &p = a.p;
   {
@@ -1294,51 +1335,51 @@ void launch_bwd_dims(const F32Args &a, hipStream_t st) {
   }
   if (split_q) {
     if constexpr (D <= 64) {
-      Probe pr_(MK ? "bwd_dq_mfma_f32_masked_split" : "bwd_dq_mfma_f32_split", st);
-      dq_f32_kernel<D, true, MK><<<dim3(static_cast<unsigned>((p.Sq + 31) / 32 * qheads)), dim3(NT), 0, st>>>(a);
+      Probe pr_(WIN ? "bwd_dq_mfma_f32_window_split" : MK ? "bwd_dq_mfma_f32_masked_split" : "bwd_dq_mfma_f32_split", st);
+      dq_f32_kernel<D, true, MK, WIN><<<dim3(static_cast<unsigned>((p.Sq + 31) / 32 * qheads)), dim3(NT), 0, st>>>(a);
     }
   } else {
-    Probe pr_(MK ? "bwd_dq_mfma_f32_masked" : "bwd_dq_mfma_f32", st);
-    dq_f32_kernel<D, false, MK><<<dim3(static_cast<unsigned>(n_qb * qheads)), dim3(NT), 0, st>>>(a);
+    Probe pr_(WIN ? "bwd_dq_mfma_f32_window" : MK ? "bwd_dq_mfma_f32_masked" : "bwd_dq_mfma_f32", st);
+    dq_f32_kernel<D, false, MK, WIN><<<dim3(static_cast<unsigned>(n_qb * qheads)), dim3(NT), 0, st>>>(a);
   }
   if (split_k) {
     if constexpr (D <= 64) {
-      Probe pr_(MK ? "bwd_dkdv_mfma_f32_masked_split" : "bwd_dkdv_mfma_f32_split", st);
-      dkdv_f32_kernel<D, true, MK><<<dim3(static_cast<unsigned>((p.Sk + 31) / 32 * kheads)), dim3(NT), 0, st>>>(a);
+      Probe pr_(WIN ? "bwd_dkdv_mfma_f32_window_split" : MK ? "bwd_dkdv_mfma_f32_masked_split" : "bwd_dkdv_mfma_f32_split", st);
+      dkdv_f32_kernel<D, true, MK, WIN><<<dim3(static_cast<unsigned>((p.Sk + 31) / 32 * kheads)), dim3(NT), 0, st>>>(a);
     }
   } else {
-    Probe pr_(MK ? "bwd_dkdv_mfma_f32_masked" : "bwd_dkdv_mfma_f32", st);
-    dkdv_f32_kernel<D, false, MK><<<dim3(static_cast<unsigned>(n_kb * kheads)), dim3(NT), 0, st>>>(a);
+    Probe pr_(WIN ? "bwd_dkdv_mfma_f32_window" : MK ? "bwd_dkdv_mfma_f32_masked" : "bwd_dkdv_mfma_f32", st);
+    dkdv_f32_kernel<D, false, MK, WIN><<<dim3(static_cast<unsigned>(n_kb * kheads)), dim3(NT), 0, st>>>(a);
   }
 }
 
-template <int D, int MK>
+template <int D, int MK, bool WIN>
 void launch_fwd_dims(const F32Args &a, hipStream_t st) {
   const int64_t heads = static_cast<int64_t>(a.p.Hq) * a.p.B;
   const int64_t n_qb = (a.p.Sq + BM - 1) / BM;
   if constexpr (D <= 64) {  // (the split rings of D = 128 would not fit in LDS)
     if (n_qb * heads < device_cus()) {
-      Probe pr_(MK ? "fwd_mfma_f32_masked_split" : "fwd_mfma_f32_split", st);
-      fwd_f32_kernel<D, true, MK><<<dim3(static_cast<unsigned>((a.p.Sq + 31) / 32 * heads)), dim3(NT), 0, st>>>(a);
+      Probe pr_(WIN ? "fwd_mfma_f32_window_split" : MK ? "fwd_mfma_f32_masked_split" : "fwd_mfma_f32_split", st);
+      fwd_f32_kernel<D, true, MK, WIN><<<dim3(static_cast<unsigned>((a.p.Sq + 31) / 32 * heads)), dim3(NT), 0, st>>>(a);
       return;
     }
   }
-  Probe pr_(MK ? "fwd_mfma_f32_masked" : "fwd_mfma_f32", st);
-  fwd_f32_kernel<D, false, MK><<<dim3(static_cast<unsigned>(n_qb * heads)), dim3(NT), 0, st>>>(a);
+  Probe pr_(WIN ? "fwd_mfma_f32_window" : MK ? "fwd_mfma_f32_masked" : "fwd_mfma_f32", st);
+  fwd_f32_kernel<D, false, MK, WIN><<<dim3(static_cast<unsigned>(n_qb * heads)), dim3(NT), 0, st>>>(a);
 }
 
-template <int MK>
+template <int MK, bool WIN = false>
 void launch_fwd_mask(const F32Args &a, hipStream_t st) {
-  if (a.p.Dqk == 128) launch_fwd_dims<128, MK>(a, st);
-  else if (a.p.Dqk == 64) launch_fwd_dims<64, MK>(a, st);
-  else launch_fwd_dims<32, MK>(a, st);
+  if (a.p.Dqk == 128) launch_fwd_dims<128, MK, WIN>(a, st);
+  else if (a.p.Dqk == 64) launch_fwd_dims<64, MK, WIN>(a, st);
+  else launch_fwd_dims<32, MK, WIN>(a, st);
 }
 
-template <int MK>
+template <int MK, bool WIN = false>
 void launch_bwd_mask(const F32Args &a, hipStream_t st) {
-  if (a.p.Dqk == 128) launch_bwd_dims<128, MK>(a, st);
-  else if (a.p.Dqk == 64) launch_bwd_dims<64, MK>(a, st);
-  else launch_bwd_dims<32, MK>(a, st);
+  if (a.p.Dqk == 128) launch_bwd_dims<128, MK, WIN>(a, st);
+  else if (a.p.Dqk == 64) launch_bwd_dims<64, MK, WIN>(a, st);
+  else launch_bwd_dims<32, MK, WIN>(a, st);
 }
 
 }  // namespace
@@ -1355,7 +1396,8 @@ hipError_t launch_mfma_f32_backward(const Problem &p, View q, View k, View v, Vi
   a.scale = static_cast<float>(p.scale);
   const int mk = mfma_mask_mode(p);
   a.lse_scaled = mk >= 2;
-  if (mk == 0) launch_bwd_mask<0>(a, st);
+  if (p.window) launch_bwd_mask<0, true>(a, st);
+  else if (mk == 0) launch_bwd_mask<0>(a, st);
   else if (mk == 1) launch_bwd_mask<1>(a, st);
   else if (mk == 2) launch_bwd_mask<2>(a, st);
   else launch_bwd_mask<3>(a, st);
@@ -1380,7 +1422,8 @@ hipError_t launch_mfma_f32_forward(const Problem &p, View q, View k, View v, Vie
   a.sl = static_cast<float>(p.scale) * kLog2e;
   a.scale = static_cast<float>(p.scale);
   const int mk = mfma_mask_mode(p);
-  if (mk == 0) launch_fwd_mask<0>(a, st);
+  if (p.window) launch_fwd_mask<0, true>(a, st);
+  else if (mk == 0) launch_fwd_mask<0>(a, st);
   else if (mk == 1) launch_fwd_mask<1>(a, st);
   else if (mk == 2) launch_fwd_mask<2>(a, st);
   else launch_fwd_mask<3>(a, st);

@@ -47,6 +47,13 @@
 // (MK = 2 for an f32 mask, 3 for f16 / bf16; 4..6 the same read as 16-byte
 // row pieces when the keys are contiguous and the rows aligned).
 //
+// Windows (template WIN): a query sees its last `window` keys and the first `sinks`.
+// The workgroup's tiles are those of the sinks and, behind a gap, those from the first
+// one that its first row's window touches, in one run (WindowTiles); only the tiles at
+// either end of a wave's windows and the sinks' last one are masked element by element.
+// Rows 128 apart share their windows but for 128 keys, so 4 tiles of window / 32 + 4 are
+// partly masked.
+//
 // Key splits (template SPLIT): a problem with fewer row blocks than the chip
 // runs at once (a chunk of a prompt against a long cache, a short prompt of one
 // sequence) gives each row block to several workgroups, every one a contiguous
@@ -91,8 +98,9 @@ __device__ __forceinline__ const T *head_ptr(View v, int b, int h) {
 }
 
 // DK = head dim of q / k, DV = of v / o (each 64 or 128).
-template <typename T, int DK, int DV, int MK, bool DR, bool SPLIT>
+template <typename T, int DK, int DV, int MK, bool DR, bool SPLIT, bool WIN>
 __global__ __launch_bounds__(NT, 2) void fwd_kernel(FwdArgs a) {
+  static_assert(!WIN || (MK == 0 && !DR && !SPLIT), "windows have no general mask, no dropout and no key splits");
   static_assert(!SPLIT || (MK == 0 && !DR), "split problems have no general mask and no dropout");
   constexpr int TILE_K = BN * DK * 2, TILE_V = BN * DV * 2;  // bytes per K / V tile
   constexpr int STAGE = TILE_K + TILE_V;
@@ -150,6 +158,13 @@ __global__ __launch_bounds__(NT, 2) void fwd_kernel(FwdArgs a) {
       __builtin_amdgcn_readfirstlane(lim > 0 ? static_cast<int>((lim + BN - 1) / BN) : 0);
   int w_tiles =
       __builtin_amdgcn_readfirstlane(wlim > 0 ? static_cast<int>((wlim + BN - 1) / BN) : 0);
+  // Window: the tiles below are those of the run that the workgroup's rows see.
+  const WindowTiles run(p, q0);
+  if constexpr (WIN) {
+    n_tiles = run.count(n_tiles);
+    w_tiles = run.count(w_tiles);
+  }
+  auto phys = [&](int j) { return WIN ? run.phys(j) : j; };
   // Split: this workgroup's tiles [t0, t1) are a problem of their own whose first
   // key is k_base; everything below counts keys from there.
   int k_base = 0;
@@ -225,8 +240,8 @@ __global__ __launch_bounds__(NT, 2) void fwd_kernel(FwdArgs a) {
     d.keep = ~static_cast<uint32_t>((n_tiles - 1 - tile) >> 31);
     // a tile past the last one reads at offsets >= 2^31, past the range
     const uint32_t far = ~d.keep & 0x80000000u;
-    d.krow = (static_cast<uint32_t>(tile * BN) * ks_b) | far;
-    d.vrow = (static_cast<uint32_t>(tile * BN) * vs_b) | far;
+    d.krow = (static_cast<uint32_t>(phys(tile) * BN) * ks_b) | far;
+    d.vrow = (static_cast<uint32_t>(phys(tile) * BN) * vs_b) | far;
     d.st = (lds0 + (tile % NS) * STAGE - spare) & d.keep;
     return d;
   };
@@ -273,6 +288,10 @@ __global__ __launch_bounds__(NT, 2) void fwd_kernel(FwdArgs a) {
     const int64_t cl = static_cast<int64_t>(qrow) + p.offset + 1 - k_base;
     if (cl < kv_end) klim = cl < 0 ? 0 : static_cast<int>(cl);
   }
+  // Window: this lane's row sees keys below p.sinks and from klow on; below wlow some
+  // row of the wave may not.
+  const int klow = WIN ? window_low(p, qrow) : 0;
+  const int wlow = WIN ? __builtin_amdgcn_readfirstlane(window_low(p, last_qw)) : 0;
   const uint8_t *kmask_b =
       keymask ? static_cast<const uint8_t *>(p.mask.data) + b * p.mask.s0 + k_base * p.mask.s3 : nullptr;
   // General mask: the (b, hq) slice as a buffer; this lane reads row qrow.
@@ -397,11 +416,11 @@ __global__ __launch_bounds__(NT, 2) void fwd_kernel(FwdArgs a) {
   };
 
   auto softmax = [&](int j, int nt) {
-    const int kv0 = j * BN;
+    const int kv0 = phys(j) * BN;
     float x[16];  // scores of this lane's query row; element i is key kv0 + crow(i, h)
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = s[i];
-    if (j >= j_edge) {
+    if (phys(j) >= j_edge || (WIN && kv0 < wlow && kv0 + BN > p.sinks)) {
       // Key kv0 + 4h + kc(i), kc a compile-time constant.
       const int lim = klim - kv0 - 4 * h;
       if constexpr (MK == 0) {
@@ -414,7 +433,8 @@ __global__ __launch_bounds__(NT, 2) void fwd_kernel(FwdArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int kc = 8 * (i >> 2) + (i & 3);
-          const bool ok = (kc < lim) & (((kbits >> kc) & 1u) != 0);
+          bool ok = (kc < lim) & (((kbits >> kc) & 1u) != 0);
+          if constexpr (WIN) ok = ok & ((kc < p.sinks - kv0 - 4 * h) | (kc >= klow - kv0 - 4 * h));
           x[i] = ok ? x[i] : -INFINITY;
         }
       } else {
@@ -643,21 +663,25 @@ template <typename T, int DK, int DV, bool DR>
 void launch_dr(const FwdArgs &a, int mk, hipStream_t st) {
   const dim3 g(a.total), blk(NT);
   switch (mk) {
-    case 1: fwd_kernel<T, DK, DV, 1, DR, false><<<g, blk, 0, st>>>(a); break;
-    case 2: fwd_kernel<T, DK, DV, 2, DR, false><<<g, blk, 0, st>>>(a); break;
-    case 3: fwd_kernel<T, DK, DV, 3, DR, false><<<g, blk, 0, st>>>(a); break;
-    case 4: fwd_kernel<T, DK, DV, 4, DR, false><<<g, blk, 0, st>>>(a); break;
-    case 5: fwd_kernel<T, DK, DV, 5, DR, false><<<g, blk, 0, st>>>(a); break;
-    case 6: fwd_kernel<T, DK, DV, 6, DR, false><<<g, blk, 0, st>>>(a); break;
-    default: fwd_kernel<T, DK, DV, 0, DR, false><<<g, blk, 0, st>>>(a); break;
+    case 1: fwd_kernel<T, DK, DV, 1, DR, false, false><<<g, blk, 0, st>>>(a); break;
+    case 2: fwd_kernel<T, DK, DV, 2, DR, false, false><<<g, blk, 0, st>>>(a); break;
+    case 3: fwd_kernel<T, DK, DV, 3, DR, false, false><<<g, blk, 0, st>>>(a); break;
+    case 4: fwd_kernel<T, DK, DV, 4, DR, false, false><<<g, blk, 0, st>>>(a); break;
+    case 5: fwd_kernel<T, DK, DV, 5, DR, false, false><<<g, blk, 0, st>>>(a); break;
+    case 6: fwd_kernel<T, DK, DV, 6, DR, false, false><<<g, blk, 0, st>>>(a); break;
+    default: fwd_kernel<T, DK, DV, 0, DR, false, false><<<g, blk, 0, st>>>(a); break;
   }
 }
 
 template <typename T, int DK, int DV>
 void launch_dims(const FwdArgs &a, hipStream_t st) {
   const int mk = mfma_mask_mode_vec(a.p);
+  if (a.p.window) {
+    fwd_kernel<T, DK, DV, 0, false, false, true><<<dim3(a.total), dim3(NT), 0, st>>>(a);
+    return;
+  }
   if (a.splits > 1) {
-    fwd_kernel<T, DK, DV, 0, false, true><<<dim3(a.total * a.splits), dim3(NT), 0, st>>>(a);
+    fwd_kernel<T, DK, DV, 0, false, true, false><<<dim3(a.total * a.splits), dim3(NT), 0, st>>>(a);
     const int64_t rows = static_cast<int64_t>(a.p.B) * a.p.Hq * a.p.Sq;
     constexpr int RPB = NT / (DV / 4);
     fwd_merge_kernel<T, DV><<<dim3(static_cast<unsigned>((rows + RPB - 1) / RPB)), dim3(NT), 0, st>>>(a);
@@ -671,7 +695,7 @@ template <typename T>
 hipError_t launch(const FwdArgs &a, hipStream_t st) {
   const Problem &p = a.p;
   const int mk = mfma_mask_mode(p);
-  Probe pr_(p.drop.on ? "fwd_mfma_dropout" : (mk ? "fwd_mfma_masked" : "fwd_mfma"), st);
+  Probe pr_(p.window ? "fwd_mfma_window" : p.drop.on ? "fwd_mfma_dropout" : (mk ? "fwd_mfma_masked" : "fwd_mfma"), st);
   if (p.Dqk == 128 && p.Dv == 128) launch_dims<T, 128, 128>(a, st);
   else if (p.Dqk == 64 && p.Dv == 64) launch_dims<T, 64, 64>(a, st);
   else if (p.Dqk == 32) launch_dims<T, 32, 32>(a, st);
@@ -708,7 +732,7 @@ bool mfma_supported(const Problem &p, int dtype) {
 // 40 / 34, 1000 rows over 1600 32.5 / 35.6; 8 heads over 1024 22.6 / 21.8.  Of 956 sizes
 // none that this splits is 1.5% slower than unsplit.
 int mfma_forward_splits(const Problem &p) {
-  if (p.drop.on || mfma_mask_mode(p) != 0) return 1;
+  if (p.drop.on || mfma_mask_mode(p) != 0 || p.window) return 1;
   const int64_t total = static_cast<int64_t>((p.Sq + BM - 1) / BM) * p.Hq * p.B;
   int64_t keys = p.Sk;  // of an average row
   if (p.causal && p.Sq / 2 + p.offset < keys) keys = p.Sq / 2 + p.offset;

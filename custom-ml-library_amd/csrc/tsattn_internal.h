@@ -104,7 +104,32 @@ struct Problem {
   MaskDesc mask;
   RopeDesc rope;
   DropDesc drop;
+  // Sliding window (0: none; causal problems): query i sees key j only where j <
+  // sinks or j > i + offset - window.
+  int window, sinks;
 };
+
+// The 32-key tiles that rows from q0 on see through a window, as one run: the tiles
+// of the sinks, `ns` of them, then those from the first one the row q0's window
+// touches, `gap` tiles later.  Tile j of the run is tile phys(j) of the keys.
+struct WindowTiles {
+  int ns, gap;
+  __device__ __forceinline__ WindowTiles(const Problem &p, int q0) {
+    int64_t lo = static_cast<int64_t>(q0) + p.offset - p.window + 1;
+    lo = lo < 0 ? 0 : (lo < p.Sk ? lo : p.Sk);
+    const int first = static_cast<int>(lo) / 32, sunk = (p.sinks + 31) / 32;
+    ns = __builtin_amdgcn_readfirstlane(sunk < first ? sunk : first);
+    gap = __builtin_amdgcn_readfirstlane(first - ns);
+  }
+  // of the run, those among the keys' first n tiles
+  __device__ __forceinline__ int count(int n) const { return n > ns + gap ? n - gap : (n < ns ? n : ns); }
+  __device__ __forceinline__ int phys(int j) const { return j < ns ? j : j + gap; }
+};
+// The first key of row q's window, within [0, Sk].
+__device__ __forceinline__ int window_low(const Problem &p, int q) {
+  const int64_t lo = static_cast<int64_t>(q) + p.offset - p.window + 1;
+  return static_cast<int>(lo < 0 ? 0 : (lo < p.Sk ? lo : p.Sk));
+}
 
 // Mask handling of the MFMA kernels (a template parameter): 0 = none, or a
 // key mask [B,1,1,K] reduced to kv_len / kv_prefix; 1 = any other boolean
@@ -115,6 +140,10 @@ inline int mfma_mask_mode(const Problem &p) {
     return p.mask.s1 == 0 && p.mask.s2 == 0 && p.kv_len != nullptr ? 0 : 1;
   if (p.mask.kind != TSATTN_MASK_ADDITIVE) return 0;
   return p.mask.dtype == TSATTN_F32 ? 2 : 3;
+}
+// Whether a windowed problem's mask is none, or a key mask reduced to lengths.
+inline bool windowed_mask(const Problem &p) {
+  return p.mask.kind == TSATTN_MASK_NONE || (p.mask.kind == TSATTN_MASK_BOOL && mfma_mask_mode(p) == 0);
 }
 // Whether the MFMA kernels can read the problem's mask: not an f64 one, and a
 // general mask with 32-bit byte offsets inside each (b, h) slice, rows and
@@ -209,6 +238,12 @@ int mfma_ds_chunk_groups(const Problem &p);
 // With RoPE folded in (p.rope.R > 0) the backward workspace also holds the
 // rotated query rows [B, Hq, Sq, Dqk] (16-bit) from this byte offset on.
 size_t mfma_rope_stage_offset(const Problem &p);
+
+// With a window (p.window > 0) both passes visit the keys (query rows) that it leaves,
+// take no general mask and no dropout, and the backward recomputes S and dP; ds is then
+// mfma_window_bytes(p) bytes in which the sinks' key blocks, which every query row sees,
+// add up in parts (0: not needed).
+size_t mfma_window_bytes(const Problem &p);
 
 // fp32 MFMA kernels (mfma_f32.hip): fp32, Dqk = Dv in {32, 64, 128}, no
 // dropout / folded RoPE, any boolean mask or an additive one in f32 / f16 / bf16.

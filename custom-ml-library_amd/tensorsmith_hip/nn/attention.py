@@ -11,7 +11,8 @@ Dropout runs in the kernels on ``hip`` / ``dense`` / ``auto`` and is refused on
 Kernel routing (all on the GPU, none on the CPU):
 
 * training / prefill: ``tsattn_sdpa_forward`` + ``tsattn_sdpa_backward``
-  (MFMA kernels for f16/bf16 and head dim 64/128, generic kernels otherwise);
+  (MFMA kernels for f16/bf16 and head dim 64/128, generic kernels otherwise),
+  with a sliding window ``tsattn_window_forward`` + ``tsattn_window_backward``;
 * inference with a handful of query rows per KV head (cached decode):
   ``tsattn_decode_forward``, split across the cache.
 """
@@ -25,7 +26,7 @@ import threading
 import numpy as np
 
 from .. import _lib
-from ..device import attention_dropout_key, current_stream
+from ..device import attention_dropout_key, current_stream, launch
 from ..tensor import Tensor, is_grad_enabled
 
 BACKENDS = {"auto", "dense", "streaming", "native", "hip"}
@@ -125,6 +126,33 @@ def _forward(lib, prob, rope, vq, vk, vv, vo, lse_ptr, tdev, stream) -> None:
         None if ws is None else ctypes.c_void_p(ws.data_ptr()), nbytes, stream), "attention forward")
 
 
+def _check_window(window, sinks, is_causal: bool, span: int):
+    """The window as the kernels take it: None where it reaches past the first of ``span`` positions."""
+    whole = lambda x: isinstance(x, (int, np.integer)) and not isinstance(x, bool)  # noqa: E731
+    if not whole(sinks) or sinks < 0 or (sinks and window is None):
+        raise ValueError("sinks must be a nonnegative number of keys in front of a window")
+    if window is None:
+        return None
+    if not whole(window) or window < 1:
+        raise ValueError("window must be a positive number of keys")
+    if not is_causal:
+        raise ValueError("a window needs causal attention")
+    return None if window >= span else int(window)
+
+
+def _banded(mask, window: int, sinks: int, qlen: int, klen: int, offset: int, dev) -> Tensor:
+    """``mask`` (or none) and the window, as one mask."""
+    import torch
+
+    i = torch.arange(offset, offset + qlen, device=dev.torch)[:, None]
+    j = torch.arange(klen, device=dev.torch)
+    seen = ((j > i - window) | (j < sinks))[None, None]
+    if mask is not None:
+        raw = mask._data
+        seen = raw & seen if raw.dtype == torch.bool else torch.where(seen, raw, -math.inf)
+    return Tensor._leaf(seen, dev)
+
+
 def scaled_dot_product_attention(
     query: Tensor,
     key: Tensor,
@@ -138,6 +166,8 @@ def scaled_dot_product_attention(
     backend: str = "auto",
     block_size: int = 64,
     enable_gqa: bool = False,
+    window: int | None = None,
+    sinks: int = 0,
     _rope: tuple | None = None,
 ) -> Tensor:
     """Attention for [batch, heads, sequence, channels] tensors.
@@ -147,6 +177,13 @@ def scaled_dot_product_attention(
     absolute position of the first query in a cached key sequence.
     ``block_size`` is accepted for signature compatibility; the kernels use
     their own tiles.
+
+    ``window`` (causal attention; not in the reference signature): a query sees
+    the last ``window`` keys up to its own position, and the first ``sinks`` keys
+    of the sequence whatever its position.  The kernels visit those keys alone
+    (``tsattn_window_forward`` / ``_backward``), forward and backward; with
+    dropout, a mask other than key padding, float64 or other head dims the
+    window enters as part of the mask instead.
 
     ``_rope = (q_pos0, k_pos0, base)`` (used by ``MultiHeadAttention``, not
     part of the reference signature): query and key are *unrotated*; the
@@ -205,6 +242,7 @@ def scaled_dot_product_attention(
         raise ValueError("attention dropout currently requires the dense backend")
     if backend == "native":
         raise ValueError("native attention requires Metal and equal query/value head dimensions")
+    window = _check_window(window, sinks, is_causal, qlen + causal_offset)
 
     code = _dtype_code(query.dtype)
     q, k, v = (_operand(t._data) for t in (query, key, value))
@@ -212,7 +250,7 @@ def scaled_dot_product_attention(
 
     tdev = q.device
     prob = _problem(b, hq, hkv, qlen, klen, dim, dim_v, code, multiplier, is_causal, causal_offset)
-    if dropout_p:
+    if dropout_p and window is None:  # (else the call with the window as a mask draws it)
         # a fresh 128-bit Philox key per call from the host stream (ts.seed),
         # recorded / replayed under a checkpoint; the backward reads the keep
         # mask the forward drew from it
@@ -253,6 +291,14 @@ def scaled_dot_product_attention(
             prob.kv_prefix = lens[1].data_ptr()
             keep.append(lens)
 
+    def as_mask():  # the same attention, the window as part of the mask
+        return scaled_dot_product_attention(
+            query, key, value, _banded(attn_mask, window, sinks, qlen, klen, causal_offset, query.device), dropout_p,
+            is_causal, scale=scale, causal_offset=causal_offset, backend=backend, block_size=block_size,
+            enable_gqa=enable_gqa, _rope=_rope)
+
+    if window is not None and (dropout_p or (attn_mask is not None and not prob.kv_len)):
+        return as_mask()
     lib = _lib.load()
     stream = ctypes.c_void_p(current_stream(query.device))
     recording = is_grad_enabled() and any(t.requires_grad for t in (query, key, value))
@@ -276,6 +322,7 @@ def scaled_dot_product_attention(
 
     use_decode = (
         not recording
+        and window is None
         and not dropout_p
         and code in (_lib.F16, _lib.BF16, _lib.F32)
         and dim == dim_v
@@ -314,6 +361,14 @@ def scaled_dot_product_attention(
             prob.dropout_bits = bits.data_ptr()
             keep.append(bits)
     lse_ptr = ctypes.c_void_p(None if lse is None else lse.data_ptr())
+
+    def attend(desc):
+        if window is None:
+            _forward(lib, prob, desc, vq, vk, vv, vo, lse_ptr, tdev, stream)
+        else:
+            _lib.check(launch(query.device, lib.tsattn_window_forward, ctypes.byref(prob), window, sinks, desc, vq,
+                              vk, vv, vo, lse_ptr), "windowed attention forward")
+
     fused = False
     if rope is not None and k_pos0 is None:
         # keys given rotated: their gradient takes no inverse rotation, which the
@@ -328,19 +383,31 @@ def scaled_dot_product_attention(
             rope[0].q_rotated = q_rot.data_ptr()
             keep.append(q_rot)
         try:
-            _forward(lib, prob, ctypes.byref(rope[0]), vq, vk, vv, vo, lse_ptr, tdev, stream)
+            attend(ctypes.byref(rope[0]))
             fused = True
         except NotImplementedError:  # not an MFMA problem: rotate the queries separately
             q = _rope_rows(q, q_pos0, base, dim, False, query.device)
             vq = _view(q)
     if not fused:
-        _forward(lib, prob, None, vq, vk, vv, vo, lse_ptr, tdev, stream)
+        try:
+            attend(None)
+        except NotImplementedError:  # a window outside the kernels
+            if window is None:
+                raise
+            return as_mask()
     if not recording:
         return Tensor._from_op(out, (query, key, value), None, "sdpa_hip")
 
+    def unrotated(dq, dk):  # rotary_embedding's VJP on the rotated operands, where the kernels have not done it
+        if rope is not None and not fused:
+            dq = _rope_rows(dq, q_pos0, base, dim, True, query.device)
+            if k_pos0 is not None:
+                dk = _rope_rows(dk, k_pos0, base, dim, True, query.device)
+        return dq, dk
+
     def backward(upstream, _keep=keep):  # _keep: mask / length buffers the kernels read
         g = _operand(upstream)
-        if (fused or code in (_lib.F16, _lib.BF16)) and (not _aligned16(g) or min(g.stride()[:3]) <= 0):
+        if (fused or code in (_lib.F16, _lib.BF16) or window is not None) and (not _aligned16(g) or min(g.stride()[:3]) <= 0):
             # the MFMA kernels (the only ones the folded-RoPE backward has) need
             # 16-byte aligned rows of a real gradient: an expanded one (a sum's
             # VJP) would send the plain backward to the generic kernels
@@ -350,6 +417,13 @@ def scaled_dot_product_attention(
         dq = torch.empty(q.shape, dtype=q.dtype, device=tdev)
         dk = torch.empty(k.shape, dtype=k.dtype, device=tdev)
         dv = torch.empty(v.shape, dtype=v.dtype, device=tdev)
+        if window is not None:
+            nbytes = lib.tsattn_window_backward_workspace(ctypes.byref(prob), window, sinks, fused)
+            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=tdev)
+            _lib.check(launch(query.device, lib.tsattn_window_backward, ctypes.byref(prob), window, sinks,
+                              ctypes.byref(rope[0]) if fused else None, vq, vk, vv, vo, _view(g), lse.data_ptr(),
+                              _view(dq), _view(dk), _view(dv), ws.data_ptr(), nbytes), "windowed attention backward")
+            return unrotated(dq, dk) + (dv,)
         nbytes = (lib.tsattn_sdpa_backward_rope_workspace if fused
                   else lib.tsattn_sdpa_backward_workspace)(ctypes.byref(prob))
         try:
@@ -368,11 +442,7 @@ def scaled_dot_product_attention(
                        "attention backward")
             return dq, dk, dv
         _lib.check(lib.tsattn_sdpa_backward(ctypes.byref(prob), *args), "attention backward")
-        if rope is not None:  # rotary_embedding's VJP on the rotated operands
-            dq = _rope_rows(dq, q_pos0, base, dim, True, query.device)
-            if k_pos0 is not None:
-                dk = _rope_rows(dk, k_pos0, base, dim, True, query.device)
-        return dq, dk, dv
+        return unrotated(dq, dk) + (dv,)
 
     return Tensor._from_op(out, (query, key, value), backward, "sdpa_hip")
 

@@ -35,7 +35,7 @@ from .. import device as _device
 from ..device import launch
 from ..tensor import Tensor, cat, is_grad_enabled, no_grad
 from . import functional as F
-from .attention import (BACKENDS, DECODE_MIN_KEYS, _dtype_code, _view, decode_int8_cache, rope_tables,
+from .attention import (BACKENDS, DECODE_MIN_KEYS, _check_window, _dtype_code, _view, decode_int8_cache, rope_tables,
                         rotary_embedding, scaled_dot_product_attention)
 from .cache import KVCache
 from .checkpoint import checkpoint
@@ -73,7 +73,7 @@ def _cached_step(x: Tensor, attention, cache, is_causal: bool = True, block=None
 
     raw = x._data
     if (raw.dtype not in (torch.float16, torch.bfloat16) or type(cache) is not KVCache
-            or cache.dtype != raw.dtype or attention.backend == "native"):
+            or cache.dtype != raw.dtype or attention.backend == "native" or attention.window is not None):
         return None
     b, t, e = raw.shape
     pos, stop = cache.length, cache.length + t
@@ -157,12 +157,17 @@ def _cached_step(x: Tensor, attention, cache, is_causal: bool = True, block=None
 
 
 class MultiHeadAttention(Module):
-    """Self/cross attention with optional grouped-query heads and rotary positions."""
+    """Self/cross attention with optional grouped-query heads and rotary positions.
+
+    ``window``, ``sinks``: causal attention to the last ``window`` positions and the
+    first ``sinks`` (``scaled_dot_product_attention``)."""
 
     def __init__(self, embed_dim: int, num_heads: int, *, num_kv_heads: int | None = None,
                  dropout: float = 0.0, bias: bool = False, rotary: bool = True,
-                 backend: str = "auto", device=None):
+                 backend: str = "auto", window: int | None = None, sinks: int = 0, device=None):
         super().__init__()
+        _check_window(window, sinks, True, 0)
+        self.window, self.sinks = window, sinks
         kv_heads = num_heads if num_kv_heads is None else num_kv_heads
         if min(embed_dim, num_heads, kv_heads) <= 0 or embed_dim % num_heads or num_heads % kv_heads:
             raise ValueError(
@@ -230,13 +235,13 @@ class MultiHeadAttention(Module):
         if q_fused is not None:
             q = Tensor._from_op(q_fused, (input,), None, "qkv_rope_append")
             attended = None
-            if cache.quantized and attn_mask is None:
+            if cache.quantized and attn_mask is None and self.window is None:
                 attended = decode_int8_cache(q, cache, is_causal=is_causal, causal_offset=offset)
             if attended is None:
                 k, v = cache.get()
                 attended = scaled_dot_product_attention(
                     q, k, v, attn_mask, 0.0, is_causal, causal_offset=offset, backend=self.backend,
-                    enable_gqa=self.num_kv_heads != self.num_heads)
+                    enable_gqa=self.num_kv_heads != self.num_heads, window=self.window, sinks=self.sinks)
             return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
         q = self.q_proj(input).reshape(batch, steps, self.num_heads, self.head_dim).permute(0, 2, 1, 3)
         k = (self.k_proj(source).reshape(batch, source.shape[1], self.num_kv_heads, self.head_dim)
@@ -265,7 +270,7 @@ class MultiHeadAttention(Module):
         if cache is not None:
             if not fused:
                 cache._append(k, v)
-            if cache.quantized and attn_mask is None:
+            if cache.quantized and attn_mask is None and self.window is None:
                 # decode straight over the int8 storage (dequantised in the kernel)
                 attended = decode_int8_cache(q, cache, is_causal=is_causal, causal_offset=offset,
                                              rope=rope and (offset, 10000.0))
@@ -275,23 +280,25 @@ class MultiHeadAttention(Module):
             attended = scaled_dot_product_attention(
                 q, k, v, attn_mask, self.dropout_p if self.training else 0.0, is_causal,
                 causal_offset=offset, backend=self.backend,
-                enable_gqa=self.num_kv_heads != self.num_heads, _rope=rope)
+                enable_gqa=self.num_kv_heads != self.num_heads, window=self.window, sinks=self.sinks,
+                _rope=rope)
         return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
 
 
     def _paged(self, input: Tensor, cache: PagedKVCache, attn_mask, is_causal: bool) -> Tensor:
         """Self-attention over a paged 4-bit cache, each row at its own position.  As over an int8 cache,
-        ``backend`` chooses only where a mask has the values read back as arrays."""
+        ``backend`` chooses only where a mask or a window has the values read back as arrays."""
         batch, steps, _ = input.shape
         lens = cache.lengths
-        if attn_mask is not None and min(lens) != max(lens):
-            raise ValueError("attention masks over a paged cache need rows of one length")
+        read_back = attn_mask is not None or self.window is not None
+        if read_back and min(lens) != max(lens):
+            raise ValueError("attention masks and windows over a paged cache need rows of one length")
         q, k, v = (proj(input).reshape(batch, steps, heads, self.head_dim).permute(0, 2, 1, 3)
                    for proj, heads in ((self.q_proj, self.num_heads), (self.k_proj, self.num_kv_heads),
                                        (self.v_proj, self.num_kv_heads)))
         base = 10000.0 if self.rotary else None
         cache.append(k, v, rotary_base=base)
-        if attn_mask is None:
+        if not read_back:
             attended = paged_attention(q, cache, is_causal=is_causal, rotary_base=base)
         else:
             if self.rotary:
@@ -299,7 +306,7 @@ class MultiHeadAttention(Module):
             k, v = cache.get()
             attended = scaled_dot_product_attention(
                 q, k, v, attn_mask, 0.0, is_causal, causal_offset=lens[0], backend=self.backend,
-                enable_gqa=self.num_kv_heads != self.num_heads)
+                enable_gqa=self.num_kv_heads != self.num_heads, window=self.window, sinks=self.sinks)
         return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
 
 
@@ -336,11 +343,13 @@ class TransformerDecoderBlock(Module):
     """Pre-RMSNorm decoder block with GQA/RoPE attention and a SwiGLU MLP."""
 
     def __init__(self, dim: int, num_heads: int, hidden_dim: int | None = None, *,
-                 num_kv_heads=None, dropout=0.0, attention_backend="auto", device=None):
+                 num_kv_heads=None, dropout=0.0, attention_backend="auto", attention_window=None,
+                 attention_sinks=0, device=None):
         super().__init__()
         self.attention_norm = RMSNorm(dim, device=device)
         self.attention = MultiHeadAttention(dim, num_heads, num_kv_heads=num_kv_heads,
                                             dropout=dropout, backend=attention_backend,
+                                            window=attention_window, sinks=attention_sinks,
                                             device=device)
         self.residual_dropout = Dropout(dropout)
         self.ffn_norm = RMSNorm(dim, device=device)
@@ -374,6 +383,8 @@ class TransformerConfig:
     tie_weights: bool = True
     attention_backend: str = "auto"
     activation_checkpointing: bool = False
+    attention_window: int | None = None  # every block's attention: the last positions, and
+    attention_sinks: int = 0             # the first ones that stay visible
 
     def __post_init__(self):
         if min(self.vocab_size, self.dim, self.num_heads, self.num_layers, self.max_seq_len) <= 0:
@@ -388,6 +399,7 @@ class TransformerConfig:
             raise ValueError("dropout must be in [0, 1)")
         if self.attention_backend not in BACKENDS:
             raise ValueError("invalid attention backend")
+        _check_window(self.attention_window, self.attention_sinks, True, 0)
 
 
 class TransformerLM(Module):
@@ -406,7 +418,9 @@ class TransformerLM(Module):
         self.blocks = [
             TransformerDecoderBlock(config.dim, config.num_heads, config.hidden_dim,
                                     num_kv_heads=config.num_kv_heads, dropout=config.dropout,
-                                    attention_backend=config.attention_backend, device=device)
+                                    attention_backend=config.attention_backend,
+                                    attention_window=config.attention_window,
+                                    attention_sinks=config.attention_sinks, device=device)
             for _ in range(config.num_layers)
         ]
         self.final_norm = RMSNorm(config.dim, device=device)

@@ -241,6 +241,28 @@ int tsattn_sdpa_backward_rope(const tsattn_problem *p, const tsattn_rope_desc *r
                               void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * Attention through a sliding window (no counterpart in the reference, where it is a
+ * mask of every pair: src/tensorsmith/nn/attention.py:102-113): query i, at position i +
+ * causal_offset, sees key j only where j is one of the last `window` keys up to its own,
+ * or one of the first `sinks`.  The kernels visit the tiles that hold such pairs alone.
+ * rope may be NULL.  Causal problems (others: TSATTN_ERR_INVALID) of the MFMA kernels,
+ * without dropout and with no mask but key padding (p->kv_len); f32 without rope.
+ * Others: TSATTN_ERR_UNSUPPORTED, nothing launched.
+ */
+int tsattn_window_forward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
+                          const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
+                          void *lse, void *stream);
+
+/* Bytes of scratch tsattn_window_backward needs (rope: whether it is given one). */
+size_t tsattn_window_backward_workspace(const tsattn_problem *p, int64_t window, int32_t sinks, int32_t rope);
+
+/* Its VJP, as tsattn_sdpa_backward(_rope); deterministic. */
+int tsattn_window_backward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
+                           const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
+                           const tsattn_view *dout, const void *lse, const tsattn_view *dq, const tsattn_view *dk,
+                           const tsattn_view *dv, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * The keep mask the attention kernels draw for problem `p` (its dropout
  * fields and sizes): out[b, h, i, j] = 1 if kept, else 0, as a contiguous
  * [B, Hq, Sq, Sk] uint8 array.  The reference's dense backend holds this mask
