@@ -435,6 +435,41 @@ int check_rows(int32_t dtype, int32_t rows, int32_t k, int32_t n, int64_t xs, in
   return TSATTN_OK;
 }
 
+// New tokens' attention over a cache.
+int check_cached(const tsattn_cached *d, tsattn::CachedProblem *p) {
+  if (!d) return fail(TSATTN_ERR_INVALID, "cached attention descriptor is NULL");
+  if (!is_float_dtype(d->dtype))
+    return fail(TSATTN_ERR_INVALID, "attention inputs must have the same floating-point dtype");
+  if (d->batch <= 0 || d->heads_q <= 0 || d->heads_kv <= 0 || d->dim <= 0 || d->len <= 0 || d->keys < d->len)
+    return fail(TSATTN_ERR_INVALID, "cached attention needs positive sizes and the new tokens in the cache");
+  if (d->heads_q % d->heads_kv)
+    return fail(TSATTN_ERR_INVALID,
+                "grouped-query attention requires enable_gqa and query heads divisible by KV heads");
+  if (!isfinite(d->scale)) return fail(TSATTN_ERR_INVALID, "attention scale must be finite");
+  if (d->window < 0 || d->sinks < 0 || (d->sinks && !d->window))
+    return fail(TSATTN_ERR_INVALID, "sinks must be a nonnegative number of keys in front of a window");
+  if (!d->words != !d->depths || (d->words && d->trees != 1 && d->trees != d->batch))
+    return fail(TSATTN_ERR_INVALID, "a tree has words and depths, one for all sequences or one for each");
+  if (d->words && d->window && d->window < d->len)
+    return fail(TSATTN_ERR_INVALID, "the window must hold the drafted tokens");
+  if (!d->cos != !d->sin) return fail(TSATTN_ERR_INVALID, "RoPE needs cos / sin tables");
+  tsattn::CachedProblem c{};
+  c.dtype = d->dtype, c.B = d->batch, c.Hq = d->heads_q, c.Hkv = d->heads_kv, c.T = d->len, c.n = d->keys;
+  c.D = d->dim, c.q8 = d->quantized != 0, c.scale = d->scale;
+  c.window = static_cast<int>(d->window < (1 << 30) ? d->window : 1 << 30);
+  c.sinks = d->sinks < d->keys ? d->sinks : d->keys;
+  if (d->words) c.words = d->words, c.depth = d->depths, c.tree_rows = d->trees;
+  if (d->cos) c.rope = tsattn::RopeDesc{d->cos, d->sin, d->dim, 0, 0, nullptr};
+  // (a rotary table's rows are read 8 bytes at a time)
+  if (!tsattn::cached_supported(c) || d->len > 256 || !(d->scale > 0.0) || d->keys > (1 << 30) ||
+      reinterpret_cast<uintptr_t>(d->cos) % 8 || reinterpret_cast<uintptr_t>(d->sin) % 8)
+    return fail(TSATTN_ERR_UNSUPPORTED,
+                "cached attention takes up to 256 tokens, f16 / bf16 and int8 caches of 32, 64, 128 or 256 channels, "
+                "f32 ones of 32, 64 or 128, a positive scale and 8-byte aligned RoPE tables");
+  *p = c;
+  return TSATTN_OK;
+}
+
 // Operands of the token probabilities: a workgroup each row (or part of one), 32-bit element offsets in a row.
 int check_probs(int32_t dtype, int64_t rows, int32_t vocab, const void *logits, int64_t row_stride,
                 const void *tokens, int32_t token_bytes, int32_t top) {
@@ -566,7 +601,7 @@ int run_step(const tsattn_step_desc &d, const StepPlan &s, char *ws, hipStream_t
     vq = tsattn::View{q, L * N, D, N};
     const tsattn::View nk{q + W * 2, L * N, D, N}, nv{q + (W + kvw) * 2, L * N, D, N};
     rc = hip_status(tsattn::launch_rope_append(d.dtype, d.batch, d.heads_kv, L, D, d.cos ? D : 0, nk, nv, vk, vv,
-                                               &vks, &vvs, d.cos, d.sin, d.pos, st),
+                                               &vks, &vvs, d.cos, d.sin, d.pos, nullptr, 0, st),
                     "step append launch");
     if (rc) return rc;
   }
@@ -943,11 +978,11 @@ int tsattn_rope(int32_t dtype, int32_t batch, int32_t heads, int32_t len, int32_
                     "RoPE launch");
 }
 
-int tsattn_rope_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len, int32_t dim,
-                       int32_t rotary_dim, const tsattn_view *k, const tsattn_view *v,
-                       const tsattn_view *k_cache, const tsattn_view *v_cache,
-                       const tsattn_view *k_scale, const tsattn_view *v_scale, const void *cos,
-                       const void *sin, int64_t pos, void *stream) {
+static int rope_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len, int32_t dim, int32_t rotary_dim,
+                       const tsattn_view *k, const tsattn_view *v, const tsattn_view *k_cache,
+                       const tsattn_view *v_cache, const tsattn_view *k_scale, const tsattn_view *v_scale,
+                       const void *cos, const void *sin, int64_t pos, const int32_t *depth, int32_t trees,
+                       void *stream) {
   int rc;
   if ((rc = check_view(k, "key rows")) || (rc = check_view(v, "value rows")) ||
       (rc = check_view(k_cache, "key cache")) || (rc = check_view(v_cache, "value cache")))
@@ -970,8 +1005,100 @@ int tsattn_rope_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len,
                                                tsattn::make_view(k), tsattn::make_view(v),
                                                tsattn::make_view(k_cache), tsattn::make_view(v_cache),
                                                k_scale ? &ks : nullptr, v_scale ? &vs : nullptr,
-                                               cos, sin, pos, static_cast<hipStream_t>(stream)),
+                                               cos, sin, pos, depth, trees, static_cast<hipStream_t>(stream)),
                     "RoPE append launch");
+}
+
+int tsattn_rope_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len, int32_t dim,
+                       int32_t rotary_dim, const tsattn_view *k, const tsattn_view *v,
+                       const tsattn_view *k_cache, const tsattn_view *v_cache,
+                       const tsattn_view *k_scale, const tsattn_view *v_scale, const void *cos,
+                       const void *sin, int64_t pos, void *stream) {
+  return rope_append(dtype, batch, heads, len, dim, rotary_dim, k, v, k_cache, v_cache, k_scale, v_scale, cos, sin,
+                     pos, nullptr, 0, stream);
+}
+
+int tsattn_draft_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len, int32_t dim, const tsattn_view *k,
+                        const tsattn_view *v, const tsattn_view *k_cache, const tsattn_view *v_cache,
+                        const tsattn_view *k_scale, const tsattn_view *v_scale, const void *cos, const void *sin,
+                        int64_t pos, const int32_t *depths, int32_t trees, void *stream) {
+  if (!depths) return fail(TSATTN_ERR_INVALID, "the drafted tokens' depths are NULL");
+  if (trees != 1 && trees != batch) return fail(TSATTN_ERR_INVALID, "one tree, or one for each sequence");
+  if (len > 256) return fail(TSATTN_ERR_UNSUPPORTED, "a tree has at most 256 tokens (got %d)", len);
+  if (!cos != !sin) return fail(TSATTN_ERR_INVALID, "RoPE needs cos / sin tables");
+  return rope_append(dtype, batch, heads, len, dim, cos ? dim : 0, k, v, k_cache, v_cache, k_scale, v_scale, cos,
+                     sin, pos, depths, trees, stream);
+}
+
+int tsattn_draft_tree(int32_t trees, int32_t len, const int32_t *parents, uint32_t *words, int32_t *depths,
+                      void *stream) {
+  if (trees <= 0 || len <= 0) return fail(TSATTN_ERR_INVALID, "a tree needs at least one token");
+  if (len > 256) return fail(TSATTN_ERR_UNSUPPORTED, "a tree has at most 256 tokens (got %d)", len);
+  if (!parents || !words || !depths) return fail(TSATTN_ERR_INVALID, "data pointer is NULL");
+  return hip_status(tsattn::launch_draft_tree(trees, len, parents, words, depths, static_cast<hipStream_t>(stream)),
+                    "draft tree launch");
+}
+
+int tsattn_cache_keep(int32_t batch, int32_t heads, int32_t n, int64_t first, int64_t limit, const void *index,
+                      int32_t index_bytes, int32_t key_bytes, int32_t value_bytes, const tsattn_view *k,
+                      const tsattn_view *v, const tsattn_view *k_scale, const tsattn_view *v_scale, void *stream) {
+  int rc;
+  if (batch <= 0 || heads <= 0 || n <= 0 || first < 0 || limit < n || key_bytes <= 0 || value_bytes <= 0)
+    return fail(TSATTN_ERR_INVALID, "kept rows need positive sizes, no more of them than there are");
+  if (n > 256) return fail(TSATTN_ERR_UNSUPPORTED, "at most 256 rows are kept (got %d)", n);
+  if (!index || (index_bytes != 4 && index_bytes != 8)) return fail(TSATTN_ERR_INVALID, "indexes are int32 or int64");
+  if ((rc = check_view(k, "key cache")) || (rc = check_view(v, "value cache"))) return rc;
+  if (!k_scale != !v_scale)
+    return fail(TSATTN_ERR_INVALID, "an int8 cache needs both key and value scales");
+  if (k_scale && ((rc = check_view(k_scale, "key scales")) || (rc = check_view(v_scale, "value scales")))) return rc;
+  tsattn::KeepArgs a{};
+  const tsattn_view *views[4] = {k, v, k_scale, v_scale};
+  for (int i = 0; i < 4; ++i) {
+    if (!views[i]) continue;
+    a.data[i] = static_cast<char *>(views[i]->data);
+    const int64_t unit = i < 2 ? 1 : static_cast<int64_t>(sizeof(float));
+    a.s0[i] = views[i]->stride[0] * unit, a.s1[i] = views[i]->stride[1] * unit, a.s2[i] = views[i]->stride[2] * unit;
+    a.bytes[i] = i == 0 ? key_bytes : i == 1 ? value_bytes : static_cast<int>(sizeof(float));
+  }
+  a.B = batch, a.H = heads, a.n = n, a.first = first, a.limit = limit, a.index = index, a.index_bytes = index_bytes;
+  return hip_status(tsattn::launch_keep(a, static_cast<hipStream_t>(stream)), "cache rows launch");
+}
+
+size_t tsattn_cached_attend_workspace(const tsattn_cached *d) {
+  tsattn::CachedProblem p;
+  return check_cached(d, &p) ? 0 : tsattn::cached_workspace_bytes(p);
+}
+
+int tsattn_cached_attend(const tsattn_cached *d, const tsattn_view *q, const tsattn_view *k, const tsattn_view *v,
+                         const tsattn_view *k_scale, const tsattn_view *v_scale, const tsattn_view *out,
+                         void *workspace, size_t workspace_bytes, void *stream) {
+  tsattn::CachedProblem p;
+  int rc = check_cached(d, &p);
+  if (rc) return rc;
+  if ((rc = check_view(q, "query")) || (rc = check_view(k, "key")) || (rc = check_view(v, "value")) ||
+      (rc = check_view(out, "output")))
+    return rc;
+  if (p.q8 && ((rc = check_view(k_scale, "key scale")) || (rc = check_view(v_scale, "value scale")))) return rc;
+  const tsattn::View vq = tsattn::make_view(q), vk = tsattn::make_view(k), vv = tsattn::make_view(v),
+                     vo = tsattn::make_view(out);
+  // 16-byte rows; a (sequence, head)'s rows within 2^31 bytes
+  const int es = p.dtype == TSATTN_F32 ? 4 : 2, ce = p.q8 ? 1 : es;
+  auto rows16 = [](const tsattn::View &x, int e) {
+    return reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && x.s0 * e % 16 == 0 && x.s1 * e % 16 == 0 && x.s2 * e % 16 == 0;
+  };
+  for (const tsattn::View *x : {&vk, &vv})
+    if (!rows16(*x, ce) || x->s2 <= 0 || (static_cast<int64_t>(p.n) + 64) * x->s2 * ce >= (int64_t(1) << 31))
+      return fail(TSATTN_ERR_UNSUPPORTED, "cached attention needs 16-byte aligned cache rows, a head's below 2^31 bytes");
+  if (!rows16(vq, es) || !rows16(vo, es))
+    return fail(TSATTN_ERR_UNSUPPORTED, "cached attention needs 16-byte aligned query and output rows");
+  const size_t need = tsattn::cached_workspace_bytes(p);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(TSATTN_ERR_INVALID, "cached attention needs %zu bytes of 16-byte aligned workspace", need);
+  tsattn::View ks{}, vs{};
+  if (p.q8) ks = tsattn::make_view(k_scale), vs = tsattn::make_view(v_scale);
+  return hip_status(tsattn::launch_cached(p, vq, vk, vv, ks, vs, vo, static_cast<float *>(workspace),
+                                          static_cast<hipStream_t>(stream)),
+                    "cached attention launch");
 }
 
 int tsattn_qkv_rope_append(int32_t dtype, int32_t batch, int32_t len, int32_t embed, int32_t heads_q,

@@ -1,0 +1,703 @@
+// Attention of a few new tokens over a key/value cache that they do not all see alike: a
+// sliding window with sinks, or a tree of drafted tokens.  f16, bf16, int8 (codes with a
+// scale a row) and f32 caches.
+//
+// Token t's position is P + its depth, P the positions in front of the new ones (a chain:
+// depth t).  It sees key j < P where j < sinks or j > position - window, and of the new
+// keys those up to its own (chain) or its ancestors' and its own (tree, a bit each).  Which
+// of 32 keys a row sees is one word, made of three comparisons and the tree's bits; only
+// tiles at the window's border, the sinks' last and the new ones need it.
+//
+// The rows of a KV head (its query heads times the tokens) are the columns of S^T = K Q^T,
+// 32 to a wave, so that the statistics of a row are a lane's own and P^T is the operand of
+// O^T += V^T P^T as it comes.  Cached keys and values are read once for up to 128 rows.
+// Up to 32 rows: every wave works alone on tiles of its own through its own LDS ring and
+// the waves' results are joined at the end; more: 2 or 4 waves of 32 rows share each tile.
+// The tiles that a window leaves lie in one run, which splits cut into equal parts, as
+// many as fill the chip; a second kernel joins those.
+//
+// Bound by HBM for few rows (keys and values once), by the softmax beside the matrix
+// instructions from about 100 rows a KV head on.
+//
+// P is rounded to the cache's type for the second product, as in the prefill kernel; f32
+// keeps it.  Over int8 caches the codes are exact in 16 bits, keys' scales multiply the
+// scores, values' scales P, which then may be small and so is rounded to bf16, for f16
+// queries as the sum of two.
+#include <type_traits>
+
+#include "f32_tile.h"
+#include "rope_math.h"
+
+namespace tsattn {
+namespace {
+
+constexpr int BN = 32;  // keys per tile
+constexpr float kTau = 8.f;
+
+struct CachedArgs {
+  int B, Hkv, rep, T, n, R;  // R = rep T rows a KV head
+  View q, k, v, o, ks, vs;
+  const uint32_t *words;
+  const int32_t *depth;
+  int tree_rows, W;
+  int window, sinks;
+  int ns, gap, run;  // the tiles in use: ns of the sinks, then those `gap` further on
+  int splits, groups;
+  float sl;  // scale * log2(e)
+  RopeDesc rope;
+  float *ws;  // partial O [splits][B Hkv R][D], then [splits][B Hkv R][2] (max, sum)
+};
+
+template <typename T, int D>
+constexpr int kPair = 2 * BN * D * (std::is_same_v<T, float> ? 4 : 2);  // bytes of a K and a V tile
+// Waves of a workgroup, WR of them sharing each tile; up to 32 rows (WR 1) as many as 64
+// KiB of tiles allow, two workgroups a CU.
+template <typename T, int D, int WR>
+constexpr int kWaves = WR > 1 ? WR : (kPair<T, D> <= 8192 ? 4 : 2);
+// Ring stages: WR > 1 and DMA: three.
+template <bool Q8, int WR>
+constexpr int kStages = WR > 1 && !Q8 ? 3 : 2;
+
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
+// Eight int8 codes as eight values of T (exact).
+template <typename T>
+__device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (i < 2 ? lo : hi) >> (16 * (i & 1));
+    y[i] = pack2<T>(static_cast<float>(static_cast<int8_t>(w & 0xFFu)),
+                    static_cast<float>(static_cast<int8_t>((w >> 8) & 0xFFu)));
+  }
+  return y;
+}
+
+template <typename T, int D, bool Q8, int WR>
+__global__ __launch_bounds__((64 * kWaves<T, D, WR>)) void cached_kernel(CachedArgs a) {
+  constexpr bool F32 = std::is_same_v<T, float>;
+  static_assert(!F32 || (!Q8 && D <= 128), "fp32 caches are not quantised, of up to 128 channels");
+  using PT = std::conditional_t<Q8, bf16, T>;  // the value tiles
+  constexpr int NP = Q8 && std::is_same_v<T, f16> ? 2 : 1;  // parts of P
+  constexpr int NWV = kWaves<T, D, WR>, WK = NWV / WR, NS = kStages<Q8, WR>;
+  constexpr int PAIR = kPair<T, D>, TILE = PAIR / 2;
+  constexpr int BLK = TILE / 1024;             // 1 KiB DMA blocks a tile
+  constexpr int LPT = (2 * BLK + WR - 1) / WR;  // DMA loads a wave issues for a pair (WR > 1)
+  constexpr int QG = D / 32, PDT = D / 32;
+  constexpr int SCALES = Q8 ? 256 : 0;
+  constexpr int STAGE = PAIR + SCALES, RING = NS * STAGE;
+  constexpr int MERGE = WK > 1 ? NWV * 32 * (D + 2) * 4 : 0;
+  constexpr int LDS_B = WK * RING > MERGE ? WK * RING : MERGE;
+  static_assert(WR == 1 || (2 * BLK) % WR == 0 || Q8, "a pair's blocks split over the waves");
+  __shared__ __attribute__((aligned(1024))) char lds[LDS_B];
+
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = WR > 1 ? w : 0, wk = WR > 1 ? 0 : w;
+  // row groups of the same keys follow each other, on one XCD
+  const int bhs = a.B * a.Hkv;
+  const int logical = xcd_remap(blockIdx.x, bhs * a.splits * a.groups);
+  const int rg = logical % a.groups, part = logical / a.groups % a.splits, bh = logical / (a.groups * a.splits);
+  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int t0 = static_cast<int>(static_cast<int64_t>(a.run) * part / a.splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(a.run) * (part + 1) / a.splits);
+  const int mine = t1 - t0 > wk ? (t1 - t0 - wk - 1) / WK + 1 : 0;  // this wave's tiles
+  auto key0 = [&](int i) __attribute__((always_inline)) {  // the first key of its tile i
+    const int j = t0 + wk + WK * i;
+    return BN * (j < a.ns ? j : j + a.gap);
+  };
+
+  // this lane's row
+  const int row = (rg * WR + wr) * 32 + c;
+  const bool live = row < a.R;
+  const int rr = live ? row / a.T : 0, t = live ? row - rr * a.T : 0;
+  const int64_t tree = static_cast<int64_t>(a.tree_rows > 1 ? b : 0) * a.T + t;
+  const int P = a.n - a.T;
+  const int pos = P + (a.words ? a.depth[tree] : t);
+  const uint32_t *words = a.words ? a.words + tree * a.W : nullptr;
+  const int low = a.window ? pos - a.window + 1 : 0;
+  // Which of the 32 keys from kv0 on the row sees.
+  auto visible = [&](int kv0) {
+    uint32_t seen = low_bits(a.sinks - kv0) | ~low_bits(low - kv0);
+    const int off = kv0 - P;
+    if (off > -BN) {
+      uint32_t x;
+      if (!words) {
+        x = low_bits(t + 1 - off);
+      } else if (off < 0) {
+        x = (words[0] << -off) | low_bits(-off);
+      } else {
+        const int i = off >> 5, sh = off & 31;
+        x = i < a.W ? words[i] >> sh : 0u;
+        if (sh && i + 1 < a.W) x |= words[i + 1] << (32 - sh);
+      }
+      seen &= x;
+    }
+    return seen;
+  };
+  // keys below `border` are hidden from some row
+  const int border = a.window ? a.n - a.window : 0;
+
+  // Q rows as B operands: 16-bit, channels 16 ks + 8 h .. + 7; f32, the half h of the row
+  constexpr int NQ = F32 ? D / 8 : D / 16;  // 16-byte pieces a lane holds
+  u32x4 qf[NQ];
+  {
+    const T *qp = static_cast<const T *>(a.q.data) + b * a.q.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.q.s1 +
+                  static_cast<int64_t>(t) * a.q.s2 + (F32 ? h * (D / 2) : 8 * h);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) qf[i] = ld16(qp + (F32 ? 4 : 16) * i);
+    if (a.rope.R > 0) {
+      if constexpr (F32) {
+        const float *cs = static_cast<const float *>(a.rope.cos) + static_cast<int64_t>(pos) * (D / 2) + h * (D / 4);
+        const float *sn = static_cast<const float *>(a.rope.sin) + static_cast<int64_t>(pos) * (D / 2) + h * (D / 4);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t b0 = qf[i][2 * e], b1 = qf[i][2 * e + 1];
+            float x0 = __builtin_bit_cast(float, b0), x1 = __builtin_bit_cast(float, b1);
+            rotate_pair(x0, x1, cs[2 * i + e], sn[2 * i + e], false);
+            qf[i][2 * e] = __builtin_bit_cast(uint32_t, x0), qf[i][2 * e + 1] = __builtin_bit_cast(uint32_t, x1);
+          }
+      } else {
+        int64_t at[NQ];
+        int p0[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) at[i] = pos, p0[i] = 8 * i + 4 * h;
+        rotate_chunks<T, NQ>(qf, a.rope, at, p0, false);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      if (!live) qf[i] = u32x4{0, 0, 0, 0};
+      asm volatile("" : "+v"(qf[i]));  // loaded before the DMA stream starts
+    }
+  }
+
+  f32x16 oacc[PDT];
+#pragma unroll
+  for (int dt = 0; dt < PDT; ++dt) oacc[dt] = f32x16{};
+  float m = -INFINITY, l = 0.f, thr = -INFINITY, nbase = 0.f;
+  const float sl = a.sl, inv_sl = 1.f / sl;
+  char *ring = lds + wk * RING;
+  const uint32_t ring0 = lds_addr(lds) + wk * RING;
+
+  using Reader = std::conditional_t<F32, TileReader<bf16, 32>, TileReader<std::conditional_t<F32, bf16, T>, D>>;
+  const Reader rd(lane);
+  // S^T of a K tile: element i is key crow(i, h)
+  auto scores = [&](const char *kt) __attribute__((always_inline)) {
+    f32x16 s = f32x16{};
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const float4 x = FTile<D>::chunk(kt, c, h * NQ + i);
+        const uint32_t q0 = qf[i][0], q1 = qf[i][1], q2 = qf[i][2], q3 = qf[i][3];
+        s = mfma32f(x.x, __builtin_bit_cast(float, q0), s);
+        s = mfma32f(x.y, __builtin_bit_cast(float, q1), s);
+        s = mfma32f(x.z, __builtin_bit_cast(float, q2), s);
+        s = mfma32f(x.w, __builtin_bit_cast(float, q3), s);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) s = mfma32<T>(rd.rows(kt, 0, i), qf[i], s);
+    }
+    return s;
+  };
+  float p[16];                  // P of the tile (f32 caches)
+  u32x4 pb[NP][F32 ? 1 : 2];    // or its packed parts
+  // The softmax of the tile from kv0 on; scales: its keys' (Q8), then its values'.
+  auto softmax = [&](f32x16 s, int kv0, const float *scales) __attribute__((always_inline)) {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = s[i];
+    if constexpr (Q8) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 f = *reinterpret_cast<const float4 *>(scales + 8 * g + 4 * h);
+        x[4 * g] *= f.x, x[4 * g + 1] *= f.y, x[4 * g + 2] *= f.z, x[4 * g + 3] *= f.w;
+      }
+    }
+    if (kv0 + BN > P || (kv0 < border && kv0 + BN > a.sinks)) {
+      const uint32_t seen = visible(kv0) >> (4 * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = (seen >> (8 * (i >> 2) + (i & 3))) & 1u ? x[i] : -INFINITY;
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+    const float mxr = half_swap_max3(mx);
+    if (__ballot(mxr > thr) != 0ull) {
+      const float m_new = fmaxf(m, mxr * sl);
+      const float corr = m_new == -INFINITY ? 1.f : fast_exp2(m - m_new);
+      m = m_new;
+      thr = (m + kTau) * inv_sl;
+      nbase = m == -INFINITY ? 0.f : -m;
+      l *= corr;
+#pragma unroll
+      for (int dt = 0; dt < PDT; ++dt) oacc[dt] *= corr;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = fast_exp2(fmaf(x[i], sl, nbase));
+      l += p[i];
+    }
+    if constexpr (Q8) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 f = *reinterpret_cast<const float4 *>(scales + 32 + 8 * g + 4 * h);
+        p[4 * g] *= f.x, p[4 * g + 1] *= f.y, p[4 * g + 2] *= f.z, p[4 * g + 3] *= f.w;
+      }
+    }
+    if constexpr (!F32) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t hi = pack2<PT>(p[i], p[i + 1]);
+        pb[0][i >> 3][(i & 7) >> 1] = hi;
+        if constexpr (NP > 1) {  // (bf16) what the first part leaves
+          const uint32_t h0 = hi << 16, h1 = hi & 0xFFFF0000u;
+          pb[1][i >> 3][(i & 7) >> 1] =
+              pack2<PT>(p[i] - __builtin_bit_cast(float, h0), p[i + 1] - __builtin_bit_cast(float, h1));
+        }
+      }
+    }
+  };
+  auto values = [&](const char *vt) __attribute__((always_inline)) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int dt = 0; dt < PDT; ++dt)
+          oacc[dt] = mfma32f(FTile<D>::elem(vt, 8 * (i >> 2) + 4 * h + (i & 3), 32 * dt + c), p[i], oacc[dt]);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int dt = 0; dt < PDT; ++dt) {
+          const u32x4 f = rd.cols(vt, ks, dt);
+#pragma unroll
+          for (int n = 0; n < NP; ++n) oacc[dt] = mfma32<PT>(f, pb[n][ks], oacc[dt]);
+        }
+    }
+  };
+
+  using KT = std::conditional_t<Q8, int8_t, T>;
+  const uint32_t ks_b = static_cast<uint32_t>(a.k.s2) * sizeof(KT), vs_b = static_cast<uint32_t>(a.v.s2) * sizeof(KT);
+  const KT *kbase = static_cast<const KT *>(a.k.data) + b * a.k.s0 + hk * a.k.s1;
+  const KT *vbase = static_cast<const KT *>(a.v.data) + b * a.v.s0 + hk * a.v.s1;
+  if constexpr (!Q8) {
+    // Keys past the cache's end, and tiles past the wave's last, read as zeros.
+    const u32x4 kdesc = make_desc(kbase, static_cast<uint32_t>(a.n) * ks_b);
+    const u32x4 vdesc = make_desc(vbase, static_cast<uint32_t>(a.n) * vs_b);
+    const uint32_t chunk = (lane & 3) ^ ((lane >> 4) & 3);
+    const uint32_t koff = (lane >> 2) * ks_b + chunk * 16, voff = (lane >> 2) * vs_b + chunk * 16;
+    // block n of a K or V tile whose first row is at byte `base`, to LDS address st
+    auto block = [&](u32x4 desc, uint32_t off, uint32_t stride, uint32_t base, uint32_t st, int n)
+                     __attribute__((always_inline)) {
+      if constexpr (F32)
+        dma16(desc, st + n * 1024, FTile<D>::dma_off(n, lane, stride), base + static_cast<uint32_t>(n * FTile<D>::RPB) * stride);
+      else
+        dma16(desc, st + n * 1024, off, base + static_cast<uint32_t>(16 * (n / QG)) * stride + (n % QG) * 64);
+    };
+    auto first_row = [&](int i, uint32_t stride) __attribute__((always_inline)) {
+      return i < mine ? static_cast<uint32_t>(key0(i)) * stride : 0x80000000u;
+    };
+    if constexpr (WR == 1) {
+      // K of a tile is issued once its stage's last K has been read, V likewise: of
+      // the stages' four tiles three are in flight while one is read.
+      auto issue_k = [&](int i) __attribute__((always_inline)) {
+        const uint32_t base = first_row(i, ks_b), st = ring0 + (i & 1) * STAGE;
+#pragma unroll
+        for (int n = 0; n < BLK; ++n) block(kdesc, koff, ks_b, base, st, n);
+      };
+      auto issue_v = [&](int i) __attribute__((always_inline)) {
+        const uint32_t base = first_row(i, vs_b), st = ring0 + (i & 1) * STAGE + TILE;
+#pragma unroll
+        for (int n = 0; n < BLK; ++n) block(vdesc, voff, vs_b, base, st, n);
+      };
+      issue_k(0);
+      issue_v(0);
+      issue_k(1);
+      for (int i = 0; i < mine; ++i) {
+        const char *kt = ring + (i & 1) * STAGE, *vt = kt + TILE;
+        wait_vm_n<2 * BLK>();  // K of tile i; its V and the next K in flight
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x16 s = scores(kt);
+        __builtin_amdgcn_sched_barrier(0);
+        issue_v(i + 1);
+        softmax(s, key0(i), nullptr);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_vm_n<2 * BLK>();  // V of tile i; the next K and V in flight
+        __builtin_amdgcn_sched_barrier(0);
+        values(vt);
+        wait_lgkm0();  // both tiles read
+        __builtin_amdgcn_sched_barrier(0);
+        issue_k(i + 2);
+      }
+      wait_vm_n<0>();
+    } else {
+      // wave w loads blocks w, w + WR, .. of a pair, K's first; two tiles ahead
+      auto issue = [&](int i) __attribute__((always_inline)) {
+        const uint32_t kb = first_row(i, ks_b), vb = first_row(i, vs_b), st = ring0 + (i % NS) * STAGE;
+#pragma unroll
+        for (int u = 0; u < LPT; ++u) {
+          const int n = w + WR * u;
+          if (n < BLK) block(kdesc, koff, ks_b, kb, st, n);
+          else block(vdesc, voff, vs_b, vb, st + TILE, n - BLK);
+        }
+      };
+      issue(0);
+      issue(1);
+      for (int i = 0; i < mine; ++i) {
+        const char *kt = ring + (i % NS) * STAGE;
+        wait_vm_n<LPT>();  // this wave's blocks of tile i
+        wait_lgkm0();
+        phase_barrier();  // every wave's; and tile i - 1 is read
+        issue(i + 2);
+        softmax(scores(kt), key0(i), nullptr);
+        values(kt + TILE);
+      }
+      wait_vm_n<0>();
+    }
+  } else {
+    // Codes come through registers, a tile ahead, and are widened into 16-bit tiles.
+    constexpr int LANES = 64 * WR, PIECES = BN * D / 16;  // 16 codes a piece
+    constexpr int NPC = (PIECES + LANES - 1) / LANES;
+    const int gl = WR > 1 ? tid : lane;
+    u32x4 kc[NPC], vc[NPC];
+    float sc = 0.f;  // lanes 0 .. 31 of the group: K's scales, 32 .. 63: V's
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+      const int kv0 = i < mine ? key0(i) : a.n;
+#pragma unroll
+      for (int u = 0; u < NPC; ++u) {
+        const int at = u * LANES + gl, key = kv0 + at / (D / 16), col = at % (D / 16) * 16;
+        kc[u] = vc[u] = u32x4{0, 0, 0, 0};
+        if (at < PIECES && key < a.n) {
+          kc[u] = ld16(kbase + static_cast<int64_t>(key) * a.k.s2 + col);
+          vc[u] = ld16(vbase + static_cast<int64_t>(key) * a.v.s2 + col);
+        }
+      }
+      if (gl < 64) {
+        const int key = kv0 + (gl & 31);
+        const View &s = gl < 32 ? a.ks : a.vs;
+        sc = key < a.n ? static_cast<const float *>(s.data)[b * s.s0 + hk * s.s1 + static_cast<int64_t>(key) * s.s2] : 0.f;
+      }
+    };
+    auto place = [&](int i) __attribute__((always_inline)) {
+      char *st = ring + (i & 1) * STAGE;
+#pragma unroll
+      for (int u = 0; u < NPC; ++u) {
+        const int at = u * LANES + gl, r = at / (D / 16), ch = at % (D / 16) * 2;
+        if (PIECES % LANES && at >= PIECES) continue;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int k = ch + e;
+          char *to = st + ((r >> 4) * QG + (k >> 2)) * 1024 + 16 * (4 * (r & 15) + ((k & 3) ^ ((r >> 2) & 3)));
+          *reinterpret_cast<u32x4 *>(to) = widen<T>(kc[u][2 * e], kc[u][2 * e + 1]);
+          *reinterpret_cast<u32x4 *>(to + TILE) = widen<PT>(vc[u][2 * e], vc[u][2 * e + 1]);
+        }
+      }
+      if (gl < 64) *reinterpret_cast<float *>(st + PAIR + 4 * gl) = sc;
+    };
+    auto settle = [&] {  // tile i is in LDS for all of its waves
+      if constexpr (WR > 1) {
+        __syncthreads();
+      } else {
+        wait_lgkm0();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+    };
+    if (mine > 0) {
+      fetch(0);
+      place(0);
+      fetch(1);
+    }
+    for (int i = 0; i < mine; ++i) {
+      settle();
+      if (i + 1 < mine) {
+        place(i + 1);
+        fetch(i + 2);
+      }
+      const char *kt = ring + (i & 1) * STAGE;
+      softmax(scores(kt), key0(i), reinterpret_cast<const float *>(kt + PAIR));
+      values(kt + TILE);
+    }
+  }
+
+  // Lane holds O^T[channel 32 dt + 8 g + 4 h + r][row c] in oacc[dt][4 g + r].
+  const int64_t rows = static_cast<int64_t>(bhs) * a.R, at = static_cast<int64_t>(bh) * a.R + row;
+  float *po = a.ws + (part * rows + at) * D;
+  float *ml = a.ws + a.splits * rows * D + 2 * (part * rows + at);
+  T *out = static_cast<T *>(const_cast<void *>(a.o.data)) + b * a.o.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.o.s1 +
+           static_cast<int64_t>(t) * a.o.s2;
+  auto store = [&](int d, float4 x, float inv) __attribute__((always_inline)) {
+    if (a.splits > 1) {
+      *reinterpret_cast<float4 *>(po + d) = x;
+    } else if constexpr (F32) {
+      *reinterpret_cast<float4 *>(out + d) = float4{x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    } else {
+      *reinterpret_cast<u32x2 *>(out + d) = u32x2{pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv)};
+    }
+  };
+  float lt = xor32_sum(l);
+  if constexpr (WK == 1) {
+    if (!live) return;
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;
+#pragma unroll
+    for (int dt = 0; dt < PDT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store(32 * dt + 8 * g + 4 * h,
+              float4{oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]}, inv);
+  } else {
+    // the waves' results, joined in their order; wave w stores groups w, w + NWV, ..
+    __syncthreads();  // every ring is read
+    float *cm = reinterpret_cast<float *>(lds), *cl = cm + NWV * 32, *co = cl + NWV * 32;
+    if (h == 0) cm[w * 32 + c] = m, cl[w * 32 + c] = lt;
+#pragma unroll
+    for (int dt = 0; dt < PDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) co[((w * PDT + dt) * 16 + e) * 64 + lane] = oacc[dt][e];
+    __syncthreads();
+    m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NWV; ++v) m = fmaxf(m, cm[v * 32 + c]);
+    float f[NWV];
+    lt = 0.f;
+#pragma unroll
+    for (int v = 0; v < NWV; ++v) {
+      const float mv = cm[v * 32 + c];
+      f[v] = mv == -INFINITY ? 0.f : fast_exp2(mv - m);
+      lt += cl[v * 32 + c] * f[v];
+    }
+    if (!live) return;
+    const float inv = lt > 0.f ? 1.f / lt : 0.f;
+    for (int g = w; g < PDT * 4; g += NWV) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < NWV; ++v)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          x[r] = fmaf(co[((v * PDT + (g >> 2)) * 16 + 4 * (g & 3) + r) * 64 + lane], f[v], x[r]);
+      store(8 * g + 4 * h, float4{x[0], x[1], x[2], x[3]}, inv);
+    }
+    if (w) return;
+  }
+  if (a.splits > 1 && h == 0) ml[0] = m, ml[1] = lt;
+}
+
+// The splits' partial rows, joined in their order: D / 4 lanes a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void cached_merge_kernel(CachedArgs a) {
+  constexpr int LPR = D / 4, RPB = 256 / LPR;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.R;
+  const int q = threadIdx.x % LPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / LPR;
+  if (row >= rows) return;
+  const float *ml = a.ws + a.splits * rows * D + 2 * row;
+  float M = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[2 * s * rows]);
+  float L = 0.f;
+  float4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float mv = ml[2 * s * rows];
+    const float f = mv == -INFINITY ? 0.f : fast_exp2(mv - M);
+    L = fmaf(ml[2 * s * rows + 1], f, L);
+    const float4 x = *reinterpret_cast<const float4 *>(a.ws + (s * rows + row) * D + 4 * q);
+    o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  const int64_t bh = row / a.R, b = bh / a.Hkv;
+  const int r = static_cast<int>(row - bh * a.R), hk = static_cast<int>(bh - b * a.Hkv);
+  T *op = static_cast<T *>(const_cast<void *>(a.o.data)) + b * a.o.s0 +
+          static_cast<int64_t>(hk * a.rep + r / a.T) * a.o.s1 + static_cast<int64_t>(r % a.T) * a.o.s2 + 4 * q;
+  if constexpr (std::is_same_v<T, float>)
+    *reinterpret_cast<float4 *>(op) = float4{o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  else
+    *reinterpret_cast<u32x2 *>(op) = u32x2{pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv)};
+}
+
+// ---------------------------------------------------------------------------
+// A tree's words and depths from its parents: a workgroup a tree, the ancestors found by
+// doubling (each round a token takes over the ancestors of the furthest one it knows).
+// ---------------------------------------------------------------------------
+constexpr int kMostTokens = 256, kWords = kMostTokens / 32;
+
+__global__ __launch_bounds__(kMostTokens) void draft_tree_kernel(int T, const int32_t *parents, uint32_t *words,
+                                                                 int32_t *depth) {
+  __shared__ uint32_t up[kMostTokens][kWords];
+  __shared__ int jump[kMostTokens];
+  const int t = threadIdx.x;
+  uint32_t mine[kWords];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) up[t][i] = mine[i] = t >> 5 == i ? 1u << (t & 31) : 0u;
+  const int parent = t < T ? parents[static_cast<int64_t>(blockIdx.x) * T + t] : -1;
+  int to = parent >= 0 && parent < t ? parent : -1;
+  jump[t] = to;
+  __syncthreads();
+  for (int far = 1; far < T; far <<= 1) {
+    int next = -1;
+    if (to >= 0) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) mine[i] |= up[to][i];
+      next = jump[to];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) up[t][i] = mine[i];
+    jump[t] = to = next;
+    __syncthreads();
+  }
+  if (t >= T) return;
+  const int W = (T + 31) / 32;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) n += __popc(mine[i]);
+  for (int i = 0; i < W; ++i) words[(static_cast<int64_t>(blockIdx.x) * T + t) * W + i] = up[t][i];
+  depth[static_cast<int64_t>(blockIdx.x) * T + t] = n - 1;
+}
+
+// ---------------------------------------------------------------------------
+// Kept rows.  A workgroup takes 64 bytes (or one scale) of every row of a (sequence,
+// head, array): it reads the rows asked for, all of them, before it writes any, so the
+// order and repetitions of the indexes do not matter.
+// ---------------------------------------------------------------------------
+template <typename X>
+__global__ __launch_bounds__(256) void keep_kernel(KeepArgs a, int slices) {
+  constexpr int LPR = 4, RPP = 256 / LPR, PASSES = kMostTokens / RPP;  // X a lane, rows a pass
+  const int slice = blockIdx.x % slices, bh = blockIdx.x / slices, which = blockIdx.y;
+  const int b = bh / a.H, h = bh - b * a.H;
+  const int col = (slice * LPR + threadIdx.x % LPR) * static_cast<int>(sizeof(X));
+  if (a.data[which] == nullptr) return;
+  const bool in = col < a.bytes[which];
+  char *base = a.data[which] + b * a.s0[which] + h * a.s1[which] + a.first * a.s2[which] + col;
+  X x[PASSES];
+  int64_t from[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = i * RPP + threadIdx.x / LPR;
+    from[i] = -1;
+    if (in && r < a.n) {
+      const int64_t at = static_cast<int64_t>(b) * a.n + r;
+      from[i] = a.index_bytes == 8 ? static_cast<const int64_t *>(a.index)[at] : static_cast<const int32_t *>(a.index)[at];
+      if (from[i] < 0 || from[i] >= a.limit) from[i] = -1;
+    }
+    if (from[i] >= 0) x[i] = *reinterpret_cast<const X *>(base + from[i] * a.s2[which]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = i * RPP + threadIdx.x / LPR;
+    if (from[i] >= 0) *reinterpret_cast<X *>(base + r * a.s2[which]) = x[i];
+  }
+}
+
+struct CachedPlan {
+  int wr, groups, ns, gap, run, splits;
+};
+
+CachedPlan plan_cached(const CachedProblem &p) {
+  CachedPlan s;
+  const int R = p.Hq / p.Hkv * p.T;
+  s.wr = R <= 32 ? 1 : R <= 64 ? 2 : 4;
+  s.groups = (R + 32 * s.wr - 1) / (32 * s.wr);
+  const int tiles = (p.n + BN - 1) / BN;
+  // the first key that some row's window holds (depth 0's)
+  const int64_t low = p.window ? static_cast<int64_t>(p.n) - p.T - p.window + 1 : 0;
+  const int first = low > 0 ? static_cast<int>(low) / BN : 0;
+  const int sunk = p.window ? (p.sinks + BN - 1) / BN : 0;
+  s.ns = sunk < first ? sunk : first;
+  s.gap = first - s.ns;
+  s.run = tiles - s.gap;
+  // two workgroups a CU, each of 4 tiles a wave or more
+  const int64_t base = static_cast<int64_t>(p.B) * p.Hkv * s.groups;
+  const int least = 4 * (s.wr > 1 ? 1 : 2);
+  int64_t n = 512 / base;
+  if (n > s.run / least) n = s.run / least;
+  s.splits = n < 1 ? 1 : static_cast<int>(n);
+  return s;
+}
+
+template <typename T, int D, bool Q8>
+void launch_wr(const CachedArgs &a, int wr, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hkv * a.splits * a.groups));
+  if (wr == 1) cached_kernel<T, D, Q8, 1><<<grid, dim3(64 * kWaves<T, D, 1>), 0, st>>>(a);
+  else if (wr == 2) cached_kernel<T, D, Q8, 2><<<grid, dim3(128), 0, st>>>(a);
+  else cached_kernel<T, D, Q8, 4><<<grid, dim3(256), 0, st>>>(a);
+  if (a.splits > 1) {
+    const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.R;
+    constexpr int RPB = 256 / (D / 4);
+    cached_merge_kernel<T, D><<<dim3(static_cast<unsigned>((rows + RPB - 1) / RPB)), dim3(256), 0, st>>>(a);
+  }
+}
+
+template <typename T, bool Q8>
+void launch_dim(const CachedArgs &a, int D, int wr, hipStream_t st) {
+  if (D == 32) launch_wr<T, 32, Q8>(a, wr, st);
+  else if (D == 64) launch_wr<T, 64, Q8>(a, wr, st);
+  else if (D == 128) launch_wr<T, 128, Q8>(a, wr, st);
+  else if constexpr (!std::is_same_v<T, float>) launch_wr<T, 256, Q8>(a, wr, st);
+}
+
+}  // namespace
+
+bool cached_supported(const CachedProblem &p) {
+  if (p.dtype == TSATTN_F32) return !p.q8 && (p.D == 32 || p.D == 64 || p.D == 128);
+  return (p.dtype == TSATTN_F16 || p.dtype == TSATTN_BF16) && (p.D == 32 || p.D == 64 || p.D == 128 || p.D == 256);
+}
+
+size_t cached_workspace_bytes(const CachedProblem &p) {
+  const CachedPlan s = plan_cached(p);
+  return s.splits < 2 ? 0 : static_cast<size_t>(s.splits) * p.B * p.Hq * p.T * (p.D + 2) * sizeof(float);
+}
+
+hipError_t launch_cached(const CachedProblem &p, View q, View k, View v, View ks, View vs, View o, float *ws,
+                         hipStream_t st) {
+  const CachedPlan s = plan_cached(p);
+  CachedArgs a{};
+  a.B = p.B, a.Hkv = p.Hkv, a.rep = p.Hq / p.Hkv, a.T = p.T, a.n = p.n, a.R = a.rep * p.T;
+  a.q = q, a.k = k, a.v = v, a.o = o, a.ks = ks, a.vs = vs;
+  a.words = p.words, a.depth = p.depth, a.tree_rows = p.tree_rows, a.W = (p.T + 31) / 32;
+  a.window = p.window, a.sinks = p.sinks;
+  a.ns = s.ns, a.gap = s.gap, a.run = s.run, a.splits = s.splits, a.groups = s.groups;
+  a.sl = static_cast<float>(p.scale) * kLog2e;
+  a.rope = p.rope;
+  a.ws = ws;
+  Probe pr_(p.words ? "cached_tree" : "cached_window", st);
+  if (p.dtype == TSATTN_F32) launch_dim<float, false>(a, p.D, s.wr, st);
+  else if (p.dtype == TSATTN_F16) p.q8 ? launch_dim<f16, true>(a, p.D, s.wr, st) : launch_dim<f16, false>(a, p.D, s.wr, st);
+  else p.q8 ? launch_dim<bf16, true>(a, p.D, s.wr, st) : launch_dim<bf16, false>(a, p.D, s.wr, st);
+  return hipGetLastError();
+}
+
+hipError_t launch_draft_tree(int trees, int T, const int32_t *parents, uint32_t *words, int32_t *depth, hipStream_t st) {
+  Probe pr_("draft_tree", st);
+  draft_tree_kernel<<<dim3(trees), dim3(kMostTokens), 0, st>>>(T, parents, words, depth);
+  return hipGetLastError();
+}
+
+hipError_t launch_keep(const KeepArgs &a, hipStream_t st) {
+  Probe pr_("cache_keep", st);
+  // pieces as wide as every array's rows and addresses allow
+  int arrays = 0, most = 0;
+  uintptr_t all = 0;
+  for (int i = 0; i < 4; ++i)
+    if (a.data[i]) {
+      arrays = i + 1;
+      most = a.bytes[i] > most ? a.bytes[i] : most;
+      if (i < 2)
+        all |= reinterpret_cast<uintptr_t>(a.data[i]) | static_cast<uintptr_t>(a.bytes[i]) |
+               static_cast<uintptr_t>(a.s0[i]) | static_cast<uintptr_t>(a.s1[i]) | static_cast<uintptr_t>(a.s2[i]);
+    }
+  if (arrays > 2 && all % 16 == 0) all |= 4;  // (scales: 4 bytes a row)
+  const int piece = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+  const int slices = (most + 4 * piece - 1) / (4 * piece);
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H * slices), arrays);
+  if (piece == 16) keep_kernel<u32x4><<<grid, dim3(256), 0, st>>>(a, slices);
+  else if (piece == 4) keep_kernel<uint32_t><<<grid, dim3(256), 0, st>>>(a, slices);
+  else keep_kernel<uint8_t><<<grid, dim3(256), 0, st>>>(a, slices);
+  return hipGetLastError();
+}
+
+}  // namespace tsattn

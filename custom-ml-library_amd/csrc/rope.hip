@@ -124,6 +124,9 @@ struct AppendArgs {
   View kc, vc, ks, vs;    // cache storage; ks / vs set for int8 caches
   const void *cos, *sin;  // [*, R / 2]
   int64_t pos;
+  // a tree's depths [1 or B, T]: row t rotates at position pos + its depth (NULL: pos + t)
+  const int32_t *depth;
+  int tree_rows;
 };
 
 // Quantise one wave-held row (PER values per lane, channels 2p, 2p + 1 for
@@ -162,8 +165,9 @@ __global__ __launch_bounds__(NT) void rope_append_kernel(AppendArgs a) {
   const int64_t tp = a.pos + t;
   const T *kx = static_cast<const T *>(a.k.data) + b * a.k.s0 + h * a.k.s1 + static_cast<int64_t>(t) * a.k.s2;
   const T *vx = static_cast<const T *>(a.v.data) + b * a.v.s0 + h * a.v.s1 + static_cast<int64_t>(t) * a.v.s2;
-  const T *cr = static_cast<const T *>(a.cos) + tp * (a.R / 2);
-  const T *sr = static_cast<const T *>(a.sin) + tp * (a.R / 2);
+  const int64_t at = a.depth ? a.pos + a.depth[(a.tree_rows > 1 ? b : 0) * a.T + t] : tp;
+  const T *cr = static_cast<const T *>(a.cos) + at * (a.R / 2);
+  const T *sr = static_cast<const T *>(a.sin) + at * (a.R / 2);
   T kr[PER][2], vr[PER][2];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -233,8 +237,8 @@ hipError_t launch_rope(int dtype, int B, int H, int T, int D, int R, View x, Vie
 
 hipError_t launch_rope_append(int dtype, int B, int H, int T, int D, int R, View k, View v, View kc,
                               View vc, const View *ks, const View *vs, const void *cos,
-                              const void *sin, int64_t pos, hipStream_t st) {
-  AppendArgs a{B, H, T, D, R, k, v, kc, vc, ks ? *ks : View{}, vs ? *vs : View{}, cos, sin, pos};
+                              const void *sin, int64_t pos, const int32_t *depth, int tree_rows, hipStream_t st) {
+  AppendArgs a{B, H, T, D, R, k, v, kc, vc, ks ? *ks : View{}, vs ? *vs : View{}, cos, sin, pos, depth, tree_rows};
   const bool q8 = ks != nullptr;
   Probe pr_(q8 ? "rope_append_int8" : "rope_append", st);
   const dim3 g = row_grid(B, H, T);

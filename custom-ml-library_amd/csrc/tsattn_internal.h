@@ -278,9 +278,42 @@ hipError_t launch_rope(int dtype, int B, int H, int T, int D, int R, View x, Vie
                        const void *cos, const void *sin, int64_t pos0, int inverse, hipStream_t st);
 // RoPE of the new K rows (R = 0: none) fused with the K/V cache append at
 // `pos`; ks / vs non-null for int8 caches (then quantised as the int8 append).
+// depth: NULL, or [tree_rows (1 or B), T]: row t rotates at pos + its depth.
 hipError_t launch_rope_append(int dtype, int B, int H, int T, int D, int R, View k, View v, View kc,
                               View vc, const View *ks, const View *vs, const void *cos,
-                              const void *sin, int64_t pos, hipStream_t st);
+                              const void *sin, int64_t pos, const int32_t *depth, int tree_rows, hipStream_t st);
+
+// New tokens' attention over a key/value cache (cached.hip): each sees the positions in
+// front of the new ones that its window and the sinks leave, and of the new ones those
+// up to itself or, in a tree, its ancestors and itself.
+struct CachedProblem {
+  int dtype, B, Hq, Hkv, T, n, D;  // n: cached positions, the T new ones included
+  bool q8;
+  double scale;
+  int window, sinks;      // window 0: none
+  const uint32_t *words;  // a tree's ancestors [tree_rows, T, ceil(T / 32)], or NULL
+  const int32_t *depth;   // [tree_rows, T]
+  int tree_rows;          // 1 or B
+  RopeDesc rope;          // R = D, or 0: q comes rotated
+};
+bool cached_supported(const CachedProblem &p);
+size_t cached_workspace_bytes(const CachedProblem &p);
+hipError_t launch_cached(const CachedProblem &p, View q, View k, View v, View ks, View vs, View o, float *ws,
+                         hipStream_t st);
+// words and depths of `trees` rows of T parents (not an earlier token: none).
+hipError_t launch_draft_tree(int trees, int T, const int32_t *parents, uint32_t *words, int32_t *depth, hipStream_t st);
+// Rows first + index[b, i] of a cache become its rows first + i; `bytes` a row, strides
+// in bytes, index int64 or int32.  An index outside [0, limit) leaves its row as it is.
+struct KeepArgs {
+  char *data[4];  // keys, values and their scales (NULL: none)
+  int64_t s0[4], s1[4], s2[4];
+  int bytes[4];
+  int B, H, n;
+  int64_t first, limit;
+  const void *index;
+  int index_bytes;
+};
+hipError_t launch_keep(const KeepArgs &a, hipStream_t st);
 
 // The q / k / v projections of the `batch x len` rows of x (embed wide; a
 // [batch, 1, len, embed] view) with

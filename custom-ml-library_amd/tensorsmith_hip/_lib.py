@@ -111,6 +111,29 @@ class StepDesc(ctypes.Structure):
     ]
 
 
+class Cached(ctypes.Structure):
+    """``tsattn_cached``: the newest tokens' attention over a cache."""
+
+    _fields_ = [
+        ("dtype", c_int32),
+        ("batch", c_int32),
+        ("heads_q", c_int32),
+        ("heads_kv", c_int32),
+        ("dim", c_int32),
+        ("len", c_int32),
+        ("keys", c_int32),
+        ("quantized", c_int32),
+        ("scale", c_double),
+        ("window", c_int64),
+        ("sinks", c_int32),
+        ("trees", c_int32),
+        ("words", c_void_p),
+        ("depths", c_void_p),
+        ("cos", c_void_p),
+        ("sin", c_void_p),
+    ]
+
+
 class Pages4(ctypes.Structure):
     """``tsattn_pages4``: a 4-bit paged cache's pool and page table."""
 
@@ -217,6 +240,20 @@ SIGNATURES = {
         [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _PV, _PV, _PV, _PV, _PV, _PV,
          c_void_p, c_void_p, c_int64, c_void_p],
     ),
+    "tsattn_draft_tree": (c_int, [c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tsattn_draft_append": (
+        c_int,
+        [c_int32, c_int32, c_int32, c_int32, c_int32, _PV, _PV, _PV, _PV, _PV, _PV, c_void_p, c_void_p, c_int64,
+         c_void_p, c_int32, c_void_p],
+    ),
+    "tsattn_cache_keep": (
+        c_int,
+        [c_int32, c_int32, c_int32, c_int64, c_int64, c_void_p, c_int32, c_int32, c_int32, _PV, _PV, _PV, _PV,
+         c_void_p],
+    ),
+    "tsattn_cached_attend_workspace": (c_size_t, [POINTER(Cached)]),
+    "tsattn_cached_attend": (
+        c_int, [POINTER(Cached), _PV, _PV, _PV, _PV, _PV, _PV, c_void_p, c_size_t, c_void_p]),
     "tsattn_qkv_rope_append": (
         c_int,
         [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _PV, c_void_p,

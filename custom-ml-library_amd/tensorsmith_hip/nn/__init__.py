@@ -4,6 +4,7 @@ from . import functional
 from .attention import rotary_embedding, scaled_dot_product_attention
 from .cache import KVCache
 from .checkpoint import checkpoint
+from .drafts import DraftTree, cached_attention
 from .layers import GELU, Dropout, Embedding, LayerNorm, Linear
 from .module import Module, Parameter
 from .paged import PagedKVCache, paged_attention
@@ -13,8 +14,8 @@ from .transformer import (
 )
 
 __all__ = [
-    "Dropout", "Embedding", "GELU", "KVCache", "LayerNorm", "Linear", "Module",
+    "Dropout", "DraftTree", "Embedding", "GELU", "KVCache", "LayerNorm", "Linear", "Module",
     "MultiHeadAttention", "PagedKVCache", "Parameter", "RMSNorm", "SiLU", "SwiGLU", "TransformerConfig",
-    "TransformerDecoderBlock", "TransformerLM", "checkpoint", "functional", "paged_attention",
+    "TransformerDecoderBlock", "TransformerLM", "cached_attention", "checkpoint", "functional", "paged_attention",
     "rotary_embedding", "sample_logits", "scaled_dot_product_attention",
 ]

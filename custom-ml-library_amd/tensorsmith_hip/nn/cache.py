@@ -25,7 +25,7 @@ import numpy as np
 import ctypes
 
 from .. import _lib
-from ..device import current_stream
+from ..device import current_stream, launch
 from .attention import _view
 from ..device import device as parse_device
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
@@ -116,6 +116,77 @@ class KVCache:
         self.length = stop
         return True
 
+    def append_tree(self, key: Tensor, value: Tensor, tree, *, rotary_base: float | None = None) -> None:
+        """Append the rows of drafted tokens [B, H, T, D] (``DraftTree``), the keys rotated by RoPE at their own
+        positions, the cached length plus their depths, where ``rotary_base`` is given: one kernel
+        (``tsattn_draft_append``)."""
+        import torch
+
+        from .drafts import _rotate_at, check_rotary
+
+        stop = self._check(key, value)
+        tree._check(self.batch_size, key.shape[2], self.device)
+        check_rotary(rotary_base, self.head_dim)
+        if (key._data.dtype != self.dtype or value._data.dtype != self.dtype
+                or self.dtype not in (torch.float32, torch.float16, torch.bfloat16)
+                or self.head_dim % 2 or self.head_dim > 512 or self.value_dim != self.head_dim):
+            if rotary_base is not None:
+                key = Tensor._leaf(_rotate_at(key._data, self.length + tree._depths, rotary_base), self.device)
+            return self._append(key, value)
+        cos = sin = None
+        if rotary_base is not None:
+            from .attention import rope_tables
+
+            cos, sin = (x.data_ptr() for x in rope_tables(rotary_base, self.head_dim, self.dtype, self._keys.device, stop))
+        k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (key._data, value._data))
+        b, h, t, d = k.shape
+        scales = (_view(self._key_scales), _view(self._value_scales)) if self.quantized else (None, None)
+        _lib.check(launch(self.device, _lib.load().tsattn_draft_append, _CODES[str(k.dtype)], b, h, t, d, _view(k),
+                          _view(v), _view(self._keys), _view(self._values), *scales, cos, sin, self.length,
+                          tree._depths.data_ptr(), tree.trees), "draft append")
+        self.length = stop
+
+    def keep(self, first: int, index) -> None:
+        """Of the positions from ``first`` on, keep those that ``index`` [B, n] names (n at most 256, counted from
+        ``first``): they become the positions first .. first + n - 1, the cache's last.  One kernel reads all of them
+        before it writes any (``tsattn_cache_keep``), so their order is free.  Indices on the host are checked; a hip
+        tensor's are not waited for, and where one is out of range the position keeps what it held."""
+        if not 0 <= first <= self.length:
+            raise ValueError("first must be between zero and the current length")
+        drafted = self.length - first
+        on_device = isinstance(index, Tensor) and index.device.type == "hip"
+        if on_device and index.device != self.device:
+            raise ValueError("kept indices must be on the cache's device")
+        if not on_device:
+            index = np.asarray(index.numpy() if isinstance(index, Tensor) else index)
+        if "int" not in str(index.dtype) and 0 not in index.shape:
+            raise TypeError("kept indices must have an integer dtype")
+        if len(index.shape) != 2 or index.shape[0] != self.batch_size or index.shape[1] > min(drafted, 256):
+            raise ValueError("kept indices must be [batch, positions], at most 256 and no more than there are")
+        import torch
+
+        if not on_device:
+            if (index < 0).any() or (index >= drafted).any():
+                raise ValueError("kept index out of range")
+            index = Tensor._leaf(torch.from_numpy(index.astype(np.int64)).to(self._keys.device), self.device)
+        n = index.shape[1]
+        if n:
+            raw = index._data if index._data.dtype in (torch.int64, torch.int32) else index._data.long()
+            raw = raw.contiguous()
+
+            def rows(x):  # in bytes
+                view = _view(x)
+                for i in range(3):
+                    view.stride[i] *= x.element_size()
+                return view, x.shape[-1] * x.element_size()
+
+            (keys, key_bytes), (values, value_bytes) = rows(self._keys), rows(self._values)
+            scales = (_view(self._key_scales), _view(self._value_scales)) if self.quantized else (None, None)
+            _lib.check(launch(self.device, _lib.load().tsattn_cache_keep, self.batch_size, self.num_heads, n, first,
+                              drafted, raw.data_ptr(), raw.element_size(), key_bytes, value_bytes, keys, values,
+                              *scales), "cache rows")
+        self.length = first + n
+
     def _project_append(self, input: Tensor, projections, num_heads: int, rotary: bool,
                         base: float = 10000.0):
         """The cached attention step's q / k / v projections (``projections``:
@@ -182,12 +253,16 @@ class KVCache:
             raise ValueError(f"cache capacity {self.max_seq_len} exceeded or empty append")
         return stop
 
-    def get(self) -> tuple[Tensor, Tensor]:
-        keys = self._keys[:, :, : self.length]
-        values = self._values[:, :, : self.length]
+    def get(self, last: int | None = None) -> tuple[Tensor, Tensor]:
+        """Keys and values of the active prefix, or of its ``last`` positions."""
+        if last is not None and not 0 <= last <= self.length:
+            raise ValueError("last must be between zero and the current length")
+        part = slice(0 if last is None else self.length - last, self.length)
+        keys = self._keys[:, :, part]
+        values = self._values[:, :, part]
         if self.quantized:
-            keys = (keys.float() * self._key_scales[:, :, : self.length]).to(self.dtype)
-            values = (values.float() * self._value_scales[:, :, : self.length]).to(self.dtype)
+            keys = (keys.float() * self._key_scales[:, :, part]).to(self.dtype)
+            values = (values.float() * self._value_scales[:, :, part]).to(self.dtype)
         return Tensor(keys, device=self.device), Tensor(values, device=self.device)
 
     def reset(self) -> None:

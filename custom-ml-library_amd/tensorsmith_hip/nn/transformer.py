@@ -39,6 +39,7 @@ from .attention import (BACKENDS, DECODE_MIN_KEYS, _check_window, _dtype_code, _
                         rotary_embedding, scaled_dot_product_attention)
 from .cache import KVCache
 from .checkpoint import checkpoint
+from .drafts import DraftTree, cached_attention
 from .layers import Dropout, Embedding, Linear
 from .module import Module, Parameter
 from .paged import PagedKVCache, paged_attention
@@ -73,7 +74,8 @@ def _cached_step(x: Tensor, attention, cache, is_causal: bool = True, block=None
 
     raw = x._data
     if (raw.dtype not in (torch.float16, torch.bfloat16) or type(cache) is not KVCache
-            or cache.dtype != raw.dtype or attention.backend == "native" or attention.window is not None):
+            or cache.dtype != raw.dtype or attention.backend == "native"
+            or (attention.window is not None and attention.window < cache.length + raw.shape[1])):
         return None
     b, t, e = raw.shape
     pos, stop = cache.length, cache.length + t
@@ -195,7 +197,9 @@ class MultiHeadAttention(Module):
                        device=self.q_proj.weight.device, dtype=dtype, quantized=quantized)
 
     def forward(self, input: Tensor, context: Tensor | None = None, *, attn_mask=None,
-                is_causal: bool = True, cache: KVCache | PagedKVCache | None = None) -> Tensor:
+                is_causal: bool = True, cache: KVCache | PagedKVCache | None = None,
+                tree: DraftTree | None = None) -> Tensor:
+        """``tree``: the input's tokens are drafted, a tree behind the cached ones (``cached_attention``)."""
         if input.ndim != 3 or input.shape[-1] != self.embed_dim:
             raise ValueError("attention input must be [batch, sequence, embed_dim]")
         source = input if context is None else context
@@ -209,6 +213,8 @@ class MultiHeadAttention(Module):
         offset = 0 if cache is None else cache.length
         if self.backend == "native":
             raise ValueError("native attention requires Metal")
+        if self.window is not None and not is_causal:
+            raise ValueError("a window needs causal attention")
         if attn_mask is not None:
             if attn_mask.requires_grad or attn_mask.device != input.device:
                 raise ValueError("attention mask must be non-differentiable and on the input device")
@@ -220,8 +226,21 @@ class MultiHeadAttention(Module):
                     raise TypeError("attention masks must be boolean or floating point")
             except ValueError as error:
                 raise ValueError("attention mask is not broadcastable to [B,H,Q,K]") from error
+        if tree is not None:
+            if not isinstance(cache, KVCache) or attn_mask is not None or not is_causal:
+                raise ValueError("drafted tokens need a KVCache and take no other mask")
+            q, k, v = (proj(input).reshape(batch, steps, heads, self.head_dim).permute(0, 2, 1, 3)
+                       for proj, heads in ((self.q_proj, self.num_heads), (self.k_proj, self.num_kv_heads),
+                                           (self.v_proj, self.num_kv_heads)))
+            base = 10000.0 if self.rotary else None
+            cache.append_tree(k, v, tree, rotary_base=base)
+            attended = cached_attention(q, cache, tree, window=self.window, sinks=self.sinks, rotary_base=base)
+            return self.out_proj(attended.permute(0, 2, 1, 3).reshape(batch, steps, self.embed_dim))
         if isinstance(cache, PagedKVCache):
             return self._paged(input, cache, attn_mask, is_causal)
+        # a window over more than it holds: the kernel that reads its part of the cache
+        windowed = (self.window is not None and cache is not None and context is None and attn_mask is None
+                    and is_causal and self.window < offset + steps)
         if cache is not None and context is None and attn_mask is None:
             stepped = _cached_step(input, self, cache, is_causal)
             if stepped is not None:
@@ -235,7 +254,9 @@ class MultiHeadAttention(Module):
         if q_fused is not None:
             q = Tensor._from_op(q_fused, (input,), None, "qkv_rope_append")
             attended = None
-            if cache.quantized and attn_mask is None and self.window is None:
+            if windowed:
+                attended = cached_attention(q, cache, window=self.window, sinks=self.sinks)
+            elif cache.quantized and attn_mask is None:
                 attended = decode_int8_cache(q, cache, is_causal=is_causal, causal_offset=offset)
             if attended is None:
                 k, v = cache.get()
@@ -270,7 +291,10 @@ class MultiHeadAttention(Module):
         if cache is not None:
             if not fused:
                 cache._append(k, v)
-            if cache.quantized and attn_mask is None and self.window is None:
+            if windowed:
+                attended = cached_attention(q, cache, window=self.window, sinks=self.sinks,
+                                            rotary_base=10000.0 if rope else None)
+            elif cache.quantized and attn_mask is None:
                 # decode straight over the int8 storage (dequantised in the kernel)
                 attended = decode_int8_cache(q, cache, is_causal=is_causal, causal_offset=offset,
                                              rope=rope and (offset, 10000.0))
@@ -355,15 +379,16 @@ class TransformerDecoderBlock(Module):
         self.ffn_norm = RMSNorm(dim, device=device)
         self.ffn = SwiGLU(dim, hidden_dim or 4 * dim, dropout, device)
 
-    def forward(self, input: Tensor, *, cache=None, attn_mask=None) -> Tensor:
-        if (cache is not None and attn_mask is None and not is_grad_enabled()
+    def forward(self, input: Tensor, *, cache=None, attn_mask=None, tree=None) -> Tensor:
+        if (cache is not None and attn_mask is None and tree is None and not is_grad_enabled()
                 and not self.attention.training and input.ndim == 3
                 and input.shape[-1] == self.attention.embed_dim):
             stepped = _cached_step(input, self.attention, cache, block=self)
             if stepped is not None:
                 return Tensor._from_op(stepped, (input,), None, "cached_step")
         hidden = input + self.residual_dropout(
-            self.attention(self.attention_norm(input), cache=cache, attn_mask=attn_mask))
+            self.attention(self.attention_norm(input), cache=cache, attn_mask=attn_mask,
+                           **({} if tree is None else {"tree": tree})))
         return hidden + self.ffn(self.ffn_norm(hidden))
 
 
@@ -433,11 +458,17 @@ class TransformerLM(Module):
         self.token_embedding.weight._data = self.token_embedding.weight._data * 0.02
 
     def forward(self, tokens: Tensor, *, caches: list[KVCache] | None = None, attn_mask=None,
-                logits_to_keep: int = 0) -> Tensor:
+                logits_to_keep: int = 0, tree: DraftTree | None = None) -> Tensor:
+        """``tree``: the tokens are drafted, a tree of them behind the caches' positions; each gets its own
+        logits.  ``KVCache.keep`` then keeps an accepted path."""
         if tokens.ndim != 2 or "int" not in str(tokens.dtype) or tokens.shape[1] == 0:
             raise ValueError("tokens must be a nonempty integer [batch, time] tensor")
         if not isinstance(logits_to_keep, int) or not 0 <= logits_to_keep <= tokens.shape[1]:
             raise ValueError("logits_to_keep must be between zero (all) and the input length")
+        if tree is not None:
+            if caches is None or not all(isinstance(cache, KVCache) for cache in caches):
+                raise ValueError("drafted tokens need one KVCache per block")
+            tree._check(tokens.shape[0], tokens.shape[1], tokens.device)
         offset = before = 0
         if caches is not None:
             # (a paged cache's rows have positions of their own)
@@ -468,7 +499,7 @@ class TransformerLM(Module):
                     hidden = checkpoint(block, hidden, attn_mask=attn_mask)
                 else:
                     hidden = block(hidden, cache=None if caches is None else caches[i],
-                                   attn_mask=attn_mask)
+                                   attn_mask=attn_mask, **({} if tree is None else {"tree": tree}))
             if logits_to_keep:
                 hidden = hidden[:, -logits_to_keep:, :]
             return F.linear(self.final_norm(hidden), self.output_weight)

@@ -396,6 +396,75 @@ int tsattn_rope_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len,
                        const void *sin, int64_t pos, void *stream);
 
 /*
+ * Drafted tokens (no counterpart in the reference, which decodes a token at a time:
+ * src/tensorsmith/nn/transformer.py:355-402): a tree of them continues each cached
+ * sequence, and its tokens follow each other in the cache.  Token t's parent is an
+ * earlier token of the tree, or none (-1, and what else is not an earlier token): the
+ * sequence's last cached token.  A token's position is the prefix's length plus its
+ * depth, the number of its ancestors.
+ *
+ * tsattn_draft_tree: parents [trees, len] (len at most 256) -> words [trees, len,
+ * ceil(len / 32)], whose bit s of token t (word s / 32, bit s % 32) says that s is t or
+ * one of its ancestors, and depths [trees, len].
+ */
+int tsattn_draft_tree(int32_t trees, int32_t len, const int32_t *parents, uint32_t *words, int32_t *depths,
+                      void *stream);
+
+/*
+ * tsattn_rope_append for drafted tokens: rows into positions pos .. pos + len - 1 of the
+ * caches, the keys rotated at position pos + depth (cos / sin as there with rotary_dim =
+ * dim, or both NULL).  trees: 1 (of all sequences) or batch.
+ */
+int tsattn_draft_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len, int32_t dim, const tsattn_view *k,
+                        const tsattn_view *v, const tsattn_view *k_cache, const tsattn_view *v_cache,
+                        const tsattn_view *k_scale, const tsattn_view *v_scale, const void *cos, const void *sin,
+                        int64_t pos, const int32_t *depths, int32_t trees, void *stream);
+
+/*
+ * Rows first + index[b, i] of a cache's arrays [batch, heads, *] become its rows first +
+ * i, i < n (at most 256), all of them read before any is written.  index: [batch, n],
+ * int64 or int32 (index_bytes); one outside [0, limit) leaves row first + i as it is.
+ * k, v: views with strides in bytes, key_bytes and value_bytes a row; k_scale, v_scale:
+ * fp32 scales a row (strides in elements), or both NULL.
+ */
+int tsattn_cache_keep(int32_t batch, int32_t heads, int32_t n, int64_t first, int64_t limit, const void *index,
+                      int32_t index_bytes, int32_t key_bytes, int32_t value_bytes, const tsattn_view *k,
+                      const tsattn_view *v, const tsattn_view *k_scale, const tsattn_view *v_scale, void *stream);
+
+/*
+ * Attention of the newest `len` tokens over a cache of `keys` positions, theirs the last
+ * (src/tensorsmith/nn/attention.py:175-198): causal, through a window (as
+ * tsattn_window_forward; 0: none), or with words and depths of drafted tokens, each of
+ * which sees the positions in front of them (through the window at its position), its
+ * ancestors and itself.  A window holds all of a tree.
+ */
+typedef struct tsattn_cached {
+  int32_t dtype; /* of q, out and the cache (or what an int8 cache stands for) */
+  int32_t batch, heads_q, heads_kv, dim, len, keys;
+  int32_t quantized; /* the cache is int8 with fp32 scales a row */
+  double scale;
+  int64_t window;
+  int32_t sinks;
+  int32_t trees; /* 1 or batch, with words */
+  const uint32_t *words; /* of tsattn_draft_tree, or NULL */
+  const int32_t *depths;
+  const void *cos, *sin; /* rotate the queries at their positions (tables [*, dim / 2]), or NULL */
+} tsattn_cached;
+
+/* Bytes of scratch tsattn_cached_attend needs (0: none, or a problem it does not take). */
+size_t tsattn_cached_attend_workspace(const tsattn_cached *d);
+
+/*
+ * q, out [batch, heads_q, len, dim]; k, v [batch, heads_kv, capacity, dim] in dtype, or
+ * int8 with k_scale, v_scale [batch, heads_kv, capacity, 1].  f16, bf16 and int8 caches of
+ * 32, 64, 128 or 256 channels, f32 ones of 32, 64 or 128, len at most 256, 16-byte aligned
+ * rows (others: TSATTN_ERR_UNSUPPORTED).  Deterministic.
+ */
+int tsattn_cached_attend(const tsattn_cached *d, const tsattn_view *q, const tsattn_view *k, const tsattn_view *v,
+                         const tsattn_view *k_scale, const tsattn_view *v_scale, const tsattn_view *out,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * The cached MultiHeadAttention step before the attention in one kernel:
  * the three input projections (MultiHeadAttention.forward, src/tensorsmith/
  * nn/transformer.py:124-138: q = x Wq^T (+ bq), k = x Wk^T (+ bk),
