@@ -322,9 +322,15 @@ int sdpa_backward(const tsattn_problem *p, const tsattn_rope_desc *rope, const t
       mfma_f32_view_ok(vk, pr.Sk) && mfma_f32_view_ok(vv, pr.Sk) && mfma_f32_view_ok(vo, pr.Sq) &&
       mfma_f32_view_ok(vg, pr.Sq) && mfma_f32_view_ok(vdq, pr.Sq) && mfma_f32_view_ok(vdk, pr.Sk) &&
       mfma_f32_view_ok(vdv, pr.Sk)) {
+    const size_t parts_bytes = tsattn::mfma_f32_window_bytes(pr), parts_off = round256(rows_need);
+    if (parts_bytes && workspace_bytes < parts_off + parts_bytes)
+      return fail(TSATTN_ERR_INVALID, "backward workspace too small: %zu < %zu bytes", workspace_bytes,
+                  parts_off + parts_bytes);
     g_last_path = 2;
-    return hip_status(tsattn::launch_mfma_f32_backward(pr, vq, vk, vv, vo, vg, static_cast<const float *>(lse),
-                                                       vdq, vdk, vdv, static_cast<float *>(workspace), st),
+    return hip_status(tsattn::launch_mfma_f32_backward(
+                          pr, vq, vk, vv, vo, vg, static_cast<const float *>(lse), vdq, vdk, vdv,
+                          static_cast<float *>(workspace),
+                          reinterpret_cast<float *>(static_cast<char *>(workspace) + parts_off), st),
                       "fp32 mfma backward launch");
   }
   if (win.given) return window_unsupported();
@@ -836,7 +842,9 @@ size_t tsattn_window_backward_workspace(const tsattn_problem *p, int64_t window,
   tsattn::Problem pr;
   if (check_window(p, window, sinks, &pr)) return 0;
   const size_t base = rope ? rope_rows_workspace(pr) : rows_workspace(p);
-  const size_t parts = tsattn::mfma_supported(pr, p->dtype) ? tsattn::mfma_window_bytes(pr) : 0;
+  const size_t parts = tsattn::mfma_supported(pr, p->dtype)       ? tsattn::mfma_window_bytes(pr)
+                       : tsattn::mfma_f32_supported(pr, p->dtype) ? tsattn::mfma_f32_window_bytes(pr)
+                                                                  : 0;
   return parts ? round256(base) + parts : base;
 }
 

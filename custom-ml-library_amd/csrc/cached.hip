@@ -50,13 +50,18 @@ struct CachedArgs {
 
 template <typename T, int D>
 constexpr int kPair = 2 * BN * D * (std::is_same_v<T, float> ? 4 : 2);  // bytes of a K and a V tile
-// Waves of a workgroup, WR of them sharing each tile; up to 32 rows (WR 1) as many as 64
-// KiB of tiles allow, two workgroups a CU.
+// Waves of a workgroup, WR of them sharing each tile.  Up to 32 rows (WR 1) a wave has
+// room for one K and one V tile, so that 8 waves of 128 channels share a CU.  A tile's
+// steps follow each other in a wave: with more room and 4 waves the step below took 97 us
+// whether 3 or 4 of its tiles were in flight, 5.6 TB/s.
 template <typename T, int D, int WR>
-constexpr int kWaves = WR > 1 ? WR : (kPair<T, D> <= 8192 ? 4 : 2);
-// Ring stages: WR > 1 and DMA: three.
-template <bool Q8, int WR>
-constexpr int kStages = WR > 1 && !Q8 ? 3 : 2;
+constexpr int kWaves = WR > 1 ? WR : (kPair<T, D> <= 16384 ? 4 : 2);
+// Waves a SIMD that the registers must leave room for.
+template <typename T, int D>
+constexpr int kTwo = kPair<T, D> <= 16384 ? 2 : 1;
+// Ring stages of a K and a V tile for several waves: three, or two of widened codes.
+template <bool Q8>
+constexpr int kStages = Q8 ? 2 : 3;
 
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
@@ -73,19 +78,55 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
   return y;
 }
 
+// 16-bit K / V tiles in LDS, 32 rows of D, row-major, 16-byte chunk k of row r at k ^
+// sw(r).  One DMA instruction fetches whole rows (of 256 bytes four: 16 rows' quarters,
+// the prefill kernel's blocks, left HBM at 5.5 TB/s).  16 rows' same chunk, and 4 rows'
+// 4 chunks beside each other (the transposing reads), lie in different banks.
+template <typename T, int D>
+struct RowTile {
+  static constexpr int RPB = 1024 / (2 * D);  // rows a DMA block
+  __device__ __forceinline__ static constexpr int sw(int r) {
+    return D >= 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : D == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : (r >> 2) & 3;
+  }
+  __device__ __forceinline__ static int at(int r, int k) { return r * 2 * D + ((k ^ sw(r)) << 4); }
+  // of the block's first row: what lane l fetches for its 16 bytes at 16 l of block n
+  __device__ __forceinline__ static uint32_t dma_off(int n, int lane, uint32_t stride) {
+    const int rr = lane / (D / 8), k = lane % (D / 8);
+    return static_cast<uint32_t>(rr) * stride + static_cast<uint32_t>((k ^ sw(n * RPB + rr)) << 4);
+  }
+  int krow, kchunk, vrow, vlo, vhi;
+  __device__ __forceinline__ explicit RowTile(int lane) {
+    const int c = lane & 31, h = lane >> 5, i = lane & 15, sel = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    const int r = 4 * h + (i >> 2);
+    krow = c * 2 * D, kchunk = (h ^ sw(c)) << 4;
+    vrow = r * 2 * D + (i & 1) * 8, vlo = (sel ^ sw(r)) << 4, vhi = (sel ^ sw(r + 8)) << 4;
+  }
+  // row c, channels 16 i + 8 h .. + 7
+  __device__ __forceinline__ u32x4 rows(const char *tile, int i) const {
+    return ld16(tile + krow + (kchunk ^ (i << 5)));
+  }
+  // channel 32 dt + c at rows 16 ks + 4 h .. + 3 and 8 further on
+  __device__ __forceinline__ u32x4 cols(const char *tile, int ks, int dt) const {
+    const char *t = tile + vrow + ks * 32 * D;
+    const u32x2 a = ds_read_tr<T>(reinterpret_cast<const T *>(t + (vlo ^ (dt << 6))));
+    const u32x2 b = ds_read_tr<T>(reinterpret_cast<const T *>(t + 16 * D + (vhi ^ (dt << 6))));
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+};
+
 template <typename T, int D, bool Q8, int WR>
-__global__ __launch_bounds__((64 * kWaves<T, D, WR>)) void cached_kernel(CachedArgs a) {
+__global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<T, D>)) void cached_kernel(CachedArgs a) {
   constexpr bool F32 = std::is_same_v<T, float>;
   static_assert(!F32 || (!Q8 && D <= 128), "fp32 caches are not quantised, of up to 128 channels");
   using PT = std::conditional_t<Q8, bf16, T>;  // the value tiles
   constexpr int NP = Q8 && std::is_same_v<T, f16> ? 2 : 1;  // parts of P
-  constexpr int NWV = kWaves<T, D, WR>, WK = NWV / WR, NS = kStages<Q8, WR>;
+  constexpr int NWV = kWaves<T, D, WR>, WK = NWV / WR, NS = kStages<Q8>;
   constexpr int PAIR = kPair<T, D>, TILE = PAIR / 2;
   constexpr int BLK = TILE / 1024;             // 1 KiB DMA blocks a tile
   constexpr int LPT = (2 * BLK + WR - 1) / WR;  // DMA loads a wave issues for a pair (WR > 1)
-  constexpr int QG = D / 32, PDT = D / 32;
+  constexpr int PDT = D / 32;
   constexpr int SCALES = Q8 ? 256 : 0;
-  constexpr int STAGE = PAIR + SCALES, RING = NS * STAGE;
+  constexpr int STAGE = PAIR + SCALES, RING = WR == 1 && !Q8 ? PAIR : NS * STAGE;
   constexpr int MERGE = WK > 1 ? NWV * 32 * (D + 2) * 4 : 0;
   constexpr int LDS_B = WK * RING > MERGE ? WK * RING : MERGE;
   static_assert(WR == 1 || (2 * BLK) % WR == 0 || Q8, "a pair's blocks split over the waves");
@@ -182,8 +223,8 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>)) void cached_kernel(CachedA
   char *ring = lds + wk * RING;
   const uint32_t ring0 = lds_addr(lds) + wk * RING;
 
-  using Reader = std::conditional_t<F32, TileReader<bf16, 32>, TileReader<std::conditional_t<F32, bf16, T>, D>>;
-  const Reader rd(lane);
+  using Rows = RowTile<std::conditional_t<F32, bf16, T>, D>;
+  const Rows rd(lane);
   // S^T of a K tile: element i is key crow(i, h)
   auto scores = [&](const char *kt) __attribute__((always_inline)) {
     f32x16 s = f32x16{};
@@ -199,7 +240,7 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>)) void cached_kernel(CachedA
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) s = mfma32<T>(rd.rows(kt, 0, i), qf[i], s);
+      for (int i = 0; i < NQ; ++i) s = mfma32<T>(rd.rows(kt, i), qf[i], s);
     }
     return s;
   };
@@ -288,50 +329,37 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>)) void cached_kernel(CachedA
     // Keys past the cache's end, and tiles past the wave's last, read as zeros.
     const u32x4 kdesc = make_desc(kbase, static_cast<uint32_t>(a.n) * ks_b);
     const u32x4 vdesc = make_desc(vbase, static_cast<uint32_t>(a.n) * vs_b);
-    const uint32_t chunk = (lane & 3) ^ ((lane >> 4) & 3);
-    const uint32_t koff = (lane >> 2) * ks_b + chunk * 16, voff = (lane >> 2) * vs_b + chunk * 16;
     // block n of a K or V tile whose first row is at byte `base`, to LDS address st
-    auto block = [&](u32x4 desc, uint32_t off, uint32_t stride, uint32_t base, uint32_t st, int n)
-                     __attribute__((always_inline)) {
-      if constexpr (F32)
-        dma16(desc, st + n * 1024, FTile<D>::dma_off(n, lane, stride), base + static_cast<uint32_t>(n * FTile<D>::RPB) * stride);
-      else
-        dma16(desc, st + n * 1024, off, base + static_cast<uint32_t>(16 * (n / QG)) * stride + (n % QG) * 64);
+    auto block = [&](u32x4 desc, uint32_t stride, uint32_t base, uint32_t st, int n) __attribute__((always_inline)) {
+      using Tile = std::conditional_t<F32, FTile<D>, Rows>;
+      dma16(desc, st + n * 1024, Tile::dma_off(n, lane, stride), base + static_cast<uint32_t>(n * Tile::RPB) * stride);
     };
     auto first_row = [&](int i, uint32_t stride) __attribute__((always_inline)) {
       return i < mine ? static_cast<uint32_t>(key0(i)) * stride : 0x80000000u;
     };
     if constexpr (WR == 1) {
-      // K of a tile is issued once its stage's last K has been read, V likewise: of
-      // the stages' four tiles three are in flight while one is read.
-      auto issue_k = [&](int i) __attribute__((always_inline)) {
-        const uint32_t base = first_row(i, ks_b), st = ring0 + (i & 1) * STAGE;
+      auto issue = [&](u32x4 desc, uint32_t stride, int i, uint32_t st) __attribute__((always_inline)) {
+        const uint32_t base = first_row(i, stride);
 #pragma unroll
-        for (int n = 0; n < BLK; ++n) block(kdesc, koff, ks_b, base, st, n);
+        for (int n = 0; n < BLK; ++n) block(desc, stride, base, st, n);
       };
-      auto issue_v = [&](int i) __attribute__((always_inline)) {
-        const uint32_t base = first_row(i, vs_b), st = ring0 + (i & 1) * STAGE + TILE;
-#pragma unroll
-        for (int n = 0; n < BLK; ++n) block(vdesc, voff, vs_b, base, st, n);
-      };
-      issue_k(0);
-      issue_v(0);
-      issue_k(1);
+      issue(kdesc, ks_b, 0, ring0);
+      issue(vdesc, vs_b, 0, ring0 + TILE);
       for (int i = 0; i < mine; ++i) {
-        const char *kt = ring + (i & 1) * STAGE, *vt = kt + TILE;
-        wait_vm_n<2 * BLK>();  // K of tile i; its V and the next K in flight
+        wait_vm_n<BLK>();  // K of tile i; V in flight
         __builtin_amdgcn_sched_barrier(0);
-        const f32x16 s = scores(kt);
+        const f32x16 s = scores(ring);
+        wait_lgkm0();  // read
         __builtin_amdgcn_sched_barrier(0);
-        issue_v(i + 1);
+        issue(kdesc, ks_b, i + 1, ring0);
         softmax(s, key0(i), nullptr);
         __builtin_amdgcn_sched_barrier(0);
-        wait_vm_n<2 * BLK>();  // V of tile i; the next K and V in flight
+        wait_vm_n<BLK>();  // V of tile i; the next K in flight
         __builtin_amdgcn_sched_barrier(0);
-        values(vt);
-        wait_lgkm0();  // both tiles read
+        values(ring + TILE);
+        wait_lgkm0();
         __builtin_amdgcn_sched_barrier(0);
-        issue_k(i + 2);
+        issue(vdesc, vs_b, i + 1, ring0 + TILE);
       }
       wait_vm_n<0>();
     } else {
@@ -341,8 +369,8 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>)) void cached_kernel(CachedA
 #pragma unroll
         for (int u = 0; u < LPT; ++u) {
           const int n = w + WR * u;
-          if (n < BLK) block(kdesc, koff, ks_b, kb, st, n);
-          else block(vdesc, voff, vs_b, vb, st + TILE, n - BLK);
+          if (n < BLK) block(kdesc, ks_b, kb, st, n);
+          else block(vdesc, vs_b, vb, st + TILE, n - BLK);
         }
       };
       issue(0);
@@ -391,7 +419,7 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>)) void cached_kernel(CachedA
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int k = ch + e;
-          char *to = st + ((r >> 4) * QG + (k >> 2)) * 1024 + 16 * (4 * (r & 15) + ((k & 3) ^ ((r >> 2) & 3)));
+          char *to = st + Rows::at(r, k);
           *reinterpret_cast<u32x4 *>(to) = widen<T>(kc[u][2 * e], kc[u][2 * e + 1]);
           *reinterpret_cast<u32x4 *>(to + TILE) = widen<PT>(vc[u][2 * e], vc[u][2 * e + 1]);
         }
@@ -610,10 +638,11 @@ CachedPlan plan_cached(const CachedProblem &p) {
   s.ns = sunk < first ? sunk : first;
   s.gap = first - s.ns;
   s.run = tiles - s.gap;
-  // two workgroups a CU, each of 4 tiles a wave or more
+  // two workgroups a CU (of small tiles four), each of 4 tiles a wave or more
   const int64_t base = static_cast<int64_t>(p.B) * p.Hkv * s.groups;
-  const int least = 4 * (s.wr > 1 ? 1 : 2);
-  int64_t n = 512 / base;
+  const int pair = 64 * p.D * (p.dtype == TSATTN_F32 ? 4 : 2);
+  const int least = 4 * (s.wr > 1 ? 1 : pair <= 16384 ? 4 : 2);
+  int64_t n = (pair <= 8192 ? 1024 : 512) / base;
   if (n > s.run / least) n = s.run / least;
   s.splits = n < 1 ? 1 : static_cast<int>(n);
   return s;

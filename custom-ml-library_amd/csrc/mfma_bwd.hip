@@ -938,36 +938,37 @@ __global__ __launch_bounds__(NT, (dkdv_wg_per_cu<DK, DV, MK, DR>())) void dkdv_k
   }
 }
 
-// Window: the parts of a sinks' key block, added up in their order; workgroup and lanes
-// hold what the dK/dV kernel's do.
+// Window: the parts of a sinks' key block, added up in their order.  A workgroup takes
+// four of the accumulator registers, its lanes what the dK/dV kernel's hold of them:
+// bound by reading the parts (8 groups, 7 parts of 128 KiB: 4 us; all registers in one
+// workgroup took 64).
 template <typename T, int DK, int DV>
 __global__ __launch_bounds__(NT) void sink_sum_kernel(BwdArgs a) {
   constexpr int REGS = DK / 2 + DV / 2;
   const Problem &p = a.p;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, w = threadIdx.x >> 6;
-  const int bh = blockIdx.x / a.sink_blocks, kb = blockIdx.x % a.sink_blocks;
+  const int g = blockIdx.x % (REGS / 4), unit = blockIdx.x / (REGS / 4);
+  const int bh = unit / a.sink_blocks, kb = unit % a.sink_blocks;
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv, key = kb * KB + 32 * w + c;
-  const float *from = a.part + ((static_cast<int64_t>(blockIdx.x) * a.parts * NW + w) * REGS) * 64 + lane;
-  T *rows[2] = {mut<T>(a.dk) + b * a.dk.s0 + hk * a.dk.s1 + static_cast<int64_t>(key) * a.dk.s2,
-                mut<T>(a.dv) + b * a.dv.s0 + hk * a.dv.s1 + static_cast<int64_t>(key) * a.dv.s2};
-  // register 16 dt + 4 g + r is channel 32 dt + 8 g + 4 h + r of the lane's key
-  for (int g = 0; g < REGS / 4; ++g) {
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.parts; ++i)
+  const float *from = a.part + ((static_cast<int64_t>(unit) * a.parts * NW + w) * REGS + 4 * g) * 64 + lane;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < a.parts; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] += from[(static_cast<int64_t>(i) * NW * REGS + 4 * g + r) * 64];
-    if (key >= p.Sk) continue;
-    const bool is_k = g < DK / 8;
-    const int d = 8 * (is_k ? g : g - DK / 8) + 4 * h;
-    const float f = is_k ? a.scale : 1.f;
-    u32x2 y{pack2<T>(x[0] * f, x[1] * f), pack2<T>(x[2] * f, x[3] * f)};
-    if (is_k && d < p.rope.R) {  // (R is a multiple of 8)
-      const int64_t at = (p.rope.kpos0 + key) * (p.rope.R / 2) + d / 2;
-      const T *cs = static_cast<const T *>(p.rope.cos) + at, *sn = static_cast<const T *>(p.rope.sin) + at;
-      y = u32x2{rotate_word<T>(y[0], cs[0], sn[0], true), rotate_word<T>(y[1], cs[1], sn[1], true)};
-    }
-    *reinterpret_cast<u32x2 *>(rows[is_k ? 0 : 1] + d) = y;
+    for (int r = 0; r < 4; ++r) x[r] += from[(static_cast<int64_t>(i) * NW * REGS + r) * 64];
+  if (key >= p.Sk) return;
+  // register 16 dt + 4 g + r is channel 32 dt + 8 g + 4 h + r of the lane's key
+  const bool is_k = g < DK / 8;
+  const int d = 8 * (is_k ? g : g - DK / 8) + 4 * h;
+  const float f = is_k ? a.scale : 1.f;
+  u32x2 y{pack2<T>(x[0] * f, x[1] * f), pack2<T>(x[2] * f, x[3] * f)};
+  if (is_k && d < p.rope.R) {  // (R is a multiple of 8)
+    const int64_t at = (p.rope.kpos0 + key) * (p.rope.R / 2) + d / 2;
+    const T *cs = static_cast<const T *>(p.rope.cos) + at, *sn = static_cast<const T *>(p.rope.sin) + at;
+    y = u32x2{rotate_word<T>(y[0], cs[0], sn[0], true), rotate_word<T>(y[1], cs[1], sn[1], true)};
   }
+  const View &o = is_k ? a.dk : a.dv;
+  *reinterpret_cast<u32x2 *>(mut<T>(o) + b * o.s0 + hk * o.s1 + static_cast<int64_t>(key) * o.s2 + d) = y;
 }
 
 // ---------------------------------------------------------------------------
@@ -1790,7 +1791,7 @@ void launch_window(const BwdArgs &a, hipStream_t st) {
   }
   if (a.sink_blocks && a.parts > 1) {
     Probe pr_("bwd_sink_sum", st);
-    sink_sum_kernel<T, DK, DV><<<dim3(a.sink_blocks * a.ng), dim3(NT), 0, st>>>(a);
+    sink_sum_kernel<T, DK, DV><<<dim3(a.sink_blocks * a.ng * (DK + DV) / 8), dim3(NT), 0, st>>>(a);
   }
 }
 

@@ -10,8 +10,8 @@
 // The matrix instruction's lanes and the tiles' layout in LDS: f32_tile.h.
 //
 // Windows (template WIN) as in the 16-bit kernels: the forward and dQ walk the run of
-// key tiles that their rows see, dK/dV the query rows that see its keys (all rows for the
-// sinks' keys, one chain here: fp32 sequences are the short ones).
+// key tiles that their rows see, dK/dV the query rows that see its keys; the sinks' key
+// blocks, which all rows see, are cut into parts.
 //
 // Masks (template MK): 0 = none, or a [B,1,1,K] key mask reduced to kv_len /
 // kv_prefix; 1 = any other boolean mask; 2 / 3 = an additive f32 / (f16 or
@@ -240,6 +240,10 @@ struct F32Args {
   int lse_scaled;
   float sl;     // scale * log2(e)
   float scale;
+  // window: the key blocks with sinks, the parts of each one's query rows, and their
+  // partial dK | dV rows (mfma_bwd.hip)
+  int sink_blocks, parts;
+  float *part;
 };
 
 // ---------------------------------------------------------------------------
@@ -985,10 +989,22 @@ __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n_kb = (p.Sk + KEYS - 1) / KEYS;
-  const int total = n_kb * p.Hkv * p.B;
+  const int sunk = WIN ? a.sink_blocks * a.parts : 0;
+  const int n_units = WIN ? sunk + n_kb - a.sink_blocks : n_kb;
+  const int total = n_units * p.Hkv * p.B;
   const int logical = xcd_remap(blockIdx.x, total);
   int bh, kb;
-  heavy_first(logical, n_kb, p.Hkv * p.B, 32, bh, kb);
+  heavy_first(logical, n_units, p.Hkv * p.B, 32, bh, kb);
+  int part = 0, parts = 1;
+  if constexpr (WIN) {
+    if (kb < sunk) {
+      parts = a.parts;
+      part = kb % parts;
+      kb /= parts;
+    } else {
+      kb += a.sink_blocks - sunk;
+    }
+  }
   const int b = bh / p.Hkv, hk = bh - b * p.Hkv;
   const int k0 = kb * KEYS, kw = SPLIT ? k0 : k0 + 32 * w, key = kw + c;
   const int kv_end = kv_end_for(p, b);
@@ -1010,6 +1026,9 @@ __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
     };
     if (key >= p.sinks) kwin = end(key);
     if (k0 >= p.sinks) q_stop = max(q_start, min(p.Sq, end(k0 + KEYS - 1)));
+    const int tiles = (q_stop - q_start + BN - 1) / BN;
+    q_stop = min(q_stop, q_start + BN * static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / parts));
+    q_start += BN * static_cast<int>(static_cast<int64_t>(tiles) * part / parts);
   }
   const int n_qt = __builtin_amdgcn_readfirstlane(k0 < kv_end ? (q_stop - q_start + BN - 1) / BN : 0);
   const int n_iter = __builtin_amdgcn_readfirstlane(n_qt * p.rep);
@@ -1224,7 +1243,14 @@ __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
                 static_cast<int64_t>(krow_i) * a.dk.s2;
   float *vrow = static_cast<float *>(const_cast<void *>(a.dv.data)) + b * a.dv.s0 + hk * a.dv.s1 +
                 static_cast<int64_t>(krow_i) * a.dv.s2;
-  const float sc = a.scale;
+  float sc = a.scale;
+  if constexpr (WIN) {
+    if (parts > 1) {
+      krow = a.part + (((static_cast<int64_t>(bh) * a.sink_blocks + kb) * parts + part) * KEYS + (key - k0)) * 2 * D;
+      vrow = krow + D;
+      sc = 1.f;
+    }
+  }
   if constexpr (!SPLIT) {
     if (key < p.Sk) {
 #pragma unroll
@@ -1269,8 +1295,42 @@ __global__ __launch_bounds__(NT, 1) void dkdv_f32_kernel(F32Args a) {
   }
 }
 
+// Window: the parts of the sinks' key blocks (`keys` keys each), added up in their order:
+// a thread four channels of a key.
+template <int D>
+__global__ __launch_bounds__(NT) void sink_sum_f32_kernel(F32Args a, int keys) {
+  const Problem &p = a.p;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * NT + threadIdx.x;
+  const int per = keys * 2 * D / 4, unit = static_cast<int>(at / per), in = static_cast<int>(at % per);
+  const int bh = unit / a.sink_blocks, key = unit % a.sink_blocks * keys + in / (2 * D / 4);
+  if (bh >= p.B * p.Hkv || key >= p.Sk) return;
+  const float4 *from = reinterpret_cast<const float4 *>(a.part) + static_cast<int64_t>(unit) * a.parts * per + in;
+  float4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < a.parts; ++i) {
+    const float4 y = from[static_cast<int64_t>(i) * per];
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+  }
+  const int d = in % (2 * D / 4) * 4, b = bh / p.Hkv, hk = bh - b * p.Hkv;
+  const bool is_k = d < D;
+  const View &o = is_k ? a.dk : a.dv;
+  const float f = is_k ? a.scale : 1.f;
+  *reinterpret_cast<float4 *>(static_cast<float *>(const_cast<void *>(o.data)) + b * o.s0 + hk * o.s1 +
+                              static_cast<int64_t>(key) * o.s2 + (is_k ? d : d - D)) =
+      float4{x.x * f, x.y * f, x.z * f, x.w * f};
+}
+
+// Key blocks of `keys` keys with sinks, and the parts of each (as mfma_bwd.hip's).
+int window_blocks(const Problem &p, int keys) { return min((p.sinks + keys - 1) / keys, (p.Sk + keys - 1) / keys); }
+int window_parts(const Problem &p, int keys) {
+  const int64_t all = (p.Sq + BN - 1) / BN, other = (keys + static_cast<int64_t>(p.window)) / BN + 1;
+  const int64_t parts = (all + other - 1) / other;
+  return static_cast<int>(parts < 64 ? parts : 64);
+}
+
 template <int D, int MK, bool WIN>
-void launch_bwd_dims(const F32Args &a, hipStream_t st) {
+void launch_bwd_dims(const F32Args &a0, hipStream_t st) {
+  F32Args a = a0;
   const Problem &p = a.p;
   {
     Probe pr_("bwd_rows_f32", st);
@@ -1285,6 +1345,12 @@ void launch_bwd_dims(const F32Args &a, hipStream_t st) {
     split_q = n_qb * qheads < device_cus();
     split_k = n_kb * kheads < device_cus();
   }
+  const int keys = split_k ? 32 : KB;
+  if constexpr (WIN) {
+    a.sink_blocks = window_blocks(p, keys);
+    a.parts = a.sink_blocks ? window_parts(p, keys) : 1;
+  }
+  const int more = WIN ? a.sink_blocks * (a.parts - 1) : 0;  // units of the sinks' blocks beyond their own
   if (split_q) {
     if constexpr (D <= 64) {
       Probe pr_(WIN ? "bwd_dq_mfma_f32_window_split" : MK ? "bwd_dq_mfma_f32_masked_split" : "bwd_dq_mfma_f32_split", st);
@@ -1297,11 +1363,18 @@ void launch_bwd_dims(const F32Args &a, hipStream_t st) {
   if (split_k) {
     if constexpr (D <= 64) {
       Probe pr_(WIN ? "bwd_dkdv_mfma_f32_window_split" : MK ? "bwd_dkdv_mfma_f32_masked_split" : "bwd_dkdv_mfma_f32_split", st);
-      dkdv_f32_kernel<D, true, MK, WIN><<<dim3(static_cast<unsigned>((p.Sk + 31) / 32 * kheads)), dim3(NT), 0, st>>>(a);
+      dkdv_f32_kernel<D, true, MK, WIN><<<dim3(static_cast<unsigned>(((p.Sk + 31) / 32 + more) * kheads)), dim3(NT), 0, st>>>(a);
     }
   } else {
     Probe pr_(WIN ? "bwd_dkdv_mfma_f32_window" : MK ? "bwd_dkdv_mfma_f32_masked" : "bwd_dkdv_mfma_f32", st);
-    dkdv_f32_kernel<D, false, MK, WIN><<<dim3(static_cast<unsigned>(n_kb * kheads)), dim3(NT), 0, st>>>(a);
+    dkdv_f32_kernel<D, false, MK, WIN><<<dim3(static_cast<unsigned>((n_kb + more) * kheads)), dim3(NT), 0, st>>>(a);
+  }
+  if constexpr (WIN) {
+    if (more) {
+      Probe pr_("bwd_sink_sum_f32", st);
+      const int64_t n = kheads * a.sink_blocks * keys * 2 * D / 4;
+      sink_sum_f32_kernel<D><<<dim3(static_cast<unsigned>((n + NT - 1) / NT)), dim3(NT), 0, st>>>(a, keys);
+    }
   }
 }
 
@@ -1336,10 +1409,23 @@ void launch_bwd_mask(const F32Args &a, hipStream_t st) {
 
 }  // namespace
 
+size_t mfma_f32_window_bytes(const Problem &p) {
+  if (!p.window || !p.sinks) return 0;
+  size_t most = 0;
+  for (const int keys : {32, KB}) {  // (which of the two runs is the launch's choice)
+    const int parts = window_parts(p, keys);
+    const size_t n = parts < 2 ? 0 : static_cast<size_t>(p.B) * p.Hkv * window_blocks(p, keys) * parts * keys * 2 * p.Dqk;
+    most = n > most ? n : most;
+  }
+  return most * sizeof(float);
+}
+
 hipError_t launch_mfma_f32_backward(const Problem &p, View q, View k, View v, View o, View dout,
-                                    const float *lse, View dq, View dk, View dv, float *rows,
+                                    const float *lse, View dq, View dk, View dv, float *rows, float *parts,
                                     hipStream_t st) {
   F32Args a{};
+  a.parts = 1;
+  a.part = parts;
   a.p = p;
   a.q = q, a.k = k, a.v = v, a.o = o, a.dout = dout, a.dq = dq, a.dk = dk, a.dv = dv;
   a.lse = const_cast<float *>(lse);

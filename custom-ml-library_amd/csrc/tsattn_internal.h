@@ -250,9 +250,11 @@ size_t mfma_window_bytes(const Problem &p);
 bool mfma_f32_supported(const Problem &p, int dtype);
 hipError_t launch_mfma_f32_forward(const Problem &p, View q, View k, View v, View o, float *lse,
                                    hipStream_t st);
-// rows: the backward workspace's row values (2 B Hq Sq floats).
+// rows: the backward workspace's row values (2 B Hq Sq floats).  parts: with a window
+// mfma_f32_window_bytes(p) bytes for the sinks' partial sums (0: not needed).
+size_t mfma_f32_window_bytes(const Problem &p);
 hipError_t launch_mfma_f32_backward(const Problem &p, View q, View k, View v, View o, View dout,
-                                    const float *lse, View dq, View dk, View dv, float *rows,
+                                    const float *lse, View dq, View dk, View dv, float *rows, float *parts,
                                     hipStream_t st);
 
 // Split-K decode.

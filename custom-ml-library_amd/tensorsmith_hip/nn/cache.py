@@ -261,8 +261,11 @@ class KVCache:
         keys = self._keys[:, :, part]
         values = self._values[:, :, part]
         if self.quantized:
-            keys = (keys.float() * self._key_scales[:, :, part]).to(self.dtype)
-            values = (values.float() * self._value_scales[:, :, part]).to(self.dtype)
+            import torch
+
+            # (one kernel each: the product in float32, rounded to the dtype as it is stored)
+            keys, values = (torch.mul(x, s[:, :, part], out=torch.empty(x.shape, dtype=self.dtype, device=x.device))
+                            for x, s in ((keys, self._key_scales), (values, self._value_scales)))
         return Tensor(keys, device=self.device), Tensor(values, device=self.device)
 
     def reset(self) -> None:
