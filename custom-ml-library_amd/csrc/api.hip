@@ -1048,12 +1048,15 @@ int tsattn_draft_tree(int32_t trees, int32_t len, const int32_t *parents, uint32
 }
 
 int tsattn_cache_keep(int32_t batch, int32_t heads, int32_t n, int64_t first, int64_t limit, const void *index,
-                      int32_t index_bytes, int32_t key_bytes, int32_t value_bytes, const tsattn_view *k,
-                      const tsattn_view *v, const tsattn_view *k_scale, const tsattn_view *v_scale, void *stream) {
+                      int32_t index_bytes, int32_t element_bytes, int32_t dim_qk, int32_t dim_v,
+                      const tsattn_view *k, const tsattn_view *v, const tsattn_view *k_scale,
+                      const tsattn_view *v_scale, void *stream) {
   int rc;
-  if (batch <= 0 || heads <= 0 || n <= 0 || first < 0 || limit < n || key_bytes <= 0 || value_bytes <= 0)
+  if (batch <= 0 || heads <= 0 || n <= 0 || first < 0 || limit < n || dim_qk <= 0 || dim_v <= 0)
     return fail(TSATTN_ERR_INVALID, "kept rows need positive sizes, no more of them than there are");
   if (n > 256) return fail(TSATTN_ERR_UNSUPPORTED, "at most 256 rows are kept (got %d)", n);
+  if (element_bytes != 1 && element_bytes != 2 && element_bytes != 4 && element_bytes != 8)
+    return fail(TSATTN_ERR_INVALID, "cached elements have 1, 2, 4 or 8 bytes");
   if (!index || (index_bytes != 4 && index_bytes != 8)) return fail(TSATTN_ERR_INVALID, "indexes are int32 or int64");
   if ((rc = check_view(k, "key cache")) || (rc = check_view(v, "value cache"))) return rc;
   if (!k_scale != !v_scale)
@@ -1064,9 +1067,9 @@ int tsattn_cache_keep(int32_t batch, int32_t heads, int32_t n, int64_t first, in
   for (int i = 0; i < 4; ++i) {
     if (!views[i]) continue;
     a.data[i] = static_cast<char *>(views[i]->data);
-    const int64_t unit = i < 2 ? 1 : static_cast<int64_t>(sizeof(float));
+    const int64_t unit = i < 2 ? element_bytes : static_cast<int64_t>(sizeof(float));
     a.s0[i] = views[i]->stride[0] * unit, a.s1[i] = views[i]->stride[1] * unit, a.s2[i] = views[i]->stride[2] * unit;
-    a.bytes[i] = i == 0 ? key_bytes : i == 1 ? value_bytes : static_cast<int>(sizeof(float));
+    a.bytes[i] = (i == 0 ? dim_qk : i == 1 ? dim_v : 1) * static_cast<int>(unit);
   }
   a.B = batch, a.H = heads, a.n = n, a.first = first, a.limit = limit, a.index = index, a.index_bytes = index_bytes;
   return hip_status(tsattn::launch_keep(a, static_cast<hipStream_t>(stream)), "cache rows launch");

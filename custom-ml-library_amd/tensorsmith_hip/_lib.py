@@ -248,8 +248,8 @@ SIGNATURES = {
     ),
     "tsattn_cache_keep": (
         c_int,
-        [c_int32, c_int32, c_int32, c_int64, c_int64, c_void_p, c_int32, c_int32, c_int32, _PV, _PV, _PV, _PV,
-         c_void_p],
+        [c_int32, c_int32, c_int32, c_int64, c_int64, c_void_p, c_int32, c_int32, c_int32, c_int32, _PV, _PV, _PV,
+         _PV, c_void_p],
     ),
     "tsattn_cached_attend_workspace": (c_size_t, [POINTER(Cached)]),
     "tsattn_cached_attend": (

@@ -49,11 +49,9 @@ def _operand(t):
 def _view(t) -> _lib.View:
     v = _lib.View()
     v.data = t.data_ptr()
-    st = list(t.stride())
-    if t.shape[-1] == 1:
-        st[-1] = 1
-    for i, s in enumerate(st):
-        v.stride[i] = s
+    v.stride[:] = t.stride()
+    if t.shape[3] == 1:
+        v.stride[3] = 1
     return v
 
 

@@ -61,6 +61,7 @@ class KVCache:
         self._key_scales = torch.ones(shape + (1,), dtype=torch.float32, device=dev) if quantized else None
         self._value_scales = (torch.ones(shape + (1,), dtype=torch.float32, device=dev)
                               if quantized else None)
+        self._described: tuple = ()
 
     def append(self, key: Tensor, value: Tensor) -> tuple[Tensor, Tensor]:
         """Append a chunk after validating all shapes and capacity."""
@@ -140,10 +141,9 @@ class KVCache:
             cos, sin = (x.data_ptr() for x in rope_tables(rotary_base, self.head_dim, self.dtype, self._keys.device, stop))
         k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (key._data, value._data))
         b, h, t, d = k.shape
-        scales = (_view(self._key_scales), _view(self._value_scales)) if self.quantized else (None, None)
         _lib.check(launch(self.device, _lib.load().tsattn_draft_append, _CODES[str(k.dtype)], b, h, t, d, _view(k),
-                          _view(v), _view(self._keys), _view(self._values), *scales, cos, sin, self.length,
-                          tree._depths.data_ptr(), tree.trees), "draft append")
+                          _view(v), *self._views(), cos, sin, self.length, tree._depths.data_ptr(), tree.trees),
+                   "draft append")
         self.length = stop
 
     def keep(self, first: int, index) -> None:
@@ -173,18 +173,9 @@ class KVCache:
         if n:
             raw = index._data if index._data.dtype in (torch.int64, torch.int32) else index._data.long()
             raw = raw.contiguous()
-
-            def rows(x):  # in bytes
-                view = _view(x)
-                for i in range(3):
-                    view.stride[i] *= x.element_size()
-                return view, x.shape[-1] * x.element_size()
-
-            (keys, key_bytes), (values, value_bytes) = rows(self._keys), rows(self._values)
-            scales = (_view(self._key_scales), _view(self._value_scales)) if self.quantized else (None, None)
             _lib.check(launch(self.device, _lib.load().tsattn_cache_keep, self.batch_size, self.num_heads, n, first,
-                              drafted, raw.data_ptr(), raw.element_size(), key_bytes, value_bytes, keys, values,
-                              *scales), "cache rows")
+                              drafted, raw.data_ptr(), raw.element_size(), self._keys.element_size(), self.head_dim,
+                              self.value_dim, *self._views()), "cache rows")
         self.length = first + n
 
     def _project_append(self, input: Tensor, projections, num_heads: int, rotary: bool,
@@ -266,7 +257,7 @@ class KVCache:
             # (one kernel each: the product in float32, rounded to the dtype as it is stored)
             keys, values = (torch.mul(x, s[:, :, part], out=torch.empty(x.shape, dtype=self.dtype, device=x.device))
                             for x, s in ((keys, self._key_scales), (values, self._value_scales)))
-        return Tensor(keys, device=self.device), Tensor(values, device=self.device)
+        return Tensor._leaf(keys, self.device), Tensor._leaf(values, self.device)
 
     def reset(self) -> None:
         """Reuse the allocation; future appends overwrite old entries."""
@@ -292,6 +283,12 @@ class KVCache:
         if self.quantized:
             self._key_scales = self._key_scales[order]
             self._value_scales = self._value_scales[order]
+
+    def _views(self) -> tuple:
+        """The library's views of the arrays (which ``reorder`` replaces), the scales' None without them."""
+        if not self._described or self._described[0] is not self._keys:
+            self._described = (self._keys, tuple(None if x is None else _view(x) for x in self.storage))
+        return self._described[1]
 
     @property
     def storage(self) -> tuple:

@@ -80,7 +80,7 @@ class DraftTree:
     def _check(self, batch: int, tokens: int, dev) -> None:
         if tokens != self.tokens or self.trees not in (1, batch):
             raise ValueError("the tree does not match the drafted tokens")
-        if dev != self.device:
+        if dev is not self.device and dev != self.device:
             raise ValueError("the tree must be on the device of its tokens")
 
     def __repr__(self):
@@ -116,15 +116,16 @@ def cached_attention(query: Tensor, cache: KVCache, tree: DraftTree | None = Non
     a tile with what it does."""
     if not isinstance(cache, KVCache):
         raise TypeError("cached_attention reads a KVCache")
-    if query.ndim != 4:
+    q, dev = query._data, query.device
+    if len(q.shape) != 4:
         raise ValueError("attention expects [batch, heads, sequence, channels]")
-    if query.device != cache.device:
+    if dev is not cache.device and dev != cache.device:
         raise ValueError("attention tensors must be on the same device")
-    if query.dtype != cache.dtype:
+    if q.dtype != cache.dtype:
         raise TypeError("the queries must have the cache's dtype")
-    if is_grad_enabled() and query.requires_grad:
+    if query.requires_grad and is_grad_enabled():
         raise RuntimeError("cached attention is inference-only; use no_grad() for differentiable inputs")
-    b, heads, tokens, dim = query.shape
+    b, heads, tokens, dim = q.shape
     if b != cache.batch_size or dim != cache.head_dim or heads == 0 or heads % cache.num_heads:
         raise ValueError("query shape does not match cache configuration")
     length = cache.length
@@ -136,35 +137,31 @@ def cached_attention(query: Tensor, cache: KVCache, tree: DraftTree | None = Non
     whole = window
     window = _check_window(window, sinks, True, length)
     if tree is not None:
-        tree._check(b, tokens, query.device)
+        tree._check(b, tokens, dev)
         if whole is not None and whole < tokens:
             raise ValueError("the window must hold the drafted tokens")
     import torch
 
-    q = _operand(query._data)
-    desc, code = _lib.Cached(), _dtype_code(q.dtype)
-    desc.dtype, desc.batch, desc.heads_q, desc.heads_kv = code, b, heads, cache.num_heads
-    desc.dim, desc.len, desc.keys, desc.quantized = dim, tokens, length, cache.quantized
-    desc.scale = 1 / math.sqrt(dim) if scale is None else scale
-    if window is not None:
-        desc.window, desc.sinks = window, sinks
-    if tree is not None:
-        desc.trees, desc.words, desc.depths = tree.trees, tree._words.data_ptr(), tree._depths.data_ptr()
+    q, code = _operand(q), _dtype_code(q.dtype)
     if cache.value_dim == dim and code != _lib.F64:
+        cos = sin = words = depths = ws = None
+        trees = 0
+        if tree is not None:
+            trees, words, depths = tree.trees, tree._words.data_ptr(), tree._depths.data_ptr()
         if rotary_base is not None:
-            cos, sin = rope_tables(rotary_base, dim, q.dtype, q.device, length)
-            desc.cos, desc.sin = cos.data_ptr(), sin.data_ptr()
-        keys, values, key_scales, value_scales = cache.storage
-        scales = (_view(key_scales), _view(value_scales)) if cache.quantized else (None, None)
+            cos, sin = (x.data_ptr() for x in rope_tables(rotary_base, dim, q.dtype, q.device, length))
+        desc = _lib.Cached(code, b, heads, cache.num_heads, dim, tokens, length, cache.quantized,
+                           1 / math.sqrt(dim) if scale is None else scale, window or 0, sinks if window else 0, trees,
+                           words, depths, cos, sin)
         lib = _lib.load()
         out = torch.empty((b, heads, tokens, dim), dtype=q.dtype, device=q.device)
         nbytes = lib.tsattn_cached_attend_workspace(desc)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         try:
-            _lib.check(launch(query.device, lib.tsattn_cached_attend, desc, _view(q), _view(keys), _view(values),
-                              *scales, _view(out), None if ws is None else ws.data_ptr(), nbytes),
-                       "cached attention")
-            return Tensor._from_op(out, (query,), None, "cached_attention")
+            _lib.check(launch(dev, lib.tsattn_cached_attend, desc, _view(q), *cache._views(), _view(out),
+                              None if ws is None else ws.data_ptr(), nbytes), "cached attention")
+            return Tensor._leaf(out, dev)
         except NotImplementedError:  # outside the kernel
             pass
     first = length - tokens

@@ -439,64 +439,70 @@ def token_log_probs(input: Tensor, target: Tensor, top_k: int = 0, *, ignore_ind
     A target of ``ignore_index`` is padding: its row is not read and gives 0, 0, -inf and -1, and no gradient.
     Nothing waits for the device, so a target outside the classes is not refused: its log probability is NaN.  So are
     the results of a row that holds a NaN or +inf, or nothing but -inf."""
-    if input.ndim < 1 or input.shape[-1] == 0:
+    x, y = input._data, target._data
+    shape, given = tuple(y.shape), tuple(x.shape)
+    if not given or given[-1] == 0:
         raise ValueError("token_log_probs expects logits of [..., classes]")
-    if input.device != target.device or "float" not in str(input.dtype):
+    dev = input.device
+    if (target.device is not dev and target.device != dev) or "float" not in str(x.dtype):
         raise ValueError("token_log_probs needs floating logits and targets on the same device")
     if target.requires_grad:
         raise ValueError("target tokens cannot require gradients")
-    if "int" not in str(target.dtype):
+    if "int" not in str(y.dtype):
         raise TypeError("target tokens must have an integer dtype")
-    if target.shape != input.shape[:-1]:
-        raise ValueError(f"target shape {target.shape} does not match logits shape {input.shape}")
-    classes = input.shape[-1]
+    if shape != given[:-1]:
+        raise ValueError(f"target shape {shape} does not match logits shape {given}")
+    classes = given[-1]
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(classes, 64):
         raise ValueError("top_k must be between zero and 64 and within the classes")
     _require_hip(input, "token_log_probs")
-    code = _code(input._data)
+    code = _code(x)
     if code < 0:
         raise TypeError("token_log_probs takes float32, float16 or bfloat16 logits")
     import torch
 
-    z = input._data.reshape(-1, classes)
-    z = z if z.stride(1) == 1 or classes == 1 else z.contiguous()
-    y = target._data.reshape(-1)
+    z = x if len(given) == 2 else x.reshape(-1, classes)
+    if z.stride(1) != 1 and classes != 1:
+        z = z.contiguous()
     if y.dtype not in (torch.int64, torch.int32):
         y = y.long()
-    y = y.contiguous()
-    rows, dev = z.shape[0], input.device
-    recording = is_grad_enabled() and input.requires_grad
-    floats = torch.empty((2 + 2 * recording + top_k, rows), dtype=torch.float32, device=z.device)
-    logp, entropy = floats[0], floats[1]
-    stats = floats[2:4] if recording else None
-    top = floats[2 + 2 * recording:] if top_k else None
-    index = torch.empty((rows, top_k), dtype=torch.int64, device=z.device) if top_k else None
+    y = y if y.is_contiguous() else y.contiguous()
+    rows, place = z.shape[0], z.device
+    recording = input.requires_grad and is_grad_enabled()
+    logp = torch.empty(shape, dtype=torch.float32, device=place)
+    entropy = torch.empty(shape, dtype=torch.float32, device=place)
+    stats = top = index = ws = None
+    if recording:
+        stats = torch.empty(2 * rows, dtype=torch.float32, device=place)
+    if top_k:
+        top = torch.empty(shape + (top_k,), dtype=torch.float32, device=place)
+        index = torch.empty(shape + (top_k,), dtype=torch.int64, device=place)
     lib = _lib.load()
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    # (logits, stride, tokens, ..): what both passes are given first
+    operands = (code, rows, classes, z.data_ptr(), z.stride(0), y.data_ptr(), y.element_size(), ignore_index, top_k)
     if rows:
         nbytes = lib.tsattn_token_probs_workspace(rows, classes, top_k)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device) if nbytes else None
-        _lib.check(launch(dev, lib.tsattn_token_probs, code, rows, classes, z.data_ptr(), z.stride(0), y.data_ptr(),
-                          y.element_size(), ignore_index, top_k, logp.data_ptr(), entropy.data_ptr(), _ptr(stats),
-                          _ptr(top), _ptr(index), _ptr(ws), nbytes), "token log probabilities")
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=place)
+        _lib.check(launch(dev, lib.tsattn_token_probs, *operands, logp.data_ptr(), entropy.data_ptr(), at(stats),
+                          at(top), at(index), at(ws), nbytes), "token log probabilities")
+    indices = Tensor._leaf(index, dev) if top_k else None
+    if not recording:
+        return TokenLogProbs(Tensor._leaf(logp, dev), Tensor._leaf(entropy, dev),
+                             Tensor._leaf(top, dev) if top_k else None, indices)
 
-    def backward(parts):
-        g, gh, gt = parts.grads
-        g, gh, gt = (None if u is None else u.reshape(-1).contiguous() for u in (g, gh, gt))
-        dz = torch.empty((rows, classes), dtype=z.dtype, device=z.device)
+    def backward(parts, _keep=(z, y)):
+        grads = [None if g is None else g if g.is_contiguous() else g.contiguous() for g in parts.grads]
+        dz = torch.empty((rows, classes), dtype=z.dtype, device=place)
         if rows:
-            _lib.check(launch(dev, lib.tsattn_token_probs_backward, code, rows, classes, z.data_ptr(), z.stride(0),
-                              y.data_ptr(), y.element_size(), ignore_index, top_k, stats.data_ptr(),
-                              entropy.data_ptr(), _ptr(index), _ptr(g), _ptr(gh), _ptr(gt), dz.data_ptr()),
-                       "token log probabilities backward")
-        return (dz.reshape(input.shape),)
+            _lib.check(launch(dev, lib.tsattn_token_probs_backward, *operands, stats.data_ptr(), entropy.data_ptr(),
+                              at(index), *(at(g) for g in grads), dz.data_ptr()), "token log probabilities backward")
+        return (dz if len(given) == 2 else dz.reshape(given),)
 
     joint = Tensor._from_op(logp, (input,), backward, "token_log_probs")
-    shape = target.shape
-
-    def result(i, raw, op):
-        return Tensor._from_op(raw, (joint,), lambda u: (_Parts(*(u if k == i else None for k in range(3))),), op)
-
     return TokenLogProbs(
-        result(0, logp.view(shape), "log_probs"), result(1, entropy.view(shape), "entropy"),
-        result(2, top.view(shape + (top_k,)), "top_log_probs") if top_k else None,
-        Tensor._leaf(index.view(shape + (top_k,)), dev) if top_k else None)
+        Tensor._from_op(logp, (joint,), lambda g: (_Parts(g, None, None),), "log_probs"),
+        Tensor._from_op(entropy, (joint,), lambda g: (_Parts(None, g, None),), "entropy"),
+        Tensor._from_op(top, (joint,), lambda g: (_Parts(None, None, g),), "top_log_probs") if top_k else None,
+        indices)

@@ -424,12 +424,13 @@ int tsattn_draft_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len
  * Rows first + index[b, i] of a cache's arrays [batch, heads, *] become its rows first +
  * i, i < n (at most 256), all of them read before any is written.  index: [batch, n],
  * int64 or int32 (index_bytes); one outside [0, limit) leaves row first + i as it is.
- * k, v: views with strides in bytes, key_bytes and value_bytes a row; k_scale, v_scale:
- * fp32 scales a row (strides in elements), or both NULL.
+ * k, v: rows of dim_qk and dim_v elements of element_bytes (1, 2, 4 or 8); k_scale,
+ * v_scale: fp32 scales a row, or both NULL.
  */
 int tsattn_cache_keep(int32_t batch, int32_t heads, int32_t n, int64_t first, int64_t limit, const void *index,
-                      int32_t index_bytes, int32_t key_bytes, int32_t value_bytes, const tsattn_view *k,
-                      const tsattn_view *v, const tsattn_view *k_scale, const tsattn_view *v_scale, void *stream);
+                      int32_t index_bytes, int32_t element_bytes, int32_t dim_qk, int32_t dim_v,
+                      const tsattn_view *k, const tsattn_view *v, const tsattn_view *k_scale,
+                      const tsattn_view *v_scale, void *stream);
 
 /*
  * Attention of the newest `len` tokens over a cache of `keys` positions, theirs the last
