@@ -9,9 +9,12 @@
 // tokens' log probabilities (at indices k_i), G = g + sum_i t_i:
 //   dz_j = -p_j (G + gh (ln p_j + H)) + [j = y] g + sum_i [j = k_i] t_i.
 //
+// In log2 units throughout, t_j = z_j log2 e - b as one fused operation, b the row's
+// largest z log2 e as it rounds: b cancels from every result, so its rounding does too.
+//
 // Bound by HBM: the forward reads the logits once, the VJP reads them and writes the
-// gradient.  One pass in each: a lane keeps a running (m, l, sum e x) and rescales it
-// once for every 16-byte piece.  A 16-bit logit takes about 11 vector instructions
+// gradient.  One pass in each: a lane keeps a running (b, l, sum 2^t t) and rescales it
+// once for every 16-byte piece.  A 16-bit logit takes about 10 vector instructions
 // (an exponential counts four), which at the chip's rate is some 7 TB/s of logits:
 // just above what HBM gives, so anything more an element would show.
 //
@@ -49,7 +52,7 @@ struct ProbArgs {
   const void *tokens;
   int token_bytes;
   int64_t ignore;
-  float *logp, *entropy, *stats;  // stats: [rows][2] = m, ln l
+  float *logp, *entropy, *stats;  // stats: [rows][2] = b, log2 l
   float *top_logp;
   int64_t *top_index;
   float *part;                   // [rows][splits][4]: m, l, sum e x (log2 units)
@@ -94,17 +97,17 @@ __device__ __forceinline__ int64_t token_of(const ProbArgs &a, int64_t row) {
 }
 
 // ---------------------------------------------------------------------------
-// Running sums: m, l = sum exp(z - m), w = sum exp(z - m) (z - m) log2 e.
+// Running sums: m the base b, l = sum 2^t, w = sum 2^t t.
 // ---------------------------------------------------------------------------
 struct Sums {
   float m, l, w;
 };
 
-// (a base that keeps exp(-inf - base) = 0 while nothing but -inf has come)
+// (a base that keeps 2^(-inf - base) = 0 while nothing but -inf has come)
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
 __device__ __forceinline__ void rebase(Sums &s, float m) {
-  const float d = (base_of(s.m) - base_of(m)) * kLog2e;
+  const float d = base_of(s.m) - base_of(m);
   const float c = __builtin_amdgcn_exp2f(d);
   // an empty sum stays empty whatever the bases (0 * inf is NaN)
   s.w = s.l == 0.f ? s.w : c * fmaf(s.l, fmaxf(d, -1e30f), s.w);
@@ -127,12 +130,12 @@ __device__ __forceinline__ Sums wave_join(Sums s) {
 // Adds N logits; `own` becomes their sum of exponentials (NaN where one is NaN or +inf).
 template <int N>
 __device__ __forceinline__ void add(Sums &s, const float (&x)[N], float mx, float &own) {
-  rebase(s, fmaxf(s.m, mx));
+  rebase(s, fmaxf(s.m, mx * kLog2e));
   const float base = base_of(s.m);
   float l = 0.f;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const float t = (x[e] - base) * kLog2e;
+    const float t = fmaf(x[e], kLog2e, -base);
     const float p = __builtin_amdgcn_exp2f(t);
     l += p;
     s.w = fmaf(p, fmaxf(t, -1e30f), s.w);  // (0 times -inf is NaN)
@@ -245,22 +248,21 @@ struct Best {
 // What a row's sums (and with TOP its best keys, one a lane) say; one wave.
 template <typename T, bool TOP>
 __device__ __forceinline__ void results(const ProbArgs &a, int64_t row, Sums s, u64 best, int lane) {
-  const float ln = logf(s.l);
   // (all logits -inf: l = 0; log p is NaN as -inf - -inf is)
-  const float m = s.m;
+  const float m = s.m, log2l = log2f(s.l);
   if (lane == 0) {
     const int64_t y = token_of(a, row);
     const float z = y >= 0 && y < a.vocab ? static_cast<float>(static_cast<const T *>(a.z)[row * a.zs + y]) : NAN;
-    a.logp[row] = (z - m) - ln;
-    a.entropy[row] = m == -INFINITY ? NAN : ln - s.w / s.l * kLn2;
+    a.logp[row] = (fmaf(z, kLog2e, -m) - log2l) * kLn2;
+    a.entropy[row] = m == -INFINITY ? NAN : (log2l - s.w / s.l) * kLn2;
     if (a.stats) {
       a.stats[2 * row] = m;
-      a.stats[2 * row + 1] = ln;
+      a.stats[2 * row + 1] = log2l;
     }
   }
   if constexpr (TOP) {
     if (lane < a.top) {
-      a.top_logp[row * a.top + lane] = (key_logit(best) - m) - ln;
+      a.top_logp[row * a.top + lane] = (fmaf(key_logit(best), kLog2e, -m) - log2l) * kLn2;
       a.top_index[row * a.top + lane] = ~static_cast<unsigned>(best);
     }
   }
@@ -278,15 +280,15 @@ __device__ __forceinline__ void ignored(const ProbArgs &a, int64_t row, int lane
   }
 }
 
-// A row as 16-byte pieces: `head` elements before the first aligned one, `pieces`,
-// then what is left.
+// A row as 16-byte pieces: `head` elements (at most 63) up to the first whole 128-byte
+// line, so that no two waves share a line, `pieces`, then what is left.
 template <typename T>
 struct Row {
   const T *z;
   int head, pieces, tail;
   __device__ __forceinline__ Row(const T *p, int vocab) : z(p) {
-    const unsigned off = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) & 15u);
-    head = min(vocab, static_cast<int>((16u - off) % 16u / sizeof(T)));
+    const unsigned off = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) & 127u);
+    head = min(vocab, static_cast<int>((128u - off) % 128u / sizeof(T)));
     pieces = (vocab - head) / kVE<T>;
     tail = vocab - head - pieces * kVE<T>;
   }
@@ -324,13 +326,18 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
   const int l0 = (WPR == 1 ? 0 : w * 64) + lane;
   if (part == 0 && (WPR == 1 || w == 0) && r.head) single(0, r.head);
   const u32x4 *pieces = reinterpret_cast<const u32x4 *>(r.z + r.head);
-  for (int i = p0; i < p1; i += LANES * U) {
-    u32x4 raw[U];
+  // U pieces a lane ahead of those it works on
+  u32x4 raw[U], next[U];
+  auto load = [&](int i, u32x4 (&x)[U]) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = i + u * LANES + l0;
-      if (at < p1) raw[u] = __builtin_nontemporal_load(pieces + at);
+      if (at < p1) x[u] = __builtin_nontemporal_load(pieces + at);
     }
+  };
+  load(p0, raw);
+  for (int i = p0; i < p1; i += LANES * U) {
+    load(i + LANES * U, next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u * LANES >= p1) break;
@@ -347,6 +354,8 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
       add(s, x, mx, own);
       if constexpr (TOP) top.offer(x, mx, own, r.head + at * VE, at < p1 ? VE : 0, a.top, lane);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = next[u];
   }
   if (part == splits - 1 && (WPR == 1 || w == NW - 1) && r.tail) single(a.vocab - r.tail, r.tail);
   s = wave_join(s);
@@ -434,7 +443,7 @@ __global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
     if (has_tail && lane < r.tail) dz[a.vocab - r.tail + lane] = static_cast<T>(0.f);
     return;
   }
-  const float m = a.stats[2 * row], ln = a.stats[2 * row + 1];
+  const float m = a.stats[2 * row], log2l = a.stats[2 * row + 1];
   float g = a.g ? a.g[row] : 0.f;
   if (y < 0 || y >= a.vocab) g = a.g ? NAN : 0.f;  // (its log probability is NaN)
   const float gh = a.gh ? a.gh[row] : 0.f;
@@ -442,10 +451,10 @@ __global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
   if constexpr (TOP)
     for (int i = 0; i < a.top; ++i) all += a.gt[row * a.top + i];
   const float c = gh == 0.f ? all : fmaf(gh, a.saved_entropy[row], all);
+  const float gl = gh * kLn2;
   auto at_logit = [&](float x) {
-    const float lp = (x - m) - ln;
-    const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
-    return -p * fmaf(gh, fmaxf(lp, -1e30f), c);
+    const float t = fmaf(x, kLog2e, -m) - log2l;  // log2 p
+    return -__builtin_amdgcn_exp2f(t) * fmaf(gl, fmaxf(t, -1e30f), c);
   };
   const int yi = y >= 0 && y < a.vocab ? static_cast<int>(y) : -1;
   auto single = [&](int j) {
@@ -453,13 +462,13 @@ __global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
     dz[j] = static_cast<T>(j == yi ? d + g : d);
   };
   if (has_head && lane < r.head) single(lane);
-  for (int i = p0 + l0; i < p1; i += LANES * U) {
-    u32x4 raw[U];
+  u32x4 raw[U], next[U];
+  auto load = [&](int i, u32x4 (&x)[U]) __attribute__((always_inline)) {
     if (alike) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (i + u * LANES < p1)
-          raw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(z + r.head) + i + u * LANES);
+          x[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(z + r.head) + i + u * LANES);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -469,9 +478,13 @@ __global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
           const T *from = z + r.head + (i + u * LANES) * VE;
 #pragma unroll
           for (int e = 0; e < VE; ++e) v[e] = from[e];
-          raw[u] = __builtin_bit_cast(u32x4, v);
+          x[u] = __builtin_bit_cast(u32x4, v);
         }
     }
+  };
+  load(p0 + l0, raw);
+  for (int i = p0 + l0; i < p1; i += LANES * U) {
+    load(i + LANES * U, next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = i + u * LANES;
@@ -487,6 +500,8 @@ __global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
       }
       store_piece(dz + j0, x);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = next[u];
   }
   if (has_tail && lane < r.tail) single(a.vocab - r.tail + lane);
   if constexpr (TOP) {
