@@ -14,9 +14,9 @@
 //
 // Bound by HBM: the forward reads the logits once, the VJP reads them and writes the
 // gradient.  One pass in each: a lane keeps a running (b, l, sum 2^t t) and rescales it
-// once for every 16-byte piece.  A 16-bit logit takes about 10 vector instructions
-// (an exponential counts four), which at the chip's rate is some 7 TB/s of logits:
-// just above what HBM gives, so anything more an element would show.
+// once for every four 16-byte pieces.  The forward is about as far from the vector units'
+// bound: 6 instructions a logit; 11 of them (selects for rows' ends and -inf on every
+// one) took 131 us where 8192 rows of 50021 bf16, a fifth of them ignored, take 105.
 //
 // A row belongs to one wave (V <= kWaveRow), to a workgroup of four, or, when the rows
 // are too few to fill the chip, to several workgroups that each take a part of it; a
@@ -121,16 +121,34 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
   return Sums{m, a.l + b.l, a.w + b.w};
 }
 __device__ __forceinline__ Sums wave_join(Sums s) {
+  float m = s.m;
 #pragma unroll
-  for (int k = 1; k < 64; k <<= 1)
-    s = join(s, Sums{__shfl_xor(s.m, k, 64), __shfl_xor(s.l, k, 64), __shfl_xor(s.w, k, 64)});
+  for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+  rebase(s, m);
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    s.l += __shfl_xor(s.l, k, 64);
+    s.w += __shfl_xor(s.w, k, 64);
+  }
   return s;
 }
 
-// Adds N logits; `own` becomes their sum of exponentials (NaN where one is NaN or +inf).
+// The largest of N values that is not a NaN (two an instruction, where fmaxf would also
+// canonicalise each; a NaN shows in the sums).
 template <int N>
-__device__ __forceinline__ void add(Sums &s, const float (&x)[N], float mx, float &own) {
-  rebase(s, fmaxf(s.m, mx * kLog2e));
+__device__ __forceinline__ float largest(const float (&x)[N]) {
+  float m = x[0];
+#pragma unroll
+  for (int e = 1; e + 1 < N; e += 2) asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(x[e]), "v"(x[e + 1]));
+  if constexpr (N % 2 == 0) asm("v_max_f32 %0, %1, %2" : "=v"(m) : "v"(m), "v"(x[N - 1]));
+  return m;
+}
+
+// Adds N logits, none above the base; `own` becomes their sum of exponentials (NaN where
+// one is NaN or +inf).  A logit of -inf makes w a NaN (0 times -inf) unless SAFE, at an
+// instruction a logit.
+template <bool SAFE, int N>
+__device__ __forceinline__ void add(Sums &s, const float (&x)[N], float &own) {
   const float base = base_of(s.m);
   float l = 0.f;
 #pragma unroll
@@ -138,7 +156,7 @@ __device__ __forceinline__ void add(Sums &s, const float (&x)[N], float mx, floa
     const float t = fmaf(x[e], kLog2e, -base);
     const float p = __builtin_amdgcn_exp2f(t);
     l += p;
-    s.w = fmaf(p, fmaxf(t, -1e30f), s.w);  // (0 times -inf is NaN)
+    s.w = fmaf(p, SAFE ? fmaxf(t, -1e30f) : t, s.w);
   }
   s.l += l;
   own = l;
@@ -316,11 +334,12 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
   Sums s{-INFINITY, 0.f, 0.f};
   Best top;
   top.buffer = buffers + (TOP ? w * PENDING : 0);
-  float own;
   // the elements in front of the first piece, one a lane
   auto single = [&](int first, int n) {
     const float x[1] = {lane < n ? static_cast<float>(r.z[first + lane]) : -INFINITY};
-    add(s, x, x[0], own);
+    float own;
+    rebase(s, fmaxf(s.m, x[0] * kLog2e));
+    add<true>(s, x, own);
     if constexpr (TOP) top.offer(x, x[0], own, first + lane, lane < n ? 1 : 0, a.top, lane);
   };
   const int l0 = (WPR == 1 ? 0 : w * 64) + lane;
@@ -338,21 +357,42 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
   load(p0, raw);
   for (int i = p0; i < p1; i += LANES * U) {
     load(i + LANES * U, next);
+    float x[U][VE], mx[U], most = s.m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u * LANES >= p1) break;
-      const int at = i + u * LANES + l0;
-      float x[VE];
-      unpack<T>(raw[u], x);
-      if (at >= p1) {
+      unpack<T>(raw[u], x[u]);
+      // (the whole workgroup's test first: selects on every piece are an instruction an element)
+      if (i + (u + 1) * LANES > p1 && i + u * LANES + l0 >= p1) {
 #pragma unroll
-        for (int e = 0; e < VE; ++e) x[e] = -INFINITY;
+        for (int e = 0; e < VE; ++e) x[u][e] = -INFINITY;
       }
-      float mx = x[0];
+      mx[u] = largest(x[u]);
+      most = fmaxf(most, mx[u] * kLog2e);
+    }
+    rebase(s, most);
+    const Sums before = s;
+    float own[U];
 #pragma unroll
-      for (int e = 1; e < VE; ++e) mx = fmaxf(mx, x[e]);
-      add(s, x, mx, own);
-      if constexpr (TOP) top.offer(x, mx, own, r.head + at * VE, at < p1 ? VE : 0, a.top, lane);
+    for (int u = 0; u < U; ++u) {
+      if (i + u * LANES >= p1) break;
+      add<false>(s, x[u], own[u]);
+    }
+    if (__ballot(s.w != s.w) != 0ull) {  // a logit of -inf: again
+      s = before;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u * LANES >= p1) break;
+        add<true>(s, x[u], own[u]);
+      }
+    }
+    if constexpr (TOP) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u * LANES >= p1) break;
+        const int at = i + u * LANES + l0;
+        top.offer(x[u], mx[u], own[u], r.head + at * VE, at < p1 ? VE : 0, a.top, lane);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) raw[u] = next[u];
