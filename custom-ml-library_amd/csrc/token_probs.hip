@@ -176,30 +176,55 @@ __device__ __forceinline__ float key_logit(u64 key) {
   const unsigned u = static_cast<unsigned>(key >> 32);
   return __builtin_bit_cast(float, (u >> 31) ? u ^ 0x80000000u : ~u);
 }
-__device__ __forceinline__ u64 from_lane(u64 x, int lane) {
-  const int lo = __shfl(static_cast<int>(x), lane, 64), hi = __shfl(static_cast<int>(x >> 32), lane, 64);
-  return static_cast<u64>(static_cast<unsigned>(hi)) << 32 | static_cast<unsigned>(lo);
+// The value of lane l ^ STRIDE, without LDS: data-parallel moves inside a row of 16,
+// v_permlane16_swap / 32_swap (the odd rows or half of one register for the even of
+// another) between them.
+template <int STRIDE>
+__device__ __forceinline__ unsigned of_lane_xor(unsigned x, int lane) {
+  if constexpr (STRIDE == 1) return __builtin_amdgcn_update_dpp(x, x, 0xB1, 0xF, 0xF, false);
+  else if constexpr (STRIDE == 2) return __builtin_amdgcn_update_dpp(x, x, 0x4E, 0xF, 0xF, false);
+  else if constexpr (STRIDE == 4) {
+    const unsigned y = __builtin_amdgcn_update_dpp(x, x, 0x104, 0xF, 0x5, false);  // row_shl:4 into the lower of each 8
+    return __builtin_amdgcn_update_dpp(y, x, 0x114, 0xF, 0xA, false);              // row_shr:4 into the upper
+  } else if constexpr (STRIDE == 8) {
+    return __builtin_amdgcn_update_dpp(x, x, 0x128, 0xF, 0xF, false);  // row_ror:8
+  } else {
+    unsigned a = x, b = x;
+    if constexpr (STRIDE == 16) asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    else asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    return lane & STRIDE ? a : b;
+  }
 }
-// One exchange of a bitonic network: lanes l and l ^ stride, the larger to the lower
+// One exchange of a bitonic network: lanes l and l ^ STRIDE, the larger to the lower
 // lane where `down`.
-__device__ __forceinline__ u64 exchange(u64 x, int lane, int stride, bool down) {
-  const u64 y = from_lane(x, lane ^ stride);
-  return (((lane & stride) == 0) == down) == (x > y) ? x : y;
+template <int STRIDE>
+__device__ __forceinline__ u64 exchange(u64 x, int lane, bool down) {
+  const unsigned lo = of_lane_xor<STRIDE>(static_cast<unsigned>(x), lane);
+  const unsigned hi = of_lane_xor<STRIDE>(static_cast<unsigned>(x >> 32), lane);
+  const u64 y = static_cast<u64>(hi) << 32 | lo;
+  return (((lane & STRIDE) == 0) == down) == (x > y) ? x : y;
 }
-__device__ __forceinline__ u64 sort_down(u64 x, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int stride = size >> 1; stride; stride >>= 1) x = exchange(x, lane, stride, (lane & size) == 0);
+template <int STRIDE>
+__device__ __forceinline__ u64 ripple(u64 x, int lane, bool down) {
+  x = exchange<STRIDE>(x, lane, down);
+  if constexpr (STRIDE > 1) x = ripple<STRIDE / 2>(x, lane, down);
   return x;
 }
-// The 64 best of two lists sorted down.
-__device__ __forceinline__ u64 merge_down(u64 best, u64 more, int lane) {
-  const u64 y = from_lane(more, 63 - lane);
-  u64 x = best > y ? best : y;
-#pragma unroll
-  for (int stride = 32; stride; stride >>= 1) x = exchange(x, lane, stride, true);
+template <int SIZE = 2>
+__device__ __forceinline__ u64 sort_up(u64 x, int lane) {
+  x = ripple<SIZE / 2>(x, lane, (lane & SIZE) != 0);
+  if constexpr (SIZE < 64) x = sort_up<SIZE * 2>(x, lane);
   return x;
+}
+// The 64 best, falling, of a list that falls and one that rises.
+__device__ __forceinline__ u64 merge_down(u64 best, u64 rising, int lane) {
+  return ripple<32>(best > rising ? best : rising, lane, true);
+}
+// A lane's value in scalar registers.
+__device__ __forceinline__ u64 of_lane(u64 x, int lane) {
+  const unsigned lo = __builtin_amdgcn_readlane(static_cast<unsigned>(x), lane);
+  const unsigned hi = __builtin_amdgcn_readlane(static_cast<unsigned>(x >> 32), lane);
+  return static_cast<u64>(hi) << 32 | lo;
 }
 
 struct Best {
@@ -211,10 +236,7 @@ struct Best {
 
   __device__ __forceinline__ void raise(u64 key) {
     if (key > least) {
-      // (the same in every lane: kept where a comparison reads it as a scalar)
-      const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(key));
-      const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(key >> 32));
-      least = static_cast<u64>(hi) << 32 | lo;
+      least = key;
       least_z = key_logit(least);
     }
   }
@@ -224,8 +246,8 @@ struct Best {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const u64 key = lane < n ? buffer[pending + lane] : 0;
-    best = merge_down(best, sort_down(key, lane), lane);
-    raise(from_lane(best, top - 1));
+    best = merge_down(best, sort_up(key, lane), lane);
+    raise(of_lane(best, top - 1));
   }
   // N logits a lane from `index` on, n of them there; call in step, indexes rising.
   template <int N>
@@ -242,7 +264,7 @@ struct Best {
         const u64 k = e < n ? key_of(x[e], index + e) : 0;
         key = k > key ? k : key;
       }
-      key = from_lane(sort_down(key, lane), top - 1);
+      key = of_lane(sort_up(key, lane), 64 - top);
       if (key) raise(key - 1);
     }
 #pragma unroll
@@ -402,7 +424,7 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
   if constexpr (TOP) top.finish(a.top, lane);
   if constexpr (WPR > 1) {
     if (lane == 0) red[w][0] = s.m, red[w][1] = s.l, red[w][2] = s.w;
-    if constexpr (TOP) top.buffer[lane] = top.best;
+    if constexpr (TOP) top.buffer[63 - lane] = top.best;  // (rising, as merge_down takes it)
     __syncthreads();
     if (w) return;
 #pragma unroll
@@ -423,24 +445,41 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
   results<T, TOP>(a, row, s, top.best, lane);
 }
 
-// The parts of a row, in their order; a wave a row.
+// The parts of a row; a workgroup a row, whose waves share the parts' top keys (in any
+// order: the keys are all different).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(NT) void probs_merge_kernel(ProbArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * NW + (threadIdx.x >> 6);
-  if (row >= a.rows || token_of(a, row) == a.ignore) return;
+  __shared__ u64 lists[TOP ? NW * 64 : 1];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = blockIdx.x;
+  if (token_of(a, row) == a.ignore) return;
+  u64 best = 0;
+  if constexpr (TOP) {
+    const u64 *keys = a.part_top + row * a.splits * a.top;
+    for (int i = w; i < a.splits; i += 4 * NW) {
+      u64 more[4];  // four loads in flight
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        more[u] = i + u * NW < a.splits && 63 - lane < a.top ? keys[(i + u * NW) * a.top + 63 - lane] : 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u * NW < a.splits) best = merge_down(best, more[u], lane);
+    }
+    lists[w * 64 + 63 - lane] = best;
+    __syncthreads();
+  }
+  if (w) return;
+  if constexpr (TOP) {
+#pragma unroll
+    for (int k = 1; k < NW; ++k) best = merge_down(best, lists[k * 64 + lane], lane);
+  }
   // (lane i starts with part i; more parts than lanes do not occur, kMaxSplits)
   Sums s{-INFINITY, 0.f, 0.f};
   if (lane < a.splits) {
     const float *p = a.part + 4 * (row * a.splits + lane);
     s = Sums{p[0], p[1], p[2]};
   }
-  s = wave_join(s);
-  u64 best = 0;
-  if constexpr (TOP)
-    for (int i = 0; i < a.splits; ++i)
-      best = merge_down(best, lane < a.top ? a.part_top[(row * a.splits + i) * a.top + lane] : 0, lane);
-  results<T, TOP>(a, row, s, best, lane);
+  results<T, TOP>(a, row, wave_join(s), best, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -586,7 +625,7 @@ void forward(ProbArgs &a, hipStream_t st) {
   }
   probs_kernel<T, NW, TOP><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(NT), 0, st>>>(a);
   if (a.splits > 1)
-    probs_merge_kernel<T, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
+    probs_merge_kernel<T, TOP><<<dim3(static_cast<unsigned>(a.rows)), dim3(NT), 0, st>>>(a);
 }
 
 template <typename T, bool TOP>
