@@ -1106,7 +1106,13 @@ int tsattn_cached_attend(const tsattn_cached *d, const tsattn_view *q, const tsa
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(TSATTN_ERR_INVALID, "cached attention needs %zu bytes of 16-byte aligned workspace", need);
   tsattn::View ks{}, vs{};
-  if (p.q8) ks = tsattn::make_view(k_scale), vs = tsattn::make_view(v_scale);
+  if (p.q8) {
+    ks = tsattn::make_view(k_scale), vs = tsattn::make_view(v_scale);
+    for (const tsattn::View *x : {&ks, &vs})
+      if (reinterpret_cast<uintptr_t>(x->data) % 4 || x->s2 <= 0 ||
+          (static_cast<int64_t>(p.n) + 64) * x->s2 * 4 >= (int64_t(1) << 31))
+        return fail(TSATTN_ERR_UNSUPPORTED, "cached attention needs aligned scales, a head's below 2^31 bytes");
+  }
   return hip_status(tsattn::launch_cached(p, vq, vk, vv, ks, vs, vo, static_cast<float *>(workspace),
                                           static_cast<hipStream_t>(stream)),
                     "cached attention launch");

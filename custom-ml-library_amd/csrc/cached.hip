@@ -49,26 +49,38 @@ struct CachedArgs {
 };
 
 template <typename T, int D>
-constexpr int kPair = 2 * BN * D * (std::is_same_v<T, float> ? 4 : 2);  // bytes of a K and a V tile
-// Waves of a workgroup, WR of them sharing each tile.  Up to 32 rows (WR 1) a wave has
-// room for one K and one V tile, so that 8 waves of 128 channels share a CU.  A tile's
-// steps follow each other in a wave: with more room and 4 waves the step below took 97 us
-// whether 3 or 4 of its tiles were in flight, 5.6 TB/s.
+constexpr int kPair = 2 * BN * D * (std::is_same_v<T, float> ? 4 : 2);  // bytes of a K and a V tile, in T
+// Waves of a workgroup, WR of them sharing each tile.  Up to 32 rows (WR 1) a wave's ring
+// of 16-bit tiles has room for one K and one V tile, so that 8 waves of 128 channels share
+// a CU: with room for more, 4 waves and 3 or 4 of a wave's tiles in flight, the step that
+// plan_cached names took the same time.
 template <typename T, int D, int WR>
 constexpr int kWaves = WR > 1 ? WR : (kPair<T, D> <= 16384 ? 4 : 2);
 // Waves a SIMD that the registers must leave room for.
 template <typename T, int D>
 constexpr int kTwo = kPair<T, D> <= 16384 ? 2 : 1;
-// Ring stages of a K and a V tile for several waves: three, or two of widened codes.
-template <bool Q8>
-constexpr int kStages = Q8 ? 2 : 3;
+// Ring stages of a K and a V tile: for several waves three, for one of its own one, or
+// two of codes, half as large.
+template <bool Q8, int WR>
+constexpr int kStages = WR > 1 ? 3 : Q8 ? 2 : 1;
 
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
-// Eight int8 codes as eight values of T (exact).
+// Eight int8 codes as eight values of T (exact).  In f16, 1024 + (code + 128) is a code
+// with its sign bit turned under the exponent byte 0x64, two to a permutation and a sum.
 template <typename T>
 __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
   u32x4 y;
+  if constexpr (std::is_same_v<T, f16>) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = (i < 2 ? lo : hi) ^ 0x80808080u;
+      const uint32_t two = __builtin_amdgcn_perm(0x64646464u, u, i & 1 ? 0x04030402u : 0x04010400u);
+      y[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, two) + h2{-1152, -1152});
+    }
+    return y;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = (i < 2 ? lo : hi) >> (16 * (i & 1));
@@ -78,17 +90,20 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
   return y;
 }
 
+// Code n of a lane's 8 bytes.
+__device__ __forceinline__ float code(u32x2 x, int n) {
+  return static_cast<float>(static_cast<int8_t>((x[n >> 2] >> (8 * (n & 3))) & 0xFFu));
+}
+
 // 16-bit K / V tiles in LDS, 32 rows of D, row-major, 16-byte chunk k of row r at k ^
-// sw(r).  One DMA instruction fetches whole rows (of 256 bytes four: 16 rows' quarters,
-// the prefill kernel's blocks, left HBM at 5.5 TB/s).  16 rows' same chunk, and 4 rows'
-// 4 chunks beside each other (the transposing reads), lie in different banks.
+// sw(r).  One DMA instruction fetches whole rows.  16 rows' same chunk, and 4 rows' 4
+// chunks beside each other (the transposing reads), lie in different banks.
 template <typename T, int D>
 struct RowTile {
   static constexpr int RPB = 1024 / (2 * D);  // rows a DMA block
   __device__ __forceinline__ static constexpr int sw(int r) {
     return D >= 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : D == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : (r >> 2) & 3;
   }
-  __device__ __forceinline__ static int at(int r, int k) { return r * 2 * D + ((k ^ sw(r)) << 4); }
   // of the block's first row: what lane l fetches for its 16 bytes at 16 l of block n
   __device__ __forceinline__ static uint32_t dma_off(int n, int lane, uint32_t stride) {
     const int rr = lane / (D / 8), k = lane % (D / 8);
@@ -114,22 +129,69 @@ struct RowTile {
   }
 };
 
+// Tiles of int8 codes, 32 rows of D bytes, the 16-byte chunk k of row r at k ^ sw(r): 16
+// rows' same chunk lie in different banks.  They are widened on the way to the matrix
+// instructions (through registers into 16-bit tiles in LDS instead, a window's step over 32
+// sequences' 4096 keys of 8 heads of 128 took 148 us, so 54, 5 TB/s; of 256 channels, whose
+// registers spilled, 16 sequences 627 and 60), which fixes the order of a lane's channels
+// in both products:
+//   scores: step 2 j + e contracts channels 32 j + 16 h + 8 e .. + 7, a chunk for two steps;
+//   values: row c of block dt of O^T is channel D / 32 c + dt, so that a lane's D / 32
+//   neighbouring bytes of a key serve one block each and nothing is transposed.
+template <int D>
+struct CodeTile {
+  static constexpr int RPB = 1024 / D, CPR = D / 16, PDT = D / 32;
+  __device__ __forceinline__ static constexpr int sw(int r) { return r * CPR / 16 & (CPR - 1); }
+  __device__ __forceinline__ static uint32_t dma_off(int n, int lane, uint32_t stride) {
+    const int rr = lane / CPR, k = lane % CPR;
+    return static_cast<uint32_t>(rr) * stride + static_cast<uint32_t>((k ^ sw(n * RPB + rr)) << 4);
+  }
+  int krow, kchunk, vbyte, h;
+  __device__ __forceinline__ explicit CodeTile(int lane) {
+    const int c = lane & 31;
+    h = lane >> 5;
+    krow = c * D, kchunk = (h ^ sw(c)) << 4;
+    vbyte = (c * PDT) ^ (sw(4 * h) << 4);
+  }
+  // row c, channels 32 j + 16 h .. + 15
+  __device__ __forceinline__ u32x4 rows(const char *tile, int j) const { return ld16(tile + krow + (kchunk ^ (j << 5))); }
+  // key 16 ks + 8 a + 4 h + b, channels PDT c .. + PDT - 1
+  __device__ __forceinline__ u32x2 key(const char *tile, int ks, int a, int b) const {
+    const char *at = tile + (16 * ks + 8 * a + 4 * h + b) * D + (vbyte ^ (sw(8 * a + b) << 4));
+    if constexpr (PDT == 8) return *reinterpret_cast<const u32x2 *>(at);
+    else if constexpr (PDT == 4) return u32x2{*reinterpret_cast<const uint32_t *>(at), 0u};
+    else if constexpr (PDT == 2) return u32x2{*reinterpret_cast<const uint16_t *>(at), 0u};
+    else return u32x2{*reinterpret_cast<const uint8_t *>(at), 0u};
+  }
+};
+
+// Lane l's 4 bytes at voff + soff go to LDS at lds + 4 l.
+__device__ __forceinline__ void dma4(u32x4 desc, uint32_t lds, uint32_t voff, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(desc),
+                 "s"(__builtin_amdgcn_readfirstlane(soff))
+               : "memory", "m0");
+}
+
 template <typename T, int D, bool Q8, int WR>
-__global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<T, D>)) void cached_kernel(CachedArgs a) {
+__global__ __launch_bounds__((64 * kWaves<T, D, WR>), (kTwo<T, D>)) void cached_kernel(CachedArgs a) {
   constexpr bool F32 = std::is_same_v<T, float>;
   static_assert(!F32 || (!Q8 && D <= 128), "fp32 caches are not quantised, of up to 128 channels");
   using PT = std::conditional_t<Q8, bf16, T>;  // the value tiles
   constexpr int NP = Q8 && std::is_same_v<T, f16> ? 2 : 1;  // parts of P
-  constexpr int NWV = kWaves<T, D, WR>, WK = NWV / WR, NS = kStages<Q8>;
-  constexpr int PAIR = kPair<T, D>, TILE = PAIR / 2;
-  constexpr int BLK = TILE / 1024;             // 1 KiB DMA blocks a tile
-  constexpr int LPT = (2 * BLK + WR - 1) / WR;  // DMA loads a wave issues for a pair (WR > 1)
+  constexpr int NWV = kWaves<T, D, WR>, WK = NWV / WR, NS = kStages<Q8, WR>;
+  constexpr int PAIR = Q8 ? kPair<T, D> / 2 : kPair<T, D>, TILE = PAIR / 2;
+  constexpr int BLK = TILE / 1024;        // 1 KiB DMA blocks a tile
+  constexpr int LK = BLK + (Q8 ? 2 : 0), LV = BLK;  // loads of a K tile (and both tiles' scales), a V tile
+  constexpr int LPT = (LK + LV + WR - 1) / WR;      // loads a wave issues for a pair (WR > 1)
   constexpr int PDT = D / 32;
-  constexpr int SCALES = Q8 ? 256 : 0;
-  constexpr int STAGE = PAIR + SCALES, RING = WR == 1 && !Q8 ? PAIR : NS * STAGE;
+  // the stages, then (codes) one place more for 64 floats of K's and 64 of V's scales, half
+  // of each in use: a tile's are read after its K's place is loaded again
+  constexpr int RING = NS * PAIR + (Q8 ? (NS + 1) * 512 : 0);
   constexpr int MERGE = WK > 1 ? NWV * 32 * (D + 2) * 4 : 0;
   constexpr int LDS_B = WK * RING > MERGE ? WK * RING : MERGE;
-  static_assert(WR == 1 || (2 * BLK) % WR == 0 || Q8, "a pair's blocks split over the waves");
+  static_assert((WR > 1 ? LPT : NS * (LK + LV)) < 64, "loads in flight that a wait can count");
   __shared__ __attribute__((aligned(1024))) char lds[LDS_B];
 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
@@ -179,14 +241,16 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
   // keys below `border` are hidden from some row
   const int border = a.window ? a.n - a.window : 0;
 
-  // Q rows as B operands: 16-bit, channels 16 ks + 8 h .. + 7; f32, the half h of the row
+  // Q rows as B operands: 16-bit, channels 16 ks + 8 h .. + 7 (over codes in CodeTile's
+  // order); f32, the half h of the row
   constexpr int NQ = F32 ? D / 8 : D / 16;  // 16-byte pieces a lane holds
   u32x4 qf[NQ];
   {
     const T *qp = static_cast<const T *>(a.q.data) + b * a.q.s0 + static_cast<int64_t>(hk * a.rep + rr) * a.q.s1 +
-                  static_cast<int64_t>(t) * a.q.s2 + (F32 ? h * (D / 2) : 8 * h);
+                  static_cast<int64_t>(t) * a.q.s2 + (F32 ? h * (D / 2) : Q8 ? 16 * h : 8 * h);
+    auto channel = [](int i) { return F32 ? 4 * i : Q8 ? 32 * (i >> 1) + 8 * (i & 1) : 16 * i; };
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) qf[i] = ld16(qp + (F32 ? 4 : 16) * i);
+    for (int i = 0; i < NQ; ++i) qf[i] = ld16(qp + channel(i));
     if (a.rope.R > 0) {
       if constexpr (F32) {
         const float *cs = static_cast<const float *>(a.rope.cos) + static_cast<int64_t>(pos) * (D / 2) + h * (D / 4);
@@ -204,7 +268,7 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
         int64_t at[NQ];
         int p0[NQ];
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) at[i] = pos, p0[i] = 8 * i + 4 * h;
+        for (int i = 0; i < NQ; ++i) at[i] = pos, p0[i] = (channel(i) + (Q8 ? 16 : 8) * h) / 2;
         rotate_chunks<T, NQ>(qf, a.rope, at, p0, false);
       }
     }
@@ -223,8 +287,8 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
   char *ring = lds + wk * RING;
   const uint32_t ring0 = lds_addr(lds) + wk * RING;
 
-  using Rows = RowTile<std::conditional_t<F32, bf16, T>, D>;
-  const Rows rd(lane);
+  using Tile = std::conditional_t<F32, FTile<D>, std::conditional_t<Q8, CodeTile<D>, RowTile<std::conditional_t<F32, bf16, T>, D>>>;
+  const std::conditional_t<F32, RowTile<bf16, D>, Tile> rd(lane);  // (FTile's reads keep no state)
   // S^T of a K tile: element i is key crow(i, h)
   auto scores = [&](const char *kt) __attribute__((always_inline)) {
     f32x16 s = f32x16{};
@@ -237,6 +301,13 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
         s = mfma32f(x.y, __builtin_bit_cast(float, q1), s);
         s = mfma32f(x.z, __builtin_bit_cast(float, q2), s);
         s = mfma32f(x.w, __builtin_bit_cast(float, q3), s);
+      }
+    } else if constexpr (Q8) {
+#pragma unroll
+      for (int j = 0; j < NQ / 2; ++j) {
+        const u32x4 x = rd.rows(kt, j);
+        s = mfma32<T>(widen<T>(x[0], x[1]), qf[2 * j], s);
+        s = mfma32<T>(widen<T>(x[2], x[3]), qf[2 * j + 1], s);
       }
     } else {
 #pragma unroll
@@ -285,7 +356,7 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
     if constexpr (Q8) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const float4 f = *reinterpret_cast<const float4 *>(scales + 32 + 8 * g + 4 * h);
+        const float4 f = *reinterpret_cast<const float4 *>(scales + 64 + 8 * g + 4 * h);
         p[4 * g] *= f.x, p[4 * g + 1] *= f.y, p[4 * g + 2] *= f.z, p[4 * g + 3] *= f.w;
       }
     }
@@ -309,6 +380,21 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
 #pragma unroll
         for (int dt = 0; dt < PDT; ++dt)
           oacc[dt] = mfma32f(FTile<D>::elem(vt, 8 * (i >> 2) + 4 * h + (i & 3), 32 * dt + c), p[i], oacc[dt]);
+    } else if constexpr (Q8) {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        u32x2 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = rd.key(vt, ks, j >> 2, j & 3);
+#pragma unroll
+        for (int dt = 0; dt < PDT; ++dt) {
+          u32x4 f;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) f[j >> 1] = pack2<PT>(code(x[j], dt), code(x[j + 1], dt));
+#pragma unroll
+          for (int n = 0; n < NP; ++n) oacc[dt] = mfma32<PT>(f, pb[n][ks], oacc[dt]);
+        }
+      }
     } else {
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks)
@@ -325,134 +411,93 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
   const uint32_t ks_b = static_cast<uint32_t>(a.k.s2) * sizeof(KT), vs_b = static_cast<uint32_t>(a.v.s2) * sizeof(KT);
   const KT *kbase = static_cast<const KT *>(a.k.data) + b * a.k.s0 + hk * a.k.s1;
   const KT *vbase = static_cast<const KT *>(a.v.data) + b * a.v.s0 + hk * a.v.s1;
-  if constexpr (!Q8) {
-    // Keys past the cache's end, and tiles past the wave's last, read as zeros.
-    const u32x4 kdesc = make_desc(kbase, static_cast<uint32_t>(a.n) * ks_b);
-    const u32x4 vdesc = make_desc(vbase, static_cast<uint32_t>(a.n) * vs_b);
-    // block n of a K or V tile whose first row is at byte `base`, to LDS address st
-    auto block = [&](u32x4 desc, uint32_t stride, uint32_t base, uint32_t st, int n) __attribute__((always_inline)) {
-      using Tile = std::conditional_t<F32, FTile<D>, Rows>;
-      dma16(desc, st + n * 1024, Tile::dma_off(n, lane, stride), base + static_cast<uint32_t>(n * Tile::RPB) * stride);
-    };
-    auto first_row = [&](int i, uint32_t stride) __attribute__((always_inline)) {
-      return i < mine ? static_cast<uint32_t>(key0(i)) * stride : 0x80000000u;
-    };
-    if constexpr (WR == 1) {
-      auto issue = [&](u32x4 desc, uint32_t stride, int i, uint32_t st) __attribute__((always_inline)) {
-        const uint32_t base = first_row(i, stride);
-#pragma unroll
-        for (int n = 0; n < BLK; ++n) block(desc, stride, base, st, n);
-      };
-      issue(kdesc, ks_b, 0, ring0);
-      issue(vdesc, vs_b, 0, ring0 + TILE);
-      for (int i = 0; i < mine; ++i) {
-        wait_vm_n<BLK>();  // K of tile i; V in flight
-        __builtin_amdgcn_sched_barrier(0);
-        const f32x16 s = scores(ring);
-        wait_lgkm0();  // read
-        __builtin_amdgcn_sched_barrier(0);
-        issue(kdesc, ks_b, i + 1, ring0);
-        softmax(s, key0(i), nullptr);
-        __builtin_amdgcn_sched_barrier(0);
-        wait_vm_n<BLK>();  // V of tile i; the next K in flight
-        __builtin_amdgcn_sched_barrier(0);
-        values(ring + TILE);
-        wait_lgkm0();
-        __builtin_amdgcn_sched_barrier(0);
-        issue(vdesc, vs_b, i + 1, ring0 + TILE);
-      }
-      wait_vm_n<0>();
+  // Keys past the cache's end, and tiles past the wave's last, read as zeros.
+  const u32x4 kdesc = make_desc(kbase, static_cast<uint32_t>(a.n) * ks_b);
+  const u32x4 vdesc = make_desc(vbase, static_cast<uint32_t>(a.n) * vs_b);
+  u32x4 ksdesc{}, vsdesc{};
+  uint32_t kss_b = 0, vss_b = 0;
+  if constexpr (Q8) {
+    kss_b = static_cast<uint32_t>(a.ks.s2) * 4, vss_b = static_cast<uint32_t>(a.vs.s2) * 4;
+    ksdesc = make_desc(static_cast<const float *>(a.ks.data) + b * a.ks.s0 + hk * a.ks.s1, static_cast<uint32_t>(a.n) * kss_b);
+    vsdesc = make_desc(static_cast<const float *>(a.vs.data) + b * a.vs.s0 + hk * a.vs.s1, static_cast<uint32_t>(a.n) * vss_b);
+  }
+  auto first_row = [&](int i, uint32_t stride) __attribute__((always_inline)) {
+    return i < mine ? static_cast<uint32_t>(key0(i)) * stride : 0x80000000u;
+  };
+  // load n of tile i: K's blocks, the scales, V's blocks
+  auto load = [&](int i, int n) __attribute__((always_inline)) {
+    const uint32_t st = ring0 + (i % NS) * PAIR, sc = ring0 + NS * PAIR + (i % (NS + 1)) * 512;
+    if (Q8 && n >= BLK && n < LK) {  // (lanes 32 .. 63 fetch the same again)
+      const bool v = n > BLK;
+      const uint32_t stride = v ? vss_b : kss_b;
+      dma4(v ? vsdesc : ksdesc, sc + (v ? 256 : 0), static_cast<uint32_t>(lane & 31) * stride, first_row(i, stride));
     } else {
-      // wave w loads blocks w, w + WR, .. of a pair, K's first; two tiles ahead
-      auto issue = [&](int i) __attribute__((always_inline)) {
-        const uint32_t kb = first_row(i, ks_b), vb = first_row(i, vs_b), st = ring0 + (i % NS) * STAGE;
-#pragma unroll
-        for (int u = 0; u < LPT; ++u) {
-          const int n = w + WR * u;
-          if (n < BLK) block(kdesc, ks_b, kb, st, n);
-          else block(vdesc, vs_b, vb, st + TILE, n - BLK);
-        }
-      };
-      issue(0);
-      issue(1);
-      for (int i = 0; i < mine; ++i) {
-        const char *kt = ring + (i % NS) * STAGE;
-        wait_vm_n<LPT>();  // this wave's blocks of tile i
-        wait_lgkm0();
-        phase_barrier();  // every wave's; and tile i - 1 is read
-        issue(i + 2);
-        softmax(scores(kt), key0(i), nullptr);
-        values(kt + TILE);
-      }
-      wait_vm_n<0>();
+      const bool v = n >= LK;
+      const int at = v ? n - LK : n;
+      const uint32_t stride = v ? vs_b : ks_b;
+      dma16(v ? vdesc : kdesc, st + (v ? TILE : 0) + at * 1024, Tile::dma_off(at, lane, stride),
+            first_row(i, stride) + static_cast<uint32_t>(at * Tile::RPB) * stride);
     }
-  } else {
-    // Codes come through registers, a tile ahead, and are widened into 16-bit tiles.
-    constexpr int LANES = 64 * WR, PIECES = BN * D / 16;  // 16 codes a piece
-    constexpr int NPC = (PIECES + LANES - 1) / LANES;
-    const int gl = WR > 1 ? tid : lane;
-    u32x4 kc[NPC], vc[NPC];
-    float sc = 0.f;  // lanes 0 .. 31 of the group: K's scales, 32 .. 63: V's
-    auto fetch = [&](int i) __attribute__((always_inline)) {
-      const int kv0 = i < mine ? key0(i) : a.n;
+  };
+  auto scales_of = [&](int i) __attribute__((always_inline)) {
+    return reinterpret_cast<const float *>(ring + NS * PAIR + (i % (NS + 1)) * 512);
+  };
+  if constexpr (WR == 1) {
+    // a tile's places are loaded again, NS tiles on, as soon as they are read
+    auto issue = [&](int i, int from, int to) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < NPC; ++u) {
-        const int at = u * LANES + gl, key = kv0 + at / (D / 16), col = at % (D / 16) * 16;
-        kc[u] = vc[u] = u32x4{0, 0, 0, 0};
-        if (at < PIECES && key < a.n) {
-          kc[u] = ld16(kbase + static_cast<int64_t>(key) * a.k.s2 + col);
-          vc[u] = ld16(vbase + static_cast<int64_t>(key) * a.v.s2 + col);
-        }
-      }
-      if (gl < 64) {
-        const int key = kv0 + (gl & 31);
-        const View &s = gl < 32 ? a.ks : a.vs;
-        sc = key < a.n ? static_cast<const float *>(s.data)[b * s.s0 + hk * s.s1 + static_cast<int64_t>(key) * s.s2] : 0.f;
-      }
+      for (int n = from; n < to; ++n) load(i, n);
     };
-    auto place = [&](int i) __attribute__((always_inline)) {
-      char *st = ring + (i & 1) * STAGE;
 #pragma unroll
-      for (int u = 0; u < NPC; ++u) {
-        const int at = u * LANES + gl, r = at / (D / 16), ch = at % (D / 16) * 2;
-        if (PIECES % LANES && at >= PIECES) continue;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int k = ch + e;
-          char *to = st + Rows::at(r, k);
-          *reinterpret_cast<u32x4 *>(to) = widen<T>(kc[u][2 * e], kc[u][2 * e + 1]);
-          *reinterpret_cast<u32x4 *>(to + TILE) = widen<PT>(vc[u][2 * e], vc[u][2 * e + 1]);
-        }
-      }
-      if (gl < 64) *reinterpret_cast<float *>(st + PAIR + 4 * gl) = sc;
-    };
-    auto settle = [&] {  // tile i is in LDS for all of its waves
-      if constexpr (WR > 1) {
-        __syncthreads();
-      } else {
-        wait_lgkm0();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-      }
-    };
-    if (mine > 0) {
-      fetch(0);
-      place(0);
-      fetch(1);
-    }
+    for (int i = 0; i < NS; ++i) issue(i, 0, LK + LV);
     for (int i = 0; i < mine; ++i) {
-      settle();
-      if (i + 1 < mine) {
-        place(i + 1);
-        fetch(i + 2);
+      const char *kt = ring + (i % NS) * PAIR;
+      wait_vm_n<NS * LV + (NS - 1) * LK>();  // K of tile i; V and what follows in flight
+      __builtin_amdgcn_sched_barrier(0);
+      const f32x16 s = scores(kt);
+      wait_lgkm0();  // read
+      __builtin_amdgcn_sched_barrier(0);
+      issue(i + NS, 0, LK);
+      softmax(s, key0(i), scales_of(i));
+      __builtin_amdgcn_sched_barrier(0);
+      wait_vm_n<NS * LK + (NS - 1) * LV>();  // V of tile i
+      __builtin_amdgcn_sched_barrier(0);
+      values(kt + TILE);
+      wait_lgkm0();
+      __builtin_amdgcn_sched_barrier(0);
+      issue(i + NS, LK, LK + LV);
+    }
+    wait_vm_n<0>();
+  } else {
+    // wave w issues loads w, w + WR, .. of a pair, the last one again where they do not
+    // come out even; two tiles ahead
+    auto issue = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < LPT; ++u) {
+        const int n = w + WR * u;
+        load(i, n < LK + LV ? n : LK + LV - 1);
       }
-      const char *kt = ring + (i & 1) * STAGE;
-      softmax(scores(kt), key0(i), reinterpret_cast<const float *>(kt + PAIR));
+    };
+    issue(0);
+    issue(1);
+    for (int i = 0; i < mine; ++i) {
+      const char *kt = ring + (i % NS) * PAIR;
+      wait_vm_n<LPT>();  // this wave's loads of tile i
+      wait_lgkm0();
+      phase_barrier();  // every wave's; and tile i - 1 is read
+      issue(i + 2);
+      softmax(scores(kt), key0(i), scales_of(i));
       values(kt + TILE);
     }
+    wait_vm_n<0>();
   }
 
-  // Lane holds O^T[channel 32 dt + 8 g + 4 h + r][row c] in oacc[dt][4 g + r].
+  // Lane holds O^T[row 8 g + 4 h + r of block dt][row c] in oacc[dt][4 g + r]: four
+  // neighbouring channels are r = 0 .. 3 of a block, over codes (CodeTile) of D / 32 blocks
+  // side by side.
+  auto block_of = [](int q, int j) { return Q8 ? (4 * (q % PDT) + j) % PDT : q >> 2; };
+  auto element = [](int q, int j) { return Q8 ? 4 * (q / PDT) + (4 * (q % PDT) + j) / PDT : 4 * (q & 3) + j; };
+  auto channel4 = [&](int q) { return Q8 ? PDT * (8 * (q / PDT) + 4 * h) + 4 * (q % PDT) : 8 * q + 4 * h; };
   const int64_t rows = static_cast<int64_t>(bhs) * a.R, at = static_cast<int64_t>(bh) * a.R + row;
   float *po = a.ws + (part * rows + at) * D;
   float *ml = a.ws + a.splits * rows * D + 2 * (part * rows + at);
@@ -472,13 +517,12 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
     if (!live) return;
     const float inv = lt > 0.f ? 1.f / lt : 0.f;
 #pragma unroll
-    for (int dt = 0; dt < PDT; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        store(32 * dt + 8 * g + 4 * h,
-              float4{oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]}, inv);
+    for (int q = 0; q < 4 * PDT; ++q)
+      store(channel4(q),
+            float4{oacc[block_of(q, 0)][element(q, 0)], oacc[block_of(q, 1)][element(q, 1)],
+                   oacc[block_of(q, 2)][element(q, 2)], oacc[block_of(q, 3)][element(q, 3)]}, inv);
   } else {
-    // the waves' results, joined in their order; wave w stores groups w, w + NWV, ..
+    // the waves' results, joined in their order; wave w stores fours w, w + NWV, .. of channels
     __syncthreads();  // every ring is read
     float *cm = reinterpret_cast<float *>(lds), *cl = cm + NWV * 32, *co = cl + NWV * 32;
     if (h == 0) cm[w * 32 + c] = m, cl[w * 32 + c] = lt;
@@ -500,14 +544,14 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (Q8 && WR == 1 ? 1 : kTwo<
     }
     if (!live) return;
     const float inv = lt > 0.f ? 1.f / lt : 0.f;
-    for (int g = w; g < PDT * 4; g += NWV) {
+    for (int q = w; q < PDT * 4; q += NWV) {
       float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int v = 0; v < NWV; ++v)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          x[r] = fmaf(co[((v * PDT + (g >> 2)) * 16 + 4 * (g & 3) + r) * 64 + lane], f[v], x[r]);
-      store(8 * g + 4 * h, float4{x[0], x[1], x[2], x[3]}, inv);
+          x[r] = fmaf(co[((v * PDT + block_of(q, r)) * 16 + element(q, r)) * 64 + lane], f[v], x[r]);
+      store(channel4(q), float4{x[0], x[1], x[2], x[3]}, inv);
     }
     if (w) return;
   }
@@ -638,11 +682,19 @@ CachedPlan plan_cached(const CachedProblem &p) {
   s.ns = sunk < first ? sunk : first;
   s.gap = first - s.ns;
   s.run = tiles - s.gap;
-  // two workgroups a CU (of small tiles four), each of 4 tiles a wave or more
+  // A wave for each SIMD: a second one costs a few tokens over 16 or 32 bits more in partial
+  // results (step of 32 sequences, window 4096 of 8 heads of 128: 96 us, with two 102).
+  // Codes, and rows enough for several waves, keep a SIMD busy beside the loads, and take
+  // two where the parts stay few (63 tokens of 16 sequences over 8000 keys, 8 heads of 128:
+  // 241 us in one part, 204 in two; 16 heads, 24 tokens of 7 sequences, codes: 38 us in 9
+  // parts, 40 in 18).  A wave has 4 tiles or more to itself, of slower f32 ones 2 (17
+  // tokens over 900 keys, 4 heads of 32: 18 us with 4, 14 with 2).
   const int64_t base = static_cast<int64_t>(p.B) * p.Hkv * s.groups;
-  const int pair = 64 * p.D * (p.dtype == TSATTN_F32 ? 4 : 2);
-  const int least = 4 * (s.wr > 1 ? 1 : pair <= 16384 ? 4 : 2);
-  int64_t n = (pair <= 8192 ? 1024 : 512) / base;
+  const int waves = s.wr > 1 ? s.wr : 64 * p.D * (p.dtype == TSATTN_F32 ? 4 : 2) <= 16384 ? 4 : 2;
+  int64_t n = 1024 / waves / base;
+  if (n < 1) n = 1;
+  if (n <= 2 && (p.q8 || s.wr > 1)) n *= 2;
+  const int least = (p.dtype == TSATTN_F32 ? 2 : 4) * (s.wr > 1 ? 1 : waves);
   if (n > s.run / least) n = s.run / least;
   s.splits = n < 1 ? 1 : static_cast<int>(n);
   return s;
