@@ -1278,6 +1278,8 @@ int tsattn_token_probs_backward(int32_t dtype, int64_t rows, int32_t vocab, cons
   if (rc) return rc;
   if (!stats || !dlogits || (g_entropy && !entropy) || (g_top && (!top || !top_indices)))
     return fail(TSATTN_ERR_INVALID, "data pointer is NULL");
+  if (reinterpret_cast<uintptr_t>(dlogits) % (dtype == TSATTN_F32 ? 4 : 2))
+    return fail(TSATTN_ERR_INVALID, "the logits' gradient must be aligned to its elements");
   return hip_status(tsattn::launch_token_probs_backward(dtype, rows, vocab, logits, row_stride, tokens, token_bytes,
                                                         ignore, top, stats, entropy, top_indices, g_log_probs,
                                                         g_entropy, g_top, dlogits, static_cast<hipStream_t>(stream)),

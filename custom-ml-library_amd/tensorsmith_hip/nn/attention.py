@@ -125,17 +125,18 @@ def _forward(lib, prob, rope, vq, vk, vv, vo, lse_ptr, tdev, stream) -> None:
 
 
 def _check_window(window, sinks, is_causal: bool, span: int):
-    """The window as the kernels take it: None where it reaches past the first of ``span`` positions."""
+    """Window and sinks as the kernels take them: (None, 0) where the window reaches past the first of ``span``
+    positions."""
     whole = lambda x: isinstance(x, (int, np.integer)) and not isinstance(x, bool)  # noqa: E731
     if not whole(sinks) or sinks < 0 or (sinks and window is None):
         raise ValueError("sinks must be a nonnegative number of keys in front of a window")
     if window is None:
-        return None
+        return None, 0
     if not whole(window) or window < 1:
         raise ValueError("window must be a positive number of keys")
     if not is_causal:
         raise ValueError("a window needs causal attention")
-    return None if window >= span else int(window)
+    return (None, 0) if window >= span else (int(window), min(int(sinks), span))
 
 
 def _banded(mask, window: int, sinks: int, qlen: int, klen: int, offset: int, dev) -> Tensor:
@@ -240,7 +241,7 @@ def scaled_dot_product_attention(
         raise ValueError("attention dropout currently requires the dense backend")
     if backend == "native":
         raise ValueError("native attention requires Metal and equal query/value head dimensions")
-    window = _check_window(window, sinks, is_causal, qlen + causal_offset)
+    window, sinks = _check_window(window, sinks, is_causal, qlen + causal_offset)
 
     code = _dtype_code(query.dtype)
     q, k, v = (_operand(t._data) for t in (query, key, value))

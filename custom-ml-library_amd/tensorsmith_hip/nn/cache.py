@@ -19,6 +19,7 @@ going through ``get``.
 from __future__ import annotations
 
 import math
+import operator
 
 import numpy as np
 
@@ -151,6 +152,7 @@ class KVCache:
         ``first``): they become the positions first .. first + n - 1, the cache's last.  One kernel reads all of them
         before it writes any (``tsattn_cache_keep``), so their order is free.  Indices on the host are checked; a hip
         tensor's are not waited for, and where one is out of range the position keeps what it held."""
+        first = operator.index(first)
         if not 0 <= first <= self.length:
             raise ValueError("first must be between zero and the current length")
         drafted = self.length - first
@@ -246,6 +248,7 @@ class KVCache:
 
     def get(self, last: int | None = None) -> tuple[Tensor, Tensor]:
         """Keys and values of the active prefix, or of its ``last`` positions."""
+        last = None if last is None else operator.index(last)
         if last is not None and not 0 <= last <= self.length:
             raise ValueError("last must be between zero and the current length")
         part = slice(0 if last is None else self.length - last, self.length)

@@ -60,6 +60,8 @@ class DraftTree:
             raise RuntimeError("tensorsmith_hip keeps draft trees on hip devices")
         self.tokens, self.trees, self._shape = shape[-1], shape[0] if len(shape) == 2 else 1, shape
         raw = parents._data if on_device else torch.from_numpy(host.astype(np.int32)).to(self.device.torch)
+        if raw.dtype == torch.int64:  # (no value wraps round to an earlier token)
+            raw = raw.clamp(-1, MOST_TOKENS)
         raw = raw.to(torch.int32).reshape(self.trees, self.tokens).contiguous()
         self._words = torch.empty((self.trees, self.tokens, -(-self.tokens // 32)), dtype=torch.int32, device=raw.device)
         self._depths = torch.empty((self.trees, self.tokens), dtype=torch.int32, device=raw.device)
@@ -135,7 +137,7 @@ def cached_attention(query: Tensor, cache: KVCache, tree: DraftTree | None = Non
         raise ValueError("attention scale must be finite")
     check_rotary(rotary_base, dim)
     whole = window
-    window = _check_window(window, sinks, True, length)
+    window, sinks = _check_window(window, sinks, True, length)
     if tree is not None:
         tree._check(b, tokens, dev)
         if whole is not None and whole < tokens:
@@ -151,7 +153,7 @@ def cached_attention(query: Tensor, cache: KVCache, tree: DraftTree | None = Non
         if rotary_base is not None:
             cos, sin = (x.data_ptr() for x in rope_tables(rotary_base, dim, q.dtype, q.device, length))
         desc = _lib.Cached(code, b, heads, cache.num_heads, dim, tokens, length, cache.quantized,
-                           1 / math.sqrt(dim) if scale is None else scale, window or 0, sinks if window else 0, trees,
+                           1 / math.sqrt(dim) if scale is None else scale, window or 0, sinks, trees,
                            words, depths, cos, sin)
         lib = _lib.load()
         out = torch.empty((b, heads, tokens, dim), dtype=q.dtype, device=q.device)
@@ -169,7 +171,7 @@ def cached_attention(query: Tensor, cache: KVCache, tree: DraftTree | None = Non
     if tree is None:
         q = query if rotary_base is None else rotary_embedding(query, first, rotary_base)
         return scaled_dot_product_attention(q, k, v, None, 0.0, True, scale=scale, causal_offset=first,
-                                            enable_gqa=True, window=window, sinks=sinks if window else 0)
+                                            enable_gqa=True, window=window, sinks=sinks)
     positions = first + tree._depths
     if rotary_base is not None:
         query = Tensor._leaf(_rotate_at(q, positions, rotary_base), query.device)

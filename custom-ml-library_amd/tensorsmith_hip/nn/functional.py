@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from typing import NamedTuple
 
 from .. import _lib
@@ -455,6 +456,7 @@ def token_log_probs(input: Tensor, target: Tensor, top_k: int = 0, *, ignore_ind
     classes = given[-1]
     if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(classes, 64):
         raise ValueError("top_k must be between zero and 64 and within the classes")
+    padding = operator.index(ignore_index)
     _require_hip(input, "token_log_probs")
     code = _code(x)
     if code < 0:
@@ -480,7 +482,7 @@ def token_log_probs(input: Tensor, target: Tensor, top_k: int = 0, *, ignore_ind
     lib = _lib.load()
     at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     # (logits, stride, tokens, ..): what both passes are given first
-    operands = (code, rows, classes, z.data_ptr(), z.stride(0), y.data_ptr(), y.element_size(), ignore_index, top_k)
+    operands = (code, rows, classes, z.data_ptr(), z.stride(0), y.data_ptr(), y.element_size(), padding, top_k)
     if rows:
         nbytes = lib.tsattn_token_probs_workspace(rows, classes, top_k)
         if nbytes:

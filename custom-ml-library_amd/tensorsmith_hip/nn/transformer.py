@@ -229,6 +229,8 @@ class MultiHeadAttention(Module):
         if tree is not None:
             if not isinstance(cache, KVCache) or attn_mask is not None or not is_causal:
                 raise ValueError("drafted tokens need a KVCache and take no other mask")
+            if self.window is not None and self.window < steps:  # (before the cache takes them)
+                raise ValueError("the window must hold the drafted tokens")
             q, k, v = (proj(input).reshape(batch, steps, heads, self.head_dim).permute(0, 2, 1, 3)
                        for proj, heads in ((self.q_proj, self.num_heads), (self.k_proj, self.num_kv_heads),
                                            (self.v_proj, self.num_kv_heads)))
@@ -311,10 +313,11 @@ class MultiHeadAttention(Module):
 
     def _paged(self, input: Tensor, cache: PagedKVCache, attn_mask, is_causal: bool) -> Tensor:
         """Self-attention over a paged 4-bit cache, each row at its own position.  As over an int8 cache,
-        ``backend`` chooses only where a mask or a window has the values read back as arrays."""
+        ``backend`` chooses only where a mask, or a window over more than it holds, has the values read back as
+        arrays."""
         batch, steps, _ = input.shape
         lens = cache.lengths
-        read_back = attn_mask is not None or self.window is not None
+        read_back = attn_mask is not None or (self.window is not None and self.window < max(lens) + steps)
         if read_back and min(lens) != max(lens):
             raise ValueError("attention masks and windows over a paged cache need rows of one length")
         q, k, v = (proj(input).reshape(batch, steps, heads, self.head_dim).permute(0, 2, 1, 3)

@@ -366,3 +366,62 @@ def test_a_captured_round_replays_and_another_stream_agrees():
         assert torch.equal(got, step(caches[1]))
         for x, y in zip(caches[0].storage[:2], caches[1].storage[:2]):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("tokens", [1, 9, 20, 40])
+def test_long_int8_caches_are_cut_in_parts(tokens, d, dtype):
+    """Scales from 2^-8 to 2^8 of neighbouring rows, so that a code under another row's scale shows."""
+    b, hkv, rep, n = 2, 3, 4, 4321
+    cache = _cache(b, hkv, n, d, dtype, int8=True)
+    for scales in cache.storage[2:]:
+        scales *= 2.0 ** torch.randint(-8, 9, scales.shape, device="cuda")
+    q = _rows(b, hkv * rep, tokens, d, dtype, 7) * 2.0 ** -8
+    for window, sinks in ((4000, 0), (777, 65)):
+        got = _attend(q, cache, window=window, sinks=sinks)
+        _close(got, _reference(q, cache, _band(tokens, n, window, sinks)), dtype)
+    parents = _parents(np.random.default_rng(tokens), b, tokens)
+    seen = torch.ones(b, 1, tokens, n, dtype=torch.bool, device="cuda")
+    seen[:, 0, :, n - tokens:] = torch.from_numpy(_ancestors(parents)).cuda()
+    _close(_attend(q, cache, nn.DraftTree(parents)), _reference(q, cache, seen), dtype)
+
+
+def test_scales_that_lie_apart_or_are_shared_by_rows():
+    """Scales of a wider stride are read where they lie; one for all rows has no kernel and is dequantised."""
+    b, hkv, n, d = 1, 2, 300, 64
+    cache = _cache(b, hkv, n, d, torch.float16, int8=True)
+    q = _rows(b, 4, 3, d, torch.float16, 7)
+    want = _attend(q, cache, window=100)
+    for name in ("_key_scales", "_value_scales"):
+        apart = torch.full((b, hkv, n, 3), 1e30, device="cuda")
+        apart[..., :1] = getattr(cache, name)
+        setattr(cache, name, apart[..., :1])
+    cache._described = ()
+    assert torch.equal(_attend(q, cache, window=100), want)
+    cache._key_scales = torch.full((b, hkv, 1, 1), 0.01, device="cuda").expand(b, hkv, n, 1)
+    cache._described = ()
+    _close(_attend(q, cache, window=100), _reference(q, cache, _band(3, n, 100, 0)), torch.float16)
+
+
+def test_windows_over_a_paged_cache():
+    """A window over all positions leaves the paged kernels on; a smaller one reads the values back."""
+    x = _wrap(torch.randn(2, 50, 128, generator=_gen(3), device="cuda").half())
+    layers = []
+    for window in (None, 50, 20):
+        ts.seed(5)
+        layers.append(nn.MultiHeadAttention(128, 4, num_kv_heads=2, rotary=False, window=window, sinks=0 if window is None else 2,
+                                            device="hip").eval().to(dtype="float16"))
+    with ts.no_grad():
+        got, caches = [], []
+        for layer in layers:
+            caches.append(nn.PagedKVCache(2, 2, 32, 64, device="hip", dtype="float16"))
+            got.append([layer(x[:, :45], cache=caches[-1])._data, layer(x[:, 45:], cache=caches[-1])._data])
+        for one, other in zip(got[0], got[1]):
+            assert torch.equal(one, other)
+        k, v = (y._data.double().repeat_interleave(2, 1) for y in caches[2].get())
+        q = layers[2].q_proj(x)._data.double().reshape(2, 50, 4, 32).permute(0, 2, 1, 3)[:, :, 45:]
+        s = (torch.matmul(q, k.transpose(-1, -2).contiguous()) / math.sqrt(32)).masked_fill(~_band(5, 50, 20, 2), -math.inf)
+        want = torch.matmul(torch.softmax(s, -1), v).permute(0, 2, 1, 3).reshape(2, 5, 128)
+        want = torch.matmul(want, layers[2].out_proj.weight._data.double().t().contiguous())
+    assert (got[2][1].double() - want).norm() <= 1e-2 * want.norm()
