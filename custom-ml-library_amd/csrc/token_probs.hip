@@ -16,9 +16,11 @@
 // gradient.  One pass in each: a lane keeps a running (b, l, sum 2^t t) and rescales it
 // once for every four 16-byte pieces.  The forward is about as far from the vector units'
 // bound: 6 instructions a logit; 11 of them (selects for rows' ends and -inf on every
-// one) took 131 us where 8192 rows of 50021 bf16, a fifth of them ignored, take 105.
+// one) took 131 us where 8192 rows of 50021 bf16, a fifth of them ignored, take 107
+// (6.1 TB/s).  The VJP of those takes 285 us, 5.2 TB/s of reads and writes, as a copy; 331
+// before its rows' pieces began on whole lines of memory.
 //
-// A row belongs to one wave (V <= kWaveRow), to a workgroup of four, or, when the rows
+// A row belongs to one wave (wave_rows), to a workgroup of four, or, when the rows
 // are too few to fill the chip, to several workgroups that each take a part of it; a
 // second kernel then combines the parts in their order.  Results depend on the sizes
 // alone, no atomics.
@@ -599,20 +601,23 @@ __global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
   }
 }
 
-// Vocabularies up to this many logits take a wave a row: then its 16 pieces a lane are
-// little more than the reduction costs (f16 pieces of 8; V 1009 f32: 4).
-constexpr int kWaveRow = 2048;
 constexpr int kMaxSplits = 64;
 
-bool wave_rows(int64_t rows, int vocab) { return vocab <= kWaveRow; }
+// Rows short enough for a wave each: four of them cost the workgroup's reduction between
+// its waves (8192 rows of 2000 bf16, forward and VJP: 14 and 15 us, a workgroup a row 21
+// and 23; of 4000: 18 and 26, against 25 and 28; of 8000 the VJP is slower, 52 and 46).
+// Few rows have the chip to themselves and gain from four waves sooner (64 rows of 3500,
+// five top tokens: 15 us a wave a row, 11 a workgroup; of 1500: 11 both).
+bool wave_rows(int64_t rows, int vocab) { return vocab <= (rows >= 4096 ? 4096 : 2048); }
 
-// Parts of a row: as many as give the chip's 256 CUs 4 workgroups each, of 8192 logits
-// or more (8 pieces a lane; shorter parts end before their loads pay for the start and
-// the second kernel).
+// Parts of a row: as many as give the chip's 256 CUs 4 workgroups each (64 rows of 50000
+// in 1 to 16 parts: 11 us all; 256 rows, forward and VJP: 14 and 17 us in one part, 14 and
+// 13 in four, 16 and 14 in eight), of 2048 logits or more (a row of 32000 with five top
+// tokens: 14.4 us, with 8192 or more 16.4, with 16384 21).
 int prob_splits(int64_t rows, int vocab) {
   if (wave_rows(rows, vocab)) return 1;
   int64_t s = 1024 / rows;
-  if (s > vocab / 8192) s = vocab / 8192;
+  if (s > vocab / 2048) s = vocab / 2048;
   if (s > kMaxSplits) s = kMaxSplits;
   return s < 1 ? 1 : static_cast<int>(s);
 }

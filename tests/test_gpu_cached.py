@@ -2,9 +2,10 @@
 the tree's plan, its append and the rows that are kept, against float64 and array
 operations.
 
-Bounds: over f16 and bf16 caches P rounds to the type (2^-12, 2^-9 a term, over int8 codes
-2^-9 and for f16 queries 2^-17) and the result once (2^-12, 2^-9): relative 2-norms of a
-row below 1e-2; in f32 below 2e-5.  A key too many or too few moves a row by the order of
+Bounds: over f16 and bf16 caches P rounds to the type (2^-11, 2^-8 a term at most, over int8
+codes 2^-8 and for f16 queries 2^-16) and the result once (2^-11, 2^-8): at most 2^-7 of the
+terms' sizes, and relative 2-norms of a row, whose roundings are independent, below 1e-2; in
+f32 below 2e-5.  A key too many or too few moves a row by the order of
 its size divided by the number of keys that it sees, which the short contexts make large.
 """
 

@@ -289,3 +289,17 @@ def test_a_model_scores_its_tokens():
     for n, p in model.named_parameters():
         scale = p._grad.double().norm()
         assert (grads[n].double() - p._grad.double()).norm() <= 1e-4 * scale, n
+
+
+@pytest.mark.parametrize("rows,v", [(4097, 3999), (4096, 4097), (1, 4097), (2, 300007)])
+def test_rows_a_wave_each_and_rows_of_many_parts(rows, v):
+    z, y = _logits(rows, v, torch.bfloat16)
+    for top in (0, 7, 64):
+        print("token probs", rows, v, top, flush=True)
+        _check(z, y, top, F.token_log_probs(_wrap(z), _wrap(y), top))
+    up = torch.randn(rows, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    leaf = _wrap(z, True)
+    F.token_log_probs(leaf, _wrap(y)).log_probs.backward(_wrap(up))
+    want, tol = _gradient(z, y, up.double(), torch.zeros_like(up).double(), None, None)
+    # (and dz rounds once, by 2^-8 at most)
+    assert ((leaf.grad._data.double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol) + 1e-38).all()

@@ -2,7 +2,7 @@
 
 The kernels differ from the causal ones in the tiles that they visit and in the elements
 that they mask there, so the bounds are the causal tests': relative 2-norms of 1e-2 in
-f16 / bf16 (P and dS round to the type, 2^-9 and 2^-12 an element) and 2e-5 in f32, and no
+f16 / bf16 (P and dS round to the type, by 2^-11 and 2^-8 of an element at most) and 2e-5 in f32, and no
 element further off than 40 times that of the larger of itself and the root mean square.  A
 wrong tile or border is an error of the order of 1 in the rows it concerns, which is why
 rows are compared one by one as well (each row's own norm, 10 times the bound).
