@@ -538,6 +538,23 @@ def rope_tables(base: float, dim: int, dtype, dev, length: int):
         return made
 
 
+def _rotate_at(raw, positions, base: float):
+    """RoPE of [B, H, T, D] at positions [B or 1, T] as array operations (``rotary_embedding``'s, with its roundings)."""
+    import torch
+
+    d = raw.shape[-1]
+    tables = rope_tables(base, d, raw.dtype, raw.device, int(positions.max()) + 1)
+    cos, sin = (x[positions.long()][:, None].repeat_interleave(2, -1) for x in tables)
+    pairs = raw.reshape(*raw.shape[:-1], d // 2, 2)
+    turned = torch.stack((-pairs[..., 1], pairs[..., 0]), dim=-1).reshape(raw.shape)
+    return raw * cos + turned * sin
+
+
+def check_rotary(base, dim: int) -> None:
+    if base is not None and (dim % 2 or not base > 0 or not math.isfinite(base)):
+        raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
+
+
 def _rope_launch(x, out, offset: int, base: float, dim: int, inverse: bool, dev) -> None:
     b, h, t, d = x.shape
     cos, sin = rope_tables(base, dim, x.dtype, x.device, offset + t)

@@ -27,7 +27,7 @@ import ctypes
 
 from .. import _lib
 from ..device import current_stream, launch
-from .attention import _view
+from .attention import _rotate_at, _view, check_rotary, rope_tables
 from ..device import device as parse_device
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
 
@@ -99,8 +99,6 @@ class KVCache:
                 or self.head_dim % 2 or self.head_dim > 512 or self.value_dim != self.head_dim):
             return False
         stop = self._check(key, value)
-        from .attention import rope_tables
-
         cos, sin = rope_tables(base, self.head_dim, self.dtype, self._keys.device, stop)
         k, v = key._data, value._data
         k = k if k.stride(-1) == 1 else k.contiguous()
@@ -124,8 +122,6 @@ class KVCache:
         (``tsattn_draft_append``)."""
         import torch
 
-        from .drafts import _rotate_at, check_rotary
-
         stop = self._check(key, value)
         tree._check(self.batch_size, key.shape[2], self.device)
         check_rotary(rotary_base, self.head_dim)
@@ -137,8 +133,6 @@ class KVCache:
             return self._append(key, value)
         cos = sin = None
         if rotary_base is not None:
-            from .attention import rope_tables
-
             cos, sin = (x.data_ptr() for x in rope_tables(rotary_base, self.head_dim, self.dtype, self._keys.device, stop))
         k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (key._data, value._data))
         b, h, t, d = k.shape
@@ -213,8 +207,6 @@ class KVCache:
         q = torch.empty((b, num_heads, t, self.head_dim), dtype=x.dtype, device=x.device)
         cos = sin = None
         if rotary:
-            from .attention import rope_tables
-
             cos, sin = rope_tables(base, self.head_dim, self.dtype, self._keys.device, stop)
         ptr = lambda z: None if z is None else ctypes.c_void_p(z.data_ptr())
         scales = ((ctypes.byref(_view(self._key_scales)), ctypes.byref(_view(self._value_scales)))
@@ -236,13 +228,13 @@ class KVCache:
             raise ValueError("cache and key/value tensors must be on the same device")
         if is_grad_enabled() and (key.requires_grad or value.requires_grad):
             raise RuntimeError("KVCache is inference-only; use no_grad() for differentiable inputs")
-        prefix = (self.batch_size, self.num_heads)
-        if key.ndim != 4 or key.shape[:2] != prefix or key.shape[-1] != self.head_dim:
+        rows, others = key._data.shape, value._data.shape
+        if len(rows) != 4 or rows[:2] != (self.batch_size, self.num_heads) or rows[3] != self.head_dim:
             raise ValueError("key shape does not match cache configuration")
-        if value.shape != key.shape[:3] + (self.value_dim,):
+        if others != (*rows[:3], self.value_dim):
             raise ValueError("value shape does not match cache configuration")
-        stop = self.length + key.shape[2]
-        if key.shape[2] == 0 or stop > self.max_seq_len:
+        stop = self.length + rows[2]
+        if rows[2] == 0 or stop > self.max_seq_len:
             raise ValueError(f"cache capacity {self.max_seq_len} exceeded or empty append")
         return stop
 

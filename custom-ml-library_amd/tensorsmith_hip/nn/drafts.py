@@ -19,8 +19,8 @@ from .. import _lib
 from ..device import device as parse_device
 from ..device import launch, require_available
 from ..tensor import Tensor, is_grad_enabled
-from .attention import (_check_window, _dtype_code, _operand, _view, rope_tables, rotary_embedding,
-                        scaled_dot_product_attention)
+from .attention import (_check_window, _dtype_code, _operand, _rotate_at, _view, check_rotary, rope_tables,
+                        rotary_embedding, scaled_dot_product_attention)
 from .cache import KVCache
 
 __all__ = ["DraftTree", "cached_attention"]
@@ -87,23 +87,6 @@ class DraftTree:
 
     def __repr__(self):
         return f"DraftTree(tokens={self.tokens}, trees={self.trees}, device='{self.device}')"
-
-
-def _rotate_at(raw, positions, base: float):
-    """RoPE of [B, H, T, D] at positions [B or 1, T] as array operations (``rotary_embedding``'s, with its roundings)."""
-    import torch
-
-    d = raw.shape[-1]
-    tables = rope_tables(base, d, raw.dtype, raw.device, int(positions.max()) + 1)
-    cos, sin = (x[positions.long()][:, None].repeat_interleave(2, -1) for x in tables)
-    pairs = raw.reshape(*raw.shape[:-1], d // 2, 2)
-    turned = torch.stack((-pairs[..., 1], pairs[..., 0]), dim=-1).reshape(raw.shape)
-    return raw * cos + turned * sin
-
-
-def check_rotary(base, dim: int) -> None:
-    if base is not None and (dim % 2 or not base > 0 or not math.isfinite(base)):
-        raise ValueError("RoPE requires a positive even rotary dimension and valid positions/base")
 
 
 def cached_attention(query: Tensor, cache: KVCache, tree: DraftTree | None = None, *, scale: float | None = None,
