@@ -59,10 +59,10 @@ constexpr int kWaves = WR > 1 ? WR : (kPair<T, D> <= 16384 ? 4 : 2);
 // Waves a SIMD that the registers must leave room for.
 template <typename T, int D>
 constexpr int kTwo = kPair<T, D> <= 16384 ? 2 : 1;
-// Ring stages of a K and a V tile: for several waves three, for one of its own one, or
+// Ring stages of a K and a V tile: for several waves four, for one of its own one, or
 // two of codes, half as large.
 template <bool Q8, int WR>
-constexpr int kStages = WR > 1 ? 3 : Q8 ? 2 : 1;
+constexpr int kStages = WR > 1 ? 4 : Q8 ? 2 : 1;
 
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
@@ -425,18 +425,24 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (kTwo<T, D>)) void cached_
     return i < mine ? static_cast<uint32_t>(key0(i)) * stride : 0x80000000u;
   };
   // load n of tile i: K's blocks, the scales, V's blocks
-  auto load = [&](int i, int n) __attribute__((always_inline)) {
-    const uint32_t st = ring0 + (i % NS) * PAIR, sc = ring0 + NS * PAIR + (i % (NS + 1)) * 512;
-    if (Q8 && n >= BLK && n < LK) {  // (lanes 32 .. 63 fetch the same again)
-      const bool v = n > BLK;
-      const uint32_t stride = v ? vss_b : kss_b;
-      dma4(v ? vsdesc : ksdesc, sc + (v ? 256 : 0), static_cast<uint32_t>(lane & 31) * stride, first_row(i, stride));
+  struct At {
+    uint32_t st, sc, k, v, ks, vs;
+  };
+  auto place = [&](int i) __attribute__((always_inline)) {
+    At t{ring0 + (i % NS) * PAIR, 0, first_row(i, ks_b), first_row(i, vs_b), 0, 0};
+    if constexpr (Q8) t.sc = ring0 + NS * PAIR + (i % (NS + 1)) * 512, t.ks = first_row(i, kss_b), t.vs = first_row(i, vss_b);
+    return t;
+  };
+  auto load = [&](const At &t, int n) __attribute__((always_inline)) {
+    if (n < BLK) {
+      dma16(kdesc, t.st + n * 1024, Tile::dma_off(n, lane, ks_b), t.k + static_cast<uint32_t>(n * Tile::RPB) * ks_b);
+    } else if (!Q8 || n >= LK) {
+      const int at = n - LK;
+      dma16(vdesc, t.st + TILE + at * 1024, Tile::dma_off(at, lane, vs_b), t.v + static_cast<uint32_t>(at * Tile::RPB) * vs_b);
+    } else if (n == BLK) {  // (lanes 32 .. 63 fetch the same again)
+      dma4(ksdesc, t.sc, static_cast<uint32_t>(lane & 31) * kss_b, t.ks);
     } else {
-      const bool v = n >= LK;
-      const int at = v ? n - LK : n;
-      const uint32_t stride = v ? vs_b : ks_b;
-      dma16(v ? vdesc : kdesc, st + (v ? TILE : 0) + at * 1024, Tile::dma_off(at, lane, stride),
-            first_row(i, stride) + static_cast<uint32_t>(at * Tile::RPB) * stride);
+      dma4(vsdesc, t.sc + 256, static_cast<uint32_t>(lane & 31) * vss_b, t.vs);
     }
   };
   auto scales_of = [&](int i) __attribute__((always_inline)) {
@@ -445,8 +451,9 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (kTwo<T, D>)) void cached_
   if constexpr (WR == 1) {
     // a tile's places are loaded again, NS tiles on, as soon as they are read
     auto issue = [&](int i, int from, int to) __attribute__((always_inline)) {
+      const At t = place(i);
 #pragma unroll
-      for (int n = from; n < to; ++n) load(i, n);
+      for (int n = from; n < to; ++n) load(t, n);
     };
 #pragma unroll
     for (int i = 0; i < NS; ++i) issue(i, 0, LK + LV);
@@ -470,24 +477,49 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (kTwo<T, D>)) void cached_
     wait_vm_n<0>();
   } else {
     // wave w issues loads w, w + WR, .. of a pair, the last one again where they do not
-    // come out even; two tiles ahead
+    // come out even; three tiles ahead
     auto issue = [&](int i) __attribute__((always_inline)) {
+      const At t = place(i);
 #pragma unroll
       for (int u = 0; u < LPT; ++u) {
         const int n = w + WR * u;
-        load(i, n < LK + LV ? n : LK + LV - 1);
+        if (WR * u + WR <= BLK) {  // (a K block whatever the wave: no branch)
+          __builtin_assume(n < BLK);
+          load(t, n);
+        } else if (WR * u >= LK && WR * u + WR <= LK + LV) {
+          __builtin_assume(n >= LK);
+          load(t, n);
+        } else {
+          load(t, n < LK + LV ? n : LK + LV - 1);
+        }
       }
     };
+    // O^T += V^T P^T of a tile and the next one's scores are one run of matrix
+    // instructions, among which the exponentials issue; the ring's stages are unrolled,
+    // so that LDS addresses are constants beside the lane's (63 tokens of 16 sequences
+    // over 8000 keys, bf16: 170 us each tile by itself with three stages, 157 this way,
+    // 150 unrolled; fragments read 3 steps ahead by hand, or a higher priority during
+    // the matrix instructions: no change)
     issue(0);
     issue(1);
-    for (int i = 0; i < mine; ++i) {
-      const char *kt = ring + (i % NS) * PAIR;
-      wait_vm_n<LPT>();  // this wave's loads of tile i
+    issue(2);
+    wait_vm_n<2 * LPT>();
+    phase_barrier();
+    f32x16 s = scores(ring);
+    auto step = [&](int i, auto stage) __attribute__((always_inline)) {
+      softmax(s, key0(i), scales_of(i));
+      wait_vm_n<LPT>();  // this wave's loads of tile i + 1
       wait_lgkm0();
       phase_barrier();  // every wave's; and tile i - 1 is read
-      issue(i + 2);
-      softmax(scores(kt), key0(i), scales_of(i));
-      values(kt + TILE);
+      issue(i + 3);
+      s = scores(ring + (stage + 1) % NS * PAIR);
+      values(ring + stage * PAIR + TILE);
+    };
+    for (int i = 0; i < mine; i += NS) {
+      step(i, std::integral_constant<int, 0>{});
+      if (i + 1 < mine) step(i + 1, std::integral_constant<int, 1>{});
+      if (i + 2 < mine) step(i + 2, std::integral_constant<int, 2>{});
+      if (i + 3 < mine) step(i + 3, std::integral_constant<int, 3>{});
     }
     wait_vm_n<0>();
   }
