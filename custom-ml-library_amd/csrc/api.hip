@@ -968,6 +968,29 @@ int tsattn_kv_append_int8(int32_t dtype, int32_t batch, int32_t heads, int32_t l
                     "int8 append launch");
 }
 
+int tsattn_kv_read_int8(int32_t dtype, int32_t batch, int32_t heads, int64_t first, int32_t len, int32_t dim_qk,
+                        int32_t dim_v, const tsattn_view *k, const tsattn_view *v, const tsattn_view *k_scale,
+                        const tsattn_view *v_scale, void *k_out, void *v_out, void *stream) {
+  int rc;
+  if ((rc = check_view(k, "key cache")) || (rc = check_view(v, "value cache")) ||
+      (rc = check_view(k_scale, "key scales")) || (rc = check_view(v_scale, "value scales")))
+    return rc;
+  if (!k_out || !v_out) return fail(TSATTN_ERR_INVALID, "data pointer is NULL");
+  if (!is_float_dtype(dtype)) return fail(TSATTN_ERR_INVALID, "cache rows are floating point (got dtype %d)", dtype);
+  if (dtype == TSATTN_F64) return fail(TSATTN_ERR_UNSUPPORTED, "int8 rows are read as f32, f16 or bf16");
+  if (batch <= 0 || heads <= 0 || first < 0 || len <= 0 || dim_qk <= 0 || dim_v <= 0)
+    return fail(TSATTN_ERR_INVALID, "rows to read need positive sizes");
+  // (32-bit element counts of a head, workgroups in one grid dimension)
+  const int64_t head = static_cast<int64_t>(len) * (dim_qk > dim_v ? dim_qk : dim_v);
+  if (head >= (int64_t(1) << 31) || static_cast<int64_t>(batch) * heads * (head / 256 + 1) >= (int64_t(1) << 31))
+    return fail(TSATTN_ERR_UNSUPPORTED, "at most 2^31 elements of a head, and 2^39 in all, are read at once");
+  return hip_status(tsattn::launch_kv_read_int8(dtype, batch, heads, first, len, dim_qk, dim_v, tsattn::make_view(k),
+                                                tsattn::make_view(v), tsattn::make_view(k_scale),
+                                                tsattn::make_view(v_scale), k_out, v_out,
+                                                static_cast<hipStream_t>(stream)),
+                    "int8 rows launch");
+}
+
 int tsattn_rope(int32_t dtype, int32_t batch, int32_t heads, int32_t len, int32_t dim,
                 int32_t rotary_dim, const tsattn_view *x, const tsattn_view *out, const void *cos,
                 const void *sin, int64_t pos0, int32_t inverse, void *stream) {

@@ -152,6 +152,60 @@ __global__ __launch_bounds__(NT) void kv_append_int8_vec_kernel(int H, int T_, u
   }
 }
 
+// Rows read back: code times its row's scale in fp32, rounded once to T, for keys
+// (blockIdx.y 0) and values.  VE codes a lane, 8 of them where the rows allow it.  HBM bound
+// (2 and a half bytes an element in 16 bits); a few kept rows of a cache cost a launch, 3 us,
+// where array operations, one for each side, took 6 us each.
+struct ReadArgs {
+  View x[2], s[2];
+  void *out[2];
+  int dim[2];
+  int64_t first;
+  int H, n;
+  uint32_t chunks;  // workgroups a (sequence, head) and side
+};
+
+// (kept from the compiler, which would round the exact product to f16 at once)
+template <typename T>
+__device__ __forceinline__ T read_code(int8_t code, float scale) {
+  float y = static_cast<float>(code) * scale;
+  asm volatile("" : "+v"(y));
+  return static_cast<T>(y);
+}
+
+template <typename T, int VE>
+__global__ __launch_bounds__(NT) void kv_read_int8_kernel(ReadArgs a) {
+  const int side = blockIdx.y;
+  const uint32_t bh = blockIdx.x / a.chunks, b = bh / a.H, h = bh - b * a.H;
+  const uint32_t pieces = a.dim[side] / VE, i = (blockIdx.x - bh * a.chunks) * NT + threadIdx.x;
+  const uint32_t t = i / pieces, d = (i - t * pieces) * VE;
+  if (t >= static_cast<uint32_t>(a.n)) return;
+  const View &x = a.x[side], &s = a.s[side];
+  const int8_t *from = static_cast<const int8_t *>(x.data) + b * x.s0 + h * x.s1 + (a.first + t) * x.s2 + d;
+  const float scale = static_cast<const float *>(s.data)[b * s.s0 + h * s.s1 + (a.first + t) * s.s2];
+  T *to = static_cast<T *>(a.out[side]) + (static_cast<int64_t>(bh) * a.n + t) * a.dim[side] + d;
+  if constexpr (VE == 1) {
+    *to = read_code<T>(*from, scale);
+  } else {
+    const uint64_t codes = *reinterpret_cast<const uint64_t *>(from);
+    alignas(16) T y[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) y[j] = read_code<T>(static_cast<int8_t>(codes >> (8 * j)), scale);
+#pragma unroll
+    for (int j = 0; j < VE * static_cast<int>(sizeof(T)) / 16; ++j)
+      reinterpret_cast<u32x4 *>(to)[j] = reinterpret_cast<const u32x4 *>(y)[j];
+  }
+}
+
+template <typename T>
+void read_int8(ReadArgs &a, int BH, bool wide, hipStream_t st) {
+  const int most = a.dim[0] > a.dim[1] ? a.dim[0] : a.dim[1];
+  a.chunks = static_cast<uint32_t>((static_cast<int64_t>(a.n) * (wide ? most / 8 : most) + NT - 1) / NT);
+  const dim3 grid(static_cast<uint32_t>(BH) * a.chunks, 2);
+  if (wide) kv_read_int8_kernel<T, 8><<<grid, dim3(NT), 0, st>>>(a);
+  else kv_read_int8_kernel<T, 1><<<grid, dim3(NT), 0, st>>>(a);
+}
+
 }  // namespace
 
 hipError_t launch_kv_append_int8(int dtype, int B, int H, int T_, int D, View src, View dst,
@@ -191,6 +245,21 @@ hipError_t launch_kv_append_int8(int dtype, int B, int H, int T_, int D, View sr
   if (dtype == TSATTN_F32) kv_append_int8_kernel<float><<<grid, block, 0, st>>>(B, H, T_, D, src, dst, scale, pos);
   else if (dtype == TSATTN_F16) kv_append_int8_kernel<f16><<<grid, block, 0, st>>>(B, H, T_, D, src, dst, scale, pos);
   else kv_append_int8_kernel<bf16><<<grid, block, 0, st>>>(B, H, T_, D, src, dst, scale, pos);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_read_int8(int dtype, int B, int H, int64_t first, int n, int Dk, int Dv, View k, View v, View ks,
+                               View vs, void *ko, void *vo, hipStream_t st) {
+  ReadArgs a{{k, v}, {ks, vs}, {ko, vo}, {Dk, Dv}, first, H, n, 0};
+  auto eights = [](const View &x, const void *out) {
+    return reinterpret_cast<uintptr_t>(x.data) % 8 == 0 && x.s0 % 8 == 0 && x.s1 % 8 == 0 && x.s2 % 8 == 0 &&
+           reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  };
+  const bool wide = Dk % 8 == 0 && Dv % 8 == 0 && eights(k, ko) && eights(v, vo);
+  Probe pr_("kv_read_int8", st);
+  if (dtype == TSATTN_F32) read_int8<float>(a, B * H, wide, st);
+  else if (dtype == TSATTN_F16) read_int8<f16>(a, B * H, wide, st);
+  else read_int8<bf16>(a, B * H, wide, st);
   return hipGetLastError();
 }
 

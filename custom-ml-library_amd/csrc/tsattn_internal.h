@@ -274,6 +274,11 @@ hipError_t launch_decode_int8(const Problem &p, int dtype, View q, View k, View 
 hipError_t launch_kv_append_int8(int dtype, int B, int H, int T, int D, View src, View dst,
                                  View scale, int64_t pos, hipStream_t st);
 
+// Rows first .. first + n - 1 of an int8 cache's keys and values in fp32, rounded to dtype, as contiguous
+// [B, H, n, D] arrays.
+hipError_t launch_kv_read_int8(int dtype, int B, int H, int64_t first, int n, int Dk, int Dv, View k, View v, View ks,
+                               View vs, void *ko, void *vo, hipStream_t st);
+
 // Interleaved-pair RoPE of x [B, H, T, D] into out (may alias x), cos / sin
 // tables [*, R / 2] in the tensor dtype, rows pos0 .. pos0 + T - 1.
 hipError_t launch_rope(int dtype, int B, int H, int T, int D, int R, View x, View out,

@@ -230,6 +230,11 @@ SIGNATURES = {
         c_int,
         [c_int32, c_int32, c_int32, c_int32, c_int32, _PV, _PV, _PV, c_int64, c_void_p],
     ),
+    "tsattn_kv_read_int8": (
+        c_int,
+        [c_int32, c_int32, c_int32, c_int64, c_int32, c_int32, c_int32, _PV, _PV, _PV, _PV, c_void_p, c_void_p,
+         c_void_p],
+    ),
     "tsattn_rope": (
         c_int,
         [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _PV, _PV, c_void_p, c_void_p,

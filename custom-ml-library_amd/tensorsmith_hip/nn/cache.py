@@ -27,7 +27,7 @@ import ctypes
 
 from .. import _lib
 from ..device import current_stream, launch
-from .attention import _rotate_at, _view, check_rotary, rope_tables
+from .attention import _dtype_code, _rotate_at, _view, check_rotary, rope_tables
 from ..device import device as parse_device
 from ..tensor import Tensor, backend_dtype, is_grad_enabled, to_numpy
 
@@ -243,16 +243,24 @@ class KVCache:
         last = None if last is None else operator.index(last)
         if last is not None and not 0 <= last <= self.length:
             raise ValueError("last must be between zero and the current length")
-        part = slice(0 if last is None else self.length - last, self.length)
-        keys = self._keys[:, :, part]
-        values = self._values[:, :, part]
-        if self.quantized:
-            import torch
+        first = 0 if last is None else self.length - last
+        part = slice(first, self.length)
+        if not self.quantized:
+            return tuple(Tensor._leaf(x[:, :, part], self.device) for x in (self._keys, self._values))
+        import torch
 
-            # (one kernel each: the product in float32, rounded to the dtype as it is stored)
-            keys, values = (torch.mul(x, s[:, :, part], out=torch.empty(x.shape, dtype=self.dtype, device=x.device))
-                            for x, s in ((keys, self._key_scales), (values, self._value_scales)))
-        return Tensor._leaf(keys, self.device), Tensor._leaf(values, self.device)
+        b, h, _, d = self._keys.shape
+        made = tuple(torch.empty((b, h, self.length - first, dim), dtype=self.dtype, device=self._keys.device)
+                     for dim in (d, self.value_dim))
+        try:
+            if self.length > first:
+                _lib.check(launch(self.device, _lib.load().tsattn_kv_read_int8, _dtype_code(self.dtype), b, h, first,
+                                  self.length - first, d, self.value_dim, *self._views(), *(x.data_ptr() for x in made)),
+                           "cached values")
+        except NotImplementedError:  # (float64, or more rows than the kernel counts)
+            for x, scale, out in zip(self.storage[:2], self.storage[2:], made):
+                torch.mul(x[:, :, part], scale[:, :, part], out=out)
+        return tuple(Tensor._leaf(x, self.device) for x in made)
 
     def reset(self) -> None:
         """Reuse the allocation; future appends overwrite old entries."""

@@ -366,6 +366,16 @@ int tsattn_kv_append_int8(int32_t dtype, int32_t batch, int32_t heads, int32_t l
                           int64_t pos, void *stream);
 
 /*
+ * The other way (KVCache.get): rows first .. first + len - 1 of an int8 cache's keys (of
+ * dim_qk) and values (dim_v) [batch, heads, *] times their fp32 scales, rounded once to dtype (f32, f16,
+ * bf16; others and 2^31 elements of a head or more: TSATTN_ERR_UNSUPPORTED), into contiguous
+ * [batch, heads, len, dim] arrays.
+ */
+int tsattn_kv_read_int8(int32_t dtype, int32_t batch, int32_t heads, int64_t first, int32_t len, int32_t dim_qk,
+                        int32_t dim_v, const tsattn_view *k, const tsattn_view *v, const tsattn_view *k_scale,
+                        const tsattn_view *v_scale, void *k_out, void *v_out, void *stream);
+
+/*
  * Interleaved-pair rotary position embedding (rotary_embedding, src/
  * tensorsmith/nn/attention.py:255-296) of x [batch, heads, len, dim] into out
  * (which may be x): channel pair (2i, 2i+1) of row t, i < rotary_dim / 2,

@@ -426,3 +426,21 @@ def test_windows_over_a_paged_cache():
         want = torch.matmul(torch.softmax(s, -1), v).permute(0, 2, 1, 3).reshape(2, 5, 128)
         want = torch.matmul(want, layers[2].out_proj.weight._data.double().t().contiguous())
     assert (got[2][1].double() - want).norm() <= 1e-2 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("d,dv,n", [(128, 128, 300), (64, 32, 7), (8, 24, 1), (5, 3, 40), (16, 12, 33), (256, 256, 1000)])
+def test_codes_are_read_as_products_rounded_once(d, dv, n, dtype):
+    """The same bits as array operations: the product in float32, then the type."""
+    b, h, room = 2, 3, n + 5
+    cache = nn.KVCache(b, h, d, room, device="hip", dtype=dtype, quantized=True, value_dim=dv)
+    for x in cache.storage[:2]:
+        x.copy_(torch.randint(-127, 128, x.shape, device="cuda", generator=_gen(n)))
+    for x in cache.storage[2:]:
+        x.copy_(2.0 ** (20 * torch.rand(x.shape, device="cuda", generator=_gen(d)) - 14))
+    cache.length = n
+    for last in (None, 1, n // 2, 0):
+        first = 0 if last is None else n - last
+        for got, x, s in zip(cache.get(last), cache.storage[:2], cache.storage[2:]):
+            want = (x[:, :, first:n].float() * s[:, :, first:n]).to(dtype)
+            assert got.shape == want.shape and torch.equal(got._data, want)

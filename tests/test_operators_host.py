@@ -229,24 +229,36 @@ def test_kept_rows_are_checked(lib):
     assert cache.length == 4 and args[:5] == (2, 2, 2, 2, 5) and args[6:10] == (4, 2, 64, 64)
 
 
-@pytest.mark.parametrize("quantized", [False, True])
-def test_the_last_rows_of_a_cache(lib, quantized):
-    cache = nn.KVCache(2, 2, 8, 12, device="hip:0", dtype="float32", quantized=quantized)
-    keys, values = torch.randn(2, 2, 9, 8), torch.randn(2, 2, 9, 8)
-    if quantized:
-        cache.storage[0][:, :, :9] = torch.randint(-127, 128, keys.shape).to(torch.int8)
-        cache.storage[1][:, :, :9] = torch.randint(-127, 128, keys.shape).to(torch.int8)
-        cache.storage[2][:, :, :9], cache.storage[3][:, :, :9] = torch.rand(2, 2, 9, 1), torch.rand(2, 2, 9, 1)
-    else:
-        cache.storage[0][:, :, :9], cache.storage[1][:, :, :9] = keys, values
+def test_the_last_rows_of_a_cache(lib):
+    cache = nn.KVCache(2, 2, 8, 12, device="hip:0", dtype="float32")
+    cache.storage[0][:, :, :9], cache.storage[1][:, :, :9] = torch.randn(2, 2, 9, 8), torch.randn(2, 2, 9, 8)
     cache.length = 9
     whole = cache.get()
-    for last in (0, 1, 4, 9):
+    for last in (0, 1, 4, 9, np.int32(3)):
         for part, all_ in zip(cache.get(last), whole):
             assert torch.equal(part._data, all_._data[:, :, 9 - last:])
     for bad in (-1, 10):
         with pytest.raises(ValueError):
             cache.get(bad)
+
+
+def test_codes_are_read_on_the_caches_device(lib):
+    cache = nn.KVCache(2, 3, 8, 12, device="hip:1", dtype="float16", quantized=True, value_dim=5)
+    assert [x.shape for x in cache.get()] == [(2, 3, 0, 8), (2, 3, 0, 5)] and not lib.calls
+    cache.length = 9
+    assert [x.shape for x in cache.get(4)] == [(2, 3, 4, 8), (2, 3, 4, 5)]
+    name, current, stream = lib.calls[-1]
+    assert (name, current, getattr(stream, "value", stream)) == ("tsattn_kv_read_int8", 1, 0x101)
+    args = lib.args[name]
+    assert args[:7] == (_lib.F16, 2, 3, 5, 4, 8, 5)
+    assert [x.data for x in args[7:11]] == [x.data_ptr() for x in cache.storage]
+    lib.__dict__.update(tsattn_kv_read_int8=lambda *a: UNSUPPORTED, tsattn_last_error=lambda: b"unsupported")
+    for x in cache.storage[:2]:
+        x[:] = torch.randint(-127, 128, x.shape).to(torch.int8)
+    for x in cache.storage[2:]:
+        x[:] = torch.rand(x.shape)
+    for got, codes, scales in zip(cache.get(4), cache.storage[:2], cache.storage[2:]):
+        assert torch.equal(got._data, (codes[:, :, 5:9].float() * scales[:, :, 5:9]).half())
 
 
 # -- the library itself ------------------------------------------------------------------
@@ -359,3 +371,14 @@ def test_the_library_refuses_token_probabilities():
                                          ge, gt, out, None))
     assert [backward(stats=None), backward(out=None), backward(ge=0x1000), backward(gt=0x1000),
             backward(out=0x1001)] == [INVALID] * 5
+
+
+def test_the_library_refuses_rows_to_read():
+    real, v = _lib.load(), _view()
+
+    def read(dtype=_lib.F16, b=2, h=2, first=3, n=5, dk=8, dv=8, k=v, ks=v, out=0x1000):
+        return _code(real.tsattn_kv_read_int8(dtype, b, h, first, n, dk, dv, k, v, ks, v, out, 0x1000, None))
+
+    assert [read(dtype=_lib.BOOL), read(b=0), read(h=0), read(n=0), read(dk=0), read(dv=0), read(k=None), read(ks=None),
+            read(out=None), read(first=-1)] == [INVALID] * 10
+    assert [read(dtype=_lib.F64), read(n=1 << 28), read(b=1 << 20, h=1 << 12)] == [UNSUPPORTED] * 3
