@@ -10,9 +10,10 @@
 //
 // The rows of a KV head (its query heads times the tokens) are the columns of S^T = K Q^T,
 // 32 to a wave, so that the statistics of a row are a lane's own and P^T is the operand of
-// O^T += V^T P^T as it comes.  Cached keys and values are read once for up to 128 rows.
-// Up to 32 rows: every wave works alone on tiles of its own through its own LDS ring and
-// the waves' results are joined at the end; more: 2 or 4 waves of 32 rows share each tile.
+// O^T += V^T P^T as it comes.
+// Every wave works alone on tiles of its own through its own LDS ring and the waves'
+// results are joined at the end, or, for many rows of many heads, 4 waves of 32 rows share
+// each tile (plan_cached).
 // The tiles that a window leaves lie in one run, which splits cut into equal parts, as
 // many as fill the chip; a second kernel joins those.
 //
@@ -59,8 +60,8 @@ constexpr int kWaves = WR > 1 ? WR : (kPair<T, D> <= 16384 ? 4 : 2);
 // Waves a SIMD that the registers must leave room for.
 template <typename T, int D>
 constexpr int kTwo = kPair<T, D> <= 16384 ? 2 : 1;
-// Ring stages of a K and a V tile: for several waves four, for one of its own one, or
-// two of codes, half as large.
+// Ring stages of a K and a V tile: of 4 waves four, of one wave one, or two of codes, half
+// as large.
 template <bool Q8, int WR>
 constexpr int kStages = WR > 1 ? 4 : Q8 ? 2 : 1;
 
@@ -174,24 +175,25 @@ __device__ __forceinline__ void dma4(u32x4 desc, uint32_t lds, uint32_t voff, ui
                : "memory", "m0");
 }
 
-template <typename T, int D, bool Q8, int WR>
+template <typename T, int D, bool Q8, int WR, bool NT>
 __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (kTwo<T, D>)) void cached_kernel(CachedArgs a) {
   constexpr bool F32 = std::is_same_v<T, float>;
   static_assert(!F32 || (!Q8 && D <= 128), "fp32 caches are not quantised, of up to 128 channels");
+  static_assert(WR == 1 || (!F32 && !Q8), "waves share tiles of 16 bits");
   using PT = std::conditional_t<Q8, bf16, T>;  // the value tiles
   constexpr int NP = Q8 && std::is_same_v<T, f16> ? 2 : 1;  // parts of P
   constexpr int NWV = kWaves<T, D, WR>, WK = NWV / WR, NS = kStages<Q8, WR>;
   constexpr int PAIR = Q8 ? kPair<T, D> / 2 : kPair<T, D>, TILE = PAIR / 2;
   constexpr int BLK = TILE / 1024;        // 1 KiB DMA blocks a tile
   constexpr int LK = BLK + (Q8 ? 2 : 0), LV = BLK;  // loads of a K tile (and both tiles' scales), a V tile
-  constexpr int LPT = (LK + LV + WR - 1) / WR;      // loads a wave issues for a pair (WR > 1)
+  constexpr int LPT = (LK + LV) / WR;               // loads a wave issues for a pair (WR > 1)
   constexpr int PDT = D / 32;
   // the stages, then (codes) one place more for 64 floats of K's and 64 of V's scales, half
   // of each in use: a tile's are read after its K's place is loaded again
   constexpr int RING = NS * PAIR + (Q8 ? (NS + 1) * 512 : 0);
   constexpr int MERGE = WK > 1 ? NWV * 32 * (D + 2) * 4 : 0;
   constexpr int LDS_B = WK * RING > MERGE ? WK * RING : MERGE;
-  static_assert((WR > 1 ? LPT : NS * (LK + LV)) < 64, "loads in flight that a wait can count");
+  static_assert((LK + LV) % WR == 0 && (WR > 1 ? LPT : NS * (LK + LV)) < 64, "loads in flight that a wait can count");
   __shared__ __attribute__((aligned(1024))) char lds[LDS_B];
 
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
@@ -433,12 +435,16 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (kTwo<T, D>)) void cached_
     if constexpr (Q8) t.sc = ring0 + NS * PAIR + (i % (NS + 1)) * 512, t.ks = first_row(i, kss_b), t.vs = first_row(i, vss_b);
     return t;
   };
+  auto fetch = [&](u32x4 desc, uint32_t to, uint32_t off, uint32_t base) __attribute__((always_inline)) {
+    if constexpr (NT) dma16_nt(desc, to, off, base);
+    else dma16(desc, to, off, base);
+  };
   auto load = [&](const At &t, int n) __attribute__((always_inline)) {
     if (n < BLK) {
-      dma16(kdesc, t.st + n * 1024, Tile::dma_off(n, lane, ks_b), t.k + static_cast<uint32_t>(n * Tile::RPB) * ks_b);
+      fetch(kdesc, t.st + n * 1024, Tile::dma_off(n, lane, ks_b), t.k + static_cast<uint32_t>(n * Tile::RPB) * ks_b);
     } else if (!Q8 || n >= LK) {
       const int at = n - LK;
-      dma16(vdesc, t.st + TILE + at * 1024, Tile::dma_off(at, lane, vs_b), t.v + static_cast<uint32_t>(at * Tile::RPB) * vs_b);
+      fetch(vdesc, t.st + TILE + at * 1024, Tile::dma_off(at, lane, vs_b), t.v + static_cast<uint32_t>(at * Tile::RPB) * vs_b);
     } else if (n == BLK) {  // (lanes 32 .. 63 fetch the same again)
       dma4(ksdesc, t.sc, static_cast<uint32_t>(lane & 31) * kss_b, t.ks);
     } else {
@@ -476,22 +482,15 @@ __global__ __launch_bounds__((64 * kWaves<T, D, WR>), (kTwo<T, D>)) void cached_
     }
     wait_vm_n<0>();
   } else {
-    // wave w issues loads w, w + WR, .. of a pair, the last one again where they do not
-    // come out even; three tiles ahead
+    // wave w issues loads w, w + WR, .. of a pair, three tiles ahead
     auto issue = [&](int i) __attribute__((always_inline)) {
       const At t = place(i);
 #pragma unroll
       for (int u = 0; u < LPT; ++u) {
         const int n = w + WR * u;
-        if (WR * u + WR <= BLK) {  // (a K block whatever the wave: no branch)
-          __builtin_assume(n < BLK);
-          load(t, n);
-        } else if (WR * u >= LK && WR * u + WR <= LK + LV) {
-          __builtin_assume(n >= LK);
-          load(t, n);
-        } else {
-          load(t, n < LK + LV ? n : LK + LV - 1);
-        }
+        if (WR * u + WR <= BLK) __builtin_assume(n < BLK);  // (a K block whatever the wave: no branch)
+        else if (WR * u >= LK) __builtin_assume(n >= LK);
+        load(t, n);
       }
     };
     // O^T += V^T P^T of a tile and the next one's scores are one run of matrix
@@ -699,12 +698,21 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a, int slices) {
 
 struct CachedPlan {
   int wr, groups, ns, gap, run, splits;
+  bool nt;
 };
 
 CachedPlan plan_cached(const CachedProblem &p) {
   CachedPlan s;
   const int R = p.Hq / p.Hkv * p.T;
-  s.wr = R <= 32 ? 1 : R <= 64 ? 2 : 4;
+  // Waves alone read a tile once for each 32 rows, from L2 after the first, and meet no
+  // barrier; waves that share read it once and pay where the matrix instructions fill the
+  // chip: 24 tokens of 4 query heads over 8192 keys, 256 heads of 128 265 us alone and 193
+  // shared, 63 tokens, 128 heads 257 and 182; 32 heads of 2048 keys, 16 tokens 18 and 25,
+  // 63 tokens 28 and 30.  Codes and fp32 gain nothing from sharing (64 heads, 12 tokens
+  // over 8192 codes 50 and 97 us; fp32, 16 over 4096 keys 103 and 182).
+  const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv;
+  const bool share = R > 32 && !p.q8 && p.dtype != TSATTN_F32 && heads * ((R + 127) / 128) >= 128;
+  s.wr = share ? 4 : 1;
   s.groups = (R + 32 * s.wr - 1) / (32 * s.wr);
   const int tiles = (p.n + BN - 1) / BN;
   // the first key that some row's window holds (depth 0's)
@@ -715,13 +723,13 @@ CachedPlan plan_cached(const CachedProblem &p) {
   s.gap = first - s.ns;
   s.run = tiles - s.gap;
   // A wave for each SIMD: a second one costs a few tokens over 16 or 32 bits more in partial
-  // results (step of 32 sequences, window 4096 of 8 heads of 128: 96 us, with two 102).
+  // results (step of 32 sequences, window 4096 of 8 heads of 128: 83 us, with two 90).
   // Codes, and rows enough for several waves, keep a SIMD busy beside the loads, and take
   // two where the parts stay few (63 tokens of 16 sequences over 8000 keys, 8 heads of 128:
   // 241 us in one part, 204 in two; 16 heads, 24 tokens of 7 sequences, codes: 38 us in 9
   // parts, 40 in 18).  A wave has 4 tiles or more to itself, of slower f32 ones 2 (17
   // tokens over 900 keys, 4 heads of 32: 18 us with 4, 14 with 2).
-  const int64_t base = static_cast<int64_t>(p.B) * p.Hkv * s.groups;
+  const int64_t base = heads * s.groups;
   const int waves = s.wr > 1 ? s.wr : 64 * p.D * (p.dtype == TSATTN_F32 ? 4 : 2) <= 16384 ? 4 : 2;
   int64_t n = 1024 / waves / base;
   if (n < 1) n = 1;
@@ -729,15 +737,26 @@ CachedPlan plan_cached(const CachedProblem &p) {
   const int least = (p.dtype == TSATTN_F32 ? 2 : 4) * (s.wr > 1 ? 1 : waves);
   if (n > s.run / least) n = s.run / least;
   s.splits = n < 1 ? 1 : static_cast<int>(n);
+  // What is read once and is more than the memory-side cache's 256 MB passes it by: that
+  // step, 537 MB, 96 -> 83 us; 268 MB 52 -> 51; of less, a cache that the step before has
+  // left there is found again (34 MB: 15 us, read past it 17).
+  const int64_t row = static_cast<int64_t>(p.D) * (p.q8 ? 1 : p.dtype == TSATTN_F32 ? 4 : 2);
+  s.nt = s.groups == 1 && heads * s.run * BN * row * 2 > (int64_t(256) << 20);
   return s;
 }
 
+template <typename T, int D, bool Q8, bool NT>
+void launch_kernel(const CachedArgs &a, int wr, dim3 grid, hipStream_t st) {
+  if constexpr (!Q8 && !std::is_same_v<T, float>)
+    if (wr == 4) return cached_kernel<T, D, Q8, 4, NT><<<grid, dim3(256), 0, st>>>(a);
+  cached_kernel<T, D, Q8, 1, NT><<<grid, dim3(64 * kWaves<T, D, 1>), 0, st>>>(a);
+}
+
 template <typename T, int D, bool Q8>
-void launch_wr(const CachedArgs &a, int wr, hipStream_t st) {
+void launch_wr(const CachedArgs &a, const CachedPlan &s, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.Hkv * a.splits * a.groups));
-  if (wr == 1) cached_kernel<T, D, Q8, 1><<<grid, dim3(64 * kWaves<T, D, 1>), 0, st>>>(a);
-  else if (wr == 2) cached_kernel<T, D, Q8, 2><<<grid, dim3(128), 0, st>>>(a);
-  else cached_kernel<T, D, Q8, 4><<<grid, dim3(256), 0, st>>>(a);
+  if (s.nt) launch_kernel<T, D, Q8, true>(a, s.wr, grid, st);
+  else launch_kernel<T, D, Q8, false>(a, s.wr, grid, st);
   if (a.splits > 1) {
     const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.R;
     constexpr int RPB = 256 / (D / 4);
@@ -746,11 +765,11 @@ void launch_wr(const CachedArgs &a, int wr, hipStream_t st) {
 }
 
 template <typename T, bool Q8>
-void launch_dim(const CachedArgs &a, int D, int wr, hipStream_t st) {
-  if (D == 32) launch_wr<T, 32, Q8>(a, wr, st);
-  else if (D == 64) launch_wr<T, 64, Q8>(a, wr, st);
-  else if (D == 128) launch_wr<T, 128, Q8>(a, wr, st);
-  else if constexpr (!std::is_same_v<T, float>) launch_wr<T, 256, Q8>(a, wr, st);
+void launch_dim(const CachedArgs &a, int D, const CachedPlan &s, hipStream_t st) {
+  if (D == 32) launch_wr<T, 32, Q8>(a, s, st);
+  else if (D == 64) launch_wr<T, 64, Q8>(a, s, st);
+  else if (D == 128) launch_wr<T, 128, Q8>(a, s, st);
+  else if constexpr (!std::is_same_v<T, float>) launch_wr<T, 256, Q8>(a, s, st);
 }
 
 }  // namespace
@@ -778,9 +797,9 @@ hipError_t launch_cached(const CachedProblem &p, View q, View k, View v, View ks
   a.rope = p.rope;
   a.ws = ws;
   Probe pr_(p.words ? "cached_tree" : "cached_window", st);
-  if (p.dtype == TSATTN_F32) launch_dim<float, false>(a, p.D, s.wr, st);
-  else if (p.dtype == TSATTN_F16) p.q8 ? launch_dim<f16, true>(a, p.D, s.wr, st) : launch_dim<f16, false>(a, p.D, s.wr, st);
-  else p.q8 ? launch_dim<bf16, true>(a, p.D, s.wr, st) : launch_dim<bf16, false>(a, p.D, s.wr, st);
+  if (p.dtype == TSATTN_F32) launch_dim<float, false>(a, p.D, s, st);
+  else if (p.dtype == TSATTN_F16) p.q8 ? launch_dim<f16, true>(a, p.D, s, st) : launch_dim<f16, false>(a, p.D, s, st);
+  else p.q8 ? launch_dim<bf16, true>(a, p.D, s, st) : launch_dim<bf16, false>(a, p.D, s, st);
   return hipGetLastError();
 }
 

@@ -444,3 +444,42 @@ def test_codes_are_read_as_products_rounded_once(d, dv, n, dtype):
         for got, x, s in zip(cache.get(last), cache.storage[:2], cache.storage[2:]):
             want = (x[:, :, first:n].float() * s[:, :, first:n]).to(dtype)
             assert got.shape == want.shape and torch.equal(got._data, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("tokens,rep,n", [(33, 1, 33), (17, 4, 300), (128, 1, 517), (70, 3, 1000)])
+def test_many_heads_share_their_tiles(tokens, rep, n, d, dtype):
+    """128 heads or more: four waves of 32 rows to a tile, whole and cut rows, from one tile to several parts."""
+    b, hkv = 16, 8
+    cache = _cache(b, hkv, n, d, dtype)
+    q = _rows(b, hkv * rep, tokens, d, dtype, 7)
+    parents = _parents(np.random.default_rng(tokens), b, tokens)
+    seen = torch.ones(b, 1, tokens, n, dtype=torch.bool, device="cuda")
+    seen[:, 0, :, n - tokens:] = torch.from_numpy(_ancestors(parents)).cuda()
+    print("shared tiles", tokens, rep, n, d, dtype, flush=True)
+    _close(_attend(q, cache, nn.DraftTree(parents)), _reference(q, cache, seen), dtype)
+    for window, sinks in ((1, 0), (31, 33), (n // 2, 3)):
+        _close(_attend(q, cache, window=max(1, window), sinks=sinks),
+               _reference(q, cache, _band(tokens, n, max(1, window), sinks)), dtype)
+
+
+@pytest.mark.parametrize("tokens,rep,n,d,dtype,int8", [(1, 4, 8300, 128, torch.float16, False),
+                                                       (12, 4, 8299, 128, torch.bfloat16, False),
+                                                       (1, 8, 16501, 128, torch.bfloat16, True),
+                                                       (3, 1, 8301, 64, torch.float32, False)])
+def test_caches_larger_than_the_memory_side_cache(tokens, rep, n, d, dtype, int8):
+    """Keys and values of more than 256 MB, which are read past it; three of the sequences are compared."""
+    b, hkv = 16, 8
+    cache = _cache(b, hkv, n, d, dtype, int8)
+    q = _rows(b, hkv * rep, tokens, d, dtype, 7)
+    for window, sinks in ((n - 77, 5), (n + 1, 0)):
+        print("large caches", tokens, rep, n, d, dtype, int8, window, flush=True)
+        got = _attend(q, cache, window=window, sinks=sinks)
+        for i in (0, 7, 15):
+            one = nn.KVCache(1, hkv, d, n, device="hip", dtype=dtype, quantized=int8)
+            for x, y in zip(one.storage, cache.storage):
+                if x is not None:
+                    x.copy_(y[i:i + 1])
+            one.length = n
+            _close(got[i:i + 1], _reference(q[i:i + 1], one, _band(tokens, n, window, sinks)), dtype)
