@@ -151,7 +151,7 @@ int check_rope(const tsattn_rope_desc *r, const tsattn::Problem &pr, tsattn::Rop
 }
 
 // A problem with a sliding window, which only the MFMA kernels take.
-int check_window(const tsattn_problem *p, int64_t window, int32_t sinks, tsattn::Problem *pr) {
+int check_window(const tsattn_problem *p, int64_t window, int32_t sinks, const void *out_low, tsattn::Problem *pr) {
   int rc = check_problem(p, pr);
   if (rc) return rc;
   if (window < 1 || sinks < 0)
@@ -161,6 +161,12 @@ int check_window(const tsattn_problem *p, int64_t window, int32_t sinks, tsattn:
     return fail(TSATTN_ERR_UNSUPPORTED, "windows take no dropout and no mask but key padding");
   pr->window = static_cast<int>(window < (1 << 30) ? window : 1 << 30);
   pr->sinks = sinks < pr->Sk ? sinks : pr->Sk;
+  if (out_low) {
+    if (p->dtype != TSATTN_F16 && p->dtype != TSATTN_BF16)
+      return fail(TSATTN_ERR_INVALID, "only 16-bit outputs have a low part");
+    if (reinterpret_cast<uintptr_t>(out_low) % 16) return fail(TSATTN_ERR_INVALID, "the low part must be 16-byte aligned");
+    pr->o_low = const_cast<void *>(out_low);
+  }
   return TSATTN_OK;
 }
 
@@ -180,13 +186,14 @@ struct Window {
   int64_t keys;  // 0: none
   int32_t sinks;
   bool given;
+  const void *out_low;
 };
 
 int sdpa_forward(const tsattn_problem *p, const tsattn_rope_desc *rope, const tsattn_view *q,
                  const tsattn_view *k, const tsattn_view *v, const tsattn_view *out, void *lse,
                  void *workspace, size_t workspace_bytes, void *stream, Window win = Window{}) {
   tsattn::Problem pr;
-  int rc = win.given ? check_window(p, win.keys, win.sinks, &pr) : check_problem(p, &pr);
+  int rc = win.given ? check_window(p, win.keys, win.sinks, win.out_low, &pr) : check_problem(p, &pr);
   if (rc) return rc;
   if ((rc = check_view(q, "query")) || (rc = check_view(k, "key")) ||
       (rc = check_view(v, "value")) || (rc = check_view(out, "output")))
@@ -269,7 +276,7 @@ int sdpa_backward(const tsattn_problem *p, const tsattn_rope_desc *rope, const t
                   const tsattn_view *dk, const tsattn_view *dv, void *workspace,
                   size_t workspace_bytes, void *stream, Window win = Window{}) {
   tsattn::Problem pr;
-  int rc = win.given ? check_window(p, win.keys, win.sinks, &pr) : check_problem(p, &pr);
+  int rc = win.given ? check_window(p, win.keys, win.sinks, win.out_low, &pr) : check_problem(p, &pr);
   if (rc) return rc;
   if ((rc = check_view(q, "query")) || (rc = check_view(k, "key")) ||
       (rc = check_view(v, "value")) || (rc = check_view(out, "output")) ||
@@ -834,13 +841,13 @@ size_t tsattn_sdpa_backward_workspace(const tsattn_problem *p) { return backward
 
 int tsattn_window_forward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
                           const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
-                          void *lse, void *stream) {
-  return sdpa_forward(p, rope, q, k, v, out, lse, nullptr, 0, stream, Window{window, sinks, true});
+                          void *lse, void *out_low, void *stream) {
+  return sdpa_forward(p, rope, q, k, v, out, lse, nullptr, 0, stream, Window{window, sinks, true, out_low});
 }
 
 size_t tsattn_window_backward_workspace(const tsattn_problem *p, int64_t window, int32_t sinks, int32_t rope) {
   tsattn::Problem pr;
-  if (check_window(p, window, sinks, &pr)) return 0;
+  if (check_window(p, window, sinks, nullptr, &pr)) return 0;
   const size_t base = rope ? rope_rows_workspace(pr) : rows_workspace(p);
   const size_t parts = tsattn::mfma_supported(pr, p->dtype)       ? tsattn::mfma_window_bytes(pr)
                        : tsattn::mfma_f32_supported(pr, p->dtype) ? tsattn::mfma_f32_window_bytes(pr)
@@ -850,10 +857,10 @@ size_t tsattn_window_backward_workspace(const tsattn_problem *p, int64_t window,
 
 int tsattn_window_backward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
                            const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
-                           const tsattn_view *dout, const void *lse, const tsattn_view *dq, const tsattn_view *dk,
-                           const tsattn_view *dv, void *workspace, size_t workspace_bytes, void *stream) {
+                           const tsattn_view *dout, const void *lse, const void *out_low, const tsattn_view *dq,
+                           const tsattn_view *dk, const tsattn_view *dv, void *workspace, size_t workspace_bytes, void *stream) {
   return sdpa_backward(p, rope, q, k, v, out, dout, lse, dq, dk, dv, workspace, workspace_bytes, stream,
-                       Window{window, sinks, true});
+                       Window{window, sinks, true, out_low});
 }
 
 size_t tsattn_sdpa_backward_rope_workspace(const tsattn_problem *p) {

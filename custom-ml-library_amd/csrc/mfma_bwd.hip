@@ -1049,7 +1049,7 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
   // The rows' Q, dO and O fragments (lane holds row qrow, channels 16 ks +
   // 8 h .. +7) and LSE, issued here; consumed after the first tiles' DMA
   // issue below, so the two latencies overlap.
-  u32x4 qf[SKQ], gf[SKV], of[SKV];
+  u32x4 qf[SKQ], gf[SKV], of[SKV], ol[WIN ? SKV : 1];
   float lse2, delta;  // -safe(lse) in exp2 units, -delta
   const int64_t row = (static_cast<int64_t>(b) * p.Hq + hq) * p.Sq + qrow;
   const float lrow_lse = qrow < p.Sq ? a.lse[row] : 0.f;
@@ -1059,12 +1059,16 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
     const rsrc_t qrs = make_rsrc(head_ptr<T>(a.q, b, hq), static_cast<uint32_t>(p.Sq) * qs_b);
     const rsrc_t grs = make_rsrc(head_ptr<T>(a.dout, b, hq), static_cast<uint32_t>(p.Sq) * gs_b);
     const rsrc_t ors = make_rsrc(head_ptr<T>(a.o, b, hq), static_cast<uint32_t>(p.Sq) * os_b);
+    // (O's low part: none reads as zeros)
+    const rsrc_t lrs = make_rsrc(static_cast<const T *>(p.o_low) + (static_cast<int64_t>(b) * p.Hq + hq) * p.Sq * DV,
+                                 WIN && p.o_low ? static_cast<uint32_t>(p.Sq) * DV * 2 : 0u);
 #pragma unroll
     for (int ks = 0; ks < STEPS; ++ks) {
       if (ks < SKQ) qf[ks] = buf_load16(qrs, static_cast<uint32_t>(qrow) * qs_b + (ks * 16 + h * 8) * 2);
       if (ks < SKV) {
         gf[ks] = buf_load16(grs, static_cast<uint32_t>(qrow) * gs_b + (ks * 16 + h * 8) * 2);
         of[ks] = buf_load16(ors, static_cast<uint32_t>(qrow) * os_b + (ks * 16 + h * 8) * 2);
+        if constexpr (WIN) ol[ks] = buf_load16(lrs, static_cast<uint32_t>(qrow) * DV * 2 + (ks * 16 + h * 8) * 2);
       }
     }
   }
@@ -1211,8 +1215,54 @@ __global__ __launch_bounds__(NT, 2) void dq_kernel(BwdArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) dsum += static_cast<float>(ge[e]) * static_cast<float>(oe[e]);
     }
+    if constexpr (WIN) {
+      // and what rounding took from O: dP - delta of a row that sees few keys is small beside
+      // delta, whose error would show (5 keys, f16: dq off by 3.6e-4 of its norm, so 3.0e-4)
+#pragma unroll
+      for (int ks = 0; ks < SKV; ++ks) {
+        const T *ge = reinterpret_cast<const T *>(&gf[ks]);
+        const T *oe = reinterpret_cast<const T *>(&ol[ks]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dsum += static_cast<float>(ge[e]) * static_cast<float>(oe[e]);
+      }
+    }
     delta = -xor32_sum(dsum);
     lse2 = isfinite(l) ? -l * kLog2e : 0.f;
+    if constexpr (WIN) {
+      // Rows of up to 8 keys: delta = sum_j P_ij dP_ij itself, as O also holds P's rounding.
+      // (2 keys: 4.7e-4 from O, 3.2e-4 with its low part, 2.9e-4 this way.  A window of 6
+      // over 2 x 16 heads x 8192 rows of 128 takes 200 us so and 106 without; up to 32 keys
+      // 554, for 3.1e-4 -> 3.0e-4 at 20, and the first rows of any window as much longer.)
+      const int sunk = min(min(p.sinks, klow), klim), seen = sunk + max(0, klim - klow);
+      const bool few = qrow < p.Sq && seen <= 8;
+      if (__ballot(few && seen > 0) != 0ull) {
+        const T *kb = head_ptr<T>(a.k, b, hk) + 8 * h, *vb = head_ptr<T>(a.v, b, hk) + 8 * h;
+        float sum = 0.f;
+        for (int t = 0; t < 8; ++t) {
+          if (__ballot(few && t < seen) == 0ull) break;
+          const int key = few && t < seen ? (t < sunk ? t : klow + t - sunk) : 0;
+          float x = 0.f, y = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < SKQ; ++ks) {
+            const u32x4 z = ld16(kb + static_cast<int64_t>(key) * a.k.s2 + 16 * ks);
+            const T *ze = reinterpret_cast<const T *>(&z), *qe = reinterpret_cast<const T *>(&qf[ks]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x += static_cast<float>(ze[e]) * static_cast<float>(qe[e]);
+          }
+#pragma unroll
+          for (int ks = 0; ks < SKV; ++ks) {
+            const u32x4 z = ld16(vb + static_cast<int64_t>(key) * a.v.s2 + 16 * ks);
+            const T *ze = reinterpret_cast<const T *>(&z), *ge = reinterpret_cast<const T *>(&gf[ks]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y += static_cast<float>(ze[e]) * static_cast<float>(ge[e]);
+          }
+          x = xor32_sum(x), y = xor32_sum(y);
+          const bool seen_key = few && t < seen && (!keymask || kmask_b[static_cast<int64_t>(key) * p.mask.s3]);
+          if (seen_key) sum += fast_exp2(fmaf(x, sl, lse2)) * y;
+        }
+        if (few) delta = -sum;
+      }
+    }
     if (h == 0 && qrow < p.Sq) store_row_values(a, static_cast<int64_t>(p.B) * p.Hq * p.Sq, row, delta, l);
   }
   // (the compiler's wait for these loads -- it does not count the DMA

@@ -625,6 +625,36 @@ __global__ __launch_bounds__(NT, 2) void fwd_kernel(FwdArgs a) {
     const int idx = u * 64 + lane, r = idx / CPR, q = idx % CPR;
     if (qw + r < p.Sq) *reinterpret_cast<u32x4 *>(ob + static_cast<int64_t>(qw + r) * a.o.s2 + q * 8) = vr[u];
   }
+  if constexpr (WIN) {
+    if (p.o_low) {  // what the rounding above took, the same way
+#pragma unroll
+      for (int dt = 0; dt < PDT; ++dt) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          u32x2 low;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x0 = oacc[dt][g * 4 + 2 * e] * inv, x1 = oacc[dt][g * 4 + 2 * e + 1] * inv;
+            const unsigned kept = pack2<T>(x0, x1);
+            const T *k2 = reinterpret_cast<const T *>(&kept);
+            low[e] = pack2<T>(x0 - static_cast<float>(k2[0]), x1 - static_cast<float>(k2[1]));
+          }
+          *reinterpret_cast<u32x2 *>(slice + c * 2 * DV + (((4 * dt + g) ^ (c % CPR)) * 16) + 8 * h) = low;
+        }
+      }
+      T *lb = static_cast<T *>(p.o_low) + (static_cast<int64_t>(b) * p.Hq + hq) * p.Sq * DV;
+#pragma unroll
+      for (int u = 0; u < 32 * CPR / 64; ++u) {
+        const int idx = u * 64 + lane, r = idx / CPR, q = idx % CPR;
+        vr[u] = *reinterpret_cast<const u32x4 *>(slice + r * 2 * DV + ((q ^ (r % CPR)) * 16));
+      }
+#pragma unroll
+      for (int u = 0; u < 32 * CPR / 64; ++u) {
+        const int idx = u * 64 + lane, r = idx / CPR, q = idx % CPR;
+        if (qw + r < p.Sq) *reinterpret_cast<u32x4 *>(lb + static_cast<int64_t>(qw + r) * DV + q * 8) = vr[u];
+      }
+    }
+  }
   if (a.lse && h == 0 && qrow < p.Sq)
     a.lse[(static_cast<int64_t>(b) * p.Hq + hq) * p.Sq + qrow] =
         lt > 0.f ? (m + log2f(lt)) * kLn2 : -INFINITY;

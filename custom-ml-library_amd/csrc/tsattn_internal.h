@@ -107,6 +107,8 @@ struct Problem {
   // Sliding window (0: none; causal problems): query i sees key j only where j <
   // sinks or j > i + offset - window.
   int window, sinks;
+  // Window, 16 bits: what rounding took from O, [B, Hq, Sq, Dv] (NULL: not kept).
+  void *o_low;
 };
 
 // The 32-key tiles that rows from q0 on see through a window, as one run: the tiles

@@ -194,11 +194,11 @@ SIGNATURES = {
         [_PP, _PV, _PV, _PV, _PV, _PV, c_void_p, _PV, _PV, _PV, c_void_p, c_size_t, c_void_p],
     ),
     "tsattn_sdpa_forward_rope": (c_int, [_PP, _PR, _PV, _PV, _PV, _PV, c_void_p, c_void_p]),
-    "tsattn_window_forward": (c_int, [_PP, c_int64, c_int32, _PR, _PV, _PV, _PV, _PV, c_void_p, c_void_p]),
+    "tsattn_window_forward": (c_int, [_PP, c_int64, c_int32, _PR, _PV, _PV, _PV, _PV, c_void_p, c_void_p, c_void_p]),
     "tsattn_window_backward_workspace": (c_size_t, [_PP, c_int64, c_int32, c_int32]),
     "tsattn_window_backward": (
         c_int,
-        [_PP, c_int64, c_int32, _PR, _PV, _PV, _PV, _PV, _PV, c_void_p, _PV, _PV, _PV, c_void_p, c_size_t,
+        [_PP, c_int64, c_int32, _PR, _PV, _PV, _PV, _PV, _PV, c_void_p, c_void_p, _PV, _PV, _PV, c_void_p, c_size_t,
          c_void_p],
     ),
     "tsattn_sdpa_forward_workspace": (c_size_t, [_PP]),

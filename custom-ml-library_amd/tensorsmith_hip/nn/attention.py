@@ -361,12 +361,18 @@ def scaled_dot_product_attention(
             keep.append(bits)
     lse_ptr = ctypes.c_void_p(None if lse is None else lse.data_ptr())
 
+    low = low_ptr = None
+    if window is not None and recording and code in (_lib.F16, _lib.BF16):
+        # what rounding takes from the output, for the backward's row sums
+        low = torch.empty(out.shape, dtype=out.dtype, device=tdev)
+        low_ptr = low.data_ptr()
+
     def attend(desc):
         if window is None:
             _forward(lib, prob, desc, vq, vk, vv, vo, lse_ptr, tdev, stream)
         else:
             _lib.check(launch(query.device, lib.tsattn_window_forward, ctypes.byref(prob), window, sinks, desc, vq,
-                              vk, vv, vo, lse_ptr), "windowed attention forward")
+                              vk, vv, vo, lse_ptr, low_ptr), "windowed attention forward")
 
     fused = False
     if rope is not None and k_pos0 is None:
@@ -421,7 +427,7 @@ def scaled_dot_product_attention(
             ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=tdev)
             _lib.check(launch(query.device, lib.tsattn_window_backward, ctypes.byref(prob), window, sinks,
                               ctypes.byref(rope[0]) if fused else None, vq, vk, vv, vo, _view(g), lse.data_ptr(),
-                              _view(dq), _view(dk), _view(dv), ws.data_ptr(), nbytes), "windowed attention backward")
+                              None if low is None else low.data_ptr(), _view(dq), _view(dk), _view(dv), ws.data_ptr(), nbytes), "windowed attention backward")
             return unrotated(dq, dk) + (dv,)
         nbytes = (lib.tsattn_sdpa_backward_rope_workspace if fused
                   else lib.tsattn_sdpa_backward_workspace)(ctypes.byref(prob))

@@ -245,13 +245,16 @@ int tsattn_sdpa_backward_rope(const tsattn_problem *p, const tsattn_rope_desc *r
  * mask of every pair: src/tensorsmith/nn/attention.py:102-113): query i, at position i +
  * causal_offset, sees key j only where j is one of the last `window` keys up to its own,
  * or one of the first `sinks`.  The kernels visit the tiles that hold such pairs alone.
- * rope may be NULL.  Causal problems (others: TSATTN_ERR_INVALID) of the MFMA kernels,
+ * rope may be NULL.  out_low: NULL, or 16-byte aligned room of out's 16-bit dtype,
+ * [batch, heads_q, len_q, dim_v], for what rounding takes from out; handed to the backward,
+ * it keeps the gradients of rows that see few keys as exact as the others'.
+ * Causal problems (others: TSATTN_ERR_INVALID) of the MFMA kernels,
  * without dropout and with no mask but key padding (p->kv_len); f32 without rope.
  * Others: TSATTN_ERR_UNSUPPORTED, nothing launched.
  */
 int tsattn_window_forward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
                           const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
-                          void *lse, void *stream);
+                          void *lse, void *out_low, void *stream);
 
 /* Bytes of scratch tsattn_window_backward needs (rope: whether it is given one). */
 size_t tsattn_window_backward_workspace(const tsattn_problem *p, int64_t window, int32_t sinks, int32_t rope);
@@ -259,8 +262,9 @@ size_t tsattn_window_backward_workspace(const tsattn_problem *p, int64_t window,
 /* Its VJP, as tsattn_sdpa_backward(_rope); deterministic. */
 int tsattn_window_backward(const tsattn_problem *p, int64_t window, int32_t sinks, const tsattn_rope_desc *rope,
                            const tsattn_view *q, const tsattn_view *k, const tsattn_view *v, const tsattn_view *out,
-                           const tsattn_view *dout, const void *lse, const tsattn_view *dq, const tsattn_view *dk,
-                           const tsattn_view *dv, void *workspace, size_t workspace_bytes, void *stream);
+                           const tsattn_view *dout, const void *lse, const void *out_low, const tsattn_view *dq,
+                           const tsattn_view *dk, const tsattn_view *dv, void *workspace, size_t workspace_bytes,
+                           void *stream);
 
 /*
  * The keep mask the attention kernels draw for problem `p` (its dropout

@@ -285,19 +285,22 @@ def _code(result):
 def test_the_library_refuses_windows():
     real, v = _lib.load(), _view()
     for window, sinks, p in ((0, 0, {}), (-1, 0, {}), (4, -1, {}), (4, 0, {"is_causal": 0}), (4, 0, {"len_q": 0})):
-        rc = real.tsattn_window_forward(ctypes.byref(_problem(**p)), window, sinks, None, v, v, v, v, None, None)
+        rc = real.tsattn_window_forward(ctypes.byref(_problem(**p)), window, sinks, None, v, v, v, v, None, None, None)
         assert _code(rc) == INVALID, (window, sinks, p)
         assert real.tsattn_window_backward_workspace(ctypes.byref(_problem(**p)), window, sinks, 0) == 0
     for p in ({"dim_qk": 48, "dim_v": 48}, {"dropout_p": 0.5}):
-        rc = real.tsattn_window_forward(ctypes.byref(_problem(**p)), 4, 0, None, v, v, v, v, None, None)
+        rc = real.tsattn_window_forward(ctypes.byref(_problem(**p)), 4, 0, None, v, v, v, v, None, None, None)
         assert _code(rc) == UNSUPPORTED, p
     # (views that are not 16-byte aligned have no windowed kernel)
-    rc = real.tsattn_window_forward(ctypes.byref(_problem()), 4, 0, None, _view(0x1002), v, v, v, None, None)
+    rc = real.tsattn_window_forward(ctypes.byref(_problem()), 4, 0, None, _view(0x1002), v, v, v, None, None, None)
     assert _code(rc) == UNSUPPORTED
+    for low, kw in ((0x1008, {}), (0x1000, {"dtype": _lib.F32})):  # (aligned, and of 16 bits)
+        rc = real.tsattn_window_forward(ctypes.byref(_problem(**kw)), 4, 0, None, v, v, v, v, None, low, None)
+        assert _code(rc) == INVALID
     need = real.tsattn_window_backward_workspace(ctypes.byref(_problem(len_q=600, len_kv=600)), 4, 1, 0)
     assert need > 0
     rc = real.tsattn_window_backward(ctypes.byref(_problem(len_q=600, len_kv=600)), 4, 1, None, v, v, v, v, v, 0x1000,
-                                     v, v, v, 0x1000, need - 1, None)
+                                     None, v, v, v, 0x1000, need - 1, None)
     assert _code(rc) == INVALID
 
 
