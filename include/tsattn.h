@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define TSATTN_ABI_VERSION 9 /* (the tsattn_pages4_* entry points came under it) */
+#define TSATTN_ABI_VERSION 9 /* (the entry points of the paged cache, windows, drafted trees and token probabilities came under it) */
 
 typedef enum {
   TSATTN_OK = 0,
