@@ -10,12 +10,11 @@
 //
 // The rows of a KV head (its query heads times the tokens) are the columns of S^T = K Q^T,
 // 32 to a wave, so that the statistics of a row are a lane's own and P^T is the operand of
-// O^T += V^T P^T as it comes.
-// Every wave works alone on tiles of its own through its own LDS ring and the waves'
-// results are joined at the end, or, for many rows of many heads, 4 waves of 32 rows share
-// each tile (plan_cached).
-// The tiles that a window leaves lie in one run, which splits cut into equal parts, as
-// many as fill the chip; a second kernel joins those.
+// O^T += V^T P^T as it comes.  Every wave works alone on tiles of its own through its own
+// LDS ring and the waves' results are joined at the end, or, for many rows of many heads, 4
+// waves of 32 rows share each tile (plan_cached).  The tiles that a window leaves lie in one
+// run, which splits cut into equal parts, as many as fill the chip; a second kernel joins
+// those.
 //
 // Bound by HBM for few rows (keys and values once), by the softmax beside the matrix
 // instructions from about 100 rows a KV head on.
@@ -51,10 +50,10 @@ struct CachedArgs {
 
 template <typename T, int D>
 constexpr int kPair = 2 * BN * D * (std::is_same_v<T, float> ? 4 : 2);  // bytes of a K and a V tile, in T
-// Waves of a workgroup, WR of them sharing each tile.  Up to 32 rows (WR 1) a wave's ring
-// of 16-bit tiles has room for one K and one V tile, so that 8 waves of 128 channels share
-// a CU: with room for more, 4 waves and 3 or 4 of a wave's tiles in flight, the step that
-// plan_cached names took the same time.
+// Waves of a workgroup, WR of them sharing each tile.  A wave of its own (WR 1) has room
+// for one K and one V tile of 16 bits, so that 8 waves of 128 channels share a CU: with
+// room for more, 4 waves and 3 or 4 of a wave's tiles in flight, the step that plan_cached
+// names took the same time.
 template <typename T, int D, int WR>
 constexpr int kWaves = WR > 1 ? WR : (kPair<T, D> <= 16384 ? 4 : 2);
 // Waves a SIMD that the registers must leave room for.
@@ -723,7 +722,8 @@ CachedPlan plan_cached(const CachedProblem &p) {
   s.gap = first - s.ns;
   s.run = tiles - s.gap;
   // A wave for each SIMD: a second one costs a few tokens over 16 or 32 bits more in partial
-  // results (step of 32 sequences, window 4096 of 8 heads of 128: 83 us, with two 90).
+  // results (step of 32 sequences, window 4096 of 8 heads of 128, through the memory-side
+  // cache: 96 us, with two 102).
   // Codes, and rows enough for several waves, keep a SIMD busy beside the loads, and take
   // two where the parts stay few (63 tokens of 16 sequences over 8000 keys, 8 heads of 128:
   // 241 us in one part, 204 in two; 16 heads, 24 tokens of 7 sequences, codes: 38 us in 9
