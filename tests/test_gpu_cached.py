@@ -483,3 +483,29 @@ def test_caches_larger_than_the_memory_side_cache(tokens, rep, n, d, dtype, int8
                     x.copy_(y[i:i + 1])
             one.length = n
             _close(got[i:i + 1], _reference(q[i:i + 1], one, _band(tokens, n, window, sinks)), dtype)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_offsets_past_32_bits(int8):
+    """The last sequence of a cache of more than 2^31 elements a side: attended, appended, kept and read back."""
+    b, h, d, room, n = 68, 8, 128, 32000, 700
+    big = nn.KVCache(b, h, d, room, device="hip", dtype=torch.float16, quantized=int8)
+    one = nn.KVCache(1, h, d, room, device="hip", dtype=torch.float16, quantized=int8)
+    assert big.storage[0].numel() > 2 ** 31
+    rows = [_rows(1, h, n, d, torch.float16, s) for s in (1, 2)]
+    tree = nn.DraftTree(_parents(np.random.default_rng(3), 1, 9)[0])
+    new = [_rows(b, x, 9, d, torch.float16, s) for x, s in ((h, 4), (h, 5), (4 * h, 6))]
+    outs = []
+    with ts.no_grad():
+        one.append(*(_wrap(x) for x in rows))
+        for x, y in zip(big.storage, one.storage):
+            if x is not None:
+                x[-1:, :, :n].copy_(y[:, :, :n])
+        big.length = n
+        for cache, at in ((big, slice(None)), (one, slice(b - 1, b))):
+            cache.append_tree(*(_wrap(x[at]) for x in new[:2]), tree, rotary_base=BASE)
+            outs.append(nn.cached_attention(_wrap(new[2][at]), cache, tree, rotary_base=BASE)._data)
+            cache.keep(n, np.tile([[8, 0, 3]], (cache.batch_size, 1)))
+            outs += [x._data for x in cache.get(5)]
+    for got, want in zip(outs[:3], outs[3:]):
+        assert (got[-1:].double() - want.double()).norm() <= 2.0 ** -10 * want.double().norm()

@@ -303,3 +303,21 @@ def test_rows_a_wave_each_and_rows_of_many_parts(rows, v):
     want, tol = _gradient(z, y, up.double(), torch.zeros_like(up).double(), None, None)
     # (and dz rounds once, by 2^-8 at most)
     assert ((leaf.grad._data.double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol) + 1e-38).all()
+
+
+def test_offsets_past_32_bits():
+    rows, v = 43000, 50021  # 2.15e9 logits
+    z = torch.zeros((rows, v), dtype=torch.bfloat16, device="cuda")
+    z[-3:], y = _logits(3, v, torch.bfloat16)[0], torch.full((rows,), -100, device="cuda")
+    y[-3:] = torch.tensor([5, 50020, 777], device="cuda")
+    leaf = _wrap(z, True)
+    got = F.token_log_probs(leaf, _wrap(y), 3)
+    tail = F.TokenLogProbs(*(_wrap(x._data[-3:]) for x in got))
+    _check(z[-3:], y[-3:], 3, tail)
+    up = torch.zeros(rows, device="cuda")
+    up[-3:] = torch.tensor([1.0, -2.0, 0.5], device="cuda")
+    got.log_probs.backward(_wrap(up))
+    want, tol = _gradient(z[-3:], y[-3:], up[-3:].double(), torch.zeros(3, device="cuda").double(), None, None)
+    grad = leaf.grad._data
+    assert ((grad[-3:].double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol) + 1e-38).all()
+    assert not grad[:5].any() and not grad[rows // 2:rows // 2 + 5].any()
