@@ -7,13 +7,18 @@
 // where both terms of H are >= 0, so that nothing cancels; a logit of -inf adds
 // nothing.  The VJP, for upstream gradients g of log p_y, gh of H and t_i of the top
 // tokens' log probabilities (at indices k_i), G = g + sum_i t_i:
-//   dz_j = -p_j (G + gh (ln p_j + H)) + [j = y] g + sum_i [j = k_i] t_i.
+//   dz_j = -p_j (G + gh (ln p_j + H)) + [j = y] g + sum_i [j = k_i] t_i,
+// p_j from z_j - m, which does not overflow upwards, and the log2 l that the forward kept.
 //
-// In log2 units throughout, t_j = z_j log2 e - b as one fused operation, b the row's
-// largest z log2 e as it rounds: b cancels from every result, so its rounding does too.
+// A lane's sums are in log2 units, t_j = z_j log2 e - b as one fused operation, b = m log2 e
+// as it rounds.  What that rounding takes, r = m log2 e - b, is in every t of the lane alike,
+// and `exact` takes it out again before sums meet, as 2^-r.  That needs an r that exp2 can
+// hold: logits past kFar (2^20, r at most 2^-4), among them masks of -1e10 or of the type's
+// lowest value, whose product with log2 e may overflow besides, turn the wave to t_j = (z_j -
+// m) log2 e from then on, two instructions a logit more.
 //
 // Bound by HBM: the forward reads the logits once, the VJP reads them and writes the
-// gradient.  One pass in each: a lane keeps a running (b, l, sum 2^t t) and rescales it
+// gradient.  One pass in each: a lane keeps a running (m, l, sum 2^t t) and rescales it
 // once for every four 16-byte pieces.  The forward is about as far from the vector units'
 // bound: 6 instructions a logit; 11 of them (selects for rows' ends and -inf on every
 // one) took 131 us where 8192 rows of 50021 bf16, a fifth of them ignored, take 107
@@ -45,6 +50,8 @@ constexpr int U = 4;         // 16-byte pieces a lane has in flight
 constexpr int PENDING = 64 + 64 * 8;  // keys a wave's buffer holds: < 64 left over, and one piece of each lane
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kFar = 1048576.f;  // logits from which z log2 e - b is not taken
+constexpr float kLeast = -1e30f;   // 2^t is 0 from here on, and times t too (t may be -inf)
 
 struct ProbArgs {
   int64_t rows;
@@ -54,10 +61,10 @@ struct ProbArgs {
   const void *tokens;
   int token_bytes;
   int64_t ignore;
-  float *logp, *entropy, *stats;  // stats: [rows][2] = b, log2 l
+  float *logp, *entropy, *stats;  // stats: [rows][2] = m, log2 l
   float *top_logp;
   int64_t *top_index;
-  float *part;                   // [rows][splits][4]: m, l, sum e x (log2 units)
+  float *part;                   // [rows][splits][4]: m, l, sum 2^t t
   unsigned long long *part_top;  // [rows][splits][top]
   // VJP
   const float *g, *gh, *gt, *saved_entropy;
@@ -99,22 +106,42 @@ __device__ __forceinline__ int64_t token_of(const ProbArgs &a, int64_t row) {
 }
 
 // ---------------------------------------------------------------------------
-// Running sums: m the base b, l = sum 2^t, w = sum 2^t t.
+// Running sums: m the largest logit, l = sum 2^t, w = sum 2^t t.
 // ---------------------------------------------------------------------------
 struct Sums {
   float m, l, w;
 };
 
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m != -INFINITY; }
 // (a base that keeps 2^(-inf - base) = 0 while nothing but -inf has come)
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+// b, rounded here (a fused operation further on would round it otherwise)
+__device__ __forceinline__ float scaled(float m) {
+  float b = base_of(m) * kLog2e;
+  asm("" : "+v"(b));
+  return b;
+}
 
-__device__ __forceinline__ void rebase(Sums &s, float m) {
-  const float d = base_of(s.m) - base_of(m);
+__device__ __forceinline__ void shift(Sums &s, float d) {
   const float c = __builtin_amdgcn_exp2f(d);
   // an empty sum stays empty whatever the bases (0 * inf is NaN)
-  s.w = s.l == 0.f ? s.w : c * fmaf(s.l, fmaxf(d, -1e30f), s.w);
+  s.w = s.l == 0.f ? s.w : c * fmaf(s.l, fmaxf(d, kLeast), s.w);
   s.l = s.l == 0.f ? s.l : s.l * c;
+}
+// Sums over t = (z - m) log2 e, to another m.
+__device__ __forceinline__ void rebase(Sums &s, float m) {
+  shift(s, (s.m - m) * kLog2e);
   s.m = m;
+}
+// Sums over t = z log2 e - b, to another m.
+__device__ __forceinline__ void rebase_near(Sums &s, float m) {
+  shift(s, scaled(s.m) - scaled(m));
+  s.m = m;
+}
+// Those as sums over (z - m) log2 e.
+__device__ __forceinline__ Sums exact(Sums s) {
+  const float b = scaled(s.m), r = fmaf(base_of(s.m), kLog2e, -b), c = __builtin_amdgcn_exp2f(-r);
+  return Sums{s.m, s.l * c, fmaf(-r, s.l, s.w) * c};
 }
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
   const float m = fmaxf(a.m, b.m);
@@ -146,19 +173,20 @@ __device__ __forceinline__ float largest(const float (&x)[N]) {
   return m;
 }
 
-// Adds N logits, none above the base; `own` becomes their sum of exponentials (NaN where
-// one is NaN or +inf).  A logit of -inf makes w a NaN (0 times -inf) unless SAFE, at an
-// instruction a logit.
-template <bool SAFE, int N>
+// Adds N logits, none above m; `own` becomes their sum of exponentials (NaN where one is
+// NaN or +inf).  NEAR: z log2 e - b, where a logit of -inf makes w a NaN (0 times -inf);
+// SAFE: the same, but that, at an instruction a logit; FAR: (z - m) log2 e, as safe.
+enum Sort { NEAR, SAFE, FAR };
+template <Sort S, int N>
 __device__ __forceinline__ void add(Sums &s, const float (&x)[N], float &own) {
-  const float base = base_of(s.m);
+  const float base = S == FAR ? base_of(s.m) : scaled(s.m);
   float l = 0.f;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const float t = fmaf(x[e], kLog2e, -base);
+    const float t = S == FAR ? (x[e] - base) * kLog2e : fmaf(x[e], kLog2e, -base);
     const float p = __builtin_amdgcn_exp2f(t);
     l += p;
-    s.w = fmaf(p, SAFE ? fmaxf(t, -1e30f) : t, s.w);
+    s.w = fmaf(p, S == NEAR ? t : fmaxf(t, kLeast), s.w);
   }
   s.l += l;
   own = l;
@@ -295,7 +323,7 @@ __device__ __forceinline__ void results(const ProbArgs &a, int64_t row, Sums s, 
   if (lane == 0) {
     const int64_t y = token_of(a, row);
     const float z = y >= 0 && y < a.vocab ? static_cast<float>(static_cast<const T *>(a.z)[row * a.zs + y]) : NAN;
-    a.logp[row] = (fmaf(z, kLog2e, -m) - log2l) * kLn2;
+    a.logp[row] = fmaf(-log2l, kLn2, z - m);
     a.entropy[row] = m == -INFINITY ? NAN : (log2l - s.w / s.l) * kLn2;
     if (a.stats) {
       a.stats[2 * row] = m;
@@ -304,7 +332,7 @@ __device__ __forceinline__ void results(const ProbArgs &a, int64_t row, Sums s, 
   }
   if constexpr (TOP) {
     if (lane < a.top) {
-      a.top_logp[row * a.top + lane] = (fmaf(key_logit(best), kLog2e, -m) - log2l) * kLn2;
+      a.top_logp[row * a.top + lane] = fmaf(-log2l, kLn2, key_logit(best) - m);
       a.top_index[row * a.top + lane] = ~static_cast<unsigned>(best);
     }
   }
@@ -358,12 +386,22 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
   Sums s{-INFINITY, 0.f, 0.f};
   Best top;
   top.buffer = buffers + (TOP ? w * PENDING : 0);
+  bool far = false;  // of the wave: its sums are over (z - m) log2 e
+  auto raise = [&](float most) __attribute__((always_inline)) {
+    if (!far && __ballot(is_far(most)) != 0ull) {
+      s = exact(s);
+      far = true;
+    }
+    if (far) rebase(s, most);
+    else rebase_near(s, most);
+  };
   // the elements in front of the first piece, one a lane
   auto single = [&](int first, int n) {
     const float x[1] = {lane < n ? static_cast<float>(r.z[first + lane]) : -INFINITY};
     float own;
-    rebase(s, fmaxf(s.m, x[0] * kLog2e));
-    add<true>(s, x, own);
+    raise(fmaxf(s.m, x[0]));
+    if (far) add<FAR>(s, x, own);
+    else add<SAFE>(s, x, own);
     if constexpr (TOP) top.offer(x, x[0], own, first + lane, lane < n ? 1 : 0, a.top, lane);
   };
   const int l0 = (WPR == 1 ? 0 : w * 64) + lane;
@@ -392,22 +430,30 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
         for (int e = 0; e < VE; ++e) x[u][e] = -INFINITY;
       }
       mx[u] = largest(x[u]);
-      most = fmaxf(most, mx[u] * kLog2e);
+      most = fmaxf(most, mx[u]);
     }
-    rebase(s, most);
+    raise(most);
     const Sums before = s;
     float own[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u * LANES >= p1) break;
-      add<false>(s, x[u], own[u]);
-    }
-    if (__ballot(s.w != s.w) != 0ull) {  // a logit of -inf: again
-      s = before;
+    if (far) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + u * LANES >= p1) break;
-        add<true>(s, x[u], own[u]);
+        add<FAR>(s, x[u], own[u]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u * LANES >= p1) break;
+        add<NEAR>(s, x[u], own[u]);
+      }
+      if (__ballot(s.w != s.w) != 0ull) {  // a logit of -inf: again
+        s = before;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i + u * LANES >= p1) break;
+          add<SAFE>(s, x[u], own[u]);
+        }
       }
     }
     if constexpr (TOP) {
@@ -422,7 +468,7 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
     for (int u = 0; u < U; ++u) raw[u] = next[u];
   }
   if (part == splits - 1 && (WPR == 1 || w == NW - 1) && r.tail) single(a.vocab - r.tail, r.tail);
-  s = wave_join(s);
+  s = wave_join(far ? s : exact(s));
   if constexpr (TOP) top.finish(a.top, lane);
   if constexpr (WPR > 1) {
     if (lane == 0) red[w][0] = s.m, red[w][1] = s.l, red[w][2] = s.w;
@@ -534,8 +580,8 @@ __global__ __launch_bounds__(NT) void probs_vjp_kernel(ProbArgs a) {
   const float c = gh == 0.f ? all : fmaf(gh, a.saved_entropy[row], all);
   const float gl = gh * kLn2;
   auto at_logit = [&](float x) {
-    const float t = fmaf(x, kLog2e, -m) - log2l;  // log2 p
-    return -__builtin_amdgcn_exp2f(t) * fmaf(gl, fmaxf(t, -1e30f), c);
+    const float t = fmaf(x - m, kLog2e, -log2l);  // log2 p
+    return -__builtin_amdgcn_exp2f(t) * fmaf(gl, fmaxf(t, kLeast), c);
   };
   const int yi = y >= 0 && y < a.vocab ? static_cast<int>(y) : -1;
   auto single = [&](int j) {

@@ -321,3 +321,60 @@ def test_offsets_past_32_bits():
     grad = leaf.grad._data
     assert ((grad[-3:].double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol) + 1e-38).all()
     assert not grad[:5].any() and not grad[rows // 2:rows // 2 + 5].any()
+
+
+def _lowest(dtype):
+    return torch.finfo(dtype).min
+
+
+def _far_rows(v, dtype, low):
+    """Rows of ordinary logits with `low` in front, in the middle, behind, everywhere but in one place and everywhere."""
+    z, _ = _logits(6, v, dtype)
+    z[0, :v // 2] = low
+    z[1, v // 3:v // 3 + v // 5] = low
+    z[2, v - v // 4:] = low
+    z[3], z[3, (2 * v) // 3] = low, 1.0
+    z[4] = low
+    z[5, :min(v, 70)] = low
+    # tokens with and without an ordinary logit
+    return z, torch.tensor([0, v // 3, v - 1, (2 * v) // 3, v // 2, v - 1], device="cuda")
+
+
+@pytest.mark.parametrize("dtype,low", [(d, low) for d in (torch.float32, torch.bfloat16)
+                                       for low in (-1e7, -1e9, -1e10, -1e20, -1e30, _lowest(d))]
+                         + [(torch.float16, _lowest(torch.float16))])
+@pytest.mark.parametrize("v", [50, 2500, 30000])
+def test_finite_masks_of_any_size(v, dtype, low):
+    z, y = _far_rows(v, dtype, low)
+    for top in (0, 5, 50):
+        print("token probs", v, dtype, low, top, flush=True)
+        _check(z, y, top, F.token_log_probs(_wrap(z), _wrap(y), top))
+    g, gh = (torch.randn(6, generator=torch.Generator(device="cuda").manual_seed(v + n), device="cuda") for n in (1, 2))
+    x = _wrap(z, True)
+    got = F.token_log_probs(x, _wrap(y))
+    (got.log_probs * _wrap(g) + got.entropy * _wrap(gh)).sum().backward()
+    want, tol = _gradient(z, y, g.double(), gh.double(), None, None)
+    tol = tol + torch.finfo(dtype).eps / 2 * (want.abs() + tol) + torch.finfo(dtype).smallest_normal
+    assert ((x._grad.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("high", [1e7, 1e10, 1e30, 3e38])
+@pytest.mark.parametrize("v", [50, 2500, 30000])
+def test_large_logits(v, high, dtype):
+    z, _ = _logits(5, v, dtype)
+    z[0, v // 2] = high
+    z[1, v - 1] = z[1, 0] = high
+    z[2] = high
+    z[3] = -high
+    z[4] = torch.linspace(0, high, v, device="cuda").to(dtype)
+    y = torch.tensor([v // 2, 1, 7, v - 1, v - 1], device="cuda")
+    for top in (0, 5):
+        print("token probs", v, dtype, high, top, flush=True)
+        _check(z, y, top, F.token_log_probs(_wrap(z), _wrap(y), top))
+    up = torch.tensor([1.0, -2.0, 0.5, 3.0, -1.0], device="cuda")
+    x = _wrap(z, True)
+    F.token_log_probs(x, _wrap(y)).log_probs.backward(_wrap(up))
+    want, tol = _gradient(z, y, up.double(), torch.zeros(5, device="cuda").double(), None, None)
+    tol = tol + torch.finfo(dtype).eps / 2 * (want.abs() + tol) + torch.finfo(dtype).smallest_normal
+    assert ((x._grad.double() - want).abs() <= tol).all()
