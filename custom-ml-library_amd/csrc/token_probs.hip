@@ -51,7 +51,7 @@ constexpr int PENDING = 64 + 64 * 8;  // keys a wave's buffer holds: < 64 left o
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = 1048576.f;  // logits from which z log2 e - b is not taken
-constexpr float kLeast = -1e30f;   // 2^t is 0 from here on, and times t too (t may be -inf)
+constexpr float kLeast = -1e4f;    // 2^t is 0 from here on, and so is its product with t and a factor below 3e34
 
 struct ProbArgs {
   int64_t rows;

@@ -378,3 +378,18 @@ def test_large_logits(v, high, dtype):
     want, tol = _gradient(z, y, up.double(), torch.zeros(5, device="cuda").double(), None, None)
     tol = tol + torch.finfo(dtype).eps / 2 * (want.abs() + tol) + torch.finfo(dtype).smallest_normal
     assert ((x._grad.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("v", [50, 2500, 30000])
+def test_large_upstream_gradients(v):
+    z, y = _logits(3, v, torch.float32)
+    z[:, v // 2] = -math.inf
+    y = torch.where(y == v // 2, 0, y)
+    g, gh = torch.tensor([1e12, -3e15, 0.0], device="cuda"), torch.tensor([-1e10, 1e20, 3e30], device="cuda")
+    print("token probs vjp", v, flush=True)
+    x = _wrap(z, True)
+    got = F.token_log_probs(x, _wrap(y))
+    (got.log_probs * _wrap(g) + got.entropy * _wrap(gh)).sum().backward()
+    want, tol = _gradient(z, y, g.double(), gh.double(), None, None)
+    assert ((x._grad.double() - want).abs() <= tol + U * (want.abs() + tol)).all()
+    assert (x._grad[:, v // 2] == 0).all()
