@@ -62,7 +62,12 @@ class KVCache:
         self._key_scales = torch.ones(shape + (1,), dtype=torch.float32, device=dev) if quantized else None
         self._value_scales = (torch.ones(shape + (1,), dtype=torch.float32, device=dev)
                               if quantized else None)
-        self._described: tuple = ()
+
+    _described: tuple = ()
+
+    def __getstate__(self):
+        """What copies and pickles take: the views of ``_views`` are this cache's arrays' own."""
+        return {name: value for name, value in self.__dict__.items() if name != "_described"}
 
     def append(self, key: Tensor, value: Tensor) -> tuple[Tensor, Tensor]:
         """Append a chunk after validating all shapes and capacity."""

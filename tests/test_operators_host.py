@@ -3,7 +3,9 @@ what they refuse, what a refusal leaves as it was, and where and with what they 
 
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 
 import numpy as np
 import pytest
@@ -240,6 +242,26 @@ def test_the_last_rows_of_a_cache(lib):
     for bad in (-1, 10):
         with pytest.raises(ValueError):
             cache.get(bad)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("again", [copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))])
+def test_a_cache_in_use_can_be_copied(lib, again, quantized):
+    cache = _cache(quantized=quantized)
+    tree = nn.DraftTree([-1, 0], device="hip:0")
+    with ts.no_grad():
+        cache.get()
+        cache.append_tree(_draw(2, 2, 2, 64), _draw(2, 2, 2, 64), tree)
+        nn.cached_attention(_draw(2, 2, 2, 64), cache, tree)
+        cache.keep(10, [[1], [0]])
+        other = again(cache)
+        assert other.length == cache.length == 11 and other.device == cache.device
+        assert all(torch.equal(a, b) and a.data_ptr() != b.data_ptr()
+                   for a, b in zip(cache.storage, other.storage) if a is not None)
+        nn.cached_attention(_draw(2, 2, 2, 64), other)
+        assert lib.args["tsattn_cached_attend"][2].data == other._keys.data_ptr()
+        shared = copy.copy(cache)  # (another cache over the same arrays)
+        assert shared._keys is cache._keys and len(shared) == 11
 
 
 def test_codes_are_read_on_the_caches_device(lib):
