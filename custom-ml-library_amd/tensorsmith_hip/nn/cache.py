@@ -287,6 +287,7 @@ class KVCache:
         import torch
 
         order = torch.as_tensor(host.astype(np.int64), device=self._keys.device)
+        self._described = ()  # (it would hold the old keys)
         self._keys, self._values = self._keys[order], self._values[order]
         if self.quantized:
             self._key_scales = self._key_scales[order]

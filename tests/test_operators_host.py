@@ -6,6 +6,7 @@ from __future__ import annotations
 import copy
 import ctypes
 import pickle
+import weakref
 
 import numpy as np
 import pytest
@@ -262,6 +263,18 @@ def test_a_cache_in_use_can_be_copied(lib, again, quantized):
         assert lib.args["tsattn_cached_attend"][2].data == other._keys.data_ptr()
         shared = copy.copy(cache)  # (another cache over the same arrays)
         assert shared._keys is cache._keys and len(shared) == 11
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_a_reordered_cache_lets_its_old_arrays_go(lib, quantized):
+    cache = _cache(quantized=quantized)
+    with ts.no_grad():
+        nn.cached_attention(_draw(2, 2, 1, 64), cache)
+        old = [weakref.ref(x) for x in cache.storage if x is not None]
+        cache.reorder([1, 0])
+        assert all(x() is None for x in old)
+        nn.cached_attention(_draw(2, 2, 1, 64), cache)
+        assert lib.args["tsattn_cached_attend"][2].data == cache._keys.data_ptr()
 
 
 def test_codes_are_read_on_the_caches_device(lib):
