@@ -1921,18 +1921,9 @@ size_t mfma_ds_bytes(const Problem &p) {
   return static_cast<size_t>(bytes);
 }
 
-// Key blocks with sinks, and the parts of each: of about the query tiles that the other
-// blocks see (B2 Hkv4 S8192, window 1024: 7 parts of 37 tiles), at most 64.
-static int window_sink_blocks(const Problem &p) { return min((p.sinks + KB - 1) / KB, (p.Sk + KB - 1) / KB); }
-static int window_parts(const Problem &p) {
-  const int64_t all = (p.Sq + QT - 1) / QT, other = (KB + static_cast<int64_t>(p.window)) / QT + 1;
-  const int64_t parts = (all + other - 1) / other;
-  return static_cast<int>(parts < 64 ? parts : 64);
-}
-
 size_t mfma_window_bytes(const Problem &p) {
-  const int blocks = p.window ? window_sink_blocks(p) : 0, parts = blocks ? window_parts(p) : 1;
-  return parts < 2 ? 0 : static_cast<size_t>(p.B) * p.Hkv * blocks * parts * KB * (p.Dqk + p.Dv) * sizeof(float);
+  const SinkParts s(p, KB);
+  return s.parts < 2 ? 0 : static_cast<size_t>(p.B) * p.Hkv * s.blocks * s.parts * KB * (p.Dqk + p.Dv) * sizeof(float);
 }
 
 hipError_t launch_mfma_backward(const Problem &p, int dtype, View q, View k, View v, View o,
@@ -1951,8 +1942,8 @@ hipError_t launch_mfma_backward(const Problem &p, int dtype, View q, View k, Vie
             p.window ? nullptr : static_cast<char *>(ds), ds_key_tiles(p), ds_packed(p), ds_slice_tiles(p),
             0, p.B * p.Hkv, 0, 1, nullptr};
   if (p.window) {
-    a.sink_blocks = window_sink_blocks(p);
-    a.parts = a.sink_blocks ? window_parts(p) : 1;
+    const SinkParts s(p, KB);
+    a.sink_blocks = s.blocks, a.parts = s.parts;
     a.part = static_cast<float *>(ds);
   }
   return dtype == TSATTN_BF16 ? launch<bf16>(a, st) : launch<f16>(a, st);

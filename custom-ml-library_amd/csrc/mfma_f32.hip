@@ -1320,14 +1320,6 @@ __global__ __launch_bounds__(NT) void sink_sum_f32_kernel(F32Args a, int keys) {
       float4{x.x * f, x.y * f, x.z * f, x.w * f};
 }
 
-// Key blocks of `keys` keys with sinks, and the parts of each (as mfma_bwd.hip's).
-int window_blocks(const Problem &p, int keys) { return min((p.sinks + keys - 1) / keys, (p.Sk + keys - 1) / keys); }
-int window_parts(const Problem &p, int keys) {
-  const int64_t all = (p.Sq + BN - 1) / BN, other = (keys + static_cast<int64_t>(p.window)) / BN + 1;
-  const int64_t parts = (all + other - 1) / other;
-  return static_cast<int>(parts < 64 ? parts : 64);
-}
-
 template <int D, int MK, bool WIN>
 void launch_bwd_dims(const F32Args &a0, hipStream_t st) {
   F32Args a = a0;
@@ -1347,8 +1339,8 @@ void launch_bwd_dims(const F32Args &a0, hipStream_t st) {
   }
   const int keys = split_k ? 32 : KB;
   if constexpr (WIN) {
-    a.sink_blocks = window_blocks(p, keys);
-    a.parts = a.sink_blocks ? window_parts(p, keys) : 1;
+    const SinkParts s(p, keys);
+    a.sink_blocks = s.blocks, a.parts = s.parts;
   }
   const int more = WIN ? a.sink_blocks * (a.parts - 1) : 0;  // units of the sinks' blocks beyond their own
   if (split_q) {
@@ -1413,8 +1405,8 @@ size_t mfma_f32_window_bytes(const Problem &p) {
   if (!p.window || !p.sinks) return 0;
   size_t most = 0;
   for (const int keys : {32, KB}) {  // (which of the two runs is the launch's choice)
-    const int parts = window_parts(p, keys);
-    const size_t n = parts < 2 ? 0 : static_cast<size_t>(p.B) * p.Hkv * window_blocks(p, keys) * parts * keys * 2 * p.Dqk;
+    const SinkParts s(p, keys);
+    const size_t n = s.parts < 2 ? 0 : static_cast<size_t>(p.B) * p.Hkv * s.blocks * s.parts * keys * 2 * p.Dqk;
     most = n > most ? n : most;
   }
   return most * sizeof(float);

@@ -133,6 +133,26 @@ __device__ __forceinline__ int window_low(const Problem &p, int q) {
   return static_cast<int>(lo < 0 ? 0 : (lo < p.Sk ? lo : p.Sk));
 }
 
+// Windowed dK/dV: the key blocks (of `keys` keys) that hold sinks, and the parts that the
+// query rows of each are cut into: as many as leave a part about the query tiles (of 32
+// rows) that the other blocks see (B2 Hkv4 S8192, window 1024: 7 parts of 37 tiles), at
+// most 64, and no more than give every one of 256 CUs 8 workgroups, which bounds the scratch
+// of the partial sums, 128 KiB a part of 128 keys and channels, at 256 MiB.  (B4 H8 S32768
+// D128, window 128, 4096 sinks, bf16, forward and backward: 1024 blocks in 2 parts 8.9 ms;
+// in 64, 8 GiB of sums, 12.1.  B1, window 512: 256 blocks in 8 parts 2.6 ms, in 50 3.1.)
+struct SinkParts {
+  int blocks, parts;
+  SinkParts(const Problem &p, int keys) : blocks(0), parts(1) {
+    if (!p.window || !p.sinks) return;
+    blocks = ((p.sinks < p.Sk ? p.sinks : p.Sk) + keys - 1) / keys;
+    const int64_t all = (static_cast<int64_t>(p.Sq) + 31) / 32, other = (keys + static_cast<int64_t>(p.window)) / 32 + 1;
+    int64_t n = (all + other - 1) / other;
+    const int64_t most = 8 * 256 / (static_cast<int64_t>(p.B) * p.Hkv * blocks);
+    n = n < most ? n : most;
+    parts = static_cast<int>(n < 1 ? 1 : n < 64 ? n : 64);
+  }
+};
+
 // Mask handling of the MFMA kernels (a template parameter): 0 = none, or a
 // key mask [B,1,1,K] reduced to kv_len / kv_prefix; 1 = any other boolean
 // mask, read per (row, key) from its strides; 2 / 3 = an additive f32 /

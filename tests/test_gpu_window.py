@@ -275,3 +275,11 @@ def test_gradients_of_few_keys_lose_nothing_to_the_rounded_output(window, d, dty
     for name, leaf, exact in zip("qk", leaves, want[1:3]):
         off = ((leaf._grad.double() - exact).norm() / exact.norm()).item()
         assert off <= 0.72 * torch.finfo(dtype).eps / 2, (name, off)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("sinks", [130, 300, 1000])
+def test_sinks_of_many_blocks_and_heads(sinks, dtype):
+    """Blocks enough to fill the chip are cut into fewer parts, down to none."""
+    print("window", sinks, dtype, flush=True)
+    _check(*_operands(32, 8, 8, 1100, 1100, 32, 32, dtype), 5, sinks)

@@ -339,6 +339,18 @@ def test_the_library_refuses_windows():
     assert _code(rc) == INVALID
 
 
+@pytest.mark.parametrize("dtype,d", [(_lib.F16, 64), (_lib.BF16, 128), (_lib.F32, 128), (_lib.F32, 32)])
+def test_the_scratch_of_sinks_is_bounded(dtype, d):
+    """At most 256 MiB of partial sums (8 workgroups a CU, each 128 keys of 128 channels), whatever the sinks."""
+    real = _lib.load()
+    for batch, heads, s, window, sinks in ((8, 8, 32768, 512, 4096), (4, 8, 32768, 128, 4096), (1, 8, 32768, 512, 4096),
+                                           (1, 1, 1 << 20, 1, 1 << 19), (64, 8, 8192, 64, 4), (2, 4, 8192, 1024, 4)):
+        p = _problem(dtype=dtype, batch=batch, heads_q=heads, heads_kv=heads, len_q=s, len_kv=s, dim_qk=d, dim_v=d)
+        need = real.tsattn_window_backward_workspace(ctypes.byref(p), window, sinks, 0)
+        rows = real.tsattn_window_backward_workspace(ctypes.byref(p), window, 0, 0)
+        assert 0 < rows <= need <= rows + (256 << 20) + 256, (batch, heads, s, window, sinks)
+
+
 def _cached(**kw):
     d = _lib.Cached(_lib.F16, 2, 4, 2, 64, 3, 10, 0, 0.125, 0, 0, 0, None, None, None, None)
     for name, value in kw.items():
