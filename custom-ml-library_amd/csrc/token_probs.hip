@@ -668,23 +668,45 @@ int prob_splits(int64_t rows, int vocab) {
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
+// The rows from `first` on, `rows` of them (rows in parts come in one piece, first = 0).
+template <typename T>
+ProbArgs some_rows(ProbArgs a, int64_t first, int64_t rows) {
+  auto from = [first](auto *p, int64_t each) { return p ? p + first * each : p; };
+  a.rows = rows;
+  a.z = from(static_cast<const T *>(a.z), a.zs);
+  a.tokens = from(static_cast<const char *>(a.tokens), a.token_bytes);
+  a.logp = from(a.logp, 1), a.entropy = from(a.entropy, 1), a.stats = from(a.stats, 2);
+  a.top_logp = from(a.top_logp, a.top), a.top_index = from(a.top_index, a.top);
+  a.g = from(a.g, 1), a.gh = from(a.gh, 1), a.gt = from(a.gt, a.top);
+  a.saved_entropy = from(a.saved_entropy, 1), a.saved_index = from(a.saved_index, a.top);
+  a.dz = from(static_cast<T *>(a.dz), a.vocab);
+  return a;
+}
+
+// A grid has fewer than 2^32 work-items: 2^23 workgroups at a time.
+constexpr int64_t kMostGroups = int64_t(1) << 23;
+
 template <typename T, bool TOP>
-void forward(ProbArgs &a, hipStream_t st) {
-  if (wave_rows(a.rows, a.vocab)) {
-    probs_kernel<T, 1, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
-    return;
+void forward(const ProbArgs &all, hipStream_t st) {
+  const bool wave = wave_rows(all.rows, all.vocab);
+  const int64_t most = kMostGroups * (wave ? NW : 1);
+  for (int64_t first = 0; first < all.rows; first += most) {
+    const ProbArgs a = some_rows<T>(all, first, all.rows - first < most ? all.rows - first : most);
+    if (wave) probs_kernel<T, 1, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
+    else probs_kernel<T, NW, TOP><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(NT), 0, st>>>(a);
+    if (a.splits > 1) probs_merge_kernel<T, TOP><<<dim3(static_cast<unsigned>(a.rows)), dim3(NT), 0, st>>>(a);
   }
-  probs_kernel<T, NW, TOP><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(NT), 0, st>>>(a);
-  if (a.splits > 1)
-    probs_merge_kernel<T, TOP><<<dim3(static_cast<unsigned>(a.rows)), dim3(NT), 0, st>>>(a);
 }
 
 template <typename T, bool TOP>
-void backward(ProbArgs &a, hipStream_t st) {
-  if (wave_rows(a.rows, a.vocab))
-    probs_vjp_kernel<T, 1, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
-  else
-    probs_vjp_kernel<T, NW, TOP><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(NT), 0, st>>>(a);
+void backward(const ProbArgs &all, hipStream_t st) {
+  const bool wave = wave_rows(all.rows, all.vocab);
+  const int64_t most = kMostGroups * (wave ? NW : 1);
+  for (int64_t first = 0; first < all.rows; first += most) {
+    const ProbArgs a = some_rows<T>(all, first, all.rows - first < most ? all.rows - first : most);
+    if (wave) probs_vjp_kernel<T, 1, TOP><<<dim3(static_cast<unsigned>((a.rows + NW - 1) / NW)), dim3(NT), 0, st>>>(a);
+    else probs_vjp_kernel<T, NW, TOP><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(NT), 0, st>>>(a);
+  }
 }
 
 }  // namespace

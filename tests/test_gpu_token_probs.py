@@ -393,3 +393,37 @@ def test_large_upstream_gradients(v):
     want, tol = _gradient(z, y, g.double(), gh.double(), None, None)
     assert ((x._grad.double() - want).abs() <= tol + U * (want.abs() + tol)).all()
     assert (x._grad[:, v // 2] == 0).all()
+
+
+@pytest.mark.parametrize("rows,v", [((1 << 26) + 5, 3), ((1 << 24) + 3, 4097)])
+def test_more_rows_than_a_grid_holds(rows, v):
+    """Of a wave and of a workgroup a row: every row's results, and the gradient of the shorter ones."""
+    z = torch.randn((rows, v) if v < 9 else (1, v), device="cuda", dtype=torch.float16).expand(rows, v)  # (long: one row)
+    y = torch.arange(rows, device="cuda", dtype=torch.int32) % v
+    y[5] = y[-2] = -100
+    print("token probs", rows, v, flush=True)
+    live = y >= 0
+    with ts.no_grad():
+        got = F.token_log_probs(_wrap(z), _wrap(y), 1)
+    assert (got.log_probs._data[~live] == 0).all() and (got.top_indices._data[~live] == -1).all()
+    d = _spread(v)
+    if v > 9:
+        lp, _, entropy = _want(z[:1], y[:1])
+        want = lp[0].float()[y.long().clamp(min=0)]
+        assert ((got.log_probs._data - want).abs() <= d + 5 * U * want.abs())[live].all()
+        assert ((got.entropy._data - entropy.float()).abs() <= d + 2 * d * math.log(v) + 6 * U * math.log(v))[live].all()
+        assert (got.top_indices._data[live] == z[0].argmax()).all()
+        return
+    for part in range(0, rows, 1 << 24):
+        zz, at = z[part:part + (1 << 24)], y[part:part + (1 << 24)].long().clamp(min=0)
+        want = torch.log_softmax(zz.double(), -1).gather(-1, at[:, None])[:, 0]
+        close = (got.log_probs._data[part:part + (1 << 24)] - want).abs() <= d + 3 * U * want.abs().clamp(min=1)
+        assert close[live[part:part + (1 << 24)]].all()
+    leaf = _wrap(z, True)
+    F.token_log_probs(leaf, _wrap(y)).log_probs.backward(_wrap(torch.ones(rows, device="cuda")))
+    for part in range(0, rows, 1 << 24):
+        zz, at = z[part:part + (1 << 24)], y[part:part + (1 << 24)].long()
+        p = torch.softmax(zz.double(), -1)
+        want = (torch.nn.functional.one_hot(at.clamp(min=0), v) - p) * (at >= 0)[:, None]
+        tol = d + 30 * U + 2.0 ** -11 * want.abs() + 2.0 ** -25  # (f16: half a step, below its normal numbers 2^-25)
+        assert ((leaf._grad[part:part + (1 << 24)].double() - want).abs() <= tol).all()
