@@ -987,10 +987,10 @@ int tsattn_kv_read_int8(int32_t dtype, int32_t batch, int32_t heads, int64_t fir
   if (dtype == TSATTN_F64) return fail(TSATTN_ERR_UNSUPPORTED, "int8 rows are read as f32, f16 or bf16");
   if (batch <= 0 || heads <= 0 || first < 0 || len <= 0 || dim_qk <= 0 || dim_v <= 0)
     return fail(TSATTN_ERR_INVALID, "rows to read need positive sizes");
-  // (32-bit element counts of a head, workgroups in one grid dimension)
+  // (32-bit element counts of a head)
   const int64_t head = static_cast<int64_t>(len) * (dim_qk > dim_v ? dim_qk : dim_v);
-  if (head >= (int64_t(1) << 31) || static_cast<int64_t>(batch) * heads * (head / 256 + 1) >= (int64_t(1) << 31))
-    return fail(TSATTN_ERR_UNSUPPORTED, "at most 2^31 elements of a head, and 2^39 in all, are read at once");
+  if (head >= (int64_t(1) << 31) - 256 || static_cast<int64_t>(batch) * heads >= (int64_t(1) << 31))
+    return fail(TSATTN_ERR_UNSUPPORTED, "fewer than 2^31 - 256 elements of a head, and 2^31 heads, are read at once");
   return hip_status(tsattn::launch_kv_read_int8(dtype, batch, heads, first, len, dim_qk, dim_v, tsattn::make_view(k),
                                                 tsattn::make_view(v), tsattn::make_view(k_scale),
                                                 tsattn::make_view(v_scale), k_out, v_out,

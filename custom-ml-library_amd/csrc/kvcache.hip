@@ -162,7 +162,7 @@ struct ReadArgs {
   int dim[2];
   int64_t first;
   int H, n;
-  uint32_t chunks;  // workgroups a (sequence, head) and side
+  uint32_t bh0, chunks;  // the first (sequence, head), and the workgroups of each and side
 };
 
 // (kept from the compiler, which would round the exact product to f16 at once)
@@ -176,8 +176,8 @@ __device__ __forceinline__ T read_code(int8_t code, float scale) {
 template <typename T, int VE>
 __global__ __launch_bounds__(NT) void kv_read_int8_kernel(ReadArgs a) {
   const int side = blockIdx.y;
-  const uint32_t bh = blockIdx.x / a.chunks, b = bh / a.H, h = bh - b * a.H;
-  const uint32_t pieces = a.dim[side] / VE, i = (blockIdx.x - bh * a.chunks) * NT + threadIdx.x;
+  const uint32_t unit = blockIdx.x / a.chunks, bh = a.bh0 + unit, b = bh / a.H, h = bh - b * a.H;
+  const uint32_t pieces = a.dim[side] / VE, i = (blockIdx.x - unit * a.chunks) * NT + threadIdx.x;
   const uint32_t t = i / pieces, d = (i - t * pieces) * VE;
   if (t >= static_cast<uint32_t>(a.n)) return;
   const View &x = a.x[side], &s = a.s[side];
@@ -198,12 +198,16 @@ __global__ __launch_bounds__(NT) void kv_read_int8_kernel(ReadArgs a) {
 }
 
 template <typename T>
-void read_int8(ReadArgs &a, int BH, bool wide, hipStream_t st) {
+void read_int8(ReadArgs &a, uint32_t BH, bool wide, hipStream_t st) {
   const int most = a.dim[0] > a.dim[1] ? a.dim[0] : a.dim[1];
   a.chunks = static_cast<uint32_t>((static_cast<int64_t>(a.n) * (wide ? most / 8 : most) + NT - 1) / NT);
-  const dim3 grid(static_cast<uint32_t>(BH) * a.chunks, 2);
-  if (wide) kv_read_int8_kernel<T, 8><<<grid, dim3(NT), 0, st>>>(a);
-  else kv_read_int8_kernel<T, 1><<<grid, dim3(NT), 0, st>>>(a);
+  // (a grid has fewer than 2^32 work-items: up to 2^23 workgroups, as one head has, at a time)
+  const uint32_t heads = (1u << 23) / a.chunks > 1 ? (1u << 23) / a.chunks : 1;
+  for (a.bh0 = 0; a.bh0 < BH; a.bh0 += heads) {
+    const dim3 grid((BH - a.bh0 < heads ? BH - a.bh0 : heads) * a.chunks, 2);
+    if (wide) kv_read_int8_kernel<T, 8><<<grid, dim3(NT), 0, st>>>(a);
+    else kv_read_int8_kernel<T, 1><<<grid, dim3(NT), 0, st>>>(a);
+  }
 }
 
 }  // namespace
@@ -250,16 +254,17 @@ hipError_t launch_kv_append_int8(int dtype, int B, int H, int T_, int D, View sr
 
 hipError_t launch_kv_read_int8(int dtype, int B, int H, int64_t first, int n, int Dk, int Dv, View k, View v, View ks,
                                View vs, void *ko, void *vo, hipStream_t st) {
-  ReadArgs a{{k, v}, {ks, vs}, {ko, vo}, {Dk, Dv}, first, H, n, 0};
+  ReadArgs a{{k, v}, {ks, vs}, {ko, vo}, {Dk, Dv}, first, H, n, 0, 0};
   auto eights = [](const View &x, const void *out) {
     return reinterpret_cast<uintptr_t>(x.data) % 8 == 0 && x.s0 % 8 == 0 && x.s1 % 8 == 0 && x.s2 % 8 == 0 &&
            reinterpret_cast<uintptr_t>(out) % 16 == 0;
   };
   const bool wide = Dk % 8 == 0 && Dv % 8 == 0 && eights(k, ko) && eights(v, vo);
   Probe pr_("kv_read_int8", st);
-  if (dtype == TSATTN_F32) read_int8<float>(a, B * H, wide, st);
-  else if (dtype == TSATTN_F16) read_int8<f16>(a, B * H, wide, st);
-  else read_int8<bf16>(a, B * H, wide, st);
+  const uint32_t BH = static_cast<uint32_t>(B) * static_cast<uint32_t>(H);
+  if (dtype == TSATTN_F32) read_int8<float>(a, BH, wide, st);
+  else if (dtype == TSATTN_F16) read_int8<f16>(a, BH, wide, st);
+  else read_int8<bf16>(a, BH, wide, st);
   return hipGetLastError();
 }
 

@@ -372,7 +372,7 @@ int tsattn_kv_append_int8(int32_t dtype, int32_t batch, int32_t heads, int32_t l
 /*
  * The other way (KVCache.get): rows first .. first + len - 1 of an int8 cache's keys (of
  * dim_qk) and values (dim_v) [batch, heads, *] times their fp32 scales, rounded once to dtype (f32, f16,
- * bf16; others and 2^31 elements of a head or more: TSATTN_ERR_UNSUPPORTED), into contiguous
+ * bf16; others and 2^31 - 256 elements of a head or more: TSATTN_ERR_UNSUPPORTED), into contiguous
  * [batch, heads, len, dim] arrays.
  */
 int tsattn_kv_read_int8(int32_t dtype, int32_t batch, int32_t heads, int64_t first, int32_t len, int32_t dim_qk,

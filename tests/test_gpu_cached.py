@@ -509,3 +509,21 @@ def test_offsets_past_32_bits(int8):
             outs += [x._data for x in cache.get(5)]
     for got, want in zip(outs[:3], outs[3:]):
         assert (got[-1:].double() - want.double()).norm() <= 2.0 ** -10 * want.double().norm()
+
+
+def test_more_codes_than_a_grid_holds():
+    """4.4e9 codes a side, read one by one: rows of 9."""
+    h, d, n = 64, 9, 7_600_000
+    cache = nn.KVCache(1, h, d, n, device="hip", dtype=torch.float16, quantized=True)
+    full = (0, 3, 31, 62, 63)
+    for x in cache.storage[:2]:
+        for head in full:
+            x[0, head].copy_(torch.randint(-127, 128, x[0, head].shape, device="cuda", generator=_gen(head)))
+    for x in cache.storage[2:]:
+        x[0, 63].copy_(2.0 ** (6 * torch.rand(x[0, 63].shape, device="cuda", generator=_gen(d)) - 14))
+    cache.length = n
+    print("cached read", h, d, n, flush=True)
+    for got, x, s in zip(cache.get(), cache.storage[:2], cache.storage[2:]):
+        for head in range(h):
+            want = (x[0, head].float() * s[0, head]).half() if head in full else 0
+            assert (got._data[0, head] == want).all(), head
