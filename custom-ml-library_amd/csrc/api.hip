@@ -150,6 +150,13 @@ int check_rope(const tsattn_rope_desc *r, const tsattn::Problem &pr, tsattn::Rop
   return TSATTN_OK;
 }
 
+// A grid has fewer than 2^32 work-items (one with more wraps round, without an error), and so
+// fewer than 2^24 workgroups of 256; half of them, for rounding and key blocks cut in parts.
+int check_groups(int64_t groups) {
+  if (groups < (int64_t(1) << 23)) return TSATTN_OK;
+  return fail(TSATTN_ERR_INVALID, "%lld workgroups do not fit into a launch", static_cast<long long>(groups));
+}
+
 // A problem with a sliding window, which only the MFMA kernels take.
 int check_window(const tsattn_problem *p, int64_t window, int32_t sinks, const void *out_low, tsattn::Problem *pr) {
   int rc = check_problem(p, pr);
@@ -161,6 +168,12 @@ int check_window(const tsattn_problem *p, int64_t window, int32_t sinks, const v
     return fail(TSATTN_ERR_UNSUPPORTED, "windows take no dropout and no mask but key padding");
   pr->window = static_cast<int>(window < (1 << 30) ? window : 1 << 30);
   pr->sinks = sinks < pr->Sk ? sinks : pr->Sk;
+  // (128 query rows or keys a workgroup; f32 backward: a pass of 8 rows or more)
+  const int64_t heads = static_cast<int64_t>(pr->B) * pr->Hq, longest = pr->Sq > pr->Sk ? pr->Sq : pr->Sk;
+  if (heads >= (int64_t(1) << 31)) return fail(TSATTN_ERR_INVALID, "at most 2^31 - 1 heads have a window");
+  if ((rc = check_groups(heads * (longest / 128 + 1))) ||
+      (p->dtype == TSATTN_F32 && (rc = check_groups(heads * (pr->Sq / 8 + 1)))))
+    return rc;
   if (out_low) {
     if (p->dtype != TSATTN_F16 && p->dtype != TSATTN_BF16)
       return fail(TSATTN_ERR_INVALID, "only 16-bit outputs have a low part");
@@ -469,6 +482,12 @@ int check_cached(const tsattn_cached *d, tsattn::CachedProblem *p) {
   tsattn::CachedProblem c{};
   c.dtype = d->dtype, c.B = d->batch, c.Hq = d->heads_q, c.Hkv = d->heads_kv, c.T = d->len, c.n = d->keys;
   c.D = d->dim, c.q8 = d->quantized != 0, c.scale = d->scale;
+  // (32 rows of a KV head a workgroup; 4 rows one that joins splits)
+  const int64_t rows = static_cast<int64_t>(d->heads_q / d->heads_kv) * d->len, heads = static_cast<int64_t>(d->batch) * d->heads_kv;
+  if (rows >= (int64_t(1) << 31) / heads)
+    return fail(TSATTN_ERR_INVALID, "cached attention takes fewer than 2^31 rows");
+  int rc;
+  if ((rc = check_groups(heads * ((rows + 31) / 32))) || (rc = check_groups(heads * rows / 4))) return rc;
   c.window = static_cast<int>(d->window < (1 << 30) ? d->window : 1 << 30);
   c.sinks = d->sinks < d->keys ? d->sinks : d->keys;
   if (d->words) c.words = d->words, c.depth = d->depths, c.tree_rows = d->trees;
@@ -1064,6 +1083,10 @@ int tsattn_draft_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len
   if (trees != 1 && trees != batch) return fail(TSATTN_ERR_INVALID, "one tree, or one for each sequence");
   if (len > 256) return fail(TSATTN_ERR_UNSUPPORTED, "a tree has at most 256 tokens (got %d)", len);
   if (!cos != !sin) return fail(TSATTN_ERR_INVALID, "RoPE needs cos / sin tables");
+  // (4 rows a workgroup; a batch or heads that are not positive: refused there)
+  const int64_t all = batch > 0 && heads > 0 ? static_cast<int64_t>(batch) * heads : 0;
+  if (all >= (int64_t(1) << 31)) return fail(TSATTN_ERR_INVALID, "at most 2^31 - 1 heads are appended to");
+  if (int rc = check_groups(all * len / 4)) return rc;
   return rope_append(dtype, batch, heads, len, dim, cos ? dim : 0, k, v, k_cache, v_cache, k_scale, v_scale, cos,
                      sin, pos, depths, trees, stream);
 }
@@ -1073,6 +1096,7 @@ int tsattn_draft_tree(int32_t trees, int32_t len, const int32_t *parents, uint32
   if (trees <= 0 || len <= 0) return fail(TSATTN_ERR_INVALID, "a tree needs at least one token");
   if (len > 256) return fail(TSATTN_ERR_UNSUPPORTED, "a tree has at most 256 tokens (got %d)", len);
   if (!parents || !words || !depths) return fail(TSATTN_ERR_INVALID, "data pointer is NULL");
+  if (int rc = check_groups(trees)) return rc;
   return hip_status(tsattn::launch_draft_tree(trees, len, parents, words, depths, static_cast<hipStream_t>(stream)),
                     "draft tree launch");
 }
@@ -1102,6 +1126,7 @@ int tsattn_cache_keep(int32_t batch, int32_t heads, int32_t n, int64_t first, in
     a.bytes[i] = (i == 0 ? dim_qk : i == 1 ? dim_v : 1) * static_cast<int>(unit);
   }
   a.B = batch, a.H = heads, a.n = n, a.first = first, a.limit = limit, a.index = index, a.index_bytes = index_bytes;
+  if ((rc = check_groups(tsattn::keep_groups(a)))) return rc;
   return hip_status(tsattn::launch_keep(a, static_cast<hipStream_t>(stream)), "cache rows launch");
 }
 

@@ -809,9 +809,11 @@ hipError_t launch_draft_tree(int trees, int T, const int32_t *parents, uint32_t 
   return hipGetLastError();
 }
 
-hipError_t launch_keep(const KeepArgs &a, hipStream_t st) {
-  Probe pr_("cache_keep", st);
-  // pieces as wide as every array's rows and addresses allow
+// Kept rows' pieces, as wide as every array's rows and addresses allow.
+struct KeepPlan {
+  int arrays, piece, slices;
+};
+static KeepPlan plan_keep(const KeepArgs &a) {
   int arrays = 0, most = 0;
   uintptr_t all = 0;
   for (int i = 0; i < 4; ++i)
@@ -824,11 +826,21 @@ hipError_t launch_keep(const KeepArgs &a, hipStream_t st) {
     }
   if (arrays > 2 && all % 16 == 0) all |= 4;  // (scales: 4 bytes a row)
   const int piece = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
-  const int slices = (most + 4 * piece - 1) / (4 * piece);
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.B) * a.H * slices), arrays);
-  if (piece == 16) keep_kernel<u32x4><<<grid, dim3(256), 0, st>>>(a, slices);
-  else if (piece == 4) keep_kernel<uint32_t><<<grid, dim3(256), 0, st>>>(a, slices);
-  else keep_kernel<uint8_t><<<grid, dim3(256), 0, st>>>(a, slices);
+  return KeepPlan{arrays, piece, most / (4 * piece) + (most % (4 * piece) != 0)};
+}
+
+int64_t keep_groups(const KeepArgs &a) {
+  const int64_t heads = static_cast<int64_t>(a.B) * a.H;
+  return heads < (int64_t(1) << 31) ? heads * plan_keep(a).slices : heads;
+}
+
+hipError_t launch_keep(const KeepArgs &a, hipStream_t st) {
+  const KeepPlan s = plan_keep(a);
+  Probe pr_("cache_keep", st);
+  const dim3 grid(static_cast<unsigned>(keep_groups(a)), s.arrays);
+  if (s.piece == 16) keep_kernel<u32x4><<<grid, dim3(256), 0, st>>>(a, s.slices);
+  else if (s.piece == 4) keep_kernel<uint32_t><<<grid, dim3(256), 0, st>>>(a, s.slices);
+  else keep_kernel<uint8_t><<<grid, dim3(256), 0, st>>>(a, s.slices);
   return hipGetLastError();
 }
 

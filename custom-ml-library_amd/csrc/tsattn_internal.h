@@ -342,6 +342,7 @@ struct KeepArgs {
   const void *index;
   int index_bytes;
 };
+int64_t keep_groups(const KeepArgs &a);  // workgroups of each array
 hipError_t launch_keep(const KeepArgs &a, hipStream_t st);
 
 // The q / k / v projections of the `batch x len` rows of x (embed wide; a

@@ -401,6 +401,27 @@ def test_the_library_refuses_trees_and_kept_rows():
     assert append(n=257) == UNSUPPORTED
 
 
+def test_more_workgroups_than_a_grid_holds_are_refused():
+    """From 2^24 workgroups of 256 on a grid wraps round without an error."""
+    real, v = _lib.load(), _view()
+    for kw in ({"batch": 1 << 23}, {"batch": 1 << 16, "heads_q": 1 << 8}, {"batch": 1 << 30, "heads_q": 1 << 20},
+               {"dtype": _lib.F32, "batch": 1 << 20, "len_q": 4096, "len_kv": 4096}):
+        args = (ctypes.byref(_problem(heads_kv=1, **kw)), 4, 1, None, v, v, v, v)
+        assert _code(real.tsattn_window_forward(*args, None, None, None)) == INVALID, kw
+        assert _code(real.tsattn_window_backward(*args, v, 0x1000, None, v, v, v, 0x1000, 1 << 62, None)) == INVALID, kw
+    for kw in ({"batch": 1 << 23}, {"batch": 1 << 16, "heads_q": 1 << 8, "heads_kv": 1 << 8},
+               {"batch": 1 << 30, "heads_q": 1 << 20, "heads_kv": 1 << 20},
+               {"batch": 1 << 12, "heads_q": 1 << 7, "heads_kv": 1, "len": 256, "keys": 256}):
+        rc = real.tsattn_cached_attend(_cached(**kw), v, v, v, None, None, v, 0x1000, 1 << 62, None)
+        assert _code(rc) == INVALID, kw
+    assert _code(real.tsattn_draft_tree(1 << 24, 3, 0x1000, 0x1000, 0x1000, None)) == INVALID
+    for b, h in ((1 << 23, 1), (1 << 16, 1 << 8), (1 << 30, 1 << 30)):
+        rc = real.tsattn_cache_keep(b, h, 2, 3, 4, 0x1000, 8, 2, 64, 64, v, v, None, None, None)
+        assert _code(rc) == INVALID, (b, h)
+        rc = real.tsattn_draft_append(_lib.F16, b, h, 9, 64, v, v, v, v, None, None, None, None, 5, 0x1000, 1, None)
+        assert _code(rc) == INVALID, (b, h)
+
+
 def test_the_library_refuses_token_probabilities():
     real = _lib.load()
 
