@@ -15,6 +15,8 @@ import math
 import operator
 from typing import NamedTuple
 
+import numpy as np
+
 from .. import _lib
 from ..amp import _autocast, _cast_inputs
 from ..device import launch, random_uniform
@@ -454,8 +456,9 @@ def token_log_probs(input: Tensor, target: Tensor, top_k: int = 0, *, ignore_ind
     if shape != given[:-1]:
         raise ValueError(f"target shape {shape} does not match logits shape {given}")
     classes = given[-1]
-    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 0 <= top_k <= min(classes, 64):
+    if isinstance(top_k, bool) or not isinstance(top_k, (int, np.integer)) or not 0 <= top_k <= min(classes, 64):
         raise ValueError("top_k must be between zero and 64 and within the classes")
+    top_k = int(top_k)
     padding = operator.index(ignore_index)
     _require_hip(input, "token_log_probs")
     code = _code(x)

@@ -78,6 +78,15 @@ def test_token_log_probs_refuses(lib):
     assert lib.args["tsattn_token_probs"][7] == -7
 
 
+@pytest.mark.parametrize("kind", [int, np.int32, np.int64, np.uint8])
+def test_top_k_of_any_integer_type(lib, kind):
+    got = F.token_log_probs(_draw(4, 9), _ints([0, 1, 2, 3]), kind(3))
+    assert got.top_log_probs.shape == got.top_indices.shape == (4, 3)
+    assert lib.args["tsattn_token_probs"][8] == 3 and type(lib.args["tsattn_token_probs"][8]) is int
+    with pytest.raises(ValueError, match="top_k"):
+        F.token_log_probs(_draw(4, 9), _ints([0, 1, 2, 3]), kind(10))
+
+
 def test_no_rows_launch_nothing(lib):
     z = _draw(0, 3, 9, grad=True)
     got = F.token_log_probs(z, _ints(np.zeros((0, 3), np.int64).tolist()).reshape(0, 3), 2)
