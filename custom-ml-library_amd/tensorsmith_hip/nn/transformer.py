@@ -164,6 +164,9 @@ class MultiHeadAttention(Module):
     ``window``, ``sinks``: causal attention to the last ``window`` positions and the
     first ``sinks`` (``scaled_dot_product_attention``)."""
 
+    window: int | None = None  # (of layers pickled before they had one, too)
+    sinks: int = 0
+
     def __init__(self, embed_dim: int, num_heads: int, *, num_kv_heads: int | None = None,
                  dropout: float = 0.0, bias: bool = False, rotary: bool = True,
                  backend: str = "auto", window: int | None = None, sinks: int = 0, device=None):

@@ -118,6 +118,17 @@ def test_windows_are_checked(lib):
     assert not lib.calls
 
 
+def test_layers_pickled_before_windows_run(lib):
+    """They hold neither window nor sinks."""
+    layer = nn.MultiHeadAttention(128, 2, rotary=False, device="hip:0")
+    del layer.__dict__["window"], layer.__dict__["sinks"]
+    layer = pickle.loads(pickle.dumps(layer)).eval()
+    assert layer(_draw(1, 3, 128, dtype=torch.float32)).shape == (1, 3, 128)
+    with ts.no_grad():
+        assert layer(_draw(1, 3, 128, dtype=torch.float32), cache=layer.new_cache(1, 8)).shape == (1, 3, 128)
+    assert not [name for name, _, _ in lib.calls if "window" in name]
+
+
 def test_windows_as_the_library_takes_them(lib):
     """Any integers, no larger than they can count; a window over everything is none."""
     q = _draw(1, 2, 60, 64)
