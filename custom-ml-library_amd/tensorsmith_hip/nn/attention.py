@@ -412,7 +412,8 @@ def scaled_dot_product_attention(
 
     def backward(upstream, _keep=keep):  # _keep: mask / length buffers the kernels read
         g = _operand(upstream)
-        if (fused or code in (_lib.F16, _lib.BF16) or window is not None) and (not _aligned16(g) or min(g.stride()[:3]) <= 0):
+        if ((fused or code in (_lib.F16, _lib.BF16) or window is not None)
+                and (not _aligned16(g) or min(g.stride()[:3]) <= 0)):
             # the MFMA kernels (the only ones the folded-RoPE backward has) need
             # 16-byte aligned rows of a real gradient: an expanded one (a sum's
             # VJP) would send the plain backward to the generic kernels
@@ -427,7 +428,8 @@ def scaled_dot_product_attention(
             ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=tdev)
             _lib.check(launch(query.device, lib.tsattn_window_backward, ctypes.byref(prob), window, sinks,
                               ctypes.byref(rope[0]) if fused else None, vq, vk, vv, vo, _view(g), lse.data_ptr(),
-                              None if low is None else low.data_ptr(), _view(dq), _view(dk), _view(dv), ws.data_ptr(), nbytes), "windowed attention backward")
+                              None if low is None else low.data_ptr(), _view(dq), _view(dk), _view(dv), ws.data_ptr(),
+                              nbytes), "windowed attention backward")
             return unrotated(dq, dk) + (dv,)
         nbytes = (lib.tsattn_sdpa_backward_rope_workspace if fused
                   else lib.tsattn_sdpa_backward_workspace)(ctypes.byref(prob))
