@@ -13,7 +13,7 @@
 // A lane's sums are in log2 units, t_j = z_j log2 e - b as one fused operation, b = m log2 e
 // as it rounds.  What that rounding takes, r = m log2 e - b, is in every t of the lane alike,
 // and `exact` takes it out again before sums meet, as 2^-r.  That needs an r that exp2 can
-// hold: logits past kFar (2^20, r at most 2^-4), among them masks of -1e10 or of the type's
+// hold: past a b of kFar (2^20, r at most 2^-5), among them masks of -1e10 or of the type's
 // lowest value, whose product with log2 e may overflow besides, turn the wave to t_j = (z_j -
 // m) log2 e from then on, two instructions a logit more.
 //
@@ -50,7 +50,7 @@ constexpr int U = 4;         // 16-byte pieces a lane has in flight
 constexpr int PENDING = 64 + 64 * 8;  // keys a wave's buffer holds: < 64 left over, and one piece of each lane
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kFar = 1048576.f;  // logits from which z log2 e - b is not taken
+constexpr float kFar = 1048576.f;  // b from which on z log2 e - b is not taken
 constexpr float kLeast = -1e4f;    // 2^t is 0 from here on, and so is its product with t and a factor below 3e34
 
 struct ProbArgs {
@@ -112,7 +112,6 @@ struct Sums {
   float m, l, w;
 };
 
-__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m != -INFINITY; }
 // (a base that keeps 2^(-inf - base) = 0 while nothing but -inf has come)
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 // b, rounded here (a fused operation further on would round it otherwise)
@@ -133,14 +132,9 @@ __device__ __forceinline__ void rebase(Sums &s, float m) {
   shift(s, (s.m - m) * kLog2e);
   s.m = m;
 }
-// Sums over t = z log2 e - b, to another m.
-__device__ __forceinline__ void rebase_near(Sums &s, float m) {
-  shift(s, scaled(s.m) - scaled(m));
-  s.m = m;
-}
-// Those as sums over (z - m) log2 e.
-__device__ __forceinline__ Sums exact(Sums s) {
-  const float b = scaled(s.m), r = fmaf(base_of(s.m), kLog2e, -b), c = __builtin_amdgcn_exp2f(-r);
+// Sums over t = z log2 e - b as sums over (z - m) log2 e.
+__device__ __forceinline__ Sums exact(Sums s, float b) {
+  const float r = fmaf(base_of(s.m), kLog2e, -b), c = __builtin_amdgcn_exp2f(-r);
   return Sums{s.m, s.l * c, fmaf(-r, s.l, s.w) * c};
 }
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
@@ -174,12 +168,11 @@ __device__ __forceinline__ float largest(const float (&x)[N]) {
 }
 
 // Adds N logits, none above m; `own` becomes their sum of exponentials (NaN where one is
-// NaN or +inf).  NEAR: z log2 e - b, where a logit of -inf makes w a NaN (0 times -inf);
-// SAFE: the same, but that, at an instruction a logit; FAR: (z - m) log2 e, as safe.
+// NaN or +inf).  NEAR: z log2 e - base, where a logit of -inf makes w a NaN (0 times -inf);
+// SAFE: the same, but that, at an instruction a logit; FAR: (z - base) log2 e, as safe.
 enum Sort { NEAR, SAFE, FAR };
 template <Sort S, int N>
-__device__ __forceinline__ void add(Sums &s, const float (&x)[N], float &own) {
-  const float base = S == FAR ? base_of(s.m) : scaled(s.m);
+__device__ __forceinline__ void add(Sums &s, const float (&x)[N], float base, float &own) {
   float l = 0.f;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -387,21 +380,29 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
   Best top;
   top.buffer = buffers + (TOP ? w * PENDING : 0);
   bool far = false;  // of the wave: its sums are over (z - m) log2 e
+  float base = 0.f;  // b, or far m
   auto raise = [&](float most) __attribute__((always_inline)) {
-    if (!far && __ballot(is_far(most)) != 0ull) {
-      s = exact(s);
+    if (!far) {
+      const float b = scaled(most);
+      if (__ballot(fabsf(b) > kFar) == 0ull) {
+        shift(s, base - b);
+        s.m = most;
+        base = b;
+        return;
+      }
+      s = exact(s, base);
       far = true;
     }
-    if (far) rebase(s, most);
-    else rebase_near(s, most);
+    rebase(s, most);
+    base = base_of(most);
   };
   // the elements in front of the first piece, one a lane
   auto single = [&](int first, int n) {
     const float x[1] = {lane < n ? static_cast<float>(r.z[first + lane]) : -INFINITY};
     float own;
     raise(fmaxf(s.m, x[0]));
-    if (far) add<FAR>(s, x, own);
-    else add<SAFE>(s, x, own);
+    if (far) add<FAR>(s, x, base, own);
+    else add<SAFE>(s, x, base, own);
     if constexpr (TOP) top.offer(x, x[0], own, first + lane, lane < n ? 1 : 0, a.top, lane);
   };
   const int l0 = (WPR == 1 ? 0 : w * 64) + lane;
@@ -439,20 +440,20 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + u * LANES >= p1) break;
-        add<FAR>(s, x[u], own[u]);
+        add<FAR>(s, x[u], base, own[u]);
       }
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + u * LANES >= p1) break;
-        add<NEAR>(s, x[u], own[u]);
+        add<NEAR>(s, x[u], base, own[u]);
       }
       if (__ballot(s.w != s.w) != 0ull) {  // a logit of -inf: again
         s = before;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (i + u * LANES >= p1) break;
-          add<SAFE>(s, x[u], own[u]);
+          add<SAFE>(s, x[u], base, own[u]);
         }
       }
     }
@@ -468,7 +469,7 @@ __global__ __launch_bounds__(NT) void probs_kernel(ProbArgs a) {
     for (int u = 0; u < U; ++u) raw[u] = next[u];
   }
   if (part == splits - 1 && (WPR == 1 || w == NW - 1) && r.tail) single(a.vocab - r.tail, r.tail);
-  s = wave_join(far ? s : exact(s));
+  s = wave_join(far ? s : exact(s, base));
   if constexpr (TOP) top.finish(a.top, lane);
   if constexpr (WPR > 1) {
     if (lane == 0) red[w][0] = s.m, red[w][1] = s.l, red[w][2] = s.w;
