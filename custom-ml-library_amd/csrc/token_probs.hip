@@ -21,7 +21,7 @@
 // gradient.  One pass in each: a lane keeps a running (m, l, sum 2^t t) and rescales it
 // once for every four 16-byte pieces.  The forward is about as far from the vector units'
 // bound: 6 instructions a logit; 11 of them (selects for rows' ends and -inf on every
-// one) took 131 us where 8192 rows of 50021 bf16, a fifth of them ignored, take 107
+// one) took 131 us where 8192 rows of 50021 bf16, a fifth of them ignored, take 108
 // (6.1 TB/s).  The VJP of those takes 285 us, 5.2 TB/s of reads and writes, as a copy; 331
 // before its rows' pieces began on whole lines of memory.
 //
