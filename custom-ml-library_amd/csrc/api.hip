@@ -151,9 +151,9 @@ int check_rope(const tsattn_rope_desc *r, const tsattn::Problem &pr, tsattn::Rop
 }
 
 // A grid has fewer than 2^32 work-items (one with more wraps round, without an error), and so
-// fewer than 2^24 workgroups of 256; half of them, for rounding and key blocks cut in parts.
+// fewer than 2^24 workgroups of 256.
 int check_groups(int64_t groups) {
-  if (groups < (int64_t(1) << 23)) return TSATTN_OK;
+  if (groups < (int64_t(1) << 24)) return TSATTN_OK;
   return fail(TSATTN_ERR_INVALID, "%lld workgroups do not fit into a launch", static_cast<long long>(groups));
 }
 
@@ -168,10 +168,10 @@ int check_window(const tsattn_problem *p, int64_t window, int32_t sinks, const v
     return fail(TSATTN_ERR_UNSUPPORTED, "windows take no dropout and no mask but key padding");
   pr->window = static_cast<int>(window < (1 << 30) ? window : 1 << 30);
   pr->sinks = sinks < pr->Sk ? sinks : pr->Sk;
-  // (128 query rows or keys a workgroup; f32 backward: a pass of 8 rows or more)
+  // (128 query rows or keys a workgroup, and the sinks' parts; f32 backward: a pass of 8 rows or more)
   const int64_t heads = static_cast<int64_t>(pr->B) * pr->Hq, longest = pr->Sq > pr->Sk ? pr->Sq : pr->Sk;
   if (heads >= (int64_t(1) << 31)) return fail(TSATTN_ERR_INVALID, "at most 2^31 - 1 heads have a window");
-  if ((rc = check_groups(heads * (longest / 128 + 1))) ||
+  if ((rc = check_groups(heads * (longest / 128 + 1) + 2048)) ||
       (p->dtype == TSATTN_F32 && (rc = check_groups(heads * (pr->Sq / 8 + 1)))))
     return rc;
   if (out_low) {
@@ -482,12 +482,12 @@ int check_cached(const tsattn_cached *d, tsattn::CachedProblem *p) {
   tsattn::CachedProblem c{};
   c.dtype = d->dtype, c.B = d->batch, c.Hq = d->heads_q, c.Hkv = d->heads_kv, c.T = d->len, c.n = d->keys;
   c.D = d->dim, c.q8 = d->quantized != 0, c.scale = d->scale;
-  // (32 rows of a KV head a workgroup; 4 rows one that joins splits)
+  // (32 rows of a KV head a workgroup, in up to 2 splits where they are many; 4 rows one that joins splits)
   const int64_t rows = static_cast<int64_t>(d->heads_q / d->heads_kv) * d->len, heads = static_cast<int64_t>(d->batch) * d->heads_kv;
   if (rows >= (int64_t(1) << 31) / heads)
     return fail(TSATTN_ERR_INVALID, "cached attention takes fewer than 2^31 rows");
   int rc;
-  if ((rc = check_groups(heads * ((rows + 31) / 32))) || (rc = check_groups(heads * rows / 4))) return rc;
+  if ((rc = check_groups(2 * heads * ((rows + 31) / 32))) || (rc = check_groups(heads * rows / 4 + 1))) return rc;
   c.window = static_cast<int>(d->window < (1 << 30) ? d->window : 1 << 30);
   c.sinks = d->sinks < d->keys ? d->sinks : d->keys;
   if (d->words) c.words = d->words, c.depth = d->depths, c.tree_rows = d->trees;
@@ -1086,7 +1086,7 @@ int tsattn_draft_append(int32_t dtype, int32_t batch, int32_t heads, int32_t len
   // (4 rows a workgroup; a batch or heads that are not positive: refused there)
   const int64_t all = batch > 0 && heads > 0 ? static_cast<int64_t>(batch) * heads : 0;
   if (all >= (int64_t(1) << 31)) return fail(TSATTN_ERR_INVALID, "at most 2^31 - 1 heads are appended to");
-  if (int rc = check_groups(all * len / 4)) return rc;
+  if (int rc = check_groups(all * len / 4 + 1)) return rc;
   return rope_append(dtype, batch, heads, len, dim, cos ? dim : 0, k, v, k_cache, v_cache, k_scale, v_scale, cos,
                      sin, pos, depths, trees, stream);
 }
