@@ -13,9 +13,10 @@
 // A lane's sums are in log2 units, t_j = z_j log2 e - b as one fused operation, b = m log2 e
 // as it rounds.  What that rounding takes, r = m log2 e - b, is in every t of the lane alike,
 // and `exact` takes it out again before sums meet, as 2^-r.  That needs an r that exp2 can
-// hold: past a b of kFar (2^20, r at most 2^-5), among them masks of -1e10 or of the type's
-// lowest value, whose product with log2 e may overflow besides, turn the wave to t_j = (z_j -
-// m) log2 e from then on, two instructions a logit more.
+// hold: a largest logit whose b is past kFar (2^20, r at most 2^-5), such as a mask of -1e10
+// or of the type's lowest value, whose product with log2 e may overflow besides, turns the
+// wave to t_j = (z_j - m) log2 e from then on, two instructions a logit more.  (For every
+// logit of every row they would cost a tenth of the forward: 116 -> 128 us.)
 //
 // Bound by HBM: the forward reads the logits once, the VJP reads them and writes the
 // gradient.  One pass in each: a lane keeps a running (m, l, sum 2^t t) and rescales it
